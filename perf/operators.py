@@ -260,10 +260,10 @@ def _run_qk(s):
     c = s["case"]
     if own:
         from paperkiln_amd import ops
-        yq, yk, rinv = ops.qk_norm_rope_fwd(s["q"], s["k"], s["wq"], s["wk"], s["pos"], c["theta"], 1e-5, c["rotary"], c["halves"])
+        yq, yk = ops.qk_norm_rope_fwd(s["q"], s["k"], s["wq"], s["wk"], s["pos"], c["theta"], 1e-5, c["rotary"], c["halves"])
         if not c["train"]:
             return {"yq": yq, "yk": yk}
-        dq, dk, dwq, dwk = ops.qk_norm_rope_bwd(s["dyq"], s["dyk"], s["q"], s["k"], s["wq"], s["wk"], s["pos"], rinv, c["theta"], c["rotary"], c["halves"])
+        dq, dk, dwq, dwk = ops.qk_norm_rope_bwd(s["dyq"], s["dyk"], s["q"], s["k"], s["wq"], s["wk"], s["pos"], c["theta"], 1e-5, c["rotary"], c["halves"])
         return {"yq": yq, "yk": yk, "dq": dq, "dk": dk, "dwq": dwq, "dwk": dwk}
     rotary = c["rotary"] or c["dk"]
     freq = c["theta"] ** (-torch.arange(0, rotary, 2, device="cuda", dtype=torch.float64) / rotary)
