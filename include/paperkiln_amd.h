@@ -284,6 +284,103 @@ int pk_set_gemm_backend(int mode);
  * setting. */
 int pk_set_head_kernel(int in_product);
 
+/* ---- post-training operators --------------------------------------------------
+ * What training a decoder past its first language-model loss adds to the operators above; the reference has no
+ * counterpart. Calls only enqueue on `stream`, allocate nothing and clear nothing by memset, so they may be
+ * recorded into a HIP graph; scalars (a step count, a seed) are then those of the recording. */
+
+/* Per-head norms of queries and keys with the position rotation, between a block's projection and pk_attn_fwd:
+ *   r = 1/sqrt(mean_j x_j^2 + eps), u_j = x_j r w_j, then pairs of the first `rotary` columns of u are turned by
+ *   pos * theta^(-2i/rotary); every head of q and k by its own r, one weight [dk] for q's heads and one for k's. */
+typedef struct pk_qk_shape {
+    int32_t B, T;        /* either may be 0 */
+    int32_t Hq, Hkv;     /* any two numbers of heads */
+    int32_t dk;          /* even, at most 256 */
+    int32_t rotary;      /* columns that are turned: even, at most dk; 0 = all */
+    int32_t halves;      /* 0: pairs are columns 2i and 2i+1, as pk_op_rope's; 1: columns i and i + rotary/2 */
+    int32_t dtype;       /* PK_F32 | PK_BF16: q, k, their outputs and gradients; weights are fp32 */
+    float eps;
+    double theta;        /* the angle is formed in 64 bits: any int32 position is as exact as a small one
+                            (pk_op_rope's is the reference's 32-bit product) */
+    int64_t pos_stride_b; /* pos[b * pos_stride_b + t], on the device; 0 = one row of positions for all sequences */
+} pk_qk_shape;
+/* yq / yk may lie where q / k do, element for element. */
+int pk_qk_norm_rope_fwd(const pk_qk_shape* s, const pk_tensor4* q, const pk_tensor4* k, const float* wq, const float* wk,
+                        const int* pos, const pk_tensor4* yq, const pk_tensor4* yk, void* stream);
+/* The gradients, from the inputs: r is formed again. dwq, dwk [dk] fp32 are overwritten; their sums are taken in a
+ * fixed order. dq / dk may lie where dyq / dyk or q / k do, element for element. */
+size_t pk_qk_norm_rope_bwd_workspace_bytes(const pk_qk_shape* s);
+int pk_qk_norm_rope_bwd(const pk_qk_shape* s, const pk_tensor4* dyq, const pk_tensor4* dyk, const pk_tensor4* q,
+                        const pk_tensor4* k, const float* wq, const float* wk, const int* pos, const pk_tensor4* dq,
+                        const pk_tensor4* dk, float* dwq, float* dwk, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Log-probabilities of chosen tokens: logits [rows, vocab] with ld elements between rows, z = scale * logits,
+ * logp[r] = z[r, targets[r]] - lse[r]. A row whose target is negative is not read: logp and lse 0. A target past the
+ * vocabulary gives NaN. Logits of -inf are words without probability; a row of nothing else gives NaN. lse may be NULL. */
+int pk_token_logprobs_fwd(const void* logits, int64_t ld, const int* targets, int64_t rows, int64_t vocab, float scale,
+                          float* logp, float* lse, int dtype, void* stream);
+/* dlogits[r, j] = dlogp[r] * scale * ([j = target] - exp(z_j - lse_r)), every row written: zeros where the target is
+ * negative or dlogp is 0 (such a row is not read). dlogits may be the logits themselves (same ld), else lies clear
+ * of them; so in the two losses below. */
+int pk_token_logprobs_bwd(const void* logits, int64_t ld, const int* targets, const float* lse, const float* dlogp,
+                          int64_t rows, int64_t vocab, float scale, void* dlogits, int64_t dld, int dtype, void* stream);
+
+/* Clipped policy loss with a KL term, loss and gradient in one pass over the logits. With rho = exp(logp - old_logp),
+ * A = advantages and d = ref_logp - logp,
+ *   L_r = -min(rho A, clamp(rho, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(d) - d - 1),  loss = sum_r weights[r] L_r;
+ * dlogits is the gradient of upstream * loss. The weights carry mask and normalisation (1/tokens, 1/(sequences *
+ * length), ...); a row of weight 0 or of a negative target is not read, its logp and gradient are 0. ref_logp may be
+ * NULL where kl_coef is 0. row_loss[rows] (64 bits) receives weights[r] L_r, loss (device, fp32) their sum in a fixed order. */
+typedef struct pk_policy_config {
+    float clip_low, clip_high, kl_coef, scale, upstream;
+} pk_policy_config;
+int pk_policy_loss(const pk_policy_config* c, const void* logits, int64_t ld, const int* targets, const float* old_logp,
+                   const float* ref_logp, const float* advantages, const float* weights, int64_t rows, int64_t vocab,
+                   void* dlogits, int64_t dld, float* logp, double* row_loss, float* loss, int dtype, void* stream);
+
+/* Preference loss over pairs of sequences, loss and gradient. Sequence s holds rows [seq_start[s], seq_start[s+1])
+ * (seq_start[2*pairs + 1] on the device, ascending; offsets past the rows are held to them); sequences 0 .. pairs-1 are
+ * the chosen answers, pairs .. 2*pairs-1 the rejected ones. Rows with a negative target (prompts, padding) count
+ * nothing. With s = sum of logp - ref_logp over a sequence's rows and e = label_smoothing,
+ *   margins[i] = u_i = beta (s_i - s_{pairs+i}),  loss = mean_i( -(1-e) log sigma(u_i) - e log sigma(-u_i) ).
+ * dlogits is the gradient of upstream * loss; rows of no sequence get zeros. logp as in pk_token_logprobs_fwd. */
+typedef struct pk_preference_config {
+    float beta, label_smoothing, scale, upstream;
+} pk_preference_config;
+size_t pk_preference_loss_workspace_bytes(int64_t rows, int64_t pairs);
+int pk_preference_loss(const pk_preference_config* c, const void* logits, int64_t ld, const int* targets,
+                       const int* seq_start, int64_t pairs, const float* ref_logp, int64_t rows, int64_t vocab,
+                       void* dlogits, int64_t dld, float* logp, float* margins, float* loss, void* workspace,
+                       size_t workspace_bytes, int dtype, void* stream);
+
+/* One AdamW step (nn::AdamW::step's formula, src/nn.cpp:301-321, bias corrections formed in 64 bits) over a list of
+ * tensors in a handful of launches, in place. With max_norm > 0 the gradients are scaled by min(1, max_norm / norm)
+ * as ops::clip_grad_norm does (src/ops.cpp:1046-1064), on the way: they are not written. norm (device, fp32)
+ * receives the global norm before the clip; it may be NULL without one.
+ * state_bits 32: m and v are fp32 [n]. 8: m is e4m3 (finite, no infinities) and v e5m2, one byte an element, each times
+ * the power of two of its block of 256 elements: m_scale, v_scale fp32 [ceil(n / 256)]. Zeroed memory is a fresh state
+ * in either. Values between two of the format's are rounded up or down at random with the value itself as the mean,
+ * drawn from (seed, the tensor's place in the list, the element's place in the tensor): give another seed each step. A v
+ * that is not zero does not become zero. A block in which a value is not finite becomes NaN.
+ * A tensor or state that is in the list twice is refused. */
+typedef struct pk_adamw_tensor {
+    float* p;
+    const void* g;           /* fp32 or bf16, the same for all (grad_dtype) */
+    void *m, *v;
+    float *m_scale, *v_scale;
+    void* copy;              /* NULL, or bf16 [n]: receives the new parameter rounded */
+    int64_t n;               /* may be 0 */
+} pk_adamw_tensor;
+typedef struct pk_adamw_config {
+    float lr, b1, b2, eps, wd, max_norm;
+    int32_t t;               /* step count, from 1 */
+    int32_t state_bits, grad_dtype;
+    uint32_t seed;
+} pk_adamw_config;
+size_t pk_adamw_many_workspace_bytes(const pk_adamw_tensor* host_tensors, int count, const pk_adamw_config* c);
+int pk_adamw_many(const pk_adamw_tensor* host_tensors, int count, const pk_adamw_config* c, void* workspace,
+                  size_t workspace_bytes, float* norm, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

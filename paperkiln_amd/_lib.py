@@ -37,6 +37,28 @@ class LlamaStats(C.Structure):
                 ("peak_activation_bytes", C.c_int64)]
 
 
+class QkShape(C.Structure):
+    _fields_ = [("B", C.c_int32), ("T", C.c_int32), ("Hq", C.c_int32), ("Hkv", C.c_int32), ("dk", C.c_int32), ("rotary", C.c_int32),
+                ("halves", C.c_int32), ("dtype", C.c_int32), ("eps", C.c_float), ("theta", C.c_double), ("pos_stride_b", C.c_int64)]
+
+
+class PolicyConfig(C.Structure):
+    _fields_ = [(n, C.c_float) for n in ("clip_low", "clip_high", "kl_coef", "scale", "upstream")]
+
+
+class PreferenceConfig(C.Structure):
+    _fields_ = [(n, C.c_float) for n in ("beta", "label_smoothing", "scale", "upstream")]
+
+
+class AdamWTensor(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("p", "g", "m", "v", "m_scale", "v_scale", "copy")] + [("n", C.c_int64)]
+
+
+class AdamWConfig(C.Structure):
+    _fields_ = [(n, C.c_float) for n in ("lr", "b1", "b2", "eps", "wd", "max_norm")] + [("t", C.c_int32), ("state_bits", C.c_int32),
+                                                                                       ("grad_dtype", C.c_int32), ("seed", C.c_uint32)]
+
+
 class PkError(RuntimeError):
     def __init__(self, code: int, msg: str):
         super().__init__(f"paperkiln_amd error {code}: {msg}")
@@ -53,7 +75,9 @@ EXPORTS = ["pk_last_error", "pk_init", "pk_attn_fwd", "pk_attn_bwd_workspace_byt
            "pk_llama_set_head_chunk",
            "pk_op_add", "pk_op_mul", "pk_op_scale", "pk_op_axpy", "pk_op_fill", "pk_op_silu_fwd", "pk_op_silu_bwd", "pk_op_silu_mul_fwd", "pk_op_silu_mul_bwd",
            "pk_op_rmsnorm_fwd", "pk_op_rmsnorm_bwd", "pk_op_rope", "pk_op_embedding_fwd", "pk_op_embedding_bwd",
-           "pk_op_cross_entropy", "pk_op_adamw", "pk_op_sumsq", "pk_op_gemm", "pk_set_gemm_backend", "pk_set_head_kernel"]
+           "pk_op_cross_entropy", "pk_op_adamw", "pk_op_sumsq", "pk_op_gemm", "pk_set_gemm_backend", "pk_set_head_kernel",
+           "pk_qk_norm_rope_fwd", "pk_qk_norm_rope_bwd_workspace_bytes", "pk_qk_norm_rope_bwd", "pk_token_logprobs_fwd", "pk_token_logprobs_bwd",
+           "pk_policy_loss", "pk_preference_loss_workspace_bytes", "pk_preference_loss", "pk_adamw_many_workspace_bytes", "pk_adamw_many"]
 
 
 def lib() -> C.CDLL:
@@ -117,6 +141,19 @@ def lib() -> C.CDLL:
         L.pk_op_gemm.argtypes = [vp, ci, vp, ci, vp, i64, i64, i64, ci, ci, ci, vp]
         L.pk_set_gemm_backend.argtypes = [ci]
         L.pk_set_head_kernel.argtypes = [ci]
+        QS, AT, AC, sz = C.POINTER(QkShape), C.POINTER(AdamWTensor), C.POINTER(AdamWConfig), C.c_size_t
+        L.pk_qk_norm_rope_fwd.argtypes = [QS, T4, T4, vp, vp, vp, T4, T4, vp]
+        L.pk_qk_norm_rope_bwd_workspace_bytes.argtypes = [QS]
+        L.pk_qk_norm_rope_bwd.argtypes = [QS, T4, T4, T4, T4, vp, vp, vp, T4, T4, vp, vp, vp, sz, vp]
+        L.pk_token_logprobs_fwd.argtypes = [vp, i64, vp, i64, i64, cf, vp, vp, ci, vp]
+        L.pk_token_logprobs_bwd.argtypes = [vp, i64, vp, vp, vp, i64, i64, cf, vp, i64, ci, vp]
+        L.pk_policy_loss.argtypes = [C.POINTER(PolicyConfig), vp, i64, vp, vp, vp, vp, vp, i64, i64, vp, i64, vp, vp, vp, ci, vp]
+        L.pk_preference_loss_workspace_bytes.argtypes = [i64, i64]
+        L.pk_preference_loss.argtypes = [C.POINTER(PreferenceConfig), vp, i64, vp, vp, i64, vp, i64, i64, vp, i64, vp, vp, vp, vp, sz, ci, vp]
+        L.pk_adamw_many_workspace_bytes.argtypes = [AT, ci, AC]
+        L.pk_adamw_many.argtypes = [AT, ci, AC, vp, sz, vp, vp]
+        for fn in (L.pk_qk_norm_rope_bwd_workspace_bytes, L.pk_preference_loss_workspace_bytes, L.pk_adamw_many_workspace_bytes):
+            fn.restype = sz
         _lib = L
     return _lib
 

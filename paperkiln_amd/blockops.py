@@ -6,11 +6,13 @@ torch CUDA tensors, fp32 or bf16, contiguous. There is no CPU path.
 from __future__ import annotations
 
 import ctypes as C
+from typing import NamedTuple
 
 import torch
 
 from . import _lib
 from ._lib import PK_BF16, PK_F32, check
+from .ops import _native
 
 
 def _dt(t: torch.Tensor) -> int:
@@ -169,6 +171,53 @@ def adamw_(p, g, m, v, lr, b1=0.9, b2=0.999, eps=1e-8, wd=0.01, t=1):
     _chk(p, g, m, v)
     check(_lib.lib().pk_op_adamw(_p(p), _p(g), _p(m), _p(v), p.numel(), lr, b1, b2, eps, wd, int(t), _s()))
     return p
+
+
+class AdamWState(NamedTuple):
+    """The moments of ``adamw_many_``, one tensor for each parameter. In 32 bits m and v are float32 and the scales None; in 8 bits m
+    is float8_e4m3fn, v float8_e5m2, and element i of either stands for its own value times scale[i // 256]."""
+    m: list
+    v: list
+    m_scale: list | None = None
+    v_scale: list | None = None
+
+
+def adamw_state(params, bits=32):
+    """Fresh moments (zeros) for ``adamw_many_``, in 32 bits or in 8."""
+    if bits not in (8, 32):
+        raise RuntimeError("adamw_state: states are held in 8 or in 32 bits")
+    zeros = lambda n, dt, p: torch.zeros(n, dtype=dt, device=p.device)  # noqa: E731
+    if bits == 32:
+        return AdamWState(*([zeros(p.shape, torch.float32, p) for p in params] for _ in range(2)))
+    return AdamWState(*([zeros(p.shape, dt, p) for p in params] for dt in (torch.float8_e4m3fn, torch.float8_e5m2)),
+                      *([zeros((p.numel() + 255) // 256, torch.float32, p) for p in params] for _ in range(2)))
+
+
+def adamw_many_(params, grads, state, lr, b1=0.9, b2=0.999, eps=1e-8, wd=0.01, t=1, max_norm=0.0, copies=None, seed=0):
+    """nn::AdamW::step on a list of fp32 parameters in a handful of launches, in place; ``clip_grad_norm_`` in front of it where
+    max_norm > 0 (the gradients themselves are left as they are), the global norm returned on the device. grads: fp32 or bf16, all the
+    same; None leaves its parameter and state untouched. copies: bf16 tensors that receive the new parameters. The 8-bit states are
+    rounded up or down at random, drawn from ``seed``: give another one each step (the step count will do)."""
+    return _native.adamw_many(params, grads, state.m, state.v, state.m_scale, state.v_scale, copies, lr, b1, b2, eps, wd, t, max_norm, seed)
+
+
+def policy_loss(logits, targets, old_logp, advantages, weights, clip_low=0.2, clip_high=0.2, ref_logp=None, kl_coef=0.0, scale=1.0,
+                upstream=1.0, out=None):
+    """Clipped policy loss with a KL term, in one pass over the logits: (loss, dlogits, logp), all on the device. With rho = exp(logp -
+    old_logp), A = advantages and d = ref_logp - logp the loss is the sum over rows of weights * (-min(rho A, clamp(rho, 1 - clip_low, 1 +
+    clip_high) A) + kl_coef (exp(d) - d - 1)); dlogits is the gradient of upstream * loss, for ``logits.backward(dlogits)``. logits: [rows,
+    vocab] fp32 or bf16 (any row stride), targets int32 [rows], the others float32 [rows]. The weights carry mask and normalisation: a
+    row of weight 0 or of a negative target is not read and gets zeros. ``out`` may be the logits."""
+    return _native.policy_loss(logits, targets, old_logp, ref_logp, advantages, weights, clip_low, clip_high, kl_coef, scale, upstream, out)
+
+
+def preference_loss(logits, targets, seq_start, ref_logp, beta=0.1, label_smoothing=0.0, scale=1.0, upstream=1.0, out=None):
+    """Preference loss over pairs of sequences: (loss, dlogits, margins, logp), all on the device. Sequence s holds rows seq_start[s] ..
+    seq_start[s+1]-1 (int32 [2 pairs + 1], ascending), the chosen answers first, then the rejected ones in the same order; rows with a
+    negative target count nothing. margins = beta * (sum of logp - ref_logp over the chosen answer - the same over the rejected one); the loss
+    is the mean of -(1 - label_smoothing) log sigma(margin) - label_smoothing log sigma(-margin), dlogits the gradient of upstream * loss.
+    ``out`` may be the logits."""
+    return _native.preference_loss(logits, targets, seq_start, ref_logp, beta, label_smoothing, scale, upstream, out)
 
 
 def clip_grad_norm_(grads, max_norm):

@@ -1,0 +1,315 @@
+// Log-probabilities of chosen tokens from a model's logits, their gradient, and the two losses that are built on them.
+//
+//   z = scale * logits     lse = log sum_j exp z_j     logp = z_t - lse     d logp / d logits_j = scale ([j = t] - exp(z_j - lse))
+//   policy:      rho = exp(logp - old);  L = -min(rho A, clamp(rho, 1 - lo, 1 + hi) A) + kl (exp(d) - d - 1), d = ref - logp;  loss = sum_r w_r L_r
+//                dL/dlogp = -(rho A where rho A <= clamp(rho) A, else 0) + kl (1 - exp d)
+//   preference:  s = sum over a sequence's rows of logp - ref;  u = beta (s_chosen - s_rejected);  loss = mean over pairs of
+//                -(1 - e) log sigma(u) - e log sigma(-u);  dL/du = e sigma(u) - (1 - e) sigma(-u)
+//
+// What bounds it: memory, the logits read and their gradient written. A policy row's coefficient depends on its own row only, so its gradient leaves
+// in the pass that reads it. A preference row's depends on both sequences of its pair, so the logits are read twice.
+// Exponentials are taken in base 2 against the largest logit; sums are in 32 bits inside a wavefront and in 64 across them, and a token's
+// log-probability, a difference of near numbers, is formed in 64, and stays there until it has been added to its loss.
+#include "post.h"
+
+namespace pk {
+namespace {
+
+constexpr float LOG2E = 1.44269504088896340736f;
+constexpr double LN2 = 0.693147180559945309417;
+
+struct Loss {
+    const void* logits;
+    void* dlogits;
+    int64_t ld, dld, rows;
+    const int* targets;
+    int vocab;
+    float scale;
+    float *logp, *lse;        // written; lse may be null
+    double* fine;             // LOGP: the log-probability in 64 bits, or null
+    float* clear;             // LOGP: a word per row to set to zero, or null
+    const float *lse_in, *coef;  // GRAD
+    bool backwards;           // GRAD: the last rows first
+    const float *old_logp, *ref_logp, *adv, *weights;  // POLICY; ref_logp may be null
+    double* row_loss;
+    float clip_low, clip_high, kl, upstream;
+};
+enum Mode { LOGP, GRAD, POLICY };
+
+// A policy row's loss and the derivative of it by the row's log-probability, both before the row's weight.
+__device__ inline void policy_row(const Loss& a, int64_t r, double logp, double& loss, double& slope) {
+    const double adv = a.adv[r], ratio = exp(logp - static_cast<double>(a.old_logp[r]));
+    const double held = fmin(fmax(ratio, 1.0 - static_cast<double>(a.clip_low)), 1.0 + static_cast<double>(a.clip_high));
+    const double free_ = ratio * adv, stop = held * adv;
+    const bool open = !(free_ > stop);  // a ratio that is no number stays one
+    loss = -(open ? free_ : stop);
+    slope = open ? -free_ : 0.0;
+    if (a.ref_logp) {
+        const double d = static_cast<double>(a.ref_logp[r]) - logp, e = exp(d);
+        loss += a.kl * (e - d - 1.0);
+        slope += a.kl * (1.0 - e);
+    }
+}
+
+// Any size, stride and alignment: a workgroup takes a row and reads it element by element, twice where a gradient is written.
+constexpr int ANY_NT = 256;
+template <typename T, Mode MODE>
+__global__ __launch_bounds__(ANY_NT) void rows_any(Loss a) {
+    __shared__ float sh_m[ANY_NT / 64];
+    __shared__ double sh_s[ANY_NT / 64];
+    const int64_t r = MODE == GRAD && a.backwards ? a.rows - 1 - blockIdx.x : blockIdx.x;
+    const int tid = threadIdx.x, V = a.vocab, t = a.targets[r];
+    const T* x = static_cast<const T*>(a.logits) + r * a.ld;
+    T* dx = MODE == LOGP ? nullptr : static_cast<T*>(a.dlogits) + r * a.dld;
+    if (MODE == LOGP && a.clear && tid == 0) a.clear[r] = 0.0f;
+    bool skip = t < 0;
+    float coef = 0.0f;
+    if (MODE == POLICY) skip = skip || a.weights[r] == 0.0f;
+    if (MODE == GRAD) coef = a.coef[r] * a.scale, skip = skip || coef == 0.0f;
+    if (skip) {
+        if (MODE != GRAD && tid == 0) {
+            a.logp[r] = 0.0f;
+            if (a.lse) a.lse[r] = 0.0f;
+            if (MODE == POLICY) a.row_loss[r] = 0.0;
+        }
+        if (MODE != LOGP)
+            for (int j = tid; j < V; j += ANY_NT) put(dx, j, 0.0f);
+        return;
+    }
+    const float s2 = a.scale * LOG2E;
+    const float xt = t < V ? elem(x, t) : NAN;  // read before the row is written over; a token that is no word has no probability
+    float lse2, target_grad;
+    if (MODE == GRAD) {
+        const double lse = a.lse_in[r];
+        lse2 = static_cast<float>(lse / LN2);
+        target_grad = coef * static_cast<float>(-expm1((static_cast<double>(xt) * s2 - lse / LN2) * LN2));
+        if (t >= V) coef = NAN;
+    } else {
+        float m = -INFINITY, s = 0.0f;
+        for (int j = tid; j < V; j += ANY_NT) m = fmaxf(m, elem(x, j));
+        for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+        if ((tid & 63) == 0) sh_m[tid >> 6] = m;
+        __syncthreads();
+        m = sh_m[0];
+        for (int w = 1; w < ANY_NT / 64; ++w) m = fmaxf(m, sh_m[w]);
+        const float m2 = m * s2;
+        for (int j = tid; j < V; j += ANY_NT) s += __builtin_amdgcn_exp2f(fmaf(elem(x, j), s2, -m2));
+        s = group_sum<64>(s);
+        if ((tid & 63) == 0) sh_s[tid >> 6] = s;
+        __syncthreads();
+        double sum = 0.0;
+        for (int w = 0; w < ANY_NT / 64; ++w) sum += sh_s[w];
+        // the token's logit by the same product as the sum's: what scale * log2(e) was rounded by then drops out where the token is likely
+        const double lse_2 = static_cast<double>(m2) + log2(sum), lse = lse_2 * LN2, logp = (static_cast<double>(xt) * s2 - lse_2) * LN2;
+        lse2 = static_cast<float>(lse_2);
+        if (MODE == POLICY) {
+            double loss, slope;
+            policy_row(a, r, logp, loss, slope);
+            const double w = a.weights[r];
+            coef = static_cast<float>(w * slope * a.upstream * a.scale);
+            target_grad = coef * static_cast<float>(-expm1(logp));
+            if (tid == 0) a.row_loss[r] = w * loss;
+        }
+        if (tid == 0) {
+            a.logp[r] = static_cast<float>(logp);
+            if (a.lse) a.lse[r] = static_cast<float>(lse);
+            if (MODE == LOGP && a.fine) a.fine[r] = logp;
+        }
+    }
+    if (MODE != LOGP)
+        for (int j = tid; j < V; j += ANY_NT) put(dx, j, j == t ? target_grad : -coef * __builtin_amdgcn_exp2f(fmaf(elem(x, j), s2, -lse2)));
+}
+
+// n values added up in 64 bits in a fixed order, times a factor.
+__global__ __launch_bounds__(1024) void loss_sum(const double* x, int64_t n, double factor, float* out) {
+    __shared__ double sh[16];
+    double s = 0.0;
+    for (int64_t i = threadIdx.x; i < n; i += 1024) s += x[i];
+    for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o);
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    for (int w = 1; w < 16; ++w) s += sh[w];
+    *out = static_cast<float>(s * factor);
+}
+
+struct Pairs {
+    const int* starts;  // 2 pairs + 1
+    const int* targets;
+    const double* logp;
+    const float* ref;
+    float *coef, *margins;
+    double* losses;
+    int64_t rows;
+    int pairs;
+    float beta, smoothing, upstream;
+};
+// A workgroup takes a pair: both sequences' sums, the pair's loss, and for every row of the two what its gradient is multiplied by.
+constexpr int PAIR_NT = 256;
+__global__ __launch_bounds__(PAIR_NT) void pair_loss(Pairs a) {
+    __shared__ double sh[2][PAIR_NT / 64];
+    const int tid = threadIdx.x, seq[2] = {static_cast<int>(blockIdx.x), a.pairs + static_cast<int>(blockIdx.x)};
+    int64_t begin[2], end[2];
+    double sum[2] = {0.0, 0.0};
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {  // offsets that lie are held to the rows there are
+        begin[k] = min(max(static_cast<int64_t>(a.starts[seq[k]]), int64_t{0}), a.rows);
+        end[k] = min(max(static_cast<int64_t>(a.starts[seq[k] + 1]), int64_t{0}), a.rows);
+        for (int64_t r = begin[k] + tid; r < end[k]; r += PAIR_NT)
+            if (a.targets[r] >= 0) sum[k] += a.logp[r] - static_cast<double>(a.ref[r]);
+        for (int o = 32; o >= 1; o >>= 1) sum[k] += __shfl_xor(sum[k], o);
+        if ((tid & 63) == 0) sh[k][tid >> 6] = sum[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        sum[k] = 0.0;
+        for (int w = 0; w < PAIR_NT / 64; ++w) sum[k] += sh[k][w];
+    }
+    const double u = a.beta * (sum[0] - sum[1]), e = a.smoothing;
+    const double small = exp(-fabs(u)), up = 1.0 / (1.0 + small), down = small / (1.0 + small);  // sigma(|u|), sigma(-|u|)
+    const double yes = u >= 0.0 ? up : down, no = u >= 0.0 ? down : up;                          // sigma(u), sigma(-u); no number stays none
+    const double tail = log1p(small), lost_no = fmax(-u, 0.0) + tail, lost_yes = fmax(u, 0.0) + tail;  // -log sigma(u), -log sigma(-u)
+    const float slope = static_cast<float>((e * yes - (1.0 - e) * no) * a.beta * a.upstream / a.pairs);
+    if (tid == 0) {
+        a.margins[blockIdx.x] = static_cast<float>(u);
+        a.losses[blockIdx.x] = u != u ? u : (1.0 - e) * lost_no + e * lost_yes;
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+        for (int64_t r = begin[k] + tid; r < end[k]; r += PAIR_NT) a.coef[r] = k ? -slope : slope;
+}
+
+template <Mode MODE>
+int launch_rows(const Loss& a, int dtype, hipStream_t st) {
+    if (a.rows == 0) return PK_OK;
+    const dim3 grid(static_cast<unsigned>(a.rows));
+    if (dtype == PK_BF16)
+        rows_any<uint16_t, MODE><<<grid, ANY_NT, 0, st>>>(a);
+    else
+        rows_any<float, MODE><<<grid, ANY_NT, 0, st>>>(a);
+    return launched();
+}
+
+// What every entry asks of its logits; dlogits only where it writes them: over the logits, row for row, or clear of them.
+int check(const char* who, const void* logits, int64_t ld, const int* targets, int64_t rows, int64_t vocab, float scale, int dtype, bool writes,
+          const void* dlogits, int64_t dld) {
+    const std::string w(who);
+    if (rows < 0 || rows > INT32_MAX || vocab <= 0 || vocab > (1 << 30)) return fail(PK_ERR_SHAPE, w + ": shape mismatch (rows or vocabulary out of range)");
+    if (!known_dtype(dtype)) return fail(PK_ERR_ARGUMENT, w + ": dtype must be PK_F32 or PK_BF16");
+    if (!(scale > 0.0f) || !std::isfinite(scale)) return fail(PK_ERR_ARGUMENT, w + ": scale must be positive");
+    if (ld < 0 || (writes && rows > 1 && dld < vocab)) return fail(PK_ERR_SHAPE, w + ": rows of logits overlap");
+    if (rows == 0) return PK_OK;
+    if (!logits || !targets || (writes && !dlogits)) return fail(PK_ERR_ARGUMENT, w + ": null pointer");
+    if (writes && !(logits == dlogits && (ld == dld || rows == 1))) {
+        const uintptr_t es = static_cast<uintptr_t>(elem_size(dtype)), x = reinterpret_cast<uintptr_t>(logits), y = reinterpret_cast<uintptr_t>(dlogits);
+        const uintptr_t xe = x + ((rows - 1) * ld + vocab) * es, ye = y + ((rows - 1) * dld + vocab) * es;
+        // two matrices may lie in one another's gaps; what no gap can hold is refused
+        if (x < ye && y < xe && !(ld == dld && ld >= 2 * vocab && (y > x ? y - x : x - y) % (ld * es) >= vocab * es &&
+                                  (y > x ? y - x : x - y) % (ld * es) <= (ld - vocab) * es))
+            return fail(PK_ERR_ARGUMENT, w + ": dlogits may lie where the logits do, row for row, or clear of them");
+    }
+    return PK_OK;
+}
+
+void touch(std::initializer_list<const void*> used, void* stream) {
+    for (const void* p : used)
+        if (p) dev_touch(p, stream);
+}
+
+size_t pad(size_t bytes) { return (bytes + 255) & ~size_t{255}; }
+
+}  // namespace
+}  // namespace pk
+
+using namespace pk;
+
+extern "C" {
+
+int pk_token_logprobs_fwd(const void* logits, int64_t ld, const int* targets, int64_t rows, int64_t vocab, float scale, float* logp, float* lse,
+                          int dtype, void* stream) {
+    return c_entry([&] {
+        if (int rc = check("pk_token_logprobs_fwd", logits, ld, targets, rows, vocab, scale, dtype, false, nullptr, 0)) return rc;
+        if (rows > 0 && !logp) return fail(PK_ERR_ARGUMENT, "pk_token_logprobs_fwd: null pointer");
+        touch({logits, targets, logp, lse}, stream);
+        Loss a{};
+        a.logits = logits, a.ld = ld, a.targets = targets, a.rows = rows, a.vocab = static_cast<int>(vocab), a.scale = scale, a.logp = logp, a.lse = lse;
+        return launch_rows<LOGP>(a, dtype, static_cast<hipStream_t>(stream));
+    });
+}
+
+int pk_token_logprobs_bwd(const void* logits, int64_t ld, const int* targets, const float* lse, const float* dlogp, int64_t rows, int64_t vocab,
+                          float scale, void* dlogits, int64_t dld, int dtype, void* stream) {
+    return c_entry([&] {
+        if (int rc = check("pk_token_logprobs_bwd", logits, ld, targets, rows, vocab, scale, dtype, true, dlogits, dld)) return rc;
+        if (rows > 0 && (!lse || !dlogp)) return fail(PK_ERR_ARGUMENT, "pk_token_logprobs_bwd: null pointer");
+        touch({logits, targets, lse, dlogp, dlogits}, stream);
+        Loss a{};
+        a.logits = logits, a.ld = ld, a.targets = targets, a.rows = rows, a.vocab = static_cast<int>(vocab), a.scale = scale;
+        a.dlogits = dlogits, a.dld = dld, a.lse_in = lse, a.coef = dlogp;
+        return launch_rows<GRAD>(a, dtype, static_cast<hipStream_t>(stream));
+    });
+}
+
+int pk_policy_loss(const pk_policy_config* c, const void* logits, int64_t ld, const int* targets, const float* old_logp, const float* ref_logp,
+                   const float* advantages, const float* weights, int64_t rows, int64_t vocab, void* dlogits, int64_t dld, float* logp,
+                   double* row_loss, float* loss, int dtype, void* stream) {
+    return c_entry([&] {
+        if (!c || !loss) return fail(PK_ERR_ARGUMENT, "pk_policy_loss: null pointer");
+        if (int rc = check("pk_policy_loss", logits, ld, targets, rows, vocab, c->scale, dtype, true, dlogits, dld)) return rc;
+        if (rows > 0 && (!old_logp || !advantages || !weights || !logp || !row_loss)) return fail(PK_ERR_ARGUMENT, "pk_policy_loss: null pointer");
+        if (!(c->clip_low >= 0.0f) || !(c->clip_high >= 0.0f)) return fail(PK_ERR_ARGUMENT, "pk_policy_loss: the clip's widths must not be negative");
+        if (!std::isfinite(c->kl_coef) || !std::isfinite(c->upstream)) return fail(PK_ERR_ARGUMENT, "pk_policy_loss: kl_coef and upstream must be finite");
+        if (c->kl_coef != 0.0f && !ref_logp && rows > 0) return fail(PK_ERR_ARGUMENT, "pk_policy_loss: a KL term needs ref_logp");
+        touch({logits, targets, old_logp, ref_logp, advantages, weights, dlogits, logp, row_loss, loss}, stream);
+        hipStream_t st = static_cast<hipStream_t>(stream);
+        Loss a{};
+        a.logits = logits, a.ld = ld, a.targets = targets, a.rows = rows, a.vocab = static_cast<int>(vocab), a.scale = c->scale;
+        a.dlogits = dlogits, a.dld = dld, a.logp = logp, a.row_loss = row_loss;
+        a.old_logp = old_logp, a.ref_logp = c->kl_coef != 0.0f ? ref_logp : nullptr, a.adv = advantages, a.weights = weights;
+        a.clip_low = c->clip_low, a.clip_high = c->clip_high, a.kl = c->kl_coef, a.upstream = c->upstream;
+        if (int rc = launch_rows<POLICY>(a, dtype, st)) return rc;
+        loss_sum<<<1, 1024, 0, st>>>(row_loss, rows, 1.0, loss);
+        return launched();
+    });
+}
+
+size_t pk_preference_loss_workspace_bytes(int64_t rows, int64_t pairs) {
+    if (rows < 0 || pairs < 0) return 0;
+    return 2 * pad(sizeof(float) * static_cast<size_t>(rows)) + pad(sizeof(double) * static_cast<size_t>(rows)) + pad(sizeof(double) * static_cast<size_t>(pairs));
+}
+
+int pk_preference_loss(const pk_preference_config* c, const void* logits, int64_t ld, const int* targets, const int* seq_start, int64_t pairs,
+                       const float* ref_logp, int64_t rows, int64_t vocab, void* dlogits, int64_t dld, float* logp, float* margins, float* loss,
+                       void* workspace, size_t workspace_bytes, int dtype, void* stream) {
+    return c_entry([&] {
+        if (!c || !loss || !margins || !seq_start) return fail(PK_ERR_ARGUMENT, "pk_preference_loss: null pointer");
+        if (pairs < 1 || pairs > (1 << 28)) return fail(PK_ERR_SHAPE, "pk_preference_loss: shape mismatch (at least one pair is wanted)");
+        if (int rc = check("pk_preference_loss", logits, ld, targets, rows, vocab, c->scale, dtype, true, dlogits, dld)) return rc;
+        if (rows > 0 && (!ref_logp || !logp)) return fail(PK_ERR_ARGUMENT, "pk_preference_loss: null pointer");
+        if (!std::isfinite(c->beta) || !std::isfinite(c->upstream)) return fail(PK_ERR_ARGUMENT, "pk_preference_loss: beta and upstream must be finite");
+        if (!(c->label_smoothing >= 0.0f && c->label_smoothing <= 1.0f))
+            return fail(PK_ERR_ARGUMENT, "pk_preference_loss: label_smoothing must lie between 0 and 1");
+        if (!workspace || workspace_bytes < pk_preference_loss_workspace_bytes(rows, pairs) || !aligned(workspace, 8))
+            return fail(PK_ERR_WORKSPACE, "pk_preference_loss: workspace too small (pk_preference_loss_workspace_bytes)");
+        touch({logits, targets, seq_start, ref_logp, dlogits, logp, margins, loss, workspace}, stream);
+        hipStream_t st = static_cast<hipStream_t>(stream);
+        char* ws = static_cast<char*>(workspace);
+        const size_t singles = pad(sizeof(float) * static_cast<size_t>(rows)), doubles = pad(sizeof(double) * static_cast<size_t>(rows));
+        float *lse = reinterpret_cast<float*>(ws), *coef = reinterpret_cast<float*>(ws + singles);
+        double *fine = reinterpret_cast<double*>(ws + 2 * singles), *losses = reinterpret_cast<double*>(ws + 2 * singles + doubles);
+        Loss a{};
+        a.logits = logits, a.ld = ld, a.targets = targets, a.rows = rows, a.vocab = static_cast<int>(vocab), a.scale = c->scale;
+        a.logp = logp, a.lse = lse, a.fine = fine, a.clear = coef;
+        if (int rc = launch_rows<LOGP>(a, dtype, st)) return rc;
+        pair_loss<<<dim3(static_cast<unsigned>(pairs)), PAIR_NT, 0, st>>>(
+            Pairs{seq_start, targets, fine, ref_logp, coef, margins, losses, rows, static_cast<int>(pairs), c->beta, c->label_smoothing, c->upstream});
+        if (int rc = launched()) return rc;
+        loss_sum<<<1, 1024, 0, st>>>(losses, pairs, 1.0 / static_cast<double>(pairs), loss);
+        if (int rc = launched()) return rc;
+        a.dlogits = dlogits, a.dld = dld, a.lse_in = lse, a.coef = coef, a.backwards = true;
+        return launch_rows<GRAD>(a, dtype, st);
+    });
+}
+
+}  // extern "C"

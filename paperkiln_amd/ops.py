@@ -112,6 +112,44 @@ def attention(q, k, v, scale, causal=True, window=0, sinks=0):
     return _native.attention(q, k, v, scale, causal, window, sinks)
 
 
+def qk_norm_rope_fwd(q, k, wq, wk, pos, theta, eps=1e-5, rotary_dim=0, halves=False, out=None):
+    """Queries and keys on their way into attention, in one pass (pk_qk_norm_rope_fwd): every head's row times
+    1/sqrt(mean(x^2) + eps) times its weight, then turned by its token's position. q: [B,T,Hq,dk], k: [B,T,Hkv,dk] (any
+    batch/token/head strides, so heads of a fused projection are read in place; dk even, at most 256), wq, wk: float32 [dk],
+    pos: int32 [T] or [B,T]. Pairs are columns 2i and 2i+1 as in ``blockops.apply_rope``, or i and i + rotary_dim/2 with
+    ``halves``; rotary_dim 0 turns all columns. Returns (yq, yk); ``out`` may supply them, q and k themselves included."""
+    return _native.qk_norm_rope_fwd(q, k, wq, wk, pos, theta, eps, rotary_dim, halves, out)
+
+
+def qk_norm_rope_bwd(dyq, dyk, q, k, wq, wk, pos, theta, eps=1e-5, rotary_dim=0, halves=False, out=None):
+    """Gradients of ``qk_norm_rope_fwd`` from its inputs: (dq, dk, dwq, dwk), the weights' in float32, summed in a fixed
+    order. ``out`` may supply (dq, dk): views of a fused gradient, or dyq and dyk themselves."""
+    return _native.qk_norm_rope_bwd(dyq, dyk, q, k, wq, wk, pos, theta, eps, rotary_dim, halves, out)
+
+
+def qk_norm_rope(q, k, wq, wk, pos, theta, eps=1e-5, rotary_dim=0, halves=False):
+    """``qk_norm_rope_fwd``, differentiable in q, k, wq and wk; keeps nothing but its inputs."""
+    return _native.qk_norm_rope(q, k, wq, wk, pos, theta, eps, rotary_dim, halves)
+
+
+def token_logprobs_fwd(logits, targets, scale=1.0):
+    """Log-probabilities of chosen tokens under softmax(scale * logits): (logp, lse), float32 [rows]. logits: [rows, vocab]
+    (any row stride), targets: int32 [rows]. A row whose target is negative is not read: logp and lse 0. A target
+    past the vocabulary gives NaN; a logit of -inf is a word without probability."""
+    return _native.token_logprobs_fwd(logits, targets, scale)
+
+
+def token_logprobs_bwd(logits, targets, lse, dlogp, scale=1.0, out=None):
+    """dlogits of ``token_logprobs_fwd`` for the rows' gradients dlogp; rows whose dlogp is 0 are not read and get zeros. ``out``
+    may be the logits."""
+    return _native.token_logprobs_bwd(logits, targets, lse, dlogp, scale, out)
+
+
+def token_logprobs(logits, targets, scale=1.0):
+    """logp of ``token_logprobs_fwd``, differentiable in the logits."""
+    return _native.token_logprobs(logits, targets, scale)
+
+
 class _CheckpointFn(torch.autograd.Function):
     """checkpoint(fn, x) of the reference (src/autograd.cpp:68-102): the forward runs fn with the
     tape off and keeps only its input and output; the backward re-runs fn on a detached copy of the

@@ -5,50 +5,11 @@
 // path (ctypes structures, torch.empty and tensor properties one by one, a Python autograd.Function whose backward takes
 // the interpreter lock on the engine's thread) cost 34 us for a forward + backward pair and 165-195 us under autograd.
 // All arithmetic still runs in libpaperkiln_amd.so.
-#include <Python.h>
-#include <ATen/ATen.h>
-#include <ATen/hip/HIPContext.h>
-#include <torch/csrc/Dtype.h>
-#include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/function.h>
-#include <torch/csrc/autograd/functions/utils.h>
-#include <torch/csrc/autograd/python_variable.h>
-#include <torch/csrc/autograd/saved_variable.h>
-#include <torch/csrc/utils/python_numbers.h>
-
-#include <mutex>
-#include <string>
-#include <utility>
-#include <vector>
-
-#include "paperkiln_amd.h"
+#include "torch_args.h"
 
 namespace {
 
-using at::Tensor;
-using torch::autograd::Node;
-using torch::autograd::SavedVariable;
-using torch::autograd::variable_list;
-
-PyObject* g_error = nullptr;  // paperkiln_amd._lib.PkError
-
-// A refused C ABI call as the package's own exception, on any thread (the autograd engine's included).
-void check(int rc) {
-    if (rc == PK_OK) return;
-    const std::string msg = pk_last_error();
-    pybind11::gil_scoped_acquire gil;
-    if (PyObject* e = PyObject_CallFunction(g_error, "is", rc, msg.c_str())) {
-        PyErr_SetObject(g_error, e);
-        Py_DECREF(e);
-    }
-    throw python_error();
-}
-
-int dtype_code(at::ScalarType t) {
-    if (t == at::kFloat) return PK_F32;
-    if (t == at::kBFloat16) return PK_BF16;
-    throw std::runtime_error("dtype must be float32 or bfloat16");
-}
+using namespace pk_torch;
 
 struct Mask {
     double scale;
@@ -78,12 +39,6 @@ pk_attn_shape shape_of(const Tensor& q, const Tensor& k, const Mask& m, at::Scal
     s.scale = static_cast<float>(m.scale);
     s.dtype = dtype_code(q.scalar_type()), s.grad_dtype = dtype_code(grad);
     return s;
-}
-
-void* stream() { return at::hip::getCurrentHIPStream().stream(); }
-
-Tensor empty_of(at::IntArrayRef sizes, at::ScalarType t, const Tensor& like) {
-    return at::empty(sizes, like.options().dtype(t).memory_format(c10::nullopt));
 }
 
 std::pair<Tensor, Tensor> forward(const Tensor& q, const Tensor& k, const Tensor& v, const Mask& m) {
@@ -172,33 +127,7 @@ Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const Mask& 
 
 // ---- Python side: positional arguments in the order ops.py passes them ----
 
-const Tensor& tensor_arg(PyObject* o, const char* what) {
-    if (!THPVariable_Check(o)) throw torch::TypeError(std::string(what) + " must be a tensor, not " + Py_TYPE(o)->tp_name);
-    return THPVariable_Unpack(o);
-}
-int int_arg(PyObject* o) {  // what Python's int() takes, inside 32 bits
-    PyObject* i = PyNumber_Long(o);
-    if (!i) throw python_error();
-    const long x = PyLong_AsLong(i);
-    Py_DECREF(i);
-    if (x == -1 && PyErr_Occurred()) throw python_error();
-    return static_cast<int>(x);
-}
-double float_arg(PyObject* o) {
-    const double x = PyFloat_AsDouble(o);
-    if (x == -1.0 && PyErr_Occurred()) throw python_error();
-    return x;
-}
-bool bool_arg(PyObject* o) {
-    const int x = PyObject_IsTrue(o);
-    if (x < 0) throw python_error();
-    return x != 0;
-}
 Mask mask_args(PyObject* const* a) { return Mask{float_arg(a[0]), bool_arg(a[1]), int_arg(a[2]), int_arg(a[3]), 0}; }
-void expect(Py_ssize_t n, Py_ssize_t want) {
-    if (n != want) throw torch::TypeError("expected " + std::to_string(want) + " arguments, got " + std::to_string(n));
-}
-
 // (q, k, v, scale, causal, window, sinks) -> (o, lse)
 PyObject* py_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
@@ -309,5 +238,8 @@ PyMODINIT_FUNC PyInit__torch_ops() {
     if (!lib) return nullptr;
     g_error = PyObject_GetAttrString(lib, "PkError");
     Py_DECREF(lib);
-    return g_error ? PyModule_Create(&g_module) : nullptr;
+    if (!g_error) return nullptr;
+    PyObject* module = PyModule_Create(&g_module);
+    if (module && PyModule_AddFunctions(module, pk_torch::post_methods()) < 0) Py_CLEAR(module);
+    return module;
 }

@@ -1,0 +1,153 @@
+"""What the post-training operators refuse, asked of the C ABI with pointers that are never followed (no GPU needed): every refusal comes before the first
+launch and leaves a message."""
+import ctypes as C
+import math
+
+import pytest
+
+from paperkiln_amd import _lib
+
+SHAPE, ARGUMENT, WORKSPACE = 1, 2, 3
+SOME = C.c_void_p(1 << 20)          # stands for a device pointer
+FAR = C.c_void_p(1 << 40)
+CLOSE = C.c_void_p((1 << 20) + 64)
+
+
+def T4(p=1 << 20):
+    return C.byref(_lib.Tensor4(p, 64, 64, 64))
+
+
+def qk(**kw):
+    d = dict(B=1, T=2, Hq=2, Hkv=1, dk=64, rotary=0, halves=0, dtype=_lib.PK_BF16, eps=1e-5, theta=1e4, pos_stride_b=0)
+    d.update(kw)
+    return _lib.QkShape(*[d[n] for n, _ in _lib.QkShape._fields_])
+
+
+QK_REFUSED = [(dict(dk=63), SHAPE), (dict(dk=258), SHAPE), (dict(dk=0), SHAPE), (dict(Hq=0), SHAPE), (dict(Hkv=-1), SHAPE), (dict(B=-1), SHAPE), (dict(T=-1), SHAPE),
+              (dict(rotary=3), SHAPE), (dict(rotary=66), SHAPE), (dict(rotary=-2), SHAPE), (dict(dtype=2), ARGUMENT), (dict(theta=0.0), ARGUMENT),
+              (dict(theta=math.nan), ARGUMENT), (dict(theta=math.inf), ARGUMENT), (dict(eps=-1.0), ARGUMENT), (dict(eps=math.nan), ARGUMENT)]
+
+
+@pytest.mark.parametrize("change,code", QK_REFUSED, ids=str)
+def test_qk_norm_rope_refuses(change, code):
+    L, s = _lib.lib(), qk(**change)
+    assert L.pk_qk_norm_rope_fwd(C.byref(s), T4(), T4(), SOME, SOME, SOME, T4(), T4(), None) == code and L.pk_last_error()
+    assert L.pk_qk_norm_rope_bwd(C.byref(s), T4(), T4(), T4(), T4(), SOME, SOME, SOME, T4(), T4(), SOME, SOME, SOME, 1 << 30, None) == code
+    assert L.pk_qk_norm_rope_bwd_workspace_bytes(C.byref(s)) == 0
+
+
+def test_qk_norm_rope_refuses_null_and_small_workspaces():
+    L, s = _lib.lib(), qk()
+    fwd = [C.byref(s), T4(), T4(), SOME, SOME, SOME, T4(), T4(), None]
+    for i in range(8):
+        a = list(fwd)
+        a[i] = T4(0) if i in (1, 2, 6, 7) else None
+        assert L.pk_qk_norm_rope_fwd(*a) == ARGUMENT, i
+    need = L.pk_qk_norm_rope_bwd_workspace_bytes(C.byref(s))
+    bwd = [C.byref(s), T4(), T4(), T4(), T4(), SOME, SOME, SOME, T4(), T4(), SOME, SOME, SOME, need, None]
+    for i in range(12):
+        a = list(bwd)
+        a[i] = T4(0) if i in (1, 2, 3, 4, 8, 9) else None
+        assert L.pk_qk_norm_rope_bwd(*a) == ARGUMENT, i
+    for ws, size in ((None, need), (SOME, need - 1), (C.c_void_p((1 << 20) + 2), need)):
+        a = list(bwd)
+        a[12], a[13] = ws, size
+        assert L.pk_qk_norm_rope_bwd(*a) == WORKSPACE
+    assert L.pk_qk_norm_rope_fwd(C.byref(qk(T=0)), T4(0), T4(0), None, None, None, T4(0), T4(0), None) == 0   # nothing to do
+
+
+# what is the same for the three entries that read logits and write their gradient
+LOGITS_REFUSED = [(dict(rows=-1), SHAPE), (dict(rows=1 << 31), SHAPE), (dict(vocab=0), SHAPE), (dict(vocab=(1 << 30) + 1), SHAPE), (dict(ld=-1), SHAPE),
+                  (dict(dld=99), SHAPE), (dict(dtype=7), ARGUMENT), (dict(scale=0.0), ARGUMENT), (dict(scale=-1.0), ARGUMENT), (dict(scale=math.inf), ARGUMENT),
+                  (dict(scale=math.nan), ARGUMENT), (dict(logits=None), ARGUMENT), (dict(targets=None), ARGUMENT), (dict(dlogits=None), ARGUMENT),
+                  (dict(dlogits=CLOSE), ARGUMENT), (dict(dlogits=SOME, dld=200), ARGUMENT)]
+
+
+def call(entry, **kw):
+    d = dict(logits=SOME, ld=100, targets=SOME, rows=4, vocab=100, scale=1.0, dlogits=FAR, dld=100, dtype=_lib.PK_F32, v=SOME, ref=SOME, loss=SOME, low=0.2, high=0.2, kl=0.1,
+             upstream=1.0, beta=0.1, smoothing=0.0, pairs=1, starts=SOME, ws=SOME, ws_bytes=1 << 20)
+    d.update(kw)
+    L = _lib.lib()
+    x = d["logits"], d["ld"], d["targets"]
+    if entry == "bwd":
+        return L.pk_token_logprobs_bwd(*x, d["v"], d["v"], d["rows"], d["vocab"], d["scale"], d["dlogits"], d["dld"], d["dtype"], None)
+    if entry == "policy":
+        c = _lib.PolicyConfig(d["low"], d["high"], d["kl"], d["scale"], d["upstream"])
+        return L.pk_policy_loss(C.byref(c), *x, d["v"], d["ref"], d["v"], d["v"], d["rows"], d["vocab"], d["dlogits"], d["dld"], d["v"], d["v"], d["loss"], d["dtype"], None)
+    c = _lib.PreferenceConfig(d["beta"], d["smoothing"], d["scale"], d["upstream"])
+    return L.pk_preference_loss(C.byref(c), *x, d["starts"], d["pairs"], d["ref"], d["rows"], d["vocab"], d["dlogits"], d["dld"], d["v"], d["v"], d["loss"], d["ws"],
+                                d["ws_bytes"], d["dtype"], None)
+
+
+@pytest.mark.parametrize("entry", ["bwd", "policy", "preference"])
+@pytest.mark.parametrize("change,code", LOGITS_REFUSED, ids=str)
+def test_losses_refuse_logits(entry, change, code):
+    assert call(entry, **change) == code and _lib.lib().pk_last_error()
+
+
+@pytest.mark.parametrize("entry,change,code", [
+    ("bwd", dict(v=None), ARGUMENT), ("policy", dict(v=None), ARGUMENT), ("policy", dict(ref=None), ARGUMENT), ("policy", dict(loss=None), ARGUMENT),
+    ("policy", dict(low=-0.1), ARGUMENT), ("policy", dict(high=math.nan), ARGUMENT), ("policy", dict(kl=math.inf), ARGUMENT), ("policy", dict(upstream=math.nan), ARGUMENT),
+    ("preference", dict(v=None), ARGUMENT), ("preference", dict(ref=None), ARGUMENT), ("preference", dict(starts=None), ARGUMENT), ("preference", dict(loss=None), ARGUMENT),
+    ("preference", dict(pairs=0), SHAPE), ("preference", dict(pairs=-3), SHAPE), ("preference", dict(beta=math.inf), ARGUMENT), ("preference", dict(smoothing=1.5), ARGUMENT),
+    ("preference", dict(smoothing=math.nan), ARGUMENT), ("preference", dict(ws=None), WORKSPACE), ("preference", dict(ws_bytes=100), WORKSPACE)], ids=str)
+def test_losses_refuse(entry, change, code):
+    assert call(entry, **change) == code and _lib.lib().pk_last_error()
+
+
+def test_token_logprobs_refuses():
+    L = _lib.lib()
+    for change, code in (((None, 100, SOME, 4, 100, 1.0, SOME), ARGUMENT), ((SOME, 100, None, 4, 100, 1.0, SOME), ARGUMENT), ((SOME, 100, SOME, 4, 100, 1.0, None), ARGUMENT),
+                         ((SOME, 100, SOME, 4, 0, 1.0, SOME), SHAPE), ((SOME, 100, SOME, 4, 100, math.nan, SOME), ARGUMENT)):
+        assert L.pk_token_logprobs_fwd(*change, None, _lib.PK_F32, None) == code
+    assert L.pk_token_logprobs_fwd(None, 100, None, 0, 100, 1.0, None, None, _lib.PK_F32, None) == 0   # nothing to do
+    assert L.pk_preference_loss_workspace_bytes(100, 3) == 512 + 512 + 1024 + 256
+
+
+def adamw(tensors, ws=SOME, ws_bytes=1 << 20, norm=SOME, **kw):
+    d = dict(lr=1e-3, b1=0.9, b2=0.99, eps=1e-8, wd=0.0, max_norm=0.0, t=1, state_bits=32, grad_dtype=_lib.PK_F32, seed=0)
+    d.update(kw)
+    table = (_lib.AdamWTensor * max(1, len(tensors)))(*tensors)
+    cfg = _lib.AdamWConfig(*[d[n] for n, _ in _lib.AdamWConfig._fields_])
+    return _lib.lib().pk_adamw_many(table, len(tensors), C.byref(cfg), ws, ws_bytes, norm, None)
+
+
+def tensor(at, n=100, g=1 << 30, scales=1 << 31, copy=None, m=None, v=None):
+    return _lib.AdamWTensor(at, g, m if m is not None else at + 4 * n, v if v is not None else at + 8 * n, scales, scales, copy, n)
+
+
+@pytest.mark.parametrize("change,code", [(dict(t=0), ARGUMENT), (dict(state_bits=16), ARGUMENT), (dict(grad_dtype=2), ARGUMENT), (dict(b1=1.0), ARGUMENT), (dict(b2=-0.1), ARGUMENT),
+                                         (dict(b2=math.nan), ARGUMENT), (dict(max_norm=1.0, norm=None), ARGUMENT), (dict(max_norm=1.0, ws=None), WORKSPACE),
+                                         (dict(max_norm=1.0, ws_bytes=263), WORKSPACE)], ids=str)
+def test_adamw_many_refuses(change, code):
+    assert adamw([tensor(1 << 20)], **change) == code and _lib.lib().pk_last_error()
+
+
+def test_adamw_many_refuses_tables():
+    one = tensor(1 << 20)
+    for bad in (tensor(0, m=1, v=1), tensor(1 << 20, g=0), tensor(1 << 20, m=0), tensor(1 << 20, v=0)):
+        assert adamw([bad]) == ARGUMENT
+    assert adamw([tensor(1 << 20, scales=0)], state_bits=8) == ARGUMENT
+    assert adamw([tensor(1 << 20, n=-1)]) == SHAPE and adamw([tensor(1 << 20, n=(1 << 40) + 1)]) == SHAPE
+    for twice in (one, tensor((1 << 20) + 4 * 99), tensor(1 << 24, m=(1 << 20) + 4 * 150), tensor(1 << 24, v=1 << 20)):
+        assert adamw([one, twice]) == ARGUMENT and b"twice" in _lib.lib().pk_last_error()
+    assert adamw([]) == 0 and adamw([_lib.AdamWTensor(0, 0, 0, 0, 0, 0, 0, 0)]) == 0   # nothing to do
+    assert _lib.lib().pk_adamw_many(None, 2, None, None, 0, None, None) == ARGUMENT
+
+
+def test_torch_front_end_refuses_tensors_of_the_cpu():
+    """Types, shapes and places are checked before any pointer is handed on."""
+    import torch
+
+    from paperkiln_amd import blockops, ops
+    z = torch.zeros
+    i32 = lambda *s: z(*s, dtype=torch.int32)  # noqa: E731
+    for fn in (lambda: ops.qk_norm_rope_fwd(z(1, 2, 2, 4), z(1, 2, 2, 4), z(4), z(4), i32(2), 1e4), lambda: ops.token_logprobs(z(3, 5), i32(3)),
+               lambda: blockops.policy_loss(z(3, 5), i32(3), z(3), z(3), z(3)), lambda: blockops.preference_loss(z(3, 5), i32(3), i32(3), z(3)),
+               lambda: blockops.adamw_many_([z(3)], [z(3)], blockops.adamw_state([z(3)], 8), 1e-3)):
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            fn()
+    with pytest.raises(RuntimeError, match="8 or in 32"):
+        blockops.adamw_state([z(3)], 16)
+    with pytest.raises(TypeError):
+        ops.token_logprobs([1.0], i32(1))
