@@ -14,6 +14,7 @@
 namespace pk {
 namespace {
 
+constexpr int FWD_MOST = 4096, BWD_MOST = 1024;  // workgroups of a launch; each of the backward's leaves sums of dw
 constexpr int MAX_DK = 256, MAX_PAIRS = MAX_DK / 2, NT = 256, WAVES = NT / 64;
 
 struct Rows {  // one [B, T, H, dk] tensor
@@ -236,7 +237,7 @@ struct Cols<uint16_t, HALVES> {
             *reinterpret_cast<u32x2*>(row + c1) = u32x2{pack_bf16(e.b[0], e.b[1]), pack_bf16(e.b[2], e.b[3])};
         } else {
             const uint32_t v0 = pack_bf16(e.a[0], e.b[0]), v1 = pack_bf16(e.a[1], e.b[1]), v2 = pack_bf16(e.a[2], e.b[2]), v3 = pack_bf16(e.a[3], e.b[3]);
-            *reinterpret_cast<u32x4*>(row + c0) = u32x4{v0, v1, v2, v3};
+            store_through(reinterpret_cast<u32x4*>(row + c0), u32x4{v0, v1, v2, v3});  // whole lines: rows of 64 columns and more
         }
     }
 };
@@ -400,7 +401,7 @@ template <typename T, int G, bool HALVES>
 __global__ __launch_bounds__(NT) void qk_bwd_rows(Qk a, int per) {
     using L = List<T, G, HALVES>;
     __shared__ float2 strips[WAVES][4 * G];
-    __shared__ float sh[WAVES][2 * 8 * G];
+    __shared__ __align__(16) float sh[WAVES * L::ROWS * 2 * 8 * G];  // 16 KB
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), stride = static_cast<int>(gridDim.x) * WAVES;
     const L list(a);
     const Eight wq = weights_of(a.w[0], list.c0, list.c1, HALVES), wk = weights_of(a.w[1], list.c0, list.c1, HALVES);
@@ -447,45 +448,56 @@ __global__ __launch_bounds__(NT) void qk_bwd_rows(Qk a, int per) {
             list.store(a.y, now, yq, yk, dx);
         }
     }
-    // the wavefront's groups, then its neighbours
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        for (int o = G; o < 64; o *= 2) {
-            dwq.a[i] += __shfl_xor(dwq.a[i], o), dwq.b[i] += __shfl_xor(dwq.b[i], o);
-            dwk.a[i] += __shfl_xor(dwk.a[i], o), dwk.b[i] += __shfl_xor(dwk.b[i], o);
-        }
-        if (list.g == 0 && list.mine) {
-            const int ca = HALVES ? list.c0 + i : i < 2 ? list.c0 + 2 * i : list.c1 + 2 * i - 4, cb = HALVES ? list.c1 + i : ca + 1;
-            sh[wave][ca] = dwq.a[i], sh[wave][cb] = dwq.b[i];
-            sh[wave][a.dk + ca] = dwk.a[i], sh[wave][a.dk + cb] = dwk.b[i];
-        }
+    // the sums of all groups of all wavefronts, columns in their order, then added up column by column
+    constexpr int PITCH = 2 * 8 * G;
+    float* const own = sh + (wave * L::ROWS + list.g) * PITCH;
+    if (list.mine) {
+        auto lay = [&](float* to, const Eight& d) {
+            *reinterpret_cast<f32x4*>(to + list.c0) = HALVES ? d.a : f32x4{d.a[0], d.b[0], d.a[1], d.b[1]};
+            *reinterpret_cast<f32x4*>(to + list.c1) = HALVES ? d.b : f32x4{d.a[2], d.b[2], d.a[3], d.b[3]};
+        };
+        lay(own, dwq);
+        lay(own + 8 * G, dwk);
     }
     __syncthreads();
     const int64_t group = blockIdx.y * static_cast<int64_t>(gridDim.x) + blockIdx.x;
-    for (int i = threadIdx.x; i < 2 * a.dk; i += NT) {
+    for (int i = threadIdx.x; i < PITCH; i += NT) {
+        const int col = i & (8 * G - 1);
+        if (col >= a.dk) continue;
         float s = 0.0f;
-        for (int w = 0; w < WAVES; ++w) s += sh[w][i];
-        a.part[group * (2 * a.dk) + i] = s;
+#pragma unroll
+        for (int k = 0; k < WAVES * L::ROWS; ++k) s += sh[k * PITCH + i];
+        a.part[group * (2 * a.dk) + (i >= 8 * G ? a.dk : 0) + col] = s;
     }
 }
 
-// The workgroups' sums of dw added up in a fixed order: 16 columns to a workgroup, four to a thread, 64 threads to a column. A thread's loads are on their
-// way together: 1024 sums of 128 columns 2.9 us, 19.7 with 16 threads to a column one load after the other.
-constexpr int SUM_SLICES = 64;
-__global__ __launch_bounds__(4 * SUM_SLICES) void qk_dw_sum(const float* part, int parts, int dk, float* dwq, float* dwk) {
-    __shared__ f32x4 sh[SUM_SLICES][4];
+// The workgroups' sums of dw added up in a fixed order: 16 columns to a workgroup, four to a thread, 256 threads to a column, whose loads are all on their way
+// together.
+constexpr int SUM_NT = 1024;
+__global__ __launch_bounds__(SUM_NT) void qk_dw_sum(const float* part, int parts, int dk, float* dwq, float* dwk) {
+    __shared__ f32x4 sh[SUM_NT / 64][4];
     const int c = threadIdx.x & 3, slice = threadIdx.x >> 2, col = static_cast<int>(blockIdx.x) * 16 + 4 * c, cols = 2 * dk;  // cols is a multiple of 4
     f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
     if (col < cols) {
-#pragma unroll 8
-        for (int i = slice; i < parts; i += SUM_SLICES) s += *reinterpret_cast<const f32x4*>(part + i * static_cast<int64_t>(cols) + col);
+        f32x4 v[BWD_MOST / (SUM_NT / 4)];
+#pragma unroll
+        for (int k = 0; k < BWD_MOST / (SUM_NT / 4); ++k) {
+            const int i = slice + k * (SUM_NT / 4);
+            v[k] = i < parts ? *reinterpret_cast<const f32x4*>(part + i * static_cast<int64_t>(cols) + col) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+#pragma unroll
+        for (int k = 0; k < BWD_MOST / (SUM_NT / 4); ++k) s += v[k];
     }
-    sh[slice][c] = s;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        for (int o = 4; o < 64; o *= 2) s[e] += __shfl_xor(s[e], o);
+    if ((threadIdx.x & 63) < 4) sh[threadIdx.x >> 6][c] = s;
     __syncthreads();
     if (threadIdx.x >= 16) return;
     const int at = static_cast<int>(threadIdx.x), to = static_cast<int>(blockIdx.x) * 16 + at;
     float r = 0.0f;
-    for (int i = 0; i < SUM_SLICES; ++i) r += sh[i][at >> 2][at & 3];
+#pragma unroll
+    for (int i = 0; i < SUM_NT / 64; ++i) r += sh[i][at >> 2][at & 3];
     if (to < cols) (to < dk ? dwq[to] : dwk[to - dk]) = r;
 }
 
@@ -505,7 +517,7 @@ bool bad(const pk_tensor4* t) { return !t || !t->ptr; }
 void fill(Qk& a, const pk_qk_shape* s) {
     a.B = s->B, a.T = s->T, a.Hq = s->Hq, a.Hkv = s->Hkv, a.dk = s->dk, a.rotary = s->rotary ? s->rotary : s->dk, a.halves = s->halves != 0;
     a.eps = s->eps, a.per_dk = 1.0f / static_cast<float>(s->dk), a.pos_sb = s->pos_stride_b, a.part = nullptr;
-    for (int i = 0; i < MAX_PAIRS / 8; ++i) a.coarse[i] = std::pow(s->theta, -16.0 * i / a.rotary);
+    for (int i = 0; i < MAX_PAIRS / 8; ++i) a.coarse[i] = i == 0 ? 1.0 : 16 * i < a.rotary ? std::pow(s->theta, -16.0 * i / a.rotary) : 0.0;
     for (int i = 0; i < 8; ++i) a.fine[i] = std::pow(s->theta, -2.0 * i / a.rotary) / 6.283185307179586476925;
 }
 Rows rows_of(const pk_tensor4* t) { return Rows{t->ptr, t->stride_b, t->stride_t, t->stride_h}; }
@@ -554,7 +566,6 @@ Plan plan_of(const pk_qk_shape* s, int most) {
     p.groups = static_cast<int>(groups < cap ? groups : cap);
     return p;
 }
-constexpr int FWD_MOST = 1024, BWD_MOST = 1024;  // workgroups of a launch; each of the backward's leaves sums of dw
 
 template <typename T, bool HALVES>
 void launch_rows(const Qk& a, const Plan& p, bool backward, hipStream_t st) {
@@ -653,7 +664,7 @@ int pk_qk_norm_rope_bwd(const pk_qk_shape* s, const pk_tensor4* dyq, const pk_te
                 qk_bwd_any<float><<<dim3(groups), NT, 0, st>>>(a);
             if (int rc = launched()) return rc;
         }
-        qk_dw_sum<<<dim3((2 * s->dk + 15) / 16), 4 * SUM_SLICES, 0, st>>>(a.part, none ? 0 : groups, s->dk, dwq, dwk);
+        qk_dw_sum<<<dim3((2 * s->dk + 15) / 16), SUM_NT, 0, st>>>(a.part, none ? 0 : groups, s->dk, dwq, dwk);
         return launched();
     });
 }
