@@ -51,7 +51,7 @@ __device__ inline void policy_row(const Loss& a, int64_t r, double logp, double&
     }
 }
 
-// Any size, stride and alignment: a workgroup takes a row and reads it element by element, twice where a gradient is written.
+// A gradient that does not lie as its logits do (another row pitch, another offset, modulo 16 bytes): a workgroup takes a row element by element.
 constexpr int ANY_NT = 256;
 template <typename T, Mode MODE>
 __global__ __launch_bounds__(ANY_NT) void rows_any(Loss a) {
@@ -120,6 +120,303 @@ __global__ __launch_bounds__(ANY_NT) void rows_any(Loss a) {
         for (int j = tid; j < V; j += ANY_NT) put(dx, j, j == t ? target_grad : -coef * __builtin_amdgcn_exp2f(fmaf(elem(x, j), s2, -lse2)));
 }
 
+// ---- rows in 16-byte pieces -------------------------------------------------------------------------------------------------
+// A row is taken apart at 16-byte boundaries of its address: whole pieces, and the few elements in front of the first and behind the last one, which go to
+// one thread each. So a row may begin anywhere; what is written has to lie as what is read, modulo 16.
+
+template <typename T>
+struct Piece;
+template <>
+struct Piece<uint16_t> {
+    static constexpr int N = 8;
+    u32x4 v;
+    template <typename F>
+    __device__ void each(F&& f) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f(__uint_as_float(v[i] << 16));
+            f(__uint_as_float(v[i] & 0xFFFF0000u));
+        }
+    }
+    template <typename F>
+    __device__ Piece map(F&& f) const {
+        Piece r;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r.v[i] = pack_bf16(f(2 * i, __uint_as_float(v[i] << 16)), f(2 * i + 1, __uint_as_float(v[i] & 0xFFFF0000u)));
+        return r;
+    }
+    __device__ static Piece nothing() { return Piece{{0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u}}; }
+};
+template <>
+struct Piece<float> {
+    static constexpr int N = 4;
+    u32x4 v;
+    template <typename F>
+    __device__ void each(F&& f) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f(__uint_as_float(v[i]));
+    }
+    template <typename F>
+    __device__ Piece map(F&& f) const {
+        Piece r;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r.v[i] = __float_as_uint(f(i, __uint_as_float(v[i])));
+        return r;
+    }
+    __device__ static Piece nothing() { return Piece{{0xFF800000u, 0xFF800000u, 0xFF800000u, 0xFF800000u}}; }
+};
+template <typename T>
+struct Cut {  // a row's pieces
+    int head, pieces, edges;
+    __device__ Cut(const T* x, int V) {
+        constexpr int N = Piece<T>::N;
+        const int past = static_cast<int>(reinterpret_cast<uintptr_t>(x) / sizeof(T)) & (N - 1);
+        head = min((N - past) & (N - 1), V);
+        pieces = (V - head) / N;
+        edges = V - pieces * N;
+    }
+    __device__ int edge(int i) const { return i < head ? i : i + pieces * Piece<T>::N; }
+};
+
+// log2 of the sum of 2^(s2 x) over a row from what each wavefront has: the largest s2 x that it took its exponentials against and their sum.
+template <int WAVES>
+__device__ inline double lse2_of(const float (&m)[WAVES], const float (&s)[WAVES]) {
+    float top = m[0];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) top = fmaxf(top, m[w]);
+    double sum = 0.0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) sum += s[w] == 0.0f ? 0.0 : static_cast<double>(s[w] * __builtin_amdgcn_exp2f(m[w] - top));  // a wavefront without a word has none to scale
+    return sum == 0.0 ? static_cast<double>(NAN) : top + log2(sum);  // a row without a word has no probabilities
+}
+
+// What a row's gradient is made of once its sum is known.
+struct RowOut {
+    float lse2, coef, target;  // log2 of the sum, the row's coefficient, the target's gradient
+};
+template <Mode MODE>
+__device__ inline RowOut finish(const Loss& a, int64_t r, float xt, float s2, double lse2) {
+    const double logp = (static_cast<double>(xt) * s2 - lse2) * LN2;
+    RowOut o{static_cast<float>(lse2), 0.0f, 0.0f};
+    if (MODE == POLICY) {
+        double loss, slope;
+        policy_row(a, r, logp, loss, slope);
+        const double w = a.weights[r];
+        o.coef = static_cast<float>(w * slope * a.upstream * a.scale);
+        o.target = o.coef * static_cast<float>(-expm1(logp));
+        a.row_loss[r] = w * loss;
+    }
+    a.logp[r] = static_cast<float>(logp);
+    if (a.lse) a.lse[r] = static_cast<float>(lse2 * LN2);
+    if (MODE == LOGP && a.fine) a.fine[r] = logp;
+    return o;
+}
+// A row that does not count: not read, its results zeros.
+template <Mode MODE>
+__device__ inline void no_row(const Loss& a, int64_t r) {
+    a.logp[r] = 0.0f;
+    if (a.lse) a.lse[r] = 0.0f;
+    if (MODE == POLICY) a.row_loss[r] = 0.0;
+}
+template <typename T, int NT>
+__device__ inline void zero_row(T* dx, const Cut<T>& cut, int tid) {
+    for (int p = tid; p < cut.pieces; p += NT) *reinterpret_cast<u32x4*>(dx + cut.head + p * Piece<T>::N) = u32x4{0, 0, 0, 0};
+    if (tid < cut.edges) put(dx, cut.edge(tid), 0.0f);
+}
+// The gradient of a piece whose first word is j0.
+template <typename T>
+__device__ inline Piece<T> gradient(const Piece<T>& x, int j0, int t, float s2, const RowOut& o) {
+    Piece<T> g = x.map([&](int, float v) { return -o.coef * __builtin_amdgcn_exp2f(fmaf(v, s2, -o.lse2)); });
+    if (static_cast<unsigned>(t - j0) < static_cast<unsigned>(Piece<T>::N))
+        g = x.map([&](int i, float v) { return j0 + i == t ? o.target : -o.coef * __builtin_amdgcn_exp2f(fmaf(v, s2, -o.lse2)); });
+    return g;
+}
+
+// Between two walks over a row the pieces stay as they are: the compiler would keep every element of the first walk in a register of its own.
+template <typename T, int PER>
+__device__ inline void keep_packed(Piece<T> (&held)[PER]) {
+    if constexpr (Piece<T>::N == 8) {
+#pragma unroll
+        for (int k = 0; k < PER; ++k) asm volatile("" : "+v"(held[k].v));
+    }
+}
+
+// ROW_NT threads hold a row, PER pieces each, so that the logits are read once. One exchange through LDS joins the wavefronts; the first one works out the
+// row's scalars in 64 bits and hands them round.
+template <typename T, Mode MODE, int ROW_NT, int PER>
+__global__ __launch_bounds__(ROW_NT) void rows_held(Loss a) {
+    constexpr int WAVES = ROW_NT / 64, N = Piece<T>::N;
+    __shared__ float sh_m[WAVES], sh_s[WAVES];
+    __shared__ RowOut sh_o;
+    const int64_t r = blockIdx.x;
+    const int tid = threadIdx.x, V = a.vocab, t = a.targets[r];
+    const T* x = static_cast<const T*>(a.logits) + r * a.ld;
+    T* dx = MODE == LOGP ? nullptr : static_cast<T*>(a.dlogits) + r * a.dld;
+    const Cut<T> cut(x, V);
+    if (MODE == LOGP && a.clear && tid == 0) a.clear[r] = 0.0f;
+    if (t < 0 || (MODE == POLICY && a.weights[r] == 0.0f)) {
+        if (tid == 0) no_row<MODE>(a, r);
+        if (MODE != LOGP) zero_row<T, ROW_NT>(dx, cut, tid);
+        return;
+    }
+    const float s2 = a.scale * LOG2E;
+    Piece<T> held[PER];
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const int p = tid + k * ROW_NT;
+        held[k] = p < cut.pieces ? *reinterpret_cast<const Piece<T>*>(x + cut.head + p * N) : Piece<T>::nothing();
+    }
+    const float edge = tid < cut.edges ? elem(x, cut.edge(tid)) : -INFINITY;
+    const float xt = t < V ? elem(x, t) : NAN;  // read before the row is written over; a token that is no word has no probability
+    float m = edge;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) held[k].each([&](float v) { m = fmaxf(m, v); });
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    const float m2 = m == -INFINITY ? 0.0f : m * s2;
+    float s = __builtin_amdgcn_exp2f(fmaf(edge, s2, -m2));
+    keep_packed(held);
+#pragma unroll
+    for (int k = 0; k < PER; ++k) held[k].each([&](float v) { s += __builtin_amdgcn_exp2f(fmaf(v, s2, -m2)); });
+    s = group_sum<64>(s);
+    RowOut o;
+    if constexpr (WAVES == 1) {
+        const float ms[1] = {m2}, ss[1] = {s};
+        if (MODE == LOGP && tid != 0) return;
+        o = finish<MODE>(a, r, xt, s2, lse2_of<1>(ms, ss));
+    } else {
+        if ((tid & 63) == 0) sh_m[tid >> 6] = s == 0.0f ? -INFINITY : m2, sh_s[tid >> 6] = s;
+        __syncthreads();
+        if (tid < 64) {
+            o = finish<MODE>(a, r, xt, s2, lse2_of<WAVES>(sh_m, sh_s));
+            if (tid == 0) sh_o = o;
+        }
+        if constexpr (MODE == LOGP) return;
+        __syncthreads();
+        o = sh_o;
+    }
+    if constexpr (MODE != LOGP) {
+        if (o.coef == 0.0f) return zero_row<T, ROW_NT>(dx, cut, tid);  // clipped
+        keep_packed(held);
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            const int p = tid + k * ROW_NT, j0 = cut.head + p * N;
+            if (p < cut.pieces) *reinterpret_cast<Piece<T>*>(dx + j0) = gradient(held[k], j0, t, s2, o);
+        }
+        if (tid < cut.edges) {
+            const int j = cut.edge(tid);
+            put(dx, j, j == t ? o.target : -o.coef * __builtin_amdgcn_exp2f(fmaf(edge, s2, -o.lse2)));
+        }
+    }
+}
+
+// Rows that no workgroup holds: read in strides with a running maximum and sum, and again for the gradient.
+constexpr int LONG_NT = 1024, LONG_U = 4;
+template <typename T, Mode MODE>
+__global__ __launch_bounds__(LONG_NT) void rows_long(Loss a) {
+    constexpr int WAVES = LONG_NT / 64, N = Piece<T>::N;
+    __shared__ float sh_m[WAVES], sh_s[WAVES];
+    __shared__ RowOut sh_o;
+    const int64_t r = blockIdx.x;
+    const int tid = threadIdx.x, V = a.vocab, t = a.targets[r];
+    const T* x = static_cast<const T*>(a.logits) + r * a.ld;
+    T* dx = MODE == LOGP ? nullptr : static_cast<T*>(a.dlogits) + r * a.dld;
+    const Cut<T> cut(x, V);
+    if (MODE == LOGP && a.clear && tid == 0) a.clear[r] = 0.0f;
+    if (t < 0 || (MODE == POLICY && a.weights[r] == 0.0f)) {
+        if (tid == 0) no_row<MODE>(a, r);
+        if (MODE != LOGP) zero_row<T, LONG_NT>(dx, cut, tid);
+        return;
+    }
+    const float s2 = a.scale * LOG2E;
+    const float edge = tid < cut.edges ? elem(x, cut.edge(tid)) : -INFINITY, xt = t < V ? elem(x, t) : NAN;
+    float m2 = edge == -INFINITY ? -INFINITY : edge * s2, s = edge == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(fmaf(edge, s2, -m2));
+    for (int p0 = tid; p0 < cut.pieces; p0 += LONG_U * LONG_NT) {
+        Piece<T> v[LONG_U];
+#pragma unroll
+        for (int u = 0; u < LONG_U; ++u) {
+            const int p = p0 + u * LONG_NT;
+            v[u] = p < cut.pieces ? *reinterpret_cast<const Piece<T>*>(x + cut.head + p * N) : Piece<T>::nothing();
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < LONG_U; ++u) v[u].each([&](float y) { top = fmaxf(top, y); });
+        const float new2 = fmaxf(m2, top * s2), ref = new2 == -INFINITY ? 0.0f : new2;
+        s = s == 0.0f ? 0.0f : s * __builtin_amdgcn_exp2f(m2 - ref);
+#pragma unroll
+        for (int u = 0; u < LONG_U; ++u) v[u].each([&](float y) { s += __builtin_amdgcn_exp2f(fmaf(y, s2, -ref)); });
+        m2 = new2;
+    }
+    // lanes, then wavefronts
+    float top = m2;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    s = group_sum<64>(s == 0.0f ? 0.0f : s * __builtin_amdgcn_exp2f(m2 - top));
+    if ((tid & 63) == 0) sh_m[tid >> 6] = s == 0.0f ? -INFINITY : top, sh_s[tid >> 6] = s;
+    __syncthreads();
+    RowOut o;
+    if (tid < 64) {
+        o = finish<MODE>(a, r, xt, s2, lse2_of<WAVES>(sh_m, sh_s));
+        if (tid == 0) sh_o = o;
+    }
+    if constexpr (MODE != LOGP) {
+        __syncthreads();
+        o = sh_o;
+        if (o.coef == 0.0f) return zero_row<T, LONG_NT>(dx, cut, tid);
+        for (int p = tid; p < cut.pieces; p += LONG_NT) {
+            const int j0 = cut.head + p * N;
+            *reinterpret_cast<Piece<T>*>(dx + j0) = gradient(*reinterpret_cast<const Piece<T>*>(x + j0), j0, t, s2, o);
+        }
+        if (tid < cut.edges) {
+            const int j = cut.edge(tid);
+            put(dx, j, j == t ? o.target : -o.coef * __builtin_amdgcn_exp2f(fmaf(edge, s2, -o.lse2)));
+        }
+    }
+}
+
+// The gradient of rows whose sums are known: every element by itself.
+constexpr int GRAD_NT = 256, GRAD_U = 4;
+template <typename T>
+__global__ __launch_bounds__(GRAD_NT) void rows_grad(Loss a) {
+    constexpr int N = Piece<T>::N;
+    const int64_t r = a.backwards ? a.rows - 1 - blockIdx.x : blockIdx.x;
+    const int tid = threadIdx.x, V = a.vocab, t = a.targets[r];
+    const T* x = static_cast<const T*>(a.logits) + r * a.ld;
+    T* dx = static_cast<T*>(a.dlogits) + r * a.dld;
+    const Cut<T> cut(x, V);
+    RowOut o;
+    o.coef = a.coef[r] * a.scale;
+    if (t < 0 || o.coef == 0.0f) return zero_row<T, GRAD_NT>(dx, cut, tid);
+    const float s2 = a.scale * LOG2E, xt = t < V ? elem(x, t) : NAN;
+    const double lse2 = a.lse_in[r] / LN2;
+    o.lse2 = static_cast<float>(lse2);
+    o.target = o.coef * -expm1f(static_cast<float>((static_cast<double>(xt) * s2 - lse2) * LN2));
+    if (t >= V) o.coef = NAN;
+    if (cut.edges) {  // the target may be among them, or read by another thread: all of it before anything is written
+        const float edge = tid < cut.edges ? elem(x, cut.edge(tid)) : 0.0f;
+        __syncthreads();
+        if (tid < cut.edges) {
+            const int j = cut.edge(tid);
+            put(dx, j, j == t ? o.target : -o.coef * __builtin_amdgcn_exp2f(fmaf(edge, s2, -o.lse2)));
+        }
+    } else {
+        __syncthreads();  // xt is read by all before its piece is written over
+    }
+    for (int p0 = tid; p0 < cut.pieces; p0 += GRAD_U * GRAD_NT) {
+        Piece<T> v[GRAD_U];
+#pragma unroll
+        for (int u = 0; u < GRAD_U; ++u) {
+            const int p = p0 + u * GRAD_NT;
+            if (p < cut.pieces) v[u] = *reinterpret_cast<const Piece<T>*>(x + cut.head + p * N);
+        }
+#pragma unroll
+        for (int u = 0; u < GRAD_U; ++u) {
+            const int p = p0 + u * GRAD_NT, j0 = cut.head + p * N;
+            if (p < cut.pieces) *reinterpret_cast<Piece<T>*>(dx + j0) = gradient(v[u], j0, t, s2, o);
+        }
+    }
+}
+
 // n values added up in 64 bits in a fixed order, times a factor.
 __global__ __launch_bounds__(1024) void loss_sum(const double* x, int64_t n, double factor, float* out) {
     __shared__ double sh[16];
@@ -180,14 +477,41 @@ __global__ __launch_bounds__(PAIR_NT) void pair_loss(Pairs a) {
         for (int64_t r = begin[k] + tid; r < end[k]; r += PAIR_NT) a.coef[r] = k ? -slope : slope;
 }
 
+// Whether what is written lies as what is read, modulo a piece, in every row.
+bool same_cut(const Loss& a, int64_t es) {
+    return (reinterpret_cast<uintptr_t>(a.logits) - reinterpret_cast<uintptr_t>(a.dlogits)) % 16 == 0 && (a.ld - a.dld) * es % 16 == 0;
+}
+template <typename T, Mode MODE>
+void launch_held(const Loss& a, hipStream_t st) {
+    const dim3 grid(static_cast<unsigned>(a.rows));
+    const int pieces = a.vocab / Piece<T>::N;
+    if (pieces <= 64) return rows_held<T, MODE, 64, 1><<<grid, 64, 0, st>>>(a);
+    if (pieces <= 128) return rows_held<T, MODE, 64, 2><<<grid, 64, 0, st>>>(a);
+    if (pieces <= 256) return rows_held<T, MODE, 64, 4><<<grid, 64, 0, st>>>(a);
+    if (pieces <= 512) return rows_held<T, MODE, 256, 2><<<grid, 256, 0, st>>>(a);
+    if (pieces <= 1024) return rows_held<T, MODE, 256, 4><<<grid, 256, 0, st>>>(a);
+    if (pieces <= 2048) return rows_held<T, MODE, 256, 8><<<grid, 256, 0, st>>>(a);
+    if (pieces <= 4096) return rows_held<T, MODE, 512, 8><<<grid, 512, 0, st>>>(a);
+    if (pieces <= 8192) return rows_held<T, MODE, 1024, 8><<<grid, 1024, 0, st>>>(a);
+    if (pieces <= 16384) return rows_held<T, MODE, 1024, 16><<<grid, 1024, 0, st>>>(a);
+    rows_long<T, MODE><<<grid, LONG_NT, 0, st>>>(a);
+}
+template <typename T, Mode MODE>
+void launch_typed(const Loss& a, hipStream_t st) {
+    if constexpr (MODE != LOGP)
+        if (!same_cut(a, sizeof(T))) return rows_any<T, MODE><<<dim3(static_cast<unsigned>(a.rows)), ANY_NT, 0, st>>>(a);
+    if constexpr (MODE == GRAD)
+        rows_grad<T><<<dim3(static_cast<unsigned>(a.rows)), GRAD_NT, 0, st>>>(a);
+    else
+        launch_held<T, MODE>(a, st);
+}
 template <Mode MODE>
 int launch_rows(const Loss& a, int dtype, hipStream_t st) {
     if (a.rows == 0) return PK_OK;
-    const dim3 grid(static_cast<unsigned>(a.rows));
     if (dtype == PK_BF16)
-        rows_any<uint16_t, MODE><<<grid, ANY_NT, 0, st>>>(a);
+        launch_typed<uint16_t, MODE>(a, st);
     else
-        rows_any<float, MODE><<<grid, ANY_NT, 0, st>>>(a);
+        launch_typed<float, MODE>(a, st);
     return launched();
 }
 
