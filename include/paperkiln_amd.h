@@ -358,7 +358,8 @@ int pk_preference_loss(const pk_preference_config* c, const void* logits, int64_
  * as ops::clip_grad_norm does (src/ops.cpp:1046-1064), on the way: they are not written. norm (device, fp32)
  * receives the global norm before the clip; it may be NULL without one.
  * state_bits 32: m and v are fp32 [n]. 8: m is e4m3 (finite, no infinities) and v e5m2, one byte an element, each times
- * the power of two of its block of 256 elements: m_scale, v_scale fp32 [ceil(n / 256)]. Zeroed memory is a fresh state
+ * the power of two (as the device's powf and torch.ldexp form it) of its block of 256 elements: m_scale, v_scale fp32
+ * [ceil(n / 256)]. Zeroed memory is a fresh state
  * in either. Values between two of the format's are rounded up or down at random with the value itself as the mean,
  * drawn from (seed, the tensor's place in the list, the element's place in the tensor): give another seed each step. A v
  * that is not zero does not become zero. A block in which a value is not finite becomes NaN.

@@ -2,8 +2,9 @@
 //
 //   g' = g min(1, max_norm / |g|)    m' = b1 m + (1 - b1) g'    v' = b2 v + (1 - b2) g'^2    p -= lr ((m' / c1) / (sqrt(v' / c2) + eps) + wd p)
 //
-// In 8 bits m is e4m3 and v e5m2 with a power of two for every 256 elements of a tensor, the largest that keeps the block's largest value inside the
-// format: scaling then rounds nothing. v' moves by a thousandth of itself in a step, far less than the 1/8 between neighbours of its format, so
+// In 8 bits m is e4m3 and v e5m2 with a power of two for every 256 elements of a tensor, the smallest that keeps the block's largest value inside the
+// format. The powers are the device's powf(2, e), which torch.ldexp is on this GPU too (one step of 32 bits under 2^e for about a sixth of the exponents): a state
+// that a program packs or unpacks with torch's operations has the bits that it has here. v' moves by a thousandth of itself in a step, far less than the 1/8 between neighbours of its format, so
 // rounding to the nearest would leave it where it is for ever; both moments are rounded up with the probability that the bits dropped stand for,
 // from a hash of the seed, the tensor's place in the list and the element's place in it. The same call gives the same bits. A v that is not zero
 // does not become zero: m / sqrt(v) would have no bound. A block that holds a value which is not finite becomes NaN as a whole.
@@ -23,8 +24,8 @@ namespace pk {
 namespace {
 
 constexpr int BLOCK = 256, NT = 256, WAVES = NT / 64;  // elements that share a scale; a wavefront takes a block
-constexpr int MAX_TENSORS = 48;                         // of one launch: the table travels in the kernel's arguments (4 KB at most)
 constexpr int BLOCKS_PER_WG = 16;
+constexpr int MAX_TENSORS = 58;  // of one launch: the table travels in the kernel's arguments (4 KB at most)
 
 struct One {
     float* p;
@@ -35,15 +36,16 @@ struct One {
     int64_t n;
 };
 struct Table {
-    int first[MAX_TENSORS + 1];  // a tensor's first workgroup
-    uint32_t key[MAX_TENSORS];
     One t[MAX_TENSORS];
+    int first[MAX_TENSORS];  // a tensor's first workgroup
+    int count, place;        // tensors, the first one's place in the caller's list
+    uint32_t seed;
 };
-static_assert(sizeof(Table) + 128 <= 4096, "kernel arguments");
 struct Step {
-    float lr, b1, b2, rest1, rest2, eps, wd, c1, c2;
-    const float* factor;  // what the gradients are multiplied by, or null
+    float lr, b1, b2, rest1, rest2, eps, wd, per_c1, per_c2;  // 1 / c1, 1 / c2
+    const float* factor;                                       // what the gradients are multiplied by, or null
 };
+static_assert(sizeof(Table) + sizeof(Step) <= 4096, "kernel arguments");
 
 // The low 32 bits scrambled: two multiplications by the fractions of the square roots of 3 and 2, shifts between them.
 __host__ __device__ inline uint32_t mix(uint32_t x) {
@@ -73,7 +75,16 @@ __device__ inline int scale_power(uint32_t largest) {
     const int e = static_cast<int>(largest >> 23) - 127 + ((largest & 0x7FFFFFu) > 0x600000u ? 1 : 0);
     return max(e - TOP, -126);
 }
-__device__ inline float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
+// powf(2, e) for e in -126 .. 127 at e + 126, formed once by a workgroup: a call a block and wavefront would cost more than the block's update.
+struct Powers {
+    const float* at;
+    __device__ float operator()(int e) const { return at[e + 126]; }
+};
+__device__ inline Powers powers(float (&table)[NT]) {
+    table[threadIdx.x] = powf(2.0f, static_cast<float>(static_cast<int>(threadIdx.x) - 126));
+    __syncthreads();
+    return Powers{table};
+}
 
 // Into 8 bits: the magnitude moved to where the format's exponent range begins at 32 bits' own, random bits added below the last kept one.
 __device__ inline uint32_t to_e4m3(float y, uint32_t chance) {
@@ -86,16 +97,26 @@ __device__ inline float of_e4m3(uint32_t c) {
 }
 __device__ inline float of_e5m2(uint32_t c) { return c > 0x7Cu ? NAN : c == 0x7Cu ? INFINITY : __uint_as_float(c << 21) * 0x1p112f; }
 
+// sqrt of x >= 0 to a step of 32 bits; small x are scaled into the range of the instruction
+__device__ inline float root(float x) {
+    const bool small = x < 0x1p-100f;
+    const float r = __builtin_amdgcn_sqrtf(small ? x * 0x1p100f : x);
+    return small ? r * 0x1p-50f : r;
+}
+// m' and v' as the formula's own roundings; p's update to a few steps of 32 bits: quotients by the corrections as products, the root and the reciprocal by their
+// instructions (one step each).
 __device__ inline void update(const Step& s, float& p, float g, float& m, float& v) {
     const float a = s.b1 * m, b = s.rest1 * g, c = s.b2 * v, d = s.rest2 * g, e = d * g;
     m = a + b;
     v = c + e;
-    p -= s.lr * ((m / s.c1) / (sqrtf(v / s.c2) + s.eps) + s.wd * p);
+    const float under = root(v * s.per_c2) + s.eps;
+    const float upd = (m * s.per_c1) * __builtin_amdgcn_rcpf(under);
+    p -= s.lr * (upd + s.wd * p);
 }
 
 // A wavefront takes a block of 256 elements, a lane its elements lane, lane + 64, lane + 128 and lane + 192.
 template <typename G, bool EIGHT>
-__device__ inline void block_any(const One& t, const Step& s, uint32_t key, int64_t block, float gs) {
+__device__ inline void block_any(const One& t, const Step& s, uint32_t key, int64_t block, float gs, Powers power_of_two) {
     const int lane = threadIdx.x & 63;
     const int64_t base = block * BLOCK;
     float p[4], m[4], v[4];
@@ -148,7 +169,75 @@ __device__ inline void block_any(const One& t, const Step& s, uint32_t key, int6
     }
 }
 
-// The tensor that a workgroup belongs to: the last one whose first workgroup is not behind it.
+// The same for whole blocks of aligned tensors: a lane takes four neighbours, 16 bytes of 32-bit tensors and four of 8-bit ones.
+__device__ inline f32x4 four(const float* p, int64_t i) { return *reinterpret_cast<const f32x4*>(p + i); }
+__device__ inline f32x4 four(const uint16_t* p, int64_t i) {
+    const u32x2 r = *reinterpret_cast<const u32x2*>(p + i);
+    return f32x4{__uint_as_float(r[0] << 16), __uint_as_float(r[0] & 0xFFFF0000u), __uint_as_float(r[1] << 16), __uint_as_float(r[1] & 0xFFFF0000u)};
+}
+template <typename G, bool EIGHT>
+__device__ inline void block_whole(const One& t, const Step& s, uint32_t key, int64_t block, float gs, Powers power_of_two) {
+    const int lane = threadIdx.x & 63;
+    const int64_t i = block * BLOCK + lane * 4;
+    const f32x4 g = four(static_cast<const G*>(t.g), i);
+    f32x4 p = four(t.p, i), m, v;
+    if constexpr (EIGHT) {
+        const uint32_t mc = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(t.m) + i), vc = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(t.v) + i);
+        const float ms = t.ms[block], vs = t.vs[block];
+        const auto m0 = __builtin_amdgcn_cvt_pk_f32_fp8(mc, false), m1 = __builtin_amdgcn_cvt_pk_f32_fp8(mc, true);
+        const auto v0 = __builtin_amdgcn_cvt_pk_f32_bf8(vc, false), v1 = __builtin_amdgcn_cvt_pk_f32_bf8(vc, true);
+        m = f32x4{m0[0] * ms, m0[1] * ms, m1[0] * ms, m1[1] * ms};
+        v = f32x4{v0[0] * vs, v0[1] * vs, v1[0] * vs, v1[1] * vs};
+    } else {
+        m = four(static_cast<const float*>(t.m), i);
+        v = four(static_cast<const float*>(t.v), i);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        float pk = p[k], mk = m[k], vk = v[k];
+        update(s, pk, g[k] * gs, mk, vk);
+        p[k] = pk, m[k] = mk, v[k] = vk;
+    }
+    *reinterpret_cast<f32x4*>(t.p + i) = p;
+    if (t.copy) *reinterpret_cast<u32x2*>(t.copy + i) = u32x2{pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3])};
+    if constexpr (!EIGHT) {
+        *reinterpret_cast<f32x4*>(static_cast<float*>(t.m) + i) = m;
+        *reinterpret_cast<f32x4*>(static_cast<float*>(t.v) + i) = v;
+    } else {
+        uint32_t mm = 0, vm = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            mm = max(mm, __float_as_uint(m[k]) & 0x7FFFFFFFu);
+            vm = max(vm, __float_as_uint(v[k]) & 0x7FFFFFFFu);
+        }
+        mm = wave_max(mm), vm = wave_max(vm);
+        const bool m_fine = mm < 0x7F800000u, v_fine = vm < 0x7F800000u;
+        const int me = scale_power<8>(mm), ve = scale_power<15>(vm);
+        if (lane == 0) {
+            t.ms[block] = m_fine ? power_of_two(me) : NAN;
+            t.vs[block] = v_fine ? power_of_two(ve) : NAN;
+        }
+        const float mi = power_of_two(-me), vi = power_of_two(-ve);
+        uint32_t mc = 0, vc = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const uint32_t h = mix((static_cast<uint32_t>(i) + k) ^ key);
+            mc |= to_e4m3(m[k] * mi, h & 0xFFFFu) << (8 * k);
+            vc |= max(to_e5m2(v[k] * vi, h >> 16), v[k] > 0.0f ? 1u : 0u) << (8 * k);
+        }
+        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(t.m) + i) = m_fine ? mc : 0x7F7F7F7Fu;
+        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(t.v) + i) = v_fine ? vc : 0x7F7F7F7Fu;
+    }
+}
+template <typename G, bool EIGHT>
+__device__ inline bool aligned_for_whole(const One& t) {
+    const auto at = [](const void* p) { return reinterpret_cast<uintptr_t>(p); };
+    const uintptr_t sixteen = at(t.p) | (sizeof(G) == 4 ? at(t.g) : 0) | (EIGHT ? 0 : at(t.m) | at(t.v));
+    const uintptr_t eight = (sizeof(G) == 2 ? at(t.g) : 0) | at(t.copy), quad = EIGHT ? at(t.m) | at(t.v) : 0;
+    return (sixteen & 15) == 0 && (eight & 7) == 0 && (quad & 3) == 0;
+}
+
+// The tensor that a workgroup belongs to: the last one whose first workgroup is not behind it (one without elements has no workgroup of its own).
 __device__ inline int tensor_of(const int* first, int count, int group) {
     int lo = 0, hi = count - 1;
     while (lo < hi) {
@@ -160,34 +249,71 @@ __device__ inline int tensor_of(const int* first, int count, int group) {
     }
     return lo;
 }
+__host__ __device__ inline uint32_t key_of(uint32_t seed, int place) { return mix(seed * 0x9E3779B9u + mix(static_cast<uint32_t>(place) + 0x3C6EF373u)); }
 
 template <typename G, bool EIGHT>
-__global__ __launch_bounds__(NT) void adamw_many_k(Table tab, Step s, int count) {
-    const int group = blockIdx.x, j = tensor_of(tab.first, count, group);
+__global__ __launch_bounds__(NT) void adamw_many_k(Table tab, Step s) {
+    const int group = blockIdx.x, j = tensor_of(tab.first, tab.count, group);
     const One t = tab.t[j];
-    const int64_t blocks = (t.n + BLOCK - 1) / BLOCK, begin = static_cast<int64_t>(group - tab.first[j]) * BLOCKS_PER_WG;
+    const int64_t blocks = (t.n + BLOCK - 1) / BLOCK, whole = aligned_for_whole<G, EIGHT>(t) ? t.n / BLOCK : 0;
+    const int64_t begin = static_cast<int64_t>(group - tab.first[j]) * BLOCKS_PER_WG, end = min(begin + BLOCKS_PER_WG, blocks);
+    const uint32_t key = key_of(tab.seed, tab.place + j);
     const float gs = s.factor ? *s.factor : 1.0f;
-    for (int k = threadIdx.x >> 6; k < BLOCKS_PER_WG && begin + k < blocks; k += WAVES) block_any<G, EIGHT>(t, s, tab.key[j], begin + k, gs);
+    __shared__ float table[EIGHT ? NT : 1];
+    Powers p2{table};
+    if constexpr (EIGHT) p2 = powers(table);
+    for (int64_t k = begin + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); k < end; k += WAVES) {
+        if (k < whole)
+            block_whole<G, EIGHT>(t, s, key, k, gs, p2);
+        else
+            block_any<G, EIGHT>(t, s, key, k, gs, p2);
+    }
 }
 
 // Sums of the gradients' squares in 64 bits, one to a workgroup.
 constexpr int SQ_ELEMS = 16384;  // of one tensor that a workgroup takes
 struct Squares {
-    int first[MAX_TENSORS + 1];
     const void* g[MAX_TENSORS];
     int64_t n[MAX_TENSORS];
+    int first[MAX_TENSORS];
+    int count;
 };
 template <typename G>
-__global__ __launch_bounds__(NT) void squares_k(Squares tab, int count, double* part) {
+__global__ __launch_bounds__(NT) void squares_k(Squares tab, double* part) {
+    constexpr int N = 16 / sizeof(G), U = 4;
     __shared__ double sh[WAVES];
-    const int group = blockIdx.x, j = tensor_of(tab.first, count, group);
-    const int64_t begin = static_cast<int64_t>(group - tab.first[j]) * SQ_ELEMS, end = min(tab.n[j], begin + SQ_ELEMS);
-    const G* g = static_cast<const G*>(tab.g[j]);
-    double s = 0.0;
-    for (int64_t i = begin + threadIdx.x; i < end; i += NT) {
-        const double x = elem(g, i);
-        s += x * x;
+    const int group = blockIdx.x, j = tensor_of(tab.first, tab.count, group);
+    const int64_t begin = static_cast<int64_t>(group - tab.first[j]) * SQ_ELEMS;
+    const int count = static_cast<int>(min(tab.n[j] - begin, static_cast<int64_t>(SQ_ELEMS)));
+    const G* g = static_cast<const G*>(tab.g[j]) + begin;
+    double q[4] = {0.0, 0.0, 0.0, 0.0};  // chains of additions
+    int from = 0;
+    if ((reinterpret_cast<uintptr_t>(g) & 15) == 0) {  // 16 bytes a lane, four loads on their way
+        from = count / N * N;
+        for (int p0 = threadIdx.x; p0 < count / N; p0 += U * NT) {
+            u32x4 v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) v[u] = p0 + u * NT < count / N ? *reinterpret_cast<const u32x4*>(g + (p0 + u * NT) * N) : u32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if constexpr (N == 4) {
+                        const double x = __uint_as_float(v[u][e]);
+                        q[e] = fma(x, x, q[e]);
+                    } else {
+                        const double x = __uint_as_float(v[u][e] << 16), y = __uint_as_float(v[u][e] & 0xFFFF0000u);
+                        q[e] = fma(y, y, fma(x, x, q[e]));
+                    }
+                }
+            }
+        }
     }
+    for (int i = from + threadIdx.x; i < count; i += NT) {
+        const double x = elem(g, i);
+        q[0] = fma(x, x, q[0]);
+    }
+    double s = (q[0] + q[1]) + (q[2] + q[3]);
     for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o);
     if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
     __syncthreads();
@@ -218,8 +344,8 @@ int run(const pk_adamw_tensor* t, int count, const pk_adamw_config* c, void* wor
     Step s;
     s.lr = c->lr, s.b1 = c->b1, s.b2 = c->b2, s.eps = c->eps, s.wd = c->wd;
     s.rest1 = 1.0f - c->b1, s.rest2 = 1.0f - c->b2;
-    s.c1 = static_cast<float>(1.0 - std::pow(static_cast<double>(c->b1), c->t));
-    s.c2 = static_cast<float>(1.0 - std::pow(static_cast<double>(c->b2), c->t));
+    s.per_c1 = static_cast<float>(1.0 / (1.0 - std::pow(static_cast<double>(c->b1), c->t)));
+    s.per_c2 = static_cast<float>(1.0 / (1.0 - std::pow(static_cast<double>(c->b2), c->t)));
     s.factor = nullptr;
     if (c->max_norm > 0.0f) {
         float* factor = static_cast<float*>(workspace);
@@ -227,15 +353,13 @@ int run(const pk_adamw_tensor* t, int count, const pk_adamw_config* c, void* wor
         int64_t parts = 0;
         for (int i = 0; i < count;) {
             Squares q;
-            int used = 0, groups = 0;
-            for (; i < count && used < MAX_TENSORS; ++i) {
-                if (t[i].n == 0) continue;
-                const int64_t more = (t[i].n + SQ_ELEMS - 1) / SQ_ELEMS;
-                q.first[used] = groups, q.g[used] = t[i].g, q.n[used] = t[i].n;
-                groups += static_cast<int>(more), ++used;
+            int64_t groups = 0;
+            for (q.count = 0; i < count && q.count < MAX_TENSORS; ++i, ++q.count) {
+                q.first[q.count] = static_cast<int>(groups), q.g[q.count] = t[i].g, q.n[q.count] = t[i].n;
+                groups += (t[i].n + SQ_ELEMS - 1) / SQ_ELEMS;
             }
-            if (!used) break;
-            squares_k<G><<<dim3(groups), NT, 0, st>>>(q, used, part + parts);
+            if (groups == 0) continue;
+            squares_k<G><<<dim3(static_cast<unsigned>(groups)), NT, 0, st>>>(q, part + parts);
             if (int rc = launched()) return rc;
             parts += groups;
         }
@@ -245,20 +369,18 @@ int run(const pk_adamw_tensor* t, int count, const pk_adamw_config* c, void* wor
     }
     for (int i = 0; i < count;) {
         Table tab;
-        int used = 0;
         int64_t groups = 0;
-        for (; i < count && used < MAX_TENSORS; ++i) {
-            if (t[i].n == 0) continue;
-            tab.first[used] = static_cast<int>(groups);
-            tab.key[used] = mix(static_cast<uint32_t>(c->seed) * 0x9E3779B9u + mix(static_cast<uint32_t>(i) + 0x3C6EF373u));
-            tab.t[used] = One{t[i].p, t[i].g, t[i].m, t[i].v, t[i].m_scale, t[i].v_scale, static_cast<uint16_t*>(t[i].copy), t[i].n};
-            groups += (t[i].n + BLOCK * BLOCKS_PER_WG - 1) / (BLOCK * BLOCKS_PER_WG), ++used;
+        tab.place = i, tab.seed = c->seed;
+        for (tab.count = 0; i < count && tab.count < MAX_TENSORS; ++i, ++tab.count) {
+            tab.first[tab.count] = static_cast<int>(groups);
+            tab.t[tab.count] = One{t[i].p, t[i].g, t[i].m, t[i].v, t[i].m_scale, t[i].v_scale, static_cast<uint16_t*>(t[i].copy), t[i].n};
+            groups += (t[i].n + BLOCK * BLOCKS_PER_WG - 1) / (BLOCK * BLOCKS_PER_WG);
         }
-        if (!used) break;
+        if (groups == 0) continue;
         if (c->state_bits == 8)
-            adamw_many_k<G, true><<<dim3(static_cast<unsigned>(groups)), NT, 0, st>>>(tab, s, used);
+            adamw_many_k<G, true><<<dim3(static_cast<unsigned>(groups)), NT, 0, st>>>(tab, s);
         else
-            adamw_many_k<G, false><<<dim3(static_cast<unsigned>(groups)), NT, 0, st>>>(tab, s, used);
+            adamw_many_k<G, false><<<dim3(static_cast<unsigned>(groups)), NT, 0, st>>>(tab, s);
         if (int rc = launched()) return rc;
     }
     return PK_OK;
@@ -284,10 +406,12 @@ int pk_adamw_many(const pk_adamw_tensor* t, int count, const pk_adamw_config* c,
         if (!known_dtype(c->grad_dtype)) return fail(PK_ERR_ARGUMENT, "pk_adamw_many: dtype must be PK_F32 or PK_BF16");
         if (!(c->b1 >= 0.0f && c->b1 < 1.0f && c->b2 >= 0.0f && c->b2 < 1.0f)) return fail(PK_ERR_ARGUMENT, "pk_adamw_many: b1 and b2 lie in [0, 1)");
         const bool clip = c->max_norm > 0.0f;
+        int64_t total = 0;  // a launch's workgroups are counted in 32 bits
         std::vector<std::pair<uintptr_t, uintptr_t>> written;
         written.reserve(3 * static_cast<size_t>(count));
         for (int i = 0; i < count; ++i) {
-            if (t[i].n < 0 || t[i].n > (int64_t{1} << 40)) return fail(PK_ERR_SHAPE, "pk_adamw_many: a tensor's size is out of range");
+            total += t[i].n > 0 ? t[i].n : 0;
+            if (t[i].n < 0 || total > (int64_t{1} << 40)) return fail(PK_ERR_SHAPE, "pk_adamw_many: a tensor's size is out of range");
             if (t[i].n == 0) continue;
             if (!t[i].p || !t[i].g || !t[i].m || !t[i].v || (c->state_bits == 8 && (!t[i].m_scale || !t[i].v_scale)))
                 return fail(PK_ERR_ARGUMENT, "pk_adamw_many: null pointer");

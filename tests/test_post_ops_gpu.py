@@ -6,6 +6,7 @@ output carries one rounding to its type, h * |value|, and what the 32-bit arithm
 it. The counts stand at each test."""
 from __future__ import annotations
 
+import functools
 import math
 
 import numpy as np
@@ -471,6 +472,13 @@ def mix32(x):
     return x ^ (x >> 16)
 
 
+@functools.lru_cache(None)
+def powers_of_two():
+    """2^-126 .. 2^127 as torch.ldexp forms them on the device: for some exponents one step of fp32 below the power."""
+    e = torch.arange(-126, 128, device="cuda", dtype=torch.int32)
+    return torch.ldexp(torch.ones(e.numel(), device="cuda"), e).cpu().numpy()
+
+
 def pack8(x, chance, square):
     """numpy restatement of the 8-bit states: codes and scales of a flat fp32 array."""
     x = np.asarray(x, np.float32)
@@ -485,8 +493,8 @@ def pack8(x, chance, square):
             continue
         part, power = np.frexp(most)
         e = max(-126, int(power) - 1 - top + (part > 0.875)) if most > 0 else -126
-        scale[i] = np.ldexp(np.float32(1), e)
-        y = np.ldexp(row, -e).astype(np.float32)
+        scale[i] = powers_of_two()[e + 126]
+        y = row * powers_of_two()[126 - e]
         bits = (np.abs(y) * np.float32(2.0) ** np.float32(-bias)).astype(np.float32).view(np.uint32).astype(np.uint64)
         bits = (bits + (chance[i] << np.uint64(drop - 16)) + np.uint64(1 << (drop - 17))) >> np.uint64(drop)
         codes[i] = np.maximum(bits, row > 0) if square else bits | (np.signbit(y).astype(np.uint64) << np.uint64(7))
