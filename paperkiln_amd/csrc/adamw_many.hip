@@ -322,11 +322,18 @@ __global__ __launch_bounds__(NT) void squares_k(Squares tab, double* part) {
 __global__ __launch_bounds__(1024) void factor_k(const double* part, int64_t parts, float max_norm, float* factor, float* norm) {
     __shared__ double sh[16];
     double s = 0.0;
-    for (int64_t i = threadIdx.x; i < parts; i += 1024) s += part[i];
+    for (int64_t i0 = threadIdx.x; i0 < parts; i0 += 4 * 1024) {
+        double v[4];  // on their way together
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = i0 + k * 1024 < parts ? part[i0 + k * 1024] : 0.0;
+        s += (v[0] + v[1]) + (v[2] + v[3]);
+    }
+#pragma unroll
     for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o);
     if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
     __syncthreads();
     if (threadIdx.x != 0) return;
+#pragma unroll
     for (int w = 1; w < 16; ++w) s += sh[w];
     const double total = sqrt(s), limit = max_norm;
     *factor = total > limit && total > 0.0 ? static_cast<float>(limit / total) : 1.0f;
@@ -337,6 +344,37 @@ int64_t parts_of(const pk_adamw_tensor* t, int count) {
     int64_t n = 0;
     for (int i = 0; i < count; ++i) n += t[i].n > 0 ? (t[i].n + SQ_ELEMS - 1) / SQ_ELEMS : 0;
     return n;
+}
+
+// Whether two of the tensors that are updated have memory in common.
+bool meet(const pk_adamw_tensor* t, int count, uintptr_t state_bytes) {
+    using Span = std::pair<uintptr_t, uintptr_t>;
+    std::vector<Span> spans[3];
+    bool ascending = true;
+    for (int k = 0; k < 3; ++k) {
+        spans[k].reserve(static_cast<size_t>(count));
+        for (int i = 0; i < count; ++i) {
+            if (t[i].n == 0) continue;
+            const uintptr_t at = reinterpret_cast<uintptr_t>(k == 0 ? t[i].p : k == 1 ? t[i].m : t[i].v);
+            ascending = ascending && (spans[k].empty() || spans[k].back().second <= at);
+            spans[k].push_back({at, at + static_cast<uintptr_t>(t[i].n) * (k ? state_bytes : 4)});
+        }
+    }
+    std::vector<Span> all;
+    if (ascending) {  // each list one slab, or in the order of an allocator: the lists' ends say all, where they are apart
+        for (const auto& s : spans)
+            if (!s.empty()) all.push_back({s.front().first, s.back().second});
+        std::sort(all.begin(), all.end());
+        bool apart = true;
+        for (size_t i = 1; i < all.size(); ++i) apart = apart && all[i - 1].second <= all[i].first;
+        if (apart) return false;
+        all.clear();
+    }
+    for (const auto& s : spans) all.insert(all.end(), s.begin(), s.end());
+    std::sort(all.begin(), all.end());
+    for (size_t i = 1; i < all.size(); ++i)
+        if (all[i].first < all[i - 1].second) return true;
+    return false;
 }
 
 template <typename G>
@@ -407,28 +445,21 @@ int pk_adamw_many(const pk_adamw_tensor* t, int count, const pk_adamw_config* c,
         if (!(c->b1 >= 0.0f && c->b1 < 1.0f && c->b2 >= 0.0f && c->b2 < 1.0f)) return fail(PK_ERR_ARGUMENT, "pk_adamw_many: b1 and b2 lie in [0, 1)");
         const bool clip = c->max_norm > 0.0f;
         int64_t total = 0;  // a launch's workgroups are counted in 32 bits
-        std::vector<std::pair<uintptr_t, uintptr_t>> written;
-        written.reserve(3 * static_cast<size_t>(count));
         for (int i = 0; i < count; ++i) {
             total += t[i].n > 0 ? t[i].n : 0;
             if (t[i].n < 0 || total > (int64_t{1} << 40)) return fail(PK_ERR_SHAPE, "pk_adamw_many: a tensor's size is out of range");
-            if (t[i].n == 0) continue;
-            if (!t[i].p || !t[i].g || !t[i].m || !t[i].v || (c->state_bits == 8 && (!t[i].m_scale || !t[i].v_scale)))
+            if (t[i].n > 0 && (!t[i].p || !t[i].g || !t[i].m || !t[i].v || (c->state_bits == 8 && (!t[i].m_scale || !t[i].v_scale))))
                 return fail(PK_ERR_ARGUMENT, "pk_adamw_many: null pointer");
-            const uintptr_t n = static_cast<uintptr_t>(t[i].n), e = n * (c->state_bits / 8);
-            const uintptr_t p = reinterpret_cast<uintptr_t>(t[i].p), m = reinterpret_cast<uintptr_t>(t[i].m), v = reinterpret_cast<uintptr_t>(t[i].v);
-            written.push_back({p, p + 4 * n}), written.push_back({m, m + e}), written.push_back({v, v + e});
         }
-        std::sort(written.begin(), written.end());
-        for (size_t i = 1; i < written.size(); ++i)
-            if (written[i].first < written[i - 1].second) return fail(PK_ERR_ARGUMENT, "pk_adamw_many: a parameter or state is in the list twice");
+        if (meet(t, count, c->state_bits / 8)) return fail(PK_ERR_ARGUMENT, "pk_adamw_many: a parameter or state is in the list twice");
         if (clip && !norm) return fail(PK_ERR_ARGUMENT, "pk_adamw_many: a clip writes the norm");
         if (clip && (!workspace || !aligned(workspace, 8) || workspace_bytes < pk_adamw_many_workspace_bytes(t, count, c)))
             return fail(PK_ERR_WORKSPACE, "pk_adamw_many: workspace too small (pk_adamw_many_workspace_bytes)");
-        for (int i = 0; i < count; ++i)
-            for (const void* p : {static_cast<const void*>(t[i].p), t[i].g, static_cast<const void*>(t[i].m), static_cast<const void*>(t[i].v),
-                                  static_cast<const void*>(t[i].m_scale), static_cast<const void*>(t[i].v_scale), static_cast<const void*>(t[i].copy)})
-                if (p) dev_touch(p, stream);
+        std::vector<const void*> used;
+        used.reserve(7 * static_cast<size_t>(count) + 2);
+        for (int i = 0; i < count; ++i) used.insert(used.end(), {t[i].p, t[i].g, t[i].m, t[i].v, t[i].m_scale, t[i].v_scale, t[i].copy});
+        used.insert(used.end(), {workspace, norm});
+        dev_touch(used.data(), used.size(), stream);
         hipStream_t st = static_cast<hipStream_t>(stream);
         return c->grad_dtype == PK_BF16 ? run<uint16_t>(t, count, c, workspace, norm, st) : run<float>(t, count, c, workspace, norm, st);
     });

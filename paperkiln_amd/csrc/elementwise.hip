@@ -139,6 +139,17 @@ void dev_touch(const void* p, void* stream) {
     if (held != P.handed_out.end()) held->second = st;
 }
 
+void dev_touch(const void* const* ps, size_t n, void* stream) {
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    Pool& P = pool();
+    std::lock_guard<std::mutex> lk(P.mu);
+    if (P.handed_out.empty()) return;
+    for (size_t i = 0; i < n; ++i) {
+        auto held = P.handed_out.find(const_cast<void*>(ps[i]));
+        if (held != P.handed_out.end()) held->second = st;
+    }
+}
+
 bool dev_owns(const void* p) {
     Pool& P = pool();
     std::lock_guard<std::mutex> lk(P.mu);

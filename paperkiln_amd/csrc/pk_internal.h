@@ -24,6 +24,7 @@ int hip_fail(hipError_t e, const char* what);
 // elementwise.hip: tells the caching allocator that one of its blocks is about to be used on `stream`, so that the
 // block, once freed, is only recycled behind that use (no-op for pointers that are not its blocks)
 void dev_touch(const void* p, void* stream);
+void dev_touch(const void* const* ps, size_t n, void* stream);  // the same for n pointers, nulls among them
 
 // Kernel-side view of one attention problem. Strides are in elements.
 struct AttnArgs {

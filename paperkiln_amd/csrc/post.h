@@ -2,6 +2,7 @@
 // sums over a wavefront's lanes, and the argument checks of their C entries.
 #pragma once
 #include <cmath>
+#include <initializer_list>
 #include <string>
 
 #include "mfma_common.h"
@@ -41,6 +42,7 @@ inline int launched() {
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? PK_OK : hip_fail(e, "kernel launch");
 }
+inline void touch(std::initializer_list<const void*> used, void* stream) { dev_touch(used.begin(), used.size(), stream); }
 // The body of a C entry: nothing thrown (a string that finds no memory) leaves it.
 template <typename F>
 int c_entry(F&& f) noexcept {

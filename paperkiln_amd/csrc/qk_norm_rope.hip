@@ -606,8 +606,7 @@ int pk_qk_norm_rope_fwd(const pk_qk_shape* s, const pk_tensor4* q, const pk_tens
         fill(a, s);
         a.x[0] = rows_of(q), a.x[1] = rows_of(k), a.y[0] = out_of(yq), a.y[1] = out_of(yk), a.dy[0] = a.dy[1] = Rows{nullptr, 0, 0, 0};
         a.w[0] = wq, a.w[1] = wk, a.pos = pos;
-        const void* used[] = {q->ptr, k->ptr, yq->ptr, yk->ptr, wq, wk, pos};
-        for (const void* p : used) dev_touch(p, stream);
+        touch({q->ptr, k->ptr, yq->ptr, yk->ptr, wq, wk, pos}, stream);
         hipStream_t st = static_cast<hipStream_t>(stream);
         if (rows_serve(a, s, false)) {
             flatten(a, false);
@@ -646,13 +645,10 @@ int pk_qk_norm_rope_bwd(const pk_qk_shape* s, const pk_tensor4* dyq, const pk_te
         a.part = static_cast<float*>(workspace);
         a.w[0] = wq, a.w[1] = wk, a.pos = pos;
         int groups = any_groups(s);
-        for (const void* p : {static_cast<const void*>(wq), static_cast<const void*>(wk), static_cast<const void*>(dwq), static_cast<const void*>(dwk),
-                              static_cast<const void*>(pos), static_cast<const void*>(workspace)})
-            dev_touch(p, stream);
+        touch({wq, wk, dwq, dwk, pos, workspace}, stream);
         if (!none) {
             a.x[0] = rows_of(q), a.x[1] = rows_of(k), a.dy[0] = rows_of(dyq), a.dy[1] = rows_of(dyk), a.y[0] = out_of(dq), a.y[1] = out_of(dk);
-            const void* used[] = {q->ptr, k->ptr, dyq->ptr, dyk->ptr, dq->ptr, dk->ptr};
-            for (const void* p : used) dev_touch(p, stream);
+            touch({q->ptr, k->ptr, dyq->ptr, dyk->ptr, dq->ptr, dk->ptr}, stream);
             if (rows_serve(a, s, true)) {
                 const Plan p = plan_of(s, BWD_MOST);
                 groups = p.groups * p.parts;

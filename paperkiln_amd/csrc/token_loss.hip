@@ -30,6 +30,9 @@ struct Loss {
     float* clear;             // LOGP: a word per row to set to zero, or null
     const float *lse_in, *coef;  // GRAD
     bool backwards;           // GRAD: the last rows first
+    const double* losses;     // GRAD: the pairs' losses, whose mean the workgroup behind the last row's writes to `loss`
+    int64_t pairs;
+    float* loss;
     const float *old_logp, *ref_logp, *adv, *weights;  // POLICY; ref_logp may be null
     double* row_loss;
     float clip_low, clip_high, kl, upstream;
@@ -51,10 +54,38 @@ __device__ inline void policy_row(const Loss& a, int64_t r, double logp, double&
     }
 }
 
+// n values added up in 64 bits in a fixed order by a workgroup, eight loads of a thread on their way together; the sum in its first thread.
+template <int NT>
+__device__ inline double sum_of(const double* x, int64_t n) {
+    __shared__ double sh[NT / 64];
+    double s = 0.0;
+    for (int64_t i0 = threadIdx.x; i0 < n; i0 += 8 * NT) {
+        double v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = i0 + k * NT < n ? x[i0 + k * NT] : 0.0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s += v[k];
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o);
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
+    __syncthreads();
+    s = sh[0];
+#pragma unroll
+    for (int w = 1; w < NT / 64; ++w) s += sh[w];
+    return s;
+}
+template <int NT>
+__device__ inline void pairs_mean(const Loss& a) {
+    const double s = sum_of<NT>(a.losses, a.pairs);
+    if (threadIdx.x == 0) *a.loss = static_cast<float>(s / static_cast<double>(a.pairs));
+}
+
 // A gradient that does not lie as its logits do (another row pitch, another offset, modulo 16 bytes): a workgroup takes a row element by element.
 constexpr int ANY_NT = 256;
 template <typename T, Mode MODE>
 __global__ __launch_bounds__(ANY_NT) void rows_any(Loss a) {
+    if (MODE == GRAD && blockIdx.x == a.rows) return pairs_mean<ANY_NT>(a);
     __shared__ float sh_m[ANY_NT / 64];
     __shared__ double sh_s[ANY_NT / 64];
     const int64_t r = MODE == GRAD && a.backwards ? a.rows - 1 - blockIdx.x : blockIdx.x;
@@ -379,6 +410,7 @@ constexpr int GRAD_NT = 256, GRAD_U = 4;
 template <typename T>
 __global__ __launch_bounds__(GRAD_NT) void rows_grad(Loss a) {
     constexpr int N = Piece<T>::N;
+    if (blockIdx.x == a.rows) return pairs_mean<GRAD_NT>(a);
     const int64_t r = a.backwards ? a.rows - 1 - blockIdx.x : blockIdx.x;
     const int tid = threadIdx.x, V = a.vocab, t = a.targets[r];
     const T* x = static_cast<const T*>(a.logits) + r * a.ld;
@@ -417,17 +449,9 @@ __global__ __launch_bounds__(GRAD_NT) void rows_grad(Loss a) {
     }
 }
 
-// n values added up in 64 bits in a fixed order, times a factor.
-__global__ __launch_bounds__(1024) void loss_sum(const double* x, int64_t n, double factor, float* out) {
-    __shared__ double sh[16];
-    double s = 0.0;
-    for (int64_t i = threadIdx.x; i < n; i += 1024) s += x[i];
-    for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o);
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
-    __syncthreads();
-    if (threadIdx.x != 0) return;
-    for (int w = 1; w < 16; ++w) s += sh[w];
-    *out = static_cast<float>(s * factor);
+__global__ __launch_bounds__(1024) void loss_sum(const double* x, int64_t n, float* out) {
+    const double s = sum_of<1024>(x, n);
+    if (threadIdx.x == 0) *out = static_cast<float>(s);
 }
 
 struct Pairs {
@@ -442,7 +466,7 @@ struct Pairs {
     float beta, smoothing, upstream;
 };
 // A workgroup takes a pair: both sequences' sums, the pair's loss, and for every row of the two what its gradient is multiplied by.
-constexpr int PAIR_NT = 256;
+constexpr int PAIR_NT = 1024;
 __global__ __launch_bounds__(PAIR_NT) void pair_loss(Pairs a) {
     __shared__ double sh[2][PAIR_NT / 64];
     const int tid = threadIdx.x, seq[2] = {static_cast<int>(blockIdx.x), a.pairs + static_cast<int>(blockIdx.x)};
@@ -499,15 +523,15 @@ void launch_held(const Loss& a, hipStream_t st) {
 template <typename T, Mode MODE>
 void launch_typed(const Loss& a, hipStream_t st) {
     if constexpr (MODE != LOGP)
-        if (!same_cut(a, sizeof(T))) return rows_any<T, MODE><<<dim3(static_cast<unsigned>(a.rows)), ANY_NT, 0, st>>>(a);
+        if (!same_cut(a, sizeof(T))) return rows_any<T, MODE><<<dim3(static_cast<unsigned>(a.rows + (a.loss ? 1 : 0))), ANY_NT, 0, st>>>(a);
     if constexpr (MODE == GRAD)
-        rows_grad<T><<<dim3(static_cast<unsigned>(a.rows)), GRAD_NT, 0, st>>>(a);
+        rows_grad<T><<<dim3(static_cast<unsigned>(a.rows + (a.loss ? 1 : 0))), GRAD_NT, 0, st>>>(a);
     else
         launch_held<T, MODE>(a, st);
 }
 template <Mode MODE>
 int launch_rows(const Loss& a, int dtype, hipStream_t st) {
-    if (a.rows == 0) return PK_OK;
+    if (a.rows == 0 && !a.loss) return PK_OK;
     if (dtype == PK_BF16)
         launch_typed<uint16_t, MODE>(a, st);
     else
@@ -519,7 +543,7 @@ int launch_rows(const Loss& a, int dtype, hipStream_t st) {
 int check(const char* who, const void* logits, int64_t ld, const int* targets, int64_t rows, int64_t vocab, float scale, int dtype, bool writes,
           const void* dlogits, int64_t dld) {
     const std::string w(who);
-    if (rows < 0 || rows > INT32_MAX || vocab <= 0 || vocab > (1 << 30)) return fail(PK_ERR_SHAPE, w + ": shape mismatch (rows or vocabulary out of range)");
+    if (rows < 0 || rows >= INT32_MAX || vocab <= 0 || vocab > (1 << 30)) return fail(PK_ERR_SHAPE, w + ": shape mismatch (rows or vocabulary out of range)");
     if (!known_dtype(dtype)) return fail(PK_ERR_ARGUMENT, w + ": dtype must be PK_F32 or PK_BF16");
     if (!(scale > 0.0f) || !std::isfinite(scale)) return fail(PK_ERR_ARGUMENT, w + ": scale must be positive");
     if (ld < 0 || (writes && rows > 1 && dld < vocab)) return fail(PK_ERR_SHAPE, w + ": rows of logits overlap");
@@ -534,11 +558,6 @@ int check(const char* who, const void* logits, int64_t ld, const int* targets, i
             return fail(PK_ERR_ARGUMENT, w + ": dlogits may lie where the logits do, row for row, or clear of them");
     }
     return PK_OK;
-}
-
-void touch(std::initializer_list<const void*> used, void* stream) {
-    for (const void* p : used)
-        if (p) dev_touch(p, stream);
 }
 
 size_t pad(size_t bytes) { return (bytes + 255) & ~size_t{255}; }
@@ -593,7 +612,7 @@ int pk_policy_loss(const pk_policy_config* c, const void* logits, int64_t ld, co
         a.old_logp = old_logp, a.ref_logp = c->kl_coef != 0.0f ? ref_logp : nullptr, a.adv = advantages, a.weights = weights;
         a.clip_low = c->clip_low, a.clip_high = c->clip_high, a.kl = c->kl_coef, a.upstream = c->upstream;
         if (int rc = launch_rows<POLICY>(a, dtype, st)) return rc;
-        loss_sum<<<1, 1024, 0, st>>>(row_loss, rows, 1.0, loss);
+        loss_sum<<<1, 1024, 0, st>>>(row_loss, rows, loss);
         return launched();
     });
 }
@@ -629,9 +648,7 @@ int pk_preference_loss(const pk_preference_config* c, const void* logits, int64_
         pair_loss<<<dim3(static_cast<unsigned>(pairs)), PAIR_NT, 0, st>>>(
             Pairs{seq_start, targets, fine, ref_logp, coef, margins, losses, rows, static_cast<int>(pairs), c->beta, c->label_smoothing, c->upstream});
         if (int rc = launched()) return rc;
-        loss_sum<<<1, 1024, 0, st>>>(losses, pairs, 1.0 / static_cast<double>(pairs), loss);
-        if (int rc = launched()) return rc;
-        a.dlogits = dlogits, a.dld = dld, a.lse_in = lse, a.coef = coef, a.backwards = true;
+        a.dlogits = dlogits, a.dld = dld, a.lse_in = lse, a.coef = coef, a.backwards = true, a.losses = losses, a.pairs = pairs, a.loss = loss;
         return launch_rows<GRAD>(a, dtype, st);
     });
 }

@@ -252,8 +252,9 @@ std::vector<Tensor> preference(const Tensor& logits, const Tensor& targets, cons
 // ---- AdamW over a list ----
 
 constexpr const char* ADAMW = "adamw_many_";
+using Refs = std::vector<const Tensor*>;  // the caller's own tensors: hundreds of them, so the call keeps the interpreter lock rather than a reference to each
 struct Lists {
-    std::vector<Tensor> p, g, m, v, ms, vs, copy;  // g: undefined where a parameter has no gradient; ms, vs, copy: empty where not asked for
+    Refs p, g, m, v, ms, vs, copy;  // g: null where a parameter has no gradient; ms, vs, copy: empty where not asked for
 };
 void dense(const char* what, const Tensor& t, const Tensor& p, int64_t n, at::ScalarType type) {
     if (t.device() != p.device()) refuse(ADAMW, std::string(what) + " must live on the device of the parameters");
@@ -274,34 +275,34 @@ Tensor adamw_many(const Lists& l, pk_adamw_config c) {
         if (c.max_norm > 0.0f) refuse(ADAMW, "a clip needs parameters");
         return Tensor();
     }
-    on_gpu(ADAMW, l.p[0]);
-    const Tensor& first = l.p[0];
+    on_gpu(ADAMW, *l.p[0]);
+    const Tensor& first = *l.p[0];
     at::ScalarType g_type = at::kFloat;
-    for (const Tensor& g : l.g)
-        if (g.defined()) {
-            g_type = g.scalar_type();
+    for (const Tensor* g : l.g)
+        if (g) {
+            g_type = g->scalar_type();
             break;
         }
     c.grad_dtype = dtype_code(g_type);
     std::vector<pk_adamw_tensor> table(count);
     for (size_t i = 0; i < count; ++i) {
-        const int64_t n = l.p[i].numel();
+        const int64_t n = l.p[i]->numel();
         pk_adamw_tensor& t = table[i];
         t = pk_adamw_tensor{};
-        if (l.p[i].device() != first.device()) refuse(ADAMW, "parameters of one call must live on one device");
-        dense("a parameter", l.p[i], l.p[i], n, at::kFloat);
-        dense("m", l.m[i], first, n, bits8 ? at::kFloat8_e4m3fn : at::kFloat);
-        dense("v", l.v[i], first, n, bits8 ? at::kFloat8_e5m2 : at::kFloat);
+        if (l.p[i]->device() != first.device()) refuse(ADAMW, "parameters of one call must live on one device");
+        dense("a parameter", *l.p[i], first, n, at::kFloat);
+        dense("m", *l.m[i], first, n, bits8 ? at::kFloat8_e4m3fn : at::kFloat);
+        dense("v", *l.v[i], first, n, bits8 ? at::kFloat8_e5m2 : at::kFloat);
         if (bits8) {
-            dense("m_scale", l.ms[i], first, (n + 255) / 256, at::kFloat);
-            dense("v_scale", l.vs[i], first, (n + 255) / 256, at::kFloat);
+            dense("m_scale", *l.ms[i], first, (n + 255) / 256, at::kFloat);
+            dense("v_scale", *l.vs[i], first, (n + 255) / 256, at::kFloat);
         }
-        if (!l.copy.empty()) dense("a copy", l.copy[i], first, n, at::kBFloat16);
-        if (!l.g[i].defined()) continue;  // stays as it is; its place in the list is kept
-        dense("a gradient", l.g[i], first, n, g_type);
-        t.p = static_cast<float*>(l.p[i].data_ptr()), t.g = l.g[i].const_data_ptr(), t.m = l.m[i].data_ptr(), t.v = l.v[i].data_ptr(), t.n = n;
-        if (bits8) t.m_scale = static_cast<float*>(l.ms[i].data_ptr()), t.v_scale = static_cast<float*>(l.vs[i].data_ptr());
-        if (!l.copy.empty()) t.copy = l.copy[i].data_ptr();
+        if (!l.copy.empty()) dense("a copy", *l.copy[i], first, n, at::kBFloat16);
+        if (!l.g[i]) continue;  // stays as it is; its place in the list is kept
+        dense("a gradient", *l.g[i], first, n, g_type);
+        t.p = static_cast<float*>(l.p[i]->data_ptr()), t.g = l.g[i]->const_data_ptr(), t.m = l.m[i]->data_ptr(), t.v = l.v[i]->data_ptr(), t.n = n;
+        if (bits8) t.m_scale = static_cast<float*>(l.ms[i]->data_ptr()), t.v_scale = static_cast<float*>(l.vs[i]->data_ptr());
+        if (!l.copy.empty()) t.copy = l.copy[i]->data_ptr();
     }
     c10::DeviceGuard on(first.device());
     at::AutoDispatchBelowAutograd below;
@@ -313,8 +314,8 @@ Tensor adamw_many(const Lists& l, pk_adamw_config c) {
     check(pk_adamw_many(table.data(), static_cast<int>(count), &c, ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? static_cast<size_t>(ws.numel()) : 0,
                         norm.defined() ? norm.data_ptr<float>() : nullptr, stream()));
     for (const auto* list : {&l.p, &l.m, &l.v, &l.ms, &l.vs, &l.copy})  // what was saved of them for a backward pass is no longer what it was
-        for (const Tensor& t : *list)
-            if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+        for (size_t i = 0; i < list->size(); ++i)
+            if (l.g[i] && !(*list)[i]->is_inference()) (*list)[i]->unsafeGetTensorImpl()->bump_version();
     return norm;
 }
 
@@ -326,30 +327,28 @@ PyObject* tuple_of(std::vector<Tensor>&& v) {
     for (size_t i = 0; i < v.size(); ++i) PyTuple_SET_ITEM(t, static_cast<Py_ssize_t>(i), THPVariable_Wrap(std::move(v[i])));
     return t;
 }
-std::vector<Tensor> list_arg(PyObject* o, const char* what, bool holes) {
-    std::vector<Tensor> v;
+Refs refs_arg(PyObject* o, const char* what, bool holes) {
+    Refs v;
     if (o == Py_None) return v;
-    PyObject* seq = PySequence_Fast(o, "expected a sequence of tensors");
-    if (!seq) throw python_error();
-    const Py_ssize_t n = PySequence_Fast_GET_SIZE(seq);
+    if (!PyList_Check(o) && !PyTuple_Check(o)) throw torch::TypeError(std::string(what) + " must be a list or a tuple of tensors");  // what holds its items
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(o);
     v.reserve(static_cast<size_t>(n));
     for (Py_ssize_t i = 0; i < n; ++i) {
-        PyObject* item = PySequence_Fast_GET_ITEM(seq, i);
+        PyObject* item = PySequence_Fast_GET_ITEM(o, i);
         if (THPVariable_Check(item))
-            v.push_back(THPVariable_Unpack(item));
+            v.push_back(&THPVariable_Unpack(item));
         else if (holes && item == Py_None)
-            v.emplace_back();
-        else {
-            Py_DECREF(seq);
+            v.push_back(nullptr);
+        else
             throw torch::TypeError(std::string(what) + " must hold tensors");
-        }
     }
-    Py_DECREF(seq);
     return v;
 }
 std::vector<Tensor> two_arg(PyObject* o) {
-    std::vector<Tensor> v = list_arg(o, "out", false);
-    if (o != Py_None && v.size() != 2) TORCH_CHECK_VALUE(false, "out must be two tensors");
+    const Refs r = refs_arg(o, "out", false);
+    if (o != Py_None && r.size() != 2) TORCH_CHECK_VALUE(false, "out must be two tensors");
+    std::vector<Tensor> v;
+    for (const Tensor* t : r) v.push_back(*t);
     return v;
 }
 Tensor optional_arg(PyObject* o, const char* what) { return o == Py_None ? Tensor() : tensor_arg(o, what); }
@@ -489,8 +488,8 @@ PyObject* py_adamw_many(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     expect(n, 15);
     Lists l;
-    l.p = list_arg(a[0], "params", false), l.g = list_arg(a[1], "grads", true), l.m = list_arg(a[2], "m", false), l.v = list_arg(a[3], "v", false);
-    l.ms = list_arg(a[4], "m_scale", false), l.vs = list_arg(a[5], "v_scale", false), l.copy = list_arg(a[6], "copies", false);
+    l.p = refs_arg(a[0], "params", false), l.g = refs_arg(a[1], "grads", true), l.m = refs_arg(a[2], "m", false), l.v = refs_arg(a[3], "v", false);
+    l.ms = refs_arg(a[4], "m_scale", false), l.vs = refs_arg(a[5], "v_scale", false), l.copy = refs_arg(a[6], "copies", false);
     pk_adamw_config c{};
     c.lr = number_arg(a[7]), c.b1 = number_arg(a[8]), c.b2 = number_arg(a[9]), c.eps = number_arg(a[10]), c.wd = number_arg(a[11]);
     c.t = whole_arg(a[12], "t"), c.max_norm = number_arg(a[13]);
@@ -500,11 +499,7 @@ PyObject* py_adamw_many(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Py_DECREF(seed);
     if (bits == static_cast<unsigned long long>(-1) && PyErr_Occurred()) throw python_error();
     c.seed = static_cast<uint32_t>(bits);
-    Tensor norm;
-    {
-        pybind11::gil_scoped_release no_gil;
-        norm = adamw_many(l, c);
-    }
+    Tensor norm = adamw_many(l, c);
     if (!norm.defined()) Py_RETURN_NONE;
     return THPVariable_Wrap(std::move(norm));
     END_HANDLE_TH_ERRORS
