@@ -29,7 +29,6 @@ struct Loss {
     double* fine;             // LOGP: the log-probability in 64 bits, or null
     float* clear;             // LOGP: a word per row to set to zero, or null
     const float *lse_in, *coef;  // GRAD
-    bool backwards;           // GRAD: the last rows first
     const double* losses;     // GRAD: the pairs' losses, whose mean the workgroup behind the last row's writes to `loss`
     int64_t pairs;
     float* loss;
@@ -88,7 +87,7 @@ __global__ __launch_bounds__(ANY_NT) void rows_any(Loss a) {
     if (MODE == GRAD && blockIdx.x == a.rows) return pairs_mean<ANY_NT>(a);
     __shared__ float sh_m[ANY_NT / 64];
     __shared__ double sh_s[ANY_NT / 64];
-    const int64_t r = MODE == GRAD && a.backwards ? a.rows - 1 - blockIdx.x : blockIdx.x;
+    const int64_t r = blockIdx.x;
     const int tid = threadIdx.x, V = a.vocab, t = a.targets[r];
     const T* x = static_cast<const T*>(a.logits) + r * a.ld;
     T* dx = MODE == LOGP ? nullptr : static_cast<T*>(a.dlogits) + r * a.dld;
@@ -209,6 +208,24 @@ struct Cut {  // a row's pieces
     __device__ int edge(int i) const { return i < head ? i : i + pieces * Piece<T>::N; }
 };
 
+// A piece read for the last time, or written, past the last-level cache or through it.
+template <bool PAST, typename T>
+__device__ inline Piece<T> load_piece(const T* x) {
+    const u32x4* p = reinterpret_cast<const u32x4*>(x);
+    if constexpr (PAST)
+        return Piece<T>{__builtin_nontemporal_load(p)};
+    else
+        return Piece<T>{*p};
+}
+template <bool PAST, typename T>
+__device__ inline void store_piece(T* x, const Piece<T>& v) {
+    u32x4* p = reinterpret_cast<u32x4*>(x);
+    if constexpr (PAST)
+        __builtin_nontemporal_store(v.v, p);
+    else
+        *p = v.v;
+}
+
 // log2 of the sum of 2^(s2 x) over a row from what each wavefront has: the largest s2 x that it took its exponentials against and their sum.
 template <int WAVES>
 __device__ inline double lse2_of(const float (&m)[WAVES], const float (&s)[WAVES]) {
@@ -249,9 +266,9 @@ __device__ inline void no_row(const Loss& a, int64_t r) {
     if (a.lse) a.lse[r] = 0.0f;
     if (MODE == POLICY) a.row_loss[r] = 0.0;
 }
-template <typename T, int NT>
+template <typename T, int NT, bool PAST>
 __device__ inline void zero_row(T* dx, const Cut<T>& cut, int tid) {
-    for (int p = tid; p < cut.pieces; p += NT) *reinterpret_cast<u32x4*>(dx + cut.head + p * Piece<T>::N) = u32x4{0, 0, 0, 0};
+    for (int p = tid; p < cut.pieces; p += NT) store_piece<PAST>(dx + cut.head + p * Piece<T>::N, Piece<T>{{0, 0, 0, 0}});
     if (tid < cut.edges) put(dx, cut.edge(tid), 0.0f);
 }
 // The gradient of a piece whose first word is j0.
@@ -274,7 +291,7 @@ __device__ inline void keep_packed(Piece<T> (&held)[PER]) {
 
 // ROW_NT threads hold a row, PER pieces each, so that the logits are read once. One exchange through LDS joins the wavefronts; the first one works out the
 // row's scalars in 64 bits and hands them round.
-template <typename T, Mode MODE, int ROW_NT, int PER>
+template <typename T, Mode MODE, int ROW_NT, int PER, bool PAST>
 __global__ __launch_bounds__(ROW_NT) void rows_held(Loss a) {
     constexpr int WAVES = ROW_NT / 64, N = Piece<T>::N;
     __shared__ float sh_m[WAVES], sh_s[WAVES];
@@ -287,7 +304,7 @@ __global__ __launch_bounds__(ROW_NT) void rows_held(Loss a) {
     if (MODE == LOGP && a.clear && tid == 0) a.clear[r] = 0.0f;
     if (t < 0 || (MODE == POLICY && a.weights[r] == 0.0f)) {
         if (tid == 0) no_row<MODE>(a, r);
-        if (MODE != LOGP) zero_row<T, ROW_NT>(dx, cut, tid);
+        if (MODE != LOGP) zero_row<T, ROW_NT, PAST>(dx, cut, tid);
         return;
     }
     const float s2 = a.scale * LOG2E;
@@ -295,7 +312,7 @@ __global__ __launch_bounds__(ROW_NT) void rows_held(Loss a) {
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
         const int p = tid + k * ROW_NT;
-        held[k] = p < cut.pieces ? *reinterpret_cast<const Piece<T>*>(x + cut.head + p * N) : Piece<T>::nothing();
+        held[k] = p < cut.pieces ? load_piece<PAST>(x + cut.head + p * N) : Piece<T>::nothing();
     }
     const float edge = tid < cut.edges ? elem(x, cut.edge(tid)) : -INFINITY;
     const float xt = t < V ? elem(x, t) : NAN;  // read before the row is written over; a token that is no word has no probability
@@ -327,12 +344,12 @@ __global__ __launch_bounds__(ROW_NT) void rows_held(Loss a) {
         o = sh_o;
     }
     if constexpr (MODE != LOGP) {
-        if (o.coef == 0.0f) return zero_row<T, ROW_NT>(dx, cut, tid);  // clipped
+        if (o.coef == 0.0f) return zero_row<T, ROW_NT, PAST>(dx, cut, tid);  // clipped
         keep_packed(held);
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
             const int p = tid + k * ROW_NT, j0 = cut.head + p * N;
-            if (p < cut.pieces) *reinterpret_cast<Piece<T>*>(dx + j0) = gradient(held[k], j0, t, s2, o);
+            if (p < cut.pieces) store_piece<PAST>(dx + j0, gradient(held[k], j0, t, s2, o));
         }
         if (tid < cut.edges) {
             const int j = cut.edge(tid);
@@ -343,7 +360,7 @@ __global__ __launch_bounds__(ROW_NT) void rows_held(Loss a) {
 
 // Rows that no workgroup holds: read in strides with a running maximum and sum, and again for the gradient.
 constexpr int LONG_NT = 1024, LONG_U = 4;
-template <typename T, Mode MODE>
+template <typename T, Mode MODE, bool PAST>
 __global__ __launch_bounds__(LONG_NT) void rows_long(Loss a) {
     constexpr int WAVES = LONG_NT / 64, N = Piece<T>::N;
     __shared__ float sh_m[WAVES], sh_s[WAVES];
@@ -356,7 +373,7 @@ __global__ __launch_bounds__(LONG_NT) void rows_long(Loss a) {
     if (MODE == LOGP && a.clear && tid == 0) a.clear[r] = 0.0f;
     if (t < 0 || (MODE == POLICY && a.weights[r] == 0.0f)) {
         if (tid == 0) no_row<MODE>(a, r);
-        if (MODE != LOGP) zero_row<T, LONG_NT>(dx, cut, tid);
+        if (MODE != LOGP) zero_row<T, LONG_NT, PAST>(dx, cut, tid);
         return;
     }
     const float s2 = a.scale * LOG2E;
@@ -393,10 +410,10 @@ __global__ __launch_bounds__(LONG_NT) void rows_long(Loss a) {
     if constexpr (MODE != LOGP) {
         __syncthreads();
         o = sh_o;
-        if (o.coef == 0.0f) return zero_row<T, LONG_NT>(dx, cut, tid);
+        if (o.coef == 0.0f) return zero_row<T, LONG_NT, PAST>(dx, cut, tid);
         for (int p = tid; p < cut.pieces; p += LONG_NT) {
             const int j0 = cut.head + p * N;
-            *reinterpret_cast<Piece<T>*>(dx + j0) = gradient(*reinterpret_cast<const Piece<T>*>(x + j0), j0, t, s2, o);
+            store_piece<PAST>(dx + j0, gradient(load_piece<PAST>(x + j0), j0, t, s2, o));
         }
         if (tid < cut.edges) {
             const int j = cut.edge(tid);
@@ -406,19 +423,19 @@ __global__ __launch_bounds__(LONG_NT) void rows_long(Loss a) {
 }
 
 // The gradient of rows whose sums are known: every element by itself.
-constexpr int GRAD_NT = 256, GRAD_U = 4;
-template <typename T>
+constexpr int GRAD_NT = 512, GRAD_U = 8;
+template <typename T, bool PAST>
 __global__ __launch_bounds__(GRAD_NT) void rows_grad(Loss a) {
     constexpr int N = Piece<T>::N;
     if (blockIdx.x == a.rows) return pairs_mean<GRAD_NT>(a);
-    const int64_t r = a.backwards ? a.rows - 1 - blockIdx.x : blockIdx.x;
+    const int64_t r = a.rows - 1 - blockIdx.x;  // the last rows first: they are what the pass before has left in the last-level cache
     const int tid = threadIdx.x, V = a.vocab, t = a.targets[r];
     const T* x = static_cast<const T*>(a.logits) + r * a.ld;
     T* dx = static_cast<T*>(a.dlogits) + r * a.dld;
     const Cut<T> cut(x, V);
     RowOut o;
     o.coef = a.coef[r] * a.scale;
-    if (t < 0 || o.coef == 0.0f) return zero_row<T, GRAD_NT>(dx, cut, tid);
+    if (t < 0 || o.coef == 0.0f) return zero_row<T, GRAD_NT, PAST>(dx, cut, tid);
     const float s2 = a.scale * LOG2E, xt = t < V ? elem(x, t) : NAN;
     const double lse2 = a.lse_in[r] / LN2;
     o.lse2 = static_cast<float>(lse2);
@@ -439,12 +456,12 @@ __global__ __launch_bounds__(GRAD_NT) void rows_grad(Loss a) {
 #pragma unroll
         for (int u = 0; u < GRAD_U; ++u) {
             const int p = p0 + u * GRAD_NT;
-            if (p < cut.pieces) v[u] = *reinterpret_cast<const Piece<T>*>(x + cut.head + p * N);
+            if (p < cut.pieces) v[u] = load_piece<PAST>(x + cut.head + p * N);
         }
 #pragma unroll
         for (int u = 0; u < GRAD_U; ++u) {
             const int p = p0 + u * GRAD_NT, j0 = cut.head + p * N;
-            if (p < cut.pieces) *reinterpret_cast<Piece<T>*>(dx + j0) = gradient(v[u], j0, t, s2, o);
+            if (p < cut.pieces) store_piece<PAST>(dx + j0, gradient(v[u], j0, t, s2, o));
         }
     }
 }
@@ -501,33 +518,42 @@ __global__ __launch_bounds__(PAIR_NT) void pair_loss(Pairs a) {
         for (int64_t r = begin[k] + tid; r < end[k]; r += PAIR_NT) a.coef[r] = k ? -slope : slope;
 }
 
+// From here on logits and gradient do not stay in the 256 MB of the last-level cache together. A gradient that passes it by leaves it to the logits, which the
+// preference loss reads again (197 MB of logits 120.7 -> 100.0 us; 524 MB 308 -> 271), and takes less time to write (policy loss 81.3 -> 72.0; 204 -> 181). The
+// product behind the loss then finds less of a small one there: loss and product of 33 MB 120.7 -> 128.7 us, 66 MB 172.8 -> 185.3, 98 MB 228.6 -> 229.3, 131 MB
+// 254.0 -> 251.9, 262 MB 392.5 -> 387.2.
+constexpr int64_t PAST_BYTES = int64_t{96} << 20;
 // Whether what is written lies as what is read, modulo a piece, in every row.
 bool same_cut(const Loss& a, int64_t es) {
     return (reinterpret_cast<uintptr_t>(a.logits) - reinterpret_cast<uintptr_t>(a.dlogits)) % 16 == 0 && (a.ld - a.dld) * es % 16 == 0;
 }
-template <typename T, Mode MODE>
+template <typename T, Mode MODE, bool PAST>
 void launch_held(const Loss& a, hipStream_t st) {
     const dim3 grid(static_cast<unsigned>(a.rows));
     const int pieces = a.vocab / Piece<T>::N;
-    if (pieces <= 64) return rows_held<T, MODE, 64, 1><<<grid, 64, 0, st>>>(a);
-    if (pieces <= 128) return rows_held<T, MODE, 64, 2><<<grid, 64, 0, st>>>(a);
-    if (pieces <= 256) return rows_held<T, MODE, 64, 4><<<grid, 64, 0, st>>>(a);
-    if (pieces <= 512) return rows_held<T, MODE, 256, 2><<<grid, 256, 0, st>>>(a);
-    if (pieces <= 1024) return rows_held<T, MODE, 256, 4><<<grid, 256, 0, st>>>(a);
-    if (pieces <= 2048) return rows_held<T, MODE, 256, 8><<<grid, 256, 0, st>>>(a);
-    if (pieces <= 4096) return rows_held<T, MODE, 512, 8><<<grid, 512, 0, st>>>(a);
-    if (pieces <= 8192) return rows_held<T, MODE, 1024, 8><<<grid, 1024, 0, st>>>(a);
-    if (pieces <= 16384) return rows_held<T, MODE, 1024, 16><<<grid, 1024, 0, st>>>(a);
-    rows_long<T, MODE><<<grid, LONG_NT, 0, st>>>(a);
+    if (pieces <= 64) return rows_held<T, MODE, 64, 1, PAST><<<grid, 64, 0, st>>>(a);
+    if (pieces <= 128) return rows_held<T, MODE, 64, 2, PAST><<<grid, 64, 0, st>>>(a);
+    if (pieces <= 256) return rows_held<T, MODE, 64, 4, PAST><<<grid, 64, 0, st>>>(a);
+    if (pieces <= 512) return rows_held<T, MODE, 256, 2, PAST><<<grid, 256, 0, st>>>(a);
+    if (pieces <= 1024) return rows_held<T, MODE, 256, 4, PAST><<<grid, 256, 0, st>>>(a);
+    if (pieces <= 2048) return rows_held<T, MODE, 256, 8, PAST><<<grid, 256, 0, st>>>(a);
+    if (pieces <= 4096) return rows_held<T, MODE, 512, 8, PAST><<<grid, 512, 0, st>>>(a);
+    if (pieces <= 8192) return rows_held<T, MODE, 1024, 8, PAST><<<grid, 1024, 0, st>>>(a);
+    if (pieces <= 16384) return rows_held<T, MODE, 1024, 16, PAST><<<grid, 1024, 0, st>>>(a);
+    rows_long<T, MODE, PAST><<<grid, LONG_NT, 0, st>>>(a);
 }
 template <typename T, Mode MODE>
 void launch_typed(const Loss& a, hipStream_t st) {
-    if constexpr (MODE != LOGP)
-        if (!same_cut(a, sizeof(T))) return rows_any<T, MODE><<<dim3(static_cast<unsigned>(a.rows + (a.loss ? 1 : 0))), ANY_NT, 0, st>>>(a);
-    if constexpr (MODE == GRAD)
-        rows_grad<T><<<dim3(static_cast<unsigned>(a.rows + (a.loss ? 1 : 0))), GRAD_NT, 0, st>>>(a);
-    else
-        launch_held<T, MODE>(a, st);
+    const bool past = a.rows * a.vocab * static_cast<int64_t>(sizeof(T)) >= PAST_BYTES;
+    const dim3 grid(static_cast<unsigned>(a.rows + (a.loss ? 1 : 0)));
+    if constexpr (MODE == LOGP) return launch_held<T, MODE, false>(a, st);  // the logits are read again for their gradient
+    else {
+        if (!same_cut(a, sizeof(T))) return rows_any<T, MODE><<<grid, ANY_NT, 0, st>>>(a);
+        if constexpr (MODE == GRAD)
+            past ? rows_grad<T, true><<<grid, GRAD_NT, 0, st>>>(a) : rows_grad<T, false><<<grid, GRAD_NT, 0, st>>>(a);
+        else
+            past ? launch_held<T, MODE, true>(a, st) : launch_held<T, MODE, false>(a, st);
+    }
 }
 template <Mode MODE>
 int launch_rows(const Loss& a, int dtype, hipStream_t st) {
@@ -648,7 +674,7 @@ int pk_preference_loss(const pk_preference_config* c, const void* logits, int64_
         pair_loss<<<dim3(static_cast<unsigned>(pairs)), PAIR_NT, 0, st>>>(
             Pairs{seq_start, targets, fine, ref_logp, coef, margins, losses, rows, static_cast<int>(pairs), c->beta, c->label_smoothing, c->upstream});
         if (int rc = launched()) return rc;
-        a.dlogits = dlogits, a.dld = dld, a.lse_in = lse, a.coef = coef, a.backwards = true, a.losses = losses, a.pairs = pairs, a.loss = loss;
+        a.dlogits = dlogits, a.dld = dld, a.lse_in = lse, a.coef = coef, a.losses = losses, a.pairs = pairs, a.loss = loss;
         return launch_rows<GRAD>(a, dtype, st);
     });
 }

@@ -1,6 +1,7 @@
 // The post-training operators of paperkiln_amd.ops and paperkiln_amd.blockops on torch tensors: argument checks, output and workspace allocation, the C ABI
 // call and, for the two that stand inside a model, the autograd node. As in torch_ops.cpp Python keeps the signatures. Every call runs on the device of its
 // tensors and on that device's current stream; outputs and workspaces come from torch's allocator on that stream.
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 
 #include <cmath>
@@ -11,6 +12,9 @@
 
 namespace pk_torch {
 namespace {
+
+// As torch_args.h's empty_of, past the dispatcher: a call on a few tokens is host time, and these are half of it.
+Tensor new_tensor(at::IntArrayRef sizes, at::ScalarType t, const Tensor& like) { return at::detail::empty_cuda(sizes, t, like.device(), c10::nullopt); }
 
 [[noreturn]] void refuse(const char* who, const std::string& what) { throw std::runtime_error(std::string(who) + ": " + what); }
 
@@ -74,7 +78,7 @@ std::pair<Tensor, Tensor> qk_fwd(const Tensor& q, const Tensor& k, const Tensor&
     const pk_qk_shape s = qk_shape(q, k, wq, wk, pos, o);
     c10::DeviceGuard on(q.device());
     at::AutoDispatchBelowAutograd below;
-    Tensor yq = out.empty() ? empty_of(q.sizes(), q.scalar_type(), q) : out[0], yk = out.empty() ? empty_of(k.sizes(), k.scalar_type(), q) : out[1];
+    Tensor yq = out.empty() ? new_tensor(q.sizes(), q.scalar_type(), q) : out[0], yk = out.empty() ? new_tensor(k.sizes(), k.scalar_type(), q) : out[1];
     like(yq, q, "out"), like(yk, k, "out");
     const pk_tensor4 q4 = heads(q, "q"), k4 = heads(k, "k"), yq4 = heads(yq, "out"), yk4 = heads(yk, "out");
     check(pk_qk_norm_rope_fwd(&s, &q4, &k4, wq.const_data_ptr<float>(), wk.const_data_ptr<float>(), pos.const_data_ptr<int>(), &yq4, &yk4, stream()));
@@ -88,11 +92,11 @@ std::vector<Tensor> qk_bwd(Tensor dyq, Tensor dyk, const Tensor& q, const Tensor
     like(dyq, q, "dyq"), like(dyk, k, "dyk");
     if (dyq.stride(3) != 1) dyq = dyq.contiguous();
     if (dyk.stride(3) != 1) dyk = dyk.contiguous();
-    Tensor dq = out.empty() ? empty_of(q.sizes(), q.scalar_type(), q) : out[0], dk = out.empty() ? empty_of(k.sizes(), k.scalar_type(), q) : out[1];
+    Tensor dq = out.empty() ? new_tensor(q.sizes(), q.scalar_type(), q) : out[0], dk = out.empty() ? new_tensor(k.sizes(), k.scalar_type(), q) : out[1];
     like(dq, q, "out"), like(dk, k, "out");
-    Tensor dwq = empty_of(wq.sizes(), at::kFloat, q), dwk = empty_of(wk.sizes(), at::kFloat, q);
+    Tensor dwq = new_tensor(wq.sizes(), at::kFloat, q), dwk = new_tensor(wk.sizes(), at::kFloat, q);
     const int64_t bytes = static_cast<int64_t>(pk_qk_norm_rope_bwd_workspace_bytes(&s));
-    Tensor ws = empty_of({bytes > 16 ? bytes : 16}, at::kByte, q);
+    Tensor ws = new_tensor({bytes > 16 ? bytes : 16}, at::kByte, q);
     const pk_tensor4 gq = heads(dyq, "dyq"), gk = heads(dyk, "dyk"), q4 = heads(q, "q"), k4 = heads(k, "k"), dq4 = heads(dq, "out"), dk4 = heads(dk, "out");
     check(pk_qk_norm_rope_bwd(&s, &gq, &gk, &q4, &k4, wq.const_data_ptr<float>(), wk.const_data_ptr<float>(), pos.const_data_ptr<int>(), &dq4, &dk4,
                               dwq.data_ptr<float>(), dwk.data_ptr<float>(), ws.data_ptr(), static_cast<size_t>(ws.numel()), stream()));
@@ -148,7 +152,7 @@ Logits matrix(const char* who, const char* what, const Tensor& x) {
     return Logits{x.size(0), x.size(1), x.size(0) > 1 ? x.stride(0) : x.size(1), dtype_code(x.scalar_type())};
 }
 Tensor gradient_of(const char* who, const Tensor& logits, const Tensor& out) {
-    if (!out.defined()) return empty_of(logits.sizes(), logits.scalar_type(), logits);
+    if (!out.defined()) return new_tensor(logits.sizes(), logits.scalar_type(), logits);
     if (out.sizes() != logits.sizes() || out.scalar_type() != logits.scalar_type() || out.device() != logits.device()) refuse(who, "shape mismatch: out");
     return out;
 }
@@ -159,7 +163,7 @@ std::pair<Tensor, Tensor> logprobs_fwd(const Tensor& logits, const Tensor& targe
     vector_of(LP, "targets", targets, at::kInt, m.rows, logits);
     c10::DeviceGuard on(logits.device());
     at::AutoDispatchBelowAutograd below;
-    Tensor logp = empty_of({m.rows}, at::kFloat, logits), lse = empty_of({m.rows}, at::kFloat, logits);
+    Tensor logp = new_tensor({m.rows}, at::kFloat, logits), lse = new_tensor({m.rows}, at::kFloat, logits);
     check(pk_token_logprobs_fwd(logits.const_data_ptr(), m.ld, targets.const_data_ptr<int>(), m.rows, m.vocab, static_cast<float>(scale), logp.data_ptr<float>(),
                                 lse.data_ptr<float>(), m.dtype, stream()));
     return {std::move(logp), std::move(lse)};
@@ -220,8 +224,8 @@ std::vector<Tensor> policy(const Tensor& logits, const Tensor& targets, const Te
     if (ref.defined()) vector_of(who, "ref_logp", ref, at::kFloat, m.rows, logits);
     c10::DeviceGuard on(logits.device());
     at::AutoDispatchBelowAutograd below;
-    Tensor d = gradient_of(who, logits, out), logp = empty_of({m.rows}, at::kFloat, logits), rows = empty_of({m.rows}, at::kDouble, logits),
-           loss = empty_of({}, at::kFloat, logits);
+    Tensor d = gradient_of(who, logits, out), logp = new_tensor({m.rows}, at::kFloat, logits), rows = new_tensor({m.rows}, at::kDouble, logits),
+           loss = new_tensor({}, at::kFloat, logits);
     const Logits g = matrix(who, "out", d);
     check(pk_policy_loss(&c, logits.const_data_ptr(), m.ld, targets.const_data_ptr<int>(), old.const_data_ptr<float>(),
                          ref.defined() ? ref.const_data_ptr<float>() : nullptr, adv.const_data_ptr<float>(), weights.const_data_ptr<float>(), m.rows, m.vocab,
@@ -240,8 +244,8 @@ std::vector<Tensor> preference(const Tensor& logits, const Tensor& targets, cons
     const int64_t pairs = (starts.numel() - 1) / 2, bytes = static_cast<int64_t>(pk_preference_loss_workspace_bytes(m.rows, pairs));
     c10::DeviceGuard on(logits.device());
     at::AutoDispatchBelowAutograd below;
-    Tensor d = gradient_of(who, logits, out), logp = empty_of({m.rows}, at::kFloat, logits), margins = empty_of({pairs}, at::kFloat, logits),
-           loss = empty_of({}, at::kFloat, logits), ws = empty_of({bytes}, at::kByte, logits);
+    Tensor d = gradient_of(who, logits, out), logp = new_tensor({m.rows}, at::kFloat, logits), margins = new_tensor({pairs}, at::kFloat, logits),
+           loss = new_tensor({}, at::kFloat, logits), ws = new_tensor({bytes}, at::kByte, logits);
     const Logits g = matrix(who, "out", d);
     check(pk_preference_loss(&c, logits.const_data_ptr(), m.ld, targets.const_data_ptr<int>(), starts.const_data_ptr<int>(), pairs, ref.const_data_ptr<float>(),
                              m.rows, m.vocab, d.data_ptr(), g.ld, logp.data_ptr<float>(), margins.data_ptr<float>(), loss.data_ptr<float>(), ws.data_ptr(),
@@ -308,8 +312,8 @@ Tensor adamw_many(const Lists& l, pk_adamw_config c) {
     at::AutoDispatchBelowAutograd below;
     Tensor norm, ws;
     if (c.max_norm > 0.0f) {
-        norm = empty_of({}, at::kFloat, first);
-        ws = empty_of({static_cast<int64_t>(pk_adamw_many_workspace_bytes(table.data(), static_cast<int>(count), &c))}, at::kByte, first);
+        norm = new_tensor({}, at::kFloat, first);
+        ws = new_tensor({static_cast<int64_t>(pk_adamw_many_workspace_bytes(table.data(), static_cast<int>(count), &c))}, at::kByte, first);
     }
     check(pk_adamw_many(table.data(), static_cast<int>(count), &c, ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? static_cast<size_t>(ws.numel()) : 0,
                         norm.defined() ? norm.data_ptr<float>() : nullptr, stream()));
