@@ -304,7 +304,8 @@ typedef struct pk_qk_shape {
                             (pk_op_rope's is the reference's 32-bit product) */
     int64_t pos_stride_b; /* pos[b * pos_stride_b + t], on the device; 0 = one row of positions for all sequences */
 } pk_qk_shape;
-/* yq / yk may lie where q / k do, element for element. */
+/* yq / yk may lie where q / k do, element for element. Results that overlap inputs, or each other, in any other way are
+ * undefined, here and in the backward. */
 int pk_qk_norm_rope_fwd(const pk_qk_shape* s, const pk_tensor4* q, const pk_tensor4* k, const float* wq, const float* wk,
                         const int* pos, const pk_tensor4* yq, const pk_tensor4* yk, void* stream);
 /* The gradients, from the inputs: r is formed again. dwq, dwk [dk] fp32 are overwritten; their sums are taken in a
@@ -363,7 +364,7 @@ int pk_preference_loss(const pk_preference_config* c, const void* logits, int64_
  * in either. Values between two of the format's are rounded up or down at random with the value itself as the mean,
  * drawn from (seed, the tensor's place in the list, the element's place in the tensor): give another seed each step. A v
  * that is not zero does not become zero. A block in which a value is not finite becomes NaN.
- * A tensor or state that is in the list twice is refused. */
+ * A parameter, state or copy that is in the list twice is refused. */
 typedef struct pk_adamw_tensor {
     float* p;
     const void* g;           /* fp32 or bf16, the same for all (grad_dtype) */

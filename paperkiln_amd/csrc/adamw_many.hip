@@ -352,18 +352,21 @@ int64_t parts_of(const pk_adamw_tensor* t, int count) {
     return n;
 }
 
-// Whether two of the tensors that are updated have memory in common.
-bool meet(const pk_adamw_tensor* t, int count, uintptr_t state_bytes) {
+// Whether two of the tensors that are written have memory in common.
+bool meet(const pk_adamw_tensor* t, int count, bool eight) {
     using Span = std::pair<uintptr_t, uintptr_t>;
-    std::vector<Span> spans[3];
+    std::vector<Span> spans[6];
     bool ascending = true;
-    for (int k = 0; k < 3; ++k) {
+    for (int k = 0; k < 6; ++k) {
+        if ((k == 3 || k == 4) && !eight) continue;
         spans[k].reserve(static_cast<size_t>(count));
         for (int i = 0; i < count; ++i) {
-            if (t[i].n == 0) continue;
-            const uintptr_t at = reinterpret_cast<uintptr_t>(k == 0 ? t[i].p : k == 1 ? t[i].m : t[i].v);
+            const void* const p = k == 0 ? t[i].p : k == 1 ? t[i].m : k == 2 ? t[i].v : k == 3 ? t[i].m_scale : k == 4 ? t[i].v_scale : t[i].copy;
+            if (t[i].n == 0 || !p) continue;
+            const uintptr_t n = static_cast<uintptr_t>(t[i].n), at = reinterpret_cast<uintptr_t>(p);
+            const uintptr_t bytes = k == 0 ? 4 * n : k < 3 ? n * (eight ? 1 : 4) : k < 5 ? 4 * ((n + BLOCK - 1) / BLOCK) : 2 * n;
             ascending = ascending && (spans[k].empty() || spans[k].back().second <= at);
-            spans[k].push_back({at, at + static_cast<uintptr_t>(t[i].n) * (k ? state_bytes : 4)});
+            spans[k].push_back({at, at + bytes});
         }
     }
     std::vector<Span> all;
@@ -449,6 +452,7 @@ int pk_adamw_many(const pk_adamw_tensor* t, int count, const pk_adamw_config* c,
         if (c->state_bits != 8 && c->state_bits != 32) return fail(PK_ERR_ARGUMENT, "pk_adamw_many: states are held in 8 or in 32 bits");
         if (!known_dtype(c->grad_dtype)) return fail(PK_ERR_ARGUMENT, "pk_adamw_many: dtype must be PK_F32 or PK_BF16");
         if (!(c->b1 >= 0.0f && c->b1 < 1.0f && c->b2 >= 0.0f && c->b2 < 1.0f)) return fail(PK_ERR_ARGUMENT, "pk_adamw_many: b1 and b2 lie in [0, 1)");
+        if (c->max_norm != c->max_norm) return fail(PK_ERR_ARGUMENT, "pk_adamw_many: max_norm is no number");
         const bool clip = c->max_norm > 0.0f;
         int64_t total = 0;  // a launch's workgroups are counted in 32 bits
         for (int i = 0; i < count; ++i) {
@@ -457,7 +461,7 @@ int pk_adamw_many(const pk_adamw_tensor* t, int count, const pk_adamw_config* c,
             if (t[i].n > 0 && (!t[i].p || !t[i].g || !t[i].m || !t[i].v || (c->state_bits == 8 && (!t[i].m_scale || !t[i].v_scale))))
                 return fail(PK_ERR_ARGUMENT, "pk_adamw_many: null pointer");
         }
-        if (meet(t, count, c->state_bits / 8)) return fail(PK_ERR_ARGUMENT, "pk_adamw_many: a parameter or state is in the list twice");
+        if (meet(t, count, c->state_bits == 8)) return fail(PK_ERR_ARGUMENT, "pk_adamw_many: a parameter, state or copy is in the list twice");
         if (clip && !norm) return fail(PK_ERR_ARGUMENT, "pk_adamw_many: a clip writes the norm");
         if (clip && (!workspace || !aligned(workspace, 8) || workspace_bytes < pk_adamw_many_workspace_bytes(t, count, c)))
             return fail(PK_ERR_WORKSPACE, "pk_adamw_many: workspace too small (pk_adamw_many_workspace_bytes)");

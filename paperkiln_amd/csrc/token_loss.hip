@@ -511,7 +511,8 @@ __global__ __launch_bounds__(PAIR_NT) void pair_loss(Pairs a) {
     const float slope = static_cast<float>((e * yes - (1.0 - e) * no) * a.beta * a.upstream / a.pairs);
     if (tid == 0) {
         a.margins[blockIdx.x] = static_cast<float>(u);
-        a.losses[blockIdx.x] = u != u ? u : (1.0 - e) * lost_no + e * lost_yes;
+        // a weight of zero drops its term, also an infinite one (a word without probability in an answer)
+        a.losses[blockIdx.x] = u != u ? u : (e < 1.0 ? (1.0 - e) * lost_no : 0.0) + (e > 0.0 ? e * lost_yes : 0.0);
     }
 #pragma unroll
     for (int k = 0; k < 2; ++k)

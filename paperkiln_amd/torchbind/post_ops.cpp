@@ -1,6 +1,7 @@
 // The post-training operators of paperkiln_amd.ops and paperkiln_amd.blockops on torch tensors: argument checks, output and workspace allocation, the C ABI
 // call and, for the two that stand inside a model, the autograd node. As in torch_ops.cpp Python keeps the signatures. Every call runs on the device of its
 // tensors and on that device's current stream; outputs and workspaces come from torch's allocator on that stream.
+#include <ATen/MemoryOverlap.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 
@@ -73,15 +74,23 @@ pk_qk_shape qk_shape(const Tensor& q, const Tensor& k, const Tensor& wq, const T
 void like(const Tensor& y, const Tensor& x, const char* what) {
     if (y.sizes() != x.sizes() || y.scalar_type() != x.scalar_type() || y.device() != x.device()) refuse(QK, std::string("shape mismatch: ") + what);
 }
+void place(const Tensor& y, const Tensor& x) {
+    like(y, x, "out");
+    at::assert_no_internal_overlap(y);
+}
+void changed(const Tensor& t) {  // what was saved of it for a backward pass is no longer what it was
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 std::pair<Tensor, Tensor> qk_fwd(const Tensor& q, const Tensor& k, const Tensor& wq, const Tensor& wk, const Tensor& pos, const QkOptions& o,
                                  const std::vector<Tensor>& out) {
     const pk_qk_shape s = qk_shape(q, k, wq, wk, pos, o);
     c10::DeviceGuard on(q.device());
     at::AutoDispatchBelowAutograd below;
     Tensor yq = out.empty() ? new_tensor(q.sizes(), q.scalar_type(), q) : out[0], yk = out.empty() ? new_tensor(k.sizes(), k.scalar_type(), q) : out[1];
-    like(yq, q, "out"), like(yk, k, "out");
+    place(yq, q), place(yk, k);
     const pk_tensor4 q4 = heads(q, "q"), k4 = heads(k, "k"), yq4 = heads(yq, "out"), yk4 = heads(yk, "out");
     check(pk_qk_norm_rope_fwd(&s, &q4, &k4, wq.const_data_ptr<float>(), wk.const_data_ptr<float>(), pos.const_data_ptr<int>(), &yq4, &yk4, stream()));
+    for (const Tensor& t : out) changed(t);
     return {std::move(yq), std::move(yk)};
 }
 std::vector<Tensor> qk_bwd(Tensor dyq, Tensor dyk, const Tensor& q, const Tensor& k, const Tensor& wq, const Tensor& wk, const Tensor& pos,
@@ -93,13 +102,14 @@ std::vector<Tensor> qk_bwd(Tensor dyq, Tensor dyk, const Tensor& q, const Tensor
     if (dyq.stride(3) != 1) dyq = dyq.contiguous();
     if (dyk.stride(3) != 1) dyk = dyk.contiguous();
     Tensor dq = out.empty() ? new_tensor(q.sizes(), q.scalar_type(), q) : out[0], dk = out.empty() ? new_tensor(k.sizes(), k.scalar_type(), q) : out[1];
-    like(dq, q, "out"), like(dk, k, "out");
+    place(dq, q), place(dk, k);
     Tensor dwq = new_tensor(wq.sizes(), at::kFloat, q), dwk = new_tensor(wk.sizes(), at::kFloat, q);
     const int64_t bytes = static_cast<int64_t>(pk_qk_norm_rope_bwd_workspace_bytes(&s));
     Tensor ws = new_tensor({bytes > 16 ? bytes : 16}, at::kByte, q);
     const pk_tensor4 gq = heads(dyq, "dyq"), gk = heads(dyk, "dyk"), q4 = heads(q, "q"), k4 = heads(k, "k"), dq4 = heads(dq, "out"), dk4 = heads(dk, "out");
     check(pk_qk_norm_rope_bwd(&s, &gq, &gk, &q4, &k4, wq.const_data_ptr<float>(), wk.const_data_ptr<float>(), pos.const_data_ptr<int>(), &dq4, &dk4,
                               dwq.data_ptr<float>(), dwk.data_ptr<float>(), ws.data_ptr(), static_cast<size_t>(ws.numel()), stream()));
+    for (const Tensor& t : out) changed(t);
     return {std::move(dq), std::move(dk), std::move(dwq), std::move(dwk)};
 }
 
@@ -179,6 +189,7 @@ Tensor logprobs_bwd(const Tensor& logits, const Tensor& targets, const Tensor& l
     const Logits g = matrix(LP, "out", d);
     check(pk_token_logprobs_bwd(logits.const_data_ptr(), m.ld, targets.const_data_ptr<int>(), lse.const_data_ptr<float>(), dlogp.const_data_ptr<float>(), m.rows,
                                 m.vocab, static_cast<float>(scale), d.data_ptr(), g.ld, m.dtype, stream()));
+    if (out.defined()) changed(out);
     return d;
 }
 struct TokenLogprobsBackward : public Node {
@@ -230,6 +241,7 @@ std::vector<Tensor> policy(const Tensor& logits, const Tensor& targets, const Te
     check(pk_policy_loss(&c, logits.const_data_ptr(), m.ld, targets.const_data_ptr<int>(), old.const_data_ptr<float>(),
                          ref.defined() ? ref.const_data_ptr<float>() : nullptr, adv.const_data_ptr<float>(), weights.const_data_ptr<float>(), m.rows, m.vocab,
                          d.data_ptr(), g.ld, logp.data_ptr<float>(), rows.data_ptr<double>(), loss.data_ptr<float>(), m.dtype, stream()));
+    if (out.defined()) changed(out);
     return {std::move(loss), std::move(d), std::move(logp)};
 }
 
@@ -250,6 +262,7 @@ std::vector<Tensor> preference(const Tensor& logits, const Tensor& targets, cons
     check(pk_preference_loss(&c, logits.const_data_ptr(), m.ld, targets.const_data_ptr<int>(), starts.const_data_ptr<int>(), pairs, ref.const_data_ptr<float>(),
                              m.rows, m.vocab, d.data_ptr(), g.ld, logp.data_ptr<float>(), margins.data_ptr<float>(), loss.data_ptr<float>(), ws.data_ptr(),
                              static_cast<size_t>(bytes), m.dtype, stream()));
+    if (out.defined()) changed(out);
     return {std::move(loss), std::move(d), std::move(margins), std::move(logp)};
 }
 
@@ -317,9 +330,9 @@ Tensor adamw_many(const Lists& l, pk_adamw_config c) {
     }
     check(pk_adamw_many(table.data(), static_cast<int>(count), &c, ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? static_cast<size_t>(ws.numel()) : 0,
                         norm.defined() ? norm.data_ptr<float>() : nullptr, stream()));
-    for (const auto* list : {&l.p, &l.m, &l.v, &l.ms, &l.vs, &l.copy})  // what was saved of them for a backward pass is no longer what it was
+    for (const auto* list : {&l.p, &l.m, &l.v, &l.ms, &l.vs, &l.copy})
         for (size_t i = 0; i < list->size(); ++i)
-            if (l.g[i] && !(*list)[i]->is_inference()) (*list)[i]->unsafeGetTensorImpl()->bump_version();
+            if (l.g[i]) changed(*(*list)[i]);
     return norm;
 }
 

@@ -117,7 +117,7 @@ def tensor(at, n=100, g=1 << 30, scales=1 << 31, copy=None, m=None, v=None):
 
 
 @pytest.mark.parametrize("change,code", [(dict(t=0), ARGUMENT), (dict(state_bits=16), ARGUMENT), (dict(grad_dtype=2), ARGUMENT), (dict(b1=1.0), ARGUMENT), (dict(b2=-0.1), ARGUMENT),
-                                         (dict(b2=math.nan), ARGUMENT), (dict(max_norm=1.0, norm=None), ARGUMENT), (dict(max_norm=1.0, ws=None), WORKSPACE),
+                                         (dict(b2=math.nan), ARGUMENT), (dict(max_norm=math.nan), ARGUMENT), (dict(max_norm=1.0, norm=None), ARGUMENT), (dict(max_norm=1.0, ws=None), WORKSPACE),
                                          (dict(max_norm=1.0, ws_bytes=263), WORKSPACE)], ids=str)
 def test_adamw_many_refuses(change, code):
     assert adamw([tensor(1 << 20)], **change) == code and _lib.lib().pk_last_error()
@@ -131,6 +131,9 @@ def test_adamw_many_refuses_tables():
     assert adamw([tensor(1 << 20, n=-1)]) == SHAPE and adamw([tensor(1 << 20, n=(1 << 40) + 1)]) == SHAPE
     for twice in (one, tensor((1 << 20) + 4 * 99), tensor(1 << 24, m=(1 << 20) + 4 * 150), tensor(1 << 24, v=1 << 20)):
         assert adamw([one, twice]) == ARGUMENT and b"twice" in _lib.lib().pk_last_error()
+    # scales of two tensors that meet, copies that do
+    assert adamw([one, tensor(1 << 24, scales=(1 << 31) + 4)], state_bits=8) == ARGUMENT
+    assert adamw([tensor(1 << 20, copy=1 << 33), tensor(1 << 24, copy=(1 << 33) + 198)]) == ARGUMENT
     assert adamw([]) == 0 and adamw([_lib.AdamWTensor(0, 0, 0, 0, 0, 0, 0, 0)]) == 0   # nothing to do
     assert _lib.lib().pk_adamw_many(None, 2, None, None, 0, None, None) == ARGUMENT
 
@@ -151,3 +154,37 @@ def test_torch_front_end_refuses_tensors_of_the_cpu():
         blockops.adamw_state([z(3)], 16)
     with pytest.raises(TypeError):
         ops.token_logprobs([1.0], i32(1))
+
+
+@pytest.fixture(scope="module")
+def post_assembly(tmp_path_factory):
+    import os
+    import shutil
+    import subprocess
+
+    from test_asm_hazards import CSRC, FLAGS
+    hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
+    if not os.path.exists(hipcc):
+        pytest.skip("hipcc not found")
+    out = tmp_path_factory.mktemp("post")
+    jobs = {src: str(out / (src + ".s")) for src in ("qk_norm_rope.hip", "token_loss.hip", "adamw_many.hip")}
+    running = [subprocess.Popen([hipcc, *FLAGS, os.path.join(CSRC, src), "-o", to], stdout=subprocess.DEVNULL, stderr=subprocess.DEVNULL) for src, to in jobs.items()]
+    assert [p.wait() for p in running] == [0] * len(running)
+    return jobs
+
+
+def test_kernels_stay_in_registers(post_assembly):
+    """Nothing spilled to memory, and no array kept in LDS by an offset from the launch's packet (which lies in the host's memory: a forward of 10 us took 22)."""
+    import re
+    for src, path in post_assembly.items():
+        text = open(path).read()
+        assert len(re.findall(r"\.amdhsa_kernel ", text)) >= 5, src
+        assert not re.findall(r"amdhsa_user_sgpr_dispatch_ptr 1", text), src
+        assert set(re.findall(r"\.vgpr_spill_count: +(\d+)", text)) == {"0"} and set(re.findall(r"\.private_segment_fixed_size: +(\d+)", text)) == {"0"}, src
+
+
+def test_stores_in_asm_statements_keep_their_data_and_addresses(post_assembly):
+    from test_asm_hazards import scalars_read_early, stores_overwritten
+    path = post_assembly["qk_norm_rope.hip"]
+    assert "global_store_dwordx4" in open(path).read()
+    assert not stores_overwritten(path) and not scalars_read_early(path)

@@ -204,6 +204,19 @@ def test_qk_norm_rope_keeps_a_bad_row_to_itself(pk):
         assert bool(torch.isnan(got[0, 2, 1]).all()) and torch.equal(got[~bad], want[~bad])
 
 
+def test_results_written_over_a_tensor_are_seen_by_autograd(pk):
+    """A tensor that another node saved and a call then writes over: the backward pass says so."""
+    q, k, wq, wk, pos, *_ = qk_inputs(1, 4, 2, 1, 64, FP32, 3, "plain")
+    leaf = q.clone().requires_grad_()
+    y = (leaf * 1.0)
+    z = y * y
+    pk.ops.qk_norm_rope_fwd(y.detach(), k, wq, wk, pos, 1e4, out=(y.detach(), k))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.sum().backward()
+    with pytest.raises(RuntimeError, match="single memory location"):
+        pk.ops.qk_norm_rope_fwd(q, k, wq, wk, pos, 1e4, out=(q[:, :, :1].expand(1, 4, 2, 64), torch.empty_like(k)))
+
+
 def test_qk_norm_rope_under_autograd(pk):
     """The node gives what the direct backward gives, also where only one output is used and where the gradient that arrives is not dense."""
     q, k, wq, wk, pos, dyq, dyk = qk_inputs(2, 19, 4, 2, 64, BF16, 3)
@@ -458,6 +471,18 @@ def test_preference_loss_far_margins_and_lying_offsets(pk):
     wild = torch.tensor([-5, 3, 900], dtype=torch.int32, device="cuda")
     ref = logp - 0.25
     assert all(torch.equal(a, b) for a, b in zip(pk.blockops.preference_loss(x, t, wild, ref), pk.blockops.preference_loss(x, t, starts, ref)))
+
+
+def test_preference_loss_of_an_answer_without_probability(pk):
+    """A forbidden word in one answer: the margin is infinite, the loss 0 or infinite, and the gradient finite wherever the softmax is."""
+    x, t, _ = loss_inputs(6, 200, FP32, 3)
+    starts, ref = torch.tensor([0, 3, 6], dtype=torch.int32, device="cuda"), torch.full((6,), -5.0, device="cuda")
+    for row, margin, loss in ((4, math.inf, 0.0), (1, -math.inf, math.inf)):
+        y = x.clone()
+        y[row, int(t[row])] = -math.inf
+        got, d, margins, logp = pk.blockops.preference_loss(y, t, starts, ref)
+        assert float(margins) == margin and float(got) == loss and float(logp[row]) == -math.inf and bool(torch.isfinite(d).all())
+        assert bool(d.any()) == (margin < 0)
 
 
 # ---- AdamW over many tensors --------------------------------------------------------------------------------------------
