@@ -534,7 +534,7 @@ void flatten(Qk& a, bool backward) {
 }
 int lanes_of(int dk) { return dk <= 32 ? 4 : dk <= 64 ? 8 : dk <= 128 ? 16 : 32; }
 
-// A launch of the row kernels: workgroups over tokens, parts that a token's heads are dealt to.
+// A launch of the row kernels: workgroups over tokens, parts that a token's heads are dealt to, `most` workgroups in all.
 struct Plan {
     int groups, parts, per;
 };
@@ -544,7 +544,7 @@ Plan plan_of(const pk_qk_shape* s, int most) {
     const int rows = 64 / lanes_of(s->dk), steps = (s->Hq + rows - 1) / rows + (s->Hkv + rows - 1) / rows;
     const int64_t tokens = static_cast<int64_t>(s->B) * s->T, want = 4096;
     int parts = 1;
-    while (parts < steps && tokens * parts < want) ++parts;
+    while (parts < steps && parts < most && tokens * parts < want) ++parts;
     Plan p;
     p.per = (steps + parts - 1) / parts;
     p.parts = (steps + p.per - 1) / p.per;

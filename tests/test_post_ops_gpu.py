@@ -95,7 +95,8 @@ QK_CASES = [  # B, T, Hq, Hkv, dk, rotary, halves, layout, pos, far
     (1, 33, 2, 1, 256, 128, True, "fused", "rows", 2 ** 31 - 100), (2, 17, 7, 1, 24, 0, False, "fused", "any", 0), (2, 17, 7, 1, 24, 16, True, "offset", "any", 0),
     (1, 40, 3, 3, 64, 0, False, "offset", "rows", 0), (1, 40, 3, 3, 128, 64, True, "offset", "rows", 0), (2, 11, 2, 5, 70, 0, True, "fused", "rows", 0),
     (2, 11, 2, 5, 254, 2, False, "fused", "rows", 0), (1, 700, 16, 16, 32, 0, False, "fused", "rows", 0), (1, 5, 1, 1, 8, 0, True, "plain", "rows", 0),
-    (1, 5, 2, 1, 40, 8, False, "plain", "rows", 0), (5, 300, 4, 1, 64, 32, True, "fused", "shared", 0)]
+    (1, 5, 2, 1, 40, 8, False, "plain", "rows", 0), (5, 300, 4, 1, 64, 32, True, "fused", "shared", 0),
+    (1, 1, 4500, 3, 128, 0, True, "plain", "rows", 5), (1, 2, 3, 2100, 256, 0, False, "plain", "rows", 5)]
 
 
 @pytest.mark.parametrize("dtype", [FP32, BF16], ids=["fp32", "bf16"])
