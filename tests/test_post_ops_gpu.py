@@ -226,6 +226,9 @@ def test_qk_norm_rope_under_autograd(pk):
     got = torch.autograd.grad([yq, yk], leaves, [dyq, dyk], retain_graph=True)
     want = pk.ops.qk_norm_rope_bwd(dyq, dyk, *(t.detach() for t in leaves), pos, 1e4, 1e-5, 32, True)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+    sideways = dyq.transpose(2, 3).contiguous().transpose(2, 3)   # head_dim not contiguous
+    assert torch.equal(torch.autograd.grad(yq, leaves[0], sideways, retain_graph=True)[0],
+                       pk.ops.qk_norm_rope_bwd(dyq, torch.zeros_like(dyk), *(t.detach() for t in leaves), pos, 1e4, 1e-5, 32, True)[0])
     got = torch.autograd.grad(yq.sum(), leaves[0], retain_graph=True)[0]
     want = pk.ops.qk_norm_rope_bwd(torch.ones_like(dyq), torch.zeros_like(dyk), *(t.detach() for t in leaves), pos, 1e4, 1e-5, 32, True)
     assert torch.equal(got, want[0])
@@ -300,6 +303,10 @@ def test_token_logprobs_against_64_bits(pk, case, dtype):
     over = x.clone()   # over the logits: the same bits where the layout is the same
     same = pk.ops.token_logprobs_bwd(x.clone(), t, lse, dlogp, scale)
     assert pk.ops.token_logprobs_bwd(over, t, lse, dlogp, scale, out=over) is over and torch.equal(over, same)
+    wide = torch.full((rows, vocab + 5), 7.0, dtype=dtype, device="cuda")   # into a wider matrix: its other columns stay
+    pk.ops.token_logprobs_bwd(x, t, lse, dlogp, scale, out=wide[:, 2:2 + vocab])
+    assert bool((wide[:, :2] == 7.0).all()) and bool((wide[:, 2 + vocab:] == 7.0).all())
+    within("dlogits into a view", wide[:, 2:2 + vocab], want, HALF[dtype] * want.abs() + coef.abs() * (slack + 2 * U * sizes(z))[:, None] + 1e-37)
 
 
 def test_token_logprobs_of_rows_that_hold_no_number(pk):
@@ -703,6 +710,69 @@ def test_adamw_many_is_adamw_and_clip(pk):
         # c2 = 1 - b2^t is formed in 32 bits there: 2^-24 / (1 - 0.999^t) of it, half of that of the update
         slack = (16 * U + U / (1 - 0.999 ** t)) * 0.01 * 40
         assert all(float((p - q).abs().max()) <= slack + 4 * U * float(q.abs().max()) for p, q in zip(ps, qs))
+
+
+# ---- past 32 bits ---------------------------------------------------------------------------------------------------------
+
+
+def test_qk_norm_rope_past_2_to_the_31(pk):
+    """Heads whose offsets pass 32 bits, in elements: the last tokens' bits are those of a call on them alone, forward and backward."""
+    T, Hq, Hkv, dk = 35000, 480, 2, 128
+    g = torch.Generator(device="cuda").manual_seed(2)
+    qkv = torch.empty(1, T, Hq + Hkv, dk, dtype=BF16, device="cuda")
+    assert qkv.numel() > 2 ** 31
+    qkv[:, :8].normal_(generator=g)
+    qkv[:, -8:].normal_(generator=g)
+    qkv[:, 8:-8].zero_()
+    q, k = qkv[:, :, :Hq], qkv[:, :, Hq:]
+    w, pos = 1 + 0.2 * torch.randn(dk, generator=g, device="cuda"), torch.arange(T, device="cuda", dtype=torch.int32)
+    yq, yk = pk.ops.qk_norm_rope_fwd(q, k, w, w, pos, 1e4)
+    last = slice(T - 8, T)
+    a, b = pk.ops.qk_norm_rope_fwd(q[:, last], k[:, last], w, w, pos[last], 1e4)
+    assert torch.equal(a, yq[:, last]) and torch.equal(b, yk[:, last]) and not yq[:, 8:64].any()
+    dq, dk_, *_ = pk.ops.qk_norm_rope_bwd(yq, yk, q, k, w, w, pos, 1e4)
+    c, d, *_ = pk.ops.qk_norm_rope_bwd(a, b, q[:, last], k[:, last], w, w, pos[last], 1e4)
+    assert torch.equal(c, dq[:, last]) and torch.equal(d, dk_[:, last])
+
+
+def test_losses_past_2_to_the_31(pk):
+    """Logits whose rows begin past 2^31 elements, in place: the last rows' bits are those of a call on them alone."""
+    rows, vocab, tail = 68000, 32000, 7
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.zeros(rows, vocab, dtype=BF16, device="cuda")
+    x[-tail:].normal_(generator=g)
+    t = torch.randint(0, vocab, (rows,), generator=g, device="cuda").to(torch.int32)
+    t[:-tail] = -1
+    old, adv, w = torch.full((rows,), -11.0, device="cuda"), torch.ones(rows, device="cuda"), torch.ones(rows, device="cuda")
+    last = x[-tail:].clone()
+    cut = lambda *v: tuple(y[-tail:].contiguous() for y in v)  # noqa: E731
+    want = pk.blockops.policy_loss(last, *cut(t, old, adv, w))
+    lp = pk.ops.token_logprobs_fwd(last, *cut(t))
+    logp, lse = pk.ops.token_logprobs_fwd(x, t)
+    assert torch.equal(logp[-tail:], lp[0]) and torch.equal(lse[-tail:], lp[1]) and not logp[:-tail].any()
+    loss, d, logp = pk.blockops.policy_loss(x, t, old, adv, w, out=x)
+    assert torch.equal(d[-tail:], want[1]) and torch.equal(logp[-tail:], want[2]) and torch.equal(loss, want[0]) and not d[:16].any() and not d[-tail - 9:-tail].any()
+    d[-tail:] = last
+    assert torch.equal(pk.ops.token_logprobs_bwd(d, t, lse, w, out=d)[-tail:], pk.ops.token_logprobs_bwd(last, *cut(t, lse, w)))
+
+
+def test_adamw_many_past_2_to_the_31(pk):
+    """One tensor of more than 2^31 elements with 8-bit moments: the last block's values and codes, whose draws come from the element's place."""
+    n, tail = 2 ** 31 + 700, 700
+    p, g = torch.zeros(n, device="cuda"), torch.zeros(n, dtype=BF16, device="cuda")
+    g[-tail:] = torch.randn(tail, generator=torch.Generator(device="cuda").manual_seed(5), device="cuda").to(BF16)
+    state = pk.blockops.adamw_state([p], 8)
+    norm = pk.blockops.adamw_many_([p], [g], state, 0.01, max_norm=1.0, seed=21)
+    gl = g[-tail:].float().cpu()
+    total = math.sqrt(float((gl.double() ** 2).sum()))
+    assert abs(float(norm) - total) <= 2 * U * total
+    z = np.zeros(tail, np.float32)
+    p2, m2, v2, upd = plain_adamw(z, gl.numpy(), z, z, 0.01, 0.9, 0.999, 1e-8, 0.01, 1, np.float32(1.0 / total) if total > 1 else np.float32(1))
+    assert (np.abs(p[-tail:].cpu().numpy() - p2) <= U * np.abs(p2) + 16 * U * 0.01 * np.abs(upd) + 1e-37).all() and not p[:4096].any()
+    h = mix32((np.arange(n - tail, n, dtype=np.uint64) & 0xFFFFFFFF) ^ mix32(21 * 0x9E3779B9 + int(mix32(0x3C6EF373))))
+    for x, chance, got, scales, square in ((m2, h & 0xFFFF, state.m[0], state.m_scale[0], False), (v2, h >> 16, state.v[0], state.v_scale[0], True)):
+        want, ws = pack8(x, chance, square)   # 2^31 is a whole number of blocks: the tail's blocks are the tensor's last three
+        assert np.array_equal(got[-tail:].view(torch.uint8).cpu().numpy(), want) and np.array_equal(scales[-3:].cpu().numpy(), ws)
 
 
 # ---- together, captured, on other streams ---------------------------------------------------------------------------------
