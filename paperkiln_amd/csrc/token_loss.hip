@@ -27,6 +27,8 @@ struct Loss {
     const int* targets;
     int vocab;
     float scale;
+    double s2;                // scale * log2(e), and as a sum of two 32-bit numbers, both of them positive
+    float s2_hi, s2_lo;
     float *logp, *lse;        // written; lse may be null
     double* fine;             // LOGP: the log-probability in 64 bits, or null
     float* clear;             // LOGP: a word per row to set to zero, or null
@@ -39,6 +41,17 @@ struct Loss {
     float clip_low, clip_high, kl, upstream;
 };
 enum Mode { LOGP, GRAD, POLICY };
+
+// 2^(s2 x) against 2^ref, the exponent from both parts of s2: rounded to 32 bits s2 would turn every row's log-probability by up to 6e-8 times its logits, always the same
+// way, and a preference loss adds up hundreds of them (margins 4e-7 off, 1e-7 so). A logit of -inf stays one: the low part is not zero nor negative.
+__device__ inline float power_of(const Loss& a, float x, float ref) { return __builtin_amdgcn_exp2f(fmaf(x, a.s2_lo, fmaf(x, a.s2_hi, -ref))); }
+void set_scale(Loss& a, float scale) {
+    a.scale = scale;
+    a.s2 = static_cast<double>(scale) * 1.4426950408889634074;
+    a.s2_hi = static_cast<float>(a.s2);
+    if (static_cast<double>(a.s2_hi) >= a.s2) a.s2_hi = std::nextafter(a.s2_hi, 0.0f);
+    a.s2_lo = static_cast<float>(a.s2 - static_cast<double>(a.s2_hi));
+}
 
 // A policy row's loss and the derivative of it by the row's log-probability, both before the row's weight.
 __device__ inline void policy_row(const Loss& a, int64_t r, double logp, double& loss, double& slope) {
@@ -114,7 +127,7 @@ __global__ __launch_bounds__(ANY_NT) void rows_any(Loss a) {
     if (MODE == GRAD) {
         const double lse = a.lse_in[r];
         lse2 = static_cast<float>(lse / LN2);
-        target_grad = coef * static_cast<float>(-expm1((static_cast<double>(xt) * s2 - lse / LN2) * LN2));
+        target_grad = coef * static_cast<float>(-expm1((static_cast<double>(xt) * a.s2 - lse / LN2) * LN2));
         if (t >= V) coef = NAN;
     } else {
         float m = -INFINITY, s = 0.0f;
@@ -125,14 +138,13 @@ __global__ __launch_bounds__(ANY_NT) void rows_any(Loss a) {
         m = sh_m[0];
         for (int w = 1; w < ANY_NT / 64; ++w) m = fmaxf(m, sh_m[w]);
         const float m2 = m * s2;
-        for (int j = tid; j < V; j += ANY_NT) s += __builtin_amdgcn_exp2f(fmaf(elem(x, j), s2, -m2));
+        for (int j = tid; j < V; j += ANY_NT) s += power_of(a, elem(x, j), m2);
         s = group_sum<64>(s);
         if ((tid & 63) == 0) sh_s[tid >> 6] = s;
         __syncthreads();
         double sum = 0.0;
         for (int w = 0; w < ANY_NT / 64; ++w) sum += sh_s[w];
-        // the token's logit by the same product as the sum's: what scale * log2(e) was rounded by then drops out where the token is likely
-        const double lse_2 = static_cast<double>(m2) + log2(sum), lse = lse_2 * LN2, logp = (static_cast<double>(xt) * s2 - lse_2) * LN2;
+        const double lse_2 = static_cast<double>(m2) + log2(sum), lse = lse_2 * LN2, logp = (static_cast<double>(xt) * a.s2 - lse_2) * LN2;
         lse2 = static_cast<float>(lse_2);
         if (MODE == POLICY) {
             double loss, slope;
@@ -252,8 +264,8 @@ struct RowOut {
     float lse2, coef, target;  // log2 of the sum, the row's coefficient, the target's gradient
 };
 template <Mode MODE>
-__device__ inline RowOut finish(const Loss& a, int64_t r, float xt, float s2, double lse2) {
-    const double logp = (static_cast<double>(xt) * s2 - lse2) * LN2;
+__device__ inline RowOut finish(const Loss& a, int64_t r, float xt, double lse2) {
+    const double logp = (static_cast<double>(xt) * a.s2 - lse2) * LN2;
     RowOut o{static_cast<float>(lse2), 0.0f, 0.0f};
     if (MODE == POLICY) {
         double loss, slope;
@@ -328,21 +340,21 @@ __global__ __launch_bounds__(ROW_NT) void rows_held(Loss a) {
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
     const float m2 = m == -INFINITY ? 0.0f : m * s2;
-    float s = __builtin_amdgcn_exp2f(fmaf(edge, s2, -m2));
+    float s = power_of(a, edge, m2);
     keep_packed(held);
 #pragma unroll
-    for (int k = 0; k < PER; ++k) held[k].each([&](float v) { s += __builtin_amdgcn_exp2f(fmaf(v, s2, -m2)); });
+    for (int k = 0; k < PER; ++k) held[k].each([&](float v) { s += power_of(a, v, m2); });
     s = group_sum<64>(s);
     RowOut o;
     if constexpr (WAVES == 1) {
         const float ms[1] = {m2}, ss[1] = {s};
         if (MODE == LOGP && tid != 0) return;
-        o = finish<MODE>(a, r, xt, s2, lse2_of<1>(ms, ss));
+        o = finish<MODE>(a, r, xt, lse2_of<1>(ms, ss));
     } else {
         if ((tid & 63) == 0) sh_m[tid >> 6] = s == 0.0f ? -INFINITY : m2, sh_s[tid >> 6] = s;
         __syncthreads();
         if (tid < 64) {
-            o = finish<MODE>(a, r, xt, s2, lse2_of<WAVES>(sh_m, sh_s));
+            o = finish<MODE>(a, r, xt, lse2_of<WAVES>(sh_m, sh_s));
             if (tid == 0) sh_o = o;
         }
         if constexpr (MODE == LOGP) return;
@@ -382,7 +394,7 @@ __global__ __launch_bounds__(LONG_NT) void rows_long(Loss a) {
     }
     const float s2 = a.scale * LOG2E;
     const float edge = tid < cut.edges ? elem(x, cut.edge(tid)) : -INFINITY, xt = t < V ? elem(x, t) : NAN;
-    float m2 = edge == -INFINITY ? -INFINITY : edge * s2, s = edge == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(fmaf(edge, s2, -m2));
+    float m2 = edge == -INFINITY ? -INFINITY : edge * s2, s = edge == -INFINITY ? 0.0f : power_of(a, edge, m2);
     for (int p0 = tid; p0 < cut.pieces; p0 += LONG_U * LONG_NT) {
         Piece<T> v[LONG_U];
 #pragma unroll
@@ -396,7 +408,7 @@ __global__ __launch_bounds__(LONG_NT) void rows_long(Loss a) {
         const float new2 = fmaxf(m2, top * s2), ref = new2 == -INFINITY ? 0.0f : new2;
         s = s == 0.0f ? 0.0f : s * __builtin_amdgcn_exp2f(m2 - ref);
 #pragma unroll
-        for (int u = 0; u < LONG_U; ++u) v[u].each([&](float y) { s += __builtin_amdgcn_exp2f(fmaf(y, s2, -ref)); });
+        for (int u = 0; u < LONG_U; ++u) v[u].each([&](float y) { s += power_of(a, y, ref); });
         m2 = new2;
     }
     // lanes, then wavefronts
@@ -408,7 +420,7 @@ __global__ __launch_bounds__(LONG_NT) void rows_long(Loss a) {
     __syncthreads();
     RowOut o;
     if (tid < 64) {
-        o = finish<MODE>(a, r, xt, s2, lse2_of<WAVES>(sh_m, sh_s));
+        o = finish<MODE>(a, r, xt, lse2_of<WAVES>(sh_m, sh_s));
         if (tid == 0) sh_o = o;
     }
     if constexpr (MODE != LOGP) {
@@ -470,7 +482,7 @@ __global__ __launch_bounds__(GRAD_NT) void rows_grad(Loss a, int per) {
             if (p < to) store_piece<PAST>(dx + j0, gradient(v[u], s2, lse2, coef));
         }
     }
-    if (holds) put(dx, t, coef * -expm1f(static_cast<float>((static_cast<double>(xt) * s2 - exact) * LN2)));
+    if (holds) put(dx, t, coef * -expm1f(static_cast<float>((static_cast<double>(xt) * a.s2 - exact) * LN2)));
 }
 
 __global__ __launch_bounds__(1024) void loss_sum(const double* x, int64_t n, float* out) {
@@ -614,7 +626,8 @@ int pk_token_logprobs_fwd(const void* logits, int64_t ld, const int* targets, in
         if (rows > 0 && !logp) return fail(PK_ERR_ARGUMENT, "pk_token_logprobs_fwd: null pointer");
         touch({logits, targets, logp, lse}, stream);
         Loss a{};
-        a.logits = logits, a.ld = ld, a.targets = targets, a.rows = rows, a.vocab = static_cast<int>(vocab), a.scale = scale, a.logp = logp, a.lse = lse;
+        a.logits = logits, a.ld = ld, a.targets = targets, a.rows = rows, a.vocab = static_cast<int>(vocab), a.logp = logp, a.lse = lse;
+        set_scale(a, scale);
         return launch_rows<LOGP>(a, dtype, static_cast<hipStream_t>(stream));
     });
 }
@@ -626,7 +639,8 @@ int pk_token_logprobs_bwd(const void* logits, int64_t ld, const int* targets, co
         if (rows > 0 && (!lse || !dlogp)) return fail(PK_ERR_ARGUMENT, "pk_token_logprobs_bwd: null pointer");
         touch({logits, targets, lse, dlogp, dlogits}, stream);
         Loss a{};
-        a.logits = logits, a.ld = ld, a.targets = targets, a.rows = rows, a.vocab = static_cast<int>(vocab), a.scale = scale;
+        a.logits = logits, a.ld = ld, a.targets = targets, a.rows = rows, a.vocab = static_cast<int>(vocab);
+        set_scale(a, scale);
         a.dlogits = dlogits, a.dld = dld, a.lse_in = lse, a.coef = dlogp;
         return launch_rows<GRAD>(a, dtype, static_cast<hipStream_t>(stream));
     });
@@ -645,7 +659,8 @@ int pk_policy_loss(const pk_policy_config* c, const void* logits, int64_t ld, co
         touch({logits, targets, old_logp, ref_logp, advantages, weights, dlogits, logp, row_loss, loss}, stream);
         hipStream_t st = static_cast<hipStream_t>(stream);
         Loss a{};
-        a.logits = logits, a.ld = ld, a.targets = targets, a.rows = rows, a.vocab = static_cast<int>(vocab), a.scale = c->scale;
+        a.logits = logits, a.ld = ld, a.targets = targets, a.rows = rows, a.vocab = static_cast<int>(vocab);
+        set_scale(a, c->scale);
         a.dlogits = dlogits, a.dld = dld, a.logp = logp, a.row_loss = row_loss;
         a.old_logp = old_logp, a.ref_logp = c->kl_coef != 0.0f ? ref_logp : nullptr, a.adv = advantages, a.weights = weights;
         a.clip_low = c->clip_low, a.clip_high = c->clip_high, a.kl = c->kl_coef, a.upstream = c->upstream;
@@ -680,7 +695,8 @@ int pk_preference_loss(const pk_preference_config* c, const void* logits, int64_
         float *lse = reinterpret_cast<float*>(ws), *coef = reinterpret_cast<float*>(ws + singles);
         double *fine = reinterpret_cast<double*>(ws + 2 * singles), *losses = reinterpret_cast<double*>(ws + 2 * singles + doubles);
         Loss a{};
-        a.logits = logits, a.ld = ld, a.targets = targets, a.rows = rows, a.vocab = static_cast<int>(vocab), a.scale = c->scale;
+        a.logits = logits, a.ld = ld, a.targets = targets, a.rows = rows, a.vocab = static_cast<int>(vocab);
+        set_scale(a, c->scale);
         a.logp = logp, a.lse = lse, a.fine = fine, a.clear = coef;
         if (int rc = launch_rows<LOGP>(a, dtype, st)) return rc;
         pair_loss<<<dim3(static_cast<unsigned>(pairs)), PAIR_NT, 0, st>>>(
