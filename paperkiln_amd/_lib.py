@@ -76,7 +76,8 @@ EXPORTS = ["pk_last_error", "pk_init", "pk_attn_fwd", "pk_attn_bwd_workspace_byt
            "pk_op_add", "pk_op_mul", "pk_op_scale", "pk_op_axpy", "pk_op_fill", "pk_op_silu_fwd", "pk_op_silu_bwd", "pk_op_silu_mul_fwd", "pk_op_silu_mul_bwd",
            "pk_op_rmsnorm_fwd", "pk_op_rmsnorm_bwd", "pk_op_rope", "pk_op_embedding_fwd", "pk_op_embedding_bwd",
            "pk_op_cross_entropy", "pk_op_adamw", "pk_op_sumsq", "pk_op_gemm", "pk_set_gemm_backend", "pk_set_head_kernel",
-           "pk_qk_norm_rope_fwd", "pk_qk_norm_rope_bwd_workspace_bytes", "pk_qk_norm_rope_bwd", "pk_token_logprobs_fwd", "pk_token_logprobs_bwd",
+           "pk_qk_norm_rope_fwd", "pk_qk_norm_rope_bwd_workspace_bytes", "pk_qk_norm_rope_bwd", "pk_token_logprobs_workspace_bytes", "pk_token_logprobs_fwd",
+           "pk_token_logprobs_bwd",
            "pk_policy_loss", "pk_preference_loss_workspace_bytes", "pk_preference_loss", "pk_adamw_many_workspace_bytes", "pk_adamw_many"]
 
 
@@ -145,14 +146,15 @@ def lib() -> C.CDLL:
         L.pk_qk_norm_rope_fwd.argtypes = [QS, T4, T4, vp, vp, vp, T4, T4, vp]
         L.pk_qk_norm_rope_bwd_workspace_bytes.argtypes = [QS]
         L.pk_qk_norm_rope_bwd.argtypes = [QS, T4, T4, T4, T4, vp, vp, vp, T4, T4, vp, vp, vp, sz, vp]
-        L.pk_token_logprobs_fwd.argtypes = [vp, i64, vp, i64, i64, cf, vp, vp, ci, vp]
+        L.pk_token_logprobs_workspace_bytes.argtypes = [i64, i64, ci]
+        L.pk_token_logprobs_fwd.argtypes = [vp, i64, vp, i64, i64, cf, vp, vp, vp, sz, ci, vp]
         L.pk_token_logprobs_bwd.argtypes = [vp, i64, vp, vp, vp, i64, i64, cf, vp, i64, ci, vp]
         L.pk_policy_loss.argtypes = [C.POINTER(PolicyConfig), vp, i64, vp, vp, vp, vp, vp, i64, i64, vp, i64, vp, vp, vp, ci, vp]
         L.pk_preference_loss_workspace_bytes.argtypes = [i64, i64]
         L.pk_preference_loss.argtypes = [C.POINTER(PreferenceConfig), vp, i64, vp, vp, i64, vp, i64, i64, vp, i64, vp, vp, vp, vp, sz, ci, vp]
         L.pk_adamw_many_workspace_bytes.argtypes = [AT, ci, AC]
         L.pk_adamw_many.argtypes = [AT, ci, AC, vp, sz, vp, vp]
-        for fn in (L.pk_qk_norm_rope_bwd_workspace_bytes, L.pk_preference_loss_workspace_bytes, L.pk_adamw_many_workspace_bytes):
+        for fn in (L.pk_qk_norm_rope_bwd_workspace_bytes, L.pk_token_logprobs_workspace_bytes, L.pk_preference_loss_workspace_bytes, L.pk_adamw_many_workspace_bytes):
             fn.restype = sz
         _lib = L
     return _lib

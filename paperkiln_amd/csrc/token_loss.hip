@@ -36,6 +36,7 @@ struct Loss {
     const double* losses;     // GRAD: the pairs' losses, whose mean the workgroup behind the last row's writes to `loss`
     int64_t pairs;
     float* loss;
+    float2* parts;            // LOGP: room for the parts of rows that are dealt out, or null
     const float *old_logp, *ref_logp, *adv, *weights;  // POLICY; ref_logp may be null
     double* row_loss;
     float clip_low, clip_high, kl, upstream;
@@ -374,33 +375,21 @@ __global__ __launch_bounds__(ROW_NT) void rows_held(Loss a) {
     }
 }
 
-// Rows that no workgroup holds: read in strides with a running maximum and sum, and again for the gradient.
-constexpr int LONG_NT = 1024, LONG_U = 4;
-template <typename T, Mode MODE, bool PAST>
-__global__ __launch_bounds__(LONG_NT) void rows_long(Loss a) {
-    constexpr int WAVES = LONG_NT / 64, N = Piece<T>::N;
-    __shared__ float sh_m[WAVES], sh_s[WAVES];
-    __shared__ RowOut sh_o;
-    const int64_t r = blockIdx.x;
-    const int tid = threadIdx.x, V = a.vocab, t = a.targets[r];
-    const T* x = static_cast<const T*>(a.logits) + r * a.ld;
-    T* dx = MODE == LOGP ? nullptr : static_cast<T*>(a.dlogits) + r * a.dld;
-    const Cut<T> cut(x, V);
-    if (MODE == LOGP && a.clear && tid == 0) a.clear[r] = 0.0f;
-    if (t < 0 || (MODE == POLICY && a.weights[r] == 0.0f)) {
-        if (tid == 0) no_row<MODE>(a, r);
-        if (MODE != LOGP) zero_row<T, LONG_NT, PAST>(dx, cut, tid);
-        return;
-    }
+// Rows that no workgroup holds are read in strides, with a running maximum and sum, and again for the gradient.
+constexpr int LONG_U = 4;
+template <typename T, int NT, bool EDGES>
+__device__ inline void running(const Loss& a, const T* x, const Cut<T>& cut, int from, int to, float edge, float* sh_m, float* sh_s) {
+    constexpr int N = Piece<T>::N;
+    const int tid = threadIdx.x;
     const float s2 = a.scale * LOG2E;
-    const float edge = tid < cut.edges ? elem(x, cut.edge(tid)) : -INFINITY, xt = t < V ? elem(x, t) : NAN;
-    float m2 = edge == -INFINITY ? -INFINITY : edge * s2, s = edge == -INFINITY ? 0.0f : power_of(a, edge, m2);
-    for (int p0 = tid; p0 < cut.pieces; p0 += LONG_U * LONG_NT) {
+    float m2 = -INFINITY, s = 0.0f;
+    if (EDGES && edge != -INFINITY) m2 = edge * s2, s = power_of(a, edge, m2);
+    for (int p0 = from + tid; p0 < to; p0 += LONG_U * NT) {
         Piece<T> v[LONG_U];
 #pragma unroll
         for (int u = 0; u < LONG_U; ++u) {
-            const int p = p0 + u * LONG_NT;
-            v[u] = p < cut.pieces ? *reinterpret_cast<const Piece<T>*>(x + cut.head + p * N) : Piece<T>::nothing();
+            const int p = p0 + u * NT;
+            v[u] = p < to ? load_piece<false>(x + cut.head + p * N) : Piece<T>::nothing();
         }
         float top = -INFINITY;
 #pragma unroll
@@ -418,6 +407,27 @@ __global__ __launch_bounds__(LONG_NT) void rows_long(Loss a) {
     s = group_sum<64>(s == 0.0f ? 0.0f : s * __builtin_amdgcn_exp2f(m2 - top));
     if ((tid & 63) == 0) sh_m[tid >> 6] = s == 0.0f ? -INFINITY : top, sh_s[tid >> 6] = s;
     __syncthreads();
+}
+
+constexpr int LONG_NT = 1024;
+template <typename T, Mode MODE, bool PAST>
+__global__ __launch_bounds__(LONG_NT) void rows_long(Loss a) {
+    constexpr int WAVES = LONG_NT / 64, N = Piece<T>::N;
+    __shared__ float sh_m[WAVES], sh_s[WAVES];
+    __shared__ RowOut sh_o;
+    const int64_t r = blockIdx.x;
+    const int tid = threadIdx.x, V = a.vocab, t = a.targets[r];
+    const T* x = static_cast<const T*>(a.logits) + r * a.ld;
+    T* dx = MODE == LOGP ? nullptr : static_cast<T*>(a.dlogits) + r * a.dld;
+    const Cut<T> cut(x, V);
+    if (MODE == LOGP && a.clear && tid == 0) a.clear[r] = 0.0f;
+    if (t < 0 || (MODE == POLICY && a.weights[r] == 0.0f)) {
+        if (tid == 0) no_row<MODE>(a, r);
+        if (MODE != LOGP) zero_row<T, LONG_NT, PAST>(dx, cut, tid);
+        return;
+    }
+    const float edge = tid < cut.edges ? elem(x, cut.edge(tid)) : -INFINITY, xt = t < V ? elem(x, t) : NAN;
+    running<T, LONG_NT, true>(a, x, cut, 0, cut.pieces, edge, sh_m, sh_s);
     RowOut o;
     if (tid < 64) {
         o = finish<MODE>(a, r, xt, lse2_of<WAVES>(sh_m, sh_s));
@@ -427,6 +437,7 @@ __global__ __launch_bounds__(LONG_NT) void rows_long(Loss a) {
         __syncthreads();
         o = sh_o;
         if (o.coef == 0.0f) return zero_row<T, LONG_NT, PAST>(dx, cut, tid);
+        const float s2 = a.scale * LOG2E;
         for (int p = tid; p < cut.pieces; p += LONG_NT) {
             const int j0 = cut.head + p * N;
             store_piece<PAST>(dx + j0, gradient(load_piece<PAST>(x + j0), s2, o.lse2, o.coef));
@@ -434,6 +445,48 @@ __global__ __launch_bounds__(LONG_NT) void rows_long(Loss a) {
         if (tid < cut.edges) put(dx, cut.edge(tid), -o.coef * __builtin_amdgcn_exp2f(fmaf(edge, s2, -o.lse2)));
         if (tid == cut.holder(t, LONG_NT)) put(dx, t, o.target);
     }
+}
+
+// A few such rows are dealt to several workgroups, `per` pieces each, which leave the largest exponent and the sum of their part; a wavefront joins a row's.
+constexpr int PART_NT = 512, MOST_PARTS = 32, FEW_ROWS = 128;
+template <typename T>
+__global__ __launch_bounds__(PART_NT) void rows_part(Loss a, int per, float2* parts) {
+    constexpr int WAVES = PART_NT / 64;
+    __shared__ float sh_m[WAVES], sh_s[WAVES];
+    const int64_t r = blockIdx.x;
+    const int tid = threadIdx.x;
+    if (a.targets[r] < 0) return;
+    const T* x = static_cast<const T*>(a.logits) + r * a.ld;
+    const Cut<T> cut(x, a.vocab);
+    const int from = static_cast<int>(blockIdx.y) * per, to = min(cut.pieces, from + per);
+    const float edge = blockIdx.y == 0 && tid < cut.edges ? elem(x, cut.edge(tid)) : -INFINITY;
+    running<T, PART_NT, true>(a, x, cut, from, to, edge, sh_m, sh_s);
+    if (tid != 0) return;
+    float top = sh_m[0], s = 0.0f;
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) top = fmaxf(top, sh_m[w]);
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) s += sh_s[w] == 0.0f ? 0.0f : sh_s[w] * __builtin_amdgcn_exp2f(sh_m[w] - top);
+    parts[r * gridDim.y + blockIdx.y] = make_float2(top, s);
+}
+template <typename T>
+__global__ __launch_bounds__(64) void rows_join(Loss a, int count, const float2* parts) {
+    const int64_t r = blockIdx.x;
+    const int lane = threadIdx.x, t = a.targets[r];
+    if (a.clear && lane == 0) a.clear[r] = 0.0f;
+    if (t < 0) {
+        if (lane == 0) no_row<LOGP>(a, r);
+        return;
+    }
+    const float2 v = lane < count ? parts[r * count + lane] : make_float2(-INFINITY, 0.0f);
+    float top = v.x;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    double sum = v.y == 0.0f ? 0.0 : static_cast<double>(v.y * __builtin_amdgcn_exp2f(v.x - top));
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
+    const T* x = static_cast<const T*>(a.logits) + r * a.ld;
+    if (lane == 0) finish<LOGP>(a, r, t < a.vocab ? elem(x, t) : NAN, sum == 0.0 ? static_cast<double>(NAN) : top + log2(sum));
 }
 
 // The gradient of rows whose sums are known: every element by itself, so a row may be dealt to several workgroups (grid.y, `per` pieces each) and written over.
@@ -547,6 +600,7 @@ constexpr int64_t PAST_BYTES = int64_t{96} << 20;
 bool same_cut(const Loss& a, int64_t es) {
     return (reinterpret_cast<uintptr_t>(a.logits) - reinterpret_cast<uintptr_t>(a.dlogits)) % 16 == 0 && (a.ld - a.dld) * es % 16 == 0;
 }
+constexpr int HELD_PIECES = 8192;
 // Threads and pieces for a row. Policy loss over 262 to 131 MB of bf16 logits, the neighbours in brackets: 1000 words 73 us (a wavefront for two pieces; 90 on two wavefronts),
 // 2000 words 106 (118 on 128 threads), 4000 words 100 (104 on 256, 106 on 64), 8000 words 91.5 (95 on 128, 100 on 512), 16000 words 90 (96 on 256), 32000 words 94 (94 on 1024), 64000
 // words 98.8 (97.7 read twice), 128000 words 101 (101 held by 1024 threads, 16 pieces each, whose log-probabilities took 54.4 instead of 46.7).
@@ -561,15 +615,27 @@ void launch_held(const Loss& a, hipStream_t st) {
     if (pieces <= 1024) return rows_held<T, MODE, 256, 4, PAST><<<grid, 256, 0, st>>>(a);
     if (pieces <= 2048) return rows_held<T, MODE, 512, 4, PAST><<<grid, 512, 0, st>>>(a);
     if (pieces <= 4096) return rows_held<T, MODE, 512, 8, PAST><<<grid, 512, 0, st>>>(a);
-    if (pieces <= 8192) return rows_held<T, MODE, 1024, 8, PAST><<<grid, 1024, 0, st>>>(a);
+    if (pieces <= HELD_PIECES) return rows_held<T, MODE, 1024, 8, PAST><<<grid, 1024, 0, st>>>(a);
     rows_long<T, MODE, PAST><<<grid, LONG_NT, 0, st>>>(a);
+}
+// Workgroups that a row is dealt to for its log-probability: one, but for a few rows that none holds. bf16, whole and dealt out: one row of 128000 words 8.7 and 5.6 us, 64 of
+// them 9.5 and 6.9, one of 200000 12.6 and 5.7, 64 13.6 and 8.8; a held row of 32000 words takes 4.1, less than the two launches.
+int parts_of_rows(int64_t rows, int64_t vocab, int64_t es) {
+    const int64_t pieces = vocab * es / 16;
+    if (rows < 1 || rows >= FEW_ROWS || pieces <= HELD_PIECES) return 1;
+    return static_cast<int>(std::min<int64_t>(std::min<int64_t>(MOST_PARTS, 512 / rows), pieces / (2 * PART_NT)));
 }
 template <typename T, Mode MODE>
 void launch_typed(const Loss& a, hipStream_t st) {
     const bool past = a.rows * a.vocab * static_cast<int64_t>(sizeof(T)) >= PAST_BYTES;
     const dim3 grid(static_cast<unsigned>(a.rows + (a.loss ? 1 : 0)));
-    if constexpr (MODE == LOGP) return launch_held<T, MODE, false>(a, st);  // the logits are read again for their gradient
-    else {
+    if constexpr (MODE == LOGP) {
+        const int parts = a.parts ? parts_of_rows(a.rows, a.vocab, sizeof(T)) : 1;
+        if (parts == 1) return launch_held<T, MODE, false>(a, st);  // the logits are read again for their gradient: not past the cache
+        const int pieces = a.vocab / Piece<T>::N, per = (pieces + parts - 1) / parts;
+        rows_part<T><<<dim3(static_cast<unsigned>(a.rows), static_cast<unsigned>(parts)), PART_NT, 0, st>>>(a, per, a.parts);
+        rows_join<T><<<dim3(static_cast<unsigned>(a.rows)), 64, 0, st>>>(a, parts, a.parts);
+    } else {
         if (!same_cut(a, sizeof(T))) return rows_any<T, MODE><<<grid, ANY_NT, 0, st>>>(a);
         if constexpr (MODE == GRAD) {
             // Few rows are dealt out, one load to a thread, as far as that fills the chip: one row of 128000 words bf16 9.4 -> 3.0 us
@@ -621,13 +687,22 @@ using namespace pk;
 
 extern "C" {
 
+size_t pk_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int dtype) {
+    if (rows < 0 || vocab <= 0 || !known_dtype(dtype)) return 0;
+    const int parts = parts_of_rows(rows, vocab, elem_size(dtype));
+    return parts == 1 ? 0 : sizeof(float2) * static_cast<size_t>(rows * parts);
+}
+
 int pk_token_logprobs_fwd(const void* logits, int64_t ld, const int* targets, int64_t rows, int64_t vocab, float scale, float* logp, float* lse,
-                          int dtype, void* stream) {
+                          void* workspace, size_t workspace_bytes, int dtype, void* stream) {
     return c_entry([&] {
         if (int rc = check("pk_token_logprobs_fwd", logits, ld, targets, rows, vocab, scale, dtype, false, nullptr, 0)) return rc;
         if (rows > 0 && !logp) return fail(PK_ERR_ARGUMENT, "pk_token_logprobs_fwd: null pointer");
-        touch({logits, targets, logp, lse}, stream);
+        if (workspace && (workspace_bytes < pk_token_logprobs_workspace_bytes(rows, vocab, dtype) || !aligned(workspace, 8)))
+            return fail(PK_ERR_WORKSPACE, "pk_token_logprobs_fwd: workspace too small (pk_token_logprobs_workspace_bytes)");
+        touch({logits, targets, logp, lse, workspace}, stream);
         Loss a{};
+        a.parts = static_cast<float2*>(workspace);
         a.logits = logits, a.ld = ld, a.targets = targets, a.rows = rows, a.vocab = static_cast<int>(vocab), a.logp = logp, a.lse = lse;
         set_scale(a, scale);
         return launch_rows<LOGP>(a, dtype, static_cast<hipStream_t>(stream));
@@ -674,7 +749,8 @@ int pk_policy_loss(const pk_policy_config* c, const void* logits, int64_t ld, co
 
 size_t pk_preference_loss_workspace_bytes(int64_t rows, int64_t pairs) {
     if (rows < 0 || pairs < 0) return 0;
-    return 2 * pad(sizeof(float) * static_cast<size_t>(rows)) + pad(sizeof(double) * static_cast<size_t>(rows)) + pad(sizeof(double) * static_cast<size_t>(pairs));
+    return 2 * pad(sizeof(float) * static_cast<size_t>(rows)) + pad(sizeof(double) * static_cast<size_t>(rows)) + pad(sizeof(double) * static_cast<size_t>(pairs)) +
+           (rows < FEW_ROWS ? pad(sizeof(float2) * static_cast<size_t>(rows) * MOST_PARTS) : 0);
 }
 
 int pk_preference_loss(const pk_preference_config* c, const void* logits, int64_t ld, const int* targets, const int* seq_start, int64_t pairs,
@@ -700,6 +776,7 @@ int pk_preference_loss(const pk_preference_config* c, const void* logits, int64_
         a.logits = logits, a.ld = ld, a.targets = targets, a.rows = rows, a.vocab = static_cast<int>(vocab);
         set_scale(a, c->scale);
         a.logp = logp, a.lse = lse, a.fine = fine, a.clear = coef;
+        if (rows < FEW_ROWS) a.parts = reinterpret_cast<float2*>(ws + 2 * singles + doubles + pad(sizeof(double) * static_cast<size_t>(pairs)));
         if (int rc = launch_rows<LOGP>(a, dtype, st)) return rc;
         pair_loss<<<dim3(static_cast<unsigned>(pairs)), PAIR_NT, 0, st>>>(
             Pairs{seq_start, targets, fine, ref_logp, coef, margins, losses, rows, static_cast<int>(pairs), c->beta, c->label_smoothing, c->upstream});

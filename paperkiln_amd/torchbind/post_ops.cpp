@@ -174,8 +174,11 @@ std::pair<Tensor, Tensor> logprobs_fwd(const Tensor& logits, const Tensor& targe
     c10::DeviceGuard on(logits.device());
     at::AutoDispatchBelowAutograd below;
     Tensor logp = new_tensor({m.rows}, at::kFloat, logits), lse = new_tensor({m.rows}, at::kFloat, logits);
+    Tensor ws;
+    const size_t bytes = pk_token_logprobs_workspace_bytes(m.rows, m.vocab, m.dtype);
+    if (bytes) ws = new_tensor({static_cast<int64_t>(bytes)}, at::kByte, logits);
     check(pk_token_logprobs_fwd(logits.const_data_ptr(), m.ld, targets.const_data_ptr<int>(), m.rows, m.vocab, static_cast<float>(scale), logp.data_ptr<float>(),
-                                lse.data_ptr<float>(), m.dtype, stream()));
+                                lse.data_ptr<float>(), bytes ? ws.data_ptr() : nullptr, bytes, m.dtype, stream()));
     return {std::move(logp), std::move(lse)};
 }
 Tensor logprobs_bwd(const Tensor& logits, const Tensor& targets, const Tensor& lse, const Tensor& dlogp, double scale, const Tensor& out) {

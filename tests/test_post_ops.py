@@ -99,9 +99,14 @@ def test_token_logprobs_refuses():
     L = _lib.lib()
     for change, code in (((None, 100, SOME, 4, 100, 1.0, SOME), ARGUMENT), ((SOME, 100, None, 4, 100, 1.0, SOME), ARGUMENT), ((SOME, 100, SOME, 4, 100, 1.0, None), ARGUMENT),
                          ((SOME, 100, SOME, 4, 0, 1.0, SOME), SHAPE), ((SOME, 100, SOME, 4, 100, math.nan, SOME), ARGUMENT)):
-        assert L.pk_token_logprobs_fwd(*change, None, _lib.PK_F32, None) == code
-    assert L.pk_token_logprobs_fwd(None, 100, None, 0, 100, 1.0, None, None, _lib.PK_F32, None) == 0   # nothing to do
-    assert L.pk_preference_loss_workspace_bytes(100, 3) == 512 + 512 + 1024 + 256
+        assert L.pk_token_logprobs_fwd(*change, None, None, 0, _lib.PK_F32, None) == code
+    assert L.pk_token_logprobs_fwd(None, 100, None, 0, 100, 1.0, None, None, None, 0, _lib.PK_F32, None) == 0   # nothing to do
+    need = L.pk_token_logprobs_workspace_bytes(3, 200000, _lib.PK_F32)   # a few rows that no workgroup holds: 32 parts of 8 bytes each
+    assert need == 3 * 32 * 8 and L.pk_token_logprobs_workspace_bytes(3, 32000, _lib.PK_F32) == 0 and L.pk_token_logprobs_workspace_bytes(128, 200000, _lib.PK_F32) == 0
+    for ws, size in ((SOME, need - 1), (C.c_void_p((1 << 20) + 4), need)):
+        assert L.pk_token_logprobs_fwd(SOME, 200000, SOME, 3, 200000, 1.0, SOME, None, ws, size, _lib.PK_F32, None) == WORKSPACE
+    assert L.pk_preference_loss_workspace_bytes(1000, 3) == 4096 + 4096 + 8192 + 256
+    assert L.pk_preference_loss_workspace_bytes(100, 3) == 512 + 512 + 1024 + 256 + 100 * 32 * 8
 
 
 def adamw(tensors, ws=SOME, ws_bytes=1 << 20, norm=SOME, **kw):

@@ -272,7 +272,8 @@ def logp_slack(z, vocab):
 ROWS = [  # rows, vocab, pitch, offset, forbidden
     (1, 1, 0, 0, 0), (3, 2, 0, 0, 0), (5, 7, 0, 0, 3), (4, 64, 0, 0, 0), (9, 511, 0, 0, 5), (3, 1000, 1008, 0, 0), (2, 2048, 0, 0, 0), (3, 4097, 0, 0, 0),
     (2, 10007, 0, 0, 7), (3, 10007, 10016, 1, 0), (2, 16384, 0, 0, 0), (3, 32000, 0, 0, 0), (2, 32003, 0, 3, 2), (2, 65537, 0, 0, 0), (2, 131072, 0, 0, 0),
-    (1, 200001, 0, 0, 0), (300, 33, 0, 0, 0), (1, 32000, 32064, 8, 0)]
+    (1, 200001, 0, 0, 0), (300, 33, 0, 0, 0), (1, 32000, 32064, 8, 0),
+    (5, 70001, 70016, 3, 9), (130, 66000, 0, 0, 0), (2, 40001, 0, 0, 5)]
 
 
 @pytest.mark.parametrize("dtype", [FP32, BF16], ids=["fp32", "bf16"])
@@ -327,6 +328,30 @@ def test_token_logprobs_of_rows_that_hold_no_number(pk):
         assert bool(torch.isfinite(d[3]).all()) and float(d[3, 40]) == 1.0 and bool(torch.isfinite(d[6]).all())
         want, _ = pk.ops.token_logprobs_fwd(fine, t)
         assert torch.equal(logp[6:], want[6:])
+
+
+def test_token_logprobs_dealt_out_and_whole(pk):
+    """A few rows past what a workgroup holds: dealt to several with a workspace, whole without one, each within the count of the other test; rows that hold no number,
+    are not read or have one word only, among them."""
+    import ctypes as C
+    L = pk.lib.lib()
+    for dtype, code in ((FP32, pk.lib.PK_F32), (BF16, pk.lib.PK_BF16)):
+        x, t, _ = loss_inputs(7, 150001, dtype, 9)
+        x[0] = -math.inf
+        x[1], x[1, 77000] = -math.inf, 2.0
+        x[2, 149999], t[3], t[4], t[1], t[0] = math.nan, -1, 150001, 77000, 5
+        z, wl, wp, _ = softmax64(x, t, 1.0)
+        wl[3], wp[3], wp[4] = 0.0, 0.0, math.nan
+        slack = logp_slack(z, 150001)
+        need = L.pk_token_logprobs_workspace_bytes(7, 150001, code)
+        assert need > 0
+        for ws in (torch.full((need,), 255, dtype=torch.uint8, device="cuda"), None):   # a workspace holds anything before
+            logp, lse = torch.full((7,), 3.0, device="cuda"), torch.full((7,), 3.0, device="cuda")
+            p = lambda y: C.c_void_p(y.data_ptr() if y is not None else None)  # noqa: E731
+            pk.lib.check(L.pk_token_logprobs_fwd(p(x), x.stride(0), p(t), 7, 150001, 1.0, p(logp), p(lse), p(ws), need if ws is not None else 0, code,
+                                                 C.c_void_p(torch.cuda.current_stream().cuda_stream)))
+            within("lse", lse, wl, U * wl.abs().nan_to_num() + slack)
+            within("logp", logp, wp, U * wp.abs().nan_to_num() + slack)
 
 
 def test_token_logprobs_under_autograd_and_empty(pk):
