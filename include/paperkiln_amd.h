@@ -315,8 +315,8 @@ int pk_qk_norm_rope_bwd(const pk_qk_shape* s, const pk_tensor4* dyq, const pk_te
                         const pk_tensor4* k, const float* wq, const float* wk, const int* pos, const pk_tensor4* dq,
                         const pk_tensor4* dk, float* dwq, float* dwk, void* workspace, size_t workspace_bytes, void* stream);
 
-/* Log-probabilities of chosen tokens: logits [rows, vocab] with ld elements between rows, z = scale * logits,
- * logp[r] = z[r, targets[r]] - lse[r]. A row whose target is negative is not read: logp and lse 0. A target past the
+/* Log-probabilities of chosen tokens: logits [rows, vocab] with ld elements between rows, z = scale * logits (scale
+ * between 2^-64 and 2^64), logp[r] = z[r, targets[r]] - lse[r]. A row whose target is negative is not read: logp and lse 0. A target past the
  * vocabulary gives NaN. Logits of -inf are words without probability; a row of nothing else gives NaN. lse may be NULL.
  * With a workspace (its bytes may be 0) a few rows of large vocabularies are dealt to several workgroups each; without
  * one (NULL) every row stays with one, which adds in another order. */
@@ -324,7 +324,8 @@ size_t pk_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int dtype)
 int pk_token_logprobs_fwd(const void* logits, int64_t ld, const int* targets, int64_t rows, int64_t vocab, float scale,
                           float* logp, float* lse, void* workspace, size_t workspace_bytes, int dtype, void* stream);
 /* dlogits[r, j] = dlogp[r] * scale * ([j = target] - exp(z_j - lse_r)), every row written: zeros where the target is
- * negative or dlogp is 0 (such a row is not read). dlogits may be the logits themselves (same ld), else lies clear
+ * negative or dlogp is 0 (such a row is not read). lse is the forward's for the same logits and scale; past 1024 in
+ * size 32 bits say too little of it, and the row's sum is formed again from its logits. dlogits may be the logits themselves (same ld), else lies clear
  * of them; so in the two losses below. */
 int pk_token_logprobs_bwd(const void* logits, int64_t ld, const int* targets, const float* lse, const float* dlogp,
                           int64_t rows, int64_t vocab, float scale, void* dlogits, int64_t dld, int dtype, void* stream);

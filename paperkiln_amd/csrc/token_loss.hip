@@ -43,9 +43,13 @@ struct Loss {
 };
 enum Mode { LOGP, GRAD, POLICY };
 
-// 2^(s2 x) against 2^ref, the exponent from both parts of s2: rounded to 32 bits s2 would turn every row's log-probability by up to 6e-8 times its logits, always the same
-// way, and a preference loss adds up hundreds of them (margins 4e-7 off, 1e-7 so). A logit of -inf stays one: the low part is not zero nor negative.
-__device__ inline float power_of(const Loss& a, float x, float ref) { return __builtin_amdgcn_exp2f(fmaf(x, a.s2_lo, fmaf(x, a.s2_hi, -ref))); }
+// 2^(s2 (x - m)). The difference is taken before the product, so a row of the type's lowest value has its probabilities too. The exponent from both parts of s2: rounded to 32
+// bits it would turn every row's log-probability by up to 6e-8 times its logits, always the same way, and a preference loss adds up hundreds of them (margins
+// 4e-7 off, 1e-7 so). A logit of -inf stays one: the low part is not zero nor negative.
+__device__ inline float power_of(const Loss& a, float x, float m) {
+    const float d = x - m;
+    return __builtin_amdgcn_exp2f(fmaf(d, a.s2_hi, d * a.s2_lo));
+}
 void set_scale(Loss& a, float scale) {
     a.scale = scale;
     a.s2 = static_cast<double>(scale) * 1.4426950408889634074;
@@ -96,13 +100,65 @@ __device__ inline void pairs_mean(const Loss& a) {
     if (threadIdx.x == 0) *a.loss = static_cast<float>(s / static_cast<double>(a.pairs));
 }
 
+// log2 of the sum of 2^(s2 x) over a row: s2 top + log2. Its two parts stay apart, since their sum, in 32 bits, knows the second one no more where logits are large.
+struct RowSum {
+    float top;
+    double log2;
+};
+__device__ inline RowSum row_sum(float top, double sum) { return RowSum{top, sum == 0.0 ? static_cast<double>(NAN) : log2(sum)}; }  // a row without a word has no probabilities
+// From what each wavefront has: the logit that it took its exponentials against and their sum; one without a word has none to scale.
+template <int WAVES>
+__device__ inline RowSum sum_of_row(const Loss& a, const float (&m)[WAVES], const float (&s)[WAVES]) {
+    float top = m[0];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) top = fmaxf(top, m[w]);
+    double sum = 0.0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) sum += s[w] == 0.0f ? 0.0 : static_cast<double>(s[w] * power_of(a, m[w], top));
+    return row_sum(top, sum);
+}
+
+// What a row's gradient is made of once its sum is known: -coef 2^(s2 (x - top) - log2), and the target's element.
+struct RowOut {
+    float top, log2, coef, target;
+    __device__ float other(float x, float s2) const { return -coef * __builtin_amdgcn_exp2f(fmaf(x - top, s2, -log2)); }
+};
+template <Mode MODE>
+__device__ inline RowOut finish(const Loss& a, int64_t r, float xt, const RowSum& sum, bool writes = true) {
+    const double logp = ((static_cast<double>(xt) - static_cast<double>(sum.top)) * a.s2 - sum.log2) * LN2;
+    RowOut o{sum.top, static_cast<float>(sum.log2), 0.0f, 0.0f};
+    double w = 0.0, loss = 0.0;
+    if (MODE == POLICY) {
+        double slope;
+        policy_row(a, r, logp, loss, slope);
+        w = a.weights[r];
+        o.coef = static_cast<float>(w * slope * a.upstream * a.scale);
+        o.target = o.coef * static_cast<float>(-expm1(logp));
+    }
+    if (writes) {
+        if (MODE == POLICY) a.row_loss[r] = w * loss;
+        a.logp[r] = static_cast<float>(logp);
+        if (a.lse) a.lse[r] = static_cast<float>((static_cast<double>(sum.top) * a.s2 + sum.log2) * LN2);
+        if (MODE == LOGP && a.fine) a.fine[r] = logp;
+    }
+    return o;
+}
+// GRAD: from a coefficient and a row's sum, or from that sum's log in 32 bits. A log of l leaves the probabilities 2^-24 l off: up to 1024 6e-5, beyond the row is read
+// once more for its sum (logits of a few thousand: 2^-12 off without; 2048 rows of 32000 words bf16 54 us, up to there 45).
+__device__ inline bool far(float lse) { return fabsf(lse) > 1024.0f; }
+__device__ inline RowOut summed_row(const Loss& a, float coef, float xt, const RowSum& sum, bool word) {
+    if (!word) coef = NAN;  // a token that is no word has no gradient
+    const double logp = ((static_cast<double>(xt) - static_cast<double>(sum.top)) * a.s2 - sum.log2) * LN2;
+    return RowOut{sum.top, static_cast<float>(sum.log2), coef, coef * -expm1f(static_cast<float>(logp))};
+}
+__device__ inline RowOut given_row(const Loss& a, int64_t r, float coef, float xt, bool word) { return summed_row(a, coef, xt, RowSum{0.0f, a.lse_in[r] * (1.0 / LN2)}, word); }
+
 // A gradient that does not lie as its logits do (another row pitch, another offset, modulo 16 bytes): a workgroup takes a row element by element.
 constexpr int ANY_NT = 256;
 template <typename T, Mode MODE>
 __global__ __launch_bounds__(ANY_NT) void rows_any(Loss a) {
     if (MODE == GRAD && blockIdx.x == a.rows) return pairs_mean<ANY_NT>(a);
-    __shared__ float sh_m[ANY_NT / 64];
-    __shared__ double sh_s[ANY_NT / 64];
+    __shared__ float sh_m[ANY_NT / 64], sh_s[ANY_NT / 64];
     const int64_t r = blockIdx.x;
     const int tid = threadIdx.x, V = a.vocab, t = a.targets[r];
     const T* x = static_cast<const T*>(a.logits) + r * a.ld;
@@ -122,47 +178,26 @@ __global__ __launch_bounds__(ANY_NT) void rows_any(Loss a) {
             for (int j = tid; j < V; j += ANY_NT) put(dx, j, 0.0f);
         return;
     }
-    const float s2 = a.scale * LOG2E;
     const float xt = t < V ? elem(x, t) : NAN;  // read before the row is written over; a token that is no word has no probability
-    float lse2, target_grad;
-    if (MODE == GRAD) {
-        const double lse = a.lse_in[r];
-        lse2 = static_cast<float>(lse / LN2);
-        target_grad = coef * static_cast<float>(-expm1((static_cast<double>(xt) * a.s2 - lse / LN2) * LN2));
-        if (t >= V) coef = NAN;
+    RowOut o;
+    const bool given = MODE == GRAD && !far(a.lse_in[r]);
+    if (given) {
+        o = given_row(a, r, coef, xt, t < V);
     } else {
         float m = -INFINITY, s = 0.0f;
         for (int j = tid; j < V; j += ANY_NT) m = fmaxf(m, elem(x, j));
-        for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-        if ((tid & 63) == 0) sh_m[tid >> 6] = m;
-        __syncthreads();
-        m = sh_m[0];
-        for (int w = 1; w < ANY_NT / 64; ++w) m = fmaxf(m, sh_m[w]);
-        const float m2 = m * s2;
-        for (int j = tid; j < V; j += ANY_NT) s += power_of(a, elem(x, j), m2);
+        for (int o_ = 32; o_ >= 1; o_ >>= 1) m = fmaxf(m, __shfl_xor(m, o_));
+        const float ref = m == -INFINITY ? 0.0f : m;
+        for (int j = tid; j < V; j += ANY_NT) s += power_of(a, elem(x, j), ref);
         s = group_sum<64>(s);
-        if ((tid & 63) == 0) sh_s[tid >> 6] = s;
+        if ((tid & 63) == 0) sh_m[tid >> 6] = s == 0.0f ? -INFINITY : ref, sh_s[tid >> 6] = s;
         __syncthreads();
-        double sum = 0.0;
-        for (int w = 0; w < ANY_NT / 64; ++w) sum += sh_s[w];
-        const double lse_2 = static_cast<double>(m2) + log2(sum), lse = lse_2 * LN2, logp = (static_cast<double>(xt) * a.s2 - lse_2) * LN2;
-        lse2 = static_cast<float>(lse_2);
-        if (MODE == POLICY) {
-            double loss, slope;
-            policy_row(a, r, logp, loss, slope);
-            const double w = a.weights[r];
-            coef = static_cast<float>(w * slope * a.upstream * a.scale);
-            target_grad = coef * static_cast<float>(-expm1(logp));
-            if (tid == 0) a.row_loss[r] = w * loss;
-        }
-        if (tid == 0) {
-            a.logp[r] = static_cast<float>(logp);
-            if (a.lse) a.lse[r] = static_cast<float>(lse);
-            if (MODE == LOGP && a.fine) a.fine[r] = logp;
-        }
+        const RowSum sum = sum_of_row<ANY_NT / 64>(a, sh_m, sh_s);
+        o = MODE == GRAD ? summed_row(a, coef, xt, sum, t < V) : finish<MODE>(a, r, xt, sum, tid == 0);
     }
+    __syncthreads();  // the target has been read by all
     if (MODE != LOGP)
-        for (int j = tid; j < V; j += ANY_NT) put(dx, j, j == t ? target_grad : -coef * __builtin_amdgcn_exp2f(fmaf(elem(x, j), s2, -lse2)));
+        for (int j = tid; j < V; j += ANY_NT) put(dx, j, j == t ? o.target : o.other(elem(x, j), a.scale * LOG2E));
 }
 
 // ---- rows in 16-byte pieces -------------------------------------------------------------------------------------------------
@@ -248,39 +283,6 @@ __device__ inline void store_piece(T* x, const Piece<T>& v) {
         *p = v.v;
 }
 
-// log2 of the sum of 2^(s2 x) over a row from what each wavefront has: the largest s2 x that it took its exponentials against and their sum.
-template <int WAVES>
-__device__ inline double lse2_of(const float (&m)[WAVES], const float (&s)[WAVES]) {
-    float top = m[0];
-#pragma unroll
-    for (int w = 1; w < WAVES; ++w) top = fmaxf(top, m[w]);
-    double sum = 0.0;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) sum += s[w] == 0.0f ? 0.0 : static_cast<double>(s[w] * __builtin_amdgcn_exp2f(m[w] - top));  // a wavefront without a word has none to scale
-    return sum == 0.0 ? static_cast<double>(NAN) : top + log2(sum);  // a row without a word has no probabilities
-}
-
-// What a row's gradient is made of once its sum is known.
-struct RowOut {
-    float lse2, coef, target;  // log2 of the sum, the row's coefficient, the target's gradient
-};
-template <Mode MODE>
-__device__ inline RowOut finish(const Loss& a, int64_t r, float xt, double lse2) {
-    const double logp = (static_cast<double>(xt) * a.s2 - lse2) * LN2;
-    RowOut o{static_cast<float>(lse2), 0.0f, 0.0f};
-    if (MODE == POLICY) {
-        double loss, slope;
-        policy_row(a, r, logp, loss, slope);
-        const double w = a.weights[r];
-        o.coef = static_cast<float>(w * slope * a.upstream * a.scale);
-        o.target = o.coef * static_cast<float>(-expm1(logp));
-        a.row_loss[r] = w * loss;
-    }
-    a.logp[r] = static_cast<float>(logp);
-    if (a.lse) a.lse[r] = static_cast<float>(lse2 * LN2);
-    if (MODE == LOGP && a.fine) a.fine[r] = logp;
-    return o;
-}
 // A row that does not count: not read, its results zeros.
 template <Mode MODE>
 __device__ inline void no_row(const Loss& a, int64_t r) {
@@ -295,8 +297,8 @@ __device__ inline void zero_row(T* dx, const Cut<T>& cut, int tid) {
 }
 // The gradient of a piece as if none of its words were the target; the thread that holds the target's piece writes that element over afterwards.
 template <typename T>
-__device__ inline Piece<T> gradient(const Piece<T>& x, float s2, float lse2, float coef) {
-    return x.map([&](int, float v) { return -coef * __builtin_amdgcn_exp2f(fmaf(v, s2, -lse2)); });
+__device__ inline Piece<T> gradient(const Piece<T>& x, float s2, const RowOut& o) {
+    return x.map([&](int, float v) { return o.other(v, s2); });
 }
 
 // Between two walks over a row the pieces stay as they are: the compiler would keep every element of the first walk in a register of its own.
@@ -326,7 +328,6 @@ __global__ __launch_bounds__(ROW_NT) void rows_held(Loss a) {
         if (MODE != LOGP) zero_row<T, ROW_NT, PAST>(dx, cut, tid);
         return;
     }
-    const float s2 = a.scale * LOG2E;
     Piece<T> held[PER];
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
@@ -340,22 +341,20 @@ __global__ __launch_bounds__(ROW_NT) void rows_held(Loss a) {
     for (int k = 0; k < PER; ++k) held[k].each([&](float v) { m = fmaxf(m, v); });
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-    const float m2 = m == -INFINITY ? 0.0f : m * s2;
-    float s = power_of(a, edge, m2);
+    const float ref = m == -INFINITY ? 0.0f : m;
+    float s = power_of(a, edge, ref);
     keep_packed(held);
 #pragma unroll
-    for (int k = 0; k < PER; ++k) held[k].each([&](float v) { s += power_of(a, v, m2); });
+    for (int k = 0; k < PER; ++k) held[k].each([&](float v) { s += power_of(a, v, ref); });
     s = group_sum<64>(s);
     RowOut o;
     if constexpr (WAVES == 1) {
-        const float ms[1] = {m2}, ss[1] = {s};
-        if (MODE == LOGP && tid != 0) return;
-        o = finish<MODE>(a, r, xt, lse2_of<1>(ms, ss));
+        o = finish<MODE>(a, r, xt, row_sum(ref, s), tid == 0);
     } else {
-        if ((tid & 63) == 0) sh_m[tid >> 6] = s == 0.0f ? -INFINITY : m2, sh_s[tid >> 6] = s;
+        if ((tid & 63) == 0) sh_m[tid >> 6] = s == 0.0f ? -INFINITY : ref, sh_s[tid >> 6] = s;
         __syncthreads();
         if (tid < 64) {
-            o = finish<MODE>(a, r, xt, lse2_of<WAVES>(sh_m, sh_s));
+            o = finish<MODE>(a, r, xt, sum_of_row<WAVES>(a, sh_m, sh_s), tid == 0);
             if (tid == 0) sh_o = o;
         }
         if constexpr (MODE == LOGP) return;
@@ -364,26 +363,25 @@ __global__ __launch_bounds__(ROW_NT) void rows_held(Loss a) {
     }
     if constexpr (MODE != LOGP) {
         if (o.coef == 0.0f) return zero_row<T, ROW_NT, PAST>(dx, cut, tid);  // clipped
+        const float s2 = a.scale * LOG2E;
         keep_packed(held);
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
             const int p = tid + k * ROW_NT;
-            if (p < cut.pieces) store_piece<PAST>(dx + cut.head + p * N, gradient(held[k], s2, o.lse2, o.coef));
+            if (p < cut.pieces) store_piece<PAST>(dx + cut.head + p * N, gradient(held[k], s2, o));
         }
-        if (tid < cut.edges) put(dx, cut.edge(tid), -o.coef * __builtin_amdgcn_exp2f(fmaf(edge, s2, -o.lse2)));
+        if (tid < cut.edges) put(dx, cut.edge(tid), o.other(edge, s2));
         if (tid == cut.holder(t, ROW_NT)) put(dx, t, o.target);
     }
 }
 
 // Rows that no workgroup holds are read in strides, with a running maximum and sum, and again for the gradient.
 constexpr int LONG_U = 4;
-template <typename T, int NT, bool EDGES>
+template <typename T, int NT>
 __device__ inline void running(const Loss& a, const T* x, const Cut<T>& cut, int from, int to, float edge, float* sh_m, float* sh_s) {
     constexpr int N = Piece<T>::N;
     const int tid = threadIdx.x;
-    const float s2 = a.scale * LOG2E;
-    float m2 = -INFINITY, s = 0.0f;
-    if (EDGES && edge != -INFINITY) m2 = edge * s2, s = power_of(a, edge, m2);
+    float m = edge, s = edge == -INFINITY ? 0.0f : power_of(a, edge, edge);
     for (int p0 = from + tid; p0 < to; p0 += LONG_U * NT) {
         Piece<T> v[LONG_U];
 #pragma unroll
@@ -391,20 +389,20 @@ __device__ inline void running(const Loss& a, const T* x, const Cut<T>& cut, int
             const int p = p0 + u * NT;
             v[u] = p < to ? load_piece<false>(x + cut.head + p * N) : Piece<T>::nothing();
         }
-        float top = -INFINITY;
+        float top = m;
 #pragma unroll
         for (int u = 0; u < LONG_U; ++u) v[u].each([&](float y) { top = fmaxf(top, y); });
-        const float new2 = fmaxf(m2, top * s2), ref = new2 == -INFINITY ? 0.0f : new2;
-        s = s == 0.0f ? 0.0f : s * __builtin_amdgcn_exp2f(m2 - ref);
+        const float ref = top == -INFINITY ? 0.0f : top;
+        s = s == 0.0f ? 0.0f : s * power_of(a, m, ref);
 #pragma unroll
         for (int u = 0; u < LONG_U; ++u) v[u].each([&](float y) { s += power_of(a, y, ref); });
-        m2 = new2;
+        m = top;
     }
     // lanes, then wavefronts
-    float top = m2;
+    float top = m;
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-    s = group_sum<64>(s == 0.0f ? 0.0f : s * __builtin_amdgcn_exp2f(m2 - top));
+    s = group_sum<64>(s == 0.0f ? 0.0f : s * power_of(a, m, top));
     if ((tid & 63) == 0) sh_m[tid >> 6] = s == 0.0f ? -INFINITY : top, sh_s[tid >> 6] = s;
     __syncthreads();
 }
@@ -427,10 +425,10 @@ __global__ __launch_bounds__(LONG_NT) void rows_long(Loss a) {
         return;
     }
     const float edge = tid < cut.edges ? elem(x, cut.edge(tid)) : -INFINITY, xt = t < V ? elem(x, t) : NAN;
-    running<T, LONG_NT, true>(a, x, cut, 0, cut.pieces, edge, sh_m, sh_s);
+    running<T, LONG_NT>(a, x, cut, 0, cut.pieces, edge, sh_m, sh_s);
     RowOut o;
     if (tid < 64) {
-        o = finish<MODE>(a, r, xt, lse2_of<WAVES>(sh_m, sh_s));
+        o = finish<MODE>(a, r, xt, sum_of_row<WAVES>(a, sh_m, sh_s), tid == 0);
         if (tid == 0) sh_o = o;
     }
     if constexpr (MODE != LOGP) {
@@ -440,14 +438,14 @@ __global__ __launch_bounds__(LONG_NT) void rows_long(Loss a) {
         const float s2 = a.scale * LOG2E;
         for (int p = tid; p < cut.pieces; p += LONG_NT) {
             const int j0 = cut.head + p * N;
-            store_piece<PAST>(dx + j0, gradient(load_piece<PAST>(x + j0), s2, o.lse2, o.coef));
+            store_piece<PAST>(dx + j0, gradient(load_piece<PAST>(x + j0), s2, o));
         }
-        if (tid < cut.edges) put(dx, cut.edge(tid), -o.coef * __builtin_amdgcn_exp2f(fmaf(edge, s2, -o.lse2)));
+        if (tid < cut.edges) put(dx, cut.edge(tid), o.other(edge, s2));
         if (tid == cut.holder(t, LONG_NT)) put(dx, t, o.target);
     }
 }
 
-// A few such rows are dealt to several workgroups, `per` pieces each, which leave the largest exponent and the sum of their part; a wavefront joins a row's.
+// A few such rows are dealt to several workgroups, `per` pieces each, which leave the largest logit and the sum of their part; a wavefront joins a row's.
 constexpr int PART_NT = 512, MOST_PARTS = 32, FEW_ROWS = 128;
 template <typename T>
 __global__ __launch_bounds__(PART_NT) void rows_part(Loss a, int per, float2* parts) {
@@ -460,13 +458,13 @@ __global__ __launch_bounds__(PART_NT) void rows_part(Loss a, int per, float2* pa
     const Cut<T> cut(x, a.vocab);
     const int from = static_cast<int>(blockIdx.y) * per, to = min(cut.pieces, from + per);
     const float edge = blockIdx.y == 0 && tid < cut.edges ? elem(x, cut.edge(tid)) : -INFINITY;
-    running<T, PART_NT, true>(a, x, cut, from, to, edge, sh_m, sh_s);
+    running<T, PART_NT>(a, x, cut, from, to, edge, sh_m, sh_s);
     if (tid != 0) return;
     float top = sh_m[0], s = 0.0f;
 #pragma unroll
     for (int w = 1; w < WAVES; ++w) top = fmaxf(top, sh_m[w]);
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) s += sh_s[w] == 0.0f ? 0.0f : sh_s[w] * __builtin_amdgcn_exp2f(sh_m[w] - top);
+    for (int w = 0; w < WAVES; ++w) s += sh_s[w] == 0.0f ? 0.0f : sh_s[w] * power_of(a, sh_m[w], top);
     parts[r * gridDim.y + blockIdx.y] = make_float2(top, s);
 }
 template <typename T>
@@ -482,11 +480,11 @@ __global__ __launch_bounds__(64) void rows_join(Loss a, int count, const float2*
     float top = v.x;
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-    double sum = v.y == 0.0f ? 0.0 : static_cast<double>(v.y * __builtin_amdgcn_exp2f(v.x - top));
+    double sum = v.y == 0.0f ? 0.0 : static_cast<double>(v.y * power_of(a, v.x, top));
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
     const T* x = static_cast<const T*>(a.logits) + r * a.ld;
-    if (lane == 0) finish<LOGP>(a, r, t < a.vocab ? elem(x, t) : NAN, sum == 0.0 ? static_cast<double>(NAN) : top + log2(sum));
+    if (lane == 0) finish<LOGP>(a, r, t < a.vocab ? elem(x, t) : NAN, row_sum(top, sum));
 }
 
 // The gradient of rows whose sums are known: every element by itself, so a row may be dealt to several workgroups (grid.y, `per` pieces each) and written over.
@@ -494,6 +492,7 @@ constexpr int GRAD_NT = 512, GRAD_U = 8;
 template <typename T, bool PAST>
 __global__ __launch_bounds__(GRAD_NT) void rows_grad(Loss a, int per) {
     constexpr int N = Piece<T>::N;
+    __shared__ float sh_m[GRAD_NT / 64], sh_s[GRAD_NT / 64];
     if (blockIdx.x == a.rows) {
         if (blockIdx.y == 0) pairs_mean<GRAD_NT>(a);
         return;
@@ -511,16 +510,23 @@ __global__ __launch_bounds__(GRAD_NT) void rows_grad(Loss a, int per) {
         if (edges) put(dx, cut.edge(tid), 0.0f);
         return;
     }
-    const float coef = t < V ? given : NAN;  // a token that is no word has no gradient
-    const double exact = a.lse_in[r] / LN2;
-    const float lse2 = static_cast<float>(exact);
+    if (far(a.lse_in[r])) {  // its log says too little in 32 bits: one workgroup forms the sum again, before it writes over the row
+        if (blockIdx.y != 0) return;
+        const float edge = tid < cut.edges ? elem(x, cut.edge(tid)) : -INFINITY, xt = t < V ? elem(x, t) : NAN;
+        running<T, GRAD_NT>(a, x, cut, 0, cut.pieces, edge, sh_m, sh_s);
+        const RowOut o = summed_row(a, given, xt, sum_of_row<GRAD_NT / 64>(a, sh_m, sh_s), t < V);
+        for (int p = tid; p < cut.pieces; p += GRAD_NT) store_piece<PAST>(dx + cut.head + p * N, gradient(load_piece<PAST>(x + cut.head + p * N), s2, o));
+        if (tid < cut.edges) put(dx, cut.edge(tid), o.other(edge, s2));
+        if (tid == cut.holder(t, GRAD_NT)) put(dx, t, o.target);
+        return;
+    }
     // the target's element, read by its holder before it is written over
     const int pt = t < V && t >= cut.head ? (t - cut.head) / N : -1;
     const bool held_here = pt >= 0 && pt < cut.pieces ? pt >= from && pt < to : blockIdx.y == 0, holds = held_here && tid == cut.holder(t, GRAD_NT, from);
-    const float xt = holds ? elem(x, t) : 0.0f;
+    const RowOut o = given_row(a, r, given, holds ? elem(x, t) : 0.0f, t < V);
     if (edges) {
         const int j = cut.edge(tid);
-        put(dx, j, -coef * __builtin_amdgcn_exp2f(fmaf(elem(x, j), s2, -lse2)));
+        put(dx, j, o.other(elem(x, j), s2));
     }
     for (int p0 = from + tid; p0 < to; p0 += GRAD_U * GRAD_NT) {
         Piece<T> v[GRAD_U];
@@ -532,10 +538,10 @@ __global__ __launch_bounds__(GRAD_NT) void rows_grad(Loss a, int per) {
 #pragma unroll
         for (int u = 0; u < GRAD_U; ++u) {
             const int p = p0 + u * GRAD_NT, j0 = cut.head + p * N;
-            if (p < to) store_piece<PAST>(dx + j0, gradient(v[u], s2, lse2, coef));
+            if (p < to) store_piece<PAST>(dx + j0, gradient(v[u], s2, o));
         }
     }
-    if (holds) put(dx, t, coef * -expm1f(static_cast<float>((static_cast<double>(xt) * a.s2 - exact) * LN2)));
+    if (holds) put(dx, t, o.target);
 }
 
 __global__ __launch_bounds__(1024) void loss_sum(const double* x, int64_t n, float* out) {
@@ -663,7 +669,7 @@ int check(const char* who, const void* logits, int64_t ld, const int* targets, i
     const std::string w(who);
     if (rows < 0 || rows >= INT32_MAX || vocab <= 0 || vocab > (1 << 30)) return fail(PK_ERR_SHAPE, w + ": shape mismatch (rows or vocabulary out of range)");
     if (!known_dtype(dtype)) return fail(PK_ERR_ARGUMENT, w + ": dtype must be PK_F32 or PK_BF16");
-    if (!(scale > 0.0f) || !std::isfinite(scale)) return fail(PK_ERR_ARGUMENT, w + ": scale must be positive");
+    if (!(scale >= 0x1p-64f && scale <= 0x1p64f)) return fail(PK_ERR_ARGUMENT, w + ": scale must lie between 2^-64 and 2^64");  // both parts of its product with log2(e) are numbers
     if (ld < 0 || (writes && rows > 1 && dld < vocab)) return fail(PK_ERR_SHAPE, w + ": rows of logits overlap");
     if (rows == 0) return PK_OK;
     if (!logits || !targets || (writes && !dlogits)) return fail(PK_ERR_ARGUMENT, w + ": null pointer");

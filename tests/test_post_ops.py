@@ -59,7 +59,7 @@ def test_qk_norm_rope_refuses_null_and_small_workspaces():
 # what is the same for the three entries that read logits and write their gradient
 LOGITS_REFUSED = [(dict(rows=-1), SHAPE), (dict(rows=1 << 31), SHAPE), (dict(vocab=0), SHAPE), (dict(vocab=(1 << 30) + 1), SHAPE), (dict(ld=-1), SHAPE),
                   (dict(dld=99), SHAPE), (dict(dtype=7), ARGUMENT), (dict(scale=0.0), ARGUMENT), (dict(scale=-1.0), ARGUMENT), (dict(scale=math.inf), ARGUMENT),
-                  (dict(scale=math.nan), ARGUMENT), (dict(logits=None), ARGUMENT), (dict(targets=None), ARGUMENT), (dict(dlogits=None), ARGUMENT),
+                  (dict(scale=math.nan), ARGUMENT), (dict(scale=1e-25), ARGUMENT), (dict(scale=1e25), ARGUMENT), (dict(logits=None), ARGUMENT), (dict(targets=None), ARGUMENT), (dict(dlogits=None), ARGUMENT),
                   (dict(dlogits=CLOSE), ARGUMENT), (dict(dlogits=SOME, dld=200), ARGUMENT)]
 
 

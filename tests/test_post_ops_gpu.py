@@ -330,6 +330,47 @@ def test_token_logprobs_of_rows_that_hold_no_number(pk):
         assert torch.equal(logp[6:], want[6:])
 
 
+@pytest.mark.parametrize("scale", [2.0 ** -64, 1e-6, 1.0, 1.4426951, 300.0, 2.0 ** 64])
+def test_token_logprobs_over_scales(pk, scale):
+    """The exponent's factor in two parts, both numbers over the whole range; words without probability stay so at each."""
+    x, t, _ = loss_inputs(6, 3001, FP32, 12)
+    x[:, 5::11] = -math.inf
+    t = torch.where(torch.isinf(x.gather(1, t.long()[:, None])[:, 0]), t - 1, t).clamp(min=0).to(torch.int32)
+    s = float(np.float32(scale))
+    z, wl, wp, _ = softmax64(x, t, s)
+    logp, lse = pk.ops.token_logprobs_fwd(x, t, scale)
+    within("lse", lse, wl, U * wl.abs() + logp_slack(z, 3001))
+    within("logp", logp, wp, U * wp.abs() + logp_slack(z, 3001))
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("rows,vocab,pitch", [(7, 61, 0), (3, 3001, 0), (200, 777, 784), (2, 150001, 0), (130, 66000, 0)])
+@pytest.mark.parametrize("base", [-2e3, 5e5, -3e38])
+def test_losses_of_far_logits(pk, base, rows, vocab, pitch, dtype):
+    """Logits far from zero: their differences alone count, and the log of the sum in 32 bits tells too little for a gradient. A difference is exact where it is
+    of use; an exponent past 104 gives nothing; so an exponent is within 2 u of 104, its log2 of the sum within u of 20, and the rest as for other logits."""
+    x, t, g = loss_inputs(rows, vocab, dtype, 17, pitch)
+    x.copy_(x.float().mul_(max(1.0, abs(base) * 2.0 ** -21) / 3.0).add_(base).clamp_(min=torch.finfo(dtype).min))
+    dlogp = torch.randn(rows, generator=g, device="cuda")
+    t[::2] = x[::2].argmax(1).to(torch.int32)
+    top = x.double().amax(1, keepdim=True)
+    _, wl, wp, p = softmax64(x.double() - top, t, 1.0)
+    near = (wp > -100.0).float()   # the others' ratio is that of two roundings
+    slack = (3 * 104 + 12 + 2 * 20 + vocab / 64) * U
+    logp, lse = pk.ops.token_logprobs_fwd(x, t)
+    within("lse", lse, wl + top[:, 0], U * (wl + top[:, 0]).abs() + slack)
+    within("logp", logp, wp, U * wp.abs() + slack)
+    hot = torch.zeros_like(p).scatter_(1, t.long()[:, None], 1.0)
+    for coef, d in ((dlogp, pk.ops.token_logprobs_bwd(x, t, lse, dlogp)), (dlogp, pk.ops.token_logprobs_bwd(x, t, lse, dlogp, out=x.new_empty((rows, vocab + 5))[:, 2:2 + vocab])),
+                    (dlogp, pk.ops.token_logprobs_bwd(x.clone(), t, lse, dlogp)),
+                    (-dlogp.abs() * near, pk.blockops.policy_loss(x, t, logp, dlogp.abs(), near)[1])):
+        want = coef.double()[:, None] * (hot - p)
+        within("dlogits", d, want, HALF[dtype] * want.abs() + coef.double().abs()[:, None] * 2 * slack + 1e-37)
+    over = x.clone()
+    pk.ops.token_logprobs_bwd(over, t, lse, dlogp, out=over)
+    assert torch.equal(over, pk.ops.token_logprobs_bwd(x.clone(), t, lse, dlogp))
+
+
 def test_token_logprobs_dealt_out_and_whole(pk):
     """A few rows past what a workgroup holds: dealt to several with a workspace, whole without one, each within the count of the other test; rows that hold no number,
     are not read or have one word only, among them."""
