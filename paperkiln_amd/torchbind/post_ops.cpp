@@ -3,6 +3,7 @@
 // tensors and on that device's current stream; outputs and workspaces come from torch's allocator on that stream.
 #include <ATen/MemoryOverlap.h>
 #include <ATen/hip/EmptyTensor.h>
+#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
 
 #include <cmath>
@@ -38,6 +39,24 @@ void no_tangent(const char* who, const Tensor& t) {
 }
 void first_order(const char* who) {
     if (at::GradMode::is_enabled()) refuse(who, "its gradient is not differentiable");
+}
+// A backward pass that is being recorded into a graph while gradients of this node's inputs belong to a stream outside of the recording (a graph of the same
+// leaves that was built before and lives on keeps their accumulation there): the engine would have that stream wait for the recording, which ends the process.
+void recordable(const char* who, Node& node) {
+    using Stream = c10::hip::HIPStreamMasqueradingAsCUDA;
+    const auto recording = [](hipStream_t s) {  // the null stream never is, and must not be asked
+        hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+        return s && hipStreamIsCapturing(s, &status) == hipSuccess && status != hipStreamCaptureStatusNone;
+    };
+    const Stream now = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA();
+    if (!recording(now.stream())) return;
+    for (size_t i = 0; i < node.num_outputs(); ++i) {
+        const auto& next = node.next_edge(i);
+        if (!next.is_valid() || !node.task_should_compute_output(i)) continue;
+        const auto other = next.function->stream();
+        if (other && *other != now.unwrap() && !recording(Stream(*other).stream()))
+            refuse(who, "a backward pass is being recorded whose inputs' gradients belong to a stream outside of the recording: drop the graphs of the same leaves first");
+    }
 }
 
 // ---- per-head norms with rotation ----
@@ -126,6 +145,7 @@ struct QkNormRopeBackward : public Node {
     }
     variable_list apply(variable_list&& in) override {
         first_order(QK);
+        recordable(QK, *this);
         Tensor tq, tk, twq, twk, tp;
         {
             const std::lock_guard<std::mutex> lock(mutex_);
@@ -207,6 +227,7 @@ struct TokenLogprobsBackward : public Node {
     }
     variable_list apply(variable_list&& in) override {
         first_order(LP);
+        recordable(LP, *this);
         Tensor x, t, l;
         {
             const std::lock_guard<std::mutex> lock(mutex_);

@@ -903,6 +903,38 @@ def test_operators_under_graph_capture(pk):
         assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip((*state.m, *state.v), (*estate.m, *estate.v)))
 
 
+def test_a_backward_pass_under_graph_capture(pk):
+    """Both nodes recorded with the passes around them and replayed between eager calls. While an eager graph of the same leaves lives, their gradients belong
+    to its stream, which must not wait for a recording: refused, and the next recording stands."""
+    q, k, wq, wk, pos, dyq, dyk = qk_inputs(2, 24, 4, 2, 64, FP32, 3)
+    x, t, g = loss_inputs(48, 700, FP32, 4)
+    q, k, x = (y.contiguous().requires_grad_() for y in (q, k, x))
+    wq, wk = wq.requires_grad_(), wk.requires_grad_()
+
+    def norms():
+        yq, yk = pk.ops.qk_norm_rope(q, k, wq, wk, pos, 1e4)
+        return torch.autograd.grad((yq * dyq).sum() + (yk * dyk).sum(), (q, k, wq, wk))
+
+    def logp():
+        return torch.autograd.grad((pk.ops.token_logprobs(x, t) * 0.5).sum(), x)
+
+    for fn, graph_that_lives in ((norms, lambda: pk.ops.qk_norm_rope(q, k, wq, wk, pos, 1e4)), (logp, lambda: pk.ops.token_logprobs(x, t))):
+        alive = graph_that_lives()
+        with pytest.raises(RuntimeError, match="outside of the recording"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                fn()
+        del alive
+        graph, out = graph_of(fn)
+        for _ in range(3):
+            with torch.no_grad():
+                for y in (q, k, x):
+                    y.copy_(torch.randn(y.shape, generator=g, device="cuda"))
+            want = fn()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
 def test_operators_on_two_streams_at_once(pk):
     """The same calls queued on two streams over different inputs: the results of one after the other."""
     sets = []
