@@ -498,6 +498,11 @@ int check(const pk_qk_shape* s, const char* who) {
     return PK_OK;
 }
 bool bad(const pk_tensor4* t) { return !t || !t->ptr; }
+// Whether a result begins where the other one does, or where something of the other one's is read: rows of both kinds would be written and read by different wavefronts.
+bool crossed(const pk_tensor4* q, const pk_tensor4* k, std::initializer_list<const pk_tensor4*> read_for_q, std::initializer_list<const pk_tensor4*> read_for_k) {
+    const auto in = [](const pk_tensor4* t, const auto& list) { return std::any_of(list.begin(), list.end(), [&](const pk_tensor4* x) { return x->ptr == t->ptr; }); };
+    return q->ptr == k->ptr || in(q, read_for_k) || in(k, read_for_q);
+}
 
 void fill(Qk& a, const pk_qk_shape* s) {
     a.B = s->B, a.T = s->T, a.Hq = s->Hq, a.Hkv = s->Hkv, a.dk = s->dk, a.rotary = s->rotary ? s->rotary : s->dk, a.halves = s->halves != 0;
@@ -588,6 +593,7 @@ int pk_qk_norm_rope_fwd(const pk_qk_shape* s, const pk_tensor4* q, const pk_tens
         if (int rc = check(s, "pk_qk_norm_rope_fwd")) return rc;
         if (static_cast<int64_t>(s->B) * s->T == 0) return static_cast<int>(PK_OK);
         if (bad(q) || bad(k) || bad(yq) || bad(yk) || !wq || !wk || !pos) return fail(PK_ERR_ARGUMENT, "pk_qk_norm_rope_fwd: null tensor");
+        if (crossed(yq, yk, {q}, {k})) return fail(PK_ERR_ARGUMENT, "pk_qk_norm_rope_fwd: a result lies over the other one's tensor");
         Qk a;
         fill(a, s);
         a.x[0] = rows_of(q), a.x[1] = rows_of(k), a.y[0] = out_of(yq), a.y[1] = out_of(yk), a.dy[0] = a.dy[1] = Rows{nullptr, 0, 0, 0};
@@ -625,6 +631,7 @@ int pk_qk_norm_rope_bwd(const pk_qk_shape* s, const pk_tensor4* dyq, const pk_te
         if (!none && (bad(dyq) || bad(dyk) || bad(q) || bad(k) || bad(dq) || bad(dk) || !pos)) return fail(PK_ERR_ARGUMENT, "pk_qk_norm_rope_bwd: null tensor");
         if (!workspace || workspace_bytes < pk_qk_norm_rope_bwd_workspace_bytes(s) || !aligned(workspace, 16))
             return fail(PK_ERR_WORKSPACE, "pk_qk_norm_rope_bwd: workspace too small (pk_qk_norm_rope_bwd_workspace_bytes)");
+        if (!none && crossed(dq, dk, {q, dyq}, {k, dyk})) return fail(PK_ERR_ARGUMENT, "pk_qk_norm_rope_bwd: a result lies over the other one's tensor");
         hipStream_t st = static_cast<hipStream_t>(stream);
         Qk a;
         fill(a, s);

@@ -56,6 +56,17 @@ def test_qk_norm_rope_refuses_null_and_small_workspaces():
     assert L.pk_qk_norm_rope_fwd(C.byref(qk(T=0)), T4(0), T4(0), None, None, None, T4(0), T4(0), None) == 0   # nothing to do
 
 
+def test_qk_norm_rope_refuses_crossed_results():
+    """A result that begins where the other one does, or where what the other one is made of does."""
+    L, s = _lib.lib(), qk()
+    at = lambda i: T4((1 + i) << 20)  # noqa: E731
+    for yq, yk in ((5, 5), (2, 6), (5, 1), (2, 1)):   # q at 1, k at 2
+        assert L.pk_qk_norm_rope_fwd(C.byref(s), at(1), at(2), SOME, SOME, SOME, at(yq), at(yk), None) == ARGUMENT and b"other" in L.pk_last_error()
+    need = L.pk_qk_norm_rope_bwd_workspace_bytes(C.byref(s))
+    for dq, dk in ((5, 5), (2, 6), (4, 6), (5, 1), (5, 3)):   # dyq, dyk at 3, 4
+        assert L.pk_qk_norm_rope_bwd(C.byref(s), at(3), at(4), at(1), at(2), SOME, SOME, SOME, at(dq), at(dk), SOME, SOME, SOME, need, None) == ARGUMENT and b"other" in L.pk_last_error()
+
+
 # what is the same for the three entries that read logits and write their gradient
 LOGITS_REFUSED = [(dict(rows=-1), SHAPE), (dict(rows=1 << 31), SHAPE), (dict(vocab=0), SHAPE), (dict(vocab=(1 << 30) + 1), SHAPE), (dict(ld=-1), SHAPE),
                   (dict(dld=99), SHAPE), (dict(dtype=7), ARGUMENT), (dict(scale=0.0), ARGUMENT), (dict(scale=-1.0), ARGUMENT), (dict(scale=math.inf), ARGUMENT),
