@@ -454,10 +454,10 @@ int pk_adamw_many(const pk_adamw_tensor* t, int count, const pk_adamw_config* c,
         if (!(c->b1 >= 0.0f && c->b1 < 1.0f && c->b2 >= 0.0f && c->b2 < 1.0f)) return fail(PK_ERR_ARGUMENT, "pk_adamw_many: b1 and b2 lie in [0, 1)");
         if (c->max_norm != c->max_norm) return fail(PK_ERR_ARGUMENT, "pk_adamw_many: max_norm is no number");
         const bool clip = c->max_norm > 0.0f;
-        int64_t total = 0;  // a launch's workgroups are counted in 32 bits
+        int64_t total = 0;  // a launch has fewer than 2^32 threads, 16 elements each
         for (int i = 0; i < count; ++i) {
             total += t[i].n > 0 ? t[i].n : 0;
-            if (t[i].n < 0 || total > (int64_t{1} << 40)) return fail(PK_ERR_SHAPE, "pk_adamw_many: a tensor's size is out of range");
+            if (t[i].n < 0 || total > (int64_t{1} << 35)) return fail(PK_ERR_SHAPE, "pk_adamw_many: a tensor's size is out of range");
             if (t[i].n > 0 && (!t[i].p || !t[i].g || !t[i].m || !t[i].v || (c->state_bits == 8 && (!t[i].m_scale || !t[i].v_scale))))
                 return fail(PK_ERR_ARGUMENT, "pk_adamw_many: null pointer");
         }

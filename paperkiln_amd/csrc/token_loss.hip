@@ -653,14 +653,27 @@ void launch_typed(const Loss& a, hipStream_t st) {
             past ? launch_held<T, MODE, true>(a, st) : launch_held<T, MODE, false>(a, st);
     }
 }
+// A launch has fewer than 2^32 threads, 1024 for a row at most: more rows than that allows go in runs.
+constexpr int64_t MOST_ROWS = (1 << 22) - 2;
 template <Mode MODE>
-int launch_rows(const Loss& a, int dtype, hipStream_t st) {
-    if (a.rows == 0 && !a.loss) return PK_OK;
-    if (dtype == PK_BF16)
-        launch_typed<uint16_t, MODE>(a, st);
-    else
-        launch_typed<float, MODE>(a, st);
-    return launched();
+int launch_rows(const Loss& all, int dtype, hipStream_t st) {
+    if (all.rows == 0 && !all.loss) return PK_OK;
+    for (int64_t r = 0; r == 0 || r < all.rows; r += MOST_ROWS) {
+        const auto on = [r](auto*& p, int64_t ld = 1) { p = p ? p + r * ld : p; };
+        const int64_t es = elem_size(dtype);
+        Loss a = all;
+        a.rows = std::min(MOST_ROWS, all.rows - r);
+        if (r + MOST_ROWS < all.rows) a.loss = nullptr;  // the last run's
+        a.logits = static_cast<const char*>(a.logits) + r * a.ld * es;
+        if (a.dlogits) a.dlogits = static_cast<char*>(a.dlogits) + r * a.dld * es;
+        on(a.targets), on(a.logp), on(a.lse), on(a.lse_in), on(a.coef), on(a.clear), on(a.fine), on(a.old_logp), on(a.ref_logp), on(a.adv), on(a.weights), on(a.row_loss);
+        if (dtype == PK_BF16)
+            launch_typed<uint16_t, MODE>(a, st);
+        else
+            launch_typed<float, MODE>(a, st);
+        if (int rc = launched()) return rc;
+    }
+    return PK_OK;
 }
 
 // What every entry asks of its logits; dlogits only where it writes them: over the logits, row for row, or clear of them.
@@ -764,7 +777,7 @@ int pk_preference_loss(const pk_preference_config* c, const void* logits, int64_
                        void* workspace, size_t workspace_bytes, int dtype, void* stream) {
     return c_entry([&] {
         if (!c || !loss || !margins || !seq_start) return fail(PK_ERR_ARGUMENT, "pk_preference_loss: null pointer");
-        if (pairs < 1 || pairs > (1 << 28)) return fail(PK_ERR_SHAPE, "pk_preference_loss: shape mismatch (at least one pair is wanted)");
+        if (pairs < 1 || pairs > MOST_ROWS) return fail(PK_ERR_SHAPE, "pk_preference_loss: shape mismatch (at least one pair is wanted)");
         if (int rc = check("pk_preference_loss", logits, ld, targets, rows, vocab, c->scale, dtype, true, dlogits, dld)) return rc;
         if (rows > 0 && (!ref_logp || !logp)) return fail(PK_ERR_ARGUMENT, "pk_preference_loss: null pointer");
         if (!std::isfinite(c->beta) || !std::isfinite(c->upstream)) return fail(PK_ERR_ARGUMENT, "pk_preference_loss: beta and upstream must be finite");

@@ -100,7 +100,7 @@ def test_losses_refuse_logits(entry, change, code):
     ("bwd", dict(v=None), ARGUMENT), ("policy", dict(v=None), ARGUMENT), ("policy", dict(ref=None), ARGUMENT), ("policy", dict(loss=None), ARGUMENT),
     ("policy", dict(low=-0.1), ARGUMENT), ("policy", dict(high=math.nan), ARGUMENT), ("policy", dict(kl=math.inf), ARGUMENT), ("policy", dict(upstream=math.nan), ARGUMENT),
     ("preference", dict(v=None), ARGUMENT), ("preference", dict(ref=None), ARGUMENT), ("preference", dict(starts=None), ARGUMENT), ("preference", dict(loss=None), ARGUMENT),
-    ("preference", dict(pairs=0), SHAPE), ("preference", dict(pairs=-3), SHAPE), ("preference", dict(beta=math.inf), ARGUMENT), ("preference", dict(smoothing=1.5), ARGUMENT),
+    ("preference", dict(pairs=0), SHAPE), ("preference", dict(pairs=1 << 22), SHAPE), ("preference", dict(pairs=-3), SHAPE), ("preference", dict(beta=math.inf), ARGUMENT), ("preference", dict(smoothing=1.5), ARGUMENT),
     ("preference", dict(smoothing=math.nan), ARGUMENT), ("preference", dict(ws=None), WORKSPACE), ("preference", dict(ws_bytes=100), WORKSPACE)], ids=str)
 def test_losses_refuse(entry, change, code):
     assert call(entry, **change) == code and _lib.lib().pk_last_error()
@@ -144,7 +144,7 @@ def test_adamw_many_refuses_tables():
     for bad in (tensor(0, m=1, v=1), tensor(1 << 20, g=0), tensor(1 << 20, m=0), tensor(1 << 20, v=0)):
         assert adamw([bad]) == ARGUMENT
     assert adamw([tensor(1 << 20, scales=0)], state_bits=8) == ARGUMENT
-    assert adamw([tensor(1 << 20, n=-1)]) == SHAPE and adamw([tensor(1 << 20, n=(1 << 40) + 1)]) == SHAPE
+    assert adamw([tensor(1 << 20, n=-1)]) == SHAPE and adamw([tensor(1 << 20, n=(1 << 40) + 1)]) == SHAPE and adamw([tensor(1 << 20, n=(1 << 35) + 1)]) == SHAPE
     for twice in (one, tensor((1 << 20) + 4 * 99), tensor(1 << 24, m=(1 << 20) + 4 * 150), tensor(1 << 24, v=1 << 20)):
         assert adamw([one, twice]) == ARGUMENT and b"twice" in _lib.lib().pk_last_error()
     # scales of two tensors that meet, copies that do

@@ -822,6 +822,44 @@ def test_losses_past_2_to_the_31(pk):
     assert torch.equal(pk.ops.token_logprobs_bwd(d, t, lse, w, out=d)[-tail:], pk.ops.token_logprobs_bwd(last, *cut(t, lse, w)))
 
 
+def test_losses_of_more_rows_than_a_launch_has_threads_for(pk):
+    """2^26 rows and three: each entry's rows are those of calls on a few of them, at both ends, around every 2^22 and between; every other row's against 64 bits."""
+    rows, vocab = 2 ** 26 + 3, 3
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(rows, vocab, generator=g, device="cuda", dtype=FP32).to(BF16)
+    t = torch.randint(-1, vocab, (rows,), generator=g, device="cuda").to(torch.int32)
+    old, adv, w = torch.full((rows,), -1.0, device="cuda"), torch.randn(rows, generator=g, device="cuda"), torch.rand(rows, generator=g, device="cuda") / rows
+    some = sorted({min(max(k * 2 ** 22 + o, 0), rows - 8) for k in range(17) for o in range(-40, 41, 8)} | {12345678})
+    part = torch.cat([torch.arange(r, r + 8, device="cuda") for r in some])
+    few = [y[part] for y in (x, t, old, adv, w)]
+    logp, lse = pk.ops.token_logprobs_fwd(x, t)
+    want = pk.ops.token_logprobs_fwd(few[0], few[1])
+    assert torch.equal(logp[part], want[0]) and torch.equal(lse[part], want[1])
+    for r in range(0, rows, 2 ** 24):
+        z = x[r:r + 2 ** 24].double()
+        used = t[r:r + 2 ** 24] >= 0
+        wl = torch.where(used, torch.logsumexp(z, 1), 0.0)
+        wp = torch.where(used, z.gather(1, t[r:r + 2 ** 24].clamp(min=0).long()[:, None])[:, 0] - wl, 0.0)
+        within("logp", logp[r:r + 2 ** 24], wp, U * wp.abs() + logp_slack(z, vocab))
+    d = pk.ops.token_logprobs_bwd(x, t, lse, adv)
+    assert torch.equal(d[part], pk.ops.token_logprobs_bwd(few[0], few[1], want[1], few[3]))
+    loss, d, logp = pk.blockops.policy_loss(x, t, old, adv, w)
+    want = pk.blockops.policy_loss(*few)
+    assert torch.equal(d[part], want[1]) and torch.equal(logp[part], want[2])
+    each = torch.where(t >= 0, -torch.minimum(torch.exp(logp.double() + 1) * adv, torch.exp(logp.double() + 1).clamp(0.8, 1.2) * adv) * w, 0.0)
+    within("loss", loss, each.sum(), U * each.abs().sum() * 8)
+    starts = torch.tensor([0, rows // 4, rows // 2, 3 * (rows // 4), rows], dtype=torch.int32, device="cuda")
+    loss, d, margins, logp = pk.blockops.preference_loss(x, t, starts, old, beta=2.0 ** -12)
+    within("margins", margins, torch.stack([sum((1 - 2 * k) * ((logp.double() + 1) * (t >= 0))[starts[i + 2 * k]:starts[i + 2 * k + 1]].sum() for k in range(2)) for i in range(2)]) * 2.0 ** -12,
+           rows / 4 * 2.0 ** -12 * 4 * U)
+    want = pk.ops.token_logprobs_bwd(*few[:2], pk.ops.token_logprobs_fwd(*few[:2])[1], torch.where(part < rows // 2, 1.0, -1.0).contiguous())
+    slope = [torch.sigmoid(-margins[i].double()) * 2.0 ** -13 for i in range(2)]
+    which = sum((part >= int(s)).long() for s in starts[1:4]) % 2
+    want = -want.double() * torch.where(which == 0, slope[0], slope[1])[:, None]
+    within("dlogits", d[part], want, want.abs() * 3 * HALF[BF16] + 1e-37)
+    assert bool(torch.isfinite(loss))
+
+
 def test_adamw_many_past_2_to_the_31(pk):
     """One tensor of more than 2^31 elements with 8-bit moments: the last block's values and codes, whose draws come from the element's place."""
     n, tail = 2 ** 31 + 700, 700
