@@ -24,8 +24,6 @@ namespace pk {
 namespace {
 
 constexpr int BLOCK = 256, NT = 256, WAVES = NT / 64;  // elements that share a scale; a wavefront takes a block
-constexpr int BLOCKS_PER_WG = 16;
-constexpr int MAX_TENSORS = 58;  // of one launch: the table travels in the kernel's arguments (4 KB at most)
 
 struct One {
     float* p;
@@ -35,17 +33,54 @@ struct One {
     uint16_t* copy;
     int64_t n;
 };
+// The list travels in the kernel's arguments, 4 KB at most, addresses in 48 bits: 126 tensors with moments in 32 bits, 58 in whole words (a launch is 4 us of the
+// host's: 96 tensors 13.8 -> 11.0 us).
+template <int PTRS>  // addresses of a tensor
 struct Table {
-    One t[MAX_TENSORS];
-    int first[MAX_TENSORS];  // a tensor's first workgroup
-    int count, place;        // tensors, the first one's place in the caller's list
+    static constexpr int MOST = (4096 - 64) / (8 + 4 * PTRS + 4 * ((PTRS + 1) / 2));
+    uint64_t size[MOST];  // elements, 40 bits; the tensor's first workgroup above
+    uint32_t low[MOST][PTRS], high[MOST][(PTRS + 1) / 2];
+    int count, place;  // tensors, the first one's place in the caller's list
     uint32_t seed;
+    int per;  // blocks of a workgroup
+    void put(int j, int64_t n, int64_t first, std::initializer_list<const void*> at) {
+        size[j] = static_cast<uint64_t>(n) | static_cast<uint64_t>(first) << 40;
+        int k = 0;
+        for (const void* p : at) {
+            const uint64_t u = reinterpret_cast<uint64_t>(p);
+            const uint32_t top = static_cast<uint32_t>(u >> 32);
+            low[j][k] = static_cast<uint32_t>(u);
+            high[j][k / 2] = k % 2 ? high[j][k / 2] | top << 16 : top;
+            ++k;
+        }
+    }
+    __device__ int64_t elements(int j) const { return static_cast<int64_t>(size[j] & ((uint64_t{1} << 40) - 1)); }
+    __device__ int first(int j) const { return static_cast<int>(size[j] >> 40); }
+    template <typename T>
+    __device__ T* at(int j, int k) const {
+        return reinterpret_cast<T*>(static_cast<uint64_t>(low[j][k]) | static_cast<uint64_t>(high[j][k / 2] >> (k % 2 * 16) & 0xFFFFu) << 32);
+    }
+    // The tensor that a workgroup belongs to: the last one whose first workgroup is not behind it (one without elements has no workgroup of its own).
+    __device__ int tensor_of(int group) const {
+        int lo = 0, hi = count - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) / 2;
+            if (first(mid) <= group)
+                lo = mid;
+            else
+                hi = mid - 1;
+        }
+        return lo;
+    }
 };
+constexpr int pointers(bool eight, bool copy) { return 4 + (eight ? 2 : 0) + (copy ? 1 : 0); }
 struct Step {
     float lr, b1, b2, rest1, rest2, eps, wd, per_c1, per_c2;  // 1 / c1, 1 / c2
     const float* factor;                                       // what the gradients are multiplied by, or null
 };
-static_assert(sizeof(Table) + sizeof(Step) <= 4096, "kernel arguments");
+static_assert(sizeof(Table<4>) + sizeof(Step) <= 4096 && sizeof(Table<5>) + sizeof(Step) <= 4096 && sizeof(Table<6>) + sizeof(Step) <= 4096 &&
+                  sizeof(Table<7>) + sizeof(Step) <= 4096 && sizeof(Table<1>) + 8 <= 4096,
+              "kernel arguments");
 
 // The low 32 bits scrambled: two multiplications by the fractions of the square roots of 3 and 2, shifts between them.
 __host__ __device__ inline uint32_t mix(uint32_t x) {
@@ -243,26 +278,16 @@ __device__ inline bool aligned_for_whole(const One& t) {
     return (sixteen & 15) == 0 && (eight & 7) == 0 && (quad & 3) == 0;
 }
 
-// The tensor that a workgroup belongs to: the last one whose first workgroup is not behind it (one without elements has no workgroup of its own).
-__device__ inline int tensor_of(const int* first, int count, int group) {
-    int lo = 0, hi = count - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) / 2;
-        if (first[mid] <= group)
-            lo = mid;
-        else
-            hi = mid - 1;
-    }
-    return lo;
-}
 __host__ __device__ inline uint32_t key_of(uint32_t seed, int place) { return mix(seed * 0x9E3779B9u + mix(static_cast<uint32_t>(place) + 0x3C6EF373u)); }
 
-template <typename G, bool EIGHT>
-__global__ __launch_bounds__(NT) void adamw_many_k(Table tab, Step s) {
-    const int group = blockIdx.x, j = tensor_of(tab.first, tab.count, group);
-    const One t = tab.t[j];
+template <typename G, bool EIGHT, bool COPY>
+__global__ __launch_bounds__(NT) void adamw_many_k(Table<pointers(EIGHT, COPY)> tab, Step s) {
+    const int group = blockIdx.x, j = tab.tensor_of(group);
+    One t{tab.template at<float>(j, 0), tab.template at<const void>(j, 1), tab.template at<void>(j, 2), tab.template at<void>(j, 3), nullptr, nullptr, nullptr, tab.elements(j)};
+    if constexpr (EIGHT) t.ms = tab.template at<float>(j, 4), t.vs = tab.template at<float>(j, 5);
+    if constexpr (COPY) t.copy = tab.template at<uint16_t>(j, EIGHT ? 6 : 4);
     const int64_t blocks = (t.n + BLOCK - 1) / BLOCK, whole = aligned_for_whole<G, EIGHT>(t) ? t.n / BLOCK : 0;
-    const int64_t begin = static_cast<int64_t>(group - tab.first[j]) * BLOCKS_PER_WG, end = min(begin + BLOCKS_PER_WG, blocks);
+    const int64_t begin = static_cast<int64_t>(group - tab.first(j)) * tab.per, end = min(begin + tab.per, blocks);
     const uint32_t key = key_of(tab.seed, tab.place + j);
     const float gs = s.factor ? *s.factor : 1.0f;
     __shared__ float table[EIGHT ? NT : 1];
@@ -278,20 +303,14 @@ __global__ __launch_bounds__(NT) void adamw_many_k(Table tab, Step s) {
 
 // Sums of the gradients' squares in 64 bits, one to a workgroup.
 constexpr int SQ_ELEMS = 16384;  // of one tensor that a workgroup takes
-struct Squares {
-    const void* g[MAX_TENSORS];
-    int64_t n[MAX_TENSORS];
-    int first[MAX_TENSORS];
-    int count;
-};
 template <typename G>
-__global__ __launch_bounds__(NT) void squares_k(Squares tab, double* part) {
+__global__ __launch_bounds__(NT) void squares_k(Table<1> tab, double* part) {
     constexpr int N = 16 / sizeof(G), U = 4;
     __shared__ double sh[WAVES];
-    const int group = blockIdx.x, j = tensor_of(tab.first, tab.count, group);
-    const int64_t begin = static_cast<int64_t>(group - tab.first[j]) * SQ_ELEMS;
-    const int count = static_cast<int>(min(tab.n[j] - begin, static_cast<int64_t>(SQ_ELEMS)));
-    const G* g = static_cast<const G*>(tab.g[j]) + begin;
+    const int group = blockIdx.x, j = tab.tensor_of(group);
+    const int64_t begin = static_cast<int64_t>(group - tab.first(j)) * SQ_ELEMS;
+    const int count = static_cast<int>(min(tab.elements(j) - begin, static_cast<int64_t>(SQ_ELEMS)));
+    const G* g = tab.template at<const G>(j, 0) + begin;
     double q[4] = {0.0, 0.0, 0.0, 0.0};  // chains of additions
     int from = 0;
     if ((reinterpret_cast<uintptr_t>(g) & 15) == 0) {  // 16 bytes a lane, four loads on their way
@@ -386,6 +405,42 @@ bool meet(const pk_adamw_tensor* t, int count, bool eight) {
     return false;
 }
 
+// Blocks that a workgroup takes. In 32 bits one to a wavefront: 96 tensors of 60000 elements 25.2 us, by 16 27.5; 35 M elements 147 and 154. In 8 bits a workgroup forms the
+// powers first, so it takes more where there are enough: 0.5 M elements 8.7 us by 4, 12.5 by 16; 5.8 M 22.9 by 4, 22.1 by 8, 25.5 by 16; 8 M 22.8 by 8, 23.0 by 16;
+// 35 M 99, 88 and 85; 120 M 328, 291 and 280.
+template <bool EIGHT>
+int blocks_of_group(int64_t blocks) {
+    if (!EIGHT) return blocks < (1 << 25) ? 4 : 16;  // a launch's threads are counted in 32 bits
+    return blocks <= 4 * 4096 ? 4 : blocks <= 8 * 4096 ? 8 : 16;
+}
+template <typename G, bool EIGHT, bool COPY>
+int launch(const pk_adamw_tensor* t, int count, uint32_t seed, const Step& s, hipStream_t st) {
+    int64_t blocks = 0;
+    for (int i = 0; i < count; ++i) blocks += (t[i].n + BLOCK - 1) / BLOCK;
+    const int per = blocks_of_group<EIGHT>(blocks);
+    for (int i = 0; i < count;) {
+        using List = Table<pointers(EIGHT, COPY)>;
+        List tab;
+        int64_t groups = 0;
+        tab.place = i, tab.seed = seed, tab.per = per;
+        for (tab.count = 0; i < count && tab.count < List::MOST; ++i, ++tab.count) {
+            const pk_adamw_tensor& x = t[i];
+            if constexpr (EIGHT && COPY)
+                tab.put(tab.count, x.n, groups, {x.p, x.g, x.m, x.v, x.m_scale, x.v_scale, x.copy});
+            else if constexpr (EIGHT)
+                tab.put(tab.count, x.n, groups, {x.p, x.g, x.m, x.v, x.m_scale, x.v_scale});
+            else if constexpr (COPY)
+                tab.put(tab.count, x.n, groups, {x.p, x.g, x.m, x.v, x.copy});
+            else
+                tab.put(tab.count, x.n, groups, {x.p, x.g, x.m, x.v});
+            groups += (x.n + BLOCK * per - 1) / (BLOCK * per);
+        }
+        if (groups == 0) continue;
+        adamw_many_k<G, EIGHT, COPY><<<dim3(static_cast<unsigned>(groups)), NT, 0, st>>>(tab, s);
+        if (int rc = launched()) return rc;
+    }
+    return PK_OK;
+}
 template <typename G>
 int run(const pk_adamw_tensor* t, int count, const pk_adamw_config* c, void* workspace, float* norm, hipStream_t st) {
     Step s;
@@ -399,10 +454,10 @@ int run(const pk_adamw_tensor* t, int count, const pk_adamw_config* c, void* wor
         double* part = reinterpret_cast<double*>(static_cast<char*>(workspace) + 256);
         int64_t parts = 0;
         for (int i = 0; i < count;) {
-            Squares q;
+            Table<1> q;
             int64_t groups = 0;
-            for (q.count = 0; i < count && q.count < MAX_TENSORS; ++i, ++q.count) {
-                q.first[q.count] = static_cast<int>(groups), q.g[q.count] = t[i].g, q.n[q.count] = t[i].n;
+            for (q.count = 0; i < count && q.count < Table<1>::MOST; ++i, ++q.count) {
+                q.put(q.count, t[i].n, groups, {t[i].g});
                 groups += (t[i].n + SQ_ELEMS - 1) / SQ_ELEMS;
             }
             if (groups == 0) continue;
@@ -414,23 +469,10 @@ int run(const pk_adamw_tensor* t, int count, const pk_adamw_config* c, void* wor
         if (int rc = launched()) return rc;
         s.factor = factor;
     }
-    for (int i = 0; i < count;) {
-        Table tab;
-        int64_t groups = 0;
-        tab.place = i, tab.seed = c->seed;
-        for (tab.count = 0; i < count && tab.count < MAX_TENSORS; ++i, ++tab.count) {
-            tab.first[tab.count] = static_cast<int>(groups);
-            tab.t[tab.count] = One{t[i].p, t[i].g, t[i].m, t[i].v, t[i].m_scale, t[i].v_scale, static_cast<uint16_t*>(t[i].copy), t[i].n};
-            groups += (t[i].n + BLOCK * BLOCKS_PER_WG - 1) / (BLOCK * BLOCKS_PER_WG);
-        }
-        if (groups == 0) continue;
-        if (c->state_bits == 8)
-            adamw_many_k<G, true><<<dim3(static_cast<unsigned>(groups)), NT, 0, st>>>(tab, s);
-        else
-            adamw_many_k<G, false><<<dim3(static_cast<unsigned>(groups)), NT, 0, st>>>(tab, s);
-        if (int rc = launched()) return rc;
-    }
-    return PK_OK;
+    bool copies = false;
+    for (int i = 0; i < count; ++i) copies = copies || t[i].copy;
+    if (c->state_bits == 8) return copies ? launch<G, true, true>(t, count, c->seed, s, st) : launch<G, true, false>(t, count, c->seed, s, st);
+    return copies ? launch<G, false, true>(t, count, c->seed, s, st) : launch<G, false, false>(t, count, c->seed, s, st);
 }
 
 }  // namespace
@@ -460,6 +502,9 @@ int pk_adamw_many(const pk_adamw_tensor* t, int count, const pk_adamw_config* c,
             if (t[i].n < 0 || total > (int64_t{1} << 35)) return fail(PK_ERR_SHAPE, "pk_adamw_many: a tensor's size is out of range");
             if (t[i].n > 0 && (!t[i].p || !t[i].g || !t[i].m || !t[i].v || (c->state_bits == 8 && (!t[i].m_scale || !t[i].v_scale))))
                 return fail(PK_ERR_ARGUMENT, "pk_adamw_many: null pointer");
+            for (const void* p : {static_cast<const void*>(t[i].p), t[i].g, static_cast<const void*>(t[i].m), static_cast<const void*>(t[i].v), static_cast<const void*>(t[i].m_scale),
+                                  static_cast<const void*>(t[i].v_scale), static_cast<const void*>(t[i].copy)})
+                if (reinterpret_cast<uint64_t>(p) >> 48) return fail(PK_ERR_ARGUMENT, "pk_adamw_many: an address past 48 bits");
         }
         if (meet(t, count, c->state_bits == 8)) return fail(PK_ERR_ARGUMENT, "pk_adamw_many: a parameter, state or copy is in the list twice");
         if (clip && !norm) return fail(PK_ERR_ARGUMENT, "pk_adamw_many: a clip writes the norm");

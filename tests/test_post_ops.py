@@ -147,6 +147,7 @@ def test_adamw_many_refuses_tables():
     assert adamw([tensor(1 << 20, n=-1)]) == SHAPE and adamw([tensor(1 << 20, n=(1 << 40) + 1)]) == SHAPE and adamw([tensor(1 << 20, n=(1 << 35) + 1)]) == SHAPE
     for twice in (one, tensor((1 << 20) + 4 * 99), tensor(1 << 24, m=(1 << 20) + 4 * 150), tensor(1 << 24, v=1 << 20)):
         assert adamw([one, twice]) == ARGUMENT and b"twice" in _lib.lib().pk_last_error()
+    assert adamw([tensor(1 << 48)]) == ARGUMENT and b"48 bits" in _lib.lib().pk_last_error()
     # scales of two tensors that meet, copies that do
     assert adamw([one, tensor(1 << 24, scales=(1 << 31) + 4)], state_bits=8) == ARGUMENT
     assert adamw([tensor(1 << 20, copy=1 << 33), tensor(1 << 24, copy=(1 << 33) + 198)]) == ARGUMENT

@@ -759,6 +759,34 @@ def test_adamw_many_skips_what_has_no_gradient(pk):
         assert torch.equal(a[i], b[i]) and torch.equal(sa.m[i].view(torch.uint8), sb.m[i].view(torch.uint8)) and torch.equal(sa.v_scale[i], sb.v_scale[i])
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_many_does_not_depend_on_how_a_list_is_dealt(pk, bits):
+    """A tensor's bits beside others of any number and size, in one launch or several, with bf16 copies or without."""
+    g = torch.Generator(device="cuda").manual_seed(9)
+    grads = [torch.randn(n, generator=g, device="cuda") for n in [70000] + [1 + 37 * k for k in range(260)]]
+
+    def run(n_more, large, copies):
+        gs = grads[:1 + n_more] + ([torch.ones(large, device="cuda")] if large else [])
+        ps = [torch.zeros_like(y) for y in gs]
+        state = pk.blockops.adamw_state(ps, bits)
+        out = [torch.empty_like(y, dtype=BF16) for y in ps] if copies else None
+        for t in (1, 2):
+            norm = pk.blockops.adamw_many_(ps, gs, state, 0.01, t=t, max_norm=1e9, copies=out, seed=t)
+        assert abs(float(norm) - math.sqrt(sum(float((y.double() ** 2).sum()) for y in gs))) <= 2 * U * float(norm)
+        if copies:
+            assert all(torch.equal(a, b.to(BF16)) for a, b in zip(out, ps))
+        return [[y.view(torch.uint8) for y in x[:1 + n_more]] for x in (ps, state.m, state.v)]
+
+    want = run(0, 0, False)
+    for n_more, large, copies in ((0, 0, True), (260, 0, False), (260, 0, True), (3, 5 * 10 ** 6, False), (3, 9 * 10 ** 6, True)):
+        got = run(n_more, large, copies)
+        assert all(torch.equal(a[0], b[0]) for a, b in zip(got, want)), (n_more, large, copies)
+        if (n_more, copies) == (260, False):
+            long = got
+        elif n_more:
+            assert all(torch.equal(a, b) for x, y in zip(got, long) for a, b in zip(x, y))
+
+
 def test_adamw_many_is_adamw_and_clip(pk):
     """32-bit states against `clip_grad_norm_` and `adamw_` one tensor at a time: the formula is the same, its roundings differ (16 u of the update)."""
     g = torch.Generator(device="cuda").manual_seed(8)
