@@ -487,14 +487,99 @@ __global__ __launch_bounds__(64) void rows_join(Loss a, int count, const float2*
     if (lane == 0) finish<LOGP>(a, r, t < a.vocab ? elem(x, t) : NAN, row_sum(top, sum));
 }
 
-// The gradient of rows whose sums are known: every element by itself, so a row may be dealt to several workgroups (grid.y, `per` pieces each) and written over.
+// ---- pairs of sequences -----------------------------------------------------------------------------------------------------
+struct Pairs {
+    const int* starts;  // 2 pairs + 1
+    const int* targets;
+    const double* logp;
+    const float* ref;
+    float *coef, *margins;
+    double* losses;
+    int64_t rows;
+    int pairs;
+    float beta, smoothing, upstream;
+};
+struct PairOut {
+    double margin, loss;
+    float slope;  // of the chosen answer's log-probability; the rejected one's is its negative
+};
+__device__ inline PairOut pair_terms(const Pairs& a, double chosen, double rejected) {
+    const double u = a.beta * (chosen - rejected), e = a.smoothing;
+    const double small = exp(-fabs(u)), up = 1.0 / (1.0 + small), down = small / (1.0 + small);  // sigma(|u|), sigma(-|u|)
+    const double yes = u >= 0.0 ? up : down, no = u >= 0.0 ? down : up;                          // sigma(u), sigma(-u); no number stays none
+    const double tail = log1p(small), lost_no = fmax(-u, 0.0) + tail, lost_yes = fmax(u, 0.0) + tail;  // -log sigma(u), -log sigma(-u)
+    // a weight of zero drops its term, also an infinite one (a word without probability in an answer)
+    return PairOut{u, u != u ? u : (e < 1.0 ? (1.0 - e) * lost_no : 0.0) + (e > 0.0 ? e * lost_yes : 0.0),
+                   static_cast<float>((e * yes - (1.0 - e) * no) * a.beta * a.upstream / a.pairs)};
+}
+__device__ inline int64_t start_of(const Pairs& a, int seq) { return min(max(static_cast<int64_t>(a.starts[seq]), int64_t{0}), a.rows); }  // offsets that lie are held to the rows there are
+// What a sequence's rows from `begin` on give to its sum, to lane l of n; four rows' loads on their way together.
+__device__ inline double sequence_part(const Pairs& a, int64_t begin, int64_t end, int l, int n) {
+    double s = 0.0;
+    for (int64_t r0 = begin + l; r0 < end; r0 += 4 * n) {
+        double logp[4];
+        float ref[4];
+        bool counts[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int64_t r = min(r0 + k * n, end - 1);
+            counts[k] = a.targets[r] >= 0 && r0 + k * n < end, logp[k] = a.logp[r], ref[k] = a.ref[r];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s += counts[k] ? logp[k] - static_cast<double>(ref[k]) : 0.0;
+    }
+    return s;
+}
+__device__ inline double wave_sum(double s) {
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o);
+    return s;
+}
+// A few short pairs are formed by who wants them: a wavefront, or a workgroup.
+__device__ inline PairOut pair_of_wave(const Pairs& a, int pair) {
+    const int lane = threadIdx.x & 63;
+    const double chosen = sequence_part(a, start_of(a, pair), start_of(a, pair + 1), lane, 64);
+    const double rejected = sequence_part(a, start_of(a, a.pairs + pair), start_of(a, a.pairs + pair + 1), lane, 64);
+    return pair_terms(a, wave_sum(chosen), wave_sum(rejected));
+}
+// Row r's sequence, or -1.
+__device__ inline int sequence_of(const Pairs& a, int64_t r) {
+    const int lane = threadIdx.x & 63;
+    const uint64_t in = __ballot(lane < 2 * a.pairs && start_of(a, lane) <= r && r < start_of(a, lane < 2 * a.pairs ? lane + 1 : 0));
+    return in ? 63 - __builtin_clzll(in) : -1;
+}
+template <int NT>
+__device__ inline void few_pairs_mean(const Pairs& a, float* mean) {
+    __shared__ double sh[NT / 64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    double s = 0.0;
+    for (int p = wave; p < a.pairs; p += NT / 64) {
+        const PairOut o = pair_of_wave(a, p);
+        if (lane == 0) a.margins[p] = static_cast<float>(o.margin);
+        s += o.loss;
+    }
+    if (lane == 0) sh[wave] = s;
+    __syncthreads();
+    s = sh[0];
+#pragma unroll
+    for (int w = 1; w < NT / 64; ++w) s += sh[w];
+    if (threadIdx.x == 0) *mean = static_cast<float>(s / a.pairs);
+}
+
+// ---- the gradient of rows whose sums are known --------------------------------------------------------------------------------
+// Every element by itself, so a row may be dealt to several workgroups (grid.y, `per` pieces each) and written over.
+// FEW: the rows' coefficients are formed here, from the pairs.
 constexpr int GRAD_NT = 512, GRAD_U = 8;
-template <typename T, bool PAST>
-__global__ __launch_bounds__(GRAD_NT) void rows_grad(Loss a, int per) {
+template <typename T, bool PAST, bool FEW>
+__global__ __launch_bounds__(GRAD_NT) void rows_grad(Loss a, int per, Pairs pairs) {
     constexpr int N = Piece<T>::N;
     __shared__ float sh_m[GRAD_NT / 64], sh_s[GRAD_NT / 64];
     if (blockIdx.x == a.rows) {
-        if (blockIdx.y == 0) pairs_mean<GRAD_NT>(a);
+        if (blockIdx.y != 0) return;
+        if constexpr (FEW)
+            few_pairs_mean<GRAD_NT>(pairs, a.loss);
+        else
+            pairs_mean<GRAD_NT>(a);
         return;
     }
     const int64_t r = a.rows - 1 - blockIdx.x;  // the last rows first: they are what the pass before has left in the last-level cache
@@ -504,7 +589,18 @@ __global__ __launch_bounds__(GRAD_NT) void rows_grad(Loss a, int per) {
     const Cut<T> cut(x, V);
     const int from = static_cast<int>(blockIdx.y) * per, to = min(cut.pieces, from + per);
     const bool edges = blockIdx.y == 0 && tid < cut.edges;
-    const float s2 = a.scale * LOG2E, given = a.coef[r] * a.scale;
+    float given = 0.0f;
+    if constexpr (FEW) {
+        const int seq = t < 0 ? -1 : sequence_of(pairs, r);
+        if (seq >= 0) {
+            const bool rejected = seq >= pairs.pairs;
+            const float slope = pair_of_wave(pairs, rejected ? seq - pairs.pairs : seq).slope;
+            given = (rejected ? -slope : slope) * a.scale;
+        }
+    } else {
+        given = a.coef[r] * a.scale;
+    }
+    const float s2 = a.scale * LOG2E;
     if (t < 0 || given == 0.0f) {
         for (int p = from + tid; p < to; p += GRAD_NT) store_piece<PAST>(dx + cut.head + p * N, Piece<T>{{0, 0, 0, 0}});
         if (edges) put(dx, cut.edge(tid), 0.0f);
@@ -549,31 +645,17 @@ __global__ __launch_bounds__(1024) void loss_sum(const double* x, int64_t n, flo
     if (threadIdx.x == 0) *out = static_cast<float>(s);
 }
 
-struct Pairs {
-    const int* starts;  // 2 pairs + 1
-    const int* targets;
-    const double* logp;
-    const float* ref;
-    float *coef, *margins;
-    double* losses;
-    int64_t rows;
-    int pairs;
-    float beta, smoothing, upstream;
-};
 // A workgroup takes a pair: both sequences' sums, the pair's loss, and for every row of the two what its gradient is multiplied by.
 constexpr int PAIR_NT = 1024;
 __global__ __launch_bounds__(PAIR_NT) void pair_loss(Pairs a) {
     __shared__ double sh[2][PAIR_NT / 64];
     const int tid = threadIdx.x, seq[2] = {static_cast<int>(blockIdx.x), a.pairs + static_cast<int>(blockIdx.x)};
     int64_t begin[2], end[2];
-    double sum[2] = {0.0, 0.0};
+    double sum[2];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {  // offsets that lie are held to the rows there are
-        begin[k] = min(max(static_cast<int64_t>(a.starts[seq[k]]), int64_t{0}), a.rows);
-        end[k] = min(max(static_cast<int64_t>(a.starts[seq[k] + 1]), int64_t{0}), a.rows);
-        for (int64_t r = begin[k] + tid; r < end[k]; r += PAIR_NT)
-            if (a.targets[r] >= 0) sum[k] += a.logp[r] - static_cast<double>(a.ref[r]);
-        for (int o = 32; o >= 1; o >>= 1) sum[k] += __shfl_xor(sum[k], o);
+    for (int k = 0; k < 2; ++k) {
+        begin[k] = start_of(a, seq[k]), end[k] = start_of(a, seq[k] + 1);
+        sum[k] = wave_sum(sequence_part(a, begin[k], end[k], tid, PAIR_NT));
         if ((tid & 63) == 0) sh[k][tid >> 6] = sum[k];
     }
     __syncthreads();
@@ -582,19 +664,11 @@ __global__ __launch_bounds__(PAIR_NT) void pair_loss(Pairs a) {
         sum[k] = 0.0;
         for (int w = 0; w < PAIR_NT / 64; ++w) sum[k] += sh[k][w];
     }
-    const double u = a.beta * (sum[0] - sum[1]), e = a.smoothing;
-    const double small = exp(-fabs(u)), up = 1.0 / (1.0 + small), down = small / (1.0 + small);  // sigma(|u|), sigma(-|u|)
-    const double yes = u >= 0.0 ? up : down, no = u >= 0.0 ? down : up;                          // sigma(u), sigma(-u); no number stays none
-    const double tail = log1p(small), lost_no = fmax(-u, 0.0) + tail, lost_yes = fmax(u, 0.0) + tail;  // -log sigma(u), -log sigma(-u)
-    const float slope = static_cast<float>((e * yes - (1.0 - e) * no) * a.beta * a.upstream / a.pairs);
-    if (tid == 0) {
-        a.margins[blockIdx.x] = static_cast<float>(u);
-        // a weight of zero drops its term, also an infinite one (a word without probability in an answer)
-        a.losses[blockIdx.x] = u != u ? u : (e < 1.0 ? (1.0 - e) * lost_no : 0.0) + (e > 0.0 ? e * lost_yes : 0.0);
-    }
+    const PairOut o = pair_terms(a, sum[0], sum[1]);
+    if (tid == 0) a.margins[blockIdx.x] = static_cast<float>(o.margin), a.losses[blockIdx.x] = o.loss;
 #pragma unroll
     for (int k = 0; k < 2; ++k)
-        for (int64_t r = begin[k] + tid; r < end[k]; r += PAIR_NT) a.coef[r] = k ? -slope : slope;
+        for (int64_t r = begin[k] + tid; r < end[k]; r += PAIR_NT) a.coef[r] = k ? -o.slope : o.slope;
 }
 
 // From here on logits and gradient do not stay in the 256 MB of the last-level cache together. A gradient that passes it by leaves it to the logits, which the
@@ -632,7 +706,7 @@ int parts_of_rows(int64_t rows, int64_t vocab, int64_t es) {
     return static_cast<int>(std::min<int64_t>(std::min<int64_t>(MOST_PARTS, 512 / rows), pieces / (2 * PART_NT)));
 }
 template <typename T, Mode MODE>
-void launch_typed(const Loss& a, hipStream_t st) {
+void launch_typed(const Loss& a, const Pairs* pairs, hipStream_t st) {
     const bool past = a.rows * a.vocab * static_cast<int64_t>(sizeof(T)) >= PAST_BYTES;
     const dim3 grid(static_cast<unsigned>(a.rows + (a.loss ? 1 : 0)));
     if constexpr (MODE == LOGP) {
@@ -648,7 +722,10 @@ void launch_typed(const Loss& a, hipStream_t st) {
             const int pieces = a.vocab / Piece<T>::N, most = static_cast<int>(std::max<int64_t>(1, 512 / std::max<int64_t>(a.rows, 1)));
             const int parts = std::min(most, std::max(1, pieces / GRAD_NT)), per = (pieces + parts - 1) / parts;
             const dim3 dealt(grid.x, static_cast<unsigned>(parts));
-            past ? rows_grad<T, true><<<dealt, GRAD_NT, 0, st>>>(a, per) : rows_grad<T, false><<<dealt, GRAD_NT, 0, st>>>(a, per);
+            if (pairs)
+                rows_grad<T, false, true><<<dealt, GRAD_NT, 0, st>>>(a, per, *pairs);
+            else
+                past ? rows_grad<T, true, false><<<dealt, GRAD_NT, 0, st>>>(a, per, Pairs{}) : rows_grad<T, false, false><<<dealt, GRAD_NT, 0, st>>>(a, per, Pairs{});
         } else
             past ? launch_held<T, MODE, true>(a, st) : launch_held<T, MODE, false>(a, st);
     }
@@ -656,7 +733,7 @@ void launch_typed(const Loss& a, hipStream_t st) {
 // A launch has fewer than 2^32 threads, 1024 for a row at most: more rows than that allows go in runs.
 constexpr int64_t MOST_ROWS = (1 << 22) - 2;
 template <Mode MODE>
-int launch_rows(const Loss& all, int dtype, hipStream_t st) {
+int launch_rows(const Loss& all, int dtype, hipStream_t st, const Pairs* pairs = nullptr) {
     if (all.rows == 0 && !all.loss) return PK_OK;
     for (int64_t r = 0; r == 0 || r < all.rows; r += MOST_ROWS) {
         const auto on = [r](auto*& p, int64_t ld = 1) { p = p ? p + r * ld : p; };
@@ -668,9 +745,9 @@ int launch_rows(const Loss& all, int dtype, hipStream_t st) {
         if (a.dlogits) a.dlogits = static_cast<char*>(a.dlogits) + r * a.dld * es;
         on(a.targets), on(a.logp), on(a.lse), on(a.lse_in), on(a.coef), on(a.clear), on(a.fine), on(a.old_logp), on(a.ref_logp), on(a.adv), on(a.weights), on(a.row_loss);
         if (dtype == PK_BF16)
-            launch_typed<uint16_t, MODE>(a, st);
+            launch_typed<uint16_t, MODE>(a, pairs, st);
         else
-            launch_typed<float, MODE>(a, st);
+            launch_typed<float, MODE>(a, pairs, st);
         if (int rc = launched()) return rc;
     }
     return PK_OK;
@@ -697,6 +774,10 @@ int check(const char* who, const void* logits, int64_t ld, const int* targets, i
     return PK_OK;
 }
 
+// Few pairs of few rows are formed by the gradient's own wavefronts, each the pair it wants: a launch less. bf16, with a launch of their own and without: 8 pairs of 4 + 4 rows of
+// 1000 words 10.6 and 7.9 us, one of 256 + 256 of 32000 25.5 and 23.5, 8 of 32 + 32 of 8000 13.6 and 12.7; past that 31 pairs of 4 + 4 11.5 and 14.4, one of 512 + 512 18.0 and 21.6.
+constexpr int MOST_FEW_PAIRS = 8, FEW_PAIRS_ROWS = 512;
+static_assert(2 * MOST_FEW_PAIRS < 64, "their starts fit into a wavefront");
 size_t pad(size_t bytes) { return (bytes + 255) & ~size_t{255}; }
 
 }  // namespace
@@ -797,11 +878,15 @@ int pk_preference_loss(const pk_preference_config* c, const void* logits, int64_
         a.logp = logp, a.lse = lse, a.fine = fine, a.clear = coef;
         if (rows < FEW_ROWS) a.parts = reinterpret_cast<float2*>(ws + 2 * singles + doubles + pad(sizeof(double) * static_cast<size_t>(pairs)));
         if (int rc = launch_rows<LOGP>(a, dtype, st)) return rc;
-        pair_loss<<<dim3(static_cast<unsigned>(pairs)), PAIR_NT, 0, st>>>(
-            Pairs{seq_start, targets, fine, ref_logp, coef, margins, losses, rows, static_cast<int>(pairs), c->beta, c->label_smoothing, c->upstream});
-        if (int rc = launched()) return rc;
-        a.dlogits = dlogits, a.dld = dld, a.lse_in = lse, a.coef = coef, a.losses = losses, a.pairs = pairs, a.loss = loss;
-        return launch_rows<GRAD>(a, dtype, st);
+        const Pairs p{seq_start, targets, fine, ref_logp, coef, margins, losses, rows, static_cast<int>(pairs), c->beta, c->label_smoothing, c->upstream};
+        a.dlogits = dlogits, a.dld = dld;
+        const bool few = rows <= FEW_PAIRS_ROWS && pairs <= MOST_FEW_PAIRS && same_cut(a, elem_size(dtype));
+        if (!few) {
+            pair_loss<<<dim3(static_cast<unsigned>(pairs)), PAIR_NT, 0, st>>>(p);
+            if (int rc = launched()) return rc;
+        }
+        a.lse_in = lse, a.coef = coef, a.losses = losses, a.pairs = pairs, a.loss = loss;
+        return launch_rows<GRAD>(a, dtype, st, few ? &p : nullptr);
     });
 }
 

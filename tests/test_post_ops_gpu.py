@@ -489,7 +489,8 @@ def test_policy_loss_of_nothing(pk):
 
 PAIRS = [  # lengths of chosen, lengths of rejected, rows behind, vocab, smoothing
     ([1], [1], 0, 50, 0.0), ([5, 0, 33], [7, 4, 0], 3, 1000, 0.1), ([300, 20], [17, 290], 0, 130, 0.0), ([9, 8, 7, 6], [1, 2, 3, 4], 1, 10007, 0.25),
-    ([3], [4], 0, 32000, 1.0), ([0], [0], 2, 64, 0.3), ([40], [41], 0, 4096, 0.5)]
+    ([3], [4], 0, 32000, 1.0), ([0], [0], 2, 64, 0.3), ([40], [41], 0, 4096, 0.5),
+    ([32] * 8, [32] * 8, 0, 700, 0.0), ([32] * 8, [32] * 8, 1, 700, 0.2), ([3] * 9, [4] * 9, 2, 3001, 0.1), ([255], [256], 1, 2000, 0.0), ([2000, 1, 0], [0, 900, 33], 9, 257, 0.1)]
 
 
 @pytest.mark.parametrize("dtype", [FP32, BF16], ids=["fp32", "bf16"])
@@ -529,6 +530,25 @@ def test_preference_loss_against_64_bits(pk, case, dtype):
     over = x.clone()
     res = pk.blockops.preference_loss(over, t, starts, ref, beta, e, scale, upstream, out=over)
     assert torch.equal(over, d) and torch.equal(res[0], loss)
+
+
+@pytest.mark.parametrize("ends", [(0, 60, 100, 160, 200), (5, 5, 5, 5, 5), (-9, 40, 190, 2 ** 31 - 1, -2 ** 31), (150, 100, 50, 0, 250)], ids=str)
+def test_preference_loss_a_launch_less_or_not(pk, ends):
+    """Two pairs formed by the gradient's wavefronts and by a launch of their own (into rows that lie otherwise): sums in 64 bits in another order, so a step of
+    32 bits in the margins, and offsets that lie held to the rows alike."""
+    x, t, g = loss_inputs(200, 900, FP32, 5)
+    t[::7] = -1
+    starts, ref = torch.tensor(ends, dtype=torch.int32, device="cuda"), -8 * torch.rand(200, generator=g, device="cuda")
+    a = pk.blockops.preference_loss(x, t, starts, ref, 0.3, 0.1)
+    b = pk.blockops.preference_loss(x, t, starts, ref, 0.3, 0.1, out=x.new_empty(200, 903)[:, 2:902])
+    assert torch.equal(a[3], b[3])
+    within("margins", a[2], b[2], 2 * U * b[2].abs() + 1e-37)
+    within("loss", a[0], b[0], 2 * U * (b[0].abs() + b[2].abs().sum()))
+    # softmax by another kernel: other orders of 32-bit sums
+    z = softmax64(x, t, 1.0)[0]
+    within("dlogits", a[1], b[1], (2 * (logp_slack(z, 900) + 4 * U * sizes(z)) * 0.15 + 4 * U)[:, None])
+    if sorted(ends) == list(ends):   # rows of no sequence
+        assert not a[1][ends[-1]:].any() and not a[1][:ends[0]].any()
 
 
 def test_preference_loss_far_margins_and_lying_offsets(pk):
