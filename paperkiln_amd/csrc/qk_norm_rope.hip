@@ -71,7 +71,7 @@ __device__ inline void columns(int p, int rotary, bool halves, int& a, int& b) {
     b = turned ? p + rotary / 2 : 2 * p + 1;
 }
 
-// Any even head size, any strides: a wavefront takes a row, a lane its pairs lane and lane + 64.
+// What the row kernels below do not serve: a wavefront takes a row, a lane its pairs lane and lane + 64.
 template <typename T>
 __global__ __launch_bounds__(NT) void qk_fwd_any(Qk a) {
     const int lane = threadIdx.x & 63, heads = a.Hq + a.Hkv, pairs = a.dk / 2;
@@ -178,7 +178,7 @@ __global__ __launch_bounds__(NT) void qk_bwd_any(Qk a) {
     }
 }
 
-// ---- rows of whole 16-byte pieces ------------------------------------------------------------------------------------------
+// ---- rows in 16-byte pieces ------------------------------------------------------------------------------------------
 // A group of G lanes takes a head's row, a lane eight of its columns as four pairs (a[i], b[i]): columns 8l .. 8l+7, or, where pairs come from two
 // halves, columns 4l .. and R/2 + 4l .., so that a pair never leaves its lane. A wavefront holds 64 / G rows of one token at a time and walks the
 // token's heads, queries and keys as one list. The angles are the token's: 64 lanes form one pair's each and hand them round through a strip of LDS.
@@ -186,19 +186,25 @@ __global__ __launch_bounds__(NT) void qk_bwd_any(Qk a) {
 struct Eight {  // vectors: as arrays the compiler kept half of one in LDS, by an offset that it read from the launch's packet in the host's memory (gqa forward 8.5 -> 22 us)
     f32x4 a, b;
 };
-template <typename T, bool HALVES>
+// Vectors that lie where their elements may. The hardware takes them anywhere; what it costs stands at `serve`.
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+typedef u32x2 u32x2_any __attribute__((aligned(2)));
+typedef f32x4 f32x4_any __attribute__((aligned(4)));
+template <typename T, bool HALVES, bool LOOSE>
 struct Cols;  // how a lane's columns are moved: two runs of four, c0 and c1 bytes behind the base
-template <bool HALVES>
-struct Cols<uint16_t, HALVES> {
+template <bool HALVES, bool LOOSE>
+struct Cols<uint16_t, HALVES, LOOSE> {
+    using Four = std::conditional_t<LOOSE, u32x4_any, u32x4>;
+    using Two = std::conditional_t<LOOSE, u32x2_any, u32x2>;
     struct Raw {
         u32x4 v;
     };
     __device__ static Raw load(const char* row, uint32_t c0, uint32_t c1) {
         if constexpr (HALVES) {
-            const u32x2 x = *reinterpret_cast<const u32x2*>(row + c0), y = *reinterpret_cast<const u32x2*>(row + c1);
+            const u32x2 x = *reinterpret_cast<const Two*>(row + c0), y = *reinterpret_cast<const Two*>(row + c1);
             return Raw{{x[0], x[1], y[0], y[1]}};
         } else {
-            return Raw{*reinterpret_cast<const u32x4*>(row + c0)};
+            return Raw{*reinterpret_cast<const Four*>(row + c0)};
         }
     }
     __device__ static Eight unpack(const Raw& r) {
@@ -218,21 +224,25 @@ struct Cols<uint16_t, HALVES> {
     }
     __device__ static void store(char* row, uint32_t c0, uint32_t c1, const Eight& e) {
         if constexpr (HALVES) {
-            *reinterpret_cast<u32x2*>(row + c0) = u32x2{pack_bf16(e.a[0], e.a[1]), pack_bf16(e.a[2], e.a[3])};
-            *reinterpret_cast<u32x2*>(row + c1) = u32x2{pack_bf16(e.b[0], e.b[1]), pack_bf16(e.b[2], e.b[3])};
+            *reinterpret_cast<Two*>(row + c0) = u32x2{pack_bf16(e.a[0], e.a[1]), pack_bf16(e.a[2], e.a[3])};
+            *reinterpret_cast<Two*>(row + c1) = u32x2{pack_bf16(e.b[0], e.b[1]), pack_bf16(e.b[2], e.b[3])};
         } else {
-            const uint32_t v0 = pack_bf16(e.a[0], e.b[0]), v1 = pack_bf16(e.a[1], e.b[1]), v2 = pack_bf16(e.a[2], e.b[2]), v3 = pack_bf16(e.a[3], e.b[3]);
-            store_through(reinterpret_cast<u32x4*>(row + c0), u32x4{v0, v1, v2, v3});  // whole lines: rows of 64 columns and more
+            const u32x4 v = {pack_bf16(e.a[0], e.b[0]), pack_bf16(e.a[1], e.b[1]), pack_bf16(e.a[2], e.b[2]), pack_bf16(e.a[3], e.b[3])};
+            if constexpr (LOOSE)
+                *reinterpret_cast<Four*>(row + c0) = v;
+            else
+                store_through(reinterpret_cast<u32x4*>(row + c0), v);  // whole lines: rows of 64 columns and more
         }
     }
 };
-template <bool HALVES>
-struct Cols<float, HALVES> {
+template <bool HALVES, bool LOOSE>
+struct Cols<float, HALVES, LOOSE> {
+    using Four = std::conditional_t<LOOSE, f32x4_any, f32x4>;
     struct Raw {
         f32x4 x, y;
     };
     __device__ static Raw load(const char* row, uint32_t c0, uint32_t c1) {
-        return Raw{*reinterpret_cast<const f32x4*>(row + c0), *reinterpret_cast<const f32x4*>(row + c1)};
+        return Raw{*reinterpret_cast<const Four*>(row + c0), *reinterpret_cast<const Four*>(row + c1)};
     }
     __device__ static Eight unpack(const Raw& r) {
         Eight e;
@@ -247,27 +257,79 @@ struct Cols<float, HALVES> {
     }
     __device__ static void store(char* row, uint32_t c0, uint32_t c1, const Eight& e) {
         if constexpr (HALVES) {
-            *reinterpret_cast<f32x4*>(row + c0) = f32x4{e.a[0], e.a[1], e.a[2], e.a[3]};
-            *reinterpret_cast<f32x4*>(row + c1) = f32x4{e.b[0], e.b[1], e.b[2], e.b[3]};
+            *reinterpret_cast<Four*>(row + c0) = f32x4{e.a[0], e.a[1], e.a[2], e.a[3]};
+            *reinterpret_cast<Four*>(row + c1) = f32x4{e.b[0], e.b[1], e.b[2], e.b[3]};
         } else {
-            *reinterpret_cast<f32x4*>(row + c0) = f32x4{e.a[0], e.b[0], e.a[1], e.b[1]};
-            *reinterpret_cast<f32x4*>(row + c1) = f32x4{e.a[2], e.b[2], e.a[3], e.b[3]};
+            *reinterpret_cast<Four*>(row + c0) = f32x4{e.a[0], e.b[0], e.a[1], e.b[1]};
+            *reinterpret_cast<Four*>(row + c1) = f32x4{e.a[2], e.b[2], e.a[3], e.b[3]};
         }
     }
 };
-// The two runs of four columns that lane l of a row's group holds.
-template <bool HALVES>
-__device__ inline void runs(int l, int rotary, int& c0, int& c1) {
-    const bool turned = HALVES && 8 * l < rotary;
-    c0 = turned ? 4 * l : 8 * l;
-    c1 = turned ? rotary / 2 + 4 * l : 8 * l + 4;
+// What lane l of a row's group holds: two runs of four columns from c0 and c1 on, pairs p0 .. p0 + 3 where they are turned.
+//
+// LOOSE: any even head size from 8 on, any number of turned columns. A run that would pass its end is moved back to it, so the lane holds columns of its neighbour's, too:
+// those count in no sum (ka, kb 0), and are not stored. With pairs of halves the turned columns and those behind them are dealt out one after the other.
+template <bool LOOSE>
+struct Share {
+    int c0, c1, p0;
+    bool mine;
+};
+template <>
+struct Share<true> : Share<false> {
+    f32x4 ka, kb;
+    bool whole;
+};
+__host__ __device__ inline int turned_lanes(int rotary) { return (rotary + 7) / 8; }
+__host__ __device__ inline int lanes_wanted(int dk, int rotary, bool halves) { return halves ? turned_lanes(rotary) + (dk - rotary + 7) / 8 : (dk + 7) / 8; }
+template <int G, bool HALVES, bool LOOSE>
+__device__ inline Share<LOOSE> share(int l, int dk, int rotary) {
+    Share<LOOSE> r;
+    if constexpr (!LOOSE) {
+        r.mine = 8 * l < dk;
+        l = r.mine ? l : 0;
+        const bool turned = HALVES && 8 * l < rotary;
+        r.c0 = turned ? 4 * l : 8 * l;
+        r.c1 = turned ? rotary / 2 + 4 * l : 8 * l + 4;
+        r.p0 = 4 * l;
+    } else {
+        r.mine = l < lanes_wanted(dk, rotary, HALVES);
+        const int half = rotary / 2, turned = turned_lanes(rotary);
+        if (HALVES && l < turned) {
+            r.p0 = max(0, min(4 * l, half - 4));
+            r.c0 = r.p0, r.c1 = half + r.p0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r.ka[i] = r.kb[i] = r.p0 + i >= 4 * l && r.p0 + i < half ? 1.0f : 0.0f;
+        } else {
+            const int from = HALVES ? rotary + 8 * (l - turned) : 8 * l;
+            r.c0 = min(from, dk - 8), r.c1 = r.c0 + 4;
+            r.p0 = HALVES ? 4 * G - 4 : r.c0 / 2;  // with halves the last four angles of the strip, which are none
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                r.ka[i] = r.c0 + (HALVES ? i : 2 * i) >= from ? 1.0f : 0.0f;
+                r.kb[i] = r.c0 + (HALVES ? 4 + i : 2 * i) >= from ? 1.0f : 0.0f;
+            }
+        }
+        r.whole = true;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (!r.mine) r.ka[i] = r.kb[i] = 0.0f;
+            r.whole = r.whole && r.ka[i] != 0.0f && r.kb[i] != 0.0f;
+        }
+        if (!r.mine) r.c0 = r.p0 = 0, r.c1 = 4;
+    }
+    return r;
 }
-// The cosines and sines of lane l's four pairs; a pair that is not turned has 1 and 0.
+// Column of a[i] and of b[i].
+template <bool HALVES>
+__device__ inline int column_a(int c0, int c1, int i) { return HALVES ? c0 + i : i < 2 ? c0 + 2 * i : c1 + 2 * i - 4; }
+template <bool HALVES>
+__device__ inline int column_b(int c0, int c1, int i) { return HALVES ? c1 + i : i < 2 ? c0 + 2 * i + 1 : c1 + 2 * i - 3; }
+// The cosines and sines of a lane's four pairs, p0 and on; a pair that is not turned has 1 and 0.
 struct Angles {
     f32x4 c, s;
 };
 template <int G>
-__device__ inline Angles angles(const Qk& a, int pos, int l, double near, double far, float2* strip) {
+__device__ inline Angles angles(const Qk& a, int pos, int p0, double near, double far, float2* strip) {
     const int lane = threadIdx.x & 63;
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
@@ -282,35 +344,30 @@ __device__ inline Angles angles(const Qk& a, int pos, int l, double near, double
     Angles r;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float2 v = strip[4 * l + i];
+        const float2 v = strip[p0 + i];
         r.c[i] = v.x, r.s[i] = v.y;
     }
     return r;
 }
-__device__ inline Eight weights_of(const float* w, int c0, int c1, bool halves) {
+template <bool HALVES>
+__device__ inline Eight weights_of(const float* w, int c0, int c1) {
     Eight e;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        e.a[i] = halves ? w[c0 + i] : i < 2 ? w[c0 + 2 * i] : w[c1 + 2 * i - 4];
-        e.b[i] = halves ? w[c1 + i] : i < 2 ? w[c0 + 2 * i + 1] : w[c1 + 2 * i - 3];
-    }
+    for (int i = 0; i < 4; ++i) e.a[i] = w[column_a<HALVES>(c0, c1, i)], e.b[i] = w[column_b<HALVES>(c0, c1, i)];
     return e;
 }
 
 // A token's list of rows, 64 / G to a step, the queries' steps first, then the keys'. What a step needs is the wavefront's (scalars) but for the lane's offset,
 // and the next step's loads are on their way while one is worked on: with four steps unrolled the compiler formed every address ahead of the loop, 2600
 // instructions with spilled scalars in place of 500.
-template <typename T, int G, bool HALVES>
-struct List {
-    using C = Cols<T, HALVES>;
+template <typename T, int G, bool HALVES, bool LOOSE>
+struct List : Share<LOOSE> {
+    using C = Cols<T, HALVES, LOOSE>;
+    using Share<LOOSE>::c0;
+    using Share<LOOSE>::c1;
     static constexpr int ROWS = 64 / G;
-    int l, g, c0, c1, q_steps, steps;
-    bool mine;
-    __device__ List(const Qk& a) {
-        const int lane = threadIdx.x & 63;
-        l = lane % G, g = lane / G;
-        mine = 8 * l < a.dk;
-        runs<HALVES>(mine ? l : 0, a.rotary, c0, c1);
+    int g, q_steps, steps;
+    __device__ List(const Qk& a) : Share<LOOSE>(share<G, HALVES, LOOSE>((threadIdx.x & 63) % G, a.dk, a.rotary)), g((threadIdx.x & 63) / G) {
         q_steps = (a.Hq + ROWS - 1) / ROWS;
         steps = q_steps + (a.Hkv + ROWS - 1) / ROWS;
     }
@@ -339,18 +396,29 @@ struct List {
     __device__ void store(const RowsOut (&y)[2], const Step& s, int64_t oq, int64_t ok, const Eight& e) const {
         uint32_t off;
         char* base = const_cast<char*>(row(y, s, oq, ok, g, off));
+        if constexpr (LOOSE) {
+            if (!this->whole) {
+                T* to = reinterpret_cast<T*>(base + off);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (this->ka[i] != 0.0f) put(to, column_a<HALVES>(c0, c1, i), e.a[i]);
+                    if (this->kb[i] != 0.0f) put(to, column_b<HALVES>(c0, c1, i), e.b[i]);
+                }
+                return;
+            }
+        }
         C::store(base, off + c0 * static_cast<uint32_t>(sizeof(T)), off + c1 * static_cast<uint32_t>(sizeof(T)), e);
     }
 };
 
 // grid.x: tokens, WAVES to a workgroup, in strides of the grid; grid.y: `per` steps of a token's list each.
-template <typename T, int G, bool HALVES>
+template <typename T, int G, bool HALVES, bool LOOSE>
 __global__ __launch_bounds__(NT) void qk_fwd_rows(Qk a, int per) {
-    using L = List<T, G, HALVES>;
+    using L = List<T, G, HALVES, LOOSE>;
     __shared__ float2 strips[WAVES][4 * G];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), stride = static_cast<int>(gridDim.x) * WAVES;
     const L list(a);
-    const Eight wq = weights_of(a.w[0], list.c0, list.c1, HALVES), wk = weights_of(a.w[1], list.c0, list.c1, HALVES);
+    const Eight wq = weights_of<HALVES>(a.w[0], list.c0, list.c1), wk = weights_of<HALVES>(a.w[1], list.c0, list.c1);
     const double near = turns_of(a, lane), far = G > 16 ? turns_of(a, lane + 64) : 0.0;
     const int first = static_cast<int>(blockIdx.y) * per, last = min(first + per, list.steps), tokens = a.B * a.T;
 #pragma unroll 1
@@ -360,7 +428,7 @@ __global__ __launch_bounds__(NT) void qk_fwd_rows(Qk a, int per) {
         const int64_t xq = b * a.x[0].sb + t * a.x[0].st, xk = b * a.x[1].sb + t * a.x[1].st, yq = b * a.y[0].sb + t * a.y[0].st, yk = b * a.y[1].sb + t * a.y[1].st;
         auto at = list.step(a, first);
         typename L::C::Raw raw = list.load(a.x, at, xq, xk);
-        const Angles turn = angles<G>(a, pos, list.l, near, far, strips[wave]);
+        const Angles turn = angles<G>(a, pos, list.p0, near, far, strips[wave]);
 #pragma unroll 1
         for (int s = first; s < last; ++s) {
             const auto now = at;
@@ -368,7 +436,12 @@ __global__ __launch_bounds__(NT) void qk_fwd_rows(Qk a, int per) {
             if (s + 1 < last) at = list.step(a, s + 1), raw = list.load(a.x, at, xq, xk);
             float ss = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) ss += x.a[i] * x.a[i] + x.b[i] * x.b[i];
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (LOOSE)
+                    ss += list.ka[i] * (x.a[i] * x.a[i]) + list.kb[i] * (x.b[i] * x.b[i]);
+                else
+                    ss += x.a[i] * x.a[i] + x.b[i] * x.b[i];
+            }
             const float r = inverse_root(group_sum<G>(list.mine ? ss : 0.0f) * a.per_dk + a.eps);
             Eight y;
 #pragma unroll
@@ -382,14 +455,14 @@ __global__ __launch_bounds__(NT) void qk_fwd_rows(Qk a, int per) {
     }
 }
 
-template <typename T, int G, bool HALVES>
+template <typename T, int G, bool HALVES, bool LOOSE>
 __global__ __launch_bounds__(NT) void qk_bwd_rows(Qk a, int per) {
-    using L = List<T, G, HALVES>;
+    using L = List<T, G, HALVES, LOOSE>;
     __shared__ float2 strips[WAVES][4 * G];
     __shared__ __align__(16) float sh[WAVES * L::ROWS * 2 * 8 * G];  // 16 KB
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), stride = static_cast<int>(gridDim.x) * WAVES;
     const L list(a);
-    const Eight wq = weights_of(a.w[0], list.c0, list.c1, HALVES), wk = weights_of(a.w[1], list.c0, list.c1, HALVES);
+    const Eight wq = weights_of<HALVES>(a.w[0], list.c0, list.c1), wk = weights_of<HALVES>(a.w[1], list.c0, list.c1);
     const double near = turns_of(a, lane), far = G > 16 ? turns_of(a, lane + 64) : 0.0;
     const int first = static_cast<int>(blockIdx.y) * per, last = min(first + per, list.steps), tokens = a.B * a.T;
     Eight dwq = {}, dwk = {};
@@ -401,7 +474,7 @@ __global__ __launch_bounds__(NT) void qk_bwd_rows(Qk a, int per) {
         const int64_t gq = b * a.dy[0].sb + t * a.dy[0].st, gk = b * a.dy[1].sb + t * a.dy[1].st;
         auto at = list.step(a, first);
         typename L::C::Raw rx = list.load(a.x, at, xq, xk), rg = list.load(a.dy, at, gq, gk);
-        const Angles turn = angles<G>(a, pos, list.l, near, far, strips[wave]);
+        const Angles turn = angles<G>(a, pos, list.p0, near, far, strips[wave]);
 #pragma unroll 1
         for (int s = first; s < last; ++s) {
             const auto now = at;
@@ -414,8 +487,13 @@ __global__ __launch_bounds__(NT) void qk_bwd_rows(Qk a, int per) {
                 const float da = dy.a[i] * turn.c[i] + dy.b[i] * turn.s[i], db = dy.b[i] * turn.c[i] - dy.a[i] * turn.s[i];
                 wdu.a[i] = da * (now.key ? wk.a[i] : wq.a[i]), wdu.b[i] = db * (now.key ? wk.b[i] : wq.b[i]);
                 dux.a[i] = da * x.a[i], dux.b[i] = db * x.b[i];
-                ss += x.a[i] * x.a[i] + x.b[i] * x.b[i];
-                sg += wdu.a[i] * x.a[i] + wdu.b[i] * x.b[i];
+                if constexpr (LOOSE) {
+                    ss += list.ka[i] * (x.a[i] * x.a[i]) + list.kb[i] * (x.b[i] * x.b[i]);
+                    sg += list.ka[i] * (wdu.a[i] * x.a[i]) + list.kb[i] * (wdu.b[i] * x.b[i]);
+                } else {
+                    ss += x.a[i] * x.a[i] + x.b[i] * x.b[i];
+                    sg += wdu.a[i] * x.a[i] + wdu.b[i] * x.b[i];
+                }
             }
             const float r = inverse_root(group_sum<G>(list.mine ? ss : 0.0f) * a.per_dk + a.eps);
             const float m = r * r * (group_sum<G>(list.mine ? sg : 0.0f) * a.per_dk);
@@ -438,6 +516,14 @@ __global__ __launch_bounds__(NT) void qk_bwd_rows(Qk a, int per) {
     float* const own = sh + (wave * L::ROWS + list.g) * PITCH;
     if (list.mine) {
         auto lay = [&](float* to, const Eight& d) {
+            if constexpr (LOOSE) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (list.ka[i] != 0.0f) to[column_a<HALVES>(list.c0, list.c1, i)] = d.a[i];
+                    if (list.kb[i] != 0.0f) to[column_b<HALVES>(list.c0, list.c1, i)] = d.b[i];
+                }
+                return;
+            }
             *reinterpret_cast<f32x4*>(to + list.c0) = HALVES ? d.a : f32x4{d.a[0], d.b[0], d.a[1], d.b[1]};
             *reinterpret_cast<f32x4*>(to + list.c1) = HALVES ? d.b : f32x4{d.a[2], d.b[2], d.a[3], d.b[3]};
         };
@@ -520,15 +606,21 @@ bool pieces(const void* p, int64_t sb, int64_t st, int64_t sh, const pk_qk_shape
     const int64_t es = elem_size(s->dtype), to = s->dtype == PK_BF16 && s->halves ? 8 : 16;
     return aligned(p, to) && sb * es % to == 0 && st * es % to == 0 && sh * es % to == 0;
 }
-bool rows_serve(const Qk& a, const pk_qk_shape* s, bool backward) {
-    if (a.dk % 8 || (a.halves && a.rotary % 8) || static_cast<int64_t>(s->B) * s->T > (1 << 30)) return false;
+// Which kernels take a call: the row kernels on whole aligned pieces, the row kernels on any rows, or those that take a wavefront for a row (head sizes under 8, the last few
+// up to 256 where two remainders want a lane each, strides that are negative or past 2^24). 8192 tokens, 14 + 2 heads, bf16, forward and backward: 64 columns aligned
+// 7.9 and 15.8 us, the same as any rows 9.6 and 17.6, one element off 10.2 and 17.6, a wavefront for a row 59 and 80; 62 columns 10.1 and 18.5 (60 and 80), 100 columns of fp32
+// 18.9 and 31 (64 and 84); 16456 tokens, 8 + 8 heads of 104 columns, 92 turned from halves, 27 and 39 (121 and 151).
+enum Serve { ALIGNED, LOOSE, ANY };
+Serve serve(const Qk& a, const pk_qk_shape* s, bool backward) {
+    if (a.dk < 8 || lanes_wanted(a.dk, a.rotary, a.halves) > 32 || static_cast<int64_t>(s->B) * s->T > (1 << 30)) return ANY;
+    bool whole = a.dk % 8 == 0 && !(a.halves && a.rotary % 8);
     for (int i = 0; i < 2; ++i) {
-        if (!pieces(a.x[i].p, a.x[i].sb, a.x[i].st, a.x[i].sh, s) || !pieces(a.y[i].p, a.y[i].sb, a.y[i].st, a.y[i].sh, s)) return false;
-        if (backward && !pieces(a.dy[i].p, a.dy[i].sb, a.dy[i].st, a.dy[i].sh, s)) return false;
+        whole = whole && pieces(a.x[i].p, a.x[i].sb, a.x[i].st, a.x[i].sh, s) && pieces(a.y[i].p, a.y[i].sb, a.y[i].st, a.y[i].sh, s);
+        whole = whole && (!backward || pieces(a.dy[i].p, a.dy[i].sb, a.dy[i].st, a.dy[i].sh, s));
         for (const int64_t sh : {a.x[i].sh, a.y[i].sh, backward ? a.dy[i].sh : 0})  // a lane's offset inside a step is held in 32 bits
-            if (sh < 0 || sh > (1 << 24)) return false;
+            if (sh < 0 || sh > (1 << 24)) return ANY;
     }
-    return true;
+    return whole ? ALIGNED : LOOSE;
 }
 // Tokens of all sequences as one run, where every tensor has them so: no division in the kernel.
 void flatten(Qk& a, bool backward) {
@@ -537,7 +629,11 @@ void flatten(Qk& a, bool backward) {
         if (a.x[i].sb != a.T * a.x[i].st || a.y[i].sb != a.T * a.y[i].st || (backward && a.dy[i].sb != a.T * a.dy[i].st)) return;
     a.T *= a.B, a.B = 1;
 }
-int lanes_of(int dk) { return dk <= 32 ? 4 : dk <= 64 ? 8 : dk <= 128 ? 16 : 32; }
+// of a row's group
+int lanes_of(const Qk& a) {
+    const int lanes = lanes_wanted(a.dk, a.rotary, a.halves);
+    return lanes <= 4 ? 4 : lanes <= 8 ? 8 : lanes <= 16 ? 16 : 32;
+}
 
 // A launch of the row kernels: workgroups over tokens, parts that a token's heads are dealt to, `most` workgroups in all.
 struct Plan {
@@ -545,8 +641,8 @@ struct Plan {
 };
 // A token's heads stay with one wavefront, which forms the angles once, where the tokens alone fill the chip; fewer tokens are dealt out, to 4096 wavefronts.
 // Forward, 32 heads of 128: 4 tokens 5.7 us by a wavefront each, 2.4 dealt out; 2048 tokens 8.6 and 7.9, dealt to 16384 wavefronts 10.1; 4096 tokens 12.5 either way.
-Plan plan_of(const pk_qk_shape* s, int most) {
-    const int rows = 64 / lanes_of(s->dk), steps = (s->Hq + rows - 1) / rows + (s->Hkv + rows - 1) / rows;
+Plan plan_of(const Qk& a, const pk_qk_shape* s, int most) {
+    const int rows = 64 / lanes_of(a), steps = (s->Hq + rows - 1) / rows + (s->Hkv + rows - 1) / rows;
     const int64_t tokens = static_cast<int64_t>(s->B) * s->T, want = 4096;
     int parts = 1;
     while (parts < steps && parts < most && tokens * parts < want) ++parts;
@@ -558,21 +654,28 @@ Plan plan_of(const pk_qk_shape* s, int most) {
     return p;
 }
 
-template <typename T, bool HALVES>
+template <typename T, bool HALVES, bool LOOSE>
 void launch_rows(const Qk& a, const Plan& p, bool backward, hipStream_t st) {
     const dim3 grid(p.groups, p.parts);
-    switch (lanes_of(a.dk)) {
-        case 4: return backward ? qk_bwd_rows<T, 4, HALVES><<<grid, NT, 0, st>>>(a, p.per) : qk_fwd_rows<T, 4, HALVES><<<grid, NT, 0, st>>>(a, p.per);
-        case 8: return backward ? qk_bwd_rows<T, 8, HALVES><<<grid, NT, 0, st>>>(a, p.per) : qk_fwd_rows<T, 8, HALVES><<<grid, NT, 0, st>>>(a, p.per);
-        case 16: return backward ? qk_bwd_rows<T, 16, HALVES><<<grid, NT, 0, st>>>(a, p.per) : qk_fwd_rows<T, 16, HALVES><<<grid, NT, 0, st>>>(a, p.per);
-        default: return backward ? qk_bwd_rows<T, 32, HALVES><<<grid, NT, 0, st>>>(a, p.per) : qk_fwd_rows<T, 32, HALVES><<<grid, NT, 0, st>>>(a, p.per);
+    switch (lanes_of(a)) {
+        case 4: return backward ? qk_bwd_rows<T, 4, HALVES, LOOSE><<<grid, NT, 0, st>>>(a, p.per) : qk_fwd_rows<T, 4, HALVES, LOOSE><<<grid, NT, 0, st>>>(a, p.per);
+        case 8: return backward ? qk_bwd_rows<T, 8, HALVES, LOOSE><<<grid, NT, 0, st>>>(a, p.per) : qk_fwd_rows<T, 8, HALVES, LOOSE><<<grid, NT, 0, st>>>(a, p.per);
+        case 16: return backward ? qk_bwd_rows<T, 16, HALVES, LOOSE><<<grid, NT, 0, st>>>(a, p.per) : qk_fwd_rows<T, 16, HALVES, LOOSE><<<grid, NT, 0, st>>>(a, p.per);
+        default: return backward ? qk_bwd_rows<T, 32, HALVES, LOOSE><<<grid, NT, 0, st>>>(a, p.per) : qk_fwd_rows<T, 32, HALVES, LOOSE><<<grid, NT, 0, st>>>(a, p.per);
     }
 }
-void launch_rows(const Qk& a, const Plan& p, bool backward, int dtype, hipStream_t st) {
-    if (dtype == PK_BF16)
-        a.halves ? launch_rows<uint16_t, true>(a, p, backward, st) : launch_rows<uint16_t, false>(a, p, backward, st);
+template <typename T>
+void launch_rows(const Qk& a, const Plan& p, bool backward, bool loose, hipStream_t st) {
+    if (loose)
+        a.halves ? launch_rows<T, true, true>(a, p, backward, st) : launch_rows<T, false, true>(a, p, backward, st);
     else
-        a.halves ? launch_rows<float, true>(a, p, backward, st) : launch_rows<float, false>(a, p, backward, st);
+        a.halves ? launch_rows<T, true, false>(a, p, backward, st) : launch_rows<T, false, false>(a, p, backward, st);
+}
+void launch_rows(const Qk& a, const Plan& p, bool backward, bool loose, int dtype, hipStream_t st) {
+    if (dtype == PK_BF16)
+        launch_rows<uint16_t>(a, p, backward, loose, st);
+    else
+        launch_rows<float>(a, p, backward, loose, st);
 }
 // workgroups of the backward that takes any row
 int any_groups(const pk_qk_shape* s) {
@@ -600,9 +703,9 @@ int pk_qk_norm_rope_fwd(const pk_qk_shape* s, const pk_tensor4* q, const pk_tens
         a.w[0] = wq, a.w[1] = wk, a.pos = pos;
         touch({q->ptr, k->ptr, yq->ptr, yk->ptr, wq, wk, pos}, stream);
         hipStream_t st = static_cast<hipStream_t>(stream);
-        if (rows_serve(a, s, false)) {
+        if (const Serve by = serve(a, s, false); by != ANY) {
             flatten(a, false);
-            launch_rows(a, plan_of(s, FWD_MOST), false, s->dtype, st);
+            launch_rows(a, plan_of(a, s, FWD_MOST), false, by == LOOSE, s->dtype, st);
             return launched();
         }
         const int64_t want = (items_of(s) + WAVES - 1) / WAVES;
@@ -617,7 +720,9 @@ int pk_qk_norm_rope_fwd(const pk_qk_shape* s, const pk_tensor4* q, const pk_tens
 
 size_t pk_qk_norm_rope_bwd_workspace_bytes(const pk_qk_shape* s) {
     if (check(s, "pk_qk_norm_rope_bwd_workspace_bytes")) return 0;
-    const Plan p = plan_of(s, BWD_MOST);
+    Qk a;
+    fill(a, s);
+    const Plan p = plan_of(a, s, BWD_MOST);
     return sizeof(float) * static_cast<size_t>(std::max(any_groups(s), p.groups * p.parts)) * 2 * s->dk;
 }
 
@@ -642,11 +747,11 @@ int pk_qk_norm_rope_bwd(const pk_qk_shape* s, const pk_tensor4* dyq, const pk_te
         if (!none) {
             a.x[0] = rows_of(q), a.x[1] = rows_of(k), a.dy[0] = rows_of(dyq), a.dy[1] = rows_of(dyk), a.y[0] = out_of(dq), a.y[1] = out_of(dk);
             touch({q->ptr, k->ptr, dyq->ptr, dyk->ptr, dq->ptr, dk->ptr}, stream);
-            if (rows_serve(a, s, true)) {
-                const Plan p = plan_of(s, BWD_MOST);
+            if (const Serve by = serve(a, s, true); by != ANY) {
+                const Plan p = plan_of(a, s, BWD_MOST);
                 groups = p.groups * p.parts;
                 flatten(a, true);
-                launch_rows(a, p, true, s->dtype, st);
+                launch_rows(a, p, true, by == LOOSE, s->dtype, st);
             } else if (s->dtype == PK_BF16)
                 qk_bwd_any<uint16_t><<<dim3(groups), NT, 0, st>>>(a);
             else

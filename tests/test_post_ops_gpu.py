@@ -96,6 +96,11 @@ QK_CASES = [  # B, T, Hq, Hkv, dk, rotary, halves, layout, pos, far
     (1, 40, 3, 3, 64, 0, False, "offset", "rows", 0), (1, 40, 3, 3, 128, 64, True, "offset", "rows", 0), (2, 11, 2, 5, 70, 0, True, "fused", "rows", 0),
     (2, 11, 2, 5, 254, 2, False, "fused", "rows", 0), (1, 700, 16, 16, 32, 0, False, "fused", "rows", 0), (1, 5, 1, 1, 8, 0, True, "plain", "rows", 0),
     (1, 5, 2, 1, 40, 8, False, "plain", "rows", 0), (5, 300, 4, 1, 64, 32, True, "fused", "shared", 0),
+    (2, 13, 3, 2, 104, 92, True, "fused", "rows", 50), (2, 13, 3, 2, 8, 2, True, "plain", "any", 50), (2, 13, 3, 2, 8, 4, True, "offset", "any", 50),
+    (2, 13, 3, 2, 8, 6, True, "fused", "any", 50), (1, 9, 5, 1, 10, 0, False, "plain", "rows", 3), (1, 9, 5, 1, 10, 10, True, "offset", "rows", 3),
+    (1, 9, 5, 1, 14, 6, True, "plain", "rows", 3), (2, 11, 4, 2, 256, 250, True, "fused", "any", 7), (2, 11, 4, 2, 250, 0, True, "offset", "any", 7),
+    (2, 11, 4, 2, 248, 234, True, "heads", "any", 7), (3, 40, 2, 2, 66, 2, True, "fused", "rows", 0), (3, 40, 2, 2, 66, 64, False, "heads", "rows", 0),
+    (2, 40, 2, 2, 6, 4, True, "fused", "rows", 9), (2, 40, 2, 2, 4, 0, False, "offset", "rows", 9), (2, 700, 8, 2, 100, 52, True, "fused", "rows", 9),
     (1, 1, 4500, 3, 128, 0, True, "plain", "rows", 5), (1, 2, 3, 2100, 256, 0, False, "plain", "rows", 5)]
 
 
