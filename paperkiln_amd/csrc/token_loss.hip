@@ -153,56 +153,9 @@ __device__ inline RowOut summed_row(const Loss& a, float coef, float xt, const R
 }
 __device__ inline RowOut given_row(const Loss& a, int64_t r, float coef, float xt, bool word) { return summed_row(a, coef, xt, RowSum{0.0f, a.lse_in[r] * (1.0 / LN2)}, word); }
 
-// A gradient that does not lie as its logits do (another row pitch, another offset, modulo 16 bytes): a workgroup takes a row element by element.
-constexpr int ANY_NT = 256;
-template <typename T, Mode MODE>
-__global__ __launch_bounds__(ANY_NT) void rows_any(Loss a) {
-    if (MODE == GRAD && blockIdx.x == a.rows) return pairs_mean<ANY_NT>(a);
-    __shared__ float sh_m[ANY_NT / 64], sh_s[ANY_NT / 64];
-    const int64_t r = blockIdx.x;
-    const int tid = threadIdx.x, V = a.vocab, t = a.targets[r];
-    const T* x = static_cast<const T*>(a.logits) + r * a.ld;
-    T* dx = MODE == LOGP ? nullptr : static_cast<T*>(a.dlogits) + r * a.dld;
-    if (MODE == LOGP && a.clear && tid == 0) a.clear[r] = 0.0f;
-    bool skip = t < 0;
-    float coef = 0.0f;
-    if (MODE == POLICY) skip = skip || a.weights[r] == 0.0f;
-    if (MODE == GRAD) coef = a.coef[r] * a.scale, skip = skip || coef == 0.0f;
-    if (skip) {
-        if (MODE != GRAD && tid == 0) {
-            a.logp[r] = 0.0f;
-            if (a.lse) a.lse[r] = 0.0f;
-            if (MODE == POLICY) a.row_loss[r] = 0.0;
-        }
-        if (MODE != LOGP)
-            for (int j = tid; j < V; j += ANY_NT) put(dx, j, 0.0f);
-        return;
-    }
-    const float xt = t < V ? elem(x, t) : NAN;  // read before the row is written over; a token that is no word has no probability
-    RowOut o;
-    const bool given = MODE == GRAD && !far(a.lse_in[r]);
-    if (given) {
-        o = given_row(a, r, coef, xt, t < V);
-    } else {
-        float m = -INFINITY, s = 0.0f;
-        for (int j = tid; j < V; j += ANY_NT) m = fmaxf(m, elem(x, j));
-        for (int o_ = 32; o_ >= 1; o_ >>= 1) m = fmaxf(m, __shfl_xor(m, o_));
-        const float ref = m == -INFINITY ? 0.0f : m;
-        for (int j = tid; j < V; j += ANY_NT) s += power_of(a, elem(x, j), ref);
-        s = group_sum<64>(s);
-        if ((tid & 63) == 0) sh_m[tid >> 6] = s == 0.0f ? -INFINITY : ref, sh_s[tid >> 6] = s;
-        __syncthreads();
-        const RowSum sum = sum_of_row<ANY_NT / 64>(a, sh_m, sh_s);
-        o = MODE == GRAD ? summed_row(a, coef, xt, sum, t < V) : finish<MODE>(a, r, xt, sum, tid == 0);
-    }
-    __syncthreads();  // the target has been read by all
-    if (MODE != LOGP)
-        for (int j = tid; j < V; j += ANY_NT) put(dx, j, j == t ? o.target : o.other(elem(x, j), a.scale * LOG2E));
-}
-
 // ---- rows in 16-byte pieces -------------------------------------------------------------------------------------------------
 // A row is taken apart at 16-byte boundaries of its address: whole pieces, and the few elements in front of the first and behind the last one, which go to
-// one thread each. So a row may begin anywhere; what is written has to lie as what is read, modulo 16.
+// one thread each. So a row may begin anywhere, and the gradient's row anywhere else: the hardware stores a piece where its elements may lie.
 
 template <typename T>
 struct Piece;
@@ -274,9 +227,10 @@ __device__ inline Piece<T> load_piece(const T* x) {
     else
         return Piece<T>{*p};
 }
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
 template <bool PAST, typename T>
 __device__ inline void store_piece(T* x, const Piece<T>& v) {
-    u32x4* p = reinterpret_cast<u32x4*>(x);
+    u32x4_any* p = reinterpret_cast<u32x4_any*>(x);
     if constexpr (PAST)
         __builtin_nontemporal_store(v.v, p);
     else
@@ -676,10 +630,6 @@ __global__ __launch_bounds__(PAIR_NT) void pair_loss(Pairs a) {
 // product behind the loss then finds less of a small one there: loss and product of 33 MB 120.7 -> 128.7 us, 66 MB 172.8 -> 185.3, 98 MB 228.6 -> 229.3, 131 MB
 // 254.0 -> 251.9, 262 MB 392.5 -> 387.2.
 constexpr int64_t PAST_BYTES = int64_t{96} << 20;
-// Whether what is written lies as what is read, modulo a piece, in every row.
-bool same_cut(const Loss& a, int64_t es) {
-    return (reinterpret_cast<uintptr_t>(a.logits) - reinterpret_cast<uintptr_t>(a.dlogits)) % 16 == 0 && (a.ld - a.dld) * es % 16 == 0;
-}
 constexpr int HELD_PIECES = 8192;
 // Threads and pieces for a row. Policy loss over 262 to 131 MB of bf16 logits, the neighbours in brackets: 1000 words 73 us (a wavefront for two pieces; 90 on two wavefronts),
 // 2000 words 106 (118 on 128 threads), 4000 words 100 (104 on 256, 106 on 64), 8000 words 91.5 (95 on 128, 100 on 512), 16000 words 90 (96 on 256), 32000 words 94 (94 on 1024), 64000
@@ -716,7 +666,6 @@ void launch_typed(const Loss& a, const Pairs* pairs, hipStream_t st) {
         rows_part<T><<<dim3(static_cast<unsigned>(a.rows), static_cast<unsigned>(parts)), PART_NT, 0, st>>>(a, per, a.parts);
         rows_join<T><<<dim3(static_cast<unsigned>(a.rows)), 64, 0, st>>>(a, parts, a.parts);
     } else {
-        if (!same_cut(a, sizeof(T))) return rows_any<T, MODE><<<grid, ANY_NT, 0, st>>>(a);
         if constexpr (MODE == GRAD) {
             // Few rows are dealt out, one load to a thread, as far as that fills the chip: one row of 128000 words bf16 9.4 -> 3.0 us
             const int pieces = a.vocab / Piece<T>::N, most = static_cast<int>(std::max<int64_t>(1, 512 / std::max<int64_t>(a.rows, 1)));
@@ -880,7 +829,7 @@ int pk_preference_loss(const pk_preference_config* c, const void* logits, int64_
         if (int rc = launch_rows<LOGP>(a, dtype, st)) return rc;
         const Pairs p{seq_start, targets, fine, ref_logp, coef, margins, losses, rows, static_cast<int>(pairs), c->beta, c->label_smoothing, c->upstream};
         a.dlogits = dlogits, a.dld = dld;
-        const bool few = rows <= FEW_PAIRS_ROWS && pairs <= MOST_FEW_PAIRS && same_cut(a, elem_size(dtype));
+        const bool few = rows <= FEW_PAIRS_ROWS && pairs <= MOST_FEW_PAIRS;
         if (!few) {
             pair_loss<<<dim3(static_cast<unsigned>(pairs)), PAIR_NT, 0, st>>>(p);
             if (int rc = launched()) return rc;

@@ -539,19 +539,18 @@ def test_preference_loss_against_64_bits(pk, case, dtype):
 
 @pytest.mark.parametrize("ends", [(0, 60, 100, 160, 200), (5, 5, 5, 5, 5), (-9, 40, 190, 2 ** 31 - 1, -2 ** 31), (150, 100, 50, 0, 250)], ids=str)
 def test_preference_loss_a_launch_less_or_not(pk, ends):
-    """Two pairs formed by the gradient's wavefronts and by a launch of their own (into rows that lie otherwise): sums in 64 bits in another order, so a step of
-    32 bits in the margins, and offsets that lie held to the rows alike."""
+    """Two pairs formed by the gradient's wavefronts and, with rows behind that count nothing, by a launch of their own: sums in 64 bits in another order, so a step
+    of 32 bits in the margins, and offsets that lie held to the rows alike."""
     x, t, g = loss_inputs(200, 900, FP32, 5)
     t[::7] = -1
     starts, ref = torch.tensor(ends, dtype=torch.int32, device="cuda"), -8 * torch.rand(200, generator=g, device="cuda")
     a = pk.blockops.preference_loss(x, t, starts, ref, 0.3, 0.1)
-    b = pk.blockops.preference_loss(x, t, starts, ref, 0.3, 0.1, out=x.new_empty(200, 903)[:, 2:902])
-    assert torch.equal(a[3], b[3])
+    more = lambda y, v: torch.cat([y, y.new_full((400, *y.shape[1:]), v)])  # noqa: E731
+    b = pk.blockops.preference_loss(more(x, 0), more(t, -1), starts, more(ref, 0), 0.3, 0.1, out=x.new_empty(600, 903)[:, 2:902])
+    assert torch.equal(a[3], b[3][:200]) and not b[3][200:].any() and not b[1][200:].any()
     within("margins", a[2], b[2], 2 * U * b[2].abs() + 1e-37)
     within("loss", a[0], b[0], 2 * U * (b[0].abs() + b[2].abs().sum()))
-    # softmax by another kernel: other orders of 32-bit sums
-    z = softmax64(x, t, 1.0)[0]
-    within("dlogits", a[1], b[1], (2 * (logp_slack(z, 900) + 4 * U * sizes(z)) * 0.15 + 4 * U)[:, None])
+    within("dlogits", a[1], b[1][:200], 8 * U * b[1][:200].abs() + 1e-37)   # a step or two in the pair's slope, a rounding
     if sorted(ends) == list(ends):   # rows of no sequence
         assert not a[1][ends[-1]:].any() and not a[1][:ends[0]].any()
 
