@@ -523,8 +523,8 @@ __device__ inline void few_pairs_mean(const Pairs& a, float* mean) {
 // ---- the gradient of rows whose sums are known --------------------------------------------------------------------------------
 // Every element by itself, so a row may be dealt to several workgroups (grid.y, `per` pieces each) and written over.
 // FEW: the rows' coefficients are formed here, from the pairs.
-constexpr int GRAD_NT = 512, GRAD_U = 8;
-template <typename T, bool PAST, bool FEW>
+constexpr int GRAD_U = 8;
+template <typename T, int GRAD_NT, bool PAST, bool FEW>
 __global__ __launch_bounds__(GRAD_NT) void rows_grad(Loss a, int per, Pairs pairs) {
     constexpr int N = Piece<T>::N;
     __shared__ float sh_m[GRAD_NT / 64], sh_s[GRAD_NT / 64];
@@ -655,6 +655,13 @@ int parts_of_rows(int64_t rows, int64_t vocab, int64_t es) {
     if (rows < 1 || rows >= FEW_ROWS || pieces <= HELD_PIECES) return 1;
     return static_cast<int>(std::min<int64_t>(std::min<int64_t>(MOST_PARTS, 512 / rows), pieces / (2 * PART_NT)));
 }
+template <typename T, int NT, bool PAST, bool FEW>
+void launch_grad(const Loss& a, const Pairs& pairs, hipStream_t st) {
+    // Few rows are dealt out, one load to a thread, as far as that fills the chip: one row of 128000 words bf16 9.4 -> 3.0 us
+    const int pieces = a.vocab / Piece<T>::N, most = static_cast<int>(std::max<int64_t>(1, 512 / std::max<int64_t>(a.rows, 1)));
+    const int parts = std::min(most, std::max(1, pieces / NT)), per = (pieces + parts - 1) / parts;
+    rows_grad<T, NT, PAST, FEW><<<dim3(static_cast<unsigned>(a.rows + (a.loss ? 1 : 0)), static_cast<unsigned>(parts)), NT, 0, st>>>(a, per, pairs);
+}
 template <typename T, Mode MODE>
 void launch_typed(const Loss& a, const Pairs* pairs, hipStream_t st) {
     const bool past = a.rows * a.vocab * static_cast<int64_t>(sizeof(T)) >= PAST_BYTES;
@@ -667,14 +674,13 @@ void launch_typed(const Loss& a, const Pairs* pairs, hipStream_t st) {
         rows_join<T><<<dim3(static_cast<unsigned>(a.rows)), 64, 0, st>>>(a, parts, a.parts);
     } else {
         if constexpr (MODE == GRAD) {
-            // Few rows are dealt out, one load to a thread, as far as that fills the chip: one row of 128000 words bf16 9.4 -> 3.0 us
-            const int pieces = a.vocab / Piece<T>::N, most = static_cast<int>(std::max<int64_t>(1, 512 / std::max<int64_t>(a.rows, 1)));
-            const int parts = std::min(most, std::max(1, pieces / GRAD_NT)), per = (pieces + parts - 1) / parts;
-            const dim3 dealt(grid.x, static_cast<unsigned>(parts));
-            if (pairs)
-                rows_grad<T, false, true><<<dealt, GRAD_NT, 0, st>>>(a, per, *pairs);
-            else
-                past ? rows_grad<T, true, false><<<dealt, GRAD_NT, 0, st>>>(a, per, Pairs{}) : rows_grad<T, false, false><<<dealt, GRAD_NT, 0, st>>>(a, per, Pairs{});
+            // Threads for a row: bf16, 65536 rows of 1000 words 48 us by 64 threads (57 by 128, 72 by 256, 122 by 512), 32768 of 2000 48 (48, 49, 70), 16384 of 4000 49 (48, 46,
+            // 49), 8192 of 8000 49 (45, 44, 42), 8192 of 32000 208 (205, 193, 180). The pairs' mean is a workgroup's too: thousands of pairs want a large one.
+            const int pieces = a.vocab / Piece<T>::N;
+            if (pairs) return launch_grad<T, 512, false, true>(a, *pairs, st);
+            if (pieces <= 256 && a.pairs <= 4096) return past ? launch_grad<T, 64, true, false>(a, Pairs{}, st) : launch_grad<T, 64, false, false>(a, Pairs{}, st);
+            if (pieces <= 512 && a.pairs <= 4096) return past ? launch_grad<T, 256, true, false>(a, Pairs{}, st) : launch_grad<T, 256, false, false>(a, Pairs{}, st);
+            past ? launch_grad<T, 512, true, false>(a, Pairs{}, st) : launch_grad<T, 512, false, false>(a, Pairs{}, st);
         } else
             past ? launch_held<T, MODE, true>(a, st) : launch_held<T, MODE, false>(a, st);
     }

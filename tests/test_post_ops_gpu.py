@@ -555,6 +555,24 @@ def test_preference_loss_a_launch_less_or_not(pk, ends):
         assert not a[1][ends[-1]:].any() and not a[1][:ends[0]].any()
 
 
+def test_preference_loss_of_thousands_of_pairs(pk):
+    """More pairs than the small workgroups of short rows add up: margins are exact in their two log-probabilities, the loss their mean."""
+    P = 5000
+    x, t, g = loss_inputs(2 * P, 60, FP32, 5)
+    starts, ref = torch.arange(2 * P + 1, device="cuda", dtype=torch.int32), -8 * torch.rand(2 * P, generator=g, device="cuda")
+    loss, d, margins, logp = pk.blockops.preference_loss(x, t, starts, ref, 0.5)
+    z, _, wp, p = softmax64(x, t, 1.0)
+    u, off = 0.5 * (wp - ref.double()), 0.5 * (logp_slack(z, 60) + U * (wp.abs() + ref.double().abs()))
+    u, off = u[:P] - u[P:], off[:P] + off[P:]
+    within("margins", margins, u, off + U * u.abs())
+    each = torch.nn.functional.softplus(-u)
+    within("loss", loss, each.mean(), (off + 4 * U * (each + 1)).mean())
+    slope = -torch.sigmoid(-u) * 0.5 / P
+    coef = torch.cat([slope, -slope])[:, None]
+    want = coef * (torch.zeros_like(p).scatter_(1, t.long()[:, None], 1.0) - p)
+    within("dlogits", d, want, U * want.abs() + coef.abs() * (logp_slack(z, 60) + 4 * U * sizes(z) + torch.cat([off, off]) + 4 * U)[:, None])
+
+
 def test_preference_loss_far_margins_and_lying_offsets(pk):
     """Margins of hundreds: loss and slope stay finite and right. Offsets outside the rows are held to them; nothing outside is read or written."""
     x, t, _ = loss_inputs(6, 200, FP32, 3)
