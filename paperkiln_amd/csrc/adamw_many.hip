@@ -149,7 +149,7 @@ __device__ inline void update(const Step& s, float& p, float g, float& m, float&
     p -= s.lr * (upd + s.wd * p);
 }
 
-// A wavefront takes a block of 256 elements, a lane its elements lane, lane + 64, lane + 128 and lane + 192.
+// A wavefront takes what a tensor has behind its last whole block of 256 elements, a lane its elements lane, lane + 64, lane + 128 and lane + 192.
 template <typename G, bool EIGHT>
 __device__ inline void block_any(const One& t, const Step& s, uint32_t key, int64_t block, float gs, Powers power_of_two) {
     const int lane = threadIdx.x & 63;
@@ -204,16 +204,21 @@ __device__ inline void block_any(const One& t, const Step& s, uint32_t key, int6
     }
 }
 
-// The same for whole blocks of aligned tensors: a lane takes four neighbours, 16 bytes of 32-bit tensors and four of 8-bit ones. Parameters and moments are not
+// The same for whole blocks: a lane takes four neighbours, 16 bytes of 32-bit tensors and four of 8-bit ones, which the hardware moves from where the elements may lie. Parameters and moments are not
 // read again before the next step and pass by the last-level cache, which keeps the gradients from the norm's pass and the copies for the next
-// products (35 M parameters, 8-bit moments, clip and copies 155.7 -> 141.7 us).
+// products (35 M parameters, 8-bit moments, clip and copies 155.7 -> 141.7 us); one element off 221 -> 137 against a block element by
+// element).
+typedef f32x4 f32x4_any __attribute__((aligned(4)));
+typedef u32x2 u32x2_any __attribute__((aligned(2)));
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+typedef uint32_t u32_any __attribute__((aligned(1)));
 template <typename V>
 __device__ inline V load_past(const void* p) { return __builtin_nontemporal_load(static_cast<const V*>(p)); }
 template <typename V>
 __device__ inline void store_past(void* p, V v) { __builtin_nontemporal_store(v, static_cast<V*>(p)); }
-__device__ inline f32x4 four(const float* p, int64_t i) { return *reinterpret_cast<const f32x4*>(p + i); }
+__device__ inline f32x4 four(const float* p, int64_t i) { return *reinterpret_cast<const f32x4_any*>(p + i); }
 __device__ inline f32x4 four(const uint16_t* p, int64_t i) {
-    const u32x2 r = *reinterpret_cast<const u32x2*>(p + i);
+    const u32x2 r = *reinterpret_cast<const u32x2_any*>(p + i);
     return f32x4{__uint_as_float(r[0] << 16), __uint_as_float(r[0] & 0xFFFF0000u), __uint_as_float(r[1] << 16), __uint_as_float(r[1] & 0xFFFF0000u)};
 }
 template <typename G, bool EIGHT>
@@ -221,17 +226,17 @@ __device__ inline void block_whole(const One& t, const Step& s, uint32_t key, in
     const int lane = threadIdx.x & 63;
     const int64_t i = block * BLOCK + lane * 4;
     const f32x4 g = four(static_cast<const G*>(t.g), i);
-    f32x4 p = load_past<f32x4>(t.p + i), m, v;
+    f32x4 p = load_past<f32x4_any>(t.p + i), m, v;
     if constexpr (EIGHT) {
-        const uint32_t mc = load_past<uint32_t>(static_cast<const uint8_t*>(t.m) + i), vc = load_past<uint32_t>(static_cast<const uint8_t*>(t.v) + i);
+        const uint32_t mc = load_past<u32_any>(static_cast<const uint8_t*>(t.m) + i), vc = load_past<u32_any>(static_cast<const uint8_t*>(t.v) + i);
         const float ms = t.ms[block], vs = t.vs[block];
         const auto m0 = __builtin_amdgcn_cvt_pk_f32_fp8(mc, false), m1 = __builtin_amdgcn_cvt_pk_f32_fp8(mc, true);
         const auto v0 = __builtin_amdgcn_cvt_pk_f32_bf8(vc, false), v1 = __builtin_amdgcn_cvt_pk_f32_bf8(vc, true);
         m = f32x4{m0[0] * ms, m0[1] * ms, m1[0] * ms, m1[1] * ms};
         v = f32x4{v0[0] * vs, v0[1] * vs, v1[0] * vs, v1[1] * vs};
     } else {
-        m = load_past<f32x4>(static_cast<const float*>(t.m) + i);
-        v = load_past<f32x4>(static_cast<const float*>(t.v) + i);
+        m = load_past<f32x4_any>(static_cast<const float*>(t.m) + i);
+        v = load_past<f32x4_any>(static_cast<const float*>(t.v) + i);
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -239,11 +244,11 @@ __device__ inline void block_whole(const One& t, const Step& s, uint32_t key, in
         update(s, pk, g[k] * gs, mk, vk);
         p[k] = pk, m[k] = mk, v[k] = vk;
     }
-    store_past(t.p + i, p);
-    if (t.copy) *reinterpret_cast<u32x2*>(t.copy + i) = u32x2{pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3])};
+    store_past<f32x4_any>(t.p + i, p);
+    if (t.copy) *reinterpret_cast<u32x2_any*>(t.copy + i) = u32x2{pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3])};
     if constexpr (!EIGHT) {
-        store_past(static_cast<float*>(t.m) + i, m);
-        store_past(static_cast<float*>(t.v) + i, v);
+        store_past<f32x4_any>(static_cast<float*>(t.m) + i, m);
+        store_past<f32x4_any>(static_cast<float*>(t.v) + i, v);
     } else {
         uint32_t mm = 0, vm = 0;
 #pragma unroll
@@ -266,18 +271,10 @@ __device__ inline void block_whole(const One& t, const Step& s, uint32_t key, in
             mc |= to_e4m3(m[k] * mi, h & 0xFFFFu) << (8 * k);
             vc |= max(to_e5m2(v[k] * vi, h >> 16), v[k] > 0.0f ? 1u : 0u) << (8 * k);
         }
-        store_past(static_cast<uint8_t*>(t.m) + i, m_fine ? mc : 0x7F7F7F7Fu);
-        store_past(static_cast<uint8_t*>(t.v) + i, v_fine ? vc : 0x7F7F7F7Fu);
+        store_past<u32_any>(static_cast<uint8_t*>(t.m) + i, m_fine ? mc : 0x7F7F7F7Fu);
+        store_past<u32_any>(static_cast<uint8_t*>(t.v) + i, v_fine ? vc : 0x7F7F7F7Fu);
     }
 }
-template <typename G, bool EIGHT>
-__device__ inline bool aligned_for_whole(const One& t) {
-    const auto at = [](const void* p) { return reinterpret_cast<uintptr_t>(p); };
-    const uintptr_t sixteen = at(t.p) | (sizeof(G) == 4 ? at(t.g) : 0) | (EIGHT ? 0 : at(t.m) | at(t.v));
-    const uintptr_t eight = (sizeof(G) == 2 ? at(t.g) : 0) | at(t.copy), quad = EIGHT ? at(t.m) | at(t.v) : 0;
-    return (sixteen & 15) == 0 && (eight & 7) == 0 && (quad & 3) == 0;
-}
-
 __host__ __device__ inline uint32_t key_of(uint32_t seed, int place) { return mix(seed * 0x9E3779B9u + mix(static_cast<uint32_t>(place) + 0x3C6EF373u)); }
 
 template <typename G, bool EIGHT, bool COPY>
@@ -286,7 +283,7 @@ __global__ __launch_bounds__(NT) void adamw_many_k(Table<pointers(EIGHT, COPY)> 
     One t{tab.template at<float>(j, 0), tab.template at<const void>(j, 1), tab.template at<void>(j, 2), tab.template at<void>(j, 3), nullptr, nullptr, nullptr, tab.elements(j)};
     if constexpr (EIGHT) t.ms = tab.template at<float>(j, 4), t.vs = tab.template at<float>(j, 5);
     if constexpr (COPY) t.copy = tab.template at<uint16_t>(j, EIGHT ? 6 : 4);
-    const int64_t blocks = (t.n + BLOCK - 1) / BLOCK, whole = aligned_for_whole<G, EIGHT>(t) ? t.n / BLOCK : 0;
+    const int64_t blocks = (t.n + BLOCK - 1) / BLOCK, whole = t.n / BLOCK;
     const int64_t begin = static_cast<int64_t>(group - tab.first(j)) * tab.per, end = min(begin + tab.per, blocks);
     const uint32_t key = key_of(tab.seed, tab.place + j);
     const float gs = s.factor ? *s.factor : 1.0f;
@@ -312,29 +309,26 @@ __global__ __launch_bounds__(NT) void squares_k(Table<1> tab, double* part) {
     const int count = static_cast<int>(min(tab.elements(j) - begin, static_cast<int64_t>(SQ_ELEMS)));
     const G* g = tab.template at<const G>(j, 0) + begin;
     double q[4] = {0.0, 0.0, 0.0, 0.0};  // chains of additions
-    int from = 0;
-    if ((reinterpret_cast<uintptr_t>(g) & 15) == 0) {  // 16 bytes a lane, four loads on their way
-        from = count / N * N;
-        for (int p0 = threadIdx.x; p0 < count / N; p0 += U * NT) {
-            u32x4 v[U];
+    // 16 bytes a lane, four loads on their way
+    for (int p0 = threadIdx.x; p0 < count / N; p0 += U * NT) {
+        u32x4 v[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) v[u] = p0 + u * NT < count / N ? *reinterpret_cast<const u32x4*>(g + (p0 + u * NT) * N) : u32x4{0, 0, 0, 0};
+        for (int u = 0; u < U; ++u) v[u] = p0 + u * NT < count / N ? *reinterpret_cast<const u32x4_any*>(g + (p0 + u * NT) * N) : u32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
+        for (int u = 0; u < U; ++u) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if constexpr (N == 4) {
-                        const double x = __uint_as_float(v[u][e]);
-                        q[e] = fma(x, x, q[e]);
-                    } else {
-                        const double x = __uint_as_float(v[u][e] << 16), y = __uint_as_float(v[u][e] & 0xFFFF0000u);
-                        q[e] = fma(y, y, fma(x, x, q[e]));
-                    }
+            for (int e = 0; e < 4; ++e) {
+                if constexpr (N == 4) {
+                    const double x = __uint_as_float(v[u][e]);
+                    q[e] = fma(x, x, q[e]);
+                } else {
+                    const double x = __uint_as_float(v[u][e] << 16), y = __uint_as_float(v[u][e] & 0xFFFF0000u);
+                    q[e] = fma(y, y, fma(x, x, q[e]));
                 }
             }
         }
     }
-    for (int i = from + threadIdx.x; i < count; i += NT) {
+    for (int i = count / N * N + threadIdx.x; i < count; i += NT) {
         const double x = elem(g, i);
         q[0] = fma(x, x, q[0]);
     }
