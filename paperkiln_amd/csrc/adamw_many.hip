@@ -206,8 +206,8 @@ __device__ inline void block_any(const One& t, const Step& s, uint32_t key, int6
 
 // The same for whole blocks: a lane takes four neighbours, 16 bytes of 32-bit tensors and four of 8-bit ones, which the hardware moves from where the elements may lie. Parameters and moments are not
 // read again before the next step and pass by the last-level cache, which keeps the gradients from the norm's pass and the copies for the next
-// products (35 M parameters, 8-bit moments, clip and copies 155.7 -> 141.7 us); one element off 221 -> 137 against a block element by
-// element).
+// products (35 M parameters, 8-bit moments, clip and copies 155.7 -> 141.7 us; one element off 221 element by element,
+// 137 so).
 typedef f32x4 f32x4_any __attribute__((aligned(4)));
 typedef u32x2 u32x2_any __attribute__((aligned(2)));
 typedef u32x4 u32x4_any __attribute__((aligned(2)));

@@ -467,20 +467,21 @@ __device__ inline PairOut pair_terms(const Pairs& a, double chosen, double rejec
                    static_cast<float>((e * yes - (1.0 - e) * no) * a.beta * a.upstream / a.pairs)};
 }
 __device__ inline int64_t start_of(const Pairs& a, int seq) { return min(max(static_cast<int64_t>(a.starts[seq]), int64_t{0}), a.rows); }  // offsets that lie are held to the rows there are
-// What a sequence's rows from `begin` on give to its sum, to lane l of n; four rows' loads on their way together.
+// What a sequence's rows from `begin` on give to its sum, to lane l of n; U rows' loads on their way together.
+template <int U>
 __device__ inline double sequence_part(const Pairs& a, int64_t begin, int64_t end, int l, int n) {
     double s = 0.0;
-    for (int64_t r0 = begin + l; r0 < end; r0 += 4 * n) {
-        double logp[4];
-        float ref[4];
-        bool counts[4];
+    for (int64_t r0 = begin + l; r0 < end; r0 += U * n) {
+        double logp[U];
+        float ref[U];
+        bool counts[U];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < U; ++k) {
             const int64_t r = min(r0 + k * n, end - 1);
             counts[k] = a.targets[r] >= 0 && r0 + k * n < end, logp[k] = a.logp[r], ref[k] = a.ref[r];
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) s += counts[k] ? logp[k] - static_cast<double>(ref[k]) : 0.0;
+        for (int k = 0; k < U; ++k) s += counts[k] ? logp[k] - static_cast<double>(ref[k]) : 0.0;
     }
     return s;
 }
@@ -492,8 +493,8 @@ __device__ inline double wave_sum(double s) {
 // A few short pairs are formed by who wants them: a wavefront, or a workgroup.
 __device__ inline PairOut pair_of_wave(const Pairs& a, int pair) {
     const int lane = threadIdx.x & 63;
-    const double chosen = sequence_part(a, start_of(a, pair), start_of(a, pair + 1), lane, 64);
-    const double rejected = sequence_part(a, start_of(a, a.pairs + pair), start_of(a, a.pairs + pair + 1), lane, 64);
+    const double chosen = sequence_part<4>(a, start_of(a, pair), start_of(a, pair + 1), lane, 64);
+    const double rejected = sequence_part<4>(a, start_of(a, a.pairs + pair), start_of(a, a.pairs + pair + 1), lane, 64);
     return pair_terms(a, wave_sum(chosen), wave_sum(rejected));
 }
 // Row r's sequence, or -1.
@@ -609,7 +610,7 @@ __global__ __launch_bounds__(PAIR_NT) void pair_loss(Pairs a) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
         begin[k] = start_of(a, seq[k]), end[k] = start_of(a, seq[k] + 1);
-        sum[k] = wave_sum(sequence_part(a, begin[k], end[k], tid, PAIR_NT));
+        sum[k] = wave_sum(sequence_part<1>(a, begin[k], end[k], tid, PAIR_NT));
         if ((tid & 63) == 0) sh[k][tid >> 6] = sum[k];
     }
     __syncthreads();
