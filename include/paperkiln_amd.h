@@ -348,7 +348,8 @@ int pk_policy_loss(const pk_policy_config* c, const void* logits, int64_t ld, co
  * the chosen answers, pairs .. 2*pairs-1 the rejected ones. Rows with a negative target (prompts, padding) count
  * nothing. With s = sum of logp - ref_logp over a sequence's rows and e = label_smoothing,
  *   margins[i] = u_i = beta (s_i - s_{pairs+i}),  loss = mean_i( -(1-e) log sigma(u_i) - e log sigma(-u_i) ).
- * dlogits is the gradient of upstream * loss; rows of no sequence get zeros. logp as in pk_token_logprobs_fwd. */
+ * dlogits is the gradient of upstream * loss; rows of no sequence get zeros. logp as in pk_token_logprobs_fwd. pairs:
+ * 1 to 2^22 - 2. */
 typedef struct pk_preference_config {
     float beta, label_smoothing, scale, upstream;
 } pk_preference_config;
@@ -368,7 +369,7 @@ int pk_preference_loss(const pk_preference_config* c, const void* logits, int64_
  * in either. Values between two of the format's are rounded up or down at random with the value itself as the mean,
  * drawn from (seed, the tensor's place in the list, the element's place in the tensor): give another seed each step. A v
  * that is not zero does not become zero. A block in which a value is not finite becomes NaN.
- * A parameter, state or copy that is in the list twice is refused. */
+ * A parameter, state or copy that is in the list twice is refused, and so are more than 2^35 elements in all. */
 typedef struct pk_adamw_tensor {
     float* p;
     const void* g;           /* fp32 or bf16, the same for all (grad_dtype) */

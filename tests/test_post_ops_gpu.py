@@ -1011,6 +1011,42 @@ def test_operators_under_graph_capture(pk):
         assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip((*state.m, *state.v), (*estate.m, *estate.v)))
 
 
+def test_larger_calls_under_graph_capture(pk):
+    """What takes more launches than the calls above: a preference loss over many rows, dealt-out rows, gradients of long logs, lists of several tables."""
+    x, t, g = loss_inputs(700, 3001, BF16, 4)
+    y, u, _ = loss_inputs(3, 150001, FP32, 5)
+    starts, ref = torch.tensor([0, 300, 700], dtype=torch.int32, device="cuda"), torch.full((700,), -8.0, device="cuda")
+    dlogp = torch.ones(3, device="cuda")
+    ps, gs = ([torch.zeros(n, device="cuda") for n in [3000] + [40] * 300] for _ in range(2))
+    state = pk.blockops.adamw_state(ps, 32)
+
+    def calls():
+        logp, lse = pk.ops.token_logprobs_fwd(y, u)
+        return (*pk.blockops.preference_loss(x, t, starts, ref), logp, lse, pk.ops.token_logprobs_bwd(y, u, lse, dlogp))
+
+    def step(ps, state):
+        return pk.blockops.adamw_many_(ps, gs, state, 0.01, t=2, max_norm=1.0)
+
+    graph, out = graph_of(calls)
+    graph2, norm = graph_of(lambda: step(ps, state))
+    for again in range(3):
+        x.copy_(torch.randn(x.shape, generator=g, device="cuda").to(BF16))
+        y.copy_(torch.randn(y.shape, generator=g, device="cuda") + 3000 * (again == 1))
+        for v in gs:
+            v.normal_(generator=g)
+        for v in (*ps, *state.m, *state.v):
+            v.fill_(0.5)
+        eager = [v.clone() for v in ps]
+        estate = pk.blockops.AdamWState([v.clone() for v in state.m], [v.clone() for v in state.v])
+        enorm = step(eager, estate)
+        want = [v.clone() for v in calls()]
+        graph.replay()
+        graph2.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), again
+        assert torch.equal(norm, enorm) and all(torch.equal(a, b) for a, b in zip((*ps, *state.m, *state.v), (*eager, *estate.m, *estate.v))), again
+
+
 def test_a_backward_pass_under_graph_capture(pk):
     """Both nodes recorded with the passes around them and replayed between eager calls. While an eager graph of the same leaves lives, their gradients belong
     to its stream, which must not wait for a recording: refused, and the next recording stands."""
