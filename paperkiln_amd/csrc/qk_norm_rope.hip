@@ -35,6 +35,7 @@ struct Qk {
     int64_t pos_sb;
     float* part;          // backward: a workgroup's sums of dw, queries' then keys'
     int B, T, Hq, Hkv, dk, rotary, halves;
+    int pack;             // row kernels: a wavefront takes 2^pack tokens at a time
     float eps, per_dk;        // 1 / dk
     // Turns that a position moves pair p by, theta^(-2p/R) / 2 pi, as coarse[p / 8] * fine[p % 8]: two factors that are rounded once each.
     double coarse[MAX_PAIRS / 8], fine[8];
@@ -180,7 +181,7 @@ __global__ __launch_bounds__(NT) void qk_bwd_any(Qk a) {
 
 // ---- rows in 16-byte pieces ------------------------------------------------------------------------------------------
 // A group of G lanes takes a head's row, a lane eight of its columns as four pairs (a[i], b[i]): columns 8l .. 8l+7, or, where pairs come from two
-// halves, columns 4l .. and R/2 + 4l .., so that a pair never leaves its lane. A wavefront holds 64 / G rows of one token at a time and walks the
+// halves, columns 4l .. and R/2 + 4l .., so that a pair never leaves its lane. A wavefront holds 64 / G rows of one token, or of a few, at a time and walks the
 // token's heads, queries and keys as one list. The angles are the token's: 64 lanes form one pair's each and hand them round through a strip of LDS.
 
 struct Eight {  // vectors: as arrays the compiler kept half of one in LDS, by an offset that it read from the launch's packet in the host's memory (gqa forward 8.5 -> 22 us)
@@ -328,16 +329,29 @@ __device__ inline int column_b(int c0, int c1, int i) { return HALVES ? c1 + i :
 struct Angles {
     f32x4 c, s;
 };
-template <int G>
-__device__ inline Angles angles(const Qk& a, int pos, int p0, double near, double far, float2* strip) {
+// `pos`: the position of the wavefront's first token. A lane forms pairs of all its tokens in turn; p0 counts over all of them.
+template <int G, bool PACKED>
+__device__ inline Angles angles(const Qk& a, const int* pos, int tokens, int p0, double near, double far, float2* strip) {
     const int lane = threadIdx.x & 63;
     __builtin_amdgcn_wave_barrier();
+    if constexpr (!PACKED) {
+        const int at = *pos;
 #pragma unroll
-    for (int k = 0; k < (G + 15) / 16; ++k) {  // 4 G pairs, 64 lanes
-        const int p = lane + 64 * k;
-        float c = 1.0f, s = 0.0f;
-        if (p < a.rotary / 2) cos_sin(pos, k ? far : near, c, s);
-        if (p < 4 * G) strip[p] = make_float2(c, s);
+        for (int k = 0; k < (G + 15) / 16; ++k) {  // 4 G pairs, 64 lanes
+            const int p = lane + 64 * k;
+            float c = 1.0f, s = 0.0f;
+            if (p < a.rotary / 2) cos_sin(at, k ? far : near, c, s);
+            if (p < 4 * G) strip[p] = make_float2(c, s);
+        }
+    } else {
+        const int p = lane % (4 * G);
+#pragma unroll 1
+        for (int k = 0; 64 * k < 4 * G << a.pack; ++k) {
+            const int e = lane + 64 * k, token = e / (4 * G);
+            float c = 1.0f, s = 0.0f;
+            if ((G > 16 ? e % (4 * G) : p) < a.rotary / 2) cos_sin(pos[min(token, tokens - 1)], G > 16 && (k & 1) ? far : near, c, s);
+            if (e < 4 * G << a.pack) strip[e] = make_float2(c, s);
+        }
     }
     asm volatile("" ::: "memory");
     __builtin_amdgcn_wave_barrier();  // the strip is this wavefront's, whose LDS operations are in order
@@ -357,45 +371,63 @@ __device__ inline Eight weights_of(const float* w, int c0, int c1) {
     return e;
 }
 
-// A token's list of rows, 64 / G to a step, the queries' steps first, then the keys'. What a step needs is the wavefront's (scalars) but for the lane's offset,
-// and the next step's loads are on their way while one is worked on: with four steps unrolled the compiler formed every address ahead of the loop, 2600
-// instructions with spilled scalars in place of 500.
-template <typename T, int G, bool HALVES, bool LOOSE>
+// A wavefront takes 2^a.pack tokens, neighbours in a sequence, and of each a list of rows, 64 / G to a step over all of them, the queries' steps first, then the keys'. What
+// a step needs is the wavefront's (scalars) but for the lane's offset, and the next step's loads are on their way while one is worked on: with four steps unrolled the
+// compiler formed every address ahead of the loop, 2600 instructions with spilled scalars in place of 500.
+template <typename T, int G, bool HALVES, bool LOOSE, bool PACKED>
 struct List : Share<LOOSE> {
     using C = Cols<T, HALVES, LOOSE>;
     using Share<LOOSE>::c0;
     using Share<LOOSE>::c1;
     static constexpr int ROWS = 64 / G;
-    int g, q_steps, steps;
-    __device__ List(const Qk& a) : Share<LOOSE>(share<G, HALVES, LOOSE>((threadIdx.x & 63) % G, a.dk, a.rotary)), g((threadIdx.x & 63) / G) {
-        q_steps = (a.Hq + ROWS - 1) / ROWS;
-        steps = q_steps + (a.Hkv + ROWS - 1) / ROWS;
+    static constexpr uint32_t SIZE = sizeof(T);
+    int row, token, each, q_steps, steps;  // the lane's place in a step; rows of a token in it
+    __device__ List(const Qk& a) : Share<LOOSE>(share<G, HALVES, LOOSE>((threadIdx.x & 63) % G, a.dk, a.rotary)) {
+        const int g = (threadIdx.x & 63) / G;
+        const int bits = (G == 4 ? 4 : G == 8 ? 3 : G == 16 ? 2 : 1) - (PACKED ? a.pack : 0);  // each is a power of two
+        each = 1 << bits;
+        token = PACKED ? g >> bits : 0, row = g & (each - 1);
+        q_steps = (a.Hq + each - 1) >> bits;
+        steps = q_steps + ((a.Hkv + each - 1) >> bits);
     }
     struct Step {
         bool key;
         int head;   // its first
         bool live;  // whether the lane's group has a row in it
     };
-    __device__ Step step(const Qk& a, int s) const {
+    __device__ Step step(const Qk& a, int s, int tokens) const {
         const bool key = s >= q_steps;
-        const int head = (key ? s - q_steps : s) * ROWS;
-        return Step{key, head, head + g < (key ? a.Hkv : a.Hq)};
+        const int head = (key ? s - q_steps : s) * each;
+        return Step{key, head, head + row < (key ? a.Hkv : a.Hq) && (!PACKED || token < tokens)};
+    }
+    // What a lane's row lies behind the step's first one by, in bytes, in queries and keys. With one token it is formed where it is used: two registers fewer a tensor.
+    struct Lane {
+        uint32_t q, k;
+    };
+    template <typename P>
+    __device__ Lane lane(const P (&x)[2]) const {
+        if constexpr (!PACKED) return Lane{0, 0};
+        return Lane{(row * static_cast<uint32_t>(x[0].sh) + token * static_cast<uint32_t>(x[0].st)) * SIZE,
+                    (row * static_cast<uint32_t>(x[1].sh) + token * static_cast<uint32_t>(x[1].st)) * SIZE};
     }
     // the lane's row; groups without one take the step's first
     template <typename P>
-    __device__ static const char* row(const P (&x)[2], const Step& s, int64_t oq, int64_t ok, int g, uint32_t& off) {
+    __device__ const char* at(const P (&x)[2], const Step& s, int64_t oq, int64_t ok, const Lane& lane, uint32_t& off) const {
         const int64_t sh = s.key ? x[1].sh : x[0].sh;
-        off = s.live ? static_cast<uint32_t>(g) * static_cast<uint32_t>(sh * sizeof(T)) : 0u;
-        return static_cast<const char*>(s.key ? x[1].p : x[0].p) + ((s.key ? ok : oq) + s.head * sh) * static_cast<int64_t>(sizeof(T));
+        if constexpr (PACKED)
+            off = s.live ? s.key ? lane.k : lane.q : 0u;
+        else
+            off = s.live ? static_cast<uint32_t>(row) * static_cast<uint32_t>(sh * SIZE) : 0u;
+        return static_cast<const char*>(s.key ? x[1].p : x[0].p) + ((s.key ? ok : oq) + s.head * sh) * static_cast<int64_t>(SIZE);
     }
-    __device__ typename C::Raw load(const Rows (&x)[2], const Step& s, int64_t oq, int64_t ok) const {
+    __device__ typename C::Raw load(const Rows (&x)[2], const Step& s, int64_t oq, int64_t ok, const Lane& lane) const {
         uint32_t off;
-        const char* base = row(x, s, oq, ok, g, off);
-        return C::load(base, off + c0 * static_cast<uint32_t>(sizeof(T)), off + c1 * static_cast<uint32_t>(sizeof(T)));
+        const char* base = at(x, s, oq, ok, lane, off);
+        return C::load(base, off + c0 * SIZE, off + c1 * SIZE);
     }
-    __device__ void store(const RowsOut (&y)[2], const Step& s, int64_t oq, int64_t ok, const Eight& e) const {
+    __device__ void store(const RowsOut (&y)[2], const Step& s, int64_t oq, int64_t ok, const Lane& lane, const Eight& e) const {
         uint32_t off;
-        char* base = const_cast<char*>(row(y, s, oq, ok, g, off));
+        char* base = const_cast<char*>(at(y, s, oq, ok, lane, off));
         if constexpr (LOOSE) {
             if (!this->whole) {
                 T* to = reinterpret_cast<T*>(base + off);
@@ -407,33 +439,33 @@ struct List : Share<LOOSE> {
                 return;
             }
         }
-        C::store(base, off + c0 * static_cast<uint32_t>(sizeof(T)), off + c1 * static_cast<uint32_t>(sizeof(T)), e);
+        C::store(base, off + c0 * SIZE, off + c1 * SIZE, e);
     }
 };
 
-// grid.x: tokens, WAVES to a workgroup, in strides of the grid; grid.y: `per` steps of a token's list each.
-template <typename T, int G, bool HALVES, bool LOOSE>
+// grid.x: wavefronts' tokens, WAVES to a workgroup, in strides of the grid; grid.y: `per` steps of a token's list each.
+template <typename T, int G, bool HALVES, bool LOOSE, bool PACKED>
 __global__ __launch_bounds__(NT) void qk_fwd_rows(Qk a, int per) {
-    using L = List<T, G, HALVES, LOOSE>;
-    __shared__ float2 strips[WAVES][4 * G];
+    using L = List<T, G, HALVES, LOOSE, PACKED>;
+    __shared__ float2 strips[WAVES][PACKED ? 256 : 4 * G];  // 64 / G tokens at most
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), stride = static_cast<int>(gridDim.x) * WAVES;
     const L list(a);
     const Eight wq = weights_of<HALVES>(a.w[0], list.c0, list.c1), wk = weights_of<HALVES>(a.w[1], list.c0, list.c1);
-    const double near = turns_of(a, lane), far = G > 16 ? turns_of(a, lane + 64) : 0.0;
-    const int first = static_cast<int>(blockIdx.y) * per, last = min(first + per, list.steps), tokens = a.B * a.T;
+    const auto lx = list.lane(a.x), ly = list.lane(a.y);
+    const double near = turns_of(a, lane % (4 * G)), far = G > 16 ? turns_of(a, lane + 64) : 0.0;
+    const int first = static_cast<int>(blockIdx.y) * per, last = min(first + per, list.steps), pack = PACKED ? a.pack : 0, runs = (a.T + (1 << pack) - 1) >> pack, items = a.B * runs;
 #pragma unroll 1
-    for (int token = blockIdx.x * WAVES + wave; token < tokens; token += stride) {
-        const int b = a.B == 1 ? 0 : __builtin_amdgcn_readfirstlane(token / a.T), t = token - b * a.T;
-        const int pos = a.pos[b * a.pos_sb + t];
+    for (int item = blockIdx.x * WAVES + wave; item < items; item += stride) {
+        const int b = a.B == 1 ? 0 : __builtin_amdgcn_readfirstlane(item / runs), t = (item - b * runs) << pack, tokens = min(1 << pack, a.T - t);
         const int64_t xq = b * a.x[0].sb + t * a.x[0].st, xk = b * a.x[1].sb + t * a.x[1].st, yq = b * a.y[0].sb + t * a.y[0].st, yk = b * a.y[1].sb + t * a.y[1].st;
-        auto at = list.step(a, first);
-        typename L::C::Raw raw = list.load(a.x, at, xq, xk);
-        const Angles turn = angles<G>(a, pos, list.p0, near, far, strips[wave]);
+        auto at = list.step(a, first, tokens);
+        typename L::C::Raw raw = list.load(a.x, at, xq, xk, lx);
+        const Angles turn = angles<G, PACKED>(a, a.pos + b * a.pos_sb + t, tokens, list.token * 4 * G + list.p0, near, far, strips[wave]);
 #pragma unroll 1
         for (int s = first; s < last; ++s) {
             const auto now = at;
             const Eight x = L::C::unpack(raw);
-            if (s + 1 < last) at = list.step(a, s + 1), raw = list.load(a.x, at, xq, xk);
+            if (s + 1 < last) at = list.step(a, s + 1, tokens), raw = list.load(a.x, at, xq, xk, lx);
             float ss = 0.0f;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -450,36 +482,36 @@ __global__ __launch_bounds__(NT) void qk_fwd_rows(Qk a, int per) {
                 y.a[i] = ua * turn.c[i] - ub * turn.s[i];
                 y.b[i] = ua * turn.s[i] + ub * turn.c[i];
             }
-            if (list.mine && now.live) list.store(a.y, now, yq, yk, y);
+            if (list.mine && now.live) list.store(a.y, now, yq, yk, ly, y);
         }
     }
 }
 
-template <typename T, int G, bool HALVES, bool LOOSE>
+template <typename T, int G, bool HALVES, bool LOOSE, bool PACKED>
 __global__ __launch_bounds__(NT) void qk_bwd_rows(Qk a, int per) {
-    using L = List<T, G, HALVES, LOOSE>;
-    __shared__ float2 strips[WAVES][4 * G];
+    using L = List<T, G, HALVES, LOOSE, PACKED>;
+    __shared__ float2 strips[WAVES][PACKED ? 256 : 4 * G];  // 64 / G tokens at most
     __shared__ __align__(16) float sh[WAVES * L::ROWS * 2 * 8 * G];  // 16 KB
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), stride = static_cast<int>(gridDim.x) * WAVES;
     const L list(a);
     const Eight wq = weights_of<HALVES>(a.w[0], list.c0, list.c1), wk = weights_of<HALVES>(a.w[1], list.c0, list.c1);
-    const double near = turns_of(a, lane), far = G > 16 ? turns_of(a, lane + 64) : 0.0;
-    const int first = static_cast<int>(blockIdx.y) * per, last = min(first + per, list.steps), tokens = a.B * a.T;
+    const auto lx = list.lane(a.x), lg = list.lane(a.dy), ly = list.lane(a.y);
+    const double near = turns_of(a, lane % (4 * G)), far = G > 16 ? turns_of(a, lane + 64) : 0.0;
+    const int first = static_cast<int>(blockIdx.y) * per, last = min(first + per, list.steps), pack = PACKED ? a.pack : 0, runs = (a.T + (1 << pack) - 1) >> pack, items = a.B * runs;
     Eight dwq = {}, dwk = {};
 #pragma unroll 1
-    for (int token = blockIdx.x * WAVES + wave; token < tokens; token += stride) {
-        const int b = a.B == 1 ? 0 : __builtin_amdgcn_readfirstlane(token / a.T), t = token - b * a.T;
-        const int pos = a.pos[b * a.pos_sb + t];
+    for (int item = blockIdx.x * WAVES + wave; item < items; item += stride) {
+        const int b = a.B == 1 ? 0 : __builtin_amdgcn_readfirstlane(item / runs), t = (item - b * runs) << pack, tokens = min(1 << pack, a.T - t);
         const int64_t xq = b * a.x[0].sb + t * a.x[0].st, xk = b * a.x[1].sb + t * a.x[1].st, yq = b * a.y[0].sb + t * a.y[0].st, yk = b * a.y[1].sb + t * a.y[1].st;
         const int64_t gq = b * a.dy[0].sb + t * a.dy[0].st, gk = b * a.dy[1].sb + t * a.dy[1].st;
-        auto at = list.step(a, first);
-        typename L::C::Raw rx = list.load(a.x, at, xq, xk), rg = list.load(a.dy, at, gq, gk);
-        const Angles turn = angles<G>(a, pos, list.p0, near, far, strips[wave]);
+        auto at = list.step(a, first, tokens);
+        typename L::C::Raw rx = list.load(a.x, at, xq, xk, lx), rg = list.load(a.dy, at, gq, gk, lg);
+        const Angles turn = angles<G, PACKED>(a, a.pos + b * a.pos_sb + t, tokens, list.token * 4 * G + list.p0, near, far, strips[wave]);
 #pragma unroll 1
         for (int s = first; s < last; ++s) {
             const auto now = at;
             const Eight x = L::C::unpack(rx), dy = L::C::unpack(rg);
-            if (s + 1 < last) at = list.step(a, s + 1), rx = list.load(a.x, at, xq, xk), rg = list.load(a.dy, at, gq, gk);
+            if (s + 1 < last) at = list.step(a, s + 1, tokens), rx = list.load(a.x, at, xq, xk, lx), rg = list.load(a.dy, at, gq, gk, lg);
             Eight wdu, dux;
             float ss = 0.0f, sg = 0.0f;
 #pragma unroll
@@ -508,12 +540,12 @@ __global__ __launch_bounds__(NT) void qk_bwd_rows(Qk a, int per) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) dwq.a[i] += dux.a[i] * r, dwq.b[i] += dux.b[i] * r;
             }
-            list.store(a.y, now, yq, yk, dx);
+            list.store(a.y, now, yq, yk, ly, dx);
         }
     }
     // the sums of all groups of all wavefronts, columns in their order, then added up column by column
     constexpr int PITCH = 2 * 8 * G;
-    float* const own = sh + (wave * L::ROWS + list.g) * PITCH;
+    float* const own = sh + (wave * L::ROWS + lane / G) * PITCH;
     if (list.mine) {
         auto lay = [&](float* to, const Eight& d) {
             if constexpr (LOOSE) {
@@ -592,7 +624,7 @@ bool crossed(const pk_tensor4* q, const pk_tensor4* k, std::initializer_list<con
 
 void fill(Qk& a, const pk_qk_shape* s) {
     a.B = s->B, a.T = s->T, a.Hq = s->Hq, a.Hkv = s->Hkv, a.dk = s->dk, a.rotary = s->rotary ? s->rotary : s->dk, a.halves = s->halves != 0;
-    a.eps = s->eps, a.per_dk = 1.0f / static_cast<float>(s->dk), a.pos_sb = s->pos_stride_b, a.part = nullptr;
+    a.eps = s->eps, a.per_dk = 1.0f / static_cast<float>(s->dk), a.pos_sb = s->pos_stride_b, a.part = nullptr, a.pack = 0;
     for (int i = 0; i < MAX_PAIRS / 8; ++i) a.coarse[i] = i == 0 ? 1.0 : 16 * i < a.rotary ? std::pow(s->theta, -16.0 * i / a.rotary) : 0.0;
     for (int i = 0; i < 8; ++i) a.fine[i] = std::pow(s->theta, -2.0 * i / a.rotary) / 6.283185307179586476925;
 }
@@ -635,15 +667,39 @@ int lanes_of(const Qk& a) {
     return lanes <= 4 ? 4 : lanes <= 8 ? 8 : lanes <= 16 ? 16 : 32;
 }
 
+int steps_of(const Qk& a) {
+    const int rows = (64 / lanes_of(a)) >> a.pack;
+    return (a.Hq + rows - 1) / rows + (a.Hkv + rows - 1) / rows;
+}
+int64_t runs_of(const Qk& a) { return a.B * ((static_cast<int64_t>(a.T) + (1 << a.pack) - 1) >> a.pack); }
+// Tokens that a wavefront takes at a time, as a power of two. With few heads most of a token's steps are groups without a row; dealt to several tokens they are none, and a step's
+// 130 instructions are what bounds such shapes. Forward and backward, bf16: 32768 tokens, 1 + 1 heads of 64 by one token 18.0 and 32.0 us, by eight 6.0 and 11.8; 75348 tokens, 4 + 1
+// heads of 32 37.6 and 64.5, by sixteen 10.4 and 21; 8192 tokens, 14 + 2 heads of 64 8.0 and 15.9, by four 6.9 and 14.4; 74251, 8 + 2 of 72 50 and 95, by two 45 and 93. The
+// rows of a step lie further apart then, and not for nothing: steps that only become a fifth fewer cost fp32, whose bytes are twice as many, 2 %, and unaligned fp32 15 %.
+int pack_of(Qk a, int dtype, bool backward) {
+    for (int i = 0; i < 2; ++i)
+        for (const int64_t st : {a.x[i].st, a.y[i].st, backward ? a.dy[i].st : 0})  // with the heads' strides a lane's offset, in 32 bits
+            if (st < 0 || st > (1 << 24)) return 0;
+    const double alone = static_cast<double>(steps_of(a)) * runs_of(a), enough = dtype == PK_BF16 ? 1.15 : 1.6;
+    int best = 0;
+    double least = alone;
+    for (a.pack = 1; (64 / lanes_of(a)) >> a.pack; ++a.pack) {
+        if (runs_of(a) < 2048) break;  // wavefronts
+        const double steps = static_cast<double>(steps_of(a)) * runs_of(a);
+        if (steps < least && steps * enough <= alone) best = a.pack, least = steps;
+    }
+    return best;
+}
+
 // A launch of the row kernels: workgroups over tokens, parts that a token's heads are dealt to, `most` workgroups in all.
 struct Plan {
     int groups, parts, per;
 };
 // A token's heads stay with one wavefront, which forms the angles once, where the tokens alone fill the chip; fewer tokens are dealt out, to 4096 wavefronts.
 // Forward, 32 heads of 128: 4 tokens 5.7 us by a wavefront each, 2.4 dealt out; 2048 tokens 8.6 and 7.9, dealt to 16384 wavefronts 10.1; 4096 tokens 12.5 either way.
-Plan plan_of(const Qk& a, const pk_qk_shape* s, int most) {
-    const int rows = 64 / lanes_of(a), steps = (s->Hq + rows - 1) / rows + (s->Hkv + rows - 1) / rows;
-    const int64_t tokens = static_cast<int64_t>(s->B) * s->T, want = 4096;
+Plan plan_of(const Qk& a, int most) {
+    const int steps = steps_of(a);
+    const int64_t tokens = runs_of(a), want = 4096;
     int parts = 1;
     while (parts < steps && parts < most && tokens * parts < want) ++parts;
     Plan p;
@@ -654,14 +710,21 @@ Plan plan_of(const Qk& a, const pk_qk_shape* s, int most) {
     return p;
 }
 
-template <typename T, bool HALVES, bool LOOSE>
+template <typename T, int G, bool HALVES, bool LOOSE>
 void launch_rows(const Qk& a, const Plan& p, bool backward, hipStream_t st) {
     const dim3 grid(p.groups, p.parts);
+    if (a.pack)
+        backward ? qk_bwd_rows<T, G, HALVES, LOOSE, true><<<grid, NT, 0, st>>>(a, p.per) : qk_fwd_rows<T, G, HALVES, LOOSE, true><<<grid, NT, 0, st>>>(a, p.per);
+    else
+        backward ? qk_bwd_rows<T, G, HALVES, LOOSE, false><<<grid, NT, 0, st>>>(a, p.per) : qk_fwd_rows<T, G, HALVES, LOOSE, false><<<grid, NT, 0, st>>>(a, p.per);
+}
+template <typename T, bool HALVES, bool LOOSE>
+void launch_rows(const Qk& a, const Plan& p, bool backward, hipStream_t st) {
     switch (lanes_of(a)) {
-        case 4: return backward ? qk_bwd_rows<T, 4, HALVES, LOOSE><<<grid, NT, 0, st>>>(a, p.per) : qk_fwd_rows<T, 4, HALVES, LOOSE><<<grid, NT, 0, st>>>(a, p.per);
-        case 8: return backward ? qk_bwd_rows<T, 8, HALVES, LOOSE><<<grid, NT, 0, st>>>(a, p.per) : qk_fwd_rows<T, 8, HALVES, LOOSE><<<grid, NT, 0, st>>>(a, p.per);
-        case 16: return backward ? qk_bwd_rows<T, 16, HALVES, LOOSE><<<grid, NT, 0, st>>>(a, p.per) : qk_fwd_rows<T, 16, HALVES, LOOSE><<<grid, NT, 0, st>>>(a, p.per);
-        default: return backward ? qk_bwd_rows<T, 32, HALVES, LOOSE><<<grid, NT, 0, st>>>(a, p.per) : qk_fwd_rows<T, 32, HALVES, LOOSE><<<grid, NT, 0, st>>>(a, p.per);
+        case 4: return launch_rows<T, 4, HALVES, LOOSE>(a, p, backward, st);
+        case 8: return launch_rows<T, 8, HALVES, LOOSE>(a, p, backward, st);
+        case 16: return launch_rows<T, 16, HALVES, LOOSE>(a, p, backward, st);
+        default: return launch_rows<T, 32, HALVES, LOOSE>(a, p, backward, st);
     }
 }
 template <typename T>
@@ -705,7 +768,8 @@ int pk_qk_norm_rope_fwd(const pk_qk_shape* s, const pk_tensor4* q, const pk_tens
         hipStream_t st = static_cast<hipStream_t>(stream);
         if (const Serve by = serve(a, s, false); by != ANY) {
             flatten(a, false);
-            launch_rows(a, plan_of(a, s, FWD_MOST), false, by == LOOSE, s->dtype, st);
+            a.pack = pack_of(a, s->dtype, false);
+            launch_rows(a, plan_of(a, FWD_MOST), false, by == LOOSE, s->dtype, st);
             return launched();
         }
         const int64_t want = (items_of(s) + WAVES - 1) / WAVES;
@@ -722,7 +786,7 @@ size_t pk_qk_norm_rope_bwd_workspace_bytes(const pk_qk_shape* s) {
     if (check(s, "pk_qk_norm_rope_bwd_workspace_bytes")) return 0;
     Qk a;
     fill(a, s);
-    const Plan p = plan_of(a, s, BWD_MOST);
+    const Plan p = plan_of(a, BWD_MOST);
     return sizeof(float) * static_cast<size_t>(std::max(any_groups(s), p.groups * p.parts)) * 2 * s->dk;
 }
 
@@ -748,9 +812,10 @@ int pk_qk_norm_rope_bwd(const pk_qk_shape* s, const pk_tensor4* dyq, const pk_te
             a.x[0] = rows_of(q), a.x[1] = rows_of(k), a.dy[0] = rows_of(dyq), a.dy[1] = rows_of(dyk), a.y[0] = out_of(dq), a.y[1] = out_of(dk);
             touch({q->ptr, k->ptr, dyq->ptr, dyk->ptr, dq->ptr, dk->ptr}, stream);
             if (const Serve by = serve(a, s, true); by != ANY) {
-                const Plan p = plan_of(a, s, BWD_MOST);
-                groups = p.groups * p.parts;
                 flatten(a, true);
+                a.pack = pack_of(a, s->dtype, true);
+                const Plan p = plan_of(a, BWD_MOST);
+                groups = p.groups * p.parts;
                 launch_rows(a, p, true, by == LOOSE, s->dtype, st);
             } else if (s->dtype == PK_BF16)
                 qk_bwd_any<uint16_t><<<dim3(groups), NT, 0, st>>>(a);

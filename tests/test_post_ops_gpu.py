@@ -101,6 +101,11 @@ QK_CASES = [  # B, T, Hq, Hkv, dk, rotary, halves, layout, pos, far
     (1, 9, 5, 1, 14, 6, True, "plain", "rows", 3), (2, 11, 4, 2, 256, 250, True, "fused", "any", 7), (2, 11, 4, 2, 250, 0, True, "offset", "any", 7),
     (2, 11, 4, 2, 248, 234, True, "heads", "any", 7), (3, 40, 2, 2, 66, 2, True, "fused", "rows", 0), (3, 40, 2, 2, 66, 64, False, "heads", "rows", 0),
     (2, 40, 2, 2, 6, 4, True, "fused", "rows", 9), (2, 40, 2, 2, 4, 0, False, "offset", "rows", 9), (2, 700, 8, 2, 100, 52, True, "fused", "rows", 9),
+    # tokens enough for a wavefront to take several at a time, sequences that end inside its run
+    (3, 6001, 1, 1, 64, 0, False, "fused", "shared", 0), (40, 1031, 4, 1, 32, 16, True, "heads", "any", 9), (5, 2003, 5, 5, 80, 0, True, "plain", "rows", 900000),
+    (2, 5003, 8, 2, 72, 40, True, "offset", "any", 3), (9000, 1, 2, 2, 128, 0, False, "plain", "rows", 3), (9000, 1, 2, 2, 128, 0, False, "fused", "shared", 3),
+    (4, 2049, 14, 2, 64, 0, False, "fused", "rows", 0), (1, 5000, 1, 1, 200, 64, True, "plain", "any", 0), (3, 6001, 2, 1, 30, 22, True, "offset", "shared", 0),
+    (2, 9001, 3, 2, 250, 0, False, "heads", "any", 0), (7000, 3, 1, 2, 16, 6, False, "heads", "shared", 4),
     (1, 1, 4500, 3, 128, 0, True, "plain", "rows", 5), (1, 2, 3, 2100, 256, 0, False, "plain", "rows", 5)]
 
 
