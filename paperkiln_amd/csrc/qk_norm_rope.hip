@@ -429,17 +429,21 @@ struct List : Share<LOOSE> {
         uint32_t off;
         char* base = const_cast<char*>(at(y, s, oq, ok, lane, off));
         if constexpr (LOOSE) {
+            T* to = reinterpret_cast<T*>(base + off);
             if (!this->whole) {
-                T* to = reinterpret_cast<T*>(base + off);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     if (this->ka[i] != 0.0f) put(to, column_a<HALVES>(c0, c1, i), e.a[i]);
                     if (this->kb[i] != 0.0f) put(to, column_b<HALVES>(c0, c1, i), e.b[i]);
                 }
-                return;
             }
+            if (this->whole) {
+                C::store(base, off + c0 * SIZE, off + c1 * SIZE, e);
+                asm volatile("s_nop 1");  // the store's data stays for two issue slots in the order of the text, too, whatever the compiler places behind the branch
+            }
+        } else {
+            C::store(base, off + c0 * SIZE, off + c1 * SIZE, e);
         }
-        C::store(base, off + c0 * SIZE, off + c1 * SIZE, e);
     }
 };
 
