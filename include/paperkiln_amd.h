@@ -335,13 +335,16 @@ int pk_token_logprobs_bwd(const void* logits, int64_t ld, const int* targets, co
  *   L_r = -min(rho A, clamp(rho, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(d) - d - 1),  loss = sum_r weights[r] L_r;
  * dlogits is the gradient of upstream * loss. The weights carry mask and normalisation (1/tokens, 1/(sequences *
  * length), ...); a row of weight 0 or of a negative target is not read, its logp and gradient are 0. ref_logp may be
- * NULL where kl_coef is 0. row_loss[rows] (64 bits) receives weights[r] L_r, loss (device, fp32) their sum in a fixed order. */
+ * NULL where kl_coef is 0. row_loss[rows] (64 bits) receives weights[r] L_r, loss (device, fp32) their sum in a fixed order.
+ * With a workspace (its bytes may be 0) a few rows of large vocabularies are dealt to several workgroups each, as above. */
+size_t pk_policy_loss_workspace_bytes(int64_t rows, int64_t vocab, int dtype);
 typedef struct pk_policy_config {
     float clip_low, clip_high, kl_coef, scale, upstream;
 } pk_policy_config;
 int pk_policy_loss(const pk_policy_config* c, const void* logits, int64_t ld, const int* targets, const float* old_logp,
                    const float* ref_logp, const float* advantages, const float* weights, int64_t rows, int64_t vocab,
-                   void* dlogits, int64_t dld, float* logp, double* row_loss, float* loss, int dtype, void* stream);
+                   void* dlogits, int64_t dld, float* logp, double* row_loss, float* loss, void* workspace,
+                   size_t workspace_bytes, int dtype, void* stream);
 
 /* Preference loss over pairs of sequences, loss and gradient. Sequence s holds rows [seq_start[s], seq_start[s+1])
  * (seq_start[2*pairs + 1] on the device, ascending; offsets past the rows are held to them); sequences 0 .. pairs-1 are

@@ -78,7 +78,7 @@ EXPORTS = ["pk_last_error", "pk_init", "pk_attn_fwd", "pk_attn_bwd_workspace_byt
            "pk_op_cross_entropy", "pk_op_adamw", "pk_op_sumsq", "pk_op_gemm", "pk_set_gemm_backend", "pk_set_head_kernel",
            "pk_qk_norm_rope_fwd", "pk_qk_norm_rope_bwd_workspace_bytes", "pk_qk_norm_rope_bwd", "pk_token_logprobs_workspace_bytes", "pk_token_logprobs_fwd",
            "pk_token_logprobs_bwd",
-           "pk_policy_loss", "pk_preference_loss_workspace_bytes", "pk_preference_loss", "pk_adamw_many_workspace_bytes", "pk_adamw_many"]
+           "pk_policy_loss_workspace_bytes", "pk_policy_loss", "pk_preference_loss_workspace_bytes", "pk_preference_loss", "pk_adamw_many_workspace_bytes", "pk_adamw_many"]
 
 
 def lib() -> C.CDLL:
@@ -149,7 +149,9 @@ def lib() -> C.CDLL:
         L.pk_token_logprobs_workspace_bytes.argtypes = [i64, i64, ci]
         L.pk_token_logprobs_fwd.argtypes = [vp, i64, vp, i64, i64, cf, vp, vp, vp, sz, ci, vp]
         L.pk_token_logprobs_bwd.argtypes = [vp, i64, vp, vp, vp, i64, i64, cf, vp, i64, ci, vp]
-        L.pk_policy_loss.argtypes = [C.POINTER(PolicyConfig), vp, i64, vp, vp, vp, vp, vp, i64, i64, vp, i64, vp, vp, vp, ci, vp]
+        L.pk_policy_loss_workspace_bytes.restype = C.c_size_t
+        L.pk_policy_loss_workspace_bytes.argtypes = [i64, i64, ci]
+        L.pk_policy_loss.argtypes = [C.POINTER(PolicyConfig), vp, i64, vp, vp, vp, vp, vp, i64, i64, vp, i64, vp, vp, vp, vp, C.c_size_t, ci, vp]
         L.pk_preference_loss_workspace_bytes.argtypes = [i64, i64]
         L.pk_preference_loss.argtypes = [C.POINTER(PreferenceConfig), vp, i64, vp, vp, i64, vp, i64, i64, vp, i64, vp, vp, vp, vp, sz, ci, vp]
         L.pk_adamw_many_workspace_bytes.argtypes = [AT, ci, AC]

@@ -33,12 +33,14 @@ struct Loss {
     double* fine;             // LOGP: the log-probability in 64 bits, or null
     float* clear;             // LOGP: a word per row to set to zero, or null
     const float *lse_in, *coef;  // GRAD
-    const double* losses;     // GRAD: the pairs' losses, whose mean the workgroup behind the last row's writes to `loss`
-    int64_t pairs;
+    const double* losses;     // GRAD: the pairs' or rows' losses, whose sum over `divisor` the workgroup behind the last row's writes to `loss`
+    int64_t terms;
+    double divisor;
     float* loss;
     float2* parts;            // LOGP: room for the parts of rows that are dealt out, or null
     const float *old_logp, *ref_logp, *adv, *weights;  // POLICY; ref_logp may be null
     double* row_loss;
+    float* coef_out;  // POLICY, a row that is dealt out: what its gradient is multiplied by
     float clip_low, clip_high, kl, upstream;
 };
 enum Mode { LOGP, GRAD, POLICY };
@@ -95,9 +97,9 @@ __device__ inline double sum_of(const double* x, int64_t n) {
     return s;
 }
 template <int NT>
-__device__ inline void pairs_mean(const Loss& a) {
-    const double s = sum_of<NT>(a.losses, a.pairs);
-    if (threadIdx.x == 0) *a.loss = static_cast<float>(s / static_cast<double>(a.pairs));
+__device__ inline void losses_sum(const Loss& a) {
+    const double s = sum_of<NT>(a.losses, a.terms);
+    if (threadIdx.x == 0) *a.loss = static_cast<float>(s / a.divisor);
 }
 
 // log2 of the sum of 2^(s2 x) over a row: s2 top + log2. Its two parts stay apart, since their sum, in 32 bits, knows the second one no more where logits are large.
@@ -133,6 +135,7 @@ __device__ inline RowOut finish(const Loss& a, int64_t r, float xt, const RowSum
         policy_row(a, r, logp, loss, slope);
         w = a.weights[r];
         o.coef = static_cast<float>(w * slope * a.upstream * a.scale);
+        if (writes && a.coef_out) a.coef_out[r] = static_cast<float>(w * slope * a.upstream);
         o.target = o.coef * static_cast<float>(-expm1(logp));
     }
     if (writes) {
@@ -242,7 +245,10 @@ template <Mode MODE>
 __device__ inline void no_row(const Loss& a, int64_t r) {
     a.logp[r] = 0.0f;
     if (a.lse) a.lse[r] = 0.0f;
-    if (MODE == POLICY) a.row_loss[r] = 0.0;
+    if (MODE == POLICY) {
+        a.row_loss[r] = 0.0;
+        if (a.coef_out) a.coef_out[r] = 0.0f;
+    }
 }
 template <typename T, int NT, bool PAST>
 __device__ inline void zero_row(T* dx, const Cut<T>& cut, int tid) {
@@ -401,13 +407,13 @@ __global__ __launch_bounds__(LONG_NT) void rows_long(Loss a) {
 
 // A few such rows are dealt to several workgroups, `per` pieces each, which leave the largest logit and the sum of their part; a wavefront joins a row's.
 constexpr int PART_NT = 512, MOST_PARTS = 32, FEW_ROWS = 128;
-template <typename T>
+template <typename T, Mode MODE>
 __global__ __launch_bounds__(PART_NT) void rows_part(Loss a, int per, float2* parts) {
     constexpr int WAVES = PART_NT / 64;
     __shared__ float sh_m[WAVES], sh_s[WAVES];
     const int64_t r = blockIdx.x;
     const int tid = threadIdx.x;
-    if (a.targets[r] < 0) return;
+    if (a.targets[r] < 0 || (MODE == POLICY && a.weights[r] == 0.0f)) return;
     const T* x = static_cast<const T*>(a.logits) + r * a.ld;
     const Cut<T> cut(x, a.vocab);
     const int from = static_cast<int>(blockIdx.y) * per, to = min(cut.pieces, from + per);
@@ -421,13 +427,13 @@ __global__ __launch_bounds__(PART_NT) void rows_part(Loss a, int per, float2* pa
     for (int w = 0; w < WAVES; ++w) s += sh_s[w] == 0.0f ? 0.0f : sh_s[w] * power_of(a, sh_m[w], top);
     parts[r * gridDim.y + blockIdx.y] = make_float2(top, s);
 }
-template <typename T>
+template <typename T, Mode MODE>
 __global__ __launch_bounds__(64) void rows_join(Loss a, int count, const float2* parts) {
     const int64_t r = blockIdx.x;
     const int lane = threadIdx.x, t = a.targets[r];
     if (a.clear && lane == 0) a.clear[r] = 0.0f;
-    if (t < 0) {
-        if (lane == 0) no_row<LOGP>(a, r);
+    if (t < 0 || (MODE == POLICY && a.weights[r] == 0.0f)) {
+        if (lane == 0) no_row<MODE>(a, r);
         return;
     }
     const float2 v = lane < count ? parts[r * count + lane] : make_float2(-INFINITY, 0.0f);
@@ -438,7 +444,7 @@ __global__ __launch_bounds__(64) void rows_join(Loss a, int count, const float2*
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
     const T* x = static_cast<const T*>(a.logits) + r * a.ld;
-    if (lane == 0) finish<LOGP>(a, r, t < a.vocab ? elem(x, t) : NAN, row_sum(top, sum));
+    if (lane == 0) finish<MODE>(a, r, t < a.vocab ? elem(x, t) : NAN, row_sum(top, sum));
 }
 
 // ---- pairs of sequences -----------------------------------------------------------------------------------------------------
@@ -534,7 +540,7 @@ __global__ __launch_bounds__(GRAD_NT) void rows_grad(Loss a, int per, Pairs pair
         if constexpr (FEW)
             few_pairs_mean<GRAD_NT>(pairs, a.loss);
         else
-            pairs_mean<GRAD_NT>(a);
+            losses_sum<GRAD_NT>(a);
         return;
     }
     const int64_t r = a.rows - 1 - blockIdx.x;  // the last rows first: they are what the pass before has left in the last-level cache
@@ -649,12 +655,19 @@ void launch_held(const Loss& a, hipStream_t st) {
     if (pieces <= HELD_PIECES) return rows_held<T, MODE, 1024, 8, PAST><<<grid, 1024, 0, st>>>(a);
     rows_long<T, MODE, PAST><<<grid, LONG_NT, 0, st>>>(a);
 }
-// Workgroups that a row is dealt to for its log-probability: one, but for a few rows that none holds. bf16, whole and dealt out: one row of 128000 words 8.7 and 5.6 us, 64 of
-// them 9.5 and 6.9, one of 200000 12.6 and 5.7, 64 13.6 and 8.8; a held row of 32000 words takes 4.1, less than the two launches.
-int parts_of_rows(int64_t rows, int64_t vocab, int64_t es) {
-    const int64_t pieces = vocab * es / 16;
-    if (rows < 1 || rows >= FEW_ROWS || pieces <= HELD_PIECES) return 1;
+// Workgroups that a row is dealt to: one, but for a few rows that none holds. bf16, log-probabilities whole and dealt out: one row of 128000 words 8.7 and 5.6 us, 64 of
+// them 9.5 and 6.9, one of 200000 12.6 and 5.7, 64 13.6 and 8.8; a held row of 32000 words takes 4.1, less than the two launches. The policy loss, with a pass of its own for the
+// gradient: one row of 34000 words 10.3 and 9.0, 31 of them 10.8 and 10.3, 127 11.9 and 13.1; one of 134000 20.2 and 9.2, 64 23.9 and 18.1, 250 36 and 41.
+int parts_of_rows(Mode mode, int64_t rows, int64_t vocab, int64_t es) {
+    const int64_t pieces = vocab * es / 16, held = mode == POLICY && rows <= 32 ? 4096 : HELD_PIECES;
+    if (rows < 1 || rows >= (mode == POLICY ? 65 : FEW_ROWS) || pieces <= held) return 1;
     return static_cast<int>(std::min<int64_t>(std::min<int64_t>(MOST_PARTS, 512 / rows), pieces / (2 * PART_NT)));
+}
+template <typename T, Mode MODE>
+void launch_dealt(const Loss& a, int parts, hipStream_t st) {
+    const int pieces = a.vocab / Piece<T>::N, per = (pieces + parts - 1) / parts;
+    rows_part<T, MODE><<<dim3(static_cast<unsigned>(a.rows), static_cast<unsigned>(parts)), PART_NT, 0, st>>>(a, per, a.parts);
+    rows_join<T, MODE><<<dim3(static_cast<unsigned>(a.rows)), 64, 0, st>>>(a, parts, a.parts);
 }
 template <typename T, int NT, bool PAST, bool FEW>
 void launch_grad(const Loss& a, const Pairs& pairs, hipStream_t st) {
@@ -668,21 +681,21 @@ void launch_typed(const Loss& a, const Pairs* pairs, hipStream_t st) {
     const bool past = a.rows * a.vocab * static_cast<int64_t>(sizeof(T)) >= PAST_BYTES;
     const dim3 grid(static_cast<unsigned>(a.rows + (a.loss ? 1 : 0)));
     if constexpr (MODE == LOGP) {
-        const int parts = a.parts ? parts_of_rows(a.rows, a.vocab, sizeof(T)) : 1;
+        const int parts = a.parts ? parts_of_rows(LOGP, a.rows, a.vocab, sizeof(T)) : 1;
         if (parts == 1) return launch_held<T, MODE, false>(a, st);  // the logits are read again for their gradient: not past the cache
-        const int pieces = a.vocab / Piece<T>::N, per = (pieces + parts - 1) / parts;
-        rows_part<T><<<dim3(static_cast<unsigned>(a.rows), static_cast<unsigned>(parts)), PART_NT, 0, st>>>(a, per, a.parts);
-        rows_join<T><<<dim3(static_cast<unsigned>(a.rows)), 64, 0, st>>>(a, parts, a.parts);
+        launch_dealt<T, MODE>(a, parts, st);
     } else {
         if constexpr (MODE == GRAD) {
             // Threads for a row: bf16, 65536 rows of 1000 words 48 us by 64 threads (57 by 128, 72 by 256, 122 by 512), 32768 of 2000 48 (48, 49, 70), 16384 of 4000 49 (48, 46,
             // 49), 8192 of 8000 49 (45, 44, 42), 8192 of 32000 208 (205, 193, 180). The pairs' mean is a workgroup's too: thousands of pairs want a large one.
             const int pieces = a.vocab / Piece<T>::N;
             if (pairs) return launch_grad<T, 512, false, true>(a, *pairs, st);
-            if (pieces <= 256 && a.pairs <= 4096) return past ? launch_grad<T, 64, true, false>(a, Pairs{}, st) : launch_grad<T, 64, false, false>(a, Pairs{}, st);
-            if (pieces <= 512 && a.pairs <= 4096) return past ? launch_grad<T, 256, true, false>(a, Pairs{}, st) : launch_grad<T, 256, false, false>(a, Pairs{}, st);
+            if (pieces <= 256 && a.terms <= 4096) return past ? launch_grad<T, 64, true, false>(a, Pairs{}, st) : launch_grad<T, 64, false, false>(a, Pairs{}, st);
+            if (pieces <= 512 && a.terms <= 4096) return past ? launch_grad<T, 256, true, false>(a, Pairs{}, st) : launch_grad<T, 256, false, false>(a, Pairs{}, st);
             past ? launch_grad<T, 512, true, false>(a, Pairs{}, st) : launch_grad<T, 512, false, false>(a, Pairs{}, st);
-        } else
+        } else if (a.parts)
+            launch_dealt<T, MODE>(a, parts_of_rows(POLICY, a.rows, a.vocab, sizeof(T)), st);
+        else
             past ? launch_held<T, MODE, true>(a, st) : launch_held<T, MODE, false>(a, st);
     }
 }
@@ -699,7 +712,7 @@ int launch_rows(const Loss& all, int dtype, hipStream_t st, const Pairs* pairs =
         if (r + MOST_ROWS < all.rows) a.loss = nullptr;  // the last run's
         a.logits = static_cast<const char*>(a.logits) + r * a.ld * es;
         if (a.dlogits) a.dlogits = static_cast<char*>(a.dlogits) + r * a.dld * es;
-        on(a.targets), on(a.logp), on(a.lse), on(a.lse_in), on(a.coef), on(a.clear), on(a.fine), on(a.old_logp), on(a.ref_logp), on(a.adv), on(a.weights), on(a.row_loss);
+        on(a.targets), on(a.logp), on(a.lse), on(a.lse_in), on(a.coef), on(a.clear), on(a.fine), on(a.old_logp), on(a.ref_logp), on(a.adv), on(a.weights), on(a.row_loss), on(a.coef_out);
         if (dtype == PK_BF16)
             launch_typed<uint16_t, MODE>(a, pairs, st);
         else
@@ -745,7 +758,7 @@ extern "C" {
 
 size_t pk_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int dtype) {
     if (rows < 0 || vocab <= 0 || !known_dtype(dtype)) return 0;
-    const int parts = parts_of_rows(rows, vocab, elem_size(dtype));
+    const int parts = parts_of_rows(LOGP, rows, vocab, elem_size(dtype));
     return parts == 1 ? 0 : sizeof(float2) * static_cast<size_t>(rows * parts);
 }
 
@@ -779,9 +792,15 @@ int pk_token_logprobs_bwd(const void* logits, int64_t ld, const int* targets, co
     });
 }
 
+size_t pk_policy_loss_workspace_bytes(int64_t rows, int64_t vocab, int dtype) {
+    if (rows < 0 || vocab <= 0 || !known_dtype(dtype)) return 0;
+    const int parts = parts_of_rows(POLICY, rows, vocab, elem_size(dtype));
+    return parts == 1 ? 0 : (sizeof(float2) * parts + 2 * sizeof(float)) * static_cast<size_t>(rows);
+}
+
 int pk_policy_loss(const pk_policy_config* c, const void* logits, int64_t ld, const int* targets, const float* old_logp, const float* ref_logp,
                    const float* advantages, const float* weights, int64_t rows, int64_t vocab, void* dlogits, int64_t dld, float* logp,
-                   double* row_loss, float* loss, int dtype, void* stream) {
+                   double* row_loss, float* loss, void* workspace, size_t workspace_bytes, int dtype, void* stream) {
     return c_entry([&] {
         if (!c || !loss) return fail(PK_ERR_ARGUMENT, "pk_policy_loss: null pointer");
         if (int rc = check("pk_policy_loss", logits, ld, targets, rows, vocab, c->scale, dtype, true, dlogits, dld)) return rc;
@@ -789,7 +808,9 @@ int pk_policy_loss(const pk_policy_config* c, const void* logits, int64_t ld, co
         if (!(c->clip_low >= 0.0f) || !(c->clip_high >= 0.0f)) return fail(PK_ERR_ARGUMENT, "pk_policy_loss: the clip's widths must not be negative");
         if (!std::isfinite(c->kl_coef) || !std::isfinite(c->upstream)) return fail(PK_ERR_ARGUMENT, "pk_policy_loss: kl_coef and upstream must be finite");
         if (c->kl_coef != 0.0f && !ref_logp && rows > 0) return fail(PK_ERR_ARGUMENT, "pk_policy_loss: a KL term needs ref_logp");
-        touch({logits, targets, old_logp, ref_logp, advantages, weights, dlogits, logp, row_loss, loss}, stream);
+        if (workspace && (workspace_bytes < pk_policy_loss_workspace_bytes(rows, vocab, dtype) || !aligned(workspace, 8)))
+            return fail(PK_ERR_WORKSPACE, "pk_policy_loss: workspace too small (pk_policy_loss_workspace_bytes)");
+        touch({logits, targets, old_logp, ref_logp, advantages, weights, dlogits, logp, row_loss, loss, workspace}, stream);
         hipStream_t st = static_cast<hipStream_t>(stream);
         Loss a{};
         a.logits = logits, a.ld = ld, a.targets = targets, a.rows = rows, a.vocab = static_cast<int>(vocab);
@@ -797,6 +818,14 @@ int pk_policy_loss(const pk_policy_config* c, const void* logits, int64_t ld, co
         a.dlogits = dlogits, a.dld = dld, a.logp = logp, a.row_loss = row_loss;
         a.old_logp = old_logp, a.ref_logp = c->kl_coef != 0.0f ? ref_logp : nullptr, a.adv = advantages, a.weights = weights;
         a.clip_low = c->clip_low, a.clip_high = c->clip_high, a.kl = c->kl_coef, a.upstream = c->upstream;
+        const int parts = workspace ? parts_of_rows(POLICY, rows, vocab, elem_size(dtype)) : 1;
+        if (parts > 1) {  // the gradient in a pass of its own, once the rows' parts are joined
+            a.parts = static_cast<float2*>(workspace);
+            a.lse = reinterpret_cast<float*>(a.parts + rows * parts), a.coef_out = a.lse + rows;
+            if (int rc = launch_rows<POLICY>(a, dtype, st)) return rc;
+            a.parts = nullptr, a.lse_in = a.lse, a.coef = a.coef_out, a.losses = row_loss, a.terms = rows, a.divisor = 1.0, a.loss = loss;
+            return launch_rows<GRAD>(a, dtype, st);
+        }
         if (int rc = launch_rows<POLICY>(a, dtype, st)) return rc;
         loss_sum<<<1, 1024, 0, st>>>(row_loss, rows, loss);
         return launched();
@@ -841,7 +870,7 @@ int pk_preference_loss(const pk_preference_config* c, const void* logits, int64_
             pair_loss<<<dim3(static_cast<unsigned>(pairs)), PAIR_NT, 0, st>>>(p);
             if (int rc = launched()) return rc;
         }
-        a.lse_in = lse, a.coef = coef, a.losses = losses, a.pairs = pairs, a.loss = loss;
+        a.lse_in = lse, a.coef = coef, a.losses = losses, a.terms = pairs, a.divisor = static_cast<double>(pairs), a.loss = loss;
         return launch_rows<GRAD>(a, dtype, st, few ? &p : nullptr);
     });
 }

@@ -260,11 +260,13 @@ std::vector<Tensor> policy(const Tensor& logits, const Tensor& targets, const Te
     c10::DeviceGuard on(logits.device());
     at::AutoDispatchBelowAutograd below;
     Tensor d = gradient_of(who, logits, out), logp = new_tensor({m.rows}, at::kFloat, logits), rows = new_tensor({m.rows}, at::kDouble, logits),
-           loss = new_tensor({}, at::kFloat, logits);
+           loss = new_tensor({}, at::kFloat, logits), ws;
+    const size_t bytes = pk_policy_loss_workspace_bytes(m.rows, m.vocab, m.dtype);
+    if (bytes) ws = new_tensor({static_cast<int64_t>(bytes)}, at::kByte, logits);
     const Logits g = matrix(who, "out", d);
     check(pk_policy_loss(&c, logits.const_data_ptr(), m.ld, targets.const_data_ptr<int>(), old.const_data_ptr<float>(),
                          ref.defined() ? ref.const_data_ptr<float>() : nullptr, adv.const_data_ptr<float>(), weights.const_data_ptr<float>(), m.rows, m.vocab,
-                         d.data_ptr(), g.ld, logp.data_ptr<float>(), rows.data_ptr<double>(), loss.data_ptr<float>(), m.dtype, stream()));
+                         d.data_ptr(), g.ld, logp.data_ptr<float>(), rows.data_ptr<double>(), loss.data_ptr<float>(), bytes ? ws.data_ptr() : nullptr, bytes, m.dtype, stream()));
     if (out.defined()) changed(out);
     return {std::move(loss), std::move(d), std::move(logp)};
 }

@@ -84,7 +84,7 @@ def call(entry, **kw):
         return L.pk_token_logprobs_bwd(*x, d["v"], d["v"], d["rows"], d["vocab"], d["scale"], d["dlogits"], d["dld"], d["dtype"], None)
     if entry == "policy":
         c = _lib.PolicyConfig(d["low"], d["high"], d["kl"], d["scale"], d["upstream"])
-        return L.pk_policy_loss(C.byref(c), *x, d["v"], d["ref"], d["v"], d["v"], d["rows"], d["vocab"], d["dlogits"], d["dld"], d["v"], d["v"], d["loss"], d["dtype"], None)
+        return L.pk_policy_loss(C.byref(c), *x, d["v"], d["ref"], d["v"], d["v"], d["rows"], d["vocab"], d["dlogits"], d["dld"], d["v"], d["v"], d["loss"], d["ws"], d["ws_bytes"], d["dtype"], None)
     c = _lib.PreferenceConfig(d["beta"], d["smoothing"], d["scale"], d["upstream"])
     return L.pk_preference_loss(C.byref(c), *x, d["starts"], d["pairs"], d["ref"], d["rows"], d["vocab"], d["dlogits"], d["dld"], d["v"], d["v"], d["loss"], d["ws"],
                                 d["ws_bytes"], d["dtype"], None)
@@ -116,6 +116,10 @@ def test_token_logprobs_refuses():
     assert need == 3 * 32 * 8 and L.pk_token_logprobs_workspace_bytes(3, 32000, _lib.PK_F32) == 0 and L.pk_token_logprobs_workspace_bytes(128, 200000, _lib.PK_F32) == 0
     for ws, size in ((SOME, need - 1), (C.c_void_p((1 << 20) + 4), need)):
         assert L.pk_token_logprobs_fwd(SOME, 200000, SOME, 3, 200000, 1.0, SOME, None, ws, size, _lib.PK_F32, None) == WORKSPACE
+    need = L.pk_policy_loss_workspace_bytes(3, 200000, _lib.PK_F32)   # the same, and two words a row
+    assert need == 3 * (32 * 8 + 8) and L.pk_policy_loss_workspace_bytes(3, 16000, _lib.PK_F32) == 0 and L.pk_policy_loss_workspace_bytes(65, 200000, _lib.PK_F32) == 0
+    for ws, size in ((SOME, need - 1), (C.c_void_p((1 << 20) + 4), need)):
+        assert call("policy", rows=3, vocab=200000, ld=200000, dld=200000, ws=ws, ws_bytes=size) == WORKSPACE
     assert L.pk_preference_loss_workspace_bytes(1000, 3) == 4096 + 4096 + 8192 + 256
     assert L.pk_preference_loss_workspace_bytes(100, 3) == 512 + 512 + 1024 + 256 + 100 * 32 * 8
 

@@ -471,6 +471,42 @@ def test_policy_loss_against_64_bits(pk, case, kl, dtype):
     assert res[1] is over and same_bits(over, same[1]) and same_bits(res[0], same[0])
 
 
+@pytest.mark.parametrize("rows,vocab,dtype", [(1, 33001, BF16), (32, 33001, BF16), (33, 66001, BF16), (64, 34007, FP32), (2, 200001, FP32)])
+def test_policy_loss_dealt_out_and_whole(pk, rows, vocab, dtype):
+    """A few long rows, dealt to several workgroups with a workspace and whole without one: each within the count of the other test, in place too; rows that do not
+    count and one that is clipped among them."""
+    import ctypes as C
+    x, t, g = loss_inputs(rows, vocab, dtype, 61)
+    z, _, lp, p = softmax64(x, t, 1.25)
+    old, ref, adv, w = lp.float() - 0.1, lp.float() + 0.2, torch.randn(rows, generator=g, device="cuda"), torch.rand(rows, generator=g, device="cuda") + 0.1
+    if rows > 4:
+        w[1], t[2], old[3], adv[3] = 0.0, -1, old[3] - 3.0, 1.0
+        x[1:3] = math.nan
+    used = ((t >= 0) & (w != 0))
+    each, slope = plain_policy(lp, old, ref, adv, w, 0.2, 0.3, 0.05)
+    wd = torch.where(used, w.double(), 0.0)
+    slack = torch.where(used, logp_slack(z, vocab) + U * (lp.abs() + 1), 0.0)
+    steep = slope.abs() + adv.double().abs() * 2 + 1.0
+    coef = torch.where(used, wd * slope * 1.25 * 0.5, 0.0)[:, None]
+    want = torch.where(used[:, None] & (coef != 0), coef * (torch.zeros_like(p).scatter_(1, t.clamp(min=0).long()[:, None], 1.0) - p), 0.0)
+    tol = HALF[dtype] * want.abs() + (wd[:, None] * 1.25 * 0.5 * 4 * steep[:, None] * (slack + 2 * U * sizes(z))[:, None]) + 1e-37
+    L, code = pk.lib.lib(), pk.lib.PK_F32 if dtype == FP32 else pk.lib.PK_BF16
+    need = L.pk_policy_loss_workspace_bytes(rows, vocab, code)
+    assert need > 0
+    c = pk.lib.PolicyConfig(0.2, 0.3, 0.05, 1.25, 0.5)
+    for ws in (torch.full((need,), 255, dtype=torch.uint8, device="cuda"), None):
+        for over in (False, True):
+            a = x.clone()
+            d = a if over else torch.full_like(x, 3.0)
+            logp, loss, row_loss = torch.full((rows,), 3.0, device="cuda"), torch.zeros((), device="cuda"), torch.full((rows,), 3.0, dtype=F64, device="cuda")
+            q = lambda y: C.c_void_p(y.data_ptr() if y is not None else None)  # noqa: E731
+            pk.lib.check(L.pk_policy_loss(C.byref(c), q(a), vocab, q(t), q(old), q(ref), q(adv), q(w), rows, vocab, q(d), vocab, q(logp), q(row_loss), q(loss),
+                                          q(ws), need if ws is not None else 0, code, C.c_void_p(torch.cuda.current_stream().cuda_stream)))
+            within("logp", logp, torch.where(used, lp, 0.0), slack + 1e-37)
+            within("loss", loss, (wd * each)[used].sum(), (wd * (4 * steep * slack + 4 * U * each.abs()))[used].sum() + 1e-37)
+            within("dlogits", d, want, tol)
+
+
 def test_policy_loss_gradient_against_differences(pk):
     """Along a direction in the logits; the loss is smooth between the clips. Two losses of fp32, each within 64 u of its terms, over a step of 2^-7; the
     third-order term of the step below 2^-11."""
@@ -1027,7 +1063,8 @@ def test_larger_calls_under_graph_capture(pk):
 
     def calls():
         logp, lse = pk.ops.token_logprobs_fwd(y, u)
-        return (*pk.blockops.preference_loss(x, t, starts, ref), logp, lse, pk.ops.token_logprobs_bwd(y, u, lse, dlogp))
+        return (*pk.blockops.preference_loss(x, t, starts, ref), logp, lse, pk.ops.token_logprobs_bwd(y, u, lse, dlogp),
+                *pk.blockops.policy_loss(y, u, ref[:3], dlogp, dlogp))
 
     def step(ps, state):
         return pk.blockops.adamw_many_(ps, gs, state, 0.01, t=2, max_norm=1.0)
