@@ -15,7 +15,8 @@ namespace pk {
 namespace {
 
 // Workgroups of a launch. Forward of 16384 tokens, 32 heads of 128: 53.3 us on 1024, 51.3 on 2048, 47.5 on 4096. Each of the backward's leaves sums of dw, and four to a
-// CU fill its registers: backward of 8192 tokens, 16 heads of 64, 18.5 us on 512, 16.5 on 1024, 19.3 on 2048.
+// CU fill its registers: backward of 8192 tokens, 16 heads of 64, a token to a wavefront, 18.5 us on 512, 16.5 on 1024,
+// 19.3 on 2048.
 constexpr int FWD_MOST = 4096, BWD_MOST = 1024;
 constexpr int MAX_DK = 256, MAX_PAIRS = MAX_DK / 2, NT = 256, WAVES = NT / 64;
 
@@ -643,7 +644,7 @@ bool pieces(const void* p, int64_t sb, int64_t st, int64_t sh, const pk_qk_shape
     return aligned(p, to) && sb * es % to == 0 && st * es % to == 0 && sh * es % to == 0;
 }
 // Which kernels take a call: the row kernels on whole aligned pieces, the row kernels on any rows, or those that take a wavefront for a row (head sizes under 8, the last few
-// up to 256 where two remainders want a lane each, strides that are negative or past 2^24). 8192 tokens, 14 + 2 heads, bf16, forward and backward: 64 columns aligned
+// up to 256 where two remainders want a lane each, strides that are negative or past 2^24). 8192 tokens, 14 + 2 heads, bf16, a token to a wavefront, forward and backward: 64 columns aligned
 // 7.9 and 15.8 us, the same as any rows 9.6 and 17.6, one element off 10.2 and 17.6, a wavefront for a row 59 and 80; 62 columns 10.1 and 18.5 (60 and 80), 100 columns of fp32
 // 18.9 and 31 (64 and 84); 16456 tokens, 8 + 8 heads of 104 columns, 92 turned from halves, 27 and 39 (121 and 151).
 enum Serve { ALIGNED, LOOSE, ANY };
