@@ -102,6 +102,25 @@ __device__ inline void losses_sum(const Loss& a) {
     if (threadIdx.x == 0) *a.loss = static_cast<float>(s / a.divisor);
 }
 
+// x added up over the wavefront's lanes, the sum in every one, by group_sum's moves.
+__device__ inline double lanes_sum(double x) {
+    const auto words = [](uint32_t lo, uint32_t hi) { return __longlong_as_double(static_cast<int64_t>(lo) | static_cast<int64_t>(hi) << 32); };
+    const auto lo = [](double v) { return static_cast<uint32_t>(__double_as_longlong(v)); };
+    const auto hi = [](double v) { return static_cast<uint32_t>(__double_as_longlong(v) >> 32); };
+    const auto l32 = __builtin_amdgcn_permlane32_swap(lo(x), lo(x), false, false), h32 = __builtin_amdgcn_permlane32_swap(hi(x), hi(x), false, false);
+    x = words(l32[0], h32[0]) + words(l32[1], h32[1]);
+    const auto l16 = __builtin_amdgcn_permlane16_swap(lo(x), lo(x), false, false), h16 = __builtin_amdgcn_permlane16_swap(hi(x), hi(x), false, false);
+    x = words(l16[0], h16[0]) + words(l16[1], h16[1]);
+    const auto moved = [&](auto ctrl) {
+        constexpr int C = decltype(ctrl)::value;
+        return words(__builtin_amdgcn_update_dpp(0, lo(x), C, 0xf, 0xf, true), __builtin_amdgcn_update_dpp(0, hi(x), C, 0xf, 0xf, true));
+    };
+    x += moved(std::integral_constant<int, 0x128>{});
+    x += moved(std::integral_constant<int, 0x141>{});
+    x += moved(std::integral_constant<int, 0x4E>{});
+    return x + moved(std::integral_constant<int, 0xB1>{});
+}
+
 // log2 of the sum of 2^(s2 x) over a row: s2 top + log2. Its two parts stay apart, since their sum, in 32 bits, knows the second one no more where logits are large.
 struct RowSum {
     float top;
@@ -110,13 +129,13 @@ struct RowSum {
 __device__ inline RowSum row_sum(float top, double sum) { return RowSum{top, sum == 0.0 ? static_cast<double>(NAN) : log2(sum)}; }  // a row without a word has no probabilities
 // From what each wavefront has: the logit that it took its exponentials against and their sum; one without a word has none to scale.
 template <int WAVES>
-__device__ inline RowSum sum_of_row(const Loss& a, const float (&m)[WAVES], const float (&s)[WAVES]) {
+__device__ inline RowSum sum_of_row(const Loss& a, const float (&m)[WAVES], const double (&s)[WAVES]) {
     float top = m[0];
 #pragma unroll
     for (int w = 1; w < WAVES; ++w) top = fmaxf(top, m[w]);
     double sum = 0.0;
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) sum += s[w] == 0.0f ? 0.0 : static_cast<double>(s[w] * power_of(a, m[w], top));
+    for (int w = 0; w < WAVES; ++w) sum += s[w] == 0.0 ? 0.0 : s[w] * power_of(a, m[w], top);
     return row_sum(top, sum);
 }
 
@@ -275,7 +294,8 @@ __device__ inline void keep_packed(Piece<T> (&held)[PER]) {
 template <typename T, Mode MODE, int ROW_NT, int PER, bool PAST>
 __global__ __launch_bounds__(ROW_NT) void rows_held(Loss a) {
     constexpr int WAVES = ROW_NT / 64, N = Piece<T>::N;
-    __shared__ float sh_m[WAVES], sh_s[WAVES];
+    __shared__ float sh_m[WAVES];
+    __shared__ double sh_s[WAVES];
     __shared__ RowOut sh_o;
     const int64_t r = blockIdx.x;
     const int tid = threadIdx.x, V = a.vocab, t = a.targets[r];
@@ -302,16 +322,25 @@ __global__ __launch_bounds__(ROW_NT) void rows_held(Loss a) {
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
     const float ref = m == -INFINITY ? 0.0f : m;
-    float s = power_of(a, edge, ref);
+    float first = power_of(a, edge, ref);
     keep_packed(held);
 #pragma unroll
-    for (int k = 0; k < PER; ++k) held[k].each([&](float v) { s += power_of(a, v, ref); });
-    s = group_sum<64>(s);
+    for (int k = 0; k < PER; ++k) held[k].each([&](float v) { first += power_of(a, v, ref); });
+    double s = group_sum<64>(first);
+    // Where one word has most of the row its log-probability is little more than the sum's own rounding, 2^-24: added up in 64 bits then, which for every row would cost
+    // the log-probabilities of 8192 x 32000 bf16 99.6 -> 111.8 us.
+    if (s < 1.25) {
+        s = power_of(a, edge, ref);
+        keep_packed(held);
+#pragma unroll
+        for (int k = 0; k < PER; ++k) held[k].each([&](float v) { s += power_of(a, v, ref); });
+        s = lanes_sum(s);
+    }
     RowOut o;
     if constexpr (WAVES == 1) {
         o = finish<MODE>(a, r, xt, row_sum(ref, s), tid == 0);
     } else {
-        if ((tid & 63) == 0) sh_m[tid >> 6] = s == 0.0f ? -INFINITY : ref, sh_s[tid >> 6] = s;
+        if ((tid & 63) == 0) sh_m[tid >> 6] = s == 0.0 ? -INFINITY : ref, sh_s[tid >> 6] = s;
         __syncthreads();
         if (tid < 64) {
             o = finish<MODE>(a, r, xt, sum_of_row<WAVES>(a, sh_m, sh_s), tid == 0);
@@ -338,10 +367,11 @@ __global__ __launch_bounds__(ROW_NT) void rows_held(Loss a) {
 // Rows that no workgroup holds are read in strides, with a running maximum and sum, and again for the gradient.
 constexpr int LONG_U = 4;
 template <typename T, int NT>
-__device__ inline void running(const Loss& a, const T* x, const Cut<T>& cut, int from, int to, float edge, float* sh_m, float* sh_s) {
+__device__ inline void running(const Loss& a, const T* x, const Cut<T>& cut, int from, int to, float edge, float* sh_m, double* sh_s) {
     constexpr int N = Piece<T>::N;
     const int tid = threadIdx.x;
-    float m = edge, s = edge == -INFINITY ? 0.0f : power_of(a, edge, edge);
+    float m = edge;
+    double s = edge == -INFINITY ? 0.0 : static_cast<double>(power_of(a, edge, edge));
     for (int p0 = from + tid; p0 < to; p0 += LONG_U * NT) {
         Piece<T> v[LONG_U];
 #pragma unroll
@@ -353,7 +383,7 @@ __device__ inline void running(const Loss& a, const T* x, const Cut<T>& cut, int
 #pragma unroll
         for (int u = 0; u < LONG_U; ++u) v[u].each([&](float y) { top = fmaxf(top, y); });
         const float ref = top == -INFINITY ? 0.0f : top;
-        s = s == 0.0f ? 0.0f : s * power_of(a, m, ref);
+        if (s != 0.0) s *= power_of(a, m, ref);
 #pragma unroll
         for (int u = 0; u < LONG_U; ++u) v[u].each([&](float y) { s += power_of(a, y, ref); });
         m = top;
@@ -362,8 +392,8 @@ __device__ inline void running(const Loss& a, const T* x, const Cut<T>& cut, int
     float top = m;
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-    s = group_sum<64>(s == 0.0f ? 0.0f : s * power_of(a, m, top));
-    if ((tid & 63) == 0) sh_m[tid >> 6] = s == 0.0f ? -INFINITY : top, sh_s[tid >> 6] = s;
+    s = lanes_sum(s == 0.0 ? 0.0 : s * power_of(a, m, top));
+    if ((tid & 63) == 0) sh_m[tid >> 6] = s == 0.0 ? -INFINITY : top, sh_s[tid >> 6] = s;
     __syncthreads();
 }
 
@@ -371,7 +401,8 @@ constexpr int LONG_NT = 1024;
 template <typename T, Mode MODE, bool PAST>
 __global__ __launch_bounds__(LONG_NT) void rows_long(Loss a) {
     constexpr int WAVES = LONG_NT / 64, N = Piece<T>::N;
-    __shared__ float sh_m[WAVES], sh_s[WAVES];
+    __shared__ float sh_m[WAVES];
+    __shared__ double sh_s[WAVES];
     __shared__ RowOut sh_o;
     const int64_t r = blockIdx.x;
     const int tid = threadIdx.x, V = a.vocab, t = a.targets[r];
@@ -410,7 +441,8 @@ constexpr int PART_NT = 512, MOST_PARTS = 32, FEW_ROWS = 128;
 template <typename T, Mode MODE>
 __global__ __launch_bounds__(PART_NT) void rows_part(Loss a, int per, float2* parts) {
     constexpr int WAVES = PART_NT / 64;
-    __shared__ float sh_m[WAVES], sh_s[WAVES];
+    __shared__ float sh_m[WAVES];
+    __shared__ double sh_s[WAVES];
     const int64_t r = blockIdx.x;
     const int tid = threadIdx.x;
     if (a.targets[r] < 0 || (MODE == POLICY && a.weights[r] == 0.0f)) return;
@@ -420,12 +452,13 @@ __global__ __launch_bounds__(PART_NT) void rows_part(Loss a, int per, float2* pa
     const float edge = blockIdx.y == 0 && tid < cut.edges ? elem(x, cut.edge(tid)) : -INFINITY;
     running<T, PART_NT>(a, x, cut, from, to, edge, sh_m, sh_s);
     if (tid != 0) return;
-    float top = sh_m[0], s = 0.0f;
+    float top = sh_m[0];
+    double s = 0.0;
 #pragma unroll
     for (int w = 1; w < WAVES; ++w) top = fmaxf(top, sh_m[w]);
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) s += sh_s[w] == 0.0f ? 0.0f : sh_s[w] * power_of(a, sh_m[w], top);
-    parts[r * gridDim.y + blockIdx.y] = make_float2(top, s);
+    for (int w = 0; w < WAVES; ++w) s += sh_s[w] == 0.0 ? 0.0 : sh_s[w] * power_of(a, sh_m[w], top);
+    parts[r * gridDim.y + blockIdx.y] = make_float2(top, static_cast<float>(s - 1.0));  // the part's largest word is 1 of it: what the others are keeps its bits
 }
 template <typename T, Mode MODE>
 __global__ __launch_bounds__(64) void rows_join(Loss a, int count, const float2* parts) {
@@ -436,11 +469,11 @@ __global__ __launch_bounds__(64) void rows_join(Loss a, int count, const float2*
         if (lane == 0) no_row<MODE>(a, r);
         return;
     }
-    const float2 v = lane < count ? parts[r * count + lane] : make_float2(-INFINITY, 0.0f);
+    const float2 v = lane < count ? parts[r * count + lane] : make_float2(-INFINITY, -1.0f);
     float top = v.x;
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-    double sum = v.y == 0.0f ? 0.0 : static_cast<double>(v.y * power_of(a, v.x, top));
+    double sum = v.y == -1.0f ? 0.0 : (1.0 + v.y) * power_of(a, v.x, top);
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
     const T* x = static_cast<const T*>(a.logits) + r * a.ld;
@@ -534,7 +567,8 @@ constexpr int GRAD_U = 8;
 template <typename T, int GRAD_NT, bool PAST, bool FEW>
 __global__ __launch_bounds__(GRAD_NT) void rows_grad(Loss a, int per, Pairs pairs) {
     constexpr int N = Piece<T>::N;
-    __shared__ float sh_m[GRAD_NT / 64], sh_s[GRAD_NT / 64];
+    __shared__ float sh_m[GRAD_NT / 64];
+    __shared__ double sh_s[GRAD_NT / 64];
     if (blockIdx.x == a.rows) {
         if (blockIdx.y != 0) return;
         if constexpr (FEW)

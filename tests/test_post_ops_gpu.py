@@ -381,6 +381,23 @@ def test_losses_of_far_logits(pk, base, rows, vocab, pitch, dtype):
     assert torch.equal(over, pk.ops.token_logprobs_bwd(x.clone(), t, lse, dlogp))
 
 
+@pytest.mark.parametrize("dtype", [FP32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("rows,vocab", [(5, 700), (9, 5003), (300, 32000), (3, 40001), (2, 150001), (130, 70000)])
+def test_losses_of_rows_with_one_likely_word(pk, rows, vocab, dtype):
+    """The log-probability of a word that has nearly all is the others' sum, a hundredth to a millionth: that sum's own error counts, not the rounding of 1 beside
+    it. An exponent is within 3 u of its size, an exponential within 4 u, log and the last rounding 4 u."""
+    x, t, g = loss_inputs(rows, vocab, dtype, 71)
+    x.mul_(1.0 / 3.0)
+    x.scatter_(1, t.long()[:, None], (math.log(vocab) + 5.0 + 9.0 * torch.rand(rows, 1, generator=g, device="cuda")).to(dtype))
+    z, _, wp, _ = softmax64(x, t, 1.0)
+    size = (z.amax(1) - z.amin(1)) / math.log(2)
+    tol = (3 * size + 12) * U * wp.abs()
+    assert float(wp.min()) > -0.02 and float(tol.max()) < 0.02 * 200 * U
+    within("logp", pk.ops.token_logprobs_fwd(x, t)[0], wp, tol)
+    one = torch.ones(rows, device="cuda")
+    within("policy's logp", pk.blockops.policy_loss(x, t, 0 * one, one, one)[2], wp, tol)
+
+
 def test_token_logprobs_dealt_out_and_whole(pk):
     """A few rows past what a workgroup holds: dealt to several with a workspace, whole without one, each within the count of the other test; rows that hold no number,
     are not read or have one word only, among them."""
