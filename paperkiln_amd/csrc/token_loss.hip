@@ -7,8 +7,8 @@
 //                -(1 - e) log sigma(u) - e log sigma(-u);  dL/du = e sigma(u) - (1 - e) sigma(-u)
 //
 // What bounds it: memory, the logits read and their gradient written. A policy row's coefficient depends on its own row only, so its gradient leaves
-// in the pass that reads it. A preference row's depends on both sequences of its pair, so the logits are read twice.
-// Exponentials are taken in base 2 against the largest logit; sums are in 32 bits inside a wavefront and in 64 across them, and a token's
+// in the pass that reads it (but for a few long rows, which several workgroups read). A preference row's depends on both sequences of its pair, so the logits are read twice.
+// Exponentials are taken in base 2 against the largest logit; sums are in 32 bits inside a wavefront, where no word has most of it, and in 64 across them, and a token's
 // log-probability, a difference of near numbers, is formed in 64, and stays there until it has been added to its loss.
 #include "post.h"
 
@@ -329,7 +329,7 @@ __global__ __launch_bounds__(ROW_NT) void rows_held(Loss a) {
     double s = group_sum<64>(first);
     // Where one word has most of the row its log-probability is little more than the sum's own rounding, 2^-24: added up in 64 bits then, which for every row would cost
     // the log-probabilities of 8192 x 32000 bf16 99.6 -> 111.8 us.
-    if (s < 1.25) {
+    if (s != 0.0 && s < 1.25) {
         s = power_of(a, edge, ref);
         keep_packed(held);
 #pragma unroll
