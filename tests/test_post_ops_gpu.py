@@ -141,6 +141,52 @@ def test_qk_norm_rope_against_64_bits(pk, case, dtype):
         within("dw" + n, dw, gw, (x.shape[0] * T * x.shape[2] + 16) * U * terms)
 
 
+def dw_terms(x, w, dy, pos, theta, eps, rotary, halves):
+    """du x r in 64 bits, element by element: what a column's dw is the sum of."""
+    each = w.double().expand(x.shape).clone().requires_grad_()
+    return torch.autograd.grad(plain_qk(x.double(), each, pos, theta, eps, rotary, halves), each, dy.double())[0]
+
+
+def dw_within(name, dw, x, w, dy, pos, rotary, halves):
+    """dw by the chain that its additions really are. A lane adds up its rows in turn: those of the tokens that its wavefront takes, a 4096th of them and one more, or fewer where a
+    token's heads are dealt out; then come 64 rows of LDS, four loads, trees of 4 and 16 and a store. r, the products and the store's rounding are 16 more, all in u of the
+    terms; the turn is 16 u of what a row's pair may be at most, since its parts may cancel. All that is under a hundredth of dw: no part of the
+    sum can be missing."""
+    terms = dw_terms(x, w, dy, pos, 1e4, 1e-5, rotary, halves)
+    tokens, heads = x.shape[0] * x.shape[1], x.shape[2]
+    chain = min((-(-tokens // 4096) + 1) * heads, -(-tokens * heads // 256) + 16) + 64 + 4 + 4 + 16
+    pair = 2 ** 0.5 * dy.double().abs().amax(-1) * (x.double() * torch.rsqrt(x.double().square().mean(-1, keepdim=True) + 1e-5)).abs().amax(-1)
+    want, tol = terms.sum((0, 1, 2)), (chain + 16) * U * terms.abs().sum((0, 1, 2)) + 16 * U * pair.sum()
+    assert float(tol.max()) < 0.01 * float(want.square().mean().sqrt()), name
+    within(name, dw, want, tol)
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("case", QK_CASES, ids=lambda c: "-".join(map(str, c)))
+def test_qk_norm_rope_weights_gradient(pk, case, dtype):
+    B, T, Hq, Hkv, dk, rotary, halves, layout, where, far = case
+    q, k, wq, wk, pos, dyq, dyk = qk_inputs(B, T, Hq, Hkv, dk, dtype, 5, layout, where, far)
+    _, _, dwq, dwk = pk.ops.qk_norm_rope_bwd(dyq, dyk, q, k, wq, wk, pos, 1e4, 1e-5, rotary, halves)
+    dw_within("dwq", dwq, q, wq, dyq, pos, rotary, halves)
+    dw_within("dwk", dwk, k, wk, dyk, pos, rotary, halves)
+
+
+def test_qk_norm_rope_weights_gradient_past_2_to_the_31(pk):
+    """Rows that count spread over all of a tensor of more than 2^31 elements, every 1021st token and the last one: one or two to a wavefront. The others' terms are zero and
+    round nothing."""
+    T, Hq, Hkv, dk = 35000, 480, 2, 128
+    g = torch.Generator(device="cuda").manual_seed(8)
+    qkv = torch.ones(1, T, Hq + Hkv, dk, dtype=BF16, device="cuda")
+    dy = torch.zeros_like(qkv)
+    some = torch.cat([torch.arange(0, T, 1021), torch.tensor([T - 1])]).cuda()
+    x, d = (torch.randn(1, len(some), Hq + Hkv, dk, generator=g, device="cuda").to(BF16) for _ in range(2))
+    qkv[:, some], dy[:, some] = x, d
+    w, pos = 1 + 0.2 * torch.randn(dk, generator=g, device="cuda"), torch.arange(T, device="cuda", dtype=torch.int32)
+    _, _, dwq, dwk = pk.ops.qk_norm_rope_bwd(dy[:, :, :Hq], dy[:, :, Hq:], qkv[:, :, :Hq], qkv[:, :, Hq:], w, w, pos, 1e4)
+    dw_within("dwq", dwq, x[:, :, :Hq], w, d[:, :, :Hq], pos[some], 0, False)
+    dw_within("dwk", dwk, x[:, :, Hq:], w, d[:, :, Hq:], pos[some], 0, False)
+
+
 def test_qk_norm_rope_gradient_against_differences(pk):
     """The derivative of sum(y * dy) along a direction against a central difference of the operator itself in fp32: the difference of two sums of n
     values, each within 32 u of |dy| max|u|, over a step of 2^-6, and the third-order term of the step, below 2^-12 of the sum."""
