@@ -159,6 +159,31 @@ def test_adamw_many_refuses_tables():
     assert _lib.lib().pk_adamw_many(None, 2, None, None, 0, None, None) == ARGUMENT
 
 
+def tensor8(at, n=1000, g=1 << 30):
+    """One with moments in 8 bits, everything in places of its own: four scales of 4 bytes in each of two."""
+    blocks = (n + 255) // 256
+    m, v = at + 4 * n, at + 5 * n
+    ms = at + 6 * n
+    return _lib.AdamWTensor(at, g, m, v, ms, ms + 4 * blocks, None, n)
+
+
+@pytest.mark.parametrize("field", ["p", "m", "v", "m_scale", "v_scale"])
+@pytest.mark.parametrize("off", [-1, 1], ids=["ends", "begins"])
+def test_adamw_many_refuses_tensors_of_8_bits_that_meet(field, off):
+    """Two tensors apart but for one word of one of them; with the clip's workspace missing the same table is refused for that, behind the check for what meets."""
+    last = dict(p=4 * 1000, m=1000, v=1000, m_scale=16, v_scale=16)[field]
+    refused = lambda a, b: (adamw([a, b], state_bits=8, max_norm=1.0, ws=None), b"twice" in _lib.lib().pk_last_error())  # noqa: E731
+    assert refused(tensor8(1 << 20), tensor8(1 << 24)) == (WORKSPACE, False)
+    for other in ("p", "m", "v", "m_scale", "v_scale"):
+        for near in (0, 1):   # a byte of it beyond, and just clear
+            a, b = tensor8(1 << 20), tensor8(1 << 24)
+            size = dict(p=4 * 1000, m=1000, v=1000, m_scale=16, v_scale=16)[other]
+            setattr(b, field, getattr(a, other) + size - near if off > 0 else getattr(a, other) - last + near)
+            # beside the last word of a lies nothing of it, but before most of its words and behind others there is
+            alone = not near and (other == "v_scale" if off > 0 else other == "p")
+            assert refused(a, b) == ((WORKSPACE, False) if alone else (ARGUMENT, True)), (other, near)
+
+
 def test_torch_front_end_refuses_tensors_of_the_cpu():
     """Types, shapes and places are checked before any pointer is handed on."""
     import torch
