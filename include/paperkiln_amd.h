@@ -304,8 +304,9 @@ typedef struct pk_qk_shape {
                             (pk_op_rope's is the reference's 32-bit product) */
     int64_t pos_stride_b; /* pos[b * pos_stride_b + t], on the device; 0 = one row of positions for all sequences */
 } pk_qk_shape;
-/* yq / yk may lie where q / k do, element for element. Results that overlap inputs, or each other, in any other way are
- * undefined, here and in the backward; one that begins where the other one or the other one's input does is refused. */
+/* yq / yk may lie where q / k do, element for element. Results that overlap their inputs in any other way, the other
+ * one's tensors, the weights, the positions or themselves are refused, here and in the backward. Heads, tokens or
+ * sequences of one buffer are told apart where both tensors repeat in the same step of it. */
 int pk_qk_norm_rope_fwd(const pk_qk_shape* s, const pk_tensor4* q, const pk_tensor4* k, const float* wq, const float* wk,
                         const int* pos, const pk_tensor4* yq, const pk_tensor4* yk, void* stream);
 /* The gradients, from the inputs: r is formed again. dwq, dwk [dk] fp32 are overwritten; their sums are taken in a

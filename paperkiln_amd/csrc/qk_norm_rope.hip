@@ -621,10 +621,103 @@ int check(const pk_qk_shape* s, const char* who) {
     return PK_OK;
 }
 bool bad(const pk_tensor4* t) { return !t || !t->ptr; }
-// Whether a result begins where the other one does, or where something of the other one's is read: rows of both kinds would be written and read by different wavefronts.
-bool crossed(const pk_tensor4* q, const pk_tensor4* k, std::initializer_list<const pk_tensor4*> read_for_q, std::initializer_list<const pk_tensor4*> read_for_k) {
-    const auto in = [](const pk_tensor4* t, const auto& list) { return std::any_of(list.begin(), list.end(), [&](const pk_tensor4* x) { return x->ptr == t->ptr; }); };
-    return q->ptr == k->ptr || in(q, read_for_k) || in(k, read_for_q);
+// Where a tensor's rows lie: three dimensions of runs of `run` bytes, those of size 1 left out.
+struct Place {
+    int64_t at, run;   // the first byte of all, strides taken by their size
+    int64_t n[3], stride[3];
+    bool back[3], repeats = false;  // which strides lead backwards; whether one leads nowhere
+    int dims = 0;
+    void add(int64_t count, int64_t bytes) {
+        if (count < 2) return;
+        if (bytes == 0) {
+            repeats = true;
+            return;
+        }
+        if ((back[dims] = bytes < 0)) at += (count - 1) * bytes, bytes = -bytes;
+        n[dims] = count, stride[dims++] = bytes;
+    }
+    int64_t span(int64_t under = INT64_MAX) const {  // of the runs that strides smaller than this join
+        int64_t bytes = run;
+        for (int i = 0; i < dims; ++i) bytes += stride[i] < under ? (n[i] - 1) * stride[i] : 0;
+        return bytes;
+    }
+    bool in_steps_of(int64_t step) const {  // all other strides are whole numbers of steps
+        return std::all_of(stride, stride + dims, [&](int64_t s) { return s < step || s % step == 0; });
+    }
+    int64_t widest() const { return dims ? *std::max_element(stride, stride + dims) : 0; }
+    int64_t drop(int64_t step) {  // one repetition of what repeats in these steps is left, the first: how many there were
+        for (int i = 0; i < dims; ++i)
+            if (stride[i] == step) {
+                const int64_t count = n[i];
+                --dims, n[i] = n[dims], stride[i] = stride[dims];
+                return count;
+            }
+        return 1;
+    }
+    bool single() const {  // no byte is in two runs
+        return !repeats && std::all_of(stride, stride + dims, [&](int64_t s) { return s >= span(s) && std::count(stride, stride + dims, s) == 1; });
+    }
+};
+Place place_of(const pk_tensor4* t, const pk_qk_shape* s, int heads) {
+    const int64_t es = elem_size(s->dtype);
+    Place p;
+    p.at = static_cast<int64_t>(reinterpret_cast<uintptr_t>(t->ptr)), p.run = s->dk * es;
+    p.add(s->B, t->stride_b * es), p.add(s->T, t->stride_t * es), p.add(heads, t->stride_h * es);
+    return p;
+}
+Place place_of(const void* v, int64_t n, int64_t rows = 1, int64_t stride = 0) {  // n words
+    Place p;
+    p.at = static_cast<int64_t>(reinterpret_cast<uintptr_t>(v)), p.run = 4 * n;
+    p.add(rows, 4 * stride);
+    return p;
+}
+bool same(const Place& a, const Place& b) {  // element for element
+    return a.at == b.at && a.run == b.run && a.dims == b.dims && a.repeats == b.repeats && std::equal(a.n, a.n + a.dims, b.n) && std::equal(a.stride, a.stride + a.dims, b.stride) &&
+           std::equal(a.back, a.back + a.dims, b.back);
+}
+// Whether two have no byte in common for sure: one behind the other, or, as heads, tokens or sequences of one buffer, in different parts of a step that both repeat in,
+// or so in every distance that what the outermost step repeats can come to.
+bool apart(const Place& a, const Place& b) {
+    if (a.at + a.span() <= b.at || b.at + b.span() <= a.at) return true;
+    const auto in_gaps_of = [&](int64_t step) {
+        if (!a.in_steps_of(step) || !b.in_steps_of(step)) return false;
+        const int64_t ahead = ((b.at - a.at) % step + step) % step;
+        return a.span(step) <= ahead && ahead + b.span(step) <= step;
+    };
+    if (std::any_of(a.stride, a.stride + a.dims, in_gaps_of) || std::any_of(b.stride, b.stride + b.dims, in_gaps_of)) return true;
+    Place u = a, v = b;
+    const int64_t step = std::max(u.widest(), v.widest());
+    if (step == 0) return false;
+    const int64_t ahead = u.drop(step) - 1, behind = v.drop(step) - 1;  // u's repetition less v's lies from -behind to ahead
+    const auto down = [step](int64_t x) { return x >= 0 ? x / step : -((step - 1 - x) / step); };
+    const int64_t first = std::max(-behind, down(v.at - u.at - u.span()) + 1), last = std::min(ahead, -down(u.at - v.at - v.span()) - 1);
+    if (last - first > 2) return false;  // repetitions that lie over one another
+    for (int64_t d = first; d <= last; ++d) {
+        u.at = a.at + d * step;
+        if (!apart(u, v)) return false;
+    }
+    return true;
+}
+// What every row of a result may be written over is its own input, element for element: rows are read and written by different wavefronts. Refused: a result over the other
+// one or over what that is made of, over the weights or positions, over its own input in any other way, over itself.
+int overlapping(const char* who, const pk_qk_shape* s, const pk_tensor4* q, const pk_tensor4* k, std::initializer_list<const pk_tensor4*> read_for_q,
+                std::initializer_list<const pk_tensor4*> read_for_k, const float* wq, const float* wk, const int* pos) {
+    const auto refuse = [who](const char* why) { return fail(PK_ERR_ARGUMENT, std::string(who) + why); };
+    const Place results[2] = {place_of(q, s, s->Hq), place_of(k, s, s->Hkv)};
+    if (!apart(results[0], results[1])) return refuse(": a result lies over the other one's tensor");
+    const Place words[3] = {place_of(wq, s->dk), place_of(wk, s->dk), s->pos_stride_b ? place_of(pos, s->T, s->B, s->pos_stride_b) : place_of(pos, s->T)};
+    for (int i = 0; i < 2; ++i) {
+        for (const pk_tensor4* x : i ? read_for_q : read_for_k)
+            if (!apart(results[i], place_of(x, s, i ? s->Hq : s->Hkv))) return refuse(": a result lies over the other one's tensor");
+        for (const pk_tensor4* x : i ? read_for_k : read_for_q)
+            if (const Place own = place_of(x, s, i ? s->Hkv : s->Hq); !same(results[i], own) && !apart(results[i], own))
+                return refuse(": a result may lie where its own input does, element for element, or clear of it");
+        for (const Place& w : words)
+            if (!apart(results[i], w)) return refuse(": a result lies over the weights or the positions");
+    }
+    for (const Place& r : results)
+        if (!r.single()) return refuse(": a result's elements share memory");
+    return PK_OK;
 }
 
 void fill(Qk& a, const pk_qk_shape* s) {
@@ -764,7 +857,7 @@ int pk_qk_norm_rope_fwd(const pk_qk_shape* s, const pk_tensor4* q, const pk_tens
         if (int rc = check(s, "pk_qk_norm_rope_fwd")) return rc;
         if (static_cast<int64_t>(s->B) * s->T == 0) return static_cast<int>(PK_OK);
         if (bad(q) || bad(k) || bad(yq) || bad(yk) || !wq || !wk || !pos) return fail(PK_ERR_ARGUMENT, "pk_qk_norm_rope_fwd: null tensor");
-        if (crossed(yq, yk, {q}, {k})) return fail(PK_ERR_ARGUMENT, "pk_qk_norm_rope_fwd: a result lies over the other one's tensor");
+        if (int rc = overlapping("pk_qk_norm_rope_fwd", s, yq, yk, {q}, {k}, wq, wk, pos)) return rc;
         Qk a;
         fill(a, s);
         a.x[0] = rows_of(q), a.x[1] = rows_of(k), a.y[0] = out_of(yq), a.y[1] = out_of(yk), a.dy[0] = a.dy[1] = Rows{nullptr, 0, 0, 0};
@@ -805,7 +898,8 @@ int pk_qk_norm_rope_bwd(const pk_qk_shape* s, const pk_tensor4* dyq, const pk_te
         if (!none && (bad(dyq) || bad(dyk) || bad(q) || bad(k) || bad(dq) || bad(dk) || !pos)) return fail(PK_ERR_ARGUMENT, "pk_qk_norm_rope_bwd: null tensor");
         if (!workspace || workspace_bytes < pk_qk_norm_rope_bwd_workspace_bytes(s) || !aligned(workspace, 16))
             return fail(PK_ERR_WORKSPACE, "pk_qk_norm_rope_bwd: workspace too small (pk_qk_norm_rope_bwd_workspace_bytes)");
-        if (!none && crossed(dq, dk, {q, dyq}, {k, dyk})) return fail(PK_ERR_ARGUMENT, "pk_qk_norm_rope_bwd: a result lies over the other one's tensor");
+        if (!none)
+            if (int rc = overlapping("pk_qk_norm_rope_bwd", s, dq, dk, {q, dyq}, {k, dyk}, wq, wk, pos)) return rc;
         hipStream_t st = static_cast<hipStream_t>(stream);
         Qk a;
         fill(a, s);

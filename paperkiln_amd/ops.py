@@ -117,13 +117,14 @@ def qk_norm_rope_fwd(q, k, wq, wk, pos, theta, eps=1e-5, rotary_dim=0, halves=Fa
     1/sqrt(mean(x^2) + eps) times its weight, then turned by its token's position. q: [B,T,Hq,dk], k: [B,T,Hkv,dk] (any
     batch/token/head strides, so heads of a fused projection are read in place; dk even, at most 256), wq, wk: float32 [dk],
     pos: int32 [T] or [B,T]. Pairs are columns 2i and 2i+1 as in ``blockops.apply_rope``, or i and i + rotary_dim/2 with
-    ``halves``; rotary_dim 0 turns all columns. Returns (yq, yk); ``out`` may supply them, q and k themselves included."""
+    ``halves``; rotary_dim 0 turns all columns. Returns (yq, yk); ``out`` may supply them, q and k themselves included; an ``out``
+    that overlaps them, or anything else of the call, in another way is refused."""
     return _native.qk_norm_rope_fwd(q, k, wq, wk, pos, theta, eps, rotary_dim, halves, out)
 
 
 def qk_norm_rope_bwd(dyq, dyk, q, k, wq, wk, pos, theta, eps=1e-5, rotary_dim=0, halves=False, out=None):
     """Gradients of ``qk_norm_rope_fwd`` from its inputs: (dq, dk, dwq, dwk), the weights' in float32, summed in a fixed
-    order. ``out`` may supply (dq, dk): views of a fused gradient, or dyq and dyk themselves."""
+    order. ``out`` may supply (dq, dk): views of a fused gradient, or dyq and dyk (or q and k) themselves; any other overlap is refused."""
     return _native.qk_norm_rope_bwd(dyq, dyk, q, k, wq, wk, pos, theta, eps, rotary_dim, halves, out)
 
 

@@ -67,6 +67,51 @@ def test_qk_norm_rope_refuses_crossed_results():
         assert L.pk_qk_norm_rope_bwd(C.byref(s), at(3), at(4), at(1), at(2), SOME, SOME, SOME, at(dq), at(dk), SOME, SOME, SOME, need, None) == ARGUMENT and b"other" in L.pk_last_error()
 
 
+# In a buffer of 2 sequences of 3 tokens, each 8 heads of 64 bf16: queries are heads 0 to 3, keys 4 and 5. Places are (elements from the buffer's first, strides of sequences, tokens, heads).
+FUSED, AWAY = (1536, 512, 64), 1 << 20
+Q, K = (0, *FUSED), (256, *FUSED)
+QK_OVERLAPS = [(512, *FUSED), (-512, *FUSED), (64, *FUSED), (1, *FUSED), (-1, *FUSED), (1536, *FUSED),   # a token, a head, an element, a sequence on
+               (384, *FUSED), (192, *FUSED),                                                          # into the next token's queries, into the keys
+               (0, 1536, 64, 512), (0, 768, 256, 64), (0, 1536, 512, 128),                              # the place, other strides
+               (1024, 1536, -512, 64), (0, 0, 512, 64), (0, 1536, 512, 0)]                              # backwards; all sequences, all heads in one place
+QK_SHARING = [(AWAY, 1536, 512, 32), (AWAY, 1536, 128, 64), (AWAY, 512, 512, 64), (AWAY, 0, 512, 64), (AWAY, 256, 512, 0)]
+
+
+def place(at):
+    return C.byref(_lib.Tensor4((1 << 30) + 2 * at[0], *at[1:]))
+
+
+@pytest.mark.parametrize("out", QK_OVERLAPS + QK_SHARING, ids=str)
+def test_qk_norm_rope_refuses_overlaps(out):
+    """Queries' results over the queries, the gradient that arrives or themselves; over the keys' tensors and the other way round."""
+    L, s, words = _lib.lib(), qk(B=2, T=3, Hq=4, Hkv=2), (SOME, SOME, SOME)
+    far = [place((AWAY << i, *FUSED)) for i in range(1, 6)]
+    end = (SOME, SOME, SOME, L.pk_qk_norm_rope_bwd_workspace_bytes(C.byref(s)), None)
+    why = lambda: [w for w in ("share memory", "clear of it", "over the other one") if w in L.pk_last_error().decode()]  # noqa: E731
+    at, q, k = place(out), place(Q), place(K)
+    assert L.pk_qk_norm_rope_fwd(C.byref(s), q, far[0], *words, at, far[1], None) == ARGUMENT and why() != ["over the other one"]
+    for dy, x in ((q, far[0]), (far[0], q)):
+        assert L.pk_qk_norm_rope_bwd(C.byref(s), dy, far[1], x, far[2], *words, at, far[3], *end) == ARGUMENT and why() != ["over the other one"]
+    if out == (192, *FUSED):
+        assert L.pk_qk_norm_rope_fwd(C.byref(s), far[0], k, *words, at, far[1], None) == ARGUMENT and why() == ["over the other one"]
+        assert L.pk_qk_norm_rope_fwd(C.byref(s), far[0], far[1], *words, at, k, None) == ARGUMENT and why() == ["over the other one"]
+        for dy, x in ((k, far[0]), (far[0], k)):
+            assert L.pk_qk_norm_rope_bwd(C.byref(s), far[1], dy, far[2], x, *words, at, far[3], *end) == ARGUMENT and why() == ["over the other one"]
+        assert L.pk_qk_norm_rope_bwd(C.byref(s), at, far[0], far[1], far[2], *words, far[3], k, *end) == ARGUMENT and why() == ["over the other one"]
+
+
+@pytest.mark.parametrize("which", range(3))
+@pytest.mark.parametrize("at", [0, 2 * 510, 2 * (1536 + 700)])
+def test_qk_norm_rope_refuses_results_over_weights_and_positions(which, at):
+    L, s, far = _lib.lib(), qk(B=2, T=3, Hq=4, Hkv=4, dk=128), (AWAY << 1, *FUSED)   # heads fill their tokens
+    words = [SOME, SOME, SOME]
+    words[which] = C.c_void_p((1 << 30) + at)
+    out, off = place((0, 1536, 512, 128)), place((AWAY << 2, 1536, 512, 128))
+    for y in ((out, off), (off, out)):
+        assert L.pk_qk_norm_rope_fwd(C.byref(s), place(far), place(far), *words, *y, None) == ARGUMENT and b"weights" in L.pk_last_error()
+        assert L.pk_qk_norm_rope_bwd(C.byref(s), *[place(far)] * 4, *words, *y, SOME, SOME, SOME, 1 << 30, None) == ARGUMENT and b"weights" in L.pk_last_error()
+
+
 # what is the same for the three entries that read logits and write their gradient
 LOGITS_REFUSED = [(dict(rows=-1), SHAPE), (dict(rows=1 << 31), SHAPE), (dict(vocab=0), SHAPE), (dict(vocab=(1 << 30) + 1), SHAPE), (dict(ld=-1), SHAPE),
                   (dict(dld=99), SHAPE), (dict(dtype=7), ARGUMENT), (dict(scale=0.0), ARGUMENT), (dict(scale=-1.0), ARGUMENT), (dict(scale=math.inf), ARGUMENT),

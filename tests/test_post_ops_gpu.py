@@ -227,6 +227,41 @@ def test_qk_norm_rope_in_place_and_into_views(pk, dtype, dk, halves):
     assert torch.equal(base[:, :, :Hq], yq) and torch.equal(base[:, :, Hq:Hq + Hkv], yk) and torch.equal(base[:, :, Hq + Hkv:], v)
 
 
+@pytest.mark.parametrize("layout", ["heads apart", "tokens inside heads", "beside", "other sequences", "other tokens", "every sixth token", "q, k and v of a head", "one token",
+                                    "sequences at a pitch of their own"])
+def test_qk_norm_rope_into_other_parts_of_the_inputs_buffer(pk, layout):
+    """Results, inputs and gradients in parts of one buffer that take turns in it: taken for apart, the bits those of calls into new tensors."""
+    B, T, H, dk = 3, 5, 2, 32
+    g = torch.Generator(device="cuda").manual_seed(1)
+    if layout == "one token":
+        B, T = 1, 1
+    shape = {"heads apart": (B, T, 6 * H, dk), "tokens inside heads": (B, 6 * H, T, dk), "beside": (6, B, T, H, dk), "other sequences": (6 * B, T, H, dk),
+             "other tokens": (B, 6 * T, H, dk), "q, k and v of a head": (B, T, H, 6, dk), "one token": (B, T, H, 6, dk),
+             "every sixth token": (B, 6 * T, H, dk), "sequences at a pitch of their own": (B, T * 6 * H * dk + 20)}[layout]
+    buffer = torch.randn(shape, generator=g, device="cuda")
+    part = {"heads apart": lambda i: buffer[:, :, i * H:(i + 1) * H], "tokens inside heads": lambda i: buffer[:, i * H:(i + 1) * H].transpose(1, 2), "beside": lambda i: buffer[i],
+            "other sequences": lambda i: buffer[i::6], "other tokens": lambda i: buffer[:, i * T:(i + 1) * T], "q, k and v of a head": lambda i: buffer[:, :, :, i],
+            "one token": lambda i: buffer[:, :, :, i], "every sixth token": lambda i: buffer[:, i::6],
+            "sequences at a pitch of their own": lambda i: buffer[:, :-20].unflatten(1, (T, 6 * H, dk))[:, :, i * H:(i + 1) * H]}[layout]
+    q, k, dyq, dyk, a, b = (part(i) for i in range(6))
+    w, pos = 1 + 0.2 * torch.randn(dk, generator=g, device="cuda"), torch.arange(T, device="cuda", dtype=torch.int32)
+    kept = [y.clone() for y in (q, k, dyq, dyk)]
+    want = pk.ops.qk_norm_rope_fwd(q, k, w, w, pos, 1e4)
+    grad = pk.ops.qk_norm_rope_bwd(dyq, dyk, q, k, w, w, pos, 1e4)
+    pk.ops.qk_norm_rope_fwd(q, k, w, w, pos, 1e4, out=(a, b))
+    assert torch.equal(a, want[0]) and torch.equal(b, want[1])
+    for out in ((a, b), (dyq, dyk), (q, k)):   # the last two write over what they are made of
+        for y, x in zip((q, k, dyq, dyk), kept):
+            y.copy_(x)
+        got = pk.ops.qk_norm_rope_bwd(dyq, dyk, q, k, w, w, pos, 1e4, out=out)
+        assert all(torch.equal(y, x) for y, x in zip((*out, *got[2:]), grad))
+        assert all(torch.equal(y, x) or y is out[0] or y is out[1] for y, x in zip((q, k, dyq, dyk), kept))
+    for y, x in zip((q, k), kept):
+        y.copy_(x)
+    pk.ops.qk_norm_rope_fwd(q, k, w, w, pos, 1e4, out=(q, k))
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+
+
 def test_qk_norm_rope_rows_do_not_depend_on_the_batch(pk):
     """A token alone, as in decoding, has the bits that it has inside a long batch."""
     for dtype in (FP32, BF16):
