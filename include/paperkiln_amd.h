@@ -373,7 +373,8 @@ int pk_preference_loss(const pk_preference_config* c, const void* logits, int64_
  * in either. Values between two of the format's are rounded up or down at random with the value itself as the mean,
  * drawn from (seed, the tensor's place in the list, the element's place in the tensor): give another seed each step. A v
  * that is not zero does not become zero. A block in which a value is not finite becomes NaN.
- * A parameter, state or copy that is in the list twice is refused, and so are more than 2^35 elements in all. */
+ * A parameter, state or copy that is in the list twice is refused, a gradient that lies over one of them (but for its
+ * own parameter's, element for element: a bf16 copy may be written over the bf16 gradient), and more than 2^35 elements in all. */
 typedef struct pk_adamw_tensor {
     float* p;
     const void* g;           /* fp32 or bf16, the same for all (grad_dtype) */

@@ -196,7 +196,8 @@ def adamw_state(params, bits=32):
 def adamw_many_(params, grads, state, lr, b1=0.9, b2=0.999, eps=1e-8, wd=0.01, t=1, max_norm=0.0, copies=None, seed=0):
     """nn::AdamW::step on a list of fp32 parameters in a handful of launches, in place; ``clip_grad_norm_`` in front of it where
     max_norm > 0 (the gradients themselves are left as they are), the global norm returned on the device. grads: fp32 or bf16, all the
-    same; None leaves its parameter and state untouched. copies: bf16 tensors that receive the new parameters. The 8-bit states are
+    same; None leaves its parameter and state untouched. copies: bf16 tensors that receive the new parameters, bf16 gradients of
+    the same parameters themselves if the program is done with them. The 8-bit states are
     rounded up or down at random, drawn from ``seed``: give another one each step (the step count will do)."""
     return _native.adamw_many(params, grads, state.m, state.v, state.m_scale, state.v_scale, copies, lr, b1, b2, eps, wd, t, max_norm, seed)
 

@@ -365,38 +365,57 @@ int64_t parts_of(const pk_adamw_tensor* t, int count) {
     return n;
 }
 
-// Whether two of the tensors that are written have memory in common.
-bool meet(const pk_adamw_tensor* t, int count, bool eight) {
-    using Span = std::pair<uintptr_t, uintptr_t>;
+// What is wrong with where a list's tensors lie, or null: two of those that are written have memory in common, or a gradient lies over one of them otherwise than over its own
+// parameter's, element for element (there a lane reads it before it writes).
+const char* misplaced(const pk_adamw_tensor* t, int count, bool eight, size_t grad_size) {
+    struct Span {
+        uintptr_t from, to;
+        int tensor;
+        size_t size;  // of an element, 0: scales
+        bool operator<(const Span& o) const { return from < o.from; }
+    };
     std::vector<Span> spans[6];
     bool ascending = true;
+    uintptr_t grads_from = UINTPTR_MAX, grads_to = 0;
+    const auto grad = [&](int i) {
+        const uintptr_t at = reinterpret_cast<uintptr_t>(t[i].g);
+        return Span{at, at + static_cast<uintptr_t>(t[i].n) * grad_size, i, grad_size};
+    };
     for (int k = 0; k < 6; ++k) {
         if ((k == 3 || k == 4) && !eight) continue;
         spans[k].reserve(static_cast<size_t>(count));
         for (int i = 0; i < count; ++i) {
             const void* const p = k == 0 ? t[i].p : k == 1 ? t[i].m : k == 2 ? t[i].v : k == 3 ? t[i].m_scale : k == 4 ? t[i].v_scale : t[i].copy;
             if (t[i].n == 0 || !p) continue;
+            const size_t size = k == 0 ? 4 : k < 3 ? eight ? 1 : 4 : k < 5 ? 0 : 2;
             const uintptr_t n = static_cast<uintptr_t>(t[i].n), at = reinterpret_cast<uintptr_t>(p);
-            const uintptr_t bytes = k == 0 ? 4 * n : k < 3 ? n * (eight ? 1 : 4) : k < 5 ? 4 * ((n + BLOCK - 1) / BLOCK) : 2 * n;
-            ascending = ascending && (spans[k].empty() || spans[k].back().second <= at);
-            spans[k].push_back({at, at + bytes});
+            ascending = ascending && (spans[k].empty() || spans[k].back().to <= at);
+            spans[k].push_back({at, at + (size ? size * n : 4 * ((n + BLOCK - 1) / BLOCK)), i, size});
         }
     }
+    for (int i = 0; i < count; ++i)
+        if (t[i].n) grads_from = std::min(grads_from, grad(i).from), grads_to = std::max(grads_to, grad(i).to);
     std::vector<Span> all;
     if (ascending) {  // each list one slab, or in the order of an allocator: the lists' ends say all, where they are apart
         for (const auto& s : spans)
-            if (!s.empty()) all.push_back({s.front().first, s.back().second});
+            if (!s.empty()) all.push_back({s.front().from, s.back().to, 0, 0});
         std::sort(all.begin(), all.end());
-        bool apart = true;
-        for (size_t i = 1; i < all.size(); ++i) apart = apart && all[i - 1].second <= all[i].first;
-        if (apart) return false;
+        bool clear = true;
+        for (size_t i = 0; i < all.size(); ++i) clear = clear && (i == 0 || all[i - 1].to <= all[i].from) && (all[i].to <= grads_from || grads_to <= all[i].from);
+        if (clear) return nullptr;
         all.clear();
     }
     for (const auto& s : spans) all.insert(all.end(), s.begin(), s.end());
     std::sort(all.begin(), all.end());
     for (size_t i = 1; i < all.size(); ++i)
-        if (all[i].first < all[i - 1].second) return true;
-    return false;
+        if (all[i].from < all[i - 1].to) return "a parameter, state or copy is in the list twice";
+    for (int i = 0; i < count; ++i) {
+        if (!t[i].n) continue;
+        const Span g = grad(i);
+        for (auto w = std::lower_bound(all.begin(), all.end(), g.from, [](const Span& s, uintptr_t from) { return s.to <= from; }); w != all.end() && w->from < g.to; ++w)
+            if (w->tensor != i || w->from != g.from || w->size != g.size) return "a gradient lies over a parameter, state or copy otherwise than element for element over its own";
+    }
+    return nullptr;
 }
 
 // Blocks that a workgroup takes. In 32 bits one to a wavefront: 96 tensors of 60000 elements 25.2 us, by 16 27.5; 35 M elements 147 and 154. In 8 bits a workgroup forms the
@@ -500,7 +519,7 @@ int pk_adamw_many(const pk_adamw_tensor* t, int count, const pk_adamw_config* c,
                                   static_cast<const void*>(t[i].v_scale), static_cast<const void*>(t[i].copy)})
                 if (reinterpret_cast<uint64_t>(p) >> 48) return fail(PK_ERR_ARGUMENT, "pk_adamw_many: an address past 48 bits");
         }
-        if (meet(t, count, c->state_bits == 8)) return fail(PK_ERR_ARGUMENT, "pk_adamw_many: a parameter, state or copy is in the list twice");
+        if (const char* why = misplaced(t, count, c->state_bits == 8, static_cast<size_t>(elem_size(c->grad_dtype)))) return fail(PK_ERR_ARGUMENT, std::string("pk_adamw_many: ") + why);
         if (clip && !norm) return fail(PK_ERR_ARGUMENT, "pk_adamw_many: a clip writes the norm");
         if (clip && (!workspace || !aligned(workspace, 8) || workspace_bytes < pk_adamw_many_workspace_bytes(t, count, c)))
             return fail(PK_ERR_WORKSPACE, "pk_adamw_many: workspace too small (pk_adamw_many_workspace_bytes)");

@@ -229,6 +229,37 @@ def test_adamw_many_refuses_tensors_of_8_bits_that_meet(field, off):
             assert refused(a, b) == ((WORKSPACE, False) if alone else (ARGUMENT, True)), (other, near)
 
 
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("grads", [_lib.PK_F32, _lib.PK_BF16], ids=["g32", "g16"])
+def test_adamw_many_refuses_gradients_over_what_is_written(bits, grads):
+    """One tensor's gradient in the place of another's parameter, state, scale or copy, in its own's but for an element, in the whole range and at both ends of it. With the
+    clip's workspace missing a table without fault is refused for that."""
+    size, n = 4 if grads == _lib.PK_F32 else 2, 1000
+
+    def table(where=None, of=0, off=0, order=1):
+        one = [tensor8(1 << 20, g=1 << 30), tensor8(1 << 24, g=1 << 31)]
+        for x in one:
+            if bits == 32:
+                x.m, x.v = x.p + 4 * n, x.p + 8 * n
+            x.copy = x.p + 16 * n
+        if where:
+            one[0].g = getattr(one[of], where) + off
+        got = adamw(one[::order], state_bits=bits, grad_dtype=grads, max_norm=1.0, ws=None)
+        return got, b"gradient" in _lib.lib().pk_last_error()
+
+    width = dict(p=4, m=bits // 8, v=bits // 8, copy=2, **(dict(m_scale=0, v_scale=0) if bits == 8 else {}))
+    assert table() == (WORKSPACE, False)
+    for where, w in width.items():
+        last = w * n - size if w else 12
+        for order in (1, -1):
+            for of in (0, 1):
+                own = of == 0 and w == size
+                assert table(where, of, 0, order) == ((WORKSPACE, False) if own else (ARGUMENT, True)), (where, of)
+                for off in (size, -size, last, -size * n + size):
+                    assert table(where, of, off, order) == (ARGUMENT, True), (where, of, off)
+        assert table("p", 0, -size * n) == (WORKSPACE, False) and table("copy", 1, 2 * n) == (WORKSPACE, False)   # just clear
+
+
 def test_torch_front_end_refuses_tensors_of_the_cpu():
     """Types, shapes and places are checked before any pointer is handed on."""
     import torch

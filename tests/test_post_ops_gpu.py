@@ -941,6 +941,29 @@ def test_adamw_many_skips_what_has_no_gradient(pk):
 
 
 @pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_many_writes_over_its_own_gradients(pk, bits):
+    """bf16 copies in the place of the bf16 gradients, whole blocks and what is behind them, with a clip: the bits of a call with copies of their own."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    ps = [torch.randn(n, generator=g, device="cuda") for n in (70001, 5, 256, 40000)]
+    gs = [torch.randn(p.shape, generator=g, device="cuda").to(BF16) for p in ps]
+    runs = []
+    for over in (False, True):
+        p, grads = [x.clone() for x in ps], [x.clone() for x in gs]
+        state, copies = pk.blockops.adamw_state(p, bits), grads if over else [torch.empty_like(x) for x in grads]
+        norm = pk.blockops.adamw_many_(p, grads, state, 0.01, max_norm=1.0, copies=copies, seed=3)
+        assert all(torch.equal(a, b.to(BF16)) for a, b in zip(copies, p))
+        runs.append([y.view(torch.uint8) for y in (*p, *state.m, *state.v, norm.view(1))])
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
+    two = [torch.zeros(300, device="cuda") for _ in range(2)]   # each the other one's gradient; each other's copies in the gradients' places
+    with pytest.raises(RuntimeError, match="element for element"):
+        pk.blockops.adamw_many_(two, two[::-1], pk.blockops.adamw_state(two, bits), 0.01)
+    halves = [y.to(BF16) for y in two]
+    with pytest.raises(RuntimeError, match="element for element"):
+        pk.blockops.adamw_many_(two, halves, pk.blockops.adamw_state(two, bits), 0.01, copies=halves[::-1])
+    assert not any(y.any() for y in (*two, *halves))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
 def test_adamw_many_does_not_depend_on_how_a_list_is_dealt(pk, bits):
     """A tensor's bits beside others of any number and size, in one launch or several, with bf16 copies or without."""
     g = torch.Generator(device="cuda").manual_seed(9)
