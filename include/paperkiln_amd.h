@@ -366,7 +366,8 @@ int pk_preference_loss(const pk_preference_config* c, const void* logits, int64_
 /* One AdamW step (nn::AdamW::step's formula, src/nn.cpp:301-321, bias corrections formed in 64 bits) over a list of
  * tensors in a handful of launches, in place. With max_norm > 0 the gradients are scaled by min(1, max_norm / norm)
  * as ops::clip_grad_norm does (src/ops.cpp:1046-1064), on the way: they are not written. norm (device, fp32)
- * receives the global norm before the clip; it may be NULL without one.
+ * receives the global norm before the clip; it may be NULL without one. Every operation is rounded to 32 bits by itself
+ * (the bias corrections as products with 1/c1 and 1/c2); with state_bits 8 the root and the quotient are each good to one step.
  * state_bits 32: m and v are fp32 [n]. 8: m is e4m3 (finite, no infinities) and v e5m2, one byte an element, each times
  * the power of two (as the device's powf and torch.ldexp form it) of its block of 256 elements: m_scale, v_scale fp32
  * [ceil(n / 256)]. Zeroed memory is a fresh state

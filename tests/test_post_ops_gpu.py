@@ -862,6 +862,29 @@ def test_adamw_many_against_plain(pk, bits, grads, clip, ns, apart):
             M[i], V[i] = up(state.m[i], state.m_scale[i]), up(state.v[i], state.v_scale[i])
 
 
+@pytest.mark.parametrize("grads", [FP32, BF16], ids=["g32", "g16"])
+@pytest.mark.parametrize("wd", [0.0, 0.1])
+def test_adamw_many_parameters_bit_for_bit(pk, grads, wd):
+    """With moments in 32 bits a step is the formula's own roundings, the parameter's too: products and sums by themselves, a root and a quotient to half a step. Whole blocks and what is
+    behind them, gradients of 2^-40 to 2^20, zeros."""
+    f, rng = np.float32, np.random.default_rng(5)
+    lr, b1, b2, eps, w = f(0.01), f(0.9), f(0.99), f(1e-8), f(wd)
+    p = rng.standard_normal(300001).astype(f)
+    m, v = np.zeros_like(p), np.zeros_like(p)
+    got = torch.from_numpy(p).cuda()
+    state = pk.blockops.adamw_state([got])
+    for t in (1, 2, 1000):
+        g = torch.from_numpy((rng.standard_normal(p.size) * 2.0 ** rng.integers(-40, 20, p.size)).astype(f)).to(grads)
+        g[::97] = 0.0
+        pk.blockops.adamw_many_([got], [g.cuda()], state, float(lr), float(b1), float(b2), float(eps), wd, t=t)
+        g = g.float().numpy()
+        m, v = b1 * m + (f(1) - b1) * g, b2 * v + ((f(1) - b2) * g) * g
+        per1, per2 = (f(1 / (1 - float(b) ** t)) for b in (b1, b2))
+        p = p - lr * ((m * per1) / (np.sqrt(v * per2) + eps) + w * p)
+        assert p.dtype == m.dtype == f and np.array_equal(state.m[0].cpu().numpy(), m) and np.array_equal(state.v[0].cpu().numpy(), v)
+        assert np.array_equal(got.cpu().numpy(), p), t
+
+
 def test_adamw_many_states_in_8_bits_do_not_stall(pk):
     """v under a constant gradient: each step moves it by (1 - b2)(g^2 - v), under 1/16 of a step of its format, so rounded to nearest it would stay where it is.
     Over 4096 elements its mean follows the formula: after 200 steps within 5 standard errors of draws whose spread is at most a step (1/4 of the
