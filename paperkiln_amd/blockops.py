@@ -186,6 +186,7 @@ def adamw_state(params, bits=32):
     """Fresh moments (zeros) for ``adamw_many_``, in 32 bits or in 8."""
     if bits not in (8, 32):
         raise RuntimeError("adamw_state: states are held in 8 or in 32 bits")
+    params = list(params)  # gone through more than once
     zeros = lambda n, dt, p: torch.zeros(n, dtype=dt, device=p.device)  # noqa: E731
     if bits == 32:
         return AdamWState(*([zeros(p.shape, torch.float32, p) for p in params] for _ in range(2)))

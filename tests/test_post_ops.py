@@ -278,6 +278,18 @@ def test_torch_front_end_refuses_tensors_of_the_cpu():
         ops.token_logprobs([1.0], i32(1))
 
 
+@pytest.mark.parametrize("bits", [8, 32])
+def test_adamw_state_of_what_can_be_gone_through_once(bits):
+    """A model's parameters() is a generator: all of the state's lists are as long as it was."""
+    import torch
+
+    from paperkiln_amd import blockops
+    sizes = [(3, 5), (700,), ()]
+    state = blockops.adamw_state((torch.zeros(s) for s in sizes), bits)
+    assert [m.shape for m in state.m] == [v.shape for v in state.v] == [torch.Size(s) for s in sizes]
+    assert state.m_scale is None if bits == 32 else [x.numel() for x in state.m_scale] == [x.numel() for x in state.v_scale] == [1, 3, 1]
+
+
 @pytest.fixture(scope="module")
 def post_assembly(tmp_path_factory):
     import os
