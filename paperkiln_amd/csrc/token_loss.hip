@@ -30,7 +30,8 @@ struct Loss {
     double s2;                // scale * log2(e), and as a sum of two 32-bit numbers, both of them positive
     float s2_hi, s2_lo;
     float *logp, *lse;        // written; lse may be null
-    double* fine;             // LOGP: the log-probability in 64 bits, or null
+    float* low;               // LOGP: what the log-probability is beyond its 32 bits, or null
+    float2* sums;             // written unless null; GRAD: the rows' sums, or null and lse_in instead
     float* clear;             // LOGP: a word per row to set to zero, or null
     const float *lse_in, *coef;  // GRAD
     const double* losses;     // GRAD: the pairs' or rows' losses, whose sum over `divisor` the workgroup behind the last row's writes to `loss`
@@ -41,6 +42,7 @@ struct Loss {
     const float *old_logp, *ref_logp, *adv, *weights;  // POLICY; ref_logp may be null
     double* row_loss;
     float* coef_out;  // POLICY, a row that is dealt out: what its gradient is multiplied by
+    int64_t coef_step;  // words from one row's to the next one's, in coef and coef_out
     float clip_low, clip_high, kl, upstream;
 };
 enum Mode { LOGP, GRAD, POLICY };
@@ -121,7 +123,8 @@ __device__ inline double lanes_sum(double x) {
     return x + moved(std::integral_constant<int, 0xB1>{});
 }
 
-// log2 of the sum of 2^(s2 x) over a row: s2 top + log2. Its two parts stay apart, since their sum, in 32 bits, knows the second one no more where logits are large.
+// log2 of the sum of 2^(s2 x) over a row: s2 top + log2. Its two parts stay apart, since their sum, in 32 bits, knows the second one no more where logits are large; each by itself
+// may go through 32 bits from one launch to another: top is a logit, log2 that of the vocabulary's size at most.
 struct RowSum {
     float top;
     double log2;
@@ -154,24 +157,32 @@ __device__ inline RowOut finish(const Loss& a, int64_t r, float xt, const RowSum
         policy_row(a, r, logp, loss, slope);
         w = a.weights[r];
         o.coef = static_cast<float>(w * slope * a.upstream * a.scale);
-        if (writes && a.coef_out) a.coef_out[r] = static_cast<float>(w * slope * a.upstream);
+        if (writes && a.coef_out) a.coef_out[r * a.coef_step] = static_cast<float>(w * slope * a.upstream);
         o.target = o.coef * static_cast<float>(-expm1(logp));
     }
     if (writes) {
         if (MODE == POLICY) a.row_loss[r] = w * loss;
-        a.logp[r] = static_cast<float>(logp);
+        const float high = static_cast<float>(logp);
+        a.logp[r] = high;
         if (a.lse) a.lse[r] = static_cast<float>((static_cast<double>(sum.top) * a.s2 + sum.log2) * LN2);
-        if (MODE == LOGP && a.fine) a.fine[r] = logp;
+        if (a.sums) a.sums[r] = make_float2(o.top, o.log2);
+        if (MODE == LOGP && a.low) a.low[r] = isfinite(high) ? static_cast<float>(logp - high) : 0.0f;
     }
     return o;
 }
-// GRAD: from a coefficient and a row's sum, or from that sum's log in 32 bits. A log of l leaves the probabilities 2^-24 l off: up to 1024 6e-5, beyond the row is read
-// once more for its sum (logits of a few thousand: 2^-12 off without; 2048 rows of 32000 words bf16 54 us, up to there 45).
+// GRAD: from a coefficient and a row's sum, or from that sum's log in 32 bits. The target's element is what the others' come to, from the token's log-probability: as a difference of its logit
+// and a rounded log of the sum it would be 1e-6 of the coefficient off at 20, all of it where one word has nearly all of the row. A log of l leaves the probabilities 2^-24 l off: up to 1024
+// 6e-5, beyond the row is read once more for its sum (logits of a few thousand: 2^-12 off without; 2048 rows of 32000 words bf16 54 us, up to there 45).
 __device__ inline bool far(float lse) { return fabsf(lse) > 1024.0f; }
 __device__ inline RowOut summed_row(const Loss& a, float coef, float xt, const RowSum& sum, bool word) {
     if (!word) coef = NAN;  // a token that is no word has no gradient
     const double logp = ((static_cast<double>(xt) - static_cast<double>(sum.top)) * a.s2 - sum.log2) * LN2;
     return RowOut{sum.top, static_cast<float>(sum.log2), coef, coef * -expm1f(static_cast<float>(logp))};
+}
+__device__ inline RowOut known_row(const Loss& a, int64_t r, float coef, bool word) {
+    if (!word) coef = NAN;
+    const float2 sum = a.sums[r];
+    return RowOut{sum.x, sum.y, coef, coef * -expm1f(a.logp[r])};
 }
 __device__ inline RowOut given_row(const Loss& a, int64_t r, float coef, float xt, bool word) { return summed_row(a, coef, xt, RowSum{0.0f, a.lse_in[r] * (1.0 / LN2)}, word); }
 
@@ -266,7 +277,7 @@ __device__ inline void no_row(const Loss& a, int64_t r) {
     if (a.lse) a.lse[r] = 0.0f;
     if (MODE == POLICY) {
         a.row_loss[r] = 0.0;
-        if (a.coef_out) a.coef_out[r] = 0.0f;
+        if (a.coef_out) a.coef_out[r * a.coef_step] = 0.0f;
     }
 }
 template <typename T, int NT, bool PAST>
@@ -484,7 +495,7 @@ __global__ __launch_bounds__(64) void rows_join(Loss a, int count, const float2*
 struct Pairs {
     const int* starts;  // 2 pairs + 1
     const int* targets;
-    const double* logp;
+    const float *logp, *low;  // a log-probability is their sum
     const float* ref;
     float *coef, *margins;
     double* losses;
@@ -511,16 +522,15 @@ template <int U>
 __device__ inline double sequence_part(const Pairs& a, int64_t begin, int64_t end, int l, int n) {
     double s = 0.0;
     for (int64_t r0 = begin + l; r0 < end; r0 += U * n) {
-        double logp[U];
-        float ref[U];
+        float logp[U], low[U], ref[U];
         bool counts[U];
 #pragma unroll
         for (int k = 0; k < U; ++k) {
             const int64_t r = min(r0 + k * n, end - 1);
-            counts[k] = a.targets[r] >= 0 && r0 + k * n < end, logp[k] = a.logp[r], ref[k] = a.ref[r];
+            counts[k] = a.targets[r] >= 0 && r0 + k * n < end, logp[k] = a.logp[r], low[k] = a.low[r], ref[k] = a.ref[r];
         }
 #pragma unroll
-        for (int k = 0; k < U; ++k) s += counts[k] ? logp[k] - static_cast<double>(ref[k]) : 0.0;
+        for (int k = 0; k < U; ++k) s += counts[k] ? static_cast<double>(logp[k]) + low[k] - static_cast<double>(ref[k]) : 0.0;
     }
     return s;
 }
@@ -562,16 +572,17 @@ __device__ inline void few_pairs_mean(const Pairs& a, float* mean) {
 
 // ---- the gradient of rows whose sums are known --------------------------------------------------------------------------------
 // Every element by itself, so a row may be dealt to several workgroups (grid.y, `per` pieces each) and written over.
-// FEW: the rows' coefficients are formed here, from the pairs.
+// What they are known by: the log of the sum that a caller keeps, or the sum itself; PAIRS: the sum, and the rows' coefficients are formed here, from the pairs.
+enum Known { LSE, SUMS, PAIRS };
 constexpr int GRAD_U = 8;
-template <typename T, int GRAD_NT, bool PAST, bool FEW>
+template <typename T, int GRAD_NT, bool PAST, Known BY>
 __global__ __launch_bounds__(GRAD_NT) void rows_grad(Loss a, int per, Pairs pairs) {
     constexpr int N = Piece<T>::N;
     __shared__ float sh_m[GRAD_NT / 64];
     __shared__ double sh_s[GRAD_NT / 64];
     if (blockIdx.x == a.rows) {
         if (blockIdx.y != 0) return;
-        if constexpr (FEW)
+        if constexpr (BY == PAIRS)
             few_pairs_mean<GRAD_NT>(pairs, a.loss);
         else
             losses_sum<GRAD_NT>(a);
@@ -585,7 +596,7 @@ __global__ __launch_bounds__(GRAD_NT) void rows_grad(Loss a, int per, Pairs pair
     const int from = static_cast<int>(blockIdx.y) * per, to = min(cut.pieces, from + per);
     const bool edges = blockIdx.y == 0 && tid < cut.edges;
     float given = 0.0f;
-    if constexpr (FEW) {
+    if constexpr (BY == PAIRS) {
         const int seq = t < 0 ? -1 : sequence_of(pairs, r);
         if (seq >= 0) {
             const bool rejected = seq >= pairs.pairs;
@@ -593,7 +604,7 @@ __global__ __launch_bounds__(GRAD_NT) void rows_grad(Loss a, int per, Pairs pair
             given = (rejected ? -slope : slope) * a.scale;
         }
     } else {
-        given = a.coef[r] * a.scale;
+        given = a.coef[r * a.coef_step] * a.scale;
     }
     const float s2 = a.scale * LOG2E;
     if (t < 0 || given == 0.0f) {
@@ -601,7 +612,7 @@ __global__ __launch_bounds__(GRAD_NT) void rows_grad(Loss a, int per, Pairs pair
         if (edges) put(dx, cut.edge(tid), 0.0f);
         return;
     }
-    if (far(a.lse_in[r])) {  // its log says too little in 32 bits: one workgroup forms the sum again, before it writes over the row
+    if (BY == LSE && far(a.lse_in[r])) {  // its log says too little in 32 bits: one workgroup forms the sum again, before it writes over the row
         if (blockIdx.y != 0) return;
         const float edge = tid < cut.edges ? elem(x, cut.edge(tid)) : -INFINITY, xt = t < V ? elem(x, t) : NAN;
         running<T, GRAD_NT>(a, x, cut, 0, cut.pieces, edge, sh_m, sh_s);
@@ -614,7 +625,7 @@ __global__ __launch_bounds__(GRAD_NT) void rows_grad(Loss a, int per, Pairs pair
     // the target's element, read by its holder before it is written over
     const int pt = t < V && t >= cut.head ? (t - cut.head) / N : -1;
     const bool held_here = pt >= 0 && pt < cut.pieces ? pt >= from && pt < to : blockIdx.y == 0, holds = held_here && tid == cut.holder(t, GRAD_NT, from);
-    const RowOut o = given_row(a, r, given, holds ? elem(x, t) : 0.0f, t < V);
+    const RowOut o = BY == LSE ? given_row(a, r, given, holds ? elem(x, t) : 0.0f, t < V) : known_row(a, r, given, t < V);
     if (edges) {
         const int j = cut.edge(tid);
         put(dx, j, o.other(elem(x, j), s2));
@@ -703,12 +714,21 @@ void launch_dealt(const Loss& a, int parts, hipStream_t st) {
     rows_part<T, MODE><<<dim3(static_cast<unsigned>(a.rows), static_cast<unsigned>(parts)), PART_NT, 0, st>>>(a, per, a.parts);
     rows_join<T, MODE><<<dim3(static_cast<unsigned>(a.rows)), 64, 0, st>>>(a, parts, a.parts);
 }
-template <typename T, int NT, bool PAST, bool FEW>
+template <typename T, int NT, bool PAST, Known BY>
 void launch_grad(const Loss& a, const Pairs& pairs, hipStream_t st) {
     // Few rows are dealt out, one load to a thread, as far as that fills the chip: one row of 128000 words bf16 9.4 -> 3.0 us
     const int pieces = a.vocab / Piece<T>::N, most = static_cast<int>(std::max<int64_t>(1, 512 / std::max<int64_t>(a.rows, 1)));
     const int parts = std::min(most, std::max(1, pieces / NT)), per = (pieces + parts - 1) / parts;
-    rows_grad<T, NT, PAST, FEW><<<dim3(static_cast<unsigned>(a.rows + (a.loss ? 1 : 0)), static_cast<unsigned>(parts)), NT, 0, st>>>(a, per, pairs);
+    rows_grad<T, NT, PAST, BY><<<dim3(static_cast<unsigned>(a.rows + (a.loss ? 1 : 0)), static_cast<unsigned>(parts)), NT, 0, st>>>(a, per, pairs);
+}
+// Threads for a row: bf16, 65536 rows of 1000 words 48 us by 64 threads (57 by 128, 72 by 256, 122 by 512), 32768 of 2000 48 (48, 49, 70), 16384 of 4000 49 (48, 46,
+// 49), 8192 of 8000 49 (45, 44, 42), 8192 of 32000 208 (205, 193, 180). The pairs' mean is a workgroup's too: thousands of pairs want a large one.
+template <typename T, Known BY>
+void launch_grads(const Loss& a, bool past, hipStream_t st) {
+    const int pieces = a.vocab / Piece<T>::N;
+    if (pieces <= 256 && a.terms <= 4096) return past ? launch_grad<T, 64, true, BY>(a, Pairs{}, st) : launch_grad<T, 64, false, BY>(a, Pairs{}, st);
+    if (pieces <= 512 && a.terms <= 4096) return past ? launch_grad<T, 256, true, BY>(a, Pairs{}, st) : launch_grad<T, 256, false, BY>(a, Pairs{}, st);
+    past ? launch_grad<T, 512, true, BY>(a, Pairs{}, st) : launch_grad<T, 512, false, BY>(a, Pairs{}, st);
 }
 template <typename T, Mode MODE>
 void launch_typed(const Loss& a, const Pairs* pairs, hipStream_t st) {
@@ -720,13 +740,8 @@ void launch_typed(const Loss& a, const Pairs* pairs, hipStream_t st) {
         launch_dealt<T, MODE>(a, parts, st);
     } else {
         if constexpr (MODE == GRAD) {
-            // Threads for a row: bf16, 65536 rows of 1000 words 48 us by 64 threads (57 by 128, 72 by 256, 122 by 512), 32768 of 2000 48 (48, 49, 70), 16384 of 4000 49 (48, 46,
-            // 49), 8192 of 8000 49 (45, 44, 42), 8192 of 32000 208 (205, 193, 180). The pairs' mean is a workgroup's too: thousands of pairs want a large one.
-            const int pieces = a.vocab / Piece<T>::N;
-            if (pairs) return launch_grad<T, 512, false, true>(a, *pairs, st);
-            if (pieces <= 256 && a.terms <= 4096) return past ? launch_grad<T, 64, true, false>(a, Pairs{}, st) : launch_grad<T, 64, false, false>(a, Pairs{}, st);
-            if (pieces <= 512 && a.terms <= 4096) return past ? launch_grad<T, 256, true, false>(a, Pairs{}, st) : launch_grad<T, 256, false, false>(a, Pairs{}, st);
-            past ? launch_grad<T, 512, true, false>(a, Pairs{}, st) : launch_grad<T, 512, false, false>(a, Pairs{}, st);
+            if (pairs) return launch_grad<T, 512, false, PAIRS>(a, *pairs, st);
+            a.sums ? launch_grads<T, SUMS>(a, past, st) : launch_grads<T, LSE>(a, past, st);
         } else if (a.parts)
             launch_dealt<T, MODE>(a, parts_of_rows(POLICY, a.rows, a.vocab, sizeof(T)), st);
         else
@@ -746,7 +761,8 @@ int launch_rows(const Loss& all, int dtype, hipStream_t st, const Pairs* pairs =
         if (r + MOST_ROWS < all.rows) a.loss = nullptr;  // the last run's
         a.logits = static_cast<const char*>(a.logits) + r * a.ld * es;
         if (a.dlogits) a.dlogits = static_cast<char*>(a.dlogits) + r * a.dld * es;
-        on(a.targets), on(a.logp), on(a.lse), on(a.lse_in), on(a.coef), on(a.clear), on(a.fine), on(a.old_logp), on(a.ref_logp), on(a.adv), on(a.weights), on(a.row_loss), on(a.coef_out);
+        on(a.targets), on(a.logp), on(a.lse), on(a.lse_in), on(a.coef, a.coef_step), on(a.clear), on(a.low), on(a.sums), on(a.old_logp), on(a.ref_logp), on(a.adv), on(a.weights);
+        on(a.row_loss), on(a.coef_out, a.coef_step);
         if (dtype == PK_BF16)
             launch_typed<uint16_t, MODE>(a, pairs, st);
         else
@@ -821,7 +837,7 @@ int pk_token_logprobs_bwd(const void* logits, int64_t ld, const int* targets, co
         Loss a{};
         a.logits = logits, a.ld = ld, a.targets = targets, a.rows = rows, a.vocab = static_cast<int>(vocab);
         set_scale(a, scale);
-        a.dlogits = dlogits, a.dld = dld, a.lse_in = lse, a.coef = dlogp;
+        a.dlogits = dlogits, a.dld = dld, a.lse_in = lse, a.coef = dlogp, a.coef_step = 1;
         return launch_rows<GRAD>(a, dtype, static_cast<hipStream_t>(stream));
     });
 }
@@ -854,10 +870,10 @@ int pk_policy_loss(const pk_policy_config* c, const void* logits, int64_t ld, co
         a.clip_low = c->clip_low, a.clip_high = c->clip_high, a.kl = c->kl_coef, a.upstream = c->upstream;
         const int parts = workspace ? parts_of_rows(POLICY, rows, vocab, elem_size(dtype)) : 1;
         if (parts > 1) {  // the gradient in a pass of its own, once the rows' parts are joined
-            a.parts = static_cast<float2*>(workspace);
-            a.lse = reinterpret_cast<float*>(a.parts + rows * parts), a.coef_out = a.lse + rows;
+            a.parts = static_cast<float2*>(workspace), a.sums = a.parts + rows * parts;
+            a.coef_out = &a.parts->x, a.coef_step = 2 * parts;  // a row's takes the place of its first part once that is read
             if (int rc = launch_rows<POLICY>(a, dtype, st)) return rc;
-            a.parts = nullptr, a.lse_in = a.lse, a.coef = a.coef_out, a.losses = row_loss, a.terms = rows, a.divisor = 1.0, a.loss = loss;
+            a.parts = nullptr, a.coef = a.coef_out, a.losses = row_loss, a.terms = rows, a.divisor = 1.0, a.loss = loss;
             return launch_rows<GRAD>(a, dtype, st);
         }
         if (int rc = launch_rows<POLICY>(a, dtype, st)) return rc;
@@ -889,22 +905,23 @@ int pk_preference_loss(const pk_preference_config* c, const void* logits, int64_
         hipStream_t st = static_cast<hipStream_t>(stream);
         char* ws = static_cast<char*>(workspace);
         const size_t singles = pad(sizeof(float) * static_cast<size_t>(rows)), doubles = pad(sizeof(double) * static_cast<size_t>(rows));
-        float *lse = reinterpret_cast<float*>(ws), *coef = reinterpret_cast<float*>(ws + singles);
-        double *fine = reinterpret_cast<double*>(ws + 2 * singles), *losses = reinterpret_cast<double*>(ws + 2 * singles + doubles);
+        float *low = reinterpret_cast<float*>(ws), *coef = reinterpret_cast<float*>(ws + singles);
+        float2* sums = reinterpret_cast<float2*>(ws + 2 * singles);
+        double* losses = reinterpret_cast<double*>(ws + 2 * singles + doubles);
         Loss a{};
         a.logits = logits, a.ld = ld, a.targets = targets, a.rows = rows, a.vocab = static_cast<int>(vocab);
         set_scale(a, c->scale);
-        a.logp = logp, a.lse = lse, a.fine = fine, a.clear = coef;
+        a.logp = logp, a.low = low, a.sums = sums, a.clear = coef;
         if (rows < FEW_ROWS) a.parts = reinterpret_cast<float2*>(ws + 2 * singles + doubles + pad(sizeof(double) * static_cast<size_t>(pairs)));
         if (int rc = launch_rows<LOGP>(a, dtype, st)) return rc;
-        const Pairs p{seq_start, targets, fine, ref_logp, coef, margins, losses, rows, static_cast<int>(pairs), c->beta, c->label_smoothing, c->upstream};
+        const Pairs p{seq_start, targets, logp, low, ref_logp, coef, margins, losses, rows, static_cast<int>(pairs), c->beta, c->label_smoothing, c->upstream};
         a.dlogits = dlogits, a.dld = dld;
         const bool few = rows <= FEW_PAIRS_ROWS && pairs <= MOST_FEW_PAIRS;
         if (!few) {
             pair_loss<<<dim3(static_cast<unsigned>(pairs)), PAIR_NT, 0, st>>>(p);
             if (int rc = launched()) return rc;
         }
-        a.lse_in = lse, a.coef = coef, a.losses = losses, a.terms = pairs, a.divisor = static_cast<double>(pairs), a.loss = loss;
+        a.coef = coef, a.coef_step = 1, a.losses = losses, a.terms = pairs, a.divisor = static_cast<double>(pairs), a.loss = loss;
         return launch_rows<GRAD>(a, dtype, st, few ? &p : nullptr);
     });
 }

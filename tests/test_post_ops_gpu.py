@@ -479,6 +479,57 @@ def test_losses_of_rows_with_one_likely_word(pk, rows, vocab, dtype):
     within("policy's logp", pk.blockops.policy_loss(x, t, 0 * one, one, one)[2], wp, tol)
 
 
+def likely_rows(rows, vocab, dtype, base):
+    """Rows of which one word, the target, has all but a hundredth to a millionth, their logits around `base`; in 64 bits the softmax and what the others come to."""
+    x, t, g = loss_inputs(rows, vocab, dtype, 73)
+    x.mul_(1.0 / 3.0)
+    x.scatter_(1, t.long()[:, None], (math.log(vocab) + 5.0 + 9.0 * torch.rand(rows, 1, generator=g, device="cuda")).to(dtype))
+    x = (x.float() + base).to(dtype)
+    z = x.double() - x.double().amax(1, keepdim=True)
+    e = torch.exp(z)
+    rest = e.scatter(1, t.long()[:, None], 0.0).sum(1)
+    p = e / (1.0 + rest)[:, None]   # the target is the largest, its e is 1
+    return x, t, g, -torch.log1p(rest), p.scatter(1, t.long()[:, None], (-rest / (1.0 + rest))[:, None]).neg(), (z.amin(1) / -math.log(2)).clamp(min=1.0)
+
+
+def likely_within(name, d, want, coef, size, dtype):
+    """Every element relative to its own value, the target's too: exponents within 3 u of their size, an exponential 4 u, the sum's log and the token's log-probability 4 u, coefficient and
+    products 8 u."""
+    want = coef.double()[:, None] * want
+    within(name, d, want, want.abs() * (HALF[dtype] + (3 * size[:, None] + 16) * U) + 1e-37)
+
+
+LIKELY = [(5, 700), (9, 5003), (300, 32000), (3, 40001), (2, 150001), (40, 70000), (600, 3001)]
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("base", [0.0, 300.0, -900.0, 5e4])
+@pytest.mark.parametrize("rows,vocab", LIKELY)
+def test_policy_loss_gradient_of_rows_with_one_likely_word(pk, rows, vocab, base, dtype):
+    """Few long rows, which are dealt out, and others alike."""
+    x, t, g, logp, want, size = likely_rows(rows, vocab, dtype, base)
+    old, adv, w = (logp + 0.05).float(), torch.randn(rows, generator=g, device="cuda"), torch.rand(rows, generator=g, device="cuda") + 0.5
+    loss, d, got = pk.blockops.policy_loss(x, t, old, adv, w, 0.5, 0.5)
+    likely_within("dlogits", d, want, -w.double() * torch.exp(logp - old.double()) * adv.double(), size, dtype)
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("base", [0.0, 300.0, -900.0, 5e4])
+@pytest.mark.parametrize("rows,vocab", LIKELY)
+def test_preference_loss_gradient_of_rows_with_one_likely_word(pk, rows, vocab, base, dtype):
+    """Pairs formed by the gradient's wavefronts and by a launch of their own; a margin moves by no more than its log-probabilities' own error."""
+    x, t, g, logp, want, size = likely_rows(rows, vocab, dtype, base)
+    half = rows // 2
+    starts, ref = torch.tensor([0, half, rows], dtype=torch.int32, device="cuda"), (logp - 0.5 * torch.rand(rows, generator=g, device="cuda")).float()
+    loss, d, margins, got = pk.blockops.preference_loss(x, t, starts, ref, 0.0625, 0.25)
+    gain = logp - ref.double()
+    u = 0.0625 * (gain[:half].sum() - gain[half:].sum())
+    slope = (0.25 * torch.sigmoid(u) - 0.75 * torch.sigmoid(-u)) * 0.0625
+    assert abs(float(slope)) > 2.0 ** -10
+    coef = torch.where(torch.arange(rows, device="cuda") < half, slope, -slope)
+    likely_within("dlogits", d, want, coef, size, dtype)
+
+
 def test_token_logprobs_dealt_out_and_whole(pk):
     """A few rows past what a workgroup holds: dealt to several with a workspace, whole without one, each within the count of the other test; rows that hold no number,
     are not read or have one word only, among them."""
