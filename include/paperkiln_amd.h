@@ -325,9 +325,10 @@ size_t pk_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int dtype)
 int pk_token_logprobs_fwd(const void* logits, int64_t ld, const int* targets, int64_t rows, int64_t vocab, float scale,
                           float* logp, float* lse, void* workspace, size_t workspace_bytes, int dtype, void* stream);
 /* dlogits[r, j] = dlogp[r] * scale * ([j = target] - exp(z_j - lse_r)), every row written: zeros where the target is
- * negative or dlogp is 0 (such a row is not read). lse is the forward's for the same logits and scale; past 1024 in
- * size 32 bits say too little of it, and the row's sum is formed again from its logits. dlogits may be the logits themselves (same ld), else lies clear
- * of them; so in the two losses below. */
+ * negative or dlogp is 0 (such a row is not read). lse is the forward's for the same logits and scale. Its rounding to
+ * 32 bits turns no element by more than 2^-17 of its value, 2^-14 in bf16: past 128 (1024) in size the row's sum is formed
+ * again from its logits, and the element of a target that has nearly all of its row is the sum of the others'. dlogits may
+ * be the logits themselves (same ld), else lies clear of them; so in the two losses below. */
 int pk_token_logprobs_bwd(const void* logits, int64_t ld, const int* targets, const float* lse, const float* dlogp,
                           int64_t rows, int64_t vocab, float scale, void* dlogits, int64_t dld, int dtype, void* stream);
 

@@ -29,6 +29,7 @@ struct Loss {
     float scale;
     double s2;                // scale * log2(e), and as a sum of two 32-bit numbers, both of them positive
     float s2_hi, s2_lo;
+    double per_s2;            // 1 / s2
     float *logp, *lse;        // written; lse may be null
     float* low;               // LOGP: what the log-probability is beyond its 32 bits, or null
     float2* sums;             // written unless null; GRAD: the rows' sums, or null and lse_in instead
@@ -57,6 +58,7 @@ __device__ inline float power_of(const Loss& a, float x, float m) {
 void set_scale(Loss& a, float scale) {
     a.scale = scale;
     a.s2 = static_cast<double>(scale) * 1.4426950408889634074;
+    a.per_s2 = 1.0 / a.s2;
     a.s2_hi = static_cast<float>(a.s2);
     if (static_cast<double>(a.s2_hi) >= a.s2) a.s2_hi = std::nextafter(a.s2_hi, 0.0f);
     a.s2_lo = static_cast<float>(a.s2 - static_cast<double>(a.s2_hi));
@@ -145,7 +147,8 @@ __device__ inline RowSum sum_of_row(const Loss& a, const float (&m)[WAVES], cons
 // What a row's gradient is made of once its sum is known: -coef 2^(s2 (x - top) - log2), and the target's element.
 struct RowOut {
     float top, log2, coef, target;
-    __device__ float other(float x, float s2) const { return -coef * __builtin_amdgcn_exp2f(fmaf(x - top, s2, -log2)); }
+    __device__ float probability(float x, float s2) const { return __builtin_amdgcn_exp2f(fmaf(x - top, s2, -log2)); }
+    __device__ float other(float x, float s2) const { return -coef * probability(x, s2); }
 };
 template <Mode MODE>
 __device__ inline RowOut finish(const Loss& a, int64_t r, float xt, const RowSum& sum, bool writes = true) {
@@ -170,10 +173,7 @@ __device__ inline RowOut finish(const Loss& a, int64_t r, float xt, const RowSum
     }
     return o;
 }
-// GRAD: from a coefficient and a row's sum, or from that sum's log in 32 bits. The target's element is what the others' come to, from the token's log-probability: as a difference of its logit
-// and a rounded log of the sum it would be 1e-6 of the coefficient off at 20, all of it where one word has nearly all of the row. A log of l leaves the probabilities 2^-24 l off: up to 1024
-// 6e-5, beyond the row is read once more for its sum (logits of a few thousand: 2^-12 off without; 2048 rows of 32000 words bf16 54 us, up to there 45).
-__device__ inline bool far(float lse) { return fabsf(lse) > 1024.0f; }
+// GRAD: from a row's sum. The target's element, -coef expm1(log-probability), is as exact as that.
 __device__ inline RowOut summed_row(const Loss& a, float coef, float xt, const RowSum& sum, bool word) {
     if (!word) coef = NAN;  // a token that is no word has no gradient
     const double logp = ((static_cast<double>(xt) - static_cast<double>(sum.top)) * a.s2 - sum.log2) * LN2;
@@ -184,7 +184,25 @@ __device__ inline RowOut known_row(const Loss& a, int64_t r, float coef, bool wo
     const float2 sum = a.sums[r];
     return RowOut{sum.x, sum.y, coef, coef * -expm1f(a.logp[r])};
 }
-__device__ inline RowOut given_row(const Loss& a, int64_t r, float coef, float xt, bool word) { return summed_row(a, coef, xt, RowSum{0.0f, a.lse_in[r] * (1.0 / LN2)}, word); }
+// From the log of the sum in 32 bits, as a logit and what is beside it.
+__device__ inline RowOut given_row(const Loss& a, float lse, float coef, float xt, bool word) {
+    const double log2 = lse * (1.0 / LN2);
+    const float top = static_cast<float>(log2 * a.per_s2);
+    return summed_row(a, coef, xt, RowSum{top, log2 - top * a.s2}, word);
+}
+// What that log's rounding, 2^-24 of it, may turn an element by: 2^-17 of it in 32 bits, 2^-14 before a rounding to bf16. The others turn by as much as the sum, so past a log of 128 or
+// 1024 the row is read once more for it (2048 rows of 32000 words bf16 54 us, up to there 45). The target, which has 1 - p of the coefficient, turns by as much of the whole
+// coefficient: where 1 - p is small (under 0.08 or 0.01 at a log of 10) its element is what the others come to as they are written.
+template <typename T>
+constexpr float ALLOWED = sizeof(T) == 4 ? 0x1p-17f : 0x1p-14f;
+template <typename T>
+__device__ inline bool far(float lse) {
+    return fabsf(lse) * 0x1p-24f > ALLOWED<T>;
+}
+template <typename T>
+__device__ inline bool faint(const Loss& a, float lse, float xt) {
+    return fabsf(lse) * 0x1p-24f > ALLOWED<T> * -expm1f(static_cast<float>(static_cast<double>(xt) * a.scale - lse));
+}
 
 // ---- rows in 16-byte pieces -------------------------------------------------------------------------------------------------
 // A row is taken apart at 16-byte boundaries of its address: whole pieces, and the few elements in front of the first and behind the last one, which go to
@@ -572,8 +590,9 @@ __device__ inline void few_pairs_mean(const Pairs& a, float* mean) {
 
 // ---- the gradient of rows whose sums are known --------------------------------------------------------------------------------
 // Every element by itself, so a row may be dealt to several workgroups (grid.y, `per` pieces each) and written over.
-// What they are known by: the log of the sum that a caller keeps, or the sum itself; PAIRS: the sum, and the rows' coefficients are formed here, from the pairs.
-enum Known { LSE, SUMS, PAIRS };
+// What they are known by: the log of the sum that a caller keeps (DEALT: and several workgroups take a row), or the sum itself; PAIRS: the sum, and the rows' coefficients are formed
+// here, from the pairs.
+enum Known { LSE, DEALT, SUMS, PAIRS };
 constexpr int GRAD_U = 8;
 template <typename T, int GRAD_NT, bool PAST, Known BY>
 __global__ __launch_bounds__(GRAD_NT) void rows_grad(Loss a, int per, Pairs pairs) {
@@ -612,7 +631,9 @@ __global__ __launch_bounds__(GRAD_NT) void rows_grad(Loss a, int per, Pairs pair
         if (edges) put(dx, cut.edge(tid), 0.0f);
         return;
     }
-    if (BY == LSE && far(a.lse_in[r])) {  // its log says too little in 32 bits: one workgroup forms the sum again, before it writes over the row
+    constexpr bool GIVEN = BY == LSE || BY == DEALT;
+    const float lse = GIVEN ? a.lse_in[r] : 0.0f;
+    if (GIVEN && far<T>(lse)) {  // one workgroup forms the sum again, before it writes over the row
         if (blockIdx.y != 0) return;
         const float edge = tid < cut.edges ? elem(x, cut.edge(tid)) : -INFINITY, xt = t < V ? elem(x, t) : NAN;
         running<T, GRAD_NT>(a, x, cut, 0, cut.pieces, edge, sh_m, sh_s);
@@ -622,14 +643,27 @@ __global__ __launch_bounds__(GRAD_NT) void rows_grad(Loss a, int per, Pairs pair
         if (tid == cut.holder(t, GRAD_NT)) put(dx, t, o.target);
         return;
     }
-    // the target's element, read by its holder before it is written over
-    const int pt = t < V && t >= cut.head ? (t - cut.head) / N : -1;
-    const bool held_here = pt >= 0 && pt < cut.pieces ? pt >= from && pt < to : blockIdx.y == 0, holds = held_here && tid == cut.holder(t, GRAD_NT, from);
-    const RowOut o = BY == LSE ? given_row(a, r, given, holds ? elem(x, t) : 0.0f, t < V) : known_row(a, r, given, t < V);
-    if (edges) {
-        const int j = cut.edge(tid);
-        put(dx, j, o.other(elem(x, j), s2));
+    // the target's piece, or -1, and who holds its element; read before they are written over
+    const int in_piece = t < V && t >= cut.head ? (t - cut.head) / N : -1, pt = in_piece < cut.pieces ? in_piece : -1, word = t - cut.head - pt * N;
+    const bool held_here = pt >= 0 ? pt >= from && pt < to : blockIdx.y == 0, holds = held_here && tid == cut.holder(t, GRAD_NT, from);
+    Piece<T> beside = Piece<T>::nothing();
+    float xt = 0.0f;
+    if (GIVEN && holds) {
+        if (pt >= 0) beside = load_piece<false>(x + cut.head + pt * N);
+        xt = elem(x, t);
     }
+    const RowOut o = GIVEN ? given_row(a, lse, given, xt, t < V) : known_row(a, r, given, t < V);
+    // What the words but the target come to, to a lane: the target's holder adds those of its piece by themselves.
+    const auto edge_but_target = [&] { return tid < cut.edges && cut.edge(tid) != t ? o.probability(elem(x, cut.edge(tid)), s2) : 0.0f; };
+    const auto beside_target = [&] {
+        float sum = 0.0f;
+        int i = 0;
+        beside.each([&](float y) { sum += i++ == word ? 0.0f : o.probability(y, s2); });
+        return sum;
+    };
+    double others = 0.0;
+    if (BY == LSE) others = (edges ? edge_but_target() : 0.0f) + (holds ? beside_target() : 0.0f);
+    if (edges) put(dx, cut.edge(tid), o.other(elem(x, cut.edge(tid)), s2));
     for (int p0 = from + tid; p0 < to; p0 += GRAD_U * GRAD_NT) {
         Piece<T> v[GRAD_U];
 #pragma unroll
@@ -637,13 +671,59 @@ __global__ __launch_bounds__(GRAD_NT) void rows_grad(Loss a, int per, Pairs pair
             const int p = p0 + u * GRAD_NT;
             if (p < to) v[u] = load_piece<PAST>(x + cut.head + p * N);
         }
+        float round = 0.0f;
 #pragma unroll
         for (int u = 0; u < GRAD_U; ++u) {
-            const int p = p0 + u * GRAD_NT, j0 = cut.head + p * N;
-            if (p < to) store_piece<PAST>(dx + j0, gradient(v[u], s2, o));
+            const int p = p0 + u * GRAD_NT;
+            if (p >= to) continue;
+            float sum = 0.0f;
+            store_piece<PAST>(dx + cut.head + p * N, v[u].map([&](int, float y) {
+                const float e = o.probability(y, s2);
+                if (BY == LSE) sum += e;
+                return -o.coef * e;
+            }));
+            if (BY == LSE) round += p == pt ? 0.0f : sum;
+        }
+        if (BY == LSE) others += round;
+    }
+    if constexpr (BY == DEALT) {  // a faint target's holder reads the others again
+        if (!held_here || t >= V) return;
+        __shared__ bool sh_faint;
+        if (holds) sh_faint = faint<T>(a, lse, xt);
+        __syncthreads();
+        if (!sh_faint) {
+            if (holds) put(dx, t, o.target);
+            return;
+        }
+        others = edge_but_target() + (holds ? beside_target() : 0.0f);
+        for (int p0 = tid; p0 < cut.pieces; p0 += GRAD_U * GRAD_NT) {
+            Piece<T> v[GRAD_U];
+#pragma unroll
+            for (int u = 0; u < GRAD_U; ++u) {
+                const int p = p0 + u * GRAD_NT;
+                v[u] = p < cut.pieces && p != pt ? load_piece<false>(x + cut.head + p * N) : Piece<T>::nothing();
+            }
+            float round = 0.0f;
+#pragma unroll
+            for (int u = 0; u < GRAD_U; ++u) v[u].each([&](float y) { round += o.probability(y, s2); });
+            others += round;
         }
     }
-    if (holds) put(dx, t, o.target);
+    if constexpr (GIVEN) {
+        float rest = group_sum<64>(static_cast<float>(others));
+        if constexpr (GRAD_NT > 64) {
+            if ((tid & 63) == 0) sh_m[tid >> 6] = rest;
+            __syncthreads();
+        }
+        if (!holds) return;
+        if constexpr (GRAD_NT > 64) {
+            rest = 0.0f;
+            for (int w = 0; w < GRAD_NT / 64; ++w) rest += sh_m[w];
+        }
+        put(dx, t, BY == DEALT || faint<T>(a, lse, xt) ? o.coef * rest : o.target);
+    } else if (holds) {
+        put(dx, t, o.target);
+    }
 }
 
 __global__ __launch_bounds__(1024) void loss_sum(const double* x, int64_t n, float* out) {
@@ -716,10 +796,18 @@ void launch_dealt(const Loss& a, int parts, hipStream_t st) {
 }
 template <typename T, int NT, bool PAST, Known BY>
 void launch_grad(const Loss& a, const Pairs& pairs, hipStream_t st) {
-    // Few rows are dealt out, one load to a thread, as far as that fills the chip: one row of 128000 words bf16 9.4 -> 3.0 us
+    // Few rows are dealt out, one load to a thread, as far as that fills the chip: one row of 128000 words bf16 11.0 -> 3.2 us, 64 of them 13.0 -> 7.0, 128 16.6 -> 12.5. From the log of a
+    // sum not to two, nor rows that a workgroup reads in one round: they gain little (192 rows 19.1 and 17.1, 64 of 10007 words 4.1 and 3.8), and where a target's element is what the others come to,
+    // whoever holds it reads the others' parts as well (192 rows 23.0, 64 of 10007 words 5.4; one row of 128000 words 10.0). Nor rows that are written over, of which it would read what others have
+    // written.
     const int pieces = a.vocab / Piece<T>::N, most = static_cast<int>(std::max<int64_t>(1, 512 / std::max<int64_t>(a.rows, 1)));
-    const int parts = std::min(most, std::max(1, pieces / NT)), per = (pieces + parts - 1) / parts;
-    rows_grad<T, NT, PAST, BY><<<dim3(static_cast<unsigned>(a.rows + (a.loss ? 1 : 0)), static_cast<unsigned>(parts)), NT, 0, st>>>(a, per, pairs);
+    const bool whole = BY == LSE && (most < 3 || pieces <= GRAD_U * NT || a.dlogits == a.logits);
+    const int parts = whole ? 1 : std::min(most, std::max(1, pieces / NT)), per = (pieces + parts - 1) / parts;
+    const dim3 grid(static_cast<unsigned>(a.rows + (a.loss ? 1 : 0)), static_cast<unsigned>(parts));
+    if constexpr (BY == LSE) {
+        if (parts > 1) return rows_grad<T, NT, PAST, DEALT><<<grid, NT, 0, st>>>(a, per, pairs);
+    }
+    rows_grad<T, NT, PAST, BY><<<grid, NT, 0, st>>>(a, per, pairs);
 }
 // Threads for a row: bf16, 65536 rows of 1000 words 48 us by 64 threads (57 by 128, 72 by 256, 122 by 512), 32768 of 2000 48 (48, 49, 70), 16384 of 4000 49 (48, 46,
 // 49), 8192 of 8000 49 (45, 44, 42), 8192 of 32000 208 (205, 193, 180). The pairs' mean is a workgroup's too: thousands of pairs want a large one.

@@ -142,8 +142,8 @@ def token_logprobs_fwd(logits, targets, scale=1.0):
 
 def token_logprobs_bwd(logits, targets, lse, dlogp, scale=1.0, out=None):
     """dlogits of ``token_logprobs_fwd`` for the rows' gradients dlogp; rows whose dlogp is 0 are not read and get zeros. lse is
-    the forward's; past 1024 in size 32 bits say too little of it, and the row's sum is formed again. ``out`` may be the
-    logits."""
+    the forward's; past 128 in size (1024 with bf16 logits) 32 bits say too little of it, and the row's sum is formed again.
+    ``out`` may be the logits."""
     return _native.token_logprobs_bwd(logits, targets, lse, dlogp, scale, out)
 
 

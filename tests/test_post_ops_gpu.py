@@ -530,6 +530,48 @@ def test_preference_loss_gradient_of_rows_with_one_likely_word(pk, rows, vocab, 
     likely_within("dlogits", d, want, coef, size, dtype)
 
 
+ALLOWED = {FP32: 2.0 ** -17, BF16: 2.0 ** -14}   # what a log of the sum in 32 bits may turn an element by
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("base", [0.0, 300.0, -900.0, 5e4])
+@pytest.mark.parametrize("rows,vocab", LIKELY)
+def test_token_logprobs_gradient_of_rows_with_one_likely_word(pk, rows, vocab, base, dtype):
+    """Direct, over the logits, into rows at another pitch and through the node: the log of the sum that the backward pass is given counts with what it is allowed to."""
+    x, t, g, logp, want, size = likely_rows(rows, vocab, dtype, base)
+    dlogp = torch.randn(rows, generator=g, device="cuda")
+    lse = pk.ops.token_logprobs_fwd(x, t)[1]
+    want = dlogp.double()[:, None] * want
+    tol = want.abs() * (HALF[dtype] + 1.01 * ALLOWED[dtype] + (3 * size[:, None] + 16) * U) + 1e-37
+    d = pk.ops.token_logprobs_bwd(x, t, lse, dlogp)
+    within("dlogits", d, want, tol)
+    wide = x.new_full((rows, vocab + 5), 7.0)
+    pk.ops.token_logprobs_bwd(x, t, lse, dlogp, out=wide[:, 2:2 + vocab])
+    over, leaf = x.clone(), x.clone().requires_grad_()
+    pk.ops.token_logprobs_bwd(over, t, lse, dlogp, out=over)
+    pk.ops.token_logprobs(leaf, t).backward(dlogp)
+    assert torch.equal(leaf.grad, d) and bool((wide[:, :2] == 7.0).all()) and bool((wide[:, 2 + vocab:] == 7.0).all())
+    within("dlogits over the logits", over, want, tol)
+    within("dlogits at another pitch", wide[:, 2:2 + vocab], want, tol)
+
+
+@pytest.mark.parametrize("rows,vocab", [(5, 700), (300, 5003), (3, 40001), (64, 33001)])
+@pytest.mark.parametrize("base", [40.0, 120.0, -900.0])
+def test_token_logprobs_gradient_at_logits_of_hundreds(pk, rows, vocab, base):
+    """Every element in 32 bits relative to its own value; the sum's own chain of additions counts too, as in logp_slack."""
+    x, t, g = loss_inputs(rows, vocab, FP32, 19)
+    x.add_(base)
+    dlogp = torch.randn(rows, generator=g, device="cuda")
+    z = x.double() - x.double().amax(1, keepdim=True)
+    p = torch.softmax(z, 1)
+    want = dlogp.double()[:, None] * (torch.zeros_like(p).scatter_(1, t.long()[:, None], 1.0) - p)
+    size = z.amin(1, keepdim=True) / -math.log(2)
+    lse = pk.ops.token_logprobs_fwd(x, t)[1]
+    for out in (None, x):
+        d = pk.ops.token_logprobs_bwd(x, t, lse, dlogp, out=out)
+        within("dlogits", d, want, want.abs() * (1.01 * ALLOWED[FP32] + (3 * size + 16 + vocab / 64) * U) + 1e-37)
+
+
 def test_token_logprobs_dealt_out_and_whole(pk):
     """A few rows past what a workgroup holds: dealt to several with a workspace, whole without one, each within the count of the other test; rows that hold no number,
     are not read or have one word only, among them."""
