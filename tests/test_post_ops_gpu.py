@@ -262,6 +262,30 @@ def test_qk_norm_rope_into_other_parts_of_the_inputs_buffer(pk, layout):
     assert torch.equal(q, want[0]) and torch.equal(k, want[1])
 
 
+@pytest.mark.parametrize("pitch", [2 ** 24, 2 ** 24 + 8, 2 ** 24 + 1])
+@pytest.mark.parametrize("dtype", [FP32, BF16], ids=["fp32", "bf16"])
+def test_qk_norm_rope_of_heads_far_apart(pk, dtype, pitch):
+    """Heads at the largest distance that the row kernels take, past it and off the pieces, as of [B, H, T, dk] memory for very many tokens: what a dense copy gives, each within the counts of
+    the test against 64 bits, and both written back at such a distance."""
+    T, Hq, Hkv, dk = 5, 5, 3, 64
+    far = torch.zeros(2 * (Hq + Hkv) * pitch, dtype=dtype, device="cuda")
+    view = lambda first, H: far[first * pitch:].as_strided((1, T, H, dk), (0, dk, pitch, 1))  # noqa: E731
+    q, k, wq, wk, pos, dyq, dyk = qk_inputs(1, T, Hq, Hkv, dk, dtype, 6, "plain")
+    fq, fk, yq, yk = view(0, Hq), view(Hq, Hkv), view(Hq + Hkv, Hq), view(2 * Hq + Hkv, Hkv)
+    fq.copy_(q), fk.copy_(k)
+    want, grad = pk.ops.qk_norm_rope_fwd(q, k, wq, wk, pos, 1e4), pk.ops.qk_norm_rope_bwd(dyq, dyk, q, k, wq, wk, pos, 1e4)
+    pk.ops.qk_norm_rope_fwd(fq, fk, wq, wk, pos, 1e4, out=(yq, yk))
+    ys = yq.clone(), yk.clone()
+    got = pk.ops.qk_norm_rope_bwd(dyq, dyk, fq, fk, wq, wk, pos, 1e4, out=(yq, yk))
+    for i, (x, w, dy) in enumerate(((q, wq, dyq), (k, wk, dyk))):
+        x, w, size = x.double(), w.double(), dy.double().abs().amax(-1, keepdim=True) * 2 ** 0.5
+        r = torch.rsqrt(x.square().mean(-1, keepdim=True) + 1e-5)
+        within("y", ys[i], want[i], 2 * HALF[dtype] * want[i].abs().double() + 2 * 32 * U * (x * r * w).abs().amax(-1, keepdim=True))
+        within("dx", got[i], grad[i], 2 * HALF[dtype] * grad[i].abs().double() + 2 * 64 * U * r * size * w.abs().max() * (1 + (x * r).abs().amax(-1, keepdim=True)))
+        within("dw", got[2 + i], grad[2 + i], 2 * (T * x.shape[2] + 16) * U * (size * (x * r).abs()).sum((0, 1, 2)))
+    assert torch.equal(fq, q) and torch.equal(fk, k)
+
+
 def test_qk_norm_rope_rows_do_not_depend_on_the_batch(pk):
     """A token alone, as in decoding, has the bits that it has inside a long batch."""
     for dtype in (FP32, BF16):
