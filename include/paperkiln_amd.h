@@ -300,7 +300,7 @@ typedef struct pk_qk_shape {
     int32_t halves;      /* 0: pairs are columns 2i and 2i+1, as pk_op_rope's; 1: columns i and i + rotary/2 */
     int32_t dtype;       /* PK_F32 | PK_BF16: q, k, their outputs and gradients; weights are fp32 */
     float eps;
-    double theta;        /* the angle is formed in 64 bits: any int32 position is as exact as a small one
+    double theta;        /* the angle is formed in 64 bits: to 1e-7 rad up to position 2^26, to 5e-7 at 2^31
                             (pk_op_rope's is the reference's 32-bit product) */
     int64_t pos_stride_b; /* pos[b * pos_stride_b + t], on the device; 0 = one row of positions for all sequences */
 } pk_qk_shape;

@@ -6,7 +6,7 @@
 //
 // What bounds it: memory. The forward reads and writes each element once, the backward reads two and writes one; r is formed again there instead of
 // being kept, because the row is in registers anyway. The angle is formed in 64 bits, in turns, and its whole turns are dropped there: at position
-// 10^6 an angle in 32 bits is 0.06 rad off.
+// 10^6 an angle in 32 bits is 0.06 rad off. Rounded to 32 bits after that it is 1e-7 rad off up to position 2^26, 1.6e-7 at 2^28, 4.3e-7 at 2^31 (theta 10^4 to 10^6, 64 to 256 columns).
 #include "post.h"
 
 #include <algorithm>
@@ -15,8 +15,8 @@ namespace pk {
 namespace {
 
 // Workgroups of a launch. Forward of 16384 tokens, 32 heads of 128: 53.3 us on 1024, 51.3 on 2048, 47.5 on 4096. Each of the backward's leaves sums of dw, and four to a
-// CU fill its registers: backward of 8192 tokens, 16 heads of 64, a token to a wavefront, 18.5 us on 512, 16.5 on 1024,
-// 19.3 on 2048.
+// CU fill its registers: backward of 8192 tokens, 14 + 2 heads of 64, four tokens to a wavefront, 16.9 us on 512, 15.2 on 1024, 15.3 on 2048; 16 + 16 heads of 64, a token to a
+// wavefront, 24.2, 21.7 and 23.5; 16384 tokens, 16 + 16 heads of 128 90.7, 83.0 and 85.0.
 constexpr int FWD_MOST = 4096, BWD_MOST = 1024;
 constexpr int MAX_DK = 256, MAX_PAIRS = MAX_DK / 2, NT = 256, WAVES = NT / 64;
 
@@ -374,7 +374,8 @@ __device__ inline Eight weights_of(const float* w, int c0, int c1) {
 
 // A wavefront takes 2^a.pack tokens, neighbours in a sequence, and of each a list of rows, 64 / G to a step over all of them, the queries' steps first, then the keys'. What
 // a step needs is the wavefront's (scalars) but for the lane's offset, and the next step's loads are on their way while one is worked on: with four steps unrolled the
-// compiler formed every address ahead of the loop, 2600 instructions with spilled scalars in place of 500.
+// compiler formed every address ahead of the loop, 2600 instructions in place of 500. Scalars that do not fit pass through lanes of vector registers: none or a few of the forward's, 13 to 31 of the
+// backward's, 55 to 78 of it where a wavefront takes several tokens.
 template <typename T, int G, bool HALVES, bool LOOSE, bool PACKED>
 struct List : Share<LOOSE> {
     using C = Cols<T, HALVES, LOOSE>;
@@ -440,7 +441,7 @@ struct List : Share<LOOSE> {
             }
             if (this->whole) {
                 C::store(base, off + c0 * SIZE, off + c1 * SIZE, e);
-                asm volatile("s_nop 1");  // the store's data stays for two issue slots in the order of the text, too, whatever the compiler places behind the branch
+                asm volatile("s_nop 1");  // no path needs it: the check of 16-byte stores reads the kernel's text in order, and the block behind the branch writes the data's registers
             }
         } else {
             C::store(base, off + c0 * SIZE, off + c1 * SIZE, e);
