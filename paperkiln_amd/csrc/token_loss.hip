@@ -184,11 +184,12 @@ __device__ inline RowOut known_row(const Loss& a, int64_t r, float coef, bool wo
     const float2 sum = a.sums[r];
     return RowOut{sum.x, sum.y, coef, coef * -expm1f(a.logp[r])};
 }
-// From the log of the sum in 32 bits, as a logit and what is beside it.
-__device__ inline RowOut given_row(const Loss& a, float lse, float coef, float xt, bool word) {
+// From the log of the sum in 32 bits, as a logit and what is beside it; without the target.
+__device__ inline RowOut given_row(const Loss& a, float lse, float coef, bool word) {
     const double log2 = lse * (1.0 / LN2);
     const float top = static_cast<float>(log2 * a.per_s2);
-    return summed_row(a, coef, xt, RowSum{top, log2 - top * a.s2}, word);
+    const auto scalar = [](float x) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x))); };  // a row's, so the workgroup's
+    return RowOut{scalar(top), static_cast<float>(log2 - top * a.s2), scalar(word ? coef : NAN), 0.0f};
 }
 // What that log's rounding, 2^-24 of it, may turn an element by: 2^-17 of it in 32 bits, 2^-14 before a rounding to bf16. The others turn by as much as the sum, so past a log of 128 or
 // 1024 the row is read once more for it (2048 rows of 32000 words bf16 54 us, up to there 45). The target, which has 1 - p of the coefficient, turns by as much of the whole
@@ -200,8 +201,8 @@ __device__ inline bool far(float lse) {
     return fabsf(lse) * 0x1p-24f > ALLOWED<T>;
 }
 template <typename T>
-__device__ inline bool faint(const Loss& a, float lse, float xt) {
-    return fabsf(lse) * 0x1p-24f > ALLOWED<T> * -expm1f(static_cast<float>(static_cast<double>(xt) * a.scale - lse));
+__device__ inline bool faint(float lse, float gone) {
+    return fabsf(lse) * 0x1p-24f > ALLOWED<T> * gone;
 }
 
 // ---- rows in 16-byte pieces -------------------------------------------------------------------------------------------------
@@ -652,18 +653,14 @@ __global__ __launch_bounds__(GRAD_NT) void rows_grad(Loss a, int per, Pairs pair
         if (pt >= 0) beside = load_piece<false>(x + cut.head + pt * N);
         xt = elem(x, t);
     }
-    const RowOut o = GIVEN ? given_row(a, lse, given, xt, t < V) : known_row(a, r, given, t < V);
-    // What the words but the target come to, to a lane: the target's holder adds those of its piece by themselves.
-    const auto edge_but_target = [&] { return tid < cut.edges && cut.edge(tid) != t ? o.probability(elem(x, cut.edge(tid)), s2) : 0.0f; };
-    const auto beside_target = [&] {
-        float sum = 0.0f;
-        int i = 0;
-        beside.each([&](float y) { sum += i++ == word ? 0.0f : o.probability(y, s2); });
-        return sum;
-    };
-    double others = 0.0;
-    if (BY == LSE) others = (edges ? edge_but_target() : 0.0f) + (holds ? beside_target() : 0.0f);
-    if (edges) put(dx, cut.edge(tid), o.other(elem(x, cut.edge(tid)), s2));
+    const RowOut o = GIVEN ? given_row(a, lse, given, t < V) : known_row(a, r, given, t < V);
+    float others = 0.0f;  // LSE: what the words of other pieces than the target's come to, to a lane
+    if (edges) {
+        const int j = cut.edge(tid);
+        const float e = o.probability(elem(x, j), s2);
+        if (BY == LSE && j != t) others = e;
+        put(dx, j, -o.coef * e);
+    }
     for (int p0 = from + tid; p0 < to; p0 += GRAD_U * GRAD_NT) {
         Piece<T> v[GRAD_U];
 #pragma unroll
@@ -686,16 +683,26 @@ __global__ __launch_bounds__(GRAD_NT) void rows_grad(Loss a, int per, Pairs pair
         }
         if (BY == LSE) others += round;
     }
-    if constexpr (BY == DEALT) {  // a faint target's holder reads the others again
+    if constexpr (!GIVEN) {
+        if (holds) put(dx, t, o.target);
+        return;
+    }
+    const float gone = -expm1f(static_cast<float>(static_cast<double>(xt) * a.scale - lse));  // 1 - p of the target, its holder's
+    const bool dim = holds && faint<T>(lse, gone);
+    bool any = GRAD_NT == 64 ? __ballot(dim) != 0 : true;
+    if constexpr (BY == DEALT) {  // the holder's workgroup reads the others again
         if (!held_here || t >= V) return;
-        __shared__ bool sh_faint;
-        if (holds) sh_faint = faint<T>(a, lse, xt);
+        __shared__ bool sh_dim;
+        if (holds) sh_dim = dim;
         __syncthreads();
-        if (!sh_faint) {
-            if (holds) put(dx, t, o.target);
-            return;
-        }
-        others = edge_but_target() + (holds ? beside_target() : 0.0f);
+        any = sh_dim;
+    }
+    if (!any) {
+        if (holds) put(dx, t, o.coef * gone);
+        return;
+    }
+    if constexpr (BY == DEALT) {
+        if (tid < cut.edges && cut.edge(tid) != t) others = o.probability(elem(x, cut.edge(tid)), s2);
         for (int p0 = tid; p0 < cut.pieces; p0 += GRAD_U * GRAD_NT) {
             Piece<T> v[GRAD_U];
 #pragma unroll
@@ -709,21 +716,18 @@ __global__ __launch_bounds__(GRAD_NT) void rows_grad(Loss a, int per, Pairs pair
             others += round;
         }
     }
-    if constexpr (GIVEN) {
-        float rest = group_sum<64>(static_cast<float>(others));
-        if constexpr (GRAD_NT > 64) {
-            if ((tid & 63) == 0) sh_m[tid >> 6] = rest;
-            __syncthreads();
-        }
-        if (!holds) return;
-        if constexpr (GRAD_NT > 64) {
-            rest = 0.0f;
-            for (int w = 0; w < GRAD_NT / 64; ++w) rest += sh_m[w];
-        }
-        put(dx, t, BY == DEALT || faint<T>(a, lse, xt) ? o.coef * rest : o.target);
-    } else if (holds) {
-        put(dx, t, o.target);
+    if (dim) {
+        int i = 0;
+        beside.each([&](float y) { others += i++ == word ? 0.0f : o.probability(y, s2); });
     }
+    float rest = group_sum<64>(others);
+    if constexpr (GRAD_NT > 64) {
+        if ((tid & 63) == 0) sh_m[tid >> 6] = rest;
+        __syncthreads();
+        rest = 0.0f;
+        for (int w = 0; w < GRAD_NT / 64; ++w) rest += sh_m[w];
+    }
+    if (holds) put(dx, t, o.coef * (dim ? rest : gone));
 }
 
 __global__ __launch_bounds__(1024) void loss_sum(const double* x, int64_t n, float* out) {
@@ -796,10 +800,10 @@ void launch_dealt(const Loss& a, int parts, hipStream_t st) {
 }
 template <typename T, int NT, bool PAST, Known BY>
 void launch_grad(const Loss& a, const Pairs& pairs, hipStream_t st) {
-    // Few rows are dealt out, one load to a thread, as far as that fills the chip: one row of 128000 words bf16 11.0 -> 3.2 us, 64 of them 13.0 -> 7.0, 128 16.6 -> 12.5. From the log of a
-    // sum not to two, nor rows that a workgroup reads in one round: they gain little (192 rows 19.1 and 17.1, 64 of 10007 words 4.1 and 3.8), and where a target's element is what the others come to,
-    // whoever holds it reads the others' parts as well (192 rows 23.0, 64 of 10007 words 5.4; one row of 128000 words 10.0). Nor rows that are written over, of which it would read what others have
-    // written.
+    // Few rows are dealt out, one load to a thread, as far as that fills the chip: one row of 128000 words bf16 11.0 -> 3.2 us, 64 of them 13.6 -> 7.1, 128 16.3 -> 12.4. From the log of a
+    // sum not to two, nor rows that a workgroup reads in one round: they gain little (192 rows 18.9 and 17.4, 64 of 10007 words 3.9 and 3.6), and where a target's element is what the others come to,
+    // whoever holds it reads the others' parts as well (192 rows 23.7, 64 of 10007 words 5.2; one row of 128000 words 10.1). Nor rows that are written over, of which it would read what others have
+    // written (one row of 128000 words 3.3 -> 10.9).
     const int pieces = a.vocab / Piece<T>::N, most = static_cast<int>(std::max<int64_t>(1, 512 / std::max<int64_t>(a.rows, 1)));
     const bool whole = BY == LSE && (most < 3 || pieces <= GRAD_U * NT || a.dlogits == a.logits);
     const int parts = whole ? 1 : std::min(most, std::max(1, pieces / NT)), per = (pieces + parts - 1) / parts;
