@@ -201,8 +201,8 @@ __device__ inline bool far(float lse) {
     return fabsf(lse) * 0x1p-24f > ALLOWED<T>;
 }
 template <typename T>
-__device__ inline bool faint(float lse, float gone) {
-    return fabsf(lse) * 0x1p-24f > ALLOWED<T> * gone;
+__device__ inline bool faint(float lse, float logp) {  // 1 - e^-x is 0.63 x or more up to x = 1, and more than 0.63 from there on
+    return fabsf(lse) * 0x1p-24f > ALLOWED<T> * 0.63f * fminf(-logp, 1.0f);
 }
 
 // ---- rows in 16-byte pieces -------------------------------------------------------------------------------------------------
@@ -648,11 +648,10 @@ __global__ __launch_bounds__(GRAD_NT) void rows_grad(Loss a, int per, Pairs pair
     const int in_piece = t < V && t >= cut.head ? (t - cut.head) / N : -1, pt = in_piece < cut.pieces ? in_piece : -1, word = t - cut.head - pt * N;
     const bool held_here = pt >= 0 ? pt >= from && pt < to : blockIdx.y == 0, holds = held_here && tid == cut.holder(t, GRAD_NT, from);
     Piece<T> beside = Piece<T>::nothing();
+    const bool all_know = GIVEN && GRAD_NT > 64 && t < V && a.dlogits != a.logits;  // the target's logit: but for its holder it may be written over
     float xt = 0.0f;
-    if (GIVEN && holds) {
-        if (pt >= 0) beside = load_piece<false>(x + cut.head + pt * N);
-        xt = elem(x, t);
-    }
+    if (GIVEN && holds && pt >= 0) beside = load_piece<false>(x + cut.head + pt * N);
+    if (GIVEN && (holds || all_know)) xt = elem(x, t);
     const RowOut o = GIVEN ? given_row(a, lse, given, t < V) : known_row(a, r, given, t < V);
     float others = 0.0f;  // LSE: what the words of other pieces than the target's come to, to a lane
     if (edges) {
@@ -687,20 +686,13 @@ __global__ __launch_bounds__(GRAD_NT) void rows_grad(Loss a, int per, Pairs pair
         if (holds) put(dx, t, o.target);
         return;
     }
-    const float gone = -expm1f(static_cast<float>(static_cast<double>(xt) * a.scale - lse));  // 1 - p of the target, its holder's
-    const bool dim = holds && faint<T>(lse, gone);
-    bool any = GRAD_NT == 64 ? __ballot(dim) != 0 : true;
-    if constexpr (BY == DEALT) {  // the holder's workgroup reads the others again
-        if (!held_here || t >= V) return;
-        __shared__ bool sh_dim;
-        if (holds) sh_dim = dim;
-        __syncthreads();
-        any = sh_dim;
-    }
-    if (!any) {
-        if (holds) put(dx, t, o.coef * gone);
+    const float logp = static_cast<float>(static_cast<double>(xt) * a.scale - lse);
+    const bool dim = (holds || all_know) && faint<T>(lse, logp);
+    if (GRAD_NT == 64 ? !__ballot(dim) : all_know && !dim) {
+        if (holds) put(dx, t, o.coef * -expm1f(logp));
         return;
     }
+    if (BY == DEALT && !held_here) return;  // the holder's workgroup reads the others again
     if constexpr (BY == DEALT) {
         if (tid < cut.edges && cut.edge(tid) != t) others = o.probability(elem(x, cut.edge(tid)), s2);
         for (int p0 = tid; p0 < cut.pieces; p0 += GRAD_U * GRAD_NT) {
@@ -716,7 +708,7 @@ __global__ __launch_bounds__(GRAD_NT) void rows_grad(Loss a, int per, Pairs pair
             others += round;
         }
     }
-    if (dim) {
+    if (dim && holds) {
         int i = 0;
         beside.each([&](float y) { others += i++ == word ? 0.0f : o.probability(y, s2); });
     }
@@ -727,7 +719,7 @@ __global__ __launch_bounds__(GRAD_NT) void rows_grad(Loss a, int per, Pairs pair
         rest = 0.0f;
         for (int w = 0; w < GRAD_NT / 64; ++w) rest += sh_m[w];
     }
-    if (holds) put(dx, t, o.coef * (dim ? rest : gone));
+    if (holds) put(dx, t, o.coef * (dim ? rest : -expm1f(logp)));
 }
 
 __global__ __launch_bounds__(1024) void loss_sum(const double* x, int64_t n, float* out) {
@@ -808,7 +800,7 @@ void launch_grad(const Loss& a, const Pairs& pairs, hipStream_t st) {
     const bool whole = BY == LSE && (most < 3 || pieces <= GRAD_U * NT || a.dlogits == a.logits);
     const int parts = whole ? 1 : std::min(most, std::max(1, pieces / NT)), per = (pieces + parts - 1) / parts;
     const dim3 grid(static_cast<unsigned>(a.rows + (a.loss ? 1 : 0)), static_cast<unsigned>(parts));
-    if constexpr (BY == LSE) {
+    if constexpr (BY == LSE && NT == 512) {
         if (parts > 1) return rows_grad<T, NT, PAST, DEALT><<<grid, NT, 0, st>>>(a, per, pairs);
     }
     rows_grad<T, NT, PAST, BY><<<grid, NT, 0, st>>>(a, per, pairs);
