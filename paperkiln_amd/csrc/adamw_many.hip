@@ -380,38 +380,45 @@ const char* misplaced(const pk_adamw_tensor* t, int count, bool eight, size_t gr
         size_t size;  // of an element, 0: scales
         bool operator<(const Span& o) const { return from < o.from; }
     };
-    std::vector<Span> spans[6];
-    bool ascending = true;
-    uintptr_t grads_from = UINTPTR_MAX, grads_to = 0;
+    const auto written = [&](int i, int k) {  // nothing: from 0 to 0
+        const void* const p = k == 0 ? t[i].p : k == 1 ? t[i].m : k == 2 ? t[i].v : k == 3 ? t[i].m_scale : k == 4 ? t[i].v_scale : t[i].copy;
+        if (t[i].n == 0 || !p || ((k == 3 || k == 4) && !eight)) return Span{0, 0, i, 0};
+        const size_t size = k == 0 ? 4 : k < 3 ? eight ? 1 : 4 : k < 5 ? 0 : 2;
+        const uintptr_t n = static_cast<uintptr_t>(t[i].n), at = reinterpret_cast<uintptr_t>(p);
+        return Span{at, at + (size ? size * n : 4 * ((n + BLOCK - 1) / BLOCK)), i, size};
+    };
     const auto grad = [&](int i) {
         const uintptr_t at = reinterpret_cast<uintptr_t>(t[i].g);
         return Span{at, at + static_cast<uintptr_t>(t[i].n) * grad_size, i, grad_size};
     };
-    for (int k = 0; k < 6; ++k) {
-        if ((k == 3 || k == 4) && !eight) continue;
-        spans[k].reserve(static_cast<size_t>(count));
+    // Each list one slab, or in the order of an allocator: the lists' ends say all, where they are apart.
+    Span lists[7];
+    int n = 0;
+    bool clear = true;
+    for (int k = 0; k < 6 && clear; ++k) {
+        Span all{0, 0, 0, 0};
         for (int i = 0; i < count; ++i) {
-            const void* const p = k == 0 ? t[i].p : k == 1 ? t[i].m : k == 2 ? t[i].v : k == 3 ? t[i].m_scale : k == 4 ? t[i].v_scale : t[i].copy;
-            if (t[i].n == 0 || !p) continue;
-            const size_t size = k == 0 ? 4 : k < 3 ? eight ? 1 : 4 : k < 5 ? 0 : 2;
-            const uintptr_t n = static_cast<uintptr_t>(t[i].n), at = reinterpret_cast<uintptr_t>(p);
-            ascending = ascending && (spans[k].empty() || spans[k].back().to <= at);
-            spans[k].push_back({at, at + (size ? size * n : 4 * ((n + BLOCK - 1) / BLOCK)), i, size});
+            const Span s = written(i, k);
+            if (s.to == 0) continue;
+            clear = clear && all.to <= s.from;
+            all = {all.to ? all.from : s.from, s.to, 0, 0};
         }
+        if (all.to) lists[n++] = all;
     }
+    Span grads{UINTPTR_MAX, 0, 0, 0};
     for (int i = 0; i < count; ++i)
-        if (t[i].n) grads_from = std::min(grads_from, grad(i).from), grads_to = std::max(grads_to, grad(i).to);
-    std::vector<Span> all;
-    if (ascending) {  // each list one slab, or in the order of an allocator: the lists' ends say all, where they are apart
-        for (const auto& s : spans)
-            if (!s.empty()) all.push_back({s.front().from, s.back().to, 0, 0});
-        std::sort(all.begin(), all.end());
-        bool clear = true;
-        for (size_t i = 0; i < all.size(); ++i) clear = clear && (i == 0 || all[i - 1].to <= all[i].from) && (all[i].to <= grads_from || grads_to <= all[i].from);
-        if (clear) return nullptr;
-        all.clear();
+        if (t[i].n) grads.from = std::min(grads.from, grad(i).from), grads.to = std::max(grads.to, grad(i).to);
+    if (clear) {
+        if (grads.to) lists[n++] = grads;
+        std::sort(lists, lists + n);
+        for (int i = 1; i < n; ++i) clear = clear && lists[i - 1].to <= lists[i].from;
     }
-    for (const auto& s : spans) all.insert(all.end(), s.begin(), s.end());
+    if (clear) return nullptr;
+    std::vector<Span> all;
+    all.reserve(static_cast<size_t>(count) * 6);
+    for (int k = 0; k < 6; ++k)
+        for (int i = 0; i < count; ++i)
+            if (const Span s = written(i, k); s.to) all.push_back(s);
     std::sort(all.begin(), all.end());
     for (size_t i = 1; i < all.size(); ++i)
         if (all[i].from < all[i - 1].to) return "a parameter, state or copy is in the list twice";
