@@ -9,7 +9,7 @@
 // What bounds it: memory, the logits read and their gradient written. A policy row's coefficient depends on its own row only, so its gradient leaves
 // in the pass that reads it (but for a few long rows, which several workgroups read). A preference row's depends on both sequences of its pair, so the logits are read twice.
 // Exponentials are taken in base 2 against the largest logit; sums are in 32 bits inside a wavefront, where no word has most of it, and in 64 across them, and a token's
-// log-probability, a difference of near numbers, is formed in 64, and stays there until it has been added to its loss.
+// log-probability, a difference of near numbers, is formed in 64, and stays there, or in two numbers of 32, until it has been added to its loss.
 #include "post.h"
 
 #include <algorithm>
