@@ -395,6 +395,41 @@ size_t pk_adamw_many_workspace_bytes(const pk_adamw_tensor* host_tensors, int co
 int pk_adamw_many(const pk_adamw_tensor* host_tensors, int count, const pk_adamw_config* c, void* workspace,
                   size_t workspace_bytes, float* norm, void* stream);
 
+/* ---- operators of a student model ----------------------------------------------
+ * What a decoder with linear-time layers, trained against a larger one, adds to the operators above. The same holds as for the post-training operators:
+ * calls only enqueue on `stream`, allocate nothing and clear nothing by memset. */
+
+/* Layer norm (ops::layernorm) with the residual addition in front of it: h = x + residual, rounded to the tensors' type, y = (h - mean) rstd w + b with
+ * mean and rstd = 1/sqrt(mean((h - mean)^2) + eps) of every row. x and residual have ldx and ldr elements between rows (0: one row for all); y and h are
+ * dense. Without a residual (NULL) h is x and is not written (NULL). w, b [cols] fp32, b may be NULL; mean, rstd [rows] fp32. */
+typedef struct pk_norm_shape {
+    int64_t rows, cols;  /* rows: 0 to 2^22 - 1; cols: 1 to 2^24 */
+    int32_t dtype;       /* PK_F32 | PK_BF16: x, residual, y, h and their gradients */
+} pk_norm_shape;
+int pk_layernorm_fwd(const pk_norm_shape* s, const void* x, int64_t ldx, const void* residual, int64_t ldr, const float* w, const float* b, float eps, void* y,
+                     void* h, float* mean, float* rstd, void* stream);
+/* The gradients from h (x without a residual) and the rows' statistics. dx is the gradient of x and of the residual alike; dh, what arrives at h by
+ * itself, is added to it where not NULL. dw, db [cols] fp32 are overwritten, their sums taken in a fixed order. Results lie clear of all else. */
+size_t pk_layernorm_bwd_workspace_bytes(const pk_norm_shape* s);
+int pk_layernorm_bwd(const pk_norm_shape* s, const void* dy, int64_t lddy, const void* h, int64_t ldh, const void* dh, int64_t lddh, const float* w, const float* mean,
+                     const float* rstd, void* dx, float* dw, float* db, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Distillation from a teacher's top logits, loss and gradient in one pass over the student's logits [rows, vocab] (ld elements between rows). Every row has `top`
+ * slots (1 to 1024): a word indices[r, k] (negative: an empty slot) and the teacher's logit for it. With tau = temperature, q = softmax(logits / tau) and
+ *   p_k = exp(teacher[r, k] / tau - teacher_lse[r]),  teacher_lse NULL: the log of the sum of exp(teacher / tau) over the row's slots,
+ *   KL_r = sum_k p_k (log p_k - log q_{indices[r, k]}),  loss = tau^2 sum_r weights[r] KL_r;
+ * dlogits is the gradient of upstream * loss, NULL: the loss alone. kl[rows] receives KL_r, row_loss[rows] (64 bits) the terms of the loss (device, fp32), which
+ * is their sum in a fixed order. The weights carry mask and normalisation: a row of weight 0 is not read, nor one learned from that has no word; kl and gradient
+ * are 0. A word that several slots name gets all of their probabilities; one past the vocabulary makes its row's KL no number; a teacher's logit of -inf adds nothing. dlogits may
+ * be the logits themselves (same ld), else lie clear of everything. */
+typedef struct pk_distill_config {
+    double temperature;  /* 2^-20 to 2^20 */
+    float upstream;
+} pk_distill_config;
+int pk_distill_loss(const pk_distill_config* c, const void* logits, int64_t ld, const int* indices, const float* teacher, const float* teacher_lse,
+                    const float* weights, int64_t rows, int64_t vocab, int64_t top, void* dlogits, int64_t dld, float* kl, double* row_loss, float* loss,
+                    int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -59,6 +59,14 @@ class AdamWConfig(C.Structure):
                                                                                        ("grad_dtype", C.c_int32), ("seed", C.c_uint32)]
 
 
+class NormShape(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("cols", C.c_int64), ("dtype", C.c_int32)]
+
+
+class DistillConfig(C.Structure):
+    _fields_ = [("temperature", C.c_double), ("upstream", C.c_float)]
+
+
 class PkError(RuntimeError):
     def __init__(self, code: int, msg: str):
         super().__init__(f"paperkiln_amd error {code}: {msg}")
@@ -78,7 +86,8 @@ EXPORTS = ["pk_last_error", "pk_init", "pk_attn_fwd", "pk_attn_bwd_workspace_byt
            "pk_op_cross_entropy", "pk_op_adamw", "pk_op_sumsq", "pk_op_gemm", "pk_set_gemm_backend", "pk_set_head_kernel",
            "pk_qk_norm_rope_fwd", "pk_qk_norm_rope_bwd_workspace_bytes", "pk_qk_norm_rope_bwd", "pk_token_logprobs_workspace_bytes", "pk_token_logprobs_fwd",
            "pk_token_logprobs_bwd",
-           "pk_policy_loss_workspace_bytes", "pk_policy_loss", "pk_preference_loss_workspace_bytes", "pk_preference_loss", "pk_adamw_many_workspace_bytes", "pk_adamw_many"]
+           "pk_policy_loss_workspace_bytes", "pk_policy_loss", "pk_preference_loss_workspace_bytes", "pk_preference_loss", "pk_adamw_many_workspace_bytes", "pk_adamw_many",
+           "pk_layernorm_fwd", "pk_layernorm_bwd_workspace_bytes", "pk_layernorm_bwd", "pk_distill_loss"]
 
 
 def lib() -> C.CDLL:
@@ -156,6 +165,12 @@ def lib() -> C.CDLL:
         L.pk_preference_loss.argtypes = [C.POINTER(PreferenceConfig), vp, i64, vp, vp, i64, vp, i64, i64, vp, i64, vp, vp, vp, vp, sz, ci, vp]
         L.pk_adamw_many_workspace_bytes.argtypes = [AT, ci, AC]
         L.pk_adamw_many.argtypes = [AT, ci, AC, vp, sz, vp, vp]
+        NS = C.POINTER(NormShape)
+        L.pk_layernorm_fwd.argtypes = [NS, vp, i64, vp, i64, vp, vp, cf, vp, vp, vp, vp, vp]
+        L.pk_layernorm_bwd_workspace_bytes.argtypes = [NS]
+        L.pk_layernorm_bwd_workspace_bytes.restype = sz
+        L.pk_layernorm_bwd.argtypes = [NS, vp, i64, vp, i64, vp, i64, vp, vp, vp, vp, vp, vp, vp, sz, vp]
+        L.pk_distill_loss.argtypes = [C.POINTER(DistillConfig), vp, i64, vp, vp, vp, vp, i64, i64, i64, vp, i64, vp, vp, vp, ci, vp]
         for fn in (L.pk_qk_norm_rope_bwd_workspace_bytes, L.pk_token_logprobs_workspace_bytes, L.pk_preference_loss_workspace_bytes, L.pk_adamw_many_workspace_bytes):
             fn.restype = sz
         _lib = L

@@ -222,6 +222,15 @@ def preference_loss(logits, targets, seq_start, ref_logp, beta=0.1, label_smooth
     return _native.preference_loss(logits, targets, seq_start, ref_logp, beta, label_smoothing, scale, upstream, out)
 
 
+def distill_loss(logits, indices, teacher_logits, weights, temperature=1.0, teacher_lse=None, upstream=1.0, grad=True, out=None):
+    """Distillation from a teacher's top logits, in one pass over the student's: (loss, dlogits, kl), all on the device. Every row has as many slots as indices (int32 [rows,
+    words], negative: an empty slot) and teacher_logits (float32) have columns. With q = softmax(logits / temperature) and p = softmax(teacher_logits / temperature) over
+    the row's slots -- exp(teacher_logits / temperature - teacher_lse) where that is given, float32 [rows] -- kl is sum p (log p - log q) of each row, the loss
+    temperature^2 * sum(weights * kl); dlogits is the gradient of upstream * loss, for ``logits.backward(dlogits)``, None with ``grad`` False. logits: [rows, vocab] fp32 or
+    bf16 (any row stride), weights: float32 [rows], mask and normalisation; a row of weight 0 is not read. ``out`` may be the logits."""
+    return _native.distill_loss(logits, indices, teacher_logits, weights, temperature, teacher_lse, upstream, grad, out)
+
+
 def clip_grad_norm_(grads, max_norm):
     """ops::clip_grad_norm: scales the fp32 gradients in place when their global norm exceeds max_norm."""
     sq = 0.0

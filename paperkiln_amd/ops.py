@@ -152,6 +152,23 @@ def token_logprobs(logits, targets, scale=1.0):
     return _native.token_logprobs(logits, targets, scale)
 
 
+def layernorm_fwd(x, w, b=None, eps=1e-5, residual=None):
+    """ops::layernorm with the residual addition in front of it: (y, h, mean, rstd), h = x + residual rounded to x's type (x itself without a residual), y = (h - mean) *
+    rstd * w + b. x, residual: [rows, cols] (any row stride), w, b: float32 [cols]; mean and rstd are float32 [rows]."""
+    return _native.layernorm_fwd(x, w, b, eps, residual)
+
+
+def layernorm_bwd(dy, h, w, mean, rstd, dh=None):
+    """Gradients of ``layernorm_fwd`` from its h and its rows' statistics: (dx, dw, db), the weights' in float32, summed in a fixed order. dx is the gradient of x and of the
+    residual alike; dh, what arrives at h by itself, is added to it."""
+    return _native.layernorm_bwd(dy, h, w, mean, rstd, dh)
+
+
+def layernorm(x, w, b=None, eps=1e-5, residual=None):
+    """y of ``layernorm_fwd``, with a residual (y, h); differentiable in all of its tensors."""
+    return _native.layernorm(x, w, b, eps, residual)
+
+
 class _CheckpointFn(torch.autograd.Function):
     """checkpoint(fn, x) of the reference (src/autograd.cpp:68-102): the forward runs fn with the
     tape off and keeps only its input and output; the backward re-runs fn on a detached copy of the

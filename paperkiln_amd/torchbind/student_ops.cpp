@@ -1,0 +1,218 @@
+// The operators of a student model of paperkiln_amd.ops and paperkiln_amd.blockops on torch tensors: layer norm with the residual addition, distillation from a
+// teacher's top logits. As in post_ops.cpp: argument checks, allocation on the current stream of the tensors' device, the C ABI call, the autograd node.
+#include "op_args.h"
+
+namespace pk_torch {
+namespace {
+
+// ---- layer norm ----
+
+constexpr const char* LN = "layernorm";
+struct Rows {
+    int64_t rows, cols, ld;
+};
+Rows rows_of(const char* what, const Tensor& x) {
+    on_gpu(LN, x);
+    if (x.dim() != 2 || x.size(1) < 1) refuse(LN, std::string("shape mismatch: ") + what + " is a [rows, cols] matrix");
+    if (x.stride(1) != 1 && x.size(1) > 1) refuse(LN, std::string(what) + ": the columns must be contiguous");
+    return Rows{x.size(0), x.size(1), x.size(0) > 1 ? x.stride(0) : x.size(1)};
+}
+Rows rows_like(const char* what, const Tensor& x, const Tensor& like) {
+    const Rows r = rows_of(what, x);
+    if (x.sizes() != like.sizes()) refuse(LN, std::string("shape mismatch: ") + what);
+    if (x.scalar_type() != like.scalar_type()) refuse(LN, std::string("dtype mismatch: ") + what);
+    if (x.device() != like.device()) refuse(LN, std::string(what) + " must live on the device of the other tensors");
+    return r;
+}
+struct Normed {
+    Tensor y, h, mean, rstd;
+};
+Normed norm_fwd(const Tensor& x, const Tensor& w, const Tensor& b, double eps, const Tensor& residual) {
+    const Rows m = rows_of("x", x);
+    const pk_norm_shape s{m.rows, m.cols, dtype_code(x.scalar_type())};
+    vector_of(LN, "w", w, at::kFloat, m.cols, x);
+    if (b.defined()) vector_of(LN, "b", b, at::kFloat, m.cols, x);
+    const Rows r = residual.defined() ? rows_like("residual", residual, x) : Rows{};
+    c10::DeviceGuard on(x.device());
+    at::AutoDispatchBelowAutograd below;
+    Normed o;
+    o.y = new_tensor(x.sizes(), x.scalar_type(), x);
+    if (residual.defined()) o.h = new_tensor(x.sizes(), x.scalar_type(), x);
+    o.mean = new_tensor({m.rows}, at::kFloat, x), o.rstd = new_tensor({m.rows}, at::kFloat, x);
+    check(pk_layernorm_fwd(&s, x.const_data_ptr(), m.ld, residual.defined() ? residual.const_data_ptr() : nullptr, r.ld, w.const_data_ptr<float>(),
+                           b.defined() ? b.const_data_ptr<float>() : nullptr, static_cast<float>(eps), o.y.data_ptr(), o.h.defined() ? o.h.data_ptr() : nullptr,
+                           o.mean.data_ptr<float>(), o.rstd.data_ptr<float>(), stream()));
+    return o;
+}
+std::vector<Tensor> norm_bwd(Tensor dy, const Tensor& h, const Tensor& w, const Tensor& mean, const Tensor& rstd, Tensor dh) {
+    const Rows m = rows_of("h", h);
+    const pk_norm_shape s{m.rows, m.cols, dtype_code(h.scalar_type())};
+    vector_of(LN, "w", w, at::kFloat, m.cols, h);
+    vector_of(LN, "mean", mean, at::kFloat, m.rows, h);
+    vector_of(LN, "rstd", rstd, at::kFloat, m.rows, h);
+    c10::DeviceGuard on(h.device());
+    at::AutoDispatchBelowAutograd below;
+    if (dy.dim() == 2 && dy.stride(1) != 1) dy = dy.contiguous();
+    if (dh.defined() && dh.dim() == 2 && dh.stride(1) != 1) dh = dh.contiguous();
+    const Rows g = rows_like("dy", dy, h), a = dh.defined() ? rows_like("dh", dh, h) : Rows{};
+    Tensor dx = new_tensor(h.sizes(), h.scalar_type(), h), dw = new_tensor({m.cols}, at::kFloat, h), db = new_tensor({m.cols}, at::kFloat, h);
+    const int64_t bytes = static_cast<int64_t>(pk_layernorm_bwd_workspace_bytes(&s));
+    Tensor ws = new_tensor({bytes}, at::kByte, h);
+    check(pk_layernorm_bwd(&s, dy.const_data_ptr(), g.ld, h.const_data_ptr(), m.ld, dh.defined() ? dh.const_data_ptr() : nullptr, a.ld, w.const_data_ptr<float>(),
+                           mean.const_data_ptr<float>(), rstd.const_data_ptr<float>(), dx.data_ptr(), dw.data_ptr<float>(), db.data_ptr<float>(), ws.data_ptr(),
+                           static_cast<size_t>(bytes), stream()));
+    return {std::move(dx), std::move(dw), std::move(db)};
+}
+// Keeps what was normalised (its own second output, where there is a residual) and the rows' statistics.
+struct LayerNormBackward : public Node {
+    SavedVariable h, w, mean, rstd;
+    bool has_residual = false;
+
+    explicit LayerNormBackward(torch::autograd::edge_list&& next) : Node(std::move(next)) {}
+    std::string name() const override { return "LayerNormBackward"; }
+    void release_variables() override {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        h.reset_data(), w.reset_data(), mean.reset_data(), rstd.reset_data();
+    }
+    variable_list apply(variable_list&& in) override {
+        first_order(LN);
+        recordable(LN, *this);
+        Tensor th, tw, tm, tr;
+        {
+            const std::lock_guard<std::mutex> lock(mutex_);
+            th = h.unpack(has_residual ? getptr() : nullptr), tw = w.unpack(), tm = mean.unpack(), tr = rstd.unpack();
+        }
+        auto g = norm_bwd(in[0].defined() ? in[0] : at::zeros_like(th), th, tw, tm, tr, has_residual ? in[1] : Tensor());
+        return {g[0], has_residual ? g[0] : Tensor(), g[1], g[2]};  // of x, the residual, w, b
+    }
+};
+Normed norm(const Tensor& x, const Tensor& w, const Tensor& b, double eps, const Tensor& residual) {
+    for (const Tensor* t : {&x, &w, &b, &residual})
+        if (t->defined()) no_tangent(LN, *t);
+    Normed o = norm_fwd(x, w, b, eps, residual);
+    const auto wants = [](const Tensor& t) { return t.defined() && t.requires_grad(); };
+    if (at::GradMode::is_enabled() && (wants(x) || wants(w) || wants(b) || wants(residual))) {
+        auto node = std::shared_ptr<LayerNormBackward>(new LayerNormBackward(torch::autograd::collect_next_edges(x, residual, w, b)), torch::autograd::deleteNode);
+        node->has_residual = residual.defined();
+        torch::autograd::set_history(o.y, node);
+        if (o.h.defined()) torch::autograd::set_history(o.h, node);
+        node->h = o.h.defined() ? SavedVariable(o.h, true) : SavedVariable(x, false);
+        node->w = SavedVariable(w, false), node->mean = SavedVariable(o.mean, false), node->rstd = SavedVariable(o.rstd, false);
+    }
+    return o;
+}
+
+// ---- distillation ----
+
+std::vector<Tensor> distill(const Tensor& logits, const Tensor& indices, const Tensor& teacher, const Tensor& weights, const pk_distill_config& c, const Tensor& lse,
+                            bool grad, const Tensor& out) {
+    constexpr const char* who = "distill_loss";
+    const Logits m = matrix(who, "logits", logits);
+    if (indices.dim() != 2 || teacher.dim() != 2 || indices.size(0) != m.rows || teacher.sizes() != indices.sizes())
+        refuse(who, "shape mismatch: indices and teacher_logits are [rows, words]");
+    const int64_t top = indices.size(1);
+    vector_of(who, "indices", indices, at::kInt, m.rows * top, logits);
+    vector_of(who, "teacher_logits", teacher, at::kFloat, m.rows * top, logits);
+    vector_of(who, "weights", weights, at::kFloat, m.rows, logits);
+    if (lse.defined()) vector_of(who, "teacher_lse", lse, at::kFloat, m.rows, logits);
+    if (!grad && out.defined()) refuse(who, "out is for the gradient");
+    c10::DeviceGuard on(logits.device());
+    at::AutoDispatchBelowAutograd below;
+    Tensor d = grad ? gradient_of(who, logits, out) : Tensor(), kl = new_tensor({m.rows}, at::kFloat, logits), rows = new_tensor({m.rows}, at::kDouble, logits),
+           loss = new_tensor({}, at::kFloat, logits);
+    const int64_t dld = grad ? matrix(who, "out", d).ld : 0;
+    check(pk_distill_loss(&c, logits.const_data_ptr(), m.ld, indices.const_data_ptr<int>(), teacher.const_data_ptr<float>(),
+                          lse.defined() ? lse.const_data_ptr<float>() : nullptr, weights.const_data_ptr<float>(), m.rows, m.vocab, top, grad ? d.data_ptr() : nullptr,
+                          dld, kl.data_ptr<float>(), rows.data_ptr<double>(), loss.data_ptr<float>(), m.dtype, stream()));
+    if (out.defined()) changed(out);
+    return {std::move(loss), std::move(d), std::move(kl)};
+}
+
+// ---- Python side: positional arguments in the order ops.py and blockops.py pass them ----
+
+PyObject* wrap(const Tensor& t) {  // None for one that there is not
+    if (!t.defined()) Py_RETURN_NONE;
+    return THPVariable_Wrap(t);
+}
+PyObject* wrapped(std::initializer_list<Tensor> list) {
+    PyObject* t = PyTuple_New(static_cast<Py_ssize_t>(list.size()));
+    if (!t) throw python_error();
+    Py_ssize_t i = 0;
+    for (const Tensor& x : list) PyTuple_SET_ITEM(t, i++, wrap(x));
+    return t;
+}
+
+// (x, w, b or None, eps, residual or None) -> (y, h or None, mean, rstd)
+PyObject* py_norm_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect(n, 5);
+    const Tensor &x = tensor_arg(a[0], "x"), &w = tensor_arg(a[1], "w");
+    const Tensor b = optional_arg(a[2], "b"), residual = optional_arg(a[4], "residual");
+    const double eps = float_arg(a[3]);
+    Normed o;
+    {
+        pybind11::gil_scoped_release no_gil;
+        o = norm_fwd(x, w, b, eps, residual);
+    }
+    return wrapped({o.y, o.h.defined() ? o.h : x, o.mean, o.rstd});
+    END_HANDLE_TH_ERRORS
+}
+// (dy, h, w, mean, rstd, dh or None) -> (dx, dw, db)
+PyObject* py_norm_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect(n, 6);
+    const Tensor &dy = tensor_arg(a[0], "dy"), &h = tensor_arg(a[1], "h"), &w = tensor_arg(a[2], "w"), &mean = tensor_arg(a[3], "mean"), &rstd = tensor_arg(a[4], "rstd");
+    const Tensor dh = optional_arg(a[5], "dh");
+    std::vector<Tensor> g;
+    {
+        pybind11::gil_scoped_release no_gil;
+        g = norm_bwd(dy, h, w, mean, rstd, dh);
+    }
+    return tuple_of(std::move(g));
+    END_HANDLE_TH_ERRORS
+}
+// (x, w, b or None, eps, residual or None) -> y, or (y, h) with a residual, on the tape
+PyObject* py_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect(n, 5);
+    const Tensor &x = tensor_arg(a[0], "x"), &w = tensor_arg(a[1], "w");
+    const Tensor b = optional_arg(a[2], "b"), residual = optional_arg(a[4], "residual");
+    const double eps = float_arg(a[3]);
+    Normed o;
+    {
+        pybind11::gil_scoped_release no_gil;
+        o = norm(x, w, b, eps, residual);
+    }
+    if (!residual.defined()) return THPVariable_Wrap(std::move(o.y));
+    return wrapped({o.y, o.h});
+    END_HANDLE_TH_ERRORS
+}
+// (logits, indices, teacher_logits, weights, temperature, teacher_lse or None, upstream, grad, out or None) -> (loss, dlogits or None, kl)
+PyObject* py_distill(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect(n, 9);
+    const Tensor &x = tensor_arg(a[0], "logits"), &i = tensor_arg(a[1], "indices"), &t = tensor_arg(a[2], "teacher_logits"), &w = tensor_arg(a[3], "weights");
+    const pk_distill_config c{float_arg(a[4]), number_arg(a[6])};
+    const Tensor lse = optional_arg(a[5], "teacher_lse"), out = optional_arg(a[8], "out");
+    const bool grad = bool_arg(a[7]);
+    std::vector<Tensor> r;
+    {
+        pybind11::gil_scoped_release no_gil;
+        r = distill(x, i, t, w, c, lse, grad, out);
+    }
+    return wrapped({r[0], r[1], r[2]});
+    END_HANDLE_TH_ERRORS
+}
+
+PyMethodDef g_methods[] = {
+    {"layernorm_fwd", reinterpret_cast<PyCFunction>(py_norm_fwd), METH_FASTCALL, "(y, h, mean, rstd)"},
+    {"layernorm_bwd", reinterpret_cast<PyCFunction>(py_norm_bwd), METH_FASTCALL, "(dx, dw, db)"},
+    {"layernorm", reinterpret_cast<PyCFunction>(py_norm), METH_FASTCALL, "y or (y, h), differentiable"},
+    {"distill_loss", reinterpret_cast<PyCFunction>(py_distill), METH_FASTCALL, "(loss, dlogits or None, kl)"},
+    {nullptr, nullptr, 0, nullptr}};
+
+}  // namespace
+
+PyMethodDef* student_methods() { return g_methods; }
+
+}  // namespace pk_torch

@@ -78,6 +78,7 @@ inline void expect(Py_ssize_t n, Py_ssize_t want) {
     if (n != want) throw torch::TypeError("expected " + std::to_string(want) + " arguments, got " + std::to_string(n));
 }
 
-PyMethodDef* post_methods();  // post_ops.cpp
+PyMethodDef* post_methods();     // post_ops.cpp
+PyMethodDef* student_methods();  // student_ops.cpp
 
 }  // namespace pk_torch

@@ -240,6 +240,6 @@ PyMODINIT_FUNC PyInit__torch_ops() {
     Py_DECREF(lib);
     if (!g_error) return nullptr;
     PyObject* module = PyModule_Create(&g_module);
-    if (module && PyModule_AddFunctions(module, pk_torch::post_methods()) < 0) Py_CLEAR(module);
+    if (module && (PyModule_AddFunctions(module, pk_torch::post_methods()) < 0 || PyModule_AddFunctions(module, pk_torch::student_methods()) < 0)) Py_CLEAR(module);
     return module;
 }
