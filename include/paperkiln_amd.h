@@ -430,6 +430,24 @@ int pk_distill_loss(const pk_distill_config* c, const void* logits, int64_t ld, 
                     const float* weights, int64_t rows, int64_t vocab, int64_t top, void* dlogits, int64_t dld, float* kl, double* row_loss, float* loss,
                     int dtype, void* stream);
 
+/* Gated delta rule: a sequence mixed through a state S [dk, dv] for every head of v, in time linear in its length,
+ *   S_t = e^{g_t} S_{t-1} + k_t u_t^T,  u_t = beta_t (v_t - e^{g_t} S_{t-1}^T k_t),  o_t = scale S_t^T q_t.
+ * q, k are [B, T, Hk, dk], v and o [B, T, Hv, dv] in any strides; a head of q and k serves Hv / Hk neighbouring heads of v. g (log-decays) and beta are fp32
+ * [B, T, Hv], dense. state_in, state_out: fp32 [B, Hv, dk, dv], dense; NULL: begins with zeros, is not wanted; they may be the same. Keys are expected of
+ * about unit length and beta in 0 to 2: past that the rule itself grows without bound. g = -inf (or below -1000) starts afresh, so several documents may follow one another in a
+ * row; a token of g 0 and beta 0, finite in q, k and v, leaves the state as it is (padding). Up to 16 tokens the rule is walked through token by token, with
+ * the state in registers and no workspace (its bytes are then 0): serving. Results lie clear of everything that is read, but for state_out. */
+typedef struct pk_delta_shape {
+    int32_t B, T;    /* either may be 0; at most 2^20 heads of sequences and 2^25 chunks of 64 tokens */
+    int32_t Hk, Hv;  /* Hv a multiple of Hk */
+    int32_t dk, dv;  /* 1 to 128, 1 to 256 */
+    int32_t dtype;   /* PK_F32 | PK_BF16: q, k, v, o and their gradients */
+    float scale;
+} pk_delta_shape;
+size_t pk_delta_rule_fwd_workspace_bytes(const pk_delta_shape* s);
+int pk_delta_rule_fwd(const pk_delta_shape* s, const pk_tensor4* q, const pk_tensor4* k, const pk_tensor4* v, const float* g, const float* beta, const float* state_in,
+                      const pk_tensor4* o, float* state_out, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

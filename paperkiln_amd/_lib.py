@@ -67,6 +67,10 @@ class DistillConfig(C.Structure):
     _fields_ = [("temperature", C.c_double), ("upstream", C.c_float)]
 
 
+class DeltaShape(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("B", "T", "Hk", "Hv", "dk", "dv", "dtype")] + [("scale", C.c_float)]
+
+
 class PkError(RuntimeError):
     def __init__(self, code: int, msg: str):
         super().__init__(f"paperkiln_amd error {code}: {msg}")
@@ -87,7 +91,8 @@ EXPORTS = ["pk_last_error", "pk_init", "pk_attn_fwd", "pk_attn_bwd_workspace_byt
            "pk_qk_norm_rope_fwd", "pk_qk_norm_rope_bwd_workspace_bytes", "pk_qk_norm_rope_bwd", "pk_token_logprobs_workspace_bytes", "pk_token_logprobs_fwd",
            "pk_token_logprobs_bwd",
            "pk_policy_loss_workspace_bytes", "pk_policy_loss", "pk_preference_loss_workspace_bytes", "pk_preference_loss", "pk_adamw_many_workspace_bytes", "pk_adamw_many",
-           "pk_layernorm_fwd", "pk_layernorm_bwd_workspace_bytes", "pk_layernorm_bwd", "pk_distill_loss"]
+           "pk_layernorm_fwd", "pk_layernorm_bwd_workspace_bytes", "pk_layernorm_bwd", "pk_distill_loss",
+           "pk_delta_rule_fwd_workspace_bytes", "pk_delta_rule_fwd"]
 
 
 def lib() -> C.CDLL:
@@ -171,6 +176,10 @@ def lib() -> C.CDLL:
         L.pk_layernorm_bwd_workspace_bytes.restype = sz
         L.pk_layernorm_bwd.argtypes = [NS, vp, i64, vp, i64, vp, i64, vp, vp, vp, vp, vp, vp, vp, sz, vp]
         L.pk_distill_loss.argtypes = [C.POINTER(DistillConfig), vp, i64, vp, vp, vp, vp, i64, i64, i64, vp, i64, vp, vp, vp, ci, vp]
+        DS = C.POINTER(DeltaShape)
+        L.pk_delta_rule_fwd_workspace_bytes.argtypes = [DS]
+        L.pk_delta_rule_fwd_workspace_bytes.restype = sz
+        L.pk_delta_rule_fwd.argtypes = [DS, T4, T4, T4, vp, vp, vp, T4, vp, vp, sz, vp]
         for fn in (L.pk_qk_norm_rope_bwd_workspace_bytes, L.pk_token_logprobs_workspace_bytes, L.pk_preference_loss_workspace_bytes, L.pk_adamw_many_workspace_bytes):
             fn.restype = sz
         _lib = L

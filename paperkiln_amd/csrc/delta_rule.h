@@ -1,0 +1,225 @@
+// What the kernels of the gated delta rule share (delta_rule.hip forward, delta_rule_bwd.hip backward).
+//
+// Chunks of 64 tokens. With G the sum of a chunk's log-decays up to a token, D_ij = exp(G_i - G_j) for j <= i, gamma_i = exp(G_i), delta_j = exp(G_63 - G_j):
+//   M_ij = beta_i D_ij k_i.k_j (j < i)     T = (I + M)^-1     A_ij = scale D_ij q_i.k_j (j <= i)
+//   R = beta (V - gamma K S)     U = T R     O = scale gamma Q S + A U     S' = gamma_63 S + K^T (delta U)
+//
+// Everything but q, k, v (and do) is a value of 32 bits that enters matrix products: it goes in as bf16 parts, x = x0 + x1 + x2 with 8 bits each, and a product
+// of two such values is the sum of the six products of parts whose places add up to 2 at most. What is left out is 2^-24 of a term, the rounding that a
+// product in 32 bits has; the matrix cores take 16 such products in the time of one in fp32. Tensors of bf16 are one part, tensors of fp32 three.
+//
+// v_mfma_f32_16x16x32_bf16, lane l = 16 g + c: A row c, k = 8g .. 8g+7; B column c, k = 8g .. 8g+7; C column c, rows 4g .. 4g+3.
+// Products are formed transposed (rows: columns of the state or of v; columns: tokens or k's columns), so that a lane's four results are
+// neighbours in a row of memory.
+#pragma once
+#include <algorithm>
+
+#include "post.h"
+
+namespace pk {
+namespace delta {
+
+constexpr int C = 64;       // tokens of a chunk
+constexpr int VB = 32;      // columns of the state that a workgroup of a scan has
+constexpr int VP = VB + 4;  // their pitch in LDS: 18 banks, so neither the stores of 8 bytes down 16 rows nor transposing reads of 4 rows meet a bank twice
+
+inline int chunks(int T) { return (T + C - 1) / C; }
+inline int blocks(int dv) { return (dv + VB - 1) / VB; }
+
+typedef f32x4 f32x4_any __attribute__((aligned(4)));
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+typedef u32x2 u32x2_any __attribute__((aligned(2)));
+
+__device__ inline f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+
+// Two values as N bf16 parts each, packed.
+template <int N>
+__device__ inline void split2(float x, float y, uint32_t (&p)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        p[i] = pack_bf16(x, y);
+        if (i + 1 < N) x -= __uint_as_float(p[i] << 16), y -= __uint_as_float(p[i] & 0xFFFF0000u);
+    }
+}
+template <int N>
+__device__ inline void split4(const f32x4& x, u32x2 (&p)[N]) {
+    uint32_t a[N], b[N];
+    split2(x[0], x[1], a), split2(x[2], x[3], b);
+#pragma unroll
+    for (int i = 0; i < N; ++i) p[i] = u32x2{a[i], b[i]};
+}
+// Eight values along k as an operand's parts.
+template <int N>
+struct Operand {
+    bf16x8 part[N];
+};
+template <int N>
+__device__ inline Operand<N> split8(const f32x4& lo, const f32x4& hi) {
+    u32x2 a[N], b[N];
+    split4(lo, a), split4(hi, b);
+    Operand<N> o;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const u32x4 v = {a[i][0], a[i][1], b[i][0], b[i][1]};
+        o.part[i] = *reinterpret_cast<const bf16x8*>(&v);
+    }
+    return o;
+}
+// c += a b: of two values in parts the products down to place MOST.
+template <int MOST, int NA, int NB>
+__device__ inline void product(const Operand<NA>& a, const Operand<NB>& b, f32x4& c) {
+#pragma unroll
+    for (int s = MOST; s >= 0; --s)  // the small ones first
+#pragma unroll
+        for (int i = 0; i < NA; ++i)
+            if (s - i >= 0 && s - i < NB) c = mfma16(a.part[i], b.part[s - i], c);
+}
+
+// ---- operands from LDS: N parts of a matrix of R rows, one behind the other ----
+// rows r0 .. r0+15, k along a row from k0 on
+template <int N, int R, int P>
+__device__ inline Operand<N> rows_of(const uint16_t* m, int r0, int k0, int lane) {
+    Operand<N> o;
+    const uint16_t* p = m + (r0 + (lane & 15)) * P + k0 + 8 * (lane >> 4);
+#pragma unroll
+    for (int i = 0; i < N; ++i) o.part[i] = lds_read8(p + i * R * P);
+    return o;
+}
+// columns c0 .. c0+15, k down the rows from k0 on
+template <int N, int R, int P>
+__device__ inline Operand<N> cols_of(const uint16_t* m, int k0, int c0, int lane) {
+    typedef short s16x8 __attribute__((ext_vector_type(8)));
+    Operand<N> o;
+    const int g = lane >> 4, j = lane & 15;
+    const uint16_t* p = m + (k0 + 8 * g + (j >> 2)) * P + c0 + 4 * (j & 3);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const s16x4 lo = lds_read_tr4(p + i * R * P), hi = lds_read_tr4(p + i * R * P + 4 * P);
+        const s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        o.part[i] = *reinterpret_cast<const bf16x8*>(&v);
+    }
+    return o;
+}
+// four values of row r from column c0 on
+template <int N, int R, int P>
+__device__ inline void put4(uint16_t* m, int r, int c0, const f32x4& x) {
+    u32x2 p[N];
+    split4(x, p);
+#pragma unroll
+    for (int i = 0; i < N; ++i) *reinterpret_cast<u32x2*>(m + (i * R + r) * P + c0) = p[i];
+}
+
+// ---- from memory ----
+template <typename T>
+constexpr int PARTS = sizeof(T) == 4 ? 3 : 1;
+// Eight values of a row of n from column c on, zeros past its end.
+__device__ inline Operand<1> load8(const uint16_t* row, int c, int n) {
+    u32x4 v = {0, 0, 0, 0};
+    if (c + 8 <= n) {
+        v = *reinterpret_cast<const u32x4_any*>(row + c);
+    } else {
+        for (int i = 0; i < 8; ++i)
+            if (c + i < n) {
+                const uint32_t e = static_cast<uint32_t>(row[c + i]) << (16 * (i & 1));
+                if (i < 2) v[0] |= e;
+                else if (i < 4) v[1] |= e;
+                else if (i < 6) v[2] |= e;
+                else v[3] |= e;
+            }
+    }
+    Operand<1> o;
+    o.part[0] = *reinterpret_cast<const bf16x8*>(&v);
+    return o;
+}
+// Four values of a row of n from column c on, as they are.
+__device__ inline f32x4 load4(const float* row, int c, int n) {
+    if (c + 4 <= n) return *reinterpret_cast<const f32x4_any*>(row + c);
+    return f32x4{c < n ? row[c] : 0.0f, c + 1 < n ? row[c + 1] : 0.0f, c + 2 < n ? row[c + 2] : 0.0f, 0.0f};
+}
+__device__ inline f32x4 load4(const uint16_t* row, int c, int n) {
+    const auto f = [](uint32_t x) { return __uint_as_float(x << 16); };
+    if (c + 4 <= n) {
+        const u32x2 v = *reinterpret_cast<const u32x2_any*>(row + c);
+        return f32x4{f(v[0]), __uint_as_float(v[0] & 0xFFFF0000u), f(v[1]), __uint_as_float(v[1] & 0xFFFF0000u)};
+    }
+    return f32x4{c < n ? f(row[c]) : 0.0f, c + 1 < n ? f(row[c + 1]) : 0.0f, c + 2 < n ? f(row[c + 2]) : 0.0f, 0.0f};
+}
+__device__ inline Operand<3> load8(const float* row, int c, int n) { return split8<3>(load4(row, c, n), load4(row, c + 4, n)); }
+__device__ inline void store4(float* row, int c, int n, const f32x4& x) {
+    if (c + 4 <= n) {
+        *reinterpret_cast<f32x4_any*>(row + c) = x;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+            if (c + i < n) row[c + i] = x[i];
+    }
+}
+__device__ inline void store4(uint16_t* row, int c, int n, const f32x4& x) {
+    const u32x2 v = {pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
+    if (c + 4 <= n) {
+        *reinterpret_cast<u32x2_any*>(row + c) = v;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+            if (c + i < n) row[c + i] = static_cast<uint16_t>(v[i >> 1] >> (16 * (i & 1)));
+    }
+}
+// A chunk's rows of q or k (n of them are there, the others zeros) as parts in LDS, by NT threads; columns past dk are zeros.
+template <typename T, int DK, int P, int NT>
+__device__ inline void tile_to_lds(const T* base, int64_t st, int n, int dk, uint16_t* m) {
+    constexpr int PER = DK / 8;
+    for (int i = threadIdx.x; i < C * PER; i += NT) {
+        const int r = i / PER, c = i % PER * 8;
+        const Operand<PARTS<T>> o = load8(base + (r < n ? r : 0) * st, c, r < n ? dk : 0);
+#pragma unroll
+        for (int p = 0; p < PARTS<T>; ++p) *reinterpret_cast<bf16x8*>(m + (p * C + r) * P + c) = o.part[p];
+    }
+}
+
+// A problem as the kernels see it. Strides are in elements.
+struct View {
+    void* ptr;
+    int64_t sb, st, sh;
+};
+template <typename T>
+__device__ inline T* head(const View& v, int b, int h) {
+    return static_cast<T*>(v.ptr) + b * v.sb + h * v.sh;
+}
+struct Rule {
+    View q, k, v, o;                // o: the forward's
+    const float *g, *beta;          // [B][T][Hv]
+    const float* state_in;          // [B][Hv][dk][dv], or null
+    float* state_out;               // or null
+    // for every unit (batch, head of v) and chunk:
+    uint16_t *inverse, *attn;       // parts of T and A, [64][64] each
+    float2* decay;                  // gamma and delta of its tokens
+    float *states, *puts;           // backward: the state that the chunk begins with, [dk][dv]; U, [64][dv]
+    // backward
+    View dout, dq, dk_, dv_;
+    float *dg, *dbeta;
+    const float* dstate_out;        // gradient of the state that the rule leaves, or null
+    float* dstate_in;               // of the one that it begins with, or null
+    uint16_t *inverse_t, *attn_t;   // transposed
+    float *dstates, *dputs;         // the gradient of the state that the chunk leaves; of R
+    int B, T, Hk, Hv, dk, dv, chunks;
+    float scale;
+};
+// Workgroups of one unit go to one XCD, whose L2 then has the unit's q, k and matrices for all of its blocks. Launch with grid.x = unit_grid.
+inline unsigned unit_grid(int64_t units, int per) { return static_cast<unsigned>((units + 7) / 8 * 8 * per); }
+__device__ inline bool unit_of(int id, int units, int per, int& unit, int& blk) {
+    const int j = id >> 3;
+    unit = quotient(j, per) * 8 + (id & 7), blk = j - quotient(j, per) * per;
+    return unit < units;
+}
+
+// What the chunks are made of that does not depend on a state, for the forward or (transposed as well) for the backward.
+int launch_chunks(const Rule& a, int dtype, bool backward, hipStream_t st);
+// The states that the chunks begin with and what they put into them.
+int launch_states(const Rule& a, int dtype, hipStream_t st);
+int check(const char* who, const pk_delta_shape* s);
+bool view_of(const pk_tensor4* t, View& v);
+inline size_t pad(size_t bytes) { return (bytes + 255) & ~size_t{255}; }
+constexpr size_t MATRIX = C * C * sizeof(uint16_t);
+
+}  // namespace delta
+}  // namespace pk

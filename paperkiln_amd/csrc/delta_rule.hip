@@ -1,0 +1,427 @@
+// Gated delta rule, forward: over a sequence in chunks of 64 tokens, and token by token.
+//
+//   S_t = e^{g_t} S_{t-1} + k_t u_t^T,   u_t = beta_t (v_t - e^{g_t} S_{t-1}^T k_t),   o_t = scale S_t^T q_t
+//
+// In chunks (delta_rule.h) one launch forms what does not depend on a state, T and A of every chunk, and a second one walks down the chunks, a workgroup for 32 columns of a
+// head's state: the columns do not know of one another. What bounds the walk is its own chain: three products and three exchanges through LDS a chunk.
+// Token by token, the state in registers, memory bounds it: the state read and written once.
+#include "delta_rule.h"
+
+namespace pk {
+namespace delta {
+namespace {
+
+// e^x, x from differences in 64 bits; a decay below e^-1000 is none.
+__device__ inline float decay_of(double x) { return __builtin_amdgcn_exp2f(static_cast<float>(x * 1.4426950408889634074)); }
+__device__ inline double held(float g) { return g < -1000.0f ? -1000.0 : static_cast<double>(g); }
+
+// ---- what does not depend on a state ----
+// A wavefront for a unit's chunk. T by forward substitution, a lane for each of its columns: row i is the unit row less M_ij times the rows j above.
+constexpr int MP = C + 4;
+template <typename T, int DK, int PA, bool BACKWARD>
+__global__ __launch_bounds__(64) void chunk_matrices(Rule a) {
+    constexpr int N = PARTS<T>, MOST = N == 1 ? 0 : 2;
+    __shared__ float m[C * MP];
+    __shared__ double total[C];
+    const int lane = threadIdx.x, g = lane >> 4, c16 = lane & 15;
+    const int64_t unit = blockIdx.x / static_cast<unsigned>(a.chunks);
+    const int chunk = blockIdx.x % static_cast<unsigned>(a.chunks), b = static_cast<int>(unit / a.Hv), h = static_cast<int>(unit % a.Hv);
+    const int t0 = chunk * C, n = min(C, a.T - t0);
+    const int64_t at = (static_cast<int64_t>(b) * a.T + t0) * a.Hv + h;
+    // the sum of the log-decays
+    double sum = lane < n ? held(a.g[at + static_cast<int64_t>(lane) * a.Hv]) : 0.0;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const double up = __shfl_up(sum, o);
+        if (lane >= o) sum += up;
+    }
+    total[lane] = sum;
+    const int64_t place = unit * a.chunks + chunk;
+    a.decay[place * C + lane] = make_float2(decay_of(sum), decay_of(__shfl(sum, 63) - sum));
+    const float beta = lane < n ? a.beta[at + static_cast<int64_t>(lane) * a.Hv] : 0.0f;
+    __syncthreads();
+    const int hk = h / (a.Hv / a.Hk);
+    const T *q = head<const T>(a.q, b, hk) + static_cast<int64_t>(t0) * a.q.st, *k = head<const T>(a.k, b, hk) + static_cast<int64_t>(t0) * a.k.st;
+    uint16_t *attn = a.attn + place * PA * (C * C), *attn_t = BACKWARD ? a.attn_t + place * 3 * (C * C) : nullptr;
+#pragma unroll 1
+    for (int it = 0; it < 4; ++it) {
+        const int i = 16 * it + c16, ri = i < n ? i : 0, di = i < n ? a.dk : 0;
+        Operand<N> ki[DK / 32], qi[DK / 32];
+#pragma unroll
+        for (int kk = 0; kk < DK / 32; ++kk) ki[kk] = load8(k + ri * a.k.st, 32 * kk + 8 * g, di), qi[kk] = load8(q + ri * a.q.st, 32 * kk + 8 * g, di);
+        const float bi = __shfl(beta, i);
+#pragma unroll 1
+        for (int jt = 0; jt < 4; ++jt) {
+            f32x4 kk4 = {0, 0, 0, 0}, qk4 = kk4, kq4 = kk4;  // rows j, column i; kq4: rows i, column j, transposed
+            if (jt <= it) {
+                const int j = 16 * jt + c16, rj = j < n ? j : 0, dj = j < n ? a.dk : 0;
+#pragma unroll
+                for (int kk = 0; kk < DK / 32; ++kk) {
+                    const Operand<N> kj = load8(k + rj * a.k.st, 32 * kk + 8 * g, dj);
+                    product<MOST>(kj, ki[kk], kk4), product<MOST>(kj, qi[kk], qk4);
+                    if (BACKWARD) product<MOST>(qi[kk], kj, kq4);
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int j = 16 * jt + 4 * g + r;
+                    const float d = j <= i ? decay_of(total[i] - total[j]) : 0.0f;
+                    kk4[r] = j < i ? bi * d * kk4[r] : 0.0f, qk4[r] = j <= i ? a.scale * d * qk4[r] : 0.0f;
+                    if (BACKWARD) {
+                        const int row = 16 * it + 4 * g + r, col = 16 * jt + c16;
+                        kq4[r] = col <= row ? a.scale * decay_of(total[row] - total[col]) * kq4[r] : 0.0f;
+                    }
+                }
+            }
+            *reinterpret_cast<f32x4*>(m + i * MP + 16 * jt + 4 * g) = kk4;
+            if (!BACKWARD) put4<PA, C, C>(attn, i, 16 * jt + 4 * g, qk4);
+            if (BACKWARD) put4<3, C, C>(attn_t, 16 * jt + c16, 16 * it + 4 * g, kq4);
+        }
+    }
+    __syncthreads();
+    float t[C];
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+        float s[4] = {i == lane ? 1.0f : 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < i; j += 4) {
+            const f32x4 row = *reinterpret_cast<const f32x4*>(m + i * MP + j);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (j + e < i) s[e] = fmaf(-row[e], t[j + e], s[e]);
+        }
+        t[i] = (s[0] + s[1]) + (s[2] + s[3]);
+    }
+    if (BACKWARD) {
+        uint16_t* out = a.inverse_t + place * 3 * (C * C);
+#pragma unroll
+        for (int i = 0; i < C; i += 4) put4<3, C, C>(out, lane, i, f32x4{t[i], t[i + 1], t[i + 2], t[i + 3]});
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < C; ++i) m[i * MP + lane] = t[i];
+    __syncthreads();
+    uint16_t* out = a.inverse + place * 3 * (C * C);
+    for (int i = lane; i < C * C / 8; i += 64) {
+        const float* from = m + i / 8 * MP + i % 8 * 8;
+        const Operand<3> o = split8<3>(*reinterpret_cast<const f32x4*>(from), *reinterpret_cast<const f32x4*>(from + 4));
+#pragma unroll
+        for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(out + p * C * C + i * 8) = o.part[p];
+    }
+}
+
+// ---- the walk down the chunks ----
+// Four wavefronts: wavefront w has 16 of the 32 columns and two of the four tiles of 16 tokens (0 and 3, or 1 and 2: T and A are lower triangles), of the state half of its rows.
+// STATES: for the backward, the states and U go to memory and there is no O.
+__device__ inline int token_tile(int wave, int i) { return (wave >> 1) ? 1 + i : 3 * i; }
+
+template <typename T, int DK, bool STATES>
+__global__ __launch_bounds__(256) void walk(Rule a) {
+    constexpr int N = PARTS<T>, KP = DK + 16, KS = DK / 32, KT = DK / 32, PO = N == 1 ? 2 : 3;  // PO: parts of U and A on their way to O
+    extern __shared__ uint16_t lds[];
+    uint16_t *kt = lds, *st = kt + N * C * KP, *rt = st + 3 * DK * VP, *dt = rt + 3 * C * VP, *ut = dt + 3 * C * VP;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c16 = lane & 15;
+    int unit, blk;
+    if (!unit_of(blockIdx.x, a.B * a.Hv, (a.dv + VB - 1) / VB, unit, blk)) return;
+    const int b = unit / a.Hv, h = unit - b * a.Hv, hk = h / (a.Hv / a.Hk);
+    const int vt = 16 * (wave & 1), vc = VB * blk + vt + 4 * g;  // this lane's four columns
+    const T *q = head<const T>(a.q, b, hk), *k = head<const T>(a.k, b, hk), *v = head<const T>(a.v, b, h);
+    T* out = STATES ? nullptr : head<T>(a.o, b, h);
+    const int64_t state_at = static_cast<int64_t>(unit) * a.dk * a.dv;
+    f32x4 S[KT];
+#pragma unroll
+    for (int i = 0; i < KT; ++i) {
+        const int r = 16 * ((wave >> 1) * KT + i) + c16;
+        S[i] = a.state_in && r < a.dk ? load4(a.state_in + state_at + static_cast<int64_t>(r) * a.dv, vc, a.dv) : f32x4{0, 0, 0, 0};
+    }
+    for (int chunk = 0; chunk < a.chunks; ++chunk) {
+        const int t0 = chunk * C, n = min(C, a.T - t0);
+        const int64_t place = static_cast<int64_t>(unit) * a.chunks + chunk;
+        const float2* decay = a.decay + place * C;
+        tile_to_lds<T, DK, KP, 256>(k + static_cast<int64_t>(t0) * a.k.st, a.k.st, n, a.dk, kt);
+#pragma unroll
+        for (int i = 0; i < KT; ++i) {
+            const int r = 16 * ((wave >> 1) * KT + i) + c16;
+            put4<3, DK, VP>(st, r, vt + 4 * g, S[i]);
+            if (STATES && r < a.dk) store4(a.states + (place * a.dk + r) * a.dv, vc, a.dv, S[i]);
+        }
+        __syncthreads();
+        // R = beta (V - gamma K S), and gamma Q S
+        f32x4 O[2] = {};
+        {
+            f32x4 P[2] = {};
+            const T* qr[2];
+            int dq[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int t = 16 * token_tile(wave, i) + c16;
+                qr[i] = q + static_cast<int64_t>(t0 + (t < n ? t : 0)) * a.q.st, dq[i] = t < n ? a.dk : 0;
+            }
+#pragma unroll
+            for (int kk = 0; kk < KS; ++kk) {
+                const Operand<3> s = cols_of<3, DK, VP>(st, 32 * kk, vt, lane);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    product<2>(s, rows_of<N, C, KP>(kt, 16 * token_tile(wave, i), 32 * kk, lane), P[i]);
+                    if (!STATES) product<PO - 1>(s, load8(qr[i], 32 * kk + 8 * g, dq[i]), O[i]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int t = 16 * token_tile(wave, i) + c16;
+                const float beta = t < n ? a.beta[(static_cast<int64_t>(b) * a.T + t0 + t) * a.Hv + h] : 0.0f, gamma = decay[t].x;
+                const f32x4 x = load4(v + static_cast<int64_t>(t0 + (t < n ? t : 0)) * a.v.st, vc, t < n ? a.dv : 0);
+                f32x4 R;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) R[r] = t < n ? beta * fmaf(-gamma, P[i][r], x[r]) : 0.0f, O[i][r] *= a.scale * gamma;
+                put4<3, C, VP>(rt, t, vt + 4 * g, R);
+            }
+        }
+        __syncthreads();
+        // U = T R
+        {
+            const uint16_t* inverse = a.inverse + place * 3 * (C * C);
+            f32x4 U[2] = {};
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk) {
+                const Operand<3> r = cols_of<3, C, VP>(rt, 32 * kk, vt, lane);
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    if (kk == 0 || token_tile(wave, i) >= 2) product<2>(r, rows_of<3, C, C>(inverse, 16 * token_tile(wave, i), 32 * kk, lane), U[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int t = 16 * token_tile(wave, i) + c16;
+                const float delta = decay[t].y;
+                if (STATES)
+                    store4(a.puts + (place * C + t) * a.dv, vc, a.dv, U[i]);
+                else
+                    put4<PO, C, VP>(ut, t, vt + 4 * g, U[i]);
+                put4<3, C, VP>(dt, t, vt + 4 * g, U[i] * delta);
+            }
+        }
+        __syncthreads();
+        // O += A U, S = gamma S + K^T (delta U)
+        if (!STATES) {
+            const uint16_t* attn = a.attn + place * PO * (C * C);
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk) {
+                const Operand<PO> u = cols_of<PO, C, VP>(ut, 32 * kk, vt, lane);
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    if (kk == 0 || token_tile(wave, i) >= 2) product<PO - 1>(u, rows_of<PO, C, C>(attn, 16 * token_tile(wave, i), 32 * kk, lane), O[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int t = 16 * token_tile(wave, i) + c16;
+                if (t < n) store4(out + static_cast<int64_t>(t0 + t) * a.o.st, vc, a.dv, O[i]);
+            }
+        }
+        const float whole = decay[C - 1].x;
+#pragma unroll
+        for (int i = 0; i < KT; ++i) S[i] *= whole;
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            const Operand<3> u = cols_of<3, C, VP>(dt, 32 * kk, vt, lane);
+#pragma unroll
+            for (int i = 0; i < KT; ++i) product<2>(u, cols_of<N, C, KP>(kt, 32 * kk, 16 * ((wave >> 1) * KT + i), lane), S[i]);
+        }
+        __syncthreads();
+    }
+    if (!a.state_out) return;
+#pragma unroll
+    for (int i = 0; i < KT; ++i) {
+        const int r = 16 * ((wave >> 1) * KT + i) + c16;
+        if (r < a.dk) store4(a.state_out + state_at + static_cast<int64_t>(r) * a.dv, vc, a.dv, S[i]);
+    }
+}
+template <typename T, int DK, bool STATES>
+constexpr size_t walk_lds() {
+    return sizeof(uint16_t) * (PARTS<T> * C * (DK + 16) + 3 * DK * VP + 6 * C * VP + (STATES ? 0 : (PARTS<T> == 1 ? 2 : 3) * C * VP));
+}
+
+// ---- token by token ----
+// A workgroup for CB columns of a head's state, four of them and every RG-th row to a thread. Both products of a token with the decayed state, S^T k and S^T q, are formed in one walk
+// over the rows and added up in one exchange: o = scale (e^g S^T q + (q.k) u).
+constexpr int STEP_NT = 256;
+template <typename T, int CB, int RPT>
+__global__ __launch_bounds__(STEP_NT) void steps(Rule a) {
+    constexpr int QUADS = CB / 4, RG = STEP_NT / QUADS, WG = 64 / QUADS, WAVES = STEP_NT / 64;
+    __shared__ f32x4 sums[2][2][WAVES][QUADS];
+    __shared__ float dots[2][WAVES];
+    const int tid = threadIdx.x, wave = tid >> 6, quad = tid % QUADS, rg = tid / QUADS;
+    const int nblk = (a.dv + CB - 1) / CB, unit = quotient(blockIdx.x, nblk), blk = blockIdx.x - unit * nblk;
+    const int b = quotient(unit, a.Hv), h = unit - b * a.Hv, hk = quotient(h, a.Hv / a.Hk), c = CB * blk + 4 * quad;
+    const T *q = head<const T>(a.q, b, hk), *k = head<const T>(a.k, b, hk), *v = head<const T>(a.v, b, h);
+    T* out = head<T>(a.o, b, h);
+    const int64_t state_at = static_cast<int64_t>(unit) * a.dk * a.dv;
+    f32x4 S[RPT];
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+        const int r = rg + i * RG;
+        S[i] = a.state_in && r < a.dk ? load4(a.state_in + state_at + static_cast<int64_t>(r) * a.dv, c, a.dv) : f32x4{0, 0, 0, 0};
+    }
+    for (int t = 0; t < a.T; ++t) {
+        float kr[RPT], qr[RPT];
+#pragma unroll
+        for (int i = 0; i < RPT; ++i) {
+            const int r = rg + i * RG;
+            kr[i] = r < a.dk ? elem(k, t * a.k.st + r) : 0.0f, qr[i] = r < a.dk ? elem(q, t * a.q.st + r) : 0.0f;
+        }
+        const int64_t at = (static_cast<int64_t>(b) * a.T + t) * a.Hv + h;
+        const float decay = decay_of(held(a.g[at])), beta = a.beta[at];
+        const f32x4 x = load4(v + t * a.v.st, c, a.dv);
+        f32x4 sk = {0, 0, 0, 0}, sq = sk;
+        float qk = 0.0f;
+#pragma unroll
+        for (int i = 0; i < RPT; ++i) {
+            S[i] *= decay;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sk[e] = fmaf(S[i][e], kr[i], sk[e]), sq[e] = fmaf(S[i][e], qr[i], sq[e]);
+            qk = fmaf(qr[i], kr[i], qk);
+        }
+#pragma unroll
+        for (int o = QUADS; o < 64; o <<= 1) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sk[e] += __shfl_xor(sk[e], o), sq[e] += __shfl_xor(sq[e], o);
+            qk += __shfl_xor(qk, o);
+        }
+        const int turn = t & 1;  // the sums of the token before may still be read
+        if ((tid & 63) < QUADS) sums[turn][0][wave][quad] = sk, sums[turn][1][wave][quad] = sq;
+        if ((tid & 63) == 0) dots[turn][wave] = qk;
+        __syncthreads();
+        sk = sums[turn][0][0][quad], sq = sums[turn][1][0][quad], qk = dots[turn][0];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) sk += sums[turn][0][w][quad], sq += sums[turn][1][w][quad], qk += dots[turn][w];
+        f32x4 u;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) u[e] = beta * (x[e] - sk[e]);
+#pragma unroll
+        for (int i = 0; i < RPT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) S[i][e] = fmaf(kr[i], u[e], S[i][e]);
+        if (rg == 0) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sq[e] = a.scale * fmaf(qk, u[e], sq[e]);
+            store4(out + t * a.o.st, c, a.dv, sq);
+        }
+    }
+    if (!a.state_out) return;
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+        const int r = rg + i * RG;
+        if (r < a.dk) store4(a.state_out + state_at + static_cast<int64_t>(r) * a.dv, c, a.dv, S[i]);
+    }
+}
+
+// ---- launches ----
+
+constexpr int FEW_TOKENS = 16;
+template <typename T, int DK, bool STATES>
+int launch_walk(const Rule& a, hipStream_t st) {
+    constexpr size_t lds = walk_lds<T, DK, STATES>();
+    static_assert(lds <= 160 * 1024, "LDS of a CU");
+    PK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(walk<T, DK, STATES>), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
+    walk<T, DK, STATES><<<unit_grid(static_cast<int64_t>(a.B) * a.Hv, blocks(a.dv)), 256, lds, st>>>(a);
+    return launched();
+}
+template <typename T, bool STATES>
+int launch_walk(const Rule& a, hipStream_t st) {
+    return a.dk <= 32 ? launch_walk<T, 32, STATES>(a, st) : a.dk <= 64 ? launch_walk<T, 64, STATES>(a, st) : launch_walk<T, 128, STATES>(a, st);
+}
+template <typename T, int DK>
+void launch_matrices(const Rule& a, bool backward, hipStream_t st) {
+    const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.B) * a.Hv * a.chunks));
+    backward ? chunk_matrices<T, DK, 3, true><<<grid, 64, 0, st>>>(a) : chunk_matrices<T, DK, (PARTS<T> == 1 ? 2 : 3), false><<<grid, 64, 0, st>>>(a);
+}
+template <typename T>
+void launch_matrices(const Rule& a, bool backward, hipStream_t st) {
+    a.dk <= 32 ? launch_matrices<T, 32>(a, backward, st) : a.dk <= 64 ? launch_matrices<T, 64>(a, backward, st) : launch_matrices<T, 128>(a, backward, st);
+}
+template <typename T>
+void launch_steps(const Rule& a, hipStream_t st) {
+    constexpr int CB = 32;
+    const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.B) * a.Hv * ((a.dv + CB - 1) / CB)));
+    if (a.dk <= 32) return steps<T, CB, 1><<<grid, STEP_NT, 0, st>>>(a);
+    if (a.dk <= 64) return steps<T, CB, 2><<<grid, STEP_NT, 0, st>>>(a);
+    steps<T, CB, 4><<<grid, STEP_NT, 0, st>>>(a);
+}
+
+struct Room {
+    size_t inverse, attn, decay, all;
+};
+Room room_of(const pk_delta_shape* s) {
+    const size_t places = static_cast<size_t>(s->B) * s->Hv * chunks(s->T);
+    Room r;
+    r.inverse = pad(places * 3 * MATRIX), r.attn = pad(places * (s->dtype == PK_F32 ? 3 : 2) * MATRIX), r.decay = pad(places * C * sizeof(float2));
+    r.all = r.inverse + r.attn + r.decay;
+    return r;
+}
+
+}  // namespace
+
+int launch_chunks(const Rule& a, int dtype, bool backward, hipStream_t st) {
+    dtype == PK_BF16 ? launch_matrices<uint16_t>(a, backward, st) : launch_matrices<float>(a, backward, st);
+    return launched();
+}
+int launch_states(const Rule& a, int dtype, hipStream_t st) { return dtype == PK_BF16 ? launch_walk<uint16_t, true>(a, st) : launch_walk<float, true>(a, st); }
+
+int check(const char* who, const pk_delta_shape* s) {
+    const std::string w(who);
+    if (!s) return fail(PK_ERR_ARGUMENT, w + ": null pointer");
+    if (s->B < 0 || s->T < 0 || s->Hk < 1 || s->Hv < 1 || s->Hv % s->Hk) return fail(PK_ERR_SHAPE, w + ": shape mismatch (heads of v are shared out evenly to those of k)");
+    if (s->dk < 1 || s->dk > 128 || s->dv < 1 || s->dv > 256) return fail(PK_ERR_SHAPE, w + ": shape mismatch (dk 1 to 128, dv 1 to 256)");
+    if (static_cast<int64_t>(s->B) * s->Hv > (1 << 20) || s->T > (1 << 26) || static_cast<int64_t>(s->B) * s->Hv * (chunks(s->T) + 1) > (1 << 25))
+        return fail(PK_ERR_SHAPE, w + ": shape mismatch (at most 2^20 heads of sequences and 2^25 chunks of 64 tokens)");
+    if (!known_dtype(s->dtype)) return fail(PK_ERR_ARGUMENT, w + ": dtype must be PK_F32 or PK_BF16");
+    if (!std::isfinite(s->scale)) return fail(PK_ERR_ARGUMENT, w + ": scale must be finite");
+    return PK_OK;
+}
+bool view_of(const pk_tensor4* t, View& v) {
+    if (!t || !t->ptr) return false;
+    v = View{t->ptr, t->stride_b, t->stride_t, t->stride_h};
+    return true;
+}
+
+}  // namespace delta
+}  // namespace pk
+
+using namespace pk;
+using namespace pk::delta;
+
+extern "C" {
+
+size_t pk_delta_rule_fwd_workspace_bytes(const pk_delta_shape* s) {
+    if (delta::check("pk_delta_rule_fwd", s) != PK_OK || s->T <= FEW_TOKENS) return 0;
+    return room_of(s).all;
+}
+
+int pk_delta_rule_fwd(const pk_delta_shape* s, const pk_tensor4* q, const pk_tensor4* k, const pk_tensor4* v, const float* g, const float* beta, const float* state_in,
+                      const pk_tensor4* o, float* state_out, void* workspace, size_t workspace_bytes, void* stream) {
+    return c_entry([&] {
+        const std::string who = "pk_delta_rule_fwd";
+        if (int rc = delta::check(who.c_str(), s)) return rc;
+        Rule a{};
+        const bool tokens = static_cast<int64_t>(s->B) * s->T > 0;
+        if (s->B == 0) return static_cast<int>(PK_OK);
+        if (tokens && (!view_of(q, a.q) || !view_of(k, a.k) || !view_of(v, a.v) || !view_of(o, a.o) || !g || !beta)) return fail(PK_ERR_ARGUMENT, who + ": null pointer");
+        const size_t need = pk_delta_rule_fwd_workspace_bytes(s);
+        if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
+            return fail(PK_ERR_WORKSPACE, who + ": workspace too small (pk_delta_rule_fwd_workspace_bytes)");
+        touch({a.q.ptr, a.k.ptr, a.v.ptr, g, beta, state_in, a.o.ptr, state_out, workspace}, stream);
+        hipStream_t st = static_cast<hipStream_t>(stream);
+        a.g = g, a.beta = beta, a.state_in = state_in, a.state_out = state_out;
+        a.B = s->B, a.T = s->T, a.Hk = s->Hk, a.Hv = s->Hv, a.dk = s->dk, a.dv = s->dv, a.chunks = chunks(s->T), a.scale = s->scale;
+        if (s->T <= FEW_TOKENS) {
+            if (s->T == 0 && (!state_out || state_out == state_in)) return static_cast<int>(PK_OK);
+            s->dtype == PK_BF16 ? launch_steps<uint16_t>(a, st) : launch_steps<float>(a, st);
+            return launched();
+        }
+        const Room r = room_of(s);
+        char* ws = static_cast<char*>(workspace);
+        a.inverse = reinterpret_cast<uint16_t*>(ws), a.attn = reinterpret_cast<uint16_t*>(ws + r.inverse), a.decay = reinterpret_cast<float2*>(ws + r.inverse + r.attn);
+        if (int rc = launch_chunks(a, s->dtype, false, st)) return rc;
+        return s->dtype == PK_BF16 ? launch_walk<uint16_t, false>(a, st) : launch_walk<float, false>(a, st);
+    });
+}
+
+}  // extern "C"

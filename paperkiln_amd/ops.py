@@ -152,6 +152,19 @@ def token_logprobs(logits, targets, scale=1.0):
     return _native.token_logprobs(logits, targets, scale)
 
 
+def gated_delta_rule_fwd(q, k, v, g, beta, scale, initial_state=None):
+    """A sequence mixed through a state S [dk, dv] for every head of v: S_t = e^g_t S_{t-1} + k_t u_t^T with u_t = beta_t (v_t - e^g_t S_{t-1}^T k_t), o_t = scale S_t^T q_t.
+    q, k: [B,T,Hk,dk], v: [B,T,Hv,dv] (any batch/token/head strides; a head of q and k serves Hv/Hk neighbouring heads of v; dk at most 128, dv 256), g (log-decays) and beta:
+    float32 [B,T,Hv], initial_state: float32 [B,Hv,dk,dv], zeros without. Returns (o, the state behind the last token). Keys are expected of about unit length. g = -inf
+    starts afresh, so that documents may follow one another in a row; a token of g 0 and beta 0 leaves the state as it is (padding)."""
+    return _native.gated_delta_rule_fwd(q, k, v, g, beta, scale, initial_state)
+
+
+def gated_delta_step_(q, k, v, g, beta, scale, state):
+    """The same for the next token, or the next few, of sequences whose state is kept: moves ``state`` (float32 [B,Hv,dk,dv]) on in place and returns o."""
+    return _native.gated_delta_step(q, k, v, g, beta, scale, state)
+
+
 def layernorm_fwd(x, w, b=None, eps=1e-5, residual=None):
     """ops::layernorm with the residual addition in front of it: (y, h, mean, rstd), h = x + residual rounded to x's type (x itself without a residual), y = (h - mean) *
     rstd * w + b. x, residual: [rows, cols] (any row stride), w, b: float32 [cols]; mean and rstd are float32 [rows]."""

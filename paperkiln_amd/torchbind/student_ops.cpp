@@ -128,6 +128,51 @@ std::vector<Tensor> distill(const Tensor& logits, const Tensor& indices, const T
     return {std::move(loss), std::move(d), std::move(kl)};
 }
 
+// ---- gated delta rule ----
+
+constexpr const char* DELTA = "gated_delta_rule";
+pk_tensor4 heads_of(const char* what, const Tensor& x) {
+    if (x.stride(3) != 1 && x.size(3) > 1 && x.numel() != 0) refuse(DELTA, std::string(what) + ": expected a [B,T,H,d] tensor with contiguous head_dim");
+    return pk_tensor4{x.data_ptr(), x.stride(0), x.stride(1), x.stride(2)};
+}
+pk_delta_shape delta_shape(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta, double scale, const Tensor& state) {
+    on_gpu(DELTA, q);
+    if (q.dim() != 4 || k.dim() != 4 || v.dim() != 4 || k.sizes() != q.sizes() || v.size(0) != q.size(0) || v.size(1) != q.size(1))
+        refuse(DELTA, "shape mismatch: q and k are [B,T,Hk,dk], v [B,T,Hv,dv]");
+    if (k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type()) refuse(DELTA, "dtype mismatch");
+    for (const Tensor* x : {&k, &v})
+        if (x->device() != q.device()) refuse(DELTA, "q, k and v must live on one device");
+    pk_delta_shape s{};
+    s.B = narrow(DELTA, q.size(0)), s.T = narrow(DELTA, q.size(1)), s.Hk = narrow(DELTA, q.size(2)), s.Hv = narrow(DELTA, v.size(2)), s.dk = narrow(DELTA, q.size(3)),
+    s.dv = narrow(DELTA, v.size(3)), s.dtype = dtype_code(q.scalar_type()), s.scale = static_cast<float>(scale);
+    const auto scalars = [&](const char* what, const Tensor& x) {
+        if (x.dim() != 3 || x.size(0) != s.B || x.size(1) != s.T || x.size(2) != s.Hv) refuse(DELTA, std::string("shape mismatch: ") + what + " is [B,T,Hv]");
+        vector_of(DELTA, what, x, at::kFloat, x.numel(), q);
+    };
+    scalars("g", g), scalars("beta", beta);
+    if (state.defined()) {
+        if (state.dim() != 4 || state.size(0) != s.B || state.size(1) != s.Hv || state.size(2) != s.dk || state.size(3) != s.dv) refuse(DELTA, "shape mismatch: the state is [B,Hv,dk,dv]");
+        vector_of(DELTA, "the state", state, at::kFloat, state.numel(), q);
+    }
+    return s;
+}
+const float* floats(const Tensor& t) { return t.defined() ? t.const_data_ptr<float>() : nullptr; }
+Tensor room(size_t bytes, const Tensor& like) { return bytes ? new_tensor({static_cast<int64_t>(bytes)}, at::kByte, like) : Tensor(); }
+
+// o, and the state behind the last token: a new one, or `into`
+std::pair<Tensor, Tensor> delta_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta, double scale, const Tensor& state, const Tensor& into) {
+    const pk_delta_shape s = delta_shape(q, k, v, g, beta, scale, state);
+    c10::DeviceGuard on(q.device());
+    at::AutoDispatchBelowAutograd below;
+    Tensor o = new_tensor(v.sizes(), v.scalar_type(), q), last = into.defined() ? into : new_tensor({s.B, s.Hv, s.dk, s.dv}, at::kFloat, q);
+    const size_t bytes = pk_delta_rule_fwd_workspace_bytes(&s);
+    Tensor ws = room(bytes, q);
+    const pk_tensor4 q4 = heads_of("q", q), k4 = heads_of("k", k), v4 = heads_of("v", v), o4 = heads_of("o", o);
+    check(pk_delta_rule_fwd(&s, &q4, &k4, &v4, floats(g), floats(beta), floats(state), &o4, last.data_ptr<float>(), bytes ? ws.data_ptr() : nullptr, bytes, stream()));
+    if (into.defined()) changed(into);
+    return {std::move(o), std::move(last)};
+}
+
 // ---- Python side: positional arguments in the order ops.py and blockops.py pass them ----
 
 PyObject* wrap(const Tensor& t) {  // None for one that there is not
@@ -204,7 +249,40 @@ PyObject* py_distill(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// (q, k, v, g, beta, scale, state or None) -> (o, state)
+PyObject* py_delta_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect(n, 7);
+    const Tensor &q = tensor_arg(a[0], "q"), &k = tensor_arg(a[1], "k"), &v = tensor_arg(a[2], "v"), &g = tensor_arg(a[3], "g"), &beta = tensor_arg(a[4], "beta");
+    const double scale = float_arg(a[5]);
+    const Tensor state = optional_arg(a[6], "state");
+    std::pair<Tensor, Tensor> r;
+    {
+        pybind11::gil_scoped_release no_gil;
+        r = delta_fwd(q, k, v, g, beta, scale, state, Tensor());
+    }
+    return wrapped({r.first, r.second});
+    END_HANDLE_TH_ERRORS
+}
+// (q, k, v, g, beta, scale, state) -> o, the state moved on in place
+PyObject* py_delta_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect(n, 7);
+    const Tensor &q = tensor_arg(a[0], "q"), &k = tensor_arg(a[1], "k"), &v = tensor_arg(a[2], "v"), &g = tensor_arg(a[3], "g"), &beta = tensor_arg(a[4], "beta"),
+                 &state = tensor_arg(a[6], "state");
+    const double scale = float_arg(a[5]);
+    Tensor o;
+    {
+        pybind11::gil_scoped_release no_gil;
+        o = delta_fwd(q, k, v, g, beta, scale, state, state).first;
+    }
+    return THPVariable_Wrap(std::move(o));
+    END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef g_methods[] = {
+    {"gated_delta_rule_fwd", reinterpret_cast<PyCFunction>(py_delta_fwd), METH_FASTCALL, "(o, state)"},
+    {"gated_delta_step", reinterpret_cast<PyCFunction>(py_delta_step), METH_FASTCALL, "o, the state moved on in place"},
     {"layernorm_fwd", reinterpret_cast<PyCFunction>(py_norm_fwd), METH_FASTCALL, "(y, h, mean, rstd)"},
     {"layernorm_bwd", reinterpret_cast<PyCFunction>(py_norm_bwd), METH_FASTCALL, "(dx, dw, db)"},
     {"layernorm", reinterpret_cast<PyCFunction>(py_norm), METH_FASTCALL, "y or (y, h), differentiable"},
