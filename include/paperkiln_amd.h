@@ -448,6 +448,14 @@ size_t pk_delta_rule_fwd_workspace_bytes(const pk_delta_shape* s);
 int pk_delta_rule_fwd(const pk_delta_shape* s, const pk_tensor4* q, const pk_tensor4* k, const pk_tensor4* v, const float* g, const float* beta, const float* state_in,
                       const pk_tensor4* o, float* state_out, void* workspace, size_t workspace_bytes, void* stream);
 
+/* The gradients, from the inputs: the states are formed again. d_o and the gradients of q, k, v as their tensors, in strides of their own; dg, dbeta [B, T, Hv];
+ * dstate_out, the gradient of the state behind the last token (NULL: zeros), dstate_in, of the first one (NULL: not wanted). Gradients of heads that several others share are
+ * their sums, in a fixed order. dg is 0 where g is below -1000. */
+size_t pk_delta_rule_bwd_workspace_bytes(const pk_delta_shape* s);
+int pk_delta_rule_bwd(const pk_delta_shape* s, const pk_tensor4* d_o, const float* dstate_out, const pk_tensor4* q, const pk_tensor4* k, const pk_tensor4* v, const float* g,
+                      const float* beta, const float* state_in, const pk_tensor4* dq, const pk_tensor4* dk, const pk_tensor4* dv, float* dg, float* dbeta, float* dstate_in,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

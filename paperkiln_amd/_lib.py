@@ -92,7 +92,8 @@ EXPORTS = ["pk_last_error", "pk_init", "pk_attn_fwd", "pk_attn_bwd_workspace_byt
            "pk_token_logprobs_bwd",
            "pk_policy_loss_workspace_bytes", "pk_policy_loss", "pk_preference_loss_workspace_bytes", "pk_preference_loss", "pk_adamw_many_workspace_bytes", "pk_adamw_many",
            "pk_layernorm_fwd", "pk_layernorm_bwd_workspace_bytes", "pk_layernorm_bwd", "pk_distill_loss",
-           "pk_delta_rule_fwd_workspace_bytes", "pk_delta_rule_fwd"]
+           "pk_delta_rule_fwd_workspace_bytes", "pk_delta_rule_fwd",
+           "pk_delta_rule_bwd_workspace_bytes", "pk_delta_rule_bwd"]
 
 
 def lib() -> C.CDLL:
@@ -179,6 +180,9 @@ def lib() -> C.CDLL:
         DS = C.POINTER(DeltaShape)
         L.pk_delta_rule_fwd_workspace_bytes.argtypes = [DS]
         L.pk_delta_rule_fwd_workspace_bytes.restype = sz
+        L.pk_delta_rule_bwd_workspace_bytes.argtypes = [DS]
+        L.pk_delta_rule_bwd_workspace_bytes.restype = sz
+        L.pk_delta_rule_bwd.argtypes = [DS, T4, vp, T4, T4, T4, vp, vp, vp, T4, T4, T4, vp, vp, vp, vp, sz, vp]
         L.pk_delta_rule_fwd.argtypes = [DS, T4, T4, T4, vp, vp, vp, T4, vp, vp, sz, vp]
         for fn in (L.pk_qk_norm_rope_bwd_workspace_bytes, L.pk_token_logprobs_workspace_bytes, L.pk_preference_loss_workspace_bytes, L.pk_adamw_many_workspace_bytes):
             fn.restype = sz

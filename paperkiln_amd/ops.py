@@ -160,6 +160,17 @@ def gated_delta_rule_fwd(q, k, v, g, beta, scale, initial_state=None):
     return _native.gated_delta_rule_fwd(q, k, v, g, beta, scale, initial_state)
 
 
+def gated_delta_rule_bwd(d_o, q, k, v, g, beta, scale, initial_state=None, d_state=None):
+    """Gradients of ``gated_delta_rule_fwd`` from its inputs, the states formed again: (dq, dk, dv, dg, dbeta, d_initial_state), the last one None without an initial
+    state. d_state: the gradient of the state behind the last token, zeros without. dg is 0 where g is below -1000."""
+    return _native.gated_delta_rule_bwd(d_o, q, k, v, g, beta, scale, initial_state, d_state)
+
+
+def gated_delta_rule(q, k, v, g, beta, scale, initial_state=None):
+    """``gated_delta_rule_fwd``, differentiable in all of its tensors; keeps nothing but them."""
+    return _native.gated_delta_rule(q, k, v, g, beta, scale, initial_state)
+
+
 def gated_delta_step_(q, k, v, g, beta, scale, state):
     """The same for the next token, or the next few, of sequences whose state is kept: moves ``state`` (float32 [B,Hv,dk,dv]) on in place and returns o."""
     return _native.gated_delta_step(q, k, v, g, beta, scale, state)

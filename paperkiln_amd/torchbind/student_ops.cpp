@@ -173,6 +173,68 @@ std::pair<Tensor, Tensor> delta_fwd(const Tensor& q, const Tensor& k, const Tens
     return {std::move(o), std::move(last)};
 }
 
+std::vector<Tensor> delta_bwd(Tensor d_o, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta, double scale, const Tensor& state,
+                              const Tensor& dlast) {
+    const pk_delta_shape s = delta_shape(q, k, v, g, beta, scale, state);
+    if (d_o.sizes() != v.sizes() || d_o.scalar_type() != v.scalar_type() || d_o.device() != q.device()) refuse(DELTA, "shape mismatch: d_o");
+    if (dlast.defined()) {
+        if (dlast.dim() != 4 || dlast.size(0) != s.B || dlast.size(1) != s.Hv || dlast.size(2) != s.dk || dlast.size(3) != s.dv)
+            refuse(DELTA, "shape mismatch: the state's gradient is [B,Hv,dk,dv]");
+        vector_of(DELTA, "the state's gradient", dlast, at::kFloat, dlast.numel(), q);
+    }
+    c10::DeviceGuard on(q.device());
+    at::AutoDispatchBelowAutograd below;
+    if (d_o.stride(3) != 1) d_o = d_o.contiguous();
+    Tensor dq = new_tensor(q.sizes(), q.scalar_type(), q), dk = new_tensor(k.sizes(), k.scalar_type(), q), dv = new_tensor(v.sizes(), v.scalar_type(), q),
+           dg = new_tensor(g.sizes(), at::kFloat, q), dbeta = new_tensor(g.sizes(), at::kFloat, q), dfirst;
+    if (state.defined()) dfirst = new_tensor(state.sizes(), at::kFloat, q);
+    const size_t bytes = pk_delta_rule_bwd_workspace_bytes(&s);
+    Tensor ws = room(bytes, q);
+    const pk_tensor4 o4 = heads_of("d_o", d_o), q4 = heads_of("q", q), k4 = heads_of("k", k), v4 = heads_of("v", v), dq4 = heads_of("dq", dq), dk4 = heads_of("dk", dk), dv4 = heads_of("dv", dv);
+    check(pk_delta_rule_bwd(&s, &o4, floats(dlast), &q4, &k4, &v4, floats(g), floats(beta), floats(state), &dq4, &dk4, &dv4, dg.data_ptr<float>(), dbeta.data_ptr<float>(),
+                            dfirst.defined() ? dfirst.data_ptr<float>() : nullptr, bytes ? ws.data_ptr() : nullptr, bytes, stream()));
+    return {std::move(dq), std::move(dk), std::move(dv), std::move(dg), std::move(dbeta), std::move(dfirst)};
+}
+// Keeps the inputs only: the backward forms the states again.
+struct GatedDeltaRuleBackward : public Node {
+    SavedVariable q, k, v, g, beta, state;
+    bool has_state = false;
+    double scale = 1.0;
+
+    explicit GatedDeltaRuleBackward(torch::autograd::edge_list&& next) : Node(std::move(next)) {}
+    std::string name() const override { return "GatedDeltaRuleBackward"; }
+    void release_variables() override {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        for (SavedVariable* x : {&q, &k, &v, &g, &beta, &state}) x->reset_data();
+    }
+    variable_list apply(variable_list&& in) override {
+        first_order(DELTA);
+        recordable(DELTA, *this);
+        Tensor tq, tk, tv, tg, tb, ts;
+        {
+            const std::lock_guard<std::mutex> lock(mutex_);
+            tq = q.unpack(), tk = k.unpack(), tv = v.unpack(), tg = g.unpack(), tb = beta.unpack();
+            if (has_state) ts = state.unpack();
+        }
+        return delta_bwd(in[0].defined() ? in[0] : at::zeros_like(tv), tq, tk, tv, tg, tb, scale, ts, in[1].defined() ? in[1].contiguous() : Tensor());
+    }
+};
+std::pair<Tensor, Tensor> delta(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta, double scale, const Tensor& state) {
+    bool wanted = false;
+    for (const Tensor* t : {&q, &k, &v, &g, &beta, &state})
+        if (t->defined()) no_tangent(DELTA, *t), wanted = wanted || t->requires_grad();
+    auto y = delta_fwd(q, k, v, g, beta, scale, state, Tensor());
+    if (at::GradMode::is_enabled() && wanted) {
+        auto node = std::shared_ptr<GatedDeltaRuleBackward>(new GatedDeltaRuleBackward(torch::autograd::collect_next_edges(q, k, v, g, beta, state)), torch::autograd::deleteNode);
+        torch::autograd::set_history(y.first, node);
+        torch::autograd::set_history(y.second, node);
+        node->q = SavedVariable(q, false), node->k = SavedVariable(k, false), node->v = SavedVariable(v, false), node->g = SavedVariable(g, false);
+        node->beta = SavedVariable(beta, false), node->scale = scale, node->has_state = state.defined();
+        if (state.defined()) node->state = SavedVariable(state, false);
+    }
+    return y;
+}
+
 // ---- Python side: positional arguments in the order ops.py and blockops.py pass them ----
 
 PyObject* wrap(const Tensor& t) {  // None for one that there is not
@@ -264,6 +326,37 @@ PyObject* py_delta_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return wrapped({r.first, r.second});
     END_HANDLE_TH_ERRORS
 }
+// (d_o, q, k, v, g, beta, scale, state or None, dstate or None) -> (dq, dk, dv, dg, dbeta, dstate or None)
+PyObject* py_delta_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect(n, 9);
+    const Tensor &d_o = tensor_arg(a[0], "d_o"), &q = tensor_arg(a[1], "q"), &k = tensor_arg(a[2], "k"), &v = tensor_arg(a[3], "v"), &g = tensor_arg(a[4], "g"),
+                 &beta = tensor_arg(a[5], "beta");
+    const double scale = float_arg(a[6]);
+    const Tensor state = optional_arg(a[7], "initial_state"), dstate = optional_arg(a[8], "d_state");
+    std::vector<Tensor> r;
+    {
+        pybind11::gil_scoped_release no_gil;
+        r = delta_bwd(d_o, q, k, v, g, beta, scale, state, dstate);
+    }
+    return wrapped({r[0], r[1], r[2], r[3], r[4], r[5]});
+    END_HANDLE_TH_ERRORS
+}
+// (q, k, v, g, beta, scale, state or None) -> (o, state), on the tape
+PyObject* py_delta(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect(n, 7);
+    const Tensor &q = tensor_arg(a[0], "q"), &k = tensor_arg(a[1], "k"), &v = tensor_arg(a[2], "v"), &g = tensor_arg(a[3], "g"), &beta = tensor_arg(a[4], "beta");
+    const double scale = float_arg(a[5]);
+    const Tensor state = optional_arg(a[6], "initial_state");
+    std::pair<Tensor, Tensor> r;
+    {
+        pybind11::gil_scoped_release no_gil;
+        r = delta(q, k, v, g, beta, scale, state);
+    }
+    return wrapped({r.first, r.second});
+    END_HANDLE_TH_ERRORS
+}
 // (q, k, v, g, beta, scale, state) -> o, the state moved on in place
 PyObject* py_delta_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
@@ -282,6 +375,8 @@ PyObject* py_delta_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 PyMethodDef g_methods[] = {
     {"gated_delta_rule_fwd", reinterpret_cast<PyCFunction>(py_delta_fwd), METH_FASTCALL, "(o, state)"},
+    {"gated_delta_rule_bwd", reinterpret_cast<PyCFunction>(py_delta_bwd), METH_FASTCALL, "(dq, dk, dv, dg, dbeta, dstate or None)"},
+    {"gated_delta_rule", reinterpret_cast<PyCFunction>(py_delta), METH_FASTCALL, "(o, state), differentiable"},
     {"gated_delta_step", reinterpret_cast<PyCFunction>(py_delta_step), METH_FASTCALL, "o, the state moved on in place"},
     {"layernorm_fwd", reinterpret_cast<PyCFunction>(py_norm_fwd), METH_FASTCALL, "(y, h, mean, rstd)"},
     {"layernorm_bwd", reinterpret_cast<PyCFunction>(py_norm_bwd), METH_FASTCALL, "(dx, dw, db)"},

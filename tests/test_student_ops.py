@@ -74,7 +74,47 @@ def test_distill_loss_refuses(change, code):
         assert distill(rows=0, **change) == code
 
 
-SOURCES = ("layernorm.hip", "distill_loss.hip")
+def T4(p, *strides):
+    return C.byref(_lib.Tensor4(p, *(strides or (6400, 64, 64)))) if p else None
+
+
+def delta(entry, **kw):
+    place = dict(q=0, k=1, v=2, o=3, d_o=4, dq=5, dk_=6, dv_=7)
+    d = dict(B=2, T=100, Hk=1, Hv=1, dk=64, dv=64, dtype=_lib.PK_BF16, scale=0.125, g=at(8), beta=at(9), s0=at(10), s1=at(11), ds1=at(12), ds0=at(13), dg=at(14), dbeta=at(15), ws=at(16),
+             ws_bytes=1 << 40, **{n: T4((1 + i) << 24) for n, i in place.items()})
+    d.update(kw)
+    L, s = _lib.lib(), _lib.DeltaShape(d["B"], d["T"], d["Hk"], d["Hv"], d["dk"], d["dv"], d["dtype"], d["scale"])
+    if entry == "fwd":
+        return L.pk_delta_rule_fwd(C.byref(s), d["q"], d["k"], d["v"], d["g"], d["beta"], d["s0"], d["o"], d["s1"], d["ws"], d["ws_bytes"], None)
+    return L.pk_delta_rule_bwd(C.byref(s), d["d_o"], d["ds1"], d["q"], d["k"], d["v"], d["g"], d["beta"], d["s0"], d["dq"], d["dk_"], d["dv_"], d["dg"], d["dbeta"], d["ds0"], d["ws"],
+                               d["ws_bytes"], None)
+
+
+DELTA = [(dict(B=-1), SHAPE), (dict(T=-1), SHAPE), (dict(Hk=0), SHAPE), (dict(Hv=0), SHAPE), (dict(Hk=2, Hv=3), SHAPE), (dict(dk=0), SHAPE), (dict(dk=129), SHAPE), (dict(dv=0), SHAPE),
+         (dict(dv=257), SHAPE), (dict(dtype=2), ARGUMENT), (dict(scale=math.nan), ARGUMENT), (dict(scale=math.inf), ARGUMENT), (dict(B=1 << 20, Hv=2), SHAPE), (dict(T=(1 << 26) + 1), SHAPE),
+         (dict(B=1 << 18, T=1 << 14), SHAPE), (dict(ws=None), WORKSPACE), (dict(ws_bytes=100), WORKSPACE), (dict(ws=C.c_void_p((17 << 24) + 8)), WORKSPACE)]
+DELTA_NULL = {"fwd": ("q", "k", "v", "g", "beta", "o"), "bwd": ("d_o", "q", "k", "v", "g", "beta", "dq", "dk_", "dv_", "dg", "dbeta")}
+
+
+@pytest.mark.parametrize("entry", ["fwd", "bwd"])
+@pytest.mark.parametrize("change,code", DELTA, ids=str)
+def test_gated_delta_rule_refuses(entry, change, code):
+    assert delta(entry, **change) == code and _lib.lib().pk_last_error()
+
+
+@pytest.mark.parametrize("entry", ["fwd", "bwd"])
+def test_gated_delta_rule_refuses_null(entry):
+    for n in DELTA_NULL[entry]:
+        assert delta(entry, **{n: None}) == ARGUMENT, n
+    assert delta(entry, B=0, **{n: None for n in DELTA_NULL[entry]}) == 0    # nothing to do
+    L = _lib.lib()
+    for T, none in ((1, True), (16, True), (17, False)):
+        assert (L.pk_delta_rule_fwd_workspace_bytes(C.byref(_lib.DeltaShape(2, T, 1, 1, 64, 64, 1, 1.0))) == 0) == none
+    assert L.pk_delta_rule_bwd_workspace_bytes(C.byref(_lib.DeltaShape(2, 1, 1, 1, 64, 64, 1, 1.0))) > 0
+    assert L.pk_delta_rule_bwd_workspace_bytes(C.byref(_lib.DeltaShape(2, 1, 1, 1, 640, 64, 1, 1.0))) == 0
+
+
+SOURCES = ("layernorm.hip", "distill_loss.hip", "delta_rule.hip", "delta_rule_bwd.hip")
 
 
 @pytest.fixture(scope="module")

@@ -1,5 +1,5 @@
-"""The operators of a student model on the GPU against plain implementations in 64 bits: layer norm with the residual addition, distillation from a teacher's top
-logits.
+"""The operators of a student model on the GPU against plain implementations in 64 bits: the gated delta rule, layer norm with the residual addition, distillation
+from a teacher's top logits.
 
 Tolerances are counted as in test_post_ops_gpu.py: u = 2^-24 is half a step of fp32 relative to a value, h half a step of the output's type (u, or 2^-8 for bf16). An
 output carries one rounding to its type, h * |value|, and what the 32-bit arithmetic before it adds up to, in u times the largest term that enters it."""
@@ -35,8 +35,313 @@ def same(a, b):
     return len(a) == len(b) and all(torch.equal(bits(x), bits(y)) for x, y in zip(a, b))
 
 
-# ---- layer norm ----------------------------------------------------------------------------------------------------------
+# ---- gated delta rule ----------------------------------------------------------------------------------------------------
 
+
+def plain_delta(q, k, v, g, beta, scale, state=None, do=None, dstate=None):
+    """Token by token in 64 bits; with do the gradients (dq, dk, dv, dg, dbeta, dstate) too, walking back."""
+    B, T, Hk, dk = q.shape
+    Hv, dv = v.shape[2:]
+    rep = Hv // Hk
+    q, k = (x.double().repeat_interleave(rep, 2) for x in (q, k))
+    v, a, b = v.double(), g.double().exp(), beta.double()
+    S = torch.zeros(B, Hv, dk, dv, dtype=F64, device=q.device) if state is None else state.double()
+    outs, steps = [], []
+    for t in range(T):
+        kept = a[:, t, :, None, None] * S
+        e = v[:, t] - (k[:, t, :, :, None] * kept).sum(2)
+        u = b[:, t, :, None] * e
+        after = kept + k[:, t, :, :, None] * u[:, :, None]
+        outs.append(scale * (q[:, t, :, :, None] * after).sum(2))
+        steps.append((S, kept, e, u, after))
+        S = after
+    o = torch.stack(outs, 1) if T else torch.zeros(B, 0, Hv, dv, dtype=F64, device=q.device)
+    if do is None:
+        return o, S
+    D = torch.zeros_like(S) if dstate is None else dstate.double()
+    dq, dk_, dv_, dg, db = (torch.zeros_like(x) for x in (q, k, v, a, b))
+    for t in reversed(range(T)):
+        before, kept, e, u, after = steps[t]
+        d = do[:, t].double()
+        dq[:, t] = scale * (after * d[:, :, None]).sum(-1)
+        D = D + scale * q[:, t, :, :, None] * d[:, :, None]
+        du = (D * k[:, t, :, :, None]).sum(2)
+        dw = b[:, t, :, None] * du
+        dv_[:, t], db[:, t] = dw, (du * e).sum(-1)
+        dk_[:, t] = (D * u[:, :, None]).sum(-1) - (kept * dw[:, :, None]).sum(-1)
+        D = D - k[:, t, :, :, None] * dw[:, :, None]
+        dg[:, t] = (D * kept).sum((-1, -2))
+        D = a[:, t, :, None, None] * D
+    dq, dk_ = (x.unflatten(2, (Hk, rep)).sum(3) for x in (dq, dk_))
+    return (o, S), (dq, dk_, dv_, dg, db, D)
+
+
+def delta_inputs(B, T, Hk, Hv, dk, dv, dtype, seed=1, layout="plain", state=True):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    randn = lambda *s: torch.randn(s, generator=gen, device="cuda")  # noqa: E731
+    unit = lambda x: x / x.square().sum(-1, keepdim=True).sqrt().clamp(min=1e-6)  # noqa: E731
+    q, k, v, do = unit(randn(B, T, Hk, dk)).to(dtype), unit(randn(B, T, Hk, dk) + 0.5).to(dtype), randn(B, T, Hv, dv).to(dtype), randn(B, T, Hv, dv).to(dtype)
+
+    def lay(x):
+        if layout == "heads":       # [B, H, T, d] memory
+            return x.transpose(1, 2).contiguous().transpose(1, 2)
+        if layout == "offset":      # one element past an aligned address, odd pitches
+            return torch.nn.functional.pad(x, (1, 2))[..., 1:-2]
+        if layout == "fused":       # between the columns of a projection
+            return torch.nn.functional.pad(x.flatten(2), (8, 24))[..., 8:-24].unflatten(2, x.shape[2:])
+        return x
+    q, k, v, do = map(lay, (q, k, v, do))
+    beta = torch.sigmoid(randn(B, T, Hv))
+    g = -torch.nn.functional.softplus(randn(B, T, Hv)) * torch.exp(-6.0 * torch.rand((1, 1, Hv), generator=gen, device="cuda"))
+    first = randn(B, Hv, dk, dv) * dk ** -0.5 if state else None
+    return q, k, v, g, beta, first, do, randn(B, Hv, dk, dv)
+
+
+NAMES = ("o", "state", "dq", "dk", "dv", "dg", "dbeta", "dstate")
+
+
+def close(name, got, want, dtype, times=1.0, dk=128, pair=0.0):
+    """The matrix cores add up 32 products at a time, six rounds of them for each 32 of a sum of values in three parts: at most 24 roundings in a row of u each, in either
+    direction: 5 u of a result's root mean square. Three such products follow one another in a chunk (K S, T R, K^T U), and what is wrong in a state shrinks as
+    the state does (unit keys, beta to 1): 9 u. Over all of an output 16 u then, times 2 for a gradient, which goes both ways, and 4 for dg, a sum of differences of terms up to four times its
+    size. dg_t is besides a sum over the chunk's pairs of tokens on either side of t, at most 32 x 32 of them, whose terms are of one size where all keys are the same and nothing decays
+    (dk = 1), while what they come to is the nearest ones': steps with beta of a half forget in two. 1024 independent roundings are 32 of one pair's. Keys of dk random
+    columns overlap by dk^-1/2, twice in a term: 32 / dk. And the pairs on one side of t go out in 64 bits: 4096 terms of `pair` at most leave 4096 * 2^-53 of it. One element: that times 16 (the largest of a million is 5 times their root mean square, and they are of different sizes), of the largest of its head and
+    sequence. The rounding to the output's type is counted by itself."""
+    got, want = got.double(), want.double()
+    assert got.shape == want.shape, name
+    if not want.numel():
+        return
+    n = 16 * times * {"o": 1, "state": 1, "dg": 4 + 32 / dk}.get(name, 2) * U
+    h = HALF[got_type(got, dtype, name)]
+    over = [i for i in range(want.dim()) if i not in (0, head_axis(name))]
+    top = want.abs().amax(over, keepdim=True)
+    within(name, got, want, h * want.abs() + 16 * n * top + 1e-30 + (2.0 ** -41 * pair if name == "dg" else 0.0))
+    if h == U:
+        far, size = float((got - want).norm()), float(want.norm())
+        assert far <= (n + U) * size + 1e-30 + (2.0 ** -41 * pair * want.numel() ** 0.5 if name == "dg" else 0.0), (name, far / max(size, 1e-300) / U)
+
+
+def got_type(got, dtype, name):
+    return FP32 if name in ("state", "dstate", "dg", "dbeta") else dtype
+
+
+def head_axis(name):
+    return 1 if name in ("state", "dstate") else 2
+
+
+def check_delta(pk, q, k, v, g, beta, first, do, dlast, scale, times=1.0):
+    dtype = q.dtype
+    kept = [t.clone() for t in (q, k, v, g, beta, do, dlast)]
+    o, state = pk.ops.gated_delta_rule_fwd(q, k, v, g, beta, scale, first)
+    grads = pk.ops.gated_delta_rule_bwd(do, q, k, v, g, beta, scale, first, dlast)
+    assert same(kept, (q, k, v, g, beta, do, dlast))
+    assert o.dtype == dtype and state.dtype == FP32 and [t.dtype for t in grads[:5]] == [dtype] * 3 + [FP32] * 2 and (grads[5] is None) == (first is None)
+    held = g.clamp(min=-1000.0)
+    (wo, ws), want = plain_delta(q, k, v, held, beta, scale, first, do, dlast)
+    want = list(want)
+    want[3] = torch.where(g < -1000.0, 0.0, want[3])
+    for n, a, b in zip(NAMES, (o, state, *grads), (wo, ws, *want)):
+        if a is not None:
+            close(n, a, b, dtype, times, q.shape[3], 2 * abs(scale) * v.shape[3] * float(do.double().abs().max() * v.double().abs().max()))
+    return (o, state, *grads), (wo, ws, *want)
+
+
+DELTAS = [  # B, T, Hk, Hv, dk, dv, layout, state
+    (1, 1, 1, 1, 1, 1, "plain", True), (2, 1, 2, 4, 64, 64, "plain", True), (1, 2, 1, 1, 3, 5, "plain", False), (2, 15, 2, 2, 32, 32, "fused", True), (3, 16, 1, 3, 40, 72, "heads", False),
+    (2, 17, 2, 2, 64, 64, "plain", True), (1, 63, 1, 1, 128, 128, "plain", True), (2, 64, 3, 3, 64, 128, "heads", True), (1, 65, 2, 6, 48, 80, "offset", True),
+    (2, 130, 1, 7, 64, 64, "fused", False), (1, 200, 2, 2, 128, 256, "plain", True), (1, 257, 1, 2, 127, 33, "offset", False), (3, 100, 2, 2, 16, 8, "plain", True),
+    (1, 300, 3, 3, 33, 31, "heads", True), (9, 70, 1, 1, 96, 96, "fused", True), (1, 500, 1, 1, 31, 1, "plain", True), (1, 129, 1, 2, 1, 255, "offset", True)]
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("case", DELTAS, ids=lambda c: "-".join(map(str, c)))
+def test_gated_delta_rule_against_64_bits(pk, case, dtype):
+    B, T, Hk, Hv, dk, dv, layout, state = case
+    check_delta(pk, *delta_inputs(B, T, Hk, Hv, dk, dv, dtype, 3, layout, state), dk ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("T", [9, 190])
+@pytest.mark.parametrize("which", ["no decay", "no beta", "documents", "strong", "mixed", "same keys", "reflections", "padding"])
+def test_gated_delta_rule_extremes(pk, which, T, dtype):
+    """Decays of 1, of 0 and of nearly 0 among others, and sums of them that go far; keys that repeat with beta 1 (T's rows go back and forth) and beta 2, whose steps are
+    reflections: nothing shrinks what is wrong there, so over 190 tokens it adds up, 3 chunks to a fourfold count."""
+    q, k, v, g, beta, first, do, dlast = delta_inputs(2, T, 2, 4, 64, 48, dtype, 5)
+    times = 1.0
+    if which == "no decay":
+        g, times = torch.zeros_like(g), 4.0
+    elif which == "no beta":
+        beta = torch.zeros_like(beta)
+    elif which == "documents":
+        g[:, 5], g[0, T // 2], g[1, T - 1, 1], g[:, 0, 2] = -math.inf, -math.inf, -math.inf, -math.inf
+    elif which == "strong":
+        g = g * 40 - 30
+    elif which == "mixed":
+        g[:, ::7], g[:, 3::11], g[:, 4] = -50.0, -1e30, -999.0
+    elif which == "same keys":
+        k, beta, g, times = k[:, :1].expand(k.shape), torch.ones_like(beta), g * 0.01, 4.0
+        k = k.contiguous()
+    elif which == "reflections":
+        beta, g, times = torch.full_like(beta, 2.0), torch.zeros_like(g), 4.0
+        k = (k.double() / k.double().norm(dim=-1, keepdim=True)).to(dtype)
+    else:
+        beta[0, T - 6:], g[0, T - 6:] = 0.0, 0.0
+    out, _ = check_delta(pk, q, k, v, g, beta, first, do, dlast, 0.125, times)
+    if which == "padding":   # the state is the one before it, to the bit where the chunks are the same
+        close("state", out[1][:1], plain_delta(*(x[:1, :T - 6] for x in (q, k, v, g, beta)), 0.125, first[:1])[1], dtype)
+    if which == "no beta":
+        assert not out[4].any()
+
+
+def test_gated_delta_rule_goes_on_from_a_state(pk):
+    """A sequence in pieces, each from the state that the one before has left, by tokens and by chunks: the whole one's values. Steps move their state on in place."""
+    for dtype in (FP32, BF16):
+        q, k, v, g, beta, first, _, _ = delta_inputs(2, 150, 2, 4, 64, 64, dtype, 6)
+        wo, ws = plain_delta(q, k, v, g, beta, 0.125, first)
+        state, parts, at = first, [], 0
+        for n in (1, 70, 3, 64, 12):
+            o, state = pk.ops.gated_delta_rule_fwd(*(x[:, at:at + n] .contiguous() if x.dim() == 3 else x[:, at:at + n] for x in (q, k, v, g, beta)), 0.125, state)
+            parts.append(o)
+            at += n
+        close("o", torch.cat(parts, 1), wo, dtype)
+        close("state", state, ws, dtype)
+        moved, parts, version = first.clone(), [], None
+        place = moved.data_ptr()
+        for a, n in ((0, 1), (1, 5), (6, 100), (106, 44)):   # more than a few tokens at once too
+            parts.append(pk.ops.gated_delta_step_(*(x[:, a:a + n].contiguous() if x.dim() == 3 else x[:, a:a + n] for x in (q, k, v, g, beta)), 0.125, moved))
+        assert moved.data_ptr() == place
+        close("o", torch.cat(parts, 1), wo, dtype)
+        close("state", moved, ws, dtype)
+
+
+def test_gated_delta_rule_of_nothing(pk):
+    q, k, v, g, beta, first, do, dlast = delta_inputs(2, 5, 1, 2, 16, 24, FP32, 7)
+    e = lambda x: x[:, :0]  # noqa: E731
+    o, state = pk.ops.gated_delta_rule_fwd(e(q), e(k), e(v), e(g), e(beta), 1.0, first)
+    assert o.shape == (2, 0, 2, 24) and torch.equal(state, first)
+    assert not pk.ops.gated_delta_rule_fwd(e(q), e(k), e(v), e(g), e(beta), 1.0)[1].any()
+    grads = pk.ops.gated_delta_rule_bwd(e(do), e(q), e(k), e(v), e(g), e(beta), 1.0, first, dlast)
+    assert torch.equal(grads[5], dlast) and grads[0].shape == (2, 0, 1, 16)
+    assert not pk.ops.gated_delta_rule_bwd(e(do), e(q), e(k), e(v), e(g), e(beta), 1.0, first)[5].any()
+    o, state = pk.ops.gated_delta_rule_fwd(q[:0], k[:0], v[:0], g[:0], beta[:0], 1.0)
+    assert o.shape == (0, 5, 2, 24) and state.shape == (0, 2, 16, 24)
+    moved = first.clone()
+    pk.ops.gated_delta_step_(e(q), e(k), e(v), e(g), e(beta), 1.0, moved)
+    assert torch.equal(moved, first)
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16], ids=["fp32", "bf16"])
+def test_gated_delta_rule_keeps_a_bad_value_to_its_head(pk, dtype):
+    """What is not finite spoils its head of its sequence from its chunk on, and nothing else: other heads, other sequences, chunks before it (forward) and after it (backward)."""
+    q, k, v, g, beta, first, do, dlast = delta_inputs(2, 200, 2, 4, 32, 40, dtype, 8)
+    fwd = lambda: pk.ops.gated_delta_rule_fwd(q, k, v, g, beta, 1.0, first)  # noqa: E731
+    bwd = lambda: pk.ops.gated_delta_rule_bwd(do, q, k, v, g, beta, 1.0, first, dlast)  # noqa: E731
+    (o, state), grads = fwd(), bwd()
+    v = v.clone()
+    v[1, 130, 2, 7] = math.nan
+    o2, state2 = fwd()
+    good = torch.ones_like(o, dtype=torch.bool)
+    good[1, 128:, 2] = False
+    assert torch.equal(o2[good], o[good]) and bool(torch.isnan(o2[1, 130:, 2, 7].float()).all())
+    assert torch.equal(state2[0], state[0]) and torch.equal(state2[1, [0, 1, 3]], state[1, [0, 1, 3]]) and torch.equal(state2[1, 2, :, :7], state[1, 2, :, :7])
+    for a, b in zip(grads, bwd()):
+        assert torch.equal(a[0], b[0])
+    v = v.nan_to_num()
+    k = k.clone()
+    k[0, 3, 1, 0] = math.inf
+    o2, _ = fwd()
+    assert torch.equal(o2[1, :, 0], o[1, :, 0]) and torch.equal(o2[0, :, :2], o[0, :, :2]) and not bool(torch.isfinite(o2[0, 3:, 2:].float()).any())
+
+
+def test_gated_delta_rule_repeats_its_bits(pk):
+    """The same call twice, and a batch's sequences by themselves: the same bits."""
+    q, k, v, g, beta, first, do, dlast = delta_inputs(3, 150, 2, 6, 64, 64, BF16, 9)
+    run = lambda i: [*pk.ops.gated_delta_rule_fwd(*(x[i] for x in (q, k, v, g, beta)), 0.125, first[i]),  # noqa: E731
+                     *pk.ops.gated_delta_rule_bwd(do[i], *(x[i] for x in (q, k, v, g, beta)), 0.125, first[i], dlast[i])]
+    whole = run(slice(None))
+    assert same(whole, run(slice(None)))
+    for i in range(3):
+        assert same([x[i:i + 1] for x in whole], run(slice(i, i + 1)))
+
+
+def test_gated_delta_rule_gradient_against_differences(pk):
+    """The derivative of sum(o do) + sum(S dS) along a direction against a central difference of the operator in fp32: two sums whose terms carry 64 u of their size, over a
+    step of 2^-6; the third-order term, of a product of at most five inputs' changes, is below 2^-10 of the terms."""
+    q, k, v, g, beta, first, do, dlast = delta_inputs(1, 70, 1, 2, 24, 20, FP32, 10)
+    grads = pk.ops.gated_delta_rule_bwd(do, q, k, v, g, beta, 0.3, first, dlast)
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    inputs = (q, k, v, g, beta, first)
+    sizes = (0.1, 0.1, 0.5, 0.05, 0.1, 0.1)
+    dirs = [s * torch.randn(x.shape, generator=gen, device="cuda") for s, x in zip(sizes, inputs)]
+    step = 2.0 ** -6
+
+    def value(e):
+        o, s = pk.ops.gated_delta_rule_fwd(*(x + e * d for x, d in zip(inputs[:5], dirs)), 0.3, first + e * dirs[5])
+        return float((o.double() * do).sum() + (s.double() * dlast).sum())
+    o, s = pk.ops.gated_delta_rule_fwd(*inputs[:5], 0.3, first)
+    terms = float((o.double() * do).abs().sum() + (s.double() * dlast).abs().sum())
+    slope = float(sum((a.double() * d).sum() for a, d in zip(grads, dirs)))
+    assert abs((value(step) - value(-step)) / (2 * step) - slope) <= (64 * U / step + 2.0 ** -10) * terms
+
+
+def test_gated_delta_rule_under_autograd(pk):
+    """The node gives what the direct backward gives, of one output alone too, for gradients that are not dense."""
+    q, k, v, g, beta, first, do, dlast = delta_inputs(2, 80, 2, 4, 32, 32, BF16, 11, "fused")
+    leaves = [x.detach().clone().requires_grad_() for x in (q, k, v, g, beta, first)]
+    o, state = pk.ops.gated_delta_rule(*leaves[:5], 0.2, leaves[5])
+    plain = [x.detach() for x in leaves]
+    assert same(torch.autograd.grad([o, state], leaves, [do, dlast], retain_graph=True), pk.ops.gated_delta_rule_bwd(do, *plain[:5], 0.2, plain[5], dlast))
+    assert same(torch.autograd.grad(o.sum(), leaves, retain_graph=True), pk.ops.gated_delta_rule_bwd(torch.ones_like(o), *plain[:5], 0.2, plain[5]))
+    sideways = do.transpose(2, 3).contiguous().transpose(2, 3)
+    assert torch.equal(torch.autograd.grad(o, leaves[0], sideways, retain_graph=True)[0], pk.ops.gated_delta_rule_bwd(do, *plain[:5], 0.2, plain[5])[0])
+    far = dlast.transpose(2, 3).contiguous().transpose(2, 3)
+    assert same(torch.autograd.grad(state, leaves, far, retain_graph=True), pk.ops.gated_delta_rule_bwd(torch.zeros_like(do), *plain[:5], 0.2, plain[5], dlast))
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        torch.autograd.grad(o.sum(), leaves[0], create_graph=True)
+    o, _ = pk.ops.gated_delta_rule(*plain[:2], leaves[2], *plain[3:5], 0.2)
+    assert torch.equal(torch.autograd.grad(o, leaves[2], do)[0], pk.ops.gated_delta_rule_bwd(do, *plain[:5], 0.2)[2])
+    with torch.no_grad():
+        assert not pk.ops.gated_delta_rule(*leaves[:5], 0.2)[0].requires_grad
+    moved = plain[5].clone()
+    kept = (moved.requires_grad_() * 1.0)
+    z = kept * kept
+    pk.ops.gated_delta_step_(*plain[:5], 0.2, kept.detach())   # a tensor that another node has saved
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.sum().backward()
+
+
+def test_gated_delta_rule_past_2_to_the_31(pk):
+    """Tokens 2^25 elements apart, the last of them past 2^31 elements of its tensor: what dense copies give, to the bit."""
+    q, k, v, g, beta, first, do, dlast = delta_inputs(1, 70, 1, 1, 32, 32, BF16, 12)
+    pitch = 1 << 25
+    far = torch.zeros(70 * pitch, dtype=BF16, device="cuda")
+    views = [far[64 * i:].as_strided(x.shape, (0, pitch, 0, 1)) for i, x in enumerate((q, k, v, do))]
+    for y, x in zip(views, (q, k, v, do)):
+        y.copy_(x)
+    for T in (70, 9):   # by chunks; by tokens, the far ones
+        part = lambda x: x[:, 70 - T:]  # noqa: E731
+        near = [part(x).contiguous() for x in (q, k, v, g, beta, do)]
+        away = [part(x) for x in views]
+        scalars = (near[3], near[4], 0.2, first)
+        assert same(pk.ops.gated_delta_rule_fwd(*away[:3], *scalars), pk.ops.gated_delta_rule_fwd(*near[:3], *scalars))
+        assert same(pk.ops.gated_delta_rule_bwd(away[3], *away[:3], *scalars, dlast), pk.ops.gated_delta_rule_bwd(near[5], *near[:3], *scalars, dlast))
+
+
+def test_gated_delta_step_of_states_past_2_to_the_31(pk):
+    """140000 heads of states of 128 x 128, more than 2^31 elements: the last ones as by themselves."""
+    B, H = 8750, 16
+    q, k, v, g, beta, _, _, _ = delta_inputs(B, 1, 1, H, 128, 128, BF16, 13, state=False)
+    state = torch.zeros(B, H, 128, 128, device="cuda")
+    state[-1], state[0] = 0.1, -0.2
+    want = [state[i:i + 1].clone() if i >= 0 else state[-1:].clone() for i in (0, -1)]
+    o = pk.ops.gated_delta_step_(q, k, v, g, beta, 0.1, state)
+    for i, w in zip((0, -1), want):
+        at = slice(i, i + 1 if i >= 0 else None)
+        assert torch.equal(o[at], pk.ops.gated_delta_step_(*(x[at] for x in (q, k, v, g, beta)), 0.1, w)) and torch.equal(state[at], w)
+
+
+# ---- layer norm ----------------------------------------------------------------------------------------------------------
 
 NORMS = [  # rows, cols, columns between rows, elements in front of the first
     (1, 1, 0, 0), (3, 2, 0, 0), (5, 7, 0, 0), (2, 8, 0, 0), (17, 64, 0, 0), (9, 511, 0, 0), (6, 512, 0, 0), (5, 513, 520, 0), (7, 1000, 1001, 1), (4, 1024, 0, 0), (3, 1025, 0, 0),
