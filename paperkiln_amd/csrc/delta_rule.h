@@ -164,6 +164,109 @@ __device__ inline void store4(uint16_t* row, int c, int n, const f32x4& x) {
             if (c + i < n) row[c + i] = static_cast<uint16_t>(v[i >> 1] >> (16 * (i & 1)));
     }
 }
+// The same without a branch, for rows whose length is a multiple of what is loaded: where a row has ended the address is that of zeros.
+// EVEN is that multiple's case; the others take the functions above.
+__device__ const uint32_t no_values[8] = {};
+template <bool EVEN, typename T>
+struct Eight;  // eight values as they lie in memory
+template <bool EVEN>
+struct Eight<EVEN, uint16_t> {
+    u32x4 v;
+    __device__ void load(const uint16_t* row, int c, int n) {
+        if constexpr (EVEN) {
+            v = *reinterpret_cast<const u32x4_any*>(c < n ? row + c : reinterpret_cast<const uint16_t*>(no_values));
+        } else {
+            const Operand<1> o = load8(row, c, n);
+            v = *reinterpret_cast<const u32x4*>(&o.part[0]);
+        }
+    }
+    __device__ Operand<1> operand() const {
+        Operand<1> o;
+        o.part[0] = *reinterpret_cast<const bf16x8*>(&v);
+        return o;
+    }
+};
+template <bool EVEN>
+struct Eight<EVEN, float> {
+    f32x4 lo, hi;
+    __device__ void load(const float* row, int c, int n) {
+        if constexpr (EVEN) {
+            const float* p = c < n ? row + c : reinterpret_cast<const float*>(no_values);
+            lo = *reinterpret_cast<const f32x4_any*>(p), hi = *reinterpret_cast<const f32x4_any*>(p + 4);
+        } else {
+            lo = load4(row, c, n), hi = load4(row, c + 4, n);
+        }
+    }
+    __device__ Operand<3> operand() const { return split8<3>(lo, hi); }
+};
+template <bool EVEN, typename T>
+struct Four;
+template <bool EVEN>
+struct Four<EVEN, uint16_t> {
+    u32x2 v;
+    __device__ void load(const uint16_t* row, int c, int n) {
+        if constexpr (EVEN) {
+            v = *reinterpret_cast<const u32x2_any*>(c < n ? row + c : reinterpret_cast<const uint16_t*>(no_values));
+        } else {
+            const f32x4 x = load4(row, c, n);
+            v = u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
+        }
+    }
+    __device__ f32x4 values() const {
+        return f32x4{__uint_as_float(v[0] << 16), __uint_as_float(v[0] & 0xFFFF0000u), __uint_as_float(v[1] << 16), __uint_as_float(v[1] & 0xFFFF0000u)};
+    }
+};
+template <bool EVEN>
+struct Four<EVEN, float> {
+    f32x4 v;
+    __device__ void load(const float* row, int c, int n) {
+        if constexpr (EVEN)
+            v = *reinterpret_cast<const f32x4_any*>(c < n ? row + c : reinterpret_cast<const float*>(no_values));
+        else
+            v = load4(row, c, n);
+    }
+    __device__ f32x4 values() const { return v; }
+};
+template <bool EVEN, typename T>
+__device__ inline void write4(T* row, int c, int n, const f32x4& x) {
+    if constexpr (EVEN) {
+        if (c >= n) return;
+        if constexpr (sizeof(T) == 4)
+            *reinterpret_cast<f32x4_any*>(row + c) = x;
+        else
+            *reinterpret_cast<u32x2_any*>(row + c) = u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
+    } else {
+        store4(row, c, n, x);
+    }
+}
+// What a thread of NT holds of a chunk's rows of q or k on their way to LDS.
+template <bool EVEN, typename T, int DK, int NT>
+struct Tile {
+    static constexpr int PER = DK / 8, COUNT = C * PER / NT;
+    Eight<EVEN, T> e[COUNT];
+    __device__ void load(const T* base, int64_t st, int n, int dk) {
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) {
+            const int at = threadIdx.x + i * NT, r = at / PER, c = at % PER * 8;
+            e[i].load(base + (r < n ? r : 0) * st, c, r < n ? dk : 0);
+        }
+    }
+    template <int P>
+    __device__ void to_lds(uint16_t* m) const {
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) {
+            const int at = threadIdx.x + i * NT, r = at / PER, c = at % PER * 8;
+            const Operand<PARTS<T>> o = e[i].operand();
+#pragma unroll
+            for (int p = 0; p < PARTS<T>; ++p) *reinterpret_cast<bf16x8*>(m + (p * C + r) * P + c) = o.part[p];
+        }
+    }
+};
+// Rows r0 .. r0+15 of a chunk's matrix [64][64] in memory, N parts, k from k0 on.
+template <int N>
+__device__ inline Operand<N> matrix_rows(const uint16_t* m, int r0, int k0, int lane) {
+    return rows_of<N, C, C>(m, r0, k0, lane);
+}
 // A chunk's rows of q or k (n of them are there, the others zeros) as parts in LDS, by NT threads; columns past dk are zeros.
 template <typename T, int DK, int P, int NT>
 __device__ inline void tile_to_lds(const T* base, int64_t st, int n, int dk, uint16_t* m) {
@@ -204,6 +307,7 @@ struct Rule {
     int B, T, Hk, Hv, dk, dv, chunks;
     float scale;
 };
+inline bool even(const Rule& a) { return a.dk % 8 == 0 && a.dv % 8 == 0; }  // rows are whole loads
 // Workgroups of one unit go to one XCD, whose L2 then has the unit's q, k and matrices for all of its blocks. Launch with grid.x = unit_grid.
 inline unsigned unit_grid(int64_t units, int per) { return static_cast<unsigned>((units + 7) / 8 * 8 * per); }
 __device__ inline bool unit_of(int id, int units, int per, int& unit, int& blk) {

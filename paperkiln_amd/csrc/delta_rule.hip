@@ -114,118 +114,154 @@ __global__ __launch_bounds__(64) void chunk_matrices(Rule a) {
 // STATES: for the backward, the states and U go to memory and there is no O.
 __device__ inline int token_tile(int wave, int i) { return (wave >> 1) ? 1 + i : 3 * i; }
 
-template <typename T, int DK, bool STATES>
+// Everything that a chunk needs from memory is asked for a chunk ahead, each as soon as the registers that hold the one before are free.
+template <typename T, int DK>
+constexpr bool TWO_K = PARTS<T> == 1 || DK < 128;  // two of K's tiles in LDS: the next one is written while this one is still read
+
+template <typename T, int DK, bool STATES, bool EVEN>
 __global__ __launch_bounds__(256) void walk(Rule a) {
     constexpr int N = PARTS<T>, KP = DK + 16, KS = DK / 32, KT = DK / 32, PO = N == 1 ? 2 : 3;  // PO: parts of U and A on their way to O
     extern __shared__ uint16_t lds[];
-    uint16_t *kt = lds, *st = kt + N * C * KP, *rt = st + 3 * DK * VP, *dt = rt + 3 * C * VP, *ut = dt + 3 * C * VP;
+    uint16_t *kt = lds, *st = kt + (TWO_K<T, DK> ? 2 : 1) * N * C * KP, *rt = st + 3 * DK * VP, *dt = rt + 3 * C * VP, *ut = dt + 3 * C * VP;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c16 = lane & 15;
     int unit, blk;
     if (!unit_of(blockIdx.x, a.B * a.Hv, (a.dv + VB - 1) / VB, unit, blk)) return;
     const int b = unit / a.Hv, h = unit - b * a.Hv, hk = h / (a.Hv / a.Hk);
     const int vt = 16 * (wave & 1), vc = VB * blk + vt + 4 * g;  // this lane's four columns
+    const int t_of[2] = {16 * token_tile(wave, 0) + c16, 16 * token_tile(wave, 1) + c16};
+    const bool low[2] = {token_tile(wave, 0) < 2, token_tile(wave, 1) < 2};  // rows of T and A with nothing past their first 32 columns
     const T *q = head<const T>(a.q, b, hk), *k = head<const T>(a.k, b, hk), *v = head<const T>(a.v, b, h);
     T* out = STATES ? nullptr : head<T>(a.o, b, h);
-    const int64_t state_at = static_cast<int64_t>(unit) * a.dk * a.dv;
+    const int64_t state_at = static_cast<int64_t>(unit) * a.dk * a.dv, first = static_cast<int64_t>(unit) * a.chunks;
+    const float* betas = a.beta + static_cast<int64_t>(b) * a.T * a.Hv + h;
     f32x4 S[KT];
 #pragma unroll
     for (int i = 0; i < KT; ++i) {
         const int r = 16 * ((wave >> 1) * KT + i) + c16;
         S[i] = a.state_in && r < a.dk ? load4(a.state_in + state_at + static_cast<int64_t>(r) * a.dv, vc, a.dv) : f32x4{0, 0, 0, 0};
     }
+    Tile<EVEN, T, DK, 256> K;
+    Eight<EVEN, T> Q[2][KS];
+    Four<EVEN, T> V[2];
+    Operand<3> inverse[2][2];
+    Operand<PO> attn[2][2];
+    float beta[2], whole;
+    float2 decay[2];
+    const auto load_k = [&](int chunk) { K.load(k + static_cast<int64_t>(chunk) * C * a.k.st, a.k.st, min(C, a.T - chunk * C), a.dk); };
+    const auto load_rows = [&](int chunk) {
+        const int n = min(C, a.T - chunk * C);
+        const float2* d = a.decay + (first + chunk) * C;
+        whole = d[C - 1].x;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const bool in = t_of[i] < n;
+            const int64_t t = static_cast<int64_t>(chunk) * C + (in ? t_of[i] : 0);
+            V[i].load(v + t * a.v.st, vc, in ? a.dv : 0);
+            beta[i] = in ? betas[t * a.Hv] : 0.0f, decay[i] = d[t_of[i]];
+            if (!STATES)
+#pragma unroll
+                for (int kk = 0; kk < KS; ++kk) Q[i][kk].load(q + t * a.q.st, 32 * kk + 8 * g, in ? a.dk : 0);
+        }
+    };
+    const auto load_inverse = [&](int chunk) {
+        const uint16_t* m = a.inverse + (first + chunk) * 3 * (C * C);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            inverse[i][0] = matrix_rows<3>(m, t_of[i] - c16, 0, lane);
+            if (!low[i]) inverse[i][1] = matrix_rows<3>(m, t_of[i] - c16, 32, lane);
+        }
+    };
+    const auto load_attn = [&](int chunk) {
+        const uint16_t* m = a.attn + (first + chunk) * PO * (C * C);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            attn[i][0] = matrix_rows<PO>(m, t_of[i] - c16, 0, lane);
+            if (!low[i]) attn[i][1] = matrix_rows<PO>(m, t_of[i] - c16, 32, lane);
+        }
+    };
+    load_k(0), load_rows(0), load_inverse(0);
+    if (!STATES) load_attn(0);
     for (int chunk = 0; chunk < a.chunks; ++chunk) {
-        const int t0 = chunk * C, n = min(C, a.T - t0);
-        const int64_t place = static_cast<int64_t>(unit) * a.chunks + chunk;
-        const float2* decay = a.decay + place * C;
-        tile_to_lds<T, DK, KP, 256>(k + static_cast<int64_t>(t0) * a.k.st, a.k.st, n, a.dk, kt);
+        const int t0 = chunk * C, n = min(C, a.T - t0), next = min(chunk + 1, a.chunks - 1);
+        const int64_t place = first + chunk;
+        uint16_t* kc = kt + (TWO_K<T, DK> ? (chunk & 1) * N * C * KP : 0);
+        if (!TWO_K<T, DK> && chunk > 0) __syncthreads();
+        K.template to_lds<KP>(kc);
 #pragma unroll
         for (int i = 0; i < KT; ++i) {
             const int r = 16 * ((wave >> 1) * KT + i) + c16;
             put4<3, DK, VP>(st, r, vt + 4 * g, S[i]);
-            if (STATES && r < a.dk) store4(a.states + (place * a.dk + r) * a.dv, vc, a.dv, S[i]);
+            if (STATES && r < a.dk) write4<EVEN>(a.states + (place * a.dk + r) * a.dv, vc, a.dv, S[i]);
         }
         __syncthreads();
+        load_k(next);
         // R = beta (V - gamma K S), and gamma Q S
-        f32x4 O[2] = {};
-        {
-            f32x4 P[2] = {};
-            const T* qr[2];
-            int dq[2];
+        f32x4 O[2] = {}, P[2] = {};
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk) {
+            const Operand<3> s = cols_of<3, DK, VP>(st, 32 * kk, vt, lane);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const int t = 16 * token_tile(wave, i) + c16;
-                qr[i] = q + static_cast<int64_t>(t0 + (t < n ? t : 0)) * a.q.st, dq[i] = t < n ? a.dk : 0;
-            }
-#pragma unroll
-            for (int kk = 0; kk < KS; ++kk) {
-                const Operand<3> s = cols_of<3, DK, VP>(st, 32 * kk, vt, lane);
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    product<2>(s, rows_of<N, C, KP>(kt, 16 * token_tile(wave, i), 32 * kk, lane), P[i]);
-                    if (!STATES) product<PO - 1>(s, load8(qr[i], 32 * kk + 8 * g, dq[i]), O[i]);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int t = 16 * token_tile(wave, i) + c16;
-                const float beta = t < n ? a.beta[(static_cast<int64_t>(b) * a.T + t0 + t) * a.Hv + h] : 0.0f, gamma = decay[t].x;
-                const f32x4 x = load4(v + static_cast<int64_t>(t0 + (t < n ? t : 0)) * a.v.st, vc, t < n ? a.dv : 0);
-                f32x4 R;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) R[r] = t < n ? beta * fmaf(-gamma, P[i][r], x[r]) : 0.0f, O[i][r] *= a.scale * gamma;
-                put4<3, C, VP>(rt, t, vt + 4 * g, R);
+                product<2>(s, rows_of<N, C, KP>(kc, t_of[i] - c16, 32 * kk, lane), P[i]);
+                if (!STATES) product<PO - 1>(s, Q[i][kk].operand(), O[i]);
             }
         }
+        float delta[2];
+        const float end = whole;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const f32x4 x = V[i].values();
+            f32x4 R;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) R[r] = beta[i] * fmaf(-decay[i].x, P[i][r], x[r]), O[i][r] *= a.scale * decay[i].x;
+            put4<3, C, VP>(rt, t_of[i], vt + 4 * g, R);
+            delta[i] = decay[i].y;
+        }
         __syncthreads();
+        load_rows(next);
         // U = T R
         {
-            const uint16_t* inverse = a.inverse + place * 3 * (C * C);
             f32x4 U[2] = {};
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk) {
                 const Operand<3> r = cols_of<3, C, VP>(rt, 32 * kk, vt, lane);
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
-                    if (kk == 0 || token_tile(wave, i) >= 2) product<2>(r, rows_of<3, C, C>(inverse, 16 * token_tile(wave, i), 32 * kk, lane), U[i]);
+                    if (kk == 0 || !low[i]) product<2>(r, inverse[i][kk], U[i]);
             }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const int t = 16 * token_tile(wave, i) + c16;
-                const float delta = decay[t].y;
                 if (STATES)
-                    store4(a.puts + (place * C + t) * a.dv, vc, a.dv, U[i]);
+                    write4<EVEN>(a.puts + (place * C + t_of[i]) * a.dv, vc, a.dv, U[i]);
                 else
-                    put4<PO, C, VP>(ut, t, vt + 4 * g, U[i]);
-                put4<3, C, VP>(dt, t, vt + 4 * g, U[i] * delta);
+                    put4<PO, C, VP>(ut, t_of[i], vt + 4 * g, U[i]);
+                put4<3, C, VP>(dt, t_of[i], vt + 4 * g, U[i] * delta[i]);
             }
         }
         __syncthreads();
-        // O += A U, S = gamma S + K^T (delta U)
+        load_inverse(next);
+        // S = gamma S + K^T (delta U), O += A U
+#pragma unroll
+        for (int i = 0; i < KT; ++i) S[i] *= end;
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            const Operand<3> u = cols_of<3, C, VP>(dt, 32 * kk, vt, lane);
+#pragma unroll
+            for (int i = 0; i < KT; ++i) product<2>(u, cols_of<N, C, KP>(kc, 32 * kk, 16 * ((wave >> 1) * KT + i), lane), S[i]);
+        }
         if (!STATES) {
-            const uint16_t* attn = a.attn + place * PO * (C * C);
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk) {
                 const Operand<PO> u = cols_of<PO, C, VP>(ut, 32 * kk, vt, lane);
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
-                    if (kk == 0 || token_tile(wave, i) >= 2) product<PO - 1>(u, rows_of<PO, C, C>(attn, 16 * token_tile(wave, i), 32 * kk, lane), O[i]);
+                    if (kk == 0 || !low[i]) product<PO - 1>(u, attn[i][kk], O[i]);
             }
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int t = 16 * token_tile(wave, i) + c16;
-                if (t < n) store4(out + static_cast<int64_t>(t0 + t) * a.o.st, vc, a.dv, O[i]);
-            }
+            for (int i = 0; i < 2; ++i)
+                if (t_of[i] < n) write4<EVEN>(out + static_cast<int64_t>(t0 + t_of[i]) * a.o.st, vc, a.dv, O[i]);
+            load_attn(next);
         }
-        const float whole = decay[C - 1].x;
-#pragma unroll
-        for (int i = 0; i < KT; ++i) S[i] *= whole;
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            const Operand<3> u = cols_of<3, C, VP>(dt, 32 * kk, vt, lane);
-#pragma unroll
-            for (int i = 0; i < KT; ++i) product<2>(u, cols_of<N, C, KP>(kt, 32 * kk, 16 * ((wave >> 1) * KT + i), lane), S[i]);
-        }
-        __syncthreads();
     }
     if (!a.state_out) return;
 #pragma unroll
@@ -236,7 +272,7 @@ __global__ __launch_bounds__(256) void walk(Rule a) {
 }
 template <typename T, int DK, bool STATES>
 constexpr size_t walk_lds() {
-    return sizeof(uint16_t) * (PARTS<T> * C * (DK + 16) + 3 * DK * VP + 6 * C * VP + (STATES ? 0 : (PARTS<T> == 1 ? 2 : 3) * C * VP));
+    return sizeof(uint16_t) * ((TWO_K<T, DK> ? 2 : 1) * PARTS<T> * C * (DK + 16) + 3 * DK * VP + 6 * C * VP + (STATES ? 0 : (PARTS<T> == 1 ? 2 : 3) * C * VP));
 }
 
 // ---- token by token ----
@@ -316,17 +352,21 @@ __global__ __launch_bounds__(STEP_NT) void steps(Rule a) {
 // ---- launches ----
 
 constexpr int FEW_TOKENS = 16;
-template <typename T, int DK, bool STATES>
+template <typename T, int DK, bool STATES, bool EVEN>
 int launch_walk(const Rule& a, hipStream_t st) {
     constexpr size_t lds = walk_lds<T, DK, STATES>();
     static_assert(lds <= 160 * 1024, "LDS of a CU");
-    PK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(walk<T, DK, STATES>), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
-    walk<T, DK, STATES><<<unit_grid(static_cast<int64_t>(a.B) * a.Hv, blocks(a.dv)), 256, lds, st>>>(a);
+    PK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(walk<T, DK, STATES, EVEN>), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
+    walk<T, DK, STATES, EVEN><<<unit_grid(static_cast<int64_t>(a.B) * a.Hv, blocks(a.dv)), 256, lds, st>>>(a);
     return launched();
+}
+template <typename T, bool STATES, bool EVEN>
+int launch_walk(const Rule& a, hipStream_t st) {
+    return a.dk <= 32 ? launch_walk<T, 32, STATES, EVEN>(a, st) : a.dk <= 64 ? launch_walk<T, 64, STATES, EVEN>(a, st) : launch_walk<T, 128, STATES, EVEN>(a, st);
 }
 template <typename T, bool STATES>
 int launch_walk(const Rule& a, hipStream_t st) {
-    return a.dk <= 32 ? launch_walk<T, 32, STATES>(a, st) : a.dk <= 64 ? launch_walk<T, 64, STATES>(a, st) : launch_walk<T, 128, STATES>(a, st);
+    return even(a) ? launch_walk<T, STATES, true>(a, st) : launch_walk<T, STATES, false>(a, st);
 }
 template <typename T, int DK>
 void launch_matrices(const Rule& a, bool backward, hipStream_t st) {
