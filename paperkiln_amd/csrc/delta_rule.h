@@ -164,6 +164,11 @@ __device__ inline void store4(uint16_t* row, int c, int n, const f32x4& x) {
             if (c + i < n) row[c + i] = static_cast<uint16_t>(v[i >> 1] >> (16 * (i & 1)));
     }
 }
+// The address space is named where an address is one of two: of any space the load would also count as one of LDS, and no load could be left on its way.
+template <typename V>
+__device__ inline V from_memory(const void* p) {
+    return *(const __attribute__((address_space(1))) V*)(p);
+}
 // The same without a branch, for rows whose length is a multiple of what is loaded: where a row has ended the address is that of zeros.
 // EVEN is that multiple's case; the others take the functions above.
 __device__ const uint32_t no_values[8] = {};
@@ -174,7 +179,7 @@ struct Eight<EVEN, uint16_t> {
     u32x4 v;
     __device__ void load(const uint16_t* row, int c, int n) {
         if constexpr (EVEN) {
-            v = *reinterpret_cast<const u32x4_any*>(c < n ? row + c : reinterpret_cast<const uint16_t*>(no_values));
+            v = from_memory<u32x4_any>(c < n ? row + c : reinterpret_cast<const uint16_t*>(no_values));
         } else {
             const Operand<1> o = load8(row, c, n);
             v = *reinterpret_cast<const u32x4*>(&o.part[0]);
@@ -192,7 +197,7 @@ struct Eight<EVEN, float> {
     __device__ void load(const float* row, int c, int n) {
         if constexpr (EVEN) {
             const float* p = c < n ? row + c : reinterpret_cast<const float*>(no_values);
-            lo = *reinterpret_cast<const f32x4_any*>(p), hi = *reinterpret_cast<const f32x4_any*>(p + 4);
+            lo = from_memory<f32x4_any>(p), hi = from_memory<f32x4_any>(p + 4);
         } else {
             lo = load4(row, c, n), hi = load4(row, c + 4, n);
         }
@@ -206,7 +211,7 @@ struct Four<EVEN, uint16_t> {
     u32x2 v;
     __device__ void load(const uint16_t* row, int c, int n) {
         if constexpr (EVEN) {
-            v = *reinterpret_cast<const u32x2_any*>(c < n ? row + c : reinterpret_cast<const uint16_t*>(no_values));
+            v = from_memory<u32x2_any>(c < n ? row + c : reinterpret_cast<const uint16_t*>(no_values));
         } else {
             const f32x4 x = load4(row, c, n);
             v = u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
@@ -221,7 +226,7 @@ struct Four<EVEN, float> {
     f32x4 v;
     __device__ void load(const float* row, int c, int n) {
         if constexpr (EVEN)
-            v = *reinterpret_cast<const f32x4_any*>(c < n ? row + c : reinterpret_cast<const float*>(no_values));
+            v = from_memory<f32x4_any>(c < n ? row + c : reinterpret_cast<const float*>(no_values));
         else
             v = load4(row, c, n);
     }

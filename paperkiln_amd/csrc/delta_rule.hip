@@ -157,7 +157,7 @@ __global__ __launch_bounds__(256) void walk(Rule a) {
             const bool in = t_of[i] < n;
             const int64_t t = static_cast<int64_t>(chunk) * C + (in ? t_of[i] : 0);
             V[i].load(v + t * a.v.st, vc, in ? a.dv : 0);
-            beta[i] = in ? betas[t * a.Hv] : 0.0f, decay[i] = d[t_of[i]];
+            beta[i] = betas[t * a.Hv], decay[i] = d[t_of[i]];
             if (!STATES)
 #pragma unroll
                 for (int kk = 0; kk < KS; ++kk) Q[i][kk].load(q + t * a.q.st, 32 * kk + 8 * g, in ? a.dk : 0);
@@ -213,7 +213,7 @@ __global__ __launch_bounds__(256) void walk(Rule a) {
             const f32x4 x = V[i].values();
             f32x4 R;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) R[r] = beta[i] * fmaf(-decay[i].x, P[i][r], x[r]), O[i][r] *= a.scale * decay[i].x;
+            for (int r = 0; r < 4; ++r) R[r] = t_of[i] < n ? beta[i] * fmaf(-decay[i].x, P[i][r], x[r]) : 0.0f, O[i][r] *= a.scale * decay[i].x;
             put4<3, C, VP>(rt, t_of[i], vt + 4 * g, R);
             delta[i] = decay[i].y;
         }
