@@ -9,8 +9,9 @@
 // product in 32 bits has; the matrix cores take 16 such products in the time of one in fp32. Tensors of bf16 are one part, tensors of fp32 three.
 //
 // v_mfma_f32_16x16x32_bf16, lane l = 16 g + c: A row c, k = 8g .. 8g+7; B column c, k = 8g .. 8g+7; C column c, rows 4g .. 4g+3.
-// Products are formed transposed (rows: columns of the state or of v; columns: tokens or k's columns), so that a lane's four results are
-// neighbours in a row of memory.
+// A and B are alike, so a product is formed in the orientation that its result is wanted in: a lane's four values are neighbours there, in a row of memory or in what LDS keeps
+// for the next product, whose operands are read along k in pieces of 16 bytes. The states in LDS are [columns][rows], R, U and their like [columns][tokens]; only K^T and Q^T are read
+// by transposing reads.
 #pragma once
 #include <algorithm>
 
@@ -20,11 +21,12 @@ namespace pk {
 namespace delta {
 
 constexpr int C = 64;       // tokens of a chunk
-constexpr int VB = 32;      // columns of the state that a workgroup of a scan has
-constexpr int VP = VB + 4;  // their pitch in LDS: 18 banks, so neither the stores of 8 bytes down 16 rows nor transposing reads of 4 rows meet a bank twice
+// Columns of the state that a workgroup of a walk has are 16 or 32 (VB). Rows in LDS are 8 values past a multiple of 32, so that reads of 16 bytes down 16 rows meet every bank once.
+constexpr int CP = C + 8;
+constexpr int GB = 32;  // columns that go by at a time in the backward's last launch
 
 inline int chunks(int T) { return (T + C - 1) / C; }
-inline int blocks(int dv) { return (dv + VB - 1) / VB; }
+inline int blocks(int dv, int vb) { return (dv + vb - 1) / vb; }
 
 typedef f32x4 f32x4_any __attribute__((aligned(4)));
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
@@ -73,6 +75,23 @@ __device__ inline void product(const Operand<NA>& a, const Operand<NB>& b, f32x4
 #pragma unroll
         for (int i = 0; i < NA; ++i)
             if (s - i >= 0 && s - i < NB) c = mfma16(a.part[i], b.part[s - i], c);
+}
+
+// The same into an accumulator for each place, so that no product waits for the one before it; their sum at the end.
+template <int MOST, int NA, int NB>
+__device__ inline void spread(const Operand<NA>& a, const Operand<NB>& b, f32x4 (&c)[MOST + 1]) {
+#pragma unroll
+    for (int s = MOST; s >= 0; --s)
+#pragma unroll
+        for (int i = 0; i < NA; ++i)
+            if (s - i >= 0 && s - i < NB) c[s] = mfma16(a.part[i], b.part[s - i], c[s]);
+}
+template <int N>
+__device__ inline f32x4 gather(const f32x4 (&c)[N]) {
+    f32x4 x = c[N - 1];
+#pragma unroll
+    for (int i = N - 2; i >= 0; --i) x += c[i];
+    return x;
 }
 
 // ---- operands from LDS: N parts of a matrix of R rows, one behind the other ----
@@ -247,13 +266,14 @@ __device__ inline void write4(T* row, int c, int n, const f32x4& x) {
 // What a thread of NT holds of a chunk's rows of q or k on their way to LDS.
 template <bool EVEN, typename T, int DK, int NT>
 struct Tile {
-    static constexpr int PER = DK / 8, COUNT = C * PER / NT;
+    static constexpr int PER = DK / 8, COUNT = (C * PER + NT - 1) / NT;
+    static constexpr bool WHOLE = C * PER % NT == 0;
     Eight<EVEN, T> e[COUNT];
     __device__ void load(const T* base, int64_t st, int n, int dk) {
 #pragma unroll
         for (int i = 0; i < COUNT; ++i) {
             const int at = threadIdx.x + i * NT, r = at / PER, c = at % PER * 8;
-            e[i].load(base + (r < n ? r : 0) * st, c, r < n ? dk : 0);
+            if (WHOLE || r < C) e[i].load(base + (r < n ? r : 0) * st, c, r < n ? dk : 0);
         }
     }
     template <int P>
@@ -261,10 +281,26 @@ struct Tile {
 #pragma unroll
         for (int i = 0; i < COUNT; ++i) {
             const int at = threadIdx.x + i * NT, r = at / PER, c = at % PER * 8;
+            if (!WHOLE && r >= C) continue;
             const Operand<PARTS<T>> o = e[i].operand();
 #pragma unroll
             for (int p = 0; p < PARTS<T>; ++p) *reinterpret_cast<bf16x8*>(m + (p * C + r) * P + c) = o.part[p];
         }
+    }
+};
+// Four tokens' values of one column, as they lie in memory. Tokens behind the last one have its values, columns behind the last one the first one's: they are multiplied by zero or not stored.
+template <typename T>
+struct Tokens {
+    T v[4];
+    __device__ void load(const T* base, int64_t st, int t, int n, int c, int cols) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = from_memory<T>(base + min(t + r, n - 1) * st + (c < cols ? c : 0));
+    }
+    __device__ f32x4 values() const {
+        if constexpr (sizeof(T) == 4)
+            return f32x4{v[0], v[1], v[2], v[3]};
+        else
+            return f32x4{elem(v, 0), elem(v, 1), elem(v, 2), elem(v, 3)};
     }
 };
 // Rows r0 .. r0+15 of a chunk's matrix [64][64] in memory, N parts, k from k0 on.
@@ -300,7 +336,7 @@ struct Rule {
     float* state_out;               // or null
     // for every unit (batch, head of v) and chunk:
     uint16_t *inverse, *attn;       // parts of T and A, [64][64] each
-    float2* decay;                  // gamma and delta of its tokens
+    float* scalars;                 // gamma, delta and beta of its tokens, 64 each
     float *states, *puts;           // backward: the state that the chunk begins with, [dk][dv]; U, [64][dv]
     // backward
     View dout, dq, dk_, dv_;

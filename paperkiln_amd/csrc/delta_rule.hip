@@ -6,6 +6,7 @@
 // head's state: the columns do not know of one another. What bounds the walk is its own chain: three products and three exchanges through LDS a chunk.
 // Token by token, the state in registers, memory bounds it: the state read and written once.
 #include "delta_rule.h"
+#include <cstdlib>
 
 namespace pk {
 namespace delta {
@@ -37,8 +38,9 @@ __global__ __launch_bounds__(64) void chunk_matrices(Rule a) {
     }
     total[lane] = sum;
     const int64_t place = unit * a.chunks + chunk;
-    a.decay[place * C + lane] = make_float2(decay_of(sum), decay_of(__shfl(sum, 63) - sum));
     const float beta = lane < n ? a.beta[at + static_cast<int64_t>(lane) * a.Hv] : 0.0f;
+    float* scalars = a.scalars + place * 3 * C;
+    scalars[lane] = decay_of(sum), scalars[C + lane] = decay_of(__shfl(sum, 63) - sum), scalars[2 * C + lane] = beta;
     __syncthreads();
     const int hk = h / (a.Hv / a.Hk);
     const T *q = head<const T>(a.q, b, hk) + static_cast<int64_t>(t0) * a.q.st, *k = head<const T>(a.k, b, hk) + static_cast<int64_t>(t0) * a.k.st;
@@ -110,74 +112,71 @@ __global__ __launch_bounds__(64) void chunk_matrices(Rule a) {
 }
 
 // ---- the walk down the chunks ----
-// Four wavefronts: wavefront w has 16 of the 32 columns and two of the four tiles of 16 tokens (0 and 3, or 1 and 2: T and A are lower triangles), of the state half of its rows.
-// STATES: for the backward, the states and U go to memory and there is no O.
-__device__ inline int token_tile(int wave, int i) { return (wave >> 1) ? 1 + i : 3 * i; }
-
+// Four wavefronts for each 16 columns: one has 16 of a chunk's tokens, and of the state a quarter of its rows.
 // Everything that a chunk needs from memory is asked for a chunk ahead, each as soon as the registers that hold the one before are free.
+// STATES: for the backward, the states and U go to memory and there is no O.
 template <typename T, int DK>
 constexpr bool TWO_K = PARTS<T> == 1 || DK < 128;  // two of K's tiles in LDS: the next one is written while this one is still read
 
-template <typename T, int DK, bool STATES, bool EVEN>
-__global__ __launch_bounds__(256) void walk(Rule a) {
-    constexpr int N = PARTS<T>, KP = DK + 16, KS = DK / 32, KT = DK / 32, PO = N == 1 ? 2 : 3;  // PO: parts of U and A on their way to O
+template <typename T, int DK, int VB, bool STATES, bool EVEN>
+__global__ __launch_bounds__(16 * VB) void walk(Rule a) {
+    constexpr int N = PARTS<T>, KP = DK + 16, SP = DK + 8, KS = DK / 32, KT = (DK + 63) / 64, PO = N == 1 ? 2 : 3;  // PO: parts of U and A on their way to O
     extern __shared__ uint16_t lds[];
-    uint16_t *kt = lds, *st = kt + (TWO_K<T, DK> ? 2 : 1) * N * C * KP, *rt = st + 3 * DK * VP, *dt = rt + 3 * C * VP, *ut = dt + 3 * C * VP;
+    uint16_t *kt = lds, *st = kt + (TWO_K<T, DK> ? 2 : 1) * N * C * KP, *rt = st + 3 * VB * SP, *dt = rt + 3 * VB * CP, *ut = dt + 3 * VB * CP;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c16 = lane & 15;
     int unit, blk;
     if (!unit_of(blockIdx.x, a.B * a.Hv, (a.dv + VB - 1) / VB, unit, blk)) return;
     const int b = unit / a.Hv, h = unit - b * a.Hv, hk = h / (a.Hv / a.Hk);
-    const int vt = 16 * (wave & 1), vc = VB * blk + vt + 4 * g;  // this lane's four columns
-    const int t_of[2] = {16 * token_tile(wave, 0) + c16, 16 * token_tile(wave, 1) + c16};
-    const bool low[2] = {token_tile(wave, 0) < 2, token_tile(wave, 1) < 2};  // rows of T and A with nothing past their first 32 columns
+    const int tile = wave >> (VB / 32), vt = VB == 32 ? 16 * (wave & 1) : 0;
+    const int column = vt + c16, vc = VB * blk + column, tokens = 16 * tile + 4 * g;  // the state's column and the four tokens of this lane,
+    const int token = 16 * tile + c16, vo = VB * blk + vt + 4 * g;                     // of O the token and the four columns
+    const bool low = tile < 2;                         // rows of T and A with nothing past their first 32 columns
+    const bool rows_here = DK > 32 || tile < DK / 16;  // a state of 32 rows is two tiles
     const T *q = head<const T>(a.q, b, hk), *k = head<const T>(a.k, b, hk), *v = head<const T>(a.v, b, h);
     T* out = STATES ? nullptr : head<T>(a.o, b, h);
-    const int64_t state_at = static_cast<int64_t>(unit) * a.dk * a.dv, first = static_cast<int64_t>(unit) * a.chunks;
-    const float* betas = a.beta + static_cast<int64_t>(b) * a.T * a.Hv + h;
-    f32x4 S[KT];
+    const int64_t state_at = static_cast<int64_t>(unit) * a.dk * a.dv + vc, first = static_cast<int64_t>(unit) * a.chunks;
+    const auto row_of = [&](int i) { return 16 * (tile * KT + i) + 4 * g; };
+    // this lane's part of a state in memory
+    const auto each_row = [&](auto&& f) {
+        if (!rows_here || vc >= a.dv) return;
 #pragma unroll
-    for (int i = 0; i < KT; ++i) {
-        const int r = 16 * ((wave >> 1) * KT + i) + c16;
-        S[i] = a.state_in && r < a.dk ? load4(a.state_in + state_at + static_cast<int64_t>(r) * a.dv, vc, a.dv) : f32x4{0, 0, 0, 0};
-    }
-    Tile<EVEN, T, DK, 256> K;
-    Eight<EVEN, T> Q[2][KS];
-    Four<EVEN, T> V[2];
-    Operand<3> inverse[2][2];
-    Operand<PO> attn[2][2];
-    float beta[2], whole;
-    float2 decay[2];
+        for (int i = 0; i < KT; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (row_of(i) + r < a.dk) f(i, r, static_cast<int64_t>(row_of(i) + r) * a.dv);
+    };
+    f32x4 S[KT] = {};
+    if (a.state_in) each_row([&](int i, int r, int64_t at) { S[i][r] = a.state_in[state_at + at]; });
+    Tile<EVEN, T, DK, 16 * VB> K;
+    Eight<EVEN, T> Q[KS];
+    Tokens<T> V;
+    Operand<3> inverse[2];
+    Operand<PO> attn[2];
+    f32x4 gamma, delta, beta;
+    float whole, gamma_o;
     const auto load_k = [&](int chunk) { K.load(k + static_cast<int64_t>(chunk) * C * a.k.st, a.k.st, min(C, a.T - chunk * C), a.dk); };
     const auto load_rows = [&](int chunk) {
         const int n = min(C, a.T - chunk * C);
-        const float2* d = a.decay + (first + chunk) * C;
-        whole = d[C - 1].x;
+        const float* d = a.scalars + (first + chunk) * 3 * C;
+        gamma = *reinterpret_cast<const f32x4*>(d + tokens), delta = *reinterpret_cast<const f32x4*>(d + C + tokens), beta = *reinterpret_cast<const f32x4*>(d + 2 * C + tokens);
+        whole = d[C - 1];
+        V.load(v + static_cast<int64_t>(chunk) * C * a.v.st, a.v.st, tokens, n, vc, a.dv);
+        if (!STATES) {
+            gamma_o = d[token];
+            const T* row = q + (static_cast<int64_t>(chunk) * C + min(token, n - 1)) * a.q.st;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const bool in = t_of[i] < n;
-            const int64_t t = static_cast<int64_t>(chunk) * C + (in ? t_of[i] : 0);
-            V[i].load(v + t * a.v.st, vc, in ? a.dv : 0);
-            beta[i] = betas[t * a.Hv], decay[i] = d[t_of[i]];
-            if (!STATES)
-#pragma unroll
-                for (int kk = 0; kk < KS; ++kk) Q[i][kk].load(q + t * a.q.st, 32 * kk + 8 * g, in ? a.dk : 0);
+            for (int kk = 0; kk < KS; ++kk) Q[kk].load(row, 32 * kk + 8 * g, a.dk);
         }
     };
     const auto load_inverse = [&](int chunk) {
         const uint16_t* m = a.inverse + (first + chunk) * 3 * (C * C);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            inverse[i][0] = matrix_rows<3>(m, t_of[i] - c16, 0, lane);
-            if (!low[i]) inverse[i][1] = matrix_rows<3>(m, t_of[i] - c16, 32, lane);
-        }
+        inverse[0] = matrix_rows<3>(m, 16 * tile, 0, lane);
+        if (!low) inverse[1] = matrix_rows<3>(m, 16 * tile, 32, lane);
     };
     const auto load_attn = [&](int chunk) {
         const uint16_t* m = a.attn + (first + chunk) * PO * (C * C);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            attn[i][0] = matrix_rows<PO>(m, t_of[i] - c16, 0, lane);
-            if (!low[i]) attn[i][1] = matrix_rows<PO>(m, t_of[i] - c16, 32, lane);
-        }
+        attn[0] = matrix_rows<PO>(m, 16 * tile, 0, lane);
+        if (!low) attn[1] = matrix_rows<PO>(m, 16 * tile, 32, lane);
     };
     load_k(0), load_rows(0), load_inverse(0);
     if (!STATES) load_attn(0);
@@ -187,92 +186,79 @@ __global__ __launch_bounds__(256) void walk(Rule a) {
         uint16_t* kc = kt + (TWO_K<T, DK> ? (chunk & 1) * N * C * KP : 0);
         if (!TWO_K<T, DK> && chunk > 0) __syncthreads();
         K.template to_lds<KP>(kc);
+        if (rows_here) {
 #pragma unroll
-        for (int i = 0; i < KT; ++i) {
-            const int r = 16 * ((wave >> 1) * KT + i) + c16;
-            put4<3, DK, VP>(st, r, vt + 4 * g, S[i]);
-            if (STATES && r < a.dk) write4<EVEN>(a.states + (place * a.dk + r) * a.dv, vc, a.dv, S[i]);
+            for (int i = 0; i < KT; ++i) put4<3, VB, SP>(st, column, row_of(i), S[i]);
+        }
+        if (STATES) {
+            float* to = a.states + place * a.dk * a.dv + vc;
+            each_row([&](int i, int r, int64_t at) { to[at] = S[i][r]; });
         }
         __syncthreads();
         load_k(next);
         // R = beta (V - gamma K S), and gamma Q S
-        f32x4 O[2] = {}, P[2] = {};
+        f32x4 O = {0, 0, 0, 0};
+        {
+            f32x4 P[3] = {}, QS[PO] = {};
 #pragma unroll
-        for (int kk = 0; kk < KS; ++kk) {
-            const Operand<3> s = cols_of<3, DK, VP>(st, 32 * kk, vt, lane);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                product<2>(s, rows_of<N, C, KP>(kc, t_of[i] - c16, 32 * kk, lane), P[i]);
-                if (!STATES) product<PO - 1>(s, Q[i][kk].operand(), O[i]);
+            for (int kk = 0; kk < KS; ++kk) {
+                const Operand<3> s = rows_of<3, VB, SP>(st, vt, 32 * kk, lane);
+                spread<2>(rows_of<N, C, KP>(kc, 16 * tile, 32 * kk, lane), s, P);
+                if (!STATES) spread<PO - 1>(s, Q[kk].operand(), QS);
             }
-        }
-        float delta[2];
-        const float end = whole;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const f32x4 x = V[i].values();
+            const f32x4 x = V.values(), p = gather(P);
             f32x4 R;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) R[r] = t_of[i] < n ? beta[i] * fmaf(-decay[i].x, P[i][r], x[r]) : 0.0f, O[i][r] *= a.scale * decay[i].x;
-            put4<3, C, VP>(rt, t_of[i], vt + 4 * g, R);
-            delta[i] = decay[i].y;
+            for (int r = 0; r < 4; ++r) R[r] = beta[r] * fmaf(-gamma[r], p[r], x[r]);
+            put4<3, VB, CP>(rt, column, tokens, R);
+            if (!STATES) O = gather(QS) * (a.scale * gamma_o);
         }
+        const f32x4 leave = delta;
+        const float end = whole;
         __syncthreads();
         load_rows(next);
         // U = T R
         {
-            f32x4 U[2] = {};
+            f32x4 sums[3] = {};
+            spread<2>(inverse[0], rows_of<3, VB, CP>(rt, vt, 0, lane), sums);
+            if (!low) spread<2>(inverse[1], rows_of<3, VB, CP>(rt, vt, 32, lane), sums);
+            const f32x4 U = gather(sums);
+            if (STATES) {
+                if (vc < a.dv)
 #pragma unroll
-            for (int kk = 0; kk < 2; ++kk) {
-                const Operand<3> r = cols_of<3, C, VP>(rt, 32 * kk, vt, lane);
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    if (kk == 0 || !low[i]) product<2>(r, inverse[i][kk], U[i]);
+                    for (int r = 0; r < 4; ++r) a.puts[(place * C + tokens + r) * a.dv + vc] = U[r];
+            } else {
+                put4<PO, VB, CP>(ut, column, tokens, U);
             }
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                if (STATES)
-                    write4<EVEN>(a.puts + (place * C + t_of[i]) * a.dv, vc, a.dv, U[i]);
-                else
-                    put4<PO, C, VP>(ut, t_of[i], vt + 4 * g, U[i]);
-                put4<3, C, VP>(dt, t_of[i], vt + 4 * g, U[i] * delta[i]);
-            }
+            put4<3, VB, CP>(dt, column, tokens, U * leave);
         }
         __syncthreads();
         load_inverse(next);
         // S = gamma S + K^T (delta U), O += A U
-#pragma unroll
-        for (int i = 0; i < KT; ++i) S[i] *= end;
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            const Operand<3> u = cols_of<3, C, VP>(dt, 32 * kk, vt, lane);
-#pragma unroll
-            for (int i = 0; i < KT; ++i) product<2>(u, cols_of<N, C, KP>(kc, 32 * kk, 16 * ((wave >> 1) * KT + i), lane), S[i]);
-        }
-        if (!STATES) {
+        if (rows_here) {
+            f32x4 sums[KT][3] = {};
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk) {
-                const Operand<PO> u = cols_of<PO, C, VP>(ut, 32 * kk, vt, lane);
+                const Operand<3> u = rows_of<3, VB, CP>(dt, vt, 32 * kk, lane);
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    if (kk == 0 || !low[i]) product<PO - 1>(u, attn[i][kk], O[i]);
+                for (int i = 0; i < KT; ++i) spread<2>(cols_of<N, C, KP>(kc, 32 * kk, 16 * (tile * KT + i), lane), u, sums[i]);
             }
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-                if (t_of[i] < n) write4<EVEN>(out + static_cast<int64_t>(t0 + t_of[i]) * a.o.st, vc, a.dv, O[i]);
+            for (int i = 0; i < KT; ++i) S[i] = S[i] * end + gather(sums[i]);
+        }
+        if (!STATES) {
+            f32x4 sums[PO] = {};
+            spread<PO - 1>(rows_of<PO, VB, CP>(ut, vt, 0, lane), attn[0], sums);
+            if (!low) spread<PO - 1>(rows_of<PO, VB, CP>(ut, vt, 32, lane), attn[1], sums);
+            if (token < n) write4<EVEN>(out + static_cast<int64_t>(t0 + token) * a.o.st, vo, a.dv, O + gather(sums));
             load_attn(next);
         }
     }
-    if (!a.state_out) return;
-#pragma unroll
-    for (int i = 0; i < KT; ++i) {
-        const int r = 16 * ((wave >> 1) * KT + i) + c16;
-        if (r < a.dk) store4(a.state_out + state_at + static_cast<int64_t>(r) * a.dv, vc, a.dv, S[i]);
-    }
+    if (a.state_out) each_row([&](int i, int r, int64_t at) { a.state_out[state_at + at] = S[i][r]; });
 }
-template <typename T, int DK, bool STATES>
+template <typename T, int DK, int VB, bool STATES>
 constexpr size_t walk_lds() {
-    return sizeof(uint16_t) * ((TWO_K<T, DK> ? 2 : 1) * PARTS<T> * C * (DK + 16) + 3 * DK * VP + 6 * C * VP + (STATES ? 0 : (PARTS<T> == 1 ? 2 : 3) * C * VP));
+    return sizeof(uint16_t) * ((TWO_K<T, DK> ? 2 : 1) * PARTS<T> * C * (DK + 16) + 3 * VB * (DK + 8) + 6 * VB * CP + (STATES ? 0 : (PARTS<T> == 1 ? 2 : 3) * VB * CP));
 }
 
 // ---- token by token ----
@@ -352,13 +338,17 @@ __global__ __launch_bounds__(STEP_NT) void steps(Rule a) {
 // ---- launches ----
 
 constexpr int FEW_TOKENS = 16;
+template <typename T, int DK, int VB, bool STATES, bool EVEN>
+int launch_walk(const Rule& a, hipStream_t st) {
+    constexpr size_t lds = walk_lds<T, DK, VB, STATES>();
+    static_assert(lds <= 160 * 1024, "LDS of a CU");
+    PK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(walk<T, DK, VB, STATES, EVEN>), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
+    walk<T, DK, VB, STATES, EVEN><<<unit_grid(static_cast<int64_t>(a.B) * a.Hv, blocks(a.dv, VB)), 16 * VB, lds, st>>>(a);
+    return launched();
+}
 template <typename T, int DK, bool STATES, bool EVEN>
 int launch_walk(const Rule& a, hipStream_t st) {
-    constexpr size_t lds = walk_lds<T, DK, STATES>();
-    static_assert(lds <= 160 * 1024, "LDS of a CU");
-    PK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(walk<T, DK, STATES, EVEN>), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
-    walk<T, DK, STATES, EVEN><<<unit_grid(static_cast<int64_t>(a.B) * a.Hv, blocks(a.dv)), 256, lds, st>>>(a);
-    return launched();
+    return getenv("PK_VB32") ? launch_walk<T, DK, 32, STATES, EVEN>(a, st) : launch_walk<T, DK, 16, STATES, EVEN>(a, st);
 }
 template <typename T, bool STATES, bool EVEN>
 int launch_walk(const Rule& a, hipStream_t st) {
@@ -387,13 +377,13 @@ void launch_steps(const Rule& a, hipStream_t st) {
 }
 
 struct Room {
-    size_t inverse, attn, decay, all;
+    size_t inverse, attn, scalars, all;
 };
 Room room_of(const pk_delta_shape* s) {
     const size_t places = static_cast<size_t>(s->B) * s->Hv * chunks(s->T);
     Room r;
-    r.inverse = pad(places * 3 * MATRIX), r.attn = pad(places * (s->dtype == PK_F32 ? 3 : 2) * MATRIX), r.decay = pad(places * C * sizeof(float2));
-    r.all = r.inverse + r.attn + r.decay;
+    r.inverse = pad(places * 3 * MATRIX), r.attn = pad(places * (s->dtype == PK_F32 ? 3 : 2) * MATRIX), r.scalars = pad(places * 3 * C * sizeof(float));
+    r.all = r.inverse + r.attn + r.scalars;
     return r;
 }
 
@@ -458,7 +448,7 @@ int pk_delta_rule_fwd(const pk_delta_shape* s, const pk_tensor4* q, const pk_ten
         }
         const Room r = room_of(s);
         char* ws = static_cast<char*>(workspace);
-        a.inverse = reinterpret_cast<uint16_t*>(ws), a.attn = reinterpret_cast<uint16_t*>(ws + r.inverse), a.decay = reinterpret_cast<float2*>(ws + r.inverse + r.attn);
+        a.inverse = reinterpret_cast<uint16_t*>(ws), a.attn = reinterpret_cast<uint16_t*>(ws + r.inverse), a.scalars = reinterpret_cast<float*>(ws + r.inverse + r.attn);
         if (int rc = launch_chunks(a, s->dtype, false, st)) return rc;
         return s->dtype == PK_BF16 ? launch_walk<uint16_t, false>(a, st) : launch_walk<float, false>(a, st);
     });

@@ -22,130 +22,135 @@ __device__ inline float decay_of(double x) { return __builtin_amdgcn_exp2f(stati
 constexpr float LEAST = -1000.0f;  // a log-decay below it is held to it, and has no derivative
 
 // ---- the walk back ----
-__device__ inline int token_tile(int wave, int i) { return (wave >> 1) ? 1 + i : 3 * i; }
-
-template <typename T, int DK>
+// As the forward's: four wavefronts for each 16 columns, loads a chunk ahead.
+template <int DK>
+constexpr bool TWO_K = DK < 128;  // a second tile of K in LDS would leave room for one workgroup on a CU in place of two
+template <typename T, int DK, int VB>
 constexpr size_t back_lds() {
-    return sizeof(uint16_t) * ((PARTS<T> == 1 ? 2 : 3) * C * (DK + 16) + 3 * DK * VP + 9 * C * VP + PARTS<T> * C * VP);
+    return sizeof(uint16_t) * ((TWO_K<DK> ? 3 : 2) * PARTS<T> * C * (DK + 16) + 3 * VB * (DK + 8) + (9 + PARTS<T>) * VB * CP);
 }
-template <typename T, int DK>
-__global__ __launch_bounds__(256) void walk_back(Rule a) {
-    constexpr int N = PARTS<T>, KP = DK + 16, KS = DK / 32, KT = DK / 32;
-    constexpr bool BOTH = N == 1;  // K and Q side by side in LDS; three parts of each take turns
+template <typename T, int DK, int VB, bool EVEN>
+__global__ __launch_bounds__(16 * VB) void walk_back(Rule a) {
+    constexpr int N = PARTS<T>, KP = DK + 16, SP = DK + 8, KS = DK / 32, KT = (DK + 63) / 64;
     extern __shared__ uint16_t lds[];
-    uint16_t *kt = lds, *qt = BOTH ? kt + C * KP : kt, *st = kt + (BOTH ? 2 : 3) * C * KP, *ut = st + 3 * DK * VP, *wt = ut + 3 * C * VP, *dt = wt + 3 * C * VP, *rt = dt + 3 * C * VP;
+    uint16_t *kt = lds, *qt = kt + (TWO_K<DK> ? 2 : 1) * N * C * KP, *st = qt + N * C * KP, *ut = st + 3 * VB * SP, *wt = ut + 3 * VB * CP, *dt = wt + 3 * VB * CP, *rt = dt + 3 * VB * CP;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c16 = lane & 15;
     int unit, blk;
     if (!unit_of(blockIdx.x, a.B * a.Hv, (a.dv + VB - 1) / VB, unit, blk)) return;
     const int b = unit / a.Hv, h = unit - b * a.Hv, hk = h / (a.Hv / a.Hk);
-    const int vt = 16 * (wave & 1), vc = VB * blk + vt + 4 * g;
+    const int tile = wave >> (VB / 32), vt = VB == 32 ? 16 * (wave & 1) : 0;
+    const int column = vt + c16, vc = VB * blk + column, tokens = 16 * tile + 4 * g;
+    const bool high = tile >= 2;  // rows of the transposed matrices with nothing in their first 32 columns
+    const bool rows_here = DK > 32 || tile < DK / 16, in = vc < a.dv;
     const T *q = head<const T>(a.q, b, hk), *k = head<const T>(a.k, b, hk), *dout = head<const T>(a.dout, b, h);
-    T* dv = head<T>(a.dv_, b, h);
-    const int64_t state_at = static_cast<int64_t>(unit) * a.dk * a.dv;
-    f32x4 S[KT];  // of the gradient of the state
+    T* dv = head<T>(a.dv_, b, h) + vc;
+    const int64_t state_at = static_cast<int64_t>(unit) * a.dk * a.dv + vc, first = static_cast<int64_t>(unit) * a.chunks;
+    const auto row_of = [&](int i) { return 16 * (tile * KT + i) + 4 * g; };
+    const auto each_row = [&](auto&& f) {
+        if (!rows_here || !in) return;
 #pragma unroll
-    for (int i = 0; i < KT; ++i) {
-        const int r = 16 * ((wave >> 1) * KT + i) + c16;
-        S[i] = a.dstate_out && r < a.dk ? load4(a.dstate_out + state_at + static_cast<int64_t>(r) * a.dv, vc, a.dv) : f32x4{0, 0, 0, 0};
-    }
+        for (int i = 0; i < KT; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (row_of(i) + r < a.dk) f(i, r, static_cast<int64_t>(row_of(i) + r) * a.dv);
+    };
+    f32x4 S[KT] = {};  // of the gradient of the state
+    if (a.dstate_out) each_row([&](int i, int r, int64_t at) { S[i][r] = a.dstate_out[state_at + at]; });
+    Tile<EVEN, T, DK, 16 * VB> K, Q;
+    Tokens<T> D;
+    Operand<3> attn_t[2], inverse_t[2];
+    f32x4 gamma, delta, beta;
+    float whole;
+    const auto load_k = [&](int chunk) { K.load(k + static_cast<int64_t>(chunk) * C * a.k.st, a.k.st, min(C, a.T - chunk * C), a.dk); };
+    const auto load_q = [&](int chunk) { Q.load(q + static_cast<int64_t>(chunk) * C * a.q.st, a.q.st, min(C, a.T - chunk * C), a.dk); };
+    const auto load_rows = [&](int chunk) {
+        const float* d = a.scalars + (first + chunk) * 3 * C;
+        gamma = *reinterpret_cast<const f32x4*>(d + tokens), delta = *reinterpret_cast<const f32x4*>(d + C + tokens), beta = *reinterpret_cast<const f32x4*>(d + 2 * C + tokens);
+        whole = d[C - 1];
+        D.load(dout + static_cast<int64_t>(chunk) * C * a.dout.st, a.dout.st, tokens, min(C, a.T - chunk * C), vc, a.dv);
+    };
+    const auto load_matrix = [&](const uint16_t* all, int chunk, Operand<3>(&o)[2]) {
+        const uint16_t* m = all + (first + chunk) * 3 * (C * C);
+        if (!high) o[0] = matrix_rows<3>(m, 16 * tile, 0, lane);
+        o[1] = matrix_rows<3>(m, 16 * tile, 32, lane);
+    };
+    if (a.chunks > 0) load_k(a.chunks - 1), load_rows(a.chunks - 1), load_matrix(a.attn_t, a.chunks - 1, attn_t), load_q(a.chunks - 1), load_matrix(a.inverse_t, a.chunks - 1, inverse_t);
     for (int chunk = a.chunks - 1; chunk >= 0; --chunk) {
-        const int t0 = chunk * C, n = min(C, a.T - t0);
-        const int64_t place = static_cast<int64_t>(unit) * a.chunks + chunk;
-        const float2* decay = a.decay + place * C;
-        tile_to_lds<T, DK, KP, 256>(k + static_cast<int64_t>(t0) * a.k.st, a.k.st, n, a.dk, kt);
-        if (BOTH) tile_to_lds<T, DK, KP, 256>(q + static_cast<int64_t>(t0) * a.q.st, a.q.st, n, a.dk, qt);
+        const int t0 = chunk * C, n = min(C, a.T - t0), next = max(chunk - 1, 0);
+        const int64_t place = first + chunk;
+        uint16_t* kc = kt + (TWO_K<DK> ? (chunk & 1) * N * C * KP : 0);
+        if (!TWO_K<DK> && chunk < a.chunks - 1) __syncthreads();
+        K.template to_lds<KP>(kc);
+        if (rows_here) {
 #pragma unroll
-        for (int i = 0; i < KT; ++i) {
-            const int r = 16 * ((wave >> 1) * KT + i) + c16;
-            put4<3, DK, VP>(st, r, vt + 4 * g, S[i]);
-            if (r < a.dk) store4(a.dstates + (place * a.dk + r) * a.dv, vc, a.dv, S[i]);
+            for (int i = 0; i < KT; ++i) put4<3, VB, SP>(st, column, row_of(i), S[i]);
         }
+        f32x4 x = D.values();
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int t = 16 * token_tile(wave, i) + c16;
-            const f32x4 x = load4(dout + static_cast<int64_t>(t0 + (t < n ? t : 0)) * a.dout.st, vc, t < n ? a.dv : 0);
-            put4<N, C, VP>(rt, t, vt + 4 * g, x);
-            put4<3, C, VP>(dt, t, vt + 4 * g, x * (a.scale * decay[t].x));
-        }
-        __syncthreads();
-        // dU = A^T dO + delta K dS'
+        for (int r = 0; r < 4; ++r) x[r] = tokens + r < n ? x[r] : 0.0f;
+        put4<N, VB, CP>(rt, column, tokens, x);
         {
-            f32x4 X[2] = {}, Y[2] = {};
-#pragma unroll
-            for (int kk = 0; kk < KS; ++kk) {
-                const Operand<3> s = cols_of<3, DK, VP>(st, 32 * kk, vt, lane);
-#pragma unroll
-                for (int i = 0; i < 2; ++i) product<2>(s, rows_of<N, C, KP>(kt, 16 * token_tile(wave, i), 32 * kk, lane), X[i]);
-            }
-            const uint16_t* attn_t = a.attn_t + place * 3 * (C * C);
-#pragma unroll
-            for (int kk = 0; kk < 2; ++kk) {
-                const Operand<N> d = cols_of<N, C, VP>(rt, 32 * kk, vt, lane);
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    if (kk == 1 || token_tile(wave, i) < 2) product<2>(d, rows_of<3, C, C>(attn_t, 16 * token_tile(wave, i), 32 * kk, lane), Y[i]);
-            }
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int t = 16 * token_tile(wave, i) + c16;
-                put4<3, C, VP>(ut, t, vt + 4 * g, Y[i] + X[i] * decay[t].y);
-            }
+            float* to = a.dstates + place * a.dk * a.dv + vc;
+            each_row([&](int i, int r, int64_t at) { to[at] = S[i][r]; });
         }
         __syncthreads();
+        load_k(next);
+        // dU = A^T dO + delta K dS'; the scaled dO and Q for the end
+        {
+            f32x4 X[3] = {}, Y[3] = {};
+#pragma unroll
+            for (int kk = 0; kk < KS; ++kk) spread<2>(rows_of<N, C, KP>(kc, 16 * tile, 32 * kk, lane), rows_of<3, VB, SP>(st, vt, 32 * kk, lane), X);
+            if (!high) spread<2>(attn_t[0], rows_of<N, VB, CP>(rt, vt, 0, lane), Y);
+            spread<2>(attn_t[1], rows_of<N, VB, CP>(rt, vt, 32, lane), Y);
+            put4<3, VB, CP>(ut, column, tokens, gather(Y) + gather(X) * delta);
+            put4<3, VB, CP>(dt, column, tokens, x * gamma * a.scale);
+            Q.template to_lds<KP>(qt);
+        }
+        const f32x4 scale_w = -beta * gamma, step = beta;
+        const float end = whole;
+        __syncthreads();
+        load_rows(next), load_matrix(a.attn_t, next, attn_t), load_q(next);
         // dR = T^T dU
         {
-            const uint16_t* inverse_t = a.inverse_t + place * 3 * (C * C);
-            f32x4 R[2] = {};
+            f32x4 sums[3] = {};
+            if (!high) spread<2>(inverse_t[0], rows_of<3, VB, CP>(ut, vt, 0, lane), sums);
+            spread<2>(inverse_t[1], rows_of<3, VB, CP>(ut, vt, 32, lane), sums);
+            const f32x4 R = gather(sums);
+            put4<3, VB, CP>(wt, column, tokens, R * scale_w);
+            if (in) {
+                float* to = a.dputs + (place * C + tokens) * a.dv + vc;
+                T* to_v = dv + static_cast<int64_t>(t0 + tokens) * a.dv_.st;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    to[r * a.dv] = R[r];
+                    if (tokens + r < n) put(to_v, r * a.dv_.st, R[r] * step[r]);
+                }
+            }
+        }
+        __syncthreads();
+        load_matrix(a.inverse_t, next, inverse_t);
+        // dS = gamma dS' + (scale gamma Q)^T dO - (beta gamma K)^T dR
+        if (rows_here) {
+            f32x4 sums[KT][3] = {};
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk) {
-                const Operand<3> u = cols_of<3, C, VP>(ut, 32 * kk, vt, lane);
+                const Operand<3> w = rows_of<3, VB, CP>(wt, vt, 32 * kk, lane), d = rows_of<3, VB, CP>(dt, vt, 32 * kk, lane);
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    if (kk == 1 || token_tile(wave, i) < 2) product<2>(u, rows_of<3, C, C>(inverse_t, 16 * token_tile(wave, i), 32 * kk, lane), R[i]);
+                for (int i = 0; i < KT; ++i) {
+                    spread<2>(cols_of<N, C, KP>(kc, 32 * kk, 16 * (tile * KT + i), lane), w, sums[i]);
+                    spread<2>(cols_of<N, C, KP>(qt, 32 * kk, 16 * (tile * KT + i), lane), d, sums[i]);
+                }
             }
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int t = 16 * token_tile(wave, i) + c16;
-                const float beta = t < n ? a.beta[(static_cast<int64_t>(b) * a.T + t0 + t) * a.Hv + h] : 0.0f;
-                store4(a.dputs + (place * C + t) * a.dv, vc, a.dv, R[i]);
-                if (t < n) store4(dv + static_cast<int64_t>(t0 + t) * a.dv_.st, vc, a.dv, R[i] * beta);
-                put4<3, C, VP>(wt, t, vt + 4 * g, R[i] * (-beta * decay[t].x));
-            }
+            for (int i = 0; i < KT; ++i) S[i] = S[i] * end + gather(sums[i]);
         }
-        __syncthreads();
-        const float whole = decay[C - 1].x;
-#pragma unroll
-        for (int i = 0; i < KT; ++i) S[i] *= whole;
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            const Operand<3> w = cols_of<3, C, VP>(wt, 32 * kk, vt, lane);
-#pragma unroll
-            for (int i = 0; i < KT; ++i) product<2>(w, cols_of<N, C, KP>(kt, 32 * kk, 16 * ((wave >> 1) * KT + i), lane), S[i]);
-        }
-        if (!BOTH) {
-            __syncthreads();
-            tile_to_lds<T, DK, KP, 256>(q + static_cast<int64_t>(t0) * a.q.st, a.q.st, n, a.dk, qt);
-            __syncthreads();
-        }
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            const Operand<3> d = cols_of<3, C, VP>(dt, 32 * kk, vt, lane);
-#pragma unroll
-            for (int i = 0; i < KT; ++i) product<2>(d, cols_of<N, C, KP>(qt, 32 * kk, 16 * ((wave >> 1) * KT + i), lane), S[i]);
-        }
-        __syncthreads();
     }
-    if (!a.dstate_in) return;
-#pragma unroll
-    for (int i = 0; i < KT; ++i) {
-        const int r = 16 * ((wave >> 1) * KT + i) + c16;
-        if (r < a.dk) store4(a.dstate_in + state_at + static_cast<int64_t>(r) * a.dv, vc, a.dv, S[i]);
-    }
+    if (a.dstate_in) each_row([&](int i, int r, int64_t at) { a.dstate_in[state_at + at] = S[i][r]; });
 }
 
 // ---- what needs all columns of a state ----
 // A workgroup for a chunk of a head of k, its heads of v one after the other; wavefront w has tokens 16w .. 16w+15, a lane one of them.
-constexpr int VQ = VB + 8, AP = C + 8, HP = C + 4;  // pitches of rows that are read along k; of H
+constexpr int VQ = GB + 8, AP = C + 8, HP = C + 4;  // pitches of rows that are read along k; of H
 template <typename T, int DK>
 constexpr int tiles() {
     return std::max((PARTS<T> == 1 ? 2 : 3) * C * (DK + 16), 2 * C * HP);
@@ -195,16 +200,16 @@ __global__ __launch_bounds__(256) void chunk_grads(Rule a, float* sums) {
         }
         f32x4 X[4] = {}, Z[4] = {}, Y[KT] = {}, Yr[KT] = {}, Yu[KT] = {};
         float inner = 0.0f, rv = 0.0f;  // of <S, dS'>; of dR_i.V_i
-        for (int v0 = 0; v0 < a.dv; v0 += VB) {
-            for (int e = tid; e < DK * (VB / 4); e += 256) {
-                const int r = e / (VB / 4), c = e % (VB / 4) * 4;
+        for (int v0 = 0; v0 < a.dv; v0 += GB) {
+            for (int e = tid; e < DK * (GB / 4); e += 256) {
+                const int r = e / (GB / 4), c = e % (GB / 4) * 4;
                 const f32x4 x = load4(states + (r < a.dk ? r : 0) * a.dv, v0 + c, r < a.dk ? a.dv : 0), y = load4(dstates + (r < a.dk ? r : 0) * a.dv, v0 + c, r < a.dk ? a.dv : 0);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) inner = fmaf(x[j], y[j], inner);
                 put4<3, DK, VQ>(s0, r, c, x), put4<3, DK, VQ>(s1, r, c, y);
             }
-            for (int e = tid; e < C * (VB / 4); e += 256) {
-                const int r = e / (VB / 4), c = e % (VB / 4) * 4;
+            for (int e = tid; e < C * (GB / 4); e += 256) {
+                const int r = e / (GB / 4), c = e % (GB / 4) * 4;
                 put4<3, C, VQ>(ut, r, c, load4(puts + r * a.dv, v0 + c, a.dv));
             }
             const int c = v0 + 8 * g;
@@ -229,8 +234,9 @@ __global__ __launch_bounds__(256) void chunk_grads(Rule a, float* sums) {
             }
             __syncthreads();
         }
-        const float2 decay = a.decay[place * C + i];
-        const float beta = here ? a.beta[scalar_at] : 0.0f;
+        const float* scalars = a.scalars + place * 3 * C;
+        const float2 decay = make_float2(scalars[i], scalars[C + i]);
+        const float beta = scalars[2 * C + i];
         // E and F, and what they give to dbeta and to the decays
         float db = 0.0f;
 #pragma unroll
@@ -289,7 +295,7 @@ __global__ __launch_bounds__(256) void chunk_grads(Rule a, float* sums) {
             double t = tails[lane], s = static_cast<double>(ends[lane]) - t + (across[0][lane] + across[1][lane]) + (across[2][lane] + across[3][lane]);
 #pragma unroll
             for (int o = 32; o >= 1; o >>= 1) t += __shfl_xor(t, o);
-            if (lane == 63) s += t + a.decay[place * C + 63].x * all;
+            if (lane == 63) s += t + scalars[C - 1] * all;
 #pragma unroll
             for (int o = 1; o < 64; o <<= 1) {
                 const double down = __shfl_down(s, o);
@@ -339,13 +345,17 @@ __global__ __launch_bounds__(256) void chunk_grads(Rule a, float* sums) {
 }
 
 // ---- launches ----
+template <typename T, int DK, int VB, bool EVEN>
+int launch_back(const Rule& a, hipStream_t st) {
+    constexpr size_t lds = back_lds<T, DK, VB>();
+    static_assert(lds <= 160 * 1024, "LDS of a CU");
+    PK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(walk_back<T, DK, VB, EVEN>), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
+    walk_back<T, DK, VB, EVEN><<<unit_grid(static_cast<int64_t>(a.B) * a.Hv, blocks(a.dv, VB)), 16 * VB, lds, st>>>(a);
+    return launched();
+}
 template <typename T, int DK>
 int launch_back(const Rule& a, hipStream_t st) {
-    constexpr size_t lds = back_lds<T, DK>();
-    static_assert(lds <= 160 * 1024, "LDS of a CU");
-    PK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(walk_back<T, DK>), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
-    walk_back<T, DK><<<unit_grid(static_cast<int64_t>(a.B) * a.Hv, blocks(a.dv)), 256, lds, st>>>(a);
-    return launched();
+    return even(a) ? launch_back<T, DK, 16, true>(a, st) : launch_back<T, DK, 16, false>(a, st);
 }
 template <typename T, int DK>
 int launch_grads(const Rule& a, float* sums, hipStream_t st) {
@@ -367,15 +377,15 @@ int launch_backward(const Rule& a, float* sums, int dtype, hipStream_t st) {
 }
 
 struct Room {
-    size_t matrix, decay, states, puts, sums, all;
+    size_t matrix, scalars, states, puts, sums, all;
 };
 Room room_of(const pk_delta_shape* s) {
     const size_t places = static_cast<size_t>(s->B) * s->Hv * chunks(s->T), groups = static_cast<size_t>(s->B) * s->Hk * chunks(s->T);
     const size_t rows = s->dk <= 32 ? 32 : s->dk <= 64 ? 64 : 128;
     Room r;
-    r.matrix = pad(places * 3 * MATRIX), r.decay = pad(places * C * sizeof(float2)), r.states = pad(places * s->dk * s->dv * sizeof(float)), r.puts = pad(places * C * s->dv * sizeof(float));
+    r.matrix = pad(places * 3 * MATRIX), r.scalars = pad(places * 3 * C * sizeof(float)), r.states = pad(places * s->dk * s->dv * sizeof(float)), r.puts = pad(places * C * s->dv * sizeof(float));
     r.sums = s->Hv > s->Hk ? pad(groups * 2 * C * rows * sizeof(float)) : 0;
-    r.all = 3 * r.matrix + r.decay + 2 * r.states + 2 * r.puts + r.sums;
+    r.all = 3 * r.matrix + r.scalars + 2 * r.states + 2 * r.puts + r.sums;
     return r;
 }
 
@@ -415,7 +425,7 @@ int pk_delta_rule_bwd(const pk_delta_shape* s, const pk_tensor4* d_o, const floa
         };
         a.inverse = reinterpret_cast<uint16_t*>(take(r.matrix)), a.inverse_t = reinterpret_cast<uint16_t*>(take(r.matrix)), a.attn_t = reinterpret_cast<uint16_t*>(take(r.matrix));
         a.attn = a.attn_t;  // not written in the backward
-        a.decay = reinterpret_cast<float2*>(take(r.decay));
+        a.scalars = reinterpret_cast<float*>(take(r.scalars));
         a.states = reinterpret_cast<float*>(take(r.states)), a.dstates = reinterpret_cast<float*>(take(r.states));
         a.puts = reinterpret_cast<float*>(take(r.puts)), a.dputs = reinterpret_cast<float*>(take(r.puts));
         float* sums = reinterpret_cast<float*>(take(r.sums));
