@@ -188,19 +188,22 @@ template <typename V>
 __device__ inline V from_memory(const void* p) {
     return *(const __attribute__((address_space(1))) V*)(p);
 }
-// The same without a branch, for rows whose length is a multiple of what is loaded: where a row has ended the address is that of zeros.
-// EVEN is that multiple's case; the others take the functions above.
+// How rows of q, k and their like are read. ANY: by the functions above. EVEN: rows are whole pieces; without a branch, where a row has ended the address is that of zeros. EXACT: rows are
+// as long as the kernel's own, so a piece lies at an offset of 32 bits from its chunk's first.
+enum Rows { ANY, EVEN, EXACT };
 __device__ const uint32_t no_values[8] = {};
-template <bool EVEN, typename T>
-struct Eight;  // eight values as they lie in memory
-template <bool EVEN>
-struct Eight<EVEN, uint16_t> {
+template <Rows BY, typename T>
+struct Eight;  // eight values as they lie in memory: row `r` (a pitch of st) of `base`, from column c on, of n
+template <Rows BY>
+struct Eight<BY, uint16_t> {
     u32x4 v;
-    __device__ void load(const uint16_t* row, int c, int n) {
-        if constexpr (EVEN) {
-            v = from_memory<u32x4_any>(c < n ? row + c : reinterpret_cast<const uint16_t*>(no_values));
+    __device__ void load(const uint16_t* base, int64_t st, int r, int c, int n) {
+        if constexpr (BY == EXACT) {
+            v = from_memory<u32x4_any>(base + (static_cast<uint32_t>(r) * static_cast<uint32_t>(st) + static_cast<uint32_t>(c)));
+        } else if constexpr (BY == EVEN) {
+            v = from_memory<u32x4_any>(c < n ? base + r * st + c : reinterpret_cast<const uint16_t*>(no_values));
         } else {
-            const Operand<1> o = load8(row, c, n);
+            const Operand<1> o = load8(base + r * st, c, n);
             v = *reinterpret_cast<const u32x4*>(&o.part[0]);
         }
     }
@@ -210,70 +213,45 @@ struct Eight<EVEN, uint16_t> {
         return o;
     }
 };
-template <bool EVEN>
-struct Eight<EVEN, float> {
+template <Rows BY>
+struct Eight<BY, float> {
     f32x4 lo, hi;
-    __device__ void load(const float* row, int c, int n) {
-        if constexpr (EVEN) {
-            const float* p = c < n ? row + c : reinterpret_cast<const float*>(no_values);
+    __device__ void load(const float* base, int64_t st, int r, int c, int n) {
+        if constexpr (BY == EXACT) {
+            const uint32_t at = static_cast<uint32_t>(r) * static_cast<uint32_t>(st) + static_cast<uint32_t>(c);
+            lo = from_memory<f32x4_any>(base + at), hi = from_memory<f32x4_any>(base + at + 4);
+        } else if constexpr (BY == EVEN) {
+            const float* p = c < n ? base + r * st + c : reinterpret_cast<const float*>(no_values);
             lo = from_memory<f32x4_any>(p), hi = from_memory<f32x4_any>(p + 4);
         } else {
-            lo = load4(row, c, n), hi = load4(row, c + 4, n);
+            lo = load4(base + r * st, c, n), hi = load4(base + r * st, c + 4, n);
         }
     }
     __device__ Operand<3> operand() const { return split8<3>(lo, hi); }
 };
-template <bool EVEN, typename T>
-struct Four;
-template <bool EVEN>
-struct Four<EVEN, uint16_t> {
-    u32x2 v;
-    __device__ void load(const uint16_t* row, int c, int n) {
-        if constexpr (EVEN) {
-            v = from_memory<u32x2_any>(c < n ? row + c : reinterpret_cast<const uint16_t*>(no_values));
-        } else {
-            const f32x4 x = load4(row, c, n);
-            v = u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
-        }
-    }
-    __device__ f32x4 values() const {
-        return f32x4{__uint_as_float(v[0] << 16), __uint_as_float(v[0] & 0xFFFF0000u), __uint_as_float(v[1] << 16), __uint_as_float(v[1] & 0xFFFF0000u)};
-    }
-};
-template <bool EVEN>
-struct Four<EVEN, float> {
-    f32x4 v;
-    __device__ void load(const float* row, int c, int n) {
-        if constexpr (EVEN)
-            v = from_memory<f32x4_any>(c < n ? row + c : reinterpret_cast<const float*>(no_values));
-        else
-            v = load4(row, c, n);
-    }
-    __device__ f32x4 values() const { return v; }
-};
-template <bool EVEN, typename T>
+template <Rows BY, typename T>
 __device__ inline void write4(T* row, int c, int n, const f32x4& x) {
-    if constexpr (EVEN) {
-        if (c >= n) return;
+    if constexpr (BY == ANY) {
+        store4(row, c, n, x);
+    } else {
+        if (BY == EVEN && c >= n) return;
         if constexpr (sizeof(T) == 4)
             *reinterpret_cast<f32x4_any*>(row + c) = x;
         else
             *reinterpret_cast<u32x2_any*>(row + c) = u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
-    } else {
-        store4(row, c, n, x);
     }
 }
 // What a thread of NT holds of a chunk's rows of q or k on their way to LDS.
-template <bool EVEN, typename T, int DK, int NT>
+template <Rows BY, typename T, int DK, int NT>
 struct Tile {
     static constexpr int PER = DK / 8, COUNT = (C * PER + NT - 1) / NT;
     static constexpr bool WHOLE = C * PER % NT == 0;
-    Eight<EVEN, T> e[COUNT];
+    Eight<BY, T> e[COUNT];
     __device__ void load(const T* base, int64_t st, int n, int dk) {
 #pragma unroll
         for (int i = 0; i < COUNT; ++i) {
             const int at = threadIdx.x + i * NT, r = at / PER, c = at % PER * 8;
-            if (WHOLE || r < C) e[i].load(base + (r < n ? r : 0) * st, c, r < n ? dk : 0);
+            if (WHOLE || r < C) e[i].load(base, st, min(r, n - 1), c, dk);  // a token behind the last one is multiplied by zeros
         }
     }
     template <int P>
@@ -289,12 +267,18 @@ struct Tile {
     }
 };
 // Four tokens' values of one column, as they lie in memory. Tokens behind the last one have its values, columns behind the last one the first one's: they are multiplied by zero or not stored.
-template <typename T>
+template <Rows BY, typename T>
 struct Tokens {
     T v[4];
     __device__ void load(const T* base, int64_t st, int t, int n, int c, int cols) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = from_memory<T>(base + min(t + r, n - 1) * st + (c < cols ? c : 0));
+        for (int r = 0; r < 4; ++r) {
+            const int at = min(t + r, n - 1);
+            if constexpr (BY == EXACT)
+                v[r] = from_memory<T>(base + (static_cast<uint32_t>(at) * static_cast<uint32_t>(st) + static_cast<uint32_t>(c)));
+            else
+                v[r] = from_memory<T>(base + at * st + (c < cols ? c : 0));
+        }
     }
     __device__ f32x4 values() const {
         if constexpr (sizeof(T) == 4)
@@ -303,10 +287,33 @@ struct Tokens {
             return f32x4{elem(v, 0), elem(v, 1), elem(v, 2), elem(v, 3)};
     }
 };
-// Rows r0 .. r0+15 of a chunk's matrix [64][64] in memory, N parts, k from k0 on.
-template <int N>
-__device__ inline Operand<N> matrix_rows(const uint16_t* m, int r0, int k0, int lane) {
-    return rows_of<N, C, C>(m, r0, k0, lane);
+// A chunk's matrices in memory: lower triangles T and A (or, transposed, upper ones) as the operands that they are read as, 16 rows and 32 values of k to a block of 64 lanes of 16
+// bytes, in whole lines; of the eight blocks the six that are not all zeros.
+constexpr int BLOCK = 16 * 32, BLOCKS = 6;
+template <bool UPPER>
+__device__ constexpr int block_of(int tile, int kk) {
+    return UPPER ? (tile < 2 ? 2 * tile + kk : tile + 2) : (tile < 2 ? tile : 2 * tile - 2 + kk);
+}
+template <int N, bool UPPER>
+__device__ inline Operand<N> matrix_block(const uint16_t* m, int tile, int kk, int lane) {
+    Operand<N> o;
+    const uint16_t* p = m + block_of<UPPER>(tile, kk) * BLOCK + 8 * lane;
+#pragma unroll
+    for (int i = 0; i < N; ++i) o.part[i] = *reinterpret_cast<const bf16x8*>(p + i * BLOCKS * BLOCK);
+    return o;
+}
+// four values of row `row` from k on
+template <int N, bool UPPER>
+__device__ inline void put_block4(uint16_t* m, int row, int k, const f32x4& x) {
+    u32x2 p[N];
+    split4(x, p);
+    uint16_t* to = m + block_of<UPPER>(row >> 4, k >> 5) * BLOCK + ((k & 31) >> 3) * 128 + (row & 15) * 8 + (k & 7);
+#pragma unroll
+    for (int i = 0; i < N; ++i) *reinterpret_cast<u32x2*>(to + i * BLOCKS * BLOCK) = p[i];
+}
+template <bool UPPER>
+__device__ inline bool has_block(int row, int k) {
+    return UPPER ? k >= 32 || row < 32 : k < 32 || row >= 32;
 }
 // A chunk's rows of q or k (n of them are there, the others zeros) as parts in LDS, by NT threads; columns past dk are zeros.
 template <typename T, int DK, int P, int NT>
@@ -335,7 +342,7 @@ struct Rule {
     const float* state_in;          // [B][Hv][dk][dv], or null
     float* state_out;               // or null
     // for every unit (batch, head of v) and chunk:
-    uint16_t *inverse, *attn;       // parts of T and A, [64][64] each
+    uint16_t *inverse, *attn;       // parts of T and A, six blocks each
     float* scalars;                 // gamma, delta and beta of its tokens, 64 each
     float *states, *puts;           // backward: the state that the chunk begins with, [dk][dv]; U, [64][dv]
     // backward
@@ -348,7 +355,19 @@ struct Rule {
     int B, T, Hk, Hv, dk, dv, chunks;
     float scale;
 };
-inline bool even(const Rule& a) { return a.dk % 8 == 0 && a.dv % 8 == 0; }  // rows are whole loads
+inline Rows rows_by(const Rule& a, int row, int vb) {
+    const auto near = [](const View& v) { return v.st >= 0 && v.st < (1 << 22); };
+    if (a.dk == row && a.dv % vb == 0 && near(a.q) && near(a.k) && near(a.v) && near(a.dout)) return EXACT;
+    return a.dk % 8 == 0 && a.dv % 8 == 0 ? EVEN : ANY;
+}
+template <typename F>
+int by_rows(Rows r, F&& f) {
+    return r == EXACT ? f(std::integral_constant<Rows, EXACT>{}) : r == EVEN ? f(std::integral_constant<Rows, EVEN>{}) : f(std::integral_constant<Rows, ANY>{});
+}
+template <typename F>
+int by_size(int dk, F&& f) {
+    return dk <= 32 ? f(std::integral_constant<int, 32>{}) : dk <= 64 ? f(std::integral_constant<int, 64>{}) : f(std::integral_constant<int, 128>{});
+}
 // Workgroups of one unit go to one XCD, whose L2 then has the unit's q, k and matrices for all of its blocks. Launch with grid.x = unit_grid.
 inline unsigned unit_grid(int64_t units, int per) { return static_cast<unsigned>((units + 7) / 8 * 8 * per); }
 __device__ inline bool unit_of(int id, int units, int per, int& unit, int& blk) {
@@ -364,7 +383,7 @@ int launch_states(const Rule& a, int dtype, hipStream_t st);
 int check(const char* who, const pk_delta_shape* s);
 bool view_of(const pk_tensor4* t, View& v);
 inline size_t pad(size_t bytes) { return (bytes + 255) & ~size_t{255}; }
-constexpr size_t MATRIX = C * C * sizeof(uint16_t);
+constexpr size_t MATRIX = BLOCKS * BLOCK * sizeof(uint16_t);
 
 }  // namespace delta
 }  // namespace pk

@@ -44,7 +44,7 @@ __global__ __launch_bounds__(64) void chunk_matrices(Rule a) {
     __syncthreads();
     const int hk = h / (a.Hv / a.Hk);
     const T *q = head<const T>(a.q, b, hk) + static_cast<int64_t>(t0) * a.q.st, *k = head<const T>(a.k, b, hk) + static_cast<int64_t>(t0) * a.k.st;
-    uint16_t *attn = a.attn + place * PA * (C * C), *attn_t = BACKWARD ? a.attn_t + place * 3 * (C * C) : nullptr;
+    uint16_t *attn = a.attn + place * PA * (BLOCKS * BLOCK), *attn_t = BACKWARD ? a.attn_t + place * 3 * (BLOCKS * BLOCK) : nullptr;
 #pragma unroll 1
     for (int it = 0; it < 4; ++it) {
         const int i = 16 * it + c16, ri = i < n ? i : 0, di = i < n ? a.dk : 0;
@@ -75,8 +75,8 @@ __global__ __launch_bounds__(64) void chunk_matrices(Rule a) {
                 }
             }
             *reinterpret_cast<f32x4*>(m + i * MP + 16 * jt + 4 * g) = kk4;
-            if (!BACKWARD) put4<PA, C, C>(attn, i, 16 * jt + 4 * g, qk4);
-            if (BACKWARD) put4<3, C, C>(attn_t, 16 * jt + c16, 16 * it + 4 * g, kq4);
+            if (!BACKWARD && has_block<false>(i, 16 * jt)) put_block4<PA, false>(attn, i, 16 * jt + 4 * g, qk4);
+            if (BACKWARD && has_block<true>(16 * jt, 16 * it)) put_block4<3, true>(attn_t, 16 * jt + c16, 16 * it + 4 * g, kq4);
         }
     }
     __syncthreads();
@@ -94,21 +94,25 @@ __global__ __launch_bounds__(64) void chunk_matrices(Rule a) {
         t[i] = (s[0] + s[1]) + (s[2] + s[3]);
     }
     if (BACKWARD) {
-        uint16_t* out = a.inverse_t + place * 3 * (C * C);
+        uint16_t* out = a.inverse_t + place * 3 * (BLOCKS * BLOCK);
 #pragma unroll
-        for (int i = 0; i < C; i += 4) put4<3, C, C>(out, lane, i, f32x4{t[i], t[i + 1], t[i + 2], t[i + 3]});
+        for (int i = 0; i < C; i += 4)
+            if (has_block<true>(lane, i)) put_block4<3, true>(out, lane, i, f32x4{t[i], t[i + 1], t[i + 2], t[i + 3]});
     }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < C; ++i) m[i * MP + lane] = t[i];
     __syncthreads();
-    uint16_t* out = a.inverse + place * 3 * (C * C);
-    for (int i = lane; i < C * C / 8; i += 64) {
-        const float* from = m + i / 8 * MP + i % 8 * 8;
-        const Operand<3> o = split8<3>(*reinterpret_cast<const f32x4*>(from), *reinterpret_cast<const f32x4*>(from + 4));
+    uint16_t* out = a.inverse + place * 3 * (BLOCKS * BLOCK);
 #pragma unroll
-        for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(out + p * C * C + i * 8) = o.part[p];
-    }
+    for (int it = 0; it < 4; ++it)
+#pragma unroll
+        for (int kk = 0; kk <= it / 2; ++kk) {
+            const float* from = m + (16 * it + c16) * MP + 32 * kk + 8 * g;
+            const Operand<3> o = split8<3>(*reinterpret_cast<const f32x4*>(from), *reinterpret_cast<const f32x4*>(from + 4));
+#pragma unroll
+            for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(out + (p * BLOCKS + block_of<false>(it, kk)) * BLOCK + 8 * lane) = o.part[p];
+        }
 }
 
 // ---- the walk down the chunks ----
@@ -118,7 +122,7 @@ __global__ __launch_bounds__(64) void chunk_matrices(Rule a) {
 template <typename T, int DK>
 constexpr bool TWO_K = PARTS<T> == 1 || DK < 128;  // two of K's tiles in LDS: the next one is written while this one is still read
 
-template <typename T, int DK, int VB, bool STATES, bool EVEN>
+template <typename T, int DK, int VB, bool STATES, Rows BY>
 __global__ __launch_bounds__(16 * VB) void walk(Rule a) {
     constexpr int N = PARTS<T>, KP = DK + 16, SP = DK + 8, KS = DK / 32, KT = (DK + 63) / 64, PO = N == 1 ? 2 : 3;  // PO: parts of U and A on their way to O
     extern __shared__ uint16_t lds[];
@@ -147,9 +151,9 @@ __global__ __launch_bounds__(16 * VB) void walk(Rule a) {
     };
     f32x4 S[KT] = {};
     if (a.state_in) each_row([&](int i, int r, int64_t at) { S[i][r] = a.state_in[state_at + at]; });
-    Tile<EVEN, T, DK, 16 * VB> K;
-    Eight<EVEN, T> Q[KS];
-    Tokens<T> V;
+    Tile<BY, T, DK, 16 * VB> K;
+    Eight<BY, T> Q[KS];
+    Tokens<BY, T> V;
     Operand<3> inverse[2];
     Operand<PO> attn[2];
     f32x4 gamma, delta, beta;
@@ -163,20 +167,19 @@ __global__ __launch_bounds__(16 * VB) void walk(Rule a) {
         V.load(v + static_cast<int64_t>(chunk) * C * a.v.st, a.v.st, tokens, n, vc, a.dv);
         if (!STATES) {
             gamma_o = d[token];
-            const T* row = q + (static_cast<int64_t>(chunk) * C + min(token, n - 1)) * a.q.st;
 #pragma unroll
-            for (int kk = 0; kk < KS; ++kk) Q[kk].load(row, 32 * kk + 8 * g, a.dk);
+            for (int kk = 0; kk < KS; ++kk) Q[kk].load(q + static_cast<int64_t>(chunk) * C * a.q.st, a.q.st, min(token, n - 1), 32 * kk + 8 * g, a.dk);
         }
     };
     const auto load_inverse = [&](int chunk) {
-        const uint16_t* m = a.inverse + (first + chunk) * 3 * (C * C);
-        inverse[0] = matrix_rows<3>(m, 16 * tile, 0, lane);
-        if (!low) inverse[1] = matrix_rows<3>(m, 16 * tile, 32, lane);
+        const uint16_t* m = a.inverse + (first + chunk) * 3 * (BLOCKS * BLOCK);
+        inverse[0] = matrix_block<3, false>(m, tile, 0, lane);
+        if (!low) inverse[1] = matrix_block<3, false>(m, tile, 1, lane);
     };
     const auto load_attn = [&](int chunk) {
-        const uint16_t* m = a.attn + (first + chunk) * PO * (C * C);
-        attn[0] = matrix_rows<PO>(m, 16 * tile, 0, lane);
-        if (!low) attn[1] = matrix_rows<PO>(m, 16 * tile, 32, lane);
+        const uint16_t* m = a.attn + (first + chunk) * PO * (BLOCKS * BLOCK);
+        attn[0] = matrix_block<PO, false>(m, tile, 0, lane);
+        if (!low) attn[1] = matrix_block<PO, false>(m, tile, 1, lane);
     };
     load_k(0), load_rows(0), load_inverse(0);
     if (!STATES) load_attn(0);
@@ -250,7 +253,7 @@ __global__ __launch_bounds__(16 * VB) void walk(Rule a) {
             f32x4 sums[PO] = {};
             spread<PO - 1>(rows_of<PO, VB, CP>(ut, vt, 0, lane), attn[0], sums);
             if (!low) spread<PO - 1>(rows_of<PO, VB, CP>(ut, vt, 32, lane), attn[1], sums);
-            if (token < n) write4<EVEN>(out + static_cast<int64_t>(t0 + token) * a.o.st, vo, a.dv, O + gather(sums));
+            if (token < n) write4<BY>(out + static_cast<int64_t>(t0 + token) * a.o.st, vo, a.dv, O + gather(sums));
             load_attn(next);
         }
     }
@@ -338,25 +341,21 @@ __global__ __launch_bounds__(STEP_NT) void steps(Rule a) {
 // ---- launches ----
 
 constexpr int FEW_TOKENS = 16;
-template <typename T, int DK, int VB, bool STATES, bool EVEN>
+template <typename T, int DK, int VB, bool STATES, Rows BY>
 int launch_walk(const Rule& a, hipStream_t st) {
     constexpr size_t lds = walk_lds<T, DK, VB, STATES>();
     static_assert(lds <= 160 * 1024, "LDS of a CU");
-    PK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(walk<T, DK, VB, STATES, EVEN>), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
-    walk<T, DK, VB, STATES, EVEN><<<unit_grid(static_cast<int64_t>(a.B) * a.Hv, blocks(a.dv, VB)), 16 * VB, lds, st>>>(a);
+    PK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(walk<T, DK, VB, STATES, BY>), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
+    walk<T, DK, VB, STATES, BY><<<unit_grid(static_cast<int64_t>(a.B) * a.Hv, blocks(a.dv, VB)), 16 * VB, lds, st>>>(a);
     return launched();
-}
-template <typename T, int DK, bool STATES, bool EVEN>
-int launch_walk(const Rule& a, hipStream_t st) {
-    return getenv("PK_VB32") ? launch_walk<T, DK, 32, STATES, EVEN>(a, st) : launch_walk<T, DK, 16, STATES, EVEN>(a, st);
-}
-template <typename T, bool STATES, bool EVEN>
-int launch_walk(const Rule& a, hipStream_t st) {
-    return a.dk <= 32 ? launch_walk<T, 32, STATES, EVEN>(a, st) : a.dk <= 64 ? launch_walk<T, 64, STATES, EVEN>(a, st) : launch_walk<T, 128, STATES, EVEN>(a, st);
 }
 template <typename T, bool STATES>
 int launch_walk(const Rule& a, hipStream_t st) {
-    return even(a) ? launch_walk<T, STATES, true>(a, st) : launch_walk<T, STATES, false>(a, st);
+    return by_size(a.dk, [&](auto dk) {
+        constexpr int DK = decltype(dk)::value;
+        return getenv("PK_VB32") ? by_rows(rows_by(a, DK, 32), [&](auto by) { return launch_walk<T, DK, 32, STATES, decltype(by)::value>(a, st); })
+        : by_rows(rows_by(a, DK, 16), [&](auto by) { return launch_walk<T, DK, 16, STATES, decltype(by)::value>(a, st); });
+    });
 }
 template <typename T, int DK>
 void launch_matrices(const Rule& a, bool backward, hipStream_t st) {

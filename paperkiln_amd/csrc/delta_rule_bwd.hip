@@ -29,7 +29,7 @@ template <typename T, int DK, int VB>
 constexpr size_t back_lds() {
     return sizeof(uint16_t) * ((TWO_K<DK> ? 3 : 2) * PARTS<T> * C * (DK + 16) + 3 * VB * (DK + 8) + (9 + PARTS<T>) * VB * CP);
 }
-template <typename T, int DK, int VB, bool EVEN>
+template <typename T, int DK, int VB, Rows BY>
 __global__ __launch_bounds__(16 * VB) void walk_back(Rule a) {
     constexpr int N = PARTS<T>, KP = DK + 16, SP = DK + 8, KS = DK / 32, KT = (DK + 63) / 64;
     extern __shared__ uint16_t lds[];
@@ -56,8 +56,8 @@ __global__ __launch_bounds__(16 * VB) void walk_back(Rule a) {
     };
     f32x4 S[KT] = {};  // of the gradient of the state
     if (a.dstate_out) each_row([&](int i, int r, int64_t at) { S[i][r] = a.dstate_out[state_at + at]; });
-    Tile<EVEN, T, DK, 16 * VB> K, Q;
-    Tokens<T> D;
+    Tile<BY, T, DK, 16 * VB> K, Q;
+    Tokens<BY, T> D;
     Operand<3> attn_t[2], inverse_t[2];
     f32x4 gamma, delta, beta;
     float whole;
@@ -70,9 +70,9 @@ __global__ __launch_bounds__(16 * VB) void walk_back(Rule a) {
         D.load(dout + static_cast<int64_t>(chunk) * C * a.dout.st, a.dout.st, tokens, min(C, a.T - chunk * C), vc, a.dv);
     };
     const auto load_matrix = [&](const uint16_t* all, int chunk, Operand<3>(&o)[2]) {
-        const uint16_t* m = all + (first + chunk) * 3 * (C * C);
-        if (!high) o[0] = matrix_rows<3>(m, 16 * tile, 0, lane);
-        o[1] = matrix_rows<3>(m, 16 * tile, 32, lane);
+        const uint16_t* m = all + (first + chunk) * 3 * (BLOCKS * BLOCK);
+        if (!high) o[0] = matrix_block<3, true>(m, tile, 0, lane);
+        o[1] = matrix_block<3, true>(m, tile, 1, lane);
     };
     if (a.chunks > 0) load_k(a.chunks - 1), load_rows(a.chunks - 1), load_matrix(a.attn_t, a.chunks - 1, attn_t), load_q(a.chunks - 1), load_matrix(a.inverse_t, a.chunks - 1, inverse_t);
     for (int chunk = a.chunks - 1; chunk >= 0; --chunk) {
@@ -345,17 +345,13 @@ __global__ __launch_bounds__(256) void chunk_grads(Rule a, float* sums) {
 }
 
 // ---- launches ----
-template <typename T, int DK, int VB, bool EVEN>
+template <typename T, int DK, int VB, Rows BY>
 int launch_back(const Rule& a, hipStream_t st) {
     constexpr size_t lds = back_lds<T, DK, VB>();
     static_assert(lds <= 160 * 1024, "LDS of a CU");
-    PK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(walk_back<T, DK, VB, EVEN>), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
-    walk_back<T, DK, VB, EVEN><<<unit_grid(static_cast<int64_t>(a.B) * a.Hv, blocks(a.dv, VB)), 16 * VB, lds, st>>>(a);
+    PK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(walk_back<T, DK, VB, BY>), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
+    walk_back<T, DK, VB, BY><<<unit_grid(static_cast<int64_t>(a.B) * a.Hv, blocks(a.dv, VB)), 16 * VB, lds, st>>>(a);
     return launched();
-}
-template <typename T, int DK>
-int launch_back(const Rule& a, hipStream_t st) {
-    return even(a) ? launch_back<T, DK, 16, true>(a, st) : launch_back<T, DK, 16, false>(a, st);
 }
 template <typename T, int DK>
 int launch_grads(const Rule& a, float* sums, hipStream_t st) {
@@ -367,13 +363,16 @@ int launch_grads(const Rule& a, float* sums, hipStream_t st) {
 }
 template <typename T>
 int launch_backward(const Rule& a, float* sums, int dtype, hipStream_t st) {
-    const auto by_rows = [&](auto&& f) { return a.dk <= 32 ? f(std::integral_constant<int, 32>{}) : a.dk <= 64 ? f(std::integral_constant<int, 64>{}) : f(std::integral_constant<int, 128>{}); };
     if (a.chunks > 0) {
         if (int rc = launch_chunks(a, dtype, true, st)) return rc;
         if (int rc = launch_states(a, dtype, st)) return rc;
     }
-    if (int rc = by_rows([&](auto dk) { return launch_back<T, decltype(dk)::value>(a, st); })) return rc;
-    return a.chunks == 0 ? PK_OK : by_rows([&](auto dk) { return launch_grads<T, decltype(dk)::value>(a, sums, st); });
+    const int rc = by_size(a.dk, [&](auto dk) {
+        constexpr int DK = decltype(dk)::value;
+        return by_rows(rows_by(a, DK, 16), [&](auto by) { return launch_back<T, DK, 16, decltype(by)::value>(a, st); });
+    });
+    if (rc || a.chunks == 0) return rc;
+    return by_size(a.dk, [&](auto dk) { return launch_grads<T, decltype(dk)::value>(a, sums, st); });
 }
 
 struct Room {
