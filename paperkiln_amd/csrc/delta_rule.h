@@ -229,6 +229,24 @@ struct Eight<BY, float> {
     }
     __device__ Operand<3> operand() const { return split8<3>(lo, hi); }
 };
+// eight values as they are
+template <Rows BY>
+__device__ inline void values_of(const Eight<BY, uint16_t>& e, f32x4& lo, f32x4& hi) {
+    lo = f32x4{__uint_as_float(e.v[0] << 16), __uint_as_float(e.v[0] & 0xFFFF0000u), __uint_as_float(e.v[1] << 16), __uint_as_float(e.v[1] & 0xFFFF0000u)};
+    hi = f32x4{__uint_as_float(e.v[2] << 16), __uint_as_float(e.v[2] & 0xFFFF0000u), __uint_as_float(e.v[3] << 16), __uint_as_float(e.v[3] & 0xFFFF0000u)};
+}
+template <Rows BY>
+__device__ inline void values_of(const Eight<BY, float>& e, f32x4& lo, f32x4& hi) { lo = e.lo, hi = e.hi; }
+// Four values of a dense matrix [rows][cols] of 32 bits: row r from column c on; zeros outside of it.
+template <Rows BY>
+__device__ inline f32x4 dense4(const float* base, int r, int c, int rows, int cols) {
+    if constexpr (BY == EXACT)
+        return from_memory<f32x4_any>(base + static_cast<uint32_t>(r * cols + c));
+    else if constexpr (BY == EVEN)
+        return from_memory<f32x4_any>(r < rows && c < cols ? base + (r * cols + c) : reinterpret_cast<const float*>(no_values));
+    else
+        return load4(base + (r < rows ? r : 0) * cols, c, r < rows ? cols : 0);
+}
 template <Rows BY, typename T>
 __device__ inline void write4(T* row, int c, int n, const f32x4& x) {
     if constexpr (BY == ANY) {

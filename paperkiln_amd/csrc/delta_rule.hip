@@ -93,12 +93,6 @@ __global__ __launch_bounds__(64) void chunk_matrices(Rule a) {
         }
         t[i] = (s[0] + s[1]) + (s[2] + s[3]);
     }
-    if (BACKWARD) {
-        uint16_t* out = a.inverse_t + place * 3 * (BLOCKS * BLOCK);
-#pragma unroll
-        for (int i = 0; i < C; i += 4)
-            if (has_block<true>(lane, i)) put_block4<3, true>(out, lane, i, f32x4{t[i], t[i + 1], t[i + 2], t[i + 3]});
-    }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < C; ++i) m[i * MP + lane] = t[i];
@@ -112,6 +106,17 @@ __global__ __launch_bounds__(64) void chunk_matrices(Rule a) {
             const Operand<3> o = split8<3>(*reinterpret_cast<const f32x4*>(from), *reinterpret_cast<const f32x4*>(from + 4));
 #pragma unroll
             for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(out + (p * BLOCKS + block_of<false>(it, kk)) * BLOCK + 8 * lane) = o.part[p];
+        }
+    if (!BACKWARD) return;
+    out = a.inverse_t + place * 3 * (BLOCKS * BLOCK);
+#pragma unroll
+    for (int it = 0; it < 4; ++it)
+#pragma unroll
+        for (int kk = it / 2; kk < 2; ++kk) {
+            const float* from = m + (32 * kk + 8 * g) * MP + 16 * it + c16;
+            const Operand<3> o = split8<3>(f32x4{from[0], from[MP], from[2 * MP], from[3 * MP]}, f32x4{from[4 * MP], from[5 * MP], from[6 * MP], from[7 * MP]});
+#pragma unroll
+            for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(out + (p * BLOCKS + block_of<true>(it, kk)) * BLOCK + 8 * lane) = o.part[p];
         }
 }
 

@@ -149,48 +149,74 @@ __global__ __launch_bounds__(16 * VB) void walk_back(Rule a) {
 }
 
 // ---- what needs all columns of a state ----
-// A workgroup for a chunk of a head of k, its heads of v one after the other; wavefront w has tokens 16w .. 16w+15, a lane one of them.
-constexpr int VQ = GB + 8, AP = C + 8, HP = C + 4;  // pitches of rows that are read along k; of H
+// A workgroup for a chunk of a head of k, its heads of v one after the other. Of its eight wavefronts w and w + 4 have tokens 16w .. 16w+15, a lane one of them; each has half of the
+// 64 x dk products' rows, the first one E, the second one F.
+constexpr int VQ = GB + 8, AP = C + 8, HP = C + 4, GRAD_NT = 512;  // pitches of rows that are read along k; of H
+// K and Q stay in LDS beside what goes by, but for three parts of 128 columns each, which come one after the other when that is done.
 template <typename T, int DK>
-constexpr int tiles() {
-    return std::max((PARTS<T> == 1 ? 2 : 3) * C * (DK + 16), 2 * C * HP);
+constexpr bool BESIDE = PARTS<T> == 1 || DK < 128;
+template <typename T, int DK>
+constexpr int tile_size() {
+    return PARTS<T> * C * (DK + 16);
 }
 template <typename T, int DK>
 constexpr size_t grads_lds() {
-    constexpr int PE = PARTS<T> == 1 ? 2 : 3;
-    return sizeof(uint16_t) * std::max((6 * DK + 3 * C) * VQ, tiles<T, DK>() + 2 * PE * C * AP);
+    constexpr int PE = PARTS<T> == 1 ? 2 : 3, by = (6 * DK + 3 * C) * VQ, then = 4 * C * HP + 2 * PE * C * AP;
+    return sizeof(uint16_t) * (BESIDE<T, DK> ? 2 * tile_size<T, DK>() + std::max(by, then) : std::max(by, tile_size<T, DK>() + then));
+}
+template <Rows BY, typename T, int DK, int P>
+__device__ inline void tile_in(const T* base, int64_t st, int n, int dk, uint16_t* m) {
+    Tile<BY, T, DK, GRAD_NT> t;
+    t.load(base, st, n, dk);
+    t.template to_lds<P>(m);
 }
 __device__ inline float over_groups(float x) {  // the four lanes of a token
     x += __shfl_xor(x, 16);
     return x + __shfl_xor(x, 32);
 }
-template <typename T, int DK>
-__global__ __launch_bounds__(256) void chunk_grads(Rule a, float* sums) {
-    constexpr int N = PARTS<T>, MOST = N == 1 ? 0 : 2, PE = N == 1 ? 2 : 3, KP = DK + 16, KS = DK / 32, KT = DK / 16;
-    constexpr bool BOTH = N == 1;
+template <typename T, int DK, Rows BY>
+__global__ __launch_bounds__(GRAD_NT, 2) void chunk_grads(Rule a, float* sums) {
+    constexpr int N = PARTS<T>, MOST = N == 1 ? 0 : 2, PE = N == 1 ? 2 : 3, KP = DK + 16, KS = DK / 32, KT = DK / 32, SN = (DK * (GB / 4) + GRAD_NT - 1) / GRAD_NT;
+    constexpr bool BOTH = BESIDE<T, DK>;
     extern __shared__ uint16_t lds[];
     __shared__ double total[C];
-    __shared__ double across[4][C];
-    __shared__ float ends[C], tails[C], dots[4];
-    uint16_t *s0 = lds, *s1 = s0 + 3 * DK * VQ, *ut = s1 + 3 * DK * VQ;                            // while the columns of the state go by
-    uint16_t *kt = lds, *qt = BOTH ? kt + C * KP : kt, *et = kt + tiles<T, DK>(), *ft = et + PE * C * AP;  // then
-    float* ht = reinterpret_cast<float*>(lds);  // before K and Q come there
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c16 = lane & 15, i = 16 * wave + c16;
+    __shared__ double across[8][C];
+    __shared__ float ends[2][C], tails[2][C], dbs[2][C], dots[8];
+    uint16_t *kt = lds, *qt = BOTH ? kt + tile_size<T, DK>() : kt, *s0 = BOTH ? qt + tile_size<T, DK>() : lds;
+    uint16_t *s1 = s0 + 3 * DK * VQ, *ut = s1 + 3 * DK * VQ;                                                          // while the columns of the state go by
+    uint16_t *hs = BOTH ? s0 : s0 + tile_size<T, DK>(), *et = hs + 4 * C * HP, *ft = et + PE * C * AP;  // then
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, tile = wave & 3, half = wave >> 2, g = lane >> 4, c16 = lane & 15, i = 16 * tile + c16;
+    float* ht = reinterpret_cast<float*>(hs) + half * C * HP;
     const int64_t group = blockIdx.x / static_cast<unsigned>(a.chunks);
     const int chunk = blockIdx.x % static_cast<unsigned>(a.chunks), b = static_cast<int>(group / a.Hk), hk = static_cast<int>(group % a.Hk), rep = a.Hv / a.Hk;
-    const int t0 = chunk * C, n = min(C, a.T - t0);
+    const int t0 = chunk * C, n = min(C, a.T - t0), mine_at = min(i, n - 1);  // a token behind the last one reads its row and counts for nothing
     const bool here = i < n;
-    const int64_t row = t0 + (here ? i : 0);
-    const T *q = head<const T>(a.q, b, hk), *k = head<const T>(a.k, b, hk), *qi = q + row * a.q.st, *ki = k + row * a.k.st;
+    const T *q = head<const T>(a.q, b, hk) + static_cast<int64_t>(t0) * a.q.st, *k = head<const T>(a.k, b, hk) + static_cast<int64_t>(t0) * a.k.st;
     float* mine = rep > 1 ? sums + static_cast<int64_t>(blockIdx.x) * 2 * C * DK + i * DK : nullptr;  // what the heads of v before have given to dQ's and dK's rows
+    if (BOTH) tile_in<BY, T, DK, KP>(k, a.k.st, n, a.dk, kt), tile_in<BY, T, DK, KP>(q, a.q.st, n, a.dk, qt);
+    const auto d_of = [&](int d) { return 16 * (half * KT + d); };
     for (int head_v = 0; head_v < rep; ++head_v) {
         const int h = hk * rep + head_v;
-        const int64_t unit = static_cast<int64_t>(b) * a.Hv + h, place = unit * a.chunks + chunk, scalar_at = (static_cast<int64_t>(b) * a.T + t0 + i) * a.Hv + h;
-        const T *v = head<const T>(a.v, b, h) + row * a.v.st, *dout = head<const T>(a.dout, b, h) + row * a.dout.st;
-        const float *states = a.states + place * a.dk * a.dv, *dstates = a.dstates + place * a.dk * a.dv, *puts = a.puts + place * C * a.dv, *dputs = a.dputs + (place * C + i) * a.dv;
+        const int64_t unit = static_cast<int64_t>(b) * a.Hv + h, place = unit * a.chunks + chunk;
+        const T *v = head<const T>(a.v, b, h) + static_cast<int64_t>(t0) * a.v.st, *dout = head<const T>(a.dout, b, h) + static_cast<int64_t>(t0) * a.dout.st;
+        const float *states = a.states + place * a.dk * a.dv, *dstates = a.dstates + place * a.dk * a.dv, *puts = a.puts + place * C * a.dv, *dputs = a.dputs + place * C * a.dv;
+        // what a block of columns needs from memory, asked for a block ahead
+        f32x4 x[SN], y[SN], u, r0, r1;
+        Eight<BY, T> dov, vv;
+        const int row = tid / (GB / 4), col = tid % (GB / 4) * 4;
+        const auto load = [&](int v0) {
+#pragma unroll
+            for (int e = 0; e < SN; ++e)
+                if (DK >= 64 || row < DK) x[e] = dense4<BY>(states, row + 64 * e, v0 + col, a.dk, a.dv), y[e] = dense4<BY>(dstates, row + 64 * e, v0 + col, a.dk, a.dv);
+            u = dense4<BY>(puts, row, v0 + col, C, a.dv);
+            r0 = dense4<BY>(dputs, i, v0 + 8 * g, C, a.dv), r1 = dense4<BY>(dputs, i, v0 + 8 * g + 4, C, a.dv);
+            dov.load(dout, a.dout.st, mine_at, v0 + 8 * g, a.dv);
+            if (half == 0) vv.load(v, a.v.st, mine_at, v0 + 8 * g, a.dv);
+        };
+        load(0);
         if (wave == 0) {  // the sum of the log-decays
-            const float x = lane < n ? a.g[(static_cast<int64_t>(b) * a.T + t0 + lane) * a.Hv + h] : 0.0f;
-            double s = x < LEAST ? LEAST : x;
+            const float f = lane < n ? a.g[(static_cast<int64_t>(b) * a.T + t0 + lane) * a.Hv + h] : 0.0f;
+            double s = f < LEAST ? LEAST : f;
 #pragma unroll
             for (int o = 1; o < 64; o <<= 1) {
                 const double up = __shfl_up(s, o);
@@ -198,39 +224,43 @@ __global__ __launch_bounds__(256) void chunk_grads(Rule a, float* sums) {
             }
             total[lane] = s;
         }
-        f32x4 X[4] = {}, Z[4] = {}, Y[KT] = {}, Yr[KT] = {}, Yu[KT] = {};
+        f32x4 X[4] = {}, Y[KT] = {}, Yr[KT] = {}, Yu[KT] = {};  // X: of dO, or of dR
         float inner = 0.0f, rv = 0.0f;  // of <S, dS'>; of dR_i.V_i
+#pragma unroll 1
         for (int v0 = 0; v0 < a.dv; v0 += GB) {
-            for (int e = tid; e < DK * (GB / 4); e += 256) {
-                const int r = e / (GB / 4), c = e % (GB / 4) * 4;
-                const f32x4 x = load4(states + (r < a.dk ? r : 0) * a.dv, v0 + c, r < a.dk ? a.dv : 0), y = load4(dstates + (r < a.dk ? r : 0) * a.dv, v0 + c, r < a.dk ? a.dv : 0);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) inner = fmaf(x[j], y[j], inner);
-                put4<3, DK, VQ>(s0, r, c, x), put4<3, DK, VQ>(s1, r, c, y);
-            }
-            for (int e = tid; e < C * (GB / 4); e += 256) {
-                const int r = e / (GB / 4), c = e % (GB / 4) * 4;
-                put4<3, C, VQ>(ut, r, c, load4(puts + r * a.dv, v0 + c, a.dv));
-            }
-            const int c = v0 + 8 * g;
-            const f32x4 r0 = load4(dputs, c, a.dv), r1 = load4(dputs, c + 4, a.dv), x0 = load4(v, c, here ? a.dv : 0), x1 = load4(v, c + 4, here ? a.dv : 0);
+            for (int e = 0; e < SN; ++e)
+                if (DK >= 64 || row < DK) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) rv = fmaf(r0[j], x0[j], fmaf(r1[j], x1[j], rv));
+                    for (int j = 0; j < 4; ++j) inner = fmaf(x[e][j], y[e][j], inner);
+                    put4<3, DK, VQ>(s0, row + 64 * e, col, x[e]), put4<3, DK, VQ>(s1, row + 64 * e, col, y[e]);
+                }
+            put4<3, C, VQ>(ut, row, col, u);
+            if (half == 0) {
+                f32x4 x0, x1;
+                values_of(vv, x0, x1);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) rv = fmaf(r0[j], x0[j], fmaf(r1[j], x1[j], rv));
+            }
             const Operand<3> dr = split8<3>(r0, r1);
-            const Operand<N> od = load8(dout, c, here ? a.dv : 0);
+            const Operand<N> od = dov.operand();
             __syncthreads();
-            const Operand<3> u = rows_of<3, C, VQ>(ut, 16 * wave, 0, lane);
+            if (v0 + GB < a.dv) load(v0 + GB);
+            const Operand<3> ui = rows_of<3, C, VQ>(ut, 16 * tile, 0, lane);
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (j <= wave) {
+                if (j <= tile) {
                     const Operand<3> uj = rows_of<3, C, VQ>(ut, 16 * j, 0, lane);
-                    product<2>(uj, od, X[j]), product<2>(uj, dr, Z[j]);
+                    if (half == 0)
+                        product<2>(uj, od, X[j]);
+                    else
+                        product<2>(uj, dr, X[j]);
                 }
 #pragma unroll
             for (int d = 0; d < KT; ++d) {
-                const Operand<3> s = rows_of<3, DK, VQ>(s0, 16 * d, 0, lane);
-                product<2>(s, od, Y[d]), product<2>(s, dr, Yr[d]);
-                product<2>(rows_of<3, DK, VQ>(s1, 16 * d, 0, lane), u, Yu[d]);
+                __builtin_amdgcn_sched_barrier(0);  // the operands of one d at a time: those of all would not fit into the registers
+                const Operand<3> s = rows_of<3, DK, VQ>(s0, d_of(d), 0, lane), t = rows_of<3, DK, VQ>(s1, d_of(d), 0, lane);
+                product<2>(s, od, Y[d]), product<2>(s, dr, Yr[d]), product<2>(t, ui, Yu[d]);
             }
             __syncthreads();
         }
@@ -239,60 +269,77 @@ __global__ __launch_bounds__(256) void chunk_grads(Rule a, float* sums) {
         const float beta = scalars[2 * C + i];
         // E and F, and what they give to dbeta and to the decays
         float db = 0.0f;
+        {
+            // rows of K and Q as operands: from LDS, or from memory
+            const auto row_k = [&](int j, int s) {
+                if constexpr (BOTH) return rows_of<N, C, KP>(kt, 16 * j, 32 * s, lane);
+                Eight<BY, T> e;
+                e.load(k, a.k.st, min(16 * j + c16, n - 1), 32 * s + 8 * g, a.dk);
+                return e.operand();
+            };
+            const auto row_own = [&](int s) {
+                if constexpr (BOTH) return rows_of<N, C, KP>(half == 0 ? qt : kt, 16 * tile, 32 * s, lane);
+                Eight<BY, T> e;
+                if (half == 0)
+                    e.load(q, a.q.st, mine_at, 32 * s + 8 * g, a.dk);
+                else
+                    e.load(k, a.k.st, mine_at, 32 * s + 8 * g, a.dk);
+                return e.operand();
+            };
+            const float factor = half == 0 ? a.scale : -beta;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            f32x4 qk = {0, 0, 0, 0}, kk = qk, H = qk;
-            if (j <= wave) {
-                const int other = 16 * j + c16;
-                const T* kj = k + static_cast<int64_t>(t0 + (other < n ? other : 0)) * a.k.st;
+            for (int j = 0; j < 4; ++j) {
+                f32x4 xk = {0, 0, 0, 0}, H = xk;
+                if (j <= tile) {
 #pragma unroll
-                for (int s = 0; s < KS; ++s) {
-                    const Operand<N> x = load8(kj, 32 * s + 8 * g, other < n ? a.dk : 0);
-                    product<MOST>(x, load8(qi, 32 * s + 8 * g, here ? a.dk : 0), qk), product<MOST>(x, load8(ki, 32 * s + 8 * g, here ? a.dk : 0), kk);
+                    for (int s = 0; s < KS; ++s) product<MOST>(row_k(j, s), row_own(s), xk);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int at = 16 * j + 4 * g + r;
+                        const float D = here && (half == 0 ? at <= i : at < i) ? decay_of(total[i] - total[at]) : 0.0f, z = D == 0.0f ? 0.0f : D * X[j][r];
+                        X[j][r] = factor * z;
+                        H[r] = at < i ? X[j][r] * xk[r] : 0.0f;
+                        db = fmaf(z, xk[r], db);
+                    }
                 }
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int at = 16 * j + 4 * g + r;
-                    const float D = at <= i ? decay_of(total[i] - total[at]) : 0.0f, z = at < i ? D * Z[j][r] : 0.0f;
-                    X[j][r] *= a.scale * D, Z[j][r] = -beta * z;
-                    if (at > i) X[j][r] = 0.0f;
-                    H[r] = at < i ? fmaf(X[j][r], qk[r], Z[j][r] * kk[r]) : 0.0f;
-                    db = fmaf(z, kk[r], db);
-                }
+                put4<PE, C, AP>(half == 0 ? et : ft, i, 16 * j + 4 * g, X[j]);
+                *reinterpret_cast<f32x4*>(ht + i * HP + 16 * j + 4 * g) = H;
             }
-            put4<PE, C, AP>(et, i, 16 * j + 4 * g, X[j]), put4<PE, C, AP>(ft, i, 16 * j + 4 * g, Z[j]);
-            *reinterpret_cast<f32x4*>(ht + i * HP + 16 * j + 4 * g) = H;
         }
         float qy = 0.0f, kr = 0.0f, ku = 0.0f;
 #pragma unroll
         for (int d = 0; d < KT; ++d) {
-            const f32x4 x = load4(qi, 16 * d + 4 * g, here ? a.dk : 0), y = load4(ki, 16 * d + 4 * g, here ? a.dk : 0);
+            f32x4 xq, xk;
+            if constexpr (N == 1) {
+                xq = load4(qt + i * KP, d_of(d) + 4 * g, DK), xk = load4(kt + i * KP, d_of(d) + 4 * g, DK);
+            } else {
+                xq = load4(q + mine_at * a.q.st, d_of(d) + 4 * g, a.dk), xk = load4(k + mine_at * a.k.st, d_of(d) + 4 * g, a.dk);
+            }
 #pragma unroll
-            for (int r = 0; r < 4; ++r) qy = fmaf(x[r], Y[d][r], qy), kr = fmaf(y[r], Yr[d][r], kr), ku = fmaf(y[r], Yu[d][r], ku);
+            for (int r = 0; r < 4; ++r) qy = fmaf(xq[r], Y[d][r], qy), kr = fmaf(xk[r], Yr[d][r], kr), ku = fmaf(xk[r], Yu[d][r], ku);
         }
-        const float in = a.scale * decay.x, back = -beta * decay.x;
+        const float in = here ? a.scale * decay.x : 0.0f, back = -beta * decay.x;
         const float tail = over_groups(ku) * decay.y, end = over_groups(fmaf(in, qy, back * kr));
-        db = over_groups(rv - fmaf(decay.x, kr, db));
+        db = over_groups(fmaf(-decay.x, kr, half == 0 ? rv : -db));
         inner = group_sum<64>(inner);
-        if (g == 0) {
-            ends[i] = end, tails[i] = tail;
-            if (here) a.dbeta[scalar_at] = db;
-        }
+        if (g == 0) ends[half][i] = end, tails[half][i] = tail, dbs[half][i] = db;
         if (lane == 0) dots[wave] = inner;
         __syncthreads();
         {
             double s = 0.0;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) s += static_cast<double>(ht[lane * HP + 16 * wave + j]) - static_cast<double>(ht[(16 * wave + j) * HP + lane]);
+            for (int j = 0; j < 16; ++j) s += static_cast<double>(ht[lane * HP + 16 * tile + j]) - static_cast<double>(ht[(16 * tile + j) * HP + lane]);
             across[wave][lane] = s;
         }
         __syncthreads();
-        tile_to_lds<T, DK, KP, 256>(k + static_cast<int64_t>(t0) * a.k.st, a.k.st, n, a.dk, kt);
-        if (BOTH) tile_to_lds<T, DK, KP, 256>(q + static_cast<int64_t>(t0) * a.q.st, a.q.st, n, a.dk, qt);
-        __syncthreads();
+        if (!BOTH) {
+            tile_in<BY, T, DK, KP>(k, a.k.st, n, a.dk, kt);
+            __syncthreads();
+        }
         if (wave == 0) {
-            const double all = static_cast<double>(dots[0]) + dots[1] + dots[2] + dots[3];
-            double t = tails[lane], s = static_cast<double>(ends[lane]) - t + (across[0][lane] + across[1][lane]) + (across[2][lane] + across[3][lane]);
+            double all = 0.0, t = static_cast<double>(tails[0][lane]) + tails[1][lane], s = static_cast<double>(ends[0][lane]) + ends[1][lane] - t;
+#pragma unroll
+            for (int w = 0; w < 8; ++w) all += dots[w], s += across[w][lane];
 #pragma unroll
             for (int o = 32; o >= 1; o >>= 1) t += __shfl_xor(t, o);
             if (lane == 63) s += t + scalars[C - 1] * all;
@@ -302,7 +349,7 @@ __global__ __launch_bounds__(256) void chunk_grads(Rule a, float* sums) {
                 if (lane + o < 64) s += down;
             }
             const int64_t at = (static_cast<int64_t>(b) * a.T + t0 + lane) * a.Hv + h;
-            if (lane < n) a.dg[at] = a.g[at] < LEAST ? 0.0f : static_cast<float>(s);
+            if (lane < n) a.dg[at] = a.g[at] < LEAST ? 0.0f : static_cast<float>(s), a.dbeta[at] = dbs[0][lane] + dbs[1][lane];
         }
         // dQ = scale gamma Y + E K, dK = delta Yu - beta gamma Yr + F K + F^T K + E^T Q
 #pragma unroll
@@ -312,33 +359,33 @@ __global__ __launch_bounds__(256) void chunk_grads(Rule a, float* sums) {
         }
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            const Operand<PE> e = rows_of<PE, C, AP>(et, 16 * wave, 32 * s, lane), f = rows_of<PE, C, AP>(ft, 16 * wave, 32 * s, lane),
-                              ft_ = cols_of<PE, C, AP>(ft, 32 * s, 16 * wave, lane);
+            const Operand<PE> e = rows_of<PE, C, AP>(et, 16 * tile, 32 * s, lane), f = rows_of<PE, C, AP>(ft, 16 * tile, 32 * s, lane),
+                              ft_ = cols_of<PE, C, AP>(ft, 32 * s, 16 * tile, lane);
 #pragma unroll
             for (int d = 0; d < KT; ++d) {
-                const Operand<N> x = cols_of<N, C, KP>(kt, 32 * s, 16 * d, lane);
+                const Operand<N> x = cols_of<N, C, KP>(kt, 32 * s, d_of(d), lane);
                 product<PE - 1>(x, e, Y[d]), product<PE - 1>(x, f, Yu[d]), product<PE - 1>(x, ft_, Yu[d]);
             }
         }
         if (!BOTH) {
             __syncthreads();
-            tile_to_lds<T, DK, KP, 256>(q + static_cast<int64_t>(t0) * a.q.st, a.q.st, n, a.dk, qt);
+            tile_in<BY, T, DK, KP>(q, a.q.st, n, a.dk, qt);
             __syncthreads();
         }
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            const Operand<PE> et_ = cols_of<PE, C, AP>(et, 32 * s, 16 * wave, lane);
+            const Operand<PE> et_ = cols_of<PE, C, AP>(et, 32 * s, 16 * tile, lane);
 #pragma unroll
-            for (int d = 0; d < KT; ++d) product<PE - 1>(cols_of<N, C, KP>(qt, 32 * s, 16 * d, lane), et_, Yu[d]);
+            for (int d = 0; d < KT; ++d) product<PE - 1>(cols_of<N, C, KP>(qt, 32 * s, d_of(d), lane), et_, Yu[d]);
         }
         const bool last = head_v == rep - 1;
-        T *dq = head<T>(a.dq, b, hk) + row * a.dq.st, *dk = head<T>(a.dk_, b, hk) + row * a.dk_.st;
+        T *dq = head<T>(a.dq, b, hk) + (static_cast<int64_t>(t0) + mine_at) * a.dq.st, *dk = head<T>(a.dk_, b, hk) + (static_cast<int64_t>(t0) + mine_at) * a.dk_.st;
 #pragma unroll
         for (int d = 0; d < KT; ++d) {
-            const int c = 16 * d + 4 * g;
+            const int c = d_of(d) + 4 * g;
             if (head_v > 0) Y[d] += *reinterpret_cast<const f32x4*>(mine + c), Yu[d] += *reinterpret_cast<const f32x4*>(mine + C * DK + c);
             if (!last) *reinterpret_cast<f32x4*>(mine + c) = Y[d], *reinterpret_cast<f32x4*>(mine + C * DK + c) = Yu[d];
-            if (last && here) store4(dq, c, a.dk, Y[d]), store4(dk, c, a.dk, Yu[d]);
+            if (last && here) write4<BY>(dq, c, a.dk, Y[d]), write4<BY>(dk, c, a.dk, Yu[d]);
         }
         __syncthreads();  // the next head's columns come where these matrices are
     }
@@ -353,12 +400,12 @@ int launch_back(const Rule& a, hipStream_t st) {
     walk_back<T, DK, VB, BY><<<unit_grid(static_cast<int64_t>(a.B) * a.Hv, blocks(a.dv, VB)), 16 * VB, lds, st>>>(a);
     return launched();
 }
-template <typename T, int DK>
+template <typename T, int DK, Rows BY>
 int launch_grads(const Rule& a, float* sums, hipStream_t st) {
     constexpr size_t lds = grads_lds<T, DK>();
     static_assert(lds <= 156 * 1024, "LDS of a CU");
-    PK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(chunk_grads<T, DK>), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
-    chunk_grads<T, DK><<<dim3(static_cast<unsigned>(static_cast<int64_t>(a.B) * a.Hk * a.chunks)), 256, lds, st>>>(a, sums);
+    PK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(chunk_grads<T, DK, BY>), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
+    chunk_grads<T, DK, BY><<<dim3(static_cast<unsigned>(static_cast<int64_t>(a.B) * a.Hk * a.chunks)), GRAD_NT, lds, st>>>(a, sums);
     return launched();
 }
 template <typename T>
@@ -372,7 +419,10 @@ int launch_backward(const Rule& a, float* sums, int dtype, hipStream_t st) {
         return by_rows(rows_by(a, DK, 16), [&](auto by) { return launch_back<T, DK, 16, decltype(by)::value>(a, st); });
     });
     if (rc || a.chunks == 0) return rc;
-    return by_size(a.dk, [&](auto dk) { return launch_grads<T, decltype(dk)::value>(a, sums, st); });
+    return by_size(a.dk, [&](auto dk) {
+        constexpr int DK = decltype(dk)::value;
+        return by_rows(rows_by(a, DK, GB), [&](auto by) { return launch_grads<T, DK, decltype(by)::value>(a, sums, st); });
+    });
 }
 
 struct Room {
