@@ -8,6 +8,7 @@
 // of two such values is the sum of the six products of parts whose places add up to 2 at most. What is left out is 2^-24 of a term, the rounding that a
 // product in 32 bits has; the matrix cores take 16 such products in the time of one in fp32. Tensors of bf16 are one part, tensors of fp32 three.
 //
+// A matrix instruction runs whatever lanes are switched on, so a branch around one has to be the wavefront's own: wavefront numbers are read into scalars.
 // v_mfma_f32_16x16x32_bf16, lane l = 16 g + c: A row c, k = 8g .. 8g+7; B column c, k = 8g .. 8g+7; C column c, rows 4g .. 4g+3.
 // A and B are alike, so a product is formed in the orientation that its result is wanted in: a lane's four values are neighbours there, in a row of memory or in what LDS keeps
 // for the next product, whose operands are read along k in pieces of 16 bytes. The states in LDS are [columns][rows], R, U and their like [columns][tokens]; only K^T and Q^T are read

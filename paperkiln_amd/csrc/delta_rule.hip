@@ -17,108 +17,161 @@ __device__ inline float decay_of(double x) { return __builtin_amdgcn_exp2f(stati
 __device__ inline double held(float g) { return g < -1000.0f ? -1000.0 : static_cast<double>(g); }
 
 // ---- what does not depend on a state ----
-// A wavefront for a unit's chunk. T by forward substitution, a lane for each of its columns: row i is the unit row less M_ij times the rows j above.
-constexpr int MP = C + 4;
-template <typename T, int DK, int PA, bool BACKWARD>
-__global__ __launch_bounds__(64) void chunk_matrices(Rule a) {
-    constexpr int N = PARTS<T>, MOST = N == 1 ? 0 : 2;
-    __shared__ float m[C * MP];
+// A workgroup for a unit's chunk. T by 16 x 16 blocks: those of the diagonal by forward substitution, a lane for each column and a wavefront for each block, the others by
+// T_ij = -T_ii sum_k M_ik T_kj, one diagonal after the other on the matrix cores. (All 64 rows by substitution are 2016 additions one behind the other: 32 us however few the chunks.)
+constexpr int MP = C + 4, XP = 20;
+template <typename T, int DK, int PA, bool BACKWARD, Rows BY>
+__global__ __launch_bounds__(256) void chunk_matrices(Rule a) {
+    constexpr int N = PARTS<T>, MOST = N == 1 ? 0 : 2, KS = DK / 32;
+    __shared__ float m[C * MP], tt[C * MP];  // M; T transposed
+    __shared__ float xs[3][16 * XP];
     __shared__ double total[C];
-    const int lane = threadIdx.x, g = lane >> 4, c16 = lane & 15;
+    __shared__ float betas[C];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c16 = lane & 15;
     const int64_t unit = blockIdx.x / static_cast<unsigned>(a.chunks);
     const int chunk = blockIdx.x % static_cast<unsigned>(a.chunks), b = static_cast<int>(unit / a.Hv), h = static_cast<int>(unit % a.Hv);
     const int t0 = chunk * C, n = min(C, a.T - t0);
-    const int64_t at = (static_cast<int64_t>(b) * a.T + t0) * a.Hv + h;
-    // the sum of the log-decays
-    double sum = lane < n ? held(a.g[at + static_cast<int64_t>(lane) * a.Hv]) : 0.0;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double up = __shfl_up(sum, o);
-        if (lane >= o) sum += up;
-    }
-    total[lane] = sum;
     const int64_t place = unit * a.chunks + chunk;
-    const float beta = lane < n ? a.beta[at + static_cast<int64_t>(lane) * a.Hv] : 0.0f;
-    float* scalars = a.scalars + place * 3 * C;
-    scalars[lane] = decay_of(sum), scalars[C + lane] = decay_of(__shfl(sum, 63) - sum), scalars[2 * C + lane] = beta;
-    __syncthreads();
     const int hk = h / (a.Hv / a.Hk);
     const T *q = head<const T>(a.q, b, hk) + static_cast<int64_t>(t0) * a.q.st, *k = head<const T>(a.k, b, hk) + static_cast<int64_t>(t0) * a.k.st;
     uint16_t *attn = a.attn + place * PA * (BLOCKS * BLOCK), *attn_t = BACKWARD ? a.attn_t + place * 3 * (BLOCKS * BLOCK) : nullptr;
-#pragma unroll 1
-    for (int it = 0; it < 4; ++it) {
-        const int i = 16 * it + c16, ri = i < n ? i : 0, di = i < n ? a.dk : 0;
-        Operand<N> ki[DK / 32], qi[DK / 32];
+    // wavefront w: rows 16w .. 16w+15 of both products, so the first one, with one tile of them, has time for the sum of the log-decays
+    const int it = wave, i = 16 * it + c16;
+    Eight<BY, T> ki[KS], qi[KS], kj[3][KS];
 #pragma unroll
-        for (int kk = 0; kk < DK / 32; ++kk) ki[kk] = load8(k + ri * a.k.st, 32 * kk + 8 * g, di), qi[kk] = load8(q + ri * a.q.st, 32 * kk + 8 * g, di);
-        const float bi = __shfl(beta, i);
-#pragma unroll 1
-        for (int jt = 0; jt < 4; ++jt) {
-            f32x4 kk4 = {0, 0, 0, 0}, qk4 = kk4, kq4 = kk4;  // rows j, column i; kq4: rows i, column j, transposed
-            if (jt <= it) {
-                const int j = 16 * jt + c16, rj = j < n ? j : 0, dj = j < n ? a.dk : 0;
+    for (int s = 0; s < KS; ++s) {
+        ki[s].load(k, a.k.st, min(i, n - 1), 32 * s + 8 * g, a.dk), qi[s].load(q, a.q.st, min(i, n - 1), 32 * s + 8 * g, a.dk);
 #pragma unroll
-                for (int kk = 0; kk < DK / 32; ++kk) {
-                    const Operand<N> kj = load8(k + rj * a.k.st, 32 * kk + 8 * g, dj);
-                    product<MOST>(kj, ki[kk], kk4), product<MOST>(kj, qi[kk], qk4);
-                    if (BACKWARD) product<MOST>(qi[kk], kj, kq4);
-                }
+        for (int j = 0; j < 3; ++j)
+            if (j < it) kj[j][s].load(k, a.k.st, min(16 * j + c16, n - 1), 32 * s + 8 * g, a.dk);
+    }
+    if (wave == 0) {
+        const int64_t at = (static_cast<int64_t>(b) * a.T + t0 + min(lane, n - 1)) * a.Hv + h;
+        double sum = lane < n ? held(a.g[at]) : 0.0;
+        const float beta = lane < n ? a.beta[at] : 0.0f;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const double up = __shfl_up(sum, o);
+            if (lane >= o) sum += up;
+        }
+        float* scalars = a.scalars + place * 3 * C;
+        total[lane] = sum, betas[lane] = beta;
+        scalars[lane] = decay_of(sum), scalars[C + lane] = decay_of(__shfl(sum, 63) - sum), scalars[2 * C + lane] = beta;
+    }
+    f32x4 kk[4] = {}, qk[4] = {};  // rows j, column i; transposed, qk: rows i, column j
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (j <= it) {
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                const Operand<N> x = j < 3 && j < it ? kj[j < 3 ? j : 0][s].operand() : ki[s].operand(), y = qi[s].operand();
+                product<MOST>(x, ki[s].operand(), kk[j]);
+                if (BACKWARD)
+                    product<MOST>(y, x, qk[j]);
+                else
+                    product<MOST>(x, y, qk[j]);
+            }
+        }
+    __syncthreads();
+    {
+        const float beta = betas[i];
+        const double own = total[i];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int j4 = 16 * j + 4 * g;
+            if (j <= it) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int j = 16 * jt + 4 * g + r;
-                    const float d = j <= i ? decay_of(total[i] - total[j]) : 0.0f;
-                    kk4[r] = j < i ? bi * d * kk4[r] : 0.0f, qk4[r] = j <= i ? a.scale * d * qk4[r] : 0.0f;
+                    const float d = j4 + r <= i ? decay_of(own - total[j4 + r]) : 0.0f;
+                    kk[j][r] = j4 + r < i ? beta * d * kk[j][r] : 0.0f;
                     if (BACKWARD) {
-                        const int row = 16 * it + 4 * g + r, col = 16 * jt + c16;
-                        kq4[r] = col <= row ? a.scale * decay_of(total[row] - total[col]) * kq4[r] : 0.0f;
+                        const int row = 16 * it + 4 * g + r, col = 16 * j + c16;
+                        qk[j][r] = col <= row ? a.scale * decay_of(total[row] - total[col]) * qk[j][r] : 0.0f;
+                    } else {
+                        qk[j][r] = j4 + r <= i ? a.scale * d * qk[j][r] : 0.0f;
                     }
                 }
+                *reinterpret_cast<f32x4*>(m + i * MP + j4) = kk[j];
             }
-            *reinterpret_cast<f32x4*>(m + i * MP + 16 * jt + 4 * g) = kk4;
-            if (!BACKWARD && has_block<false>(i, 16 * jt)) put_block4<PA, false>(attn, i, 16 * jt + 4 * g, qk4);
-            if (BACKWARD && has_block<true>(16 * jt, 16 * it)) put_block4<3, true>(attn_t, 16 * jt + c16, 16 * it + 4 * g, kq4);
+            if (j <= it || (j & 1)) {  // a tile of zeros completes a block
+                if (BACKWARD && (j <= it || j == it + 1))
+                    put_block4<3, true>(attn_t, 16 * j + c16, 16 * it + 4 * g, qk[j]);
+                else if (!BACKWARD && (j <= it || j == it + 1))
+                    put_block4<PA, false>(attn, i, j4, qk[j]);
+            }
         }
     }
     __syncthreads();
-    float t[C];
+    {
+        const float* block = m + 16 * wave * MP + 16 * wave;
+        f32x4 row[16][4];
+        float t[16];
 #pragma unroll
-    for (int i = 0; i < C; ++i) {
-        float s[4] = {i == lane ? 1.0f : 0.0f, 0.0f, 0.0f, 0.0f};
+        for (int i = 1; i < 16; ++i)
 #pragma unroll
-        for (int j = 0; j < i; j += 4) {
-            const f32x4 row = *reinterpret_cast<const f32x4*>(m + i * MP + j);
+            for (int j = 0; j < i; j += 4) row[i][j / 4] = *reinterpret_cast<const f32x4*>(block + i * MP + j);
+        __builtin_amdgcn_sched_barrier(0);  // all rows at once: read where they are wanted each would be waited for
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (j + e < i) s[e] = fmaf(-row[e], t[j + e], s[e]);
+        for (int i = 0; i < 16; ++i) {
+            float s[2] = {i == c16 ? 1.0f : 0.0f, 0.0f};
+#pragma unroll
+            for (int j = 0; j < i; ++j) s[j & 1] = fmaf(-row[i][j / 4][j & 3], t[j], s[j & 1]);
+            t[i] = s[0] + s[1];
         }
-        t[i] = (s[0] + s[1]) + (s[2] + s[3]);
+        if (g == 0) {
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) *reinterpret_cast<f32x4*>(tt + (16 * wave + c16) * MP + 16 * wave + i) = f32x4{t[i], t[i + 1], t[i + 2], t[i + 3]};
+        }
     }
     __syncthreads();
+    const Operand<3> zeros = split8<3>(f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0});
+    const auto eight = [](const float* p) { return split8<3>(*reinterpret_cast<const f32x4*>(p), *reinterpret_cast<const f32x4*>(p + 4)); };
+    const auto down = [](const float* p) { return split8<3>(f32x4{p[0], p[MP], p[2 * MP], p[3 * MP]}, f32x4{p[4 * MP], p[5 * MP], p[6 * MP], p[7 * MP]}); };
 #pragma unroll
-    for (int i = 0; i < C; ++i) m[i * MP + lane] = t[i];
-    __syncthreads();
+    for (int d = 1; d < 4; ++d) {
+        if (wave >= d) {
+            const int it = wave, jt = wave - d;
+            f32x4 sums[3] = {};
+#pragma unroll
+            for (int k0 = 0; k0 < 16 * d; k0 += 32) {
+                const bool in = k0 + 8 * g < 16 * d;  // half of the last step's values of k may be past the sum
+                const int at = 16 * jt + (in ? k0 + 8 * g : 0);
+                const Operand<3> x = eight(m + (16 * it + c16) * MP + at), y = eight(tt + (16 * jt + c16) * MP + at);
+                spread<2>(in ? x : zeros, in ? y : zeros, sums);
+            }
+            float* mine = xs[wave - 1];
+            *reinterpret_cast<f32x4*>(mine + c16 * XP + 4 * g) = gather(sums);
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_wave_barrier();
+            f32x4 more[3] = {};
+            const int at = g < 2 ? 8 * g : 0;
+            const Operand<3> x = down(tt + (16 * it + at) * MP + 16 * it + c16), y = eight(mine + c16 * XP + at);
+            spread<2>(g < 2 ? x : zeros, g < 2 ? y : zeros, more);
+            *reinterpret_cast<f32x4*>(tt + (16 * jt + c16) * MP + 16 * it + 4 * g) = -gather(more);
+        }
+        __syncthreads();
+    }
+    // T, and transposed, a block to a wavefront at a time; what lies past the diagonal's blocks is zero
     uint16_t* out = a.inverse + place * 3 * (BLOCKS * BLOCK);
+    for (int e = wave; e < BLOCKS; e += 4) {
+        const int it = e < 2 ? e : e < 4 ? 2 : 3, kk = e < 2 ? 0 : (e & 1);
+        const bool in = 2 * kk + (g >> 1) <= it;
+        const Operand<3> o = down(tt + (in ? 32 * kk + 8 * g : 0) * MP + 16 * it + c16);
 #pragma unroll
-    for (int it = 0; it < 4; ++it)
-#pragma unroll
-        for (int kk = 0; kk <= it / 2; ++kk) {
-            const float* from = m + (16 * it + c16) * MP + 32 * kk + 8 * g;
-            const Operand<3> o = split8<3>(*reinterpret_cast<const f32x4*>(from), *reinterpret_cast<const f32x4*>(from + 4));
-#pragma unroll
-            for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(out + (p * BLOCKS + block_of<false>(it, kk)) * BLOCK + 8 * lane) = o.part[p];
-        }
+        for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(out + (p * BLOCKS + e) * BLOCK + 8 * lane) = in ? o.part[p] : zeros.part[p];
+    }
     if (!BACKWARD) return;
     out = a.inverse_t + place * 3 * (BLOCKS * BLOCK);
+    for (int e = wave ^ 2; e < BLOCKS; e += 4) {
+        const int it = e < 4 ? e / 2 : e - 2, kk = e < 4 ? (e & 1) : 1;
+        const bool in = 2 * kk + (g >> 1) >= it;
+        const Operand<3> o = eight(tt + (16 * it + c16) * MP + (in ? 32 * kk + 8 * g : 16 * it));
 #pragma unroll
-    for (int it = 0; it < 4; ++it)
-#pragma unroll
-        for (int kk = it / 2; kk < 2; ++kk) {
-            const float* from = m + (32 * kk + 8 * g) * MP + 16 * it + c16;
-            const Operand<3> o = split8<3>(f32x4{from[0], from[MP], from[2 * MP], from[3 * MP]}, f32x4{from[4 * MP], from[5 * MP], from[6 * MP], from[7 * MP]});
-#pragma unroll
-            for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(out + (p * BLOCKS + block_of<true>(it, kk)) * BLOCK + 8 * lane) = o.part[p];
-        }
+        for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(out + (p * BLOCKS + e) * BLOCK + 8 * lane) = in ? o.part[p] : zeros.part[p];
+    }
 }
+static_assert(block_of<false>(1, 0) == 1 && block_of<false>(2, 0) == 2 && block_of<false>(2, 1) == 3 && block_of<false>(3, 0) == 4 && block_of<false>(3, 1) == 5, "the order that T is written in");
+static_assert(block_of<true>(0, 1) == 1 && block_of<true>(1, 0) == 2 && block_of<true>(1, 1) == 3 && block_of<true>(2, 1) == 5 - 1 && block_of<true>(3, 1) == 5, "and transposed");
 
 // ---- the walk down the chunks ----
 // Four wavefronts for each 16 columns: one has 16 of a chunk's tokens, and of the state a quarter of its rows.
@@ -132,7 +185,7 @@ __global__ __launch_bounds__(16 * VB) void walk(Rule a) {
     constexpr int N = PARTS<T>, KP = DK + 16, SP = DK + 8, KS = DK / 32, KT = (DK + 63) / 64, PO = N == 1 ? 2 : 3;  // PO: parts of U and A on their way to O
     extern __shared__ uint16_t lds[];
     uint16_t *kt = lds, *st = kt + (TWO_K<T, DK> ? 2 : 1) * N * C * KP, *rt = st + 3 * VB * SP, *dt = rt + 3 * VB * CP, *ut = dt + 3 * VB * CP;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c16 = lane & 15;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c16 = lane & 15;
     int unit, blk;
     if (!unit_of(blockIdx.x, a.B * a.Hv, (a.dv + VB - 1) / VB, unit, blk)) return;
     const int b = unit / a.Hv, h = unit - b * a.Hv, hk = h / (a.Hv / a.Hk);
@@ -362,14 +415,17 @@ int launch_walk(const Rule& a, hipStream_t st) {
         : by_rows(rows_by(a, DK, 16), [&](auto by) { return launch_walk<T, DK, 16, STATES, decltype(by)::value>(a, st); });
     });
 }
-template <typename T, int DK>
-void launch_matrices(const Rule& a, bool backward, hipStream_t st) {
-    const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.B) * a.Hv * a.chunks));
-    backward ? chunk_matrices<T, DK, 3, true><<<grid, 64, 0, st>>>(a) : chunk_matrices<T, DK, (PARTS<T> == 1 ? 2 : 3), false><<<grid, 64, 0, st>>>(a);
-}
 template <typename T>
-void launch_matrices(const Rule& a, bool backward, hipStream_t st) {
-    a.dk <= 32 ? launch_matrices<T, 32>(a, backward, st) : a.dk <= 64 ? launch_matrices<T, 64>(a, backward, st) : launch_matrices<T, 128>(a, backward, st);
+int launch_matrices(const Rule& a, bool backward, hipStream_t st) {
+    return by_size(a.dk, [&](auto dk) {
+        constexpr int DK = decltype(dk)::value;
+        const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.B) * a.Hv * a.chunks));
+        return by_rows(rows_by(a, DK, 1), [&](auto by) {
+            constexpr Rows BY = decltype(by)::value;
+            backward ? chunk_matrices<T, DK, 3, true, BY><<<grid, 256, 0, st>>>(a) : chunk_matrices<T, DK, (PARTS<T> == 1 ? 2 : 3), false, BY><<<grid, 256, 0, st>>>(a);
+            return launched();
+        });
+    });
 }
 template <typename T>
 void launch_steps(const Rule& a, hipStream_t st) {
@@ -394,8 +450,7 @@ Room room_of(const pk_delta_shape* s) {
 }  // namespace
 
 int launch_chunks(const Rule& a, int dtype, bool backward, hipStream_t st) {
-    dtype == PK_BF16 ? launch_matrices<uint16_t>(a, backward, st) : launch_matrices<float>(a, backward, st);
-    return launched();
+    return dtype == PK_BF16 ? launch_matrices<uint16_t>(a, backward, st) : launch_matrices<float>(a, backward, st);
 }
 int launch_states(const Rule& a, int dtype, hipStream_t st) { return dtype == PK_BF16 ? launch_walk<uint16_t, true>(a, st) : launch_walk<float, true>(a, st); }
 

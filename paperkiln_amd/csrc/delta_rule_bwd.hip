@@ -34,7 +34,7 @@ __global__ __launch_bounds__(16 * VB) void walk_back(Rule a) {
     constexpr int N = PARTS<T>, KP = DK + 16, SP = DK + 8, KS = DK / 32, KT = (DK + 63) / 64;
     extern __shared__ uint16_t lds[];
     uint16_t *kt = lds, *qt = kt + (TWO_K<DK> ? 2 : 1) * N * C * KP, *st = qt + N * C * KP, *ut = st + 3 * VB * SP, *wt = ut + 3 * VB * CP, *dt = wt + 3 * VB * CP, *rt = dt + 3 * VB * CP;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c16 = lane & 15;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c16 = lane & 15;
     int unit, blk;
     if (!unit_of(blockIdx.x, a.B * a.Hv, (a.dv + VB - 1) / VB, unit, blk)) return;
     const int b = unit / a.Hv, h = unit - b * a.Hv, hk = h / (a.Hv / a.Hk);
@@ -185,7 +185,7 @@ __global__ __launch_bounds__(GRAD_NT, 2) void chunk_grads(Rule a, float* sums) {
     uint16_t *kt = lds, *qt = BOTH ? kt + tile_size<T, DK>() : kt, *s0 = BOTH ? qt + tile_size<T, DK>() : lds;
     uint16_t *s1 = s0 + 3 * DK * VQ, *ut = s1 + 3 * DK * VQ;                                                          // while the columns of the state go by
     uint16_t *hs = BOTH ? s0 : s0 + tile_size<T, DK>(), *et = hs + 4 * C * HP, *ft = et + PE * C * AP;  // then
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, tile = wave & 3, half = wave >> 2, g = lane >> 4, c16 = lane & 15, i = 16 * tile + c16;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), tile = wave & 3, half = wave >> 2, g = lane >> 4, c16 = lane & 15, i = 16 * tile + c16;
     float* ht = reinterpret_cast<float*>(hs) + half * C * HP;
     const int64_t group = blockIdx.x / static_cast<unsigned>(a.chunks);
     const int chunk = blockIdx.x % static_cast<unsigned>(a.chunks), b = static_cast<int>(group / a.Hk), hk = static_cast<int>(group % a.Hk), rep = a.Hv / a.Hk;
