@@ -387,6 +387,9 @@ template <typename F>
 int by_size(int dk, F&& f) {
     return dk <= 32 ? f(std::integral_constant<int, 32>{}) : dk <= 64 ? f(std::integral_constant<int, 64>{}) : f(std::integral_constant<int, 128>{});
 }
+// Columns to a workgroup of a walk: 32 where that many workgroups fill the chip, and a unit's matrices, q and k are then fetched half as often; else 16, a chunk of which takes half
+// the time.
+inline bool wide(const Rule& a) { return static_cast<int64_t>(a.B) * a.Hv * blocks(a.dv, 32) >= 256; }
 // Workgroups of one unit go to one XCD, whose L2 then has the unit's q, k and matrices for all of its blocks. Launch with grid.x = unit_grid.
 inline unsigned unit_grid(int64_t units, int per) { return static_cast<unsigned>((units + 7) / 8 * 8 * per); }
 __device__ inline bool unit_of(int id, int units, int per, int& unit, int& blk) {

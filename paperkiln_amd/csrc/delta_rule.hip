@@ -6,7 +6,6 @@
 // head's state: the columns do not know of one another. What bounds the walk is its own chain: three products and three exchanges through LDS a chunk.
 // Token by token, the state in registers, memory bounds it: the state read and written once.
 #include "delta_rule.h"
-#include <cstdlib>
 
 namespace pk {
 namespace delta {
@@ -21,7 +20,7 @@ __device__ inline double held(float g) { return g < -1000.0f ? -1000.0 : static_
 // T_ij = -T_ii sum_k M_ik T_kj, one diagonal after the other on the matrix cores. (All 64 rows by substitution are 2016 additions one behind the other: 32 us however few the chunks.)
 constexpr int MP = C + 4, XP = 20;
 template <typename T, int DK, int PA, bool BACKWARD, Rows BY>
-__global__ __launch_bounds__(256) void chunk_matrices(Rule a) {
+__global__ __launch_bounds__(256, PARTS<T> == 1 ? 4 : 2) void chunk_matrices(Rule a) {
     constexpr int N = PARTS<T>, MOST = N == 1 ? 0 : 2, KS = DK / 32;
     __shared__ float m[C * MP], tt[C * MP];  // M; T transposed
     __shared__ float xs[3][16 * XP];
@@ -106,18 +105,29 @@ __global__ __launch_bounds__(256) void chunk_matrices(Rule a) {
         const float* block = m + 16 * wave * MP + 16 * wave;
         f32x4 row[16][4];
         float t[16];
+        const auto read = [&](auto from, auto to) {  // rows one behind the other would each be waited for
 #pragma unroll
-        for (int i = 1; i < 16; ++i)
+            for (int i = decltype(from)::value; i < decltype(to)::value; ++i)
 #pragma unroll
-            for (int j = 0; j < i; j += 4) row[i][j / 4] = *reinterpret_cast<const f32x4*>(block + i * MP + j);
-        __builtin_amdgcn_sched_barrier(0);  // all rows at once: read where they are wanted each would be waited for
+                for (int j = 0; j < i; j += 4) row[i][j / 4] = *reinterpret_cast<const f32x4*>(block + i * MP + j);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        const auto solve = [&](auto from, auto to) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            float s[2] = {i == c16 ? 1.0f : 0.0f, 0.0f};
+            for (int i = decltype(from)::value; i < decltype(to)::value; ++i) {
+                float s[2] = {i == c16 ? 1.0f : 0.0f, 0.0f};
 #pragma unroll
-            for (int j = 0; j < i; ++j) s[j & 1] = fmaf(-row[i][j / 4][j & 3], t[j], s[j & 1]);
-            t[i] = s[0] + s[1];
-        }
+                for (int j = 0; j < i; ++j) s[j & 1] = fmaf(-row[i][j / 4][j & 3], t[j], s[j & 1]);
+                t[i] = s[0] + s[1];
+            }
+        };
+        using std::integral_constant;
+        read(integral_constant<int, 1>{}, integral_constant<int, 9>{});
+        solve(integral_constant<int, 0>{}, integral_constant<int, 5>{});
+        read(integral_constant<int, 9>{}, integral_constant<int, 13>{});
+        solve(integral_constant<int, 5>{}, integral_constant<int, 9>{});
+        read(integral_constant<int, 13>{}, integral_constant<int, 16>{});
+        solve(integral_constant<int, 9>{}, integral_constant<int, 16>{});
         if (g == 0) {
 #pragma unroll
             for (int i = 0; i < 16; i += 4) *reinterpret_cast<f32x4*>(tt + (16 * wave + c16) * MP + 16 * wave + i) = f32x4{t[i], t[i + 1], t[i + 2], t[i + 3]};
@@ -411,8 +421,8 @@ template <typename T, bool STATES>
 int launch_walk(const Rule& a, hipStream_t st) {
     return by_size(a.dk, [&](auto dk) {
         constexpr int DK = decltype(dk)::value;
-        return getenv("PK_VB32") ? by_rows(rows_by(a, DK, 32), [&](auto by) { return launch_walk<T, DK, 32, STATES, decltype(by)::value>(a, st); })
-        : by_rows(rows_by(a, DK, 16), [&](auto by) { return launch_walk<T, DK, 16, STATES, decltype(by)::value>(a, st); });
+        if (wide(a)) return by_rows(rows_by(a, DK, 32), [&](auto by) { return launch_walk<T, DK, 32, STATES, decltype(by)::value>(a, st); });
+        return by_rows(rows_by(a, DK, 16), [&](auto by) { return launch_walk<T, DK, 16, STATES, decltype(by)::value>(a, st); });
     });
 }
 template <typename T>

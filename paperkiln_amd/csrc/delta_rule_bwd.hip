@@ -416,6 +416,8 @@ int launch_backward(const Rule& a, float* sums, int dtype, hipStream_t st) {
     }
     const int rc = by_size(a.dk, [&](auto dk) {
         constexpr int DK = decltype(dk)::value;
+        if constexpr (back_lds<T, DK, 32>() <= 160 * 1024)
+            if (wide(a)) return by_rows(rows_by(a, DK, 32), [&](auto by) { return launch_back<T, DK, 32, decltype(by)::value>(a, st); });
         return by_rows(rows_by(a, DK, 16), [&](auto by) { return launch_back<T, DK, 16, decltype(by)::value>(a, st); });
     });
     if (rc || a.chunks == 0) return rc;

@@ -151,7 +151,10 @@ DELTAS = [  # B, T, Hk, Hv, dk, dv, layout, state
     (1, 1, 1, 1, 1, 1, "plain", True), (2, 1, 2, 4, 64, 64, "plain", True), (1, 2, 1, 1, 3, 5, "plain", False), (2, 15, 2, 2, 32, 32, "fused", True), (3, 16, 1, 3, 40, 72, "heads", False),
     (2, 17, 2, 2, 64, 64, "plain", True), (1, 63, 1, 1, 128, 128, "plain", True), (2, 64, 3, 3, 64, 128, "heads", True), (1, 65, 2, 6, 48, 80, "offset", True),
     (2, 130, 1, 7, 64, 64, "fused", False), (1, 200, 2, 2, 128, 256, "plain", True), (1, 257, 1, 2, 127, 33, "offset", False), (3, 100, 2, 2, 16, 8, "plain", True),
-    (1, 300, 3, 3, 33, 31, "heads", True), (9, 70, 1, 1, 96, 96, "fused", True), (1, 500, 1, 1, 31, 1, "plain", True), (1, 129, 1, 2, 1, 255, "offset", True)]
+    (1, 300, 3, 3, 33, 31, "heads", True), (9, 70, 1, 1, 96, 96, "fused", True), (1, 500, 1, 1, 31, 1, "plain", True), (1, 129, 1, 2, 1, 255, "offset", True),
+    # heads enough for workgroups of 32 columns: whole blocks, rows of whole pieces, any
+    (32, 100, 4, 8, 32, 64, "fused", True), (16, 130, 16, 16, 64, 32, "heads", False), (9, 70, 8, 32, 128, 32, "plain", True), (40, 75, 2, 8, 24, 40, "plain", True),
+    (70, 66, 1, 4, 96, 16, "fused", False), (64, 90, 2, 4, 31, 17, "offset", True), (64, 65, 2, 4, 101, 9, "plain", False)]
 
 
 @pytest.mark.parametrize("dtype", [FP32, BF16], ids=["fp32", "bf16"])
