@@ -20,7 +20,7 @@ __device__ inline double held(float g) { return g < -1000.0f ? -1000.0 : static_
 // T_ij = -T_ii sum_k M_ik T_kj, one diagonal after the other on the matrix cores. (All 64 rows by substitution are 2016 additions one behind the other: 32 us however few the chunks.)
 constexpr int MP = C + 4, XP = 20;
 template <typename T, int DK, int PA, bool BACKWARD, Rows BY>
-__global__ __launch_bounds__(256, PARTS<T> == 1 ? 4 : 2) void chunk_matrices(Rule a) {
+__global__ __launch_bounds__(256, PARTS<T> == 1 ? 3 : 2) void chunk_matrices(Rule a) {
     constexpr int N = PARTS<T>, MOST = N == 1 ? 0 : 2, KS = DK / 32;
     __shared__ float m[C * MP], tt[C * MP];  // M; T transposed
     __shared__ float xs[3][16 * XP];

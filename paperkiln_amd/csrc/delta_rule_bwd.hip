@@ -177,7 +177,7 @@ __device__ inline float over_groups(float x) {  // the four lanes of a token
 template <typename T, int DK, Rows BY>
 __global__ __launch_bounds__(GRAD_NT, 2) void chunk_grads(Rule a, float* sums) {
     constexpr int N = PARTS<T>, MOST = N == 1 ? 0 : 2, PE = N == 1 ? 2 : 3, KP = DK + 16, KS = DK / 32, KT = DK / 32, SN = (DK * (GB / 4) + GRAD_NT - 1) / GRAD_NT;
-    constexpr bool BOTH = BESIDE<T, DK>;
+    constexpr bool BOTH = BESIDE<T, DK>, AHEAD = BOTH || BY != ANY;  // with everything held the loads ahead of rows of any size would not fit into the registers
     extern __shared__ uint16_t lds[];
     __shared__ double total[C];
     __shared__ double across[8][C];
@@ -192,7 +192,7 @@ __global__ __launch_bounds__(GRAD_NT, 2) void chunk_grads(Rule a, float* sums) {
     const int t0 = chunk * C, n = min(C, a.T - t0), mine_at = min(i, n - 1);  // a token behind the last one reads its row and counts for nothing
     const bool here = i < n;
     const T *q = head<const T>(a.q, b, hk) + static_cast<int64_t>(t0) * a.q.st, *k = head<const T>(a.k, b, hk) + static_cast<int64_t>(t0) * a.k.st;
-    float* mine = rep > 1 ? sums + static_cast<int64_t>(blockIdx.x) * 2 * C * DK + i * DK : nullptr;  // what the heads of v before have given to dQ's and dK's rows
+    float* rows = sums + static_cast<int64_t>(blockIdx.x) * 2 * C * DK;  // what the heads of v before have given to dQ's and dK's rows, where there are several
     if (BOTH) tile_in<BY, T, DK, KP>(k, a.k.st, n, a.dk, kt), tile_in<BY, T, DK, KP>(q, a.q.st, n, a.dk, qt);
     const auto d_of = [&](int d) { return 16 * (half * KT + d); };
     for (int head_v = 0; head_v < rep; ++head_v) {
@@ -245,7 +245,7 @@ __global__ __launch_bounds__(GRAD_NT, 2) void chunk_grads(Rule a, float* sums) {
             const Operand<3> dr = split8<3>(r0, r1);
             const Operand<N> od = dov.operand();
             __syncthreads();
-            if (v0 + GB < a.dv) load(v0 + GB);
+            if (AHEAD && v0 + GB < a.dv) load(v0 + GB);
             const Operand<3> ui = rows_of<3, C, VQ>(ut, 16 * tile, 0, lane);
 #pragma unroll
             for (int j = 0; j < 4; ++j)
@@ -262,58 +262,71 @@ __global__ __launch_bounds__(GRAD_NT, 2) void chunk_grads(Rule a, float* sums) {
                 const Operand<3> s = rows_of<3, DK, VQ>(s0, d_of(d), 0, lane), t = rows_of<3, DK, VQ>(s1, d_of(d), 0, lane);
                 product<2>(s, od, Y[d]), product<2>(s, dr, Yr[d]), product<2>(t, ui, Yu[d]);
             }
+            if (!AHEAD && v0 + GB < a.dv) load(v0 + GB);
             __syncthreads();
         }
+        // Addresses from here on are formed of numbers that the compiler cannot know: formed before the columns go by, they would be held, or spilled, through all of that.
+        int lane_then = lane, i_then = i, mine_then = mine_at;
+        asm volatile("" : "+v"(lane_then), "+v"(i_then), "+v"(mine_then));
         const float* scalars = a.scalars + place * 3 * C;
-        const float2 decay = make_float2(scalars[i], scalars[C + i]);
-        const float beta = scalars[2 * C + i];
+        const float2 decay = make_float2(scalars[i_then], scalars[C + i_then]);
+        const float beta = scalars[2 * C + i_then];
         // E and F, and what they give to dbeta and to the decays
         float db = 0.0f;
         {
+            const int g = lane_then >> 4, c16 = lane_then & 15, i = i_then;
             // rows of K and Q as operands: from LDS, or from memory
             const auto row_k = [&](int j, int s) {
-                if constexpr (BOTH) return rows_of<N, C, KP>(kt, 16 * j, 32 * s, lane);
+                if constexpr (BOTH) return rows_of<N, C, KP>(kt, 16 * j, 32 * s, lane_then);
                 Eight<BY, T> e;
                 e.load(k, a.k.st, min(16 * j + c16, n - 1), 32 * s + 8 * g, a.dk);
                 return e.operand();
             };
             const auto row_own = [&](int s) {
-                if constexpr (BOTH) return rows_of<N, C, KP>(half == 0 ? qt : kt, 16 * tile, 32 * s, lane);
+                if constexpr (BOTH) return rows_of<N, C, KP>(half == 0 ? qt : kt, 16 * tile, 32 * s, lane_then);
                 Eight<BY, T> e;
                 if (half == 0)
-                    e.load(q, a.q.st, mine_at, 32 * s + 8 * g, a.dk);
+                    e.load(q, a.q.st, mine_then, 32 * s + 8 * g, a.dk);
                 else
-                    e.load(k, a.k.st, mine_at, 32 * s + 8 * g, a.dk);
+                    e.load(k, a.k.st, mine_then, 32 * s + 8 * g, a.dk);
                 return e.operand();
             };
             const float factor = half == 0 ? a.scale : -beta;
+            f32x4 xk[4] = {};
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                __builtin_amdgcn_sched_barrier(0);
+                const Operand<N> own = row_own(s);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (j <= tile) product<MOST>(row_k(j, s), own, xk[j]);
+            }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                f32x4 xk = {0, 0, 0, 0}, H = xk;
+                f32x4 H = {0, 0, 0, 0};
                 if (j <= tile) {
-#pragma unroll
-                    for (int s = 0; s < KS; ++s) product<MOST>(row_k(j, s), row_own(s), xk);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const int at = 16 * j + 4 * g + r;
                         const float D = here && (half == 0 ? at <= i : at < i) ? decay_of(total[i] - total[at]) : 0.0f, z = D == 0.0f ? 0.0f : D * X[j][r];
                         X[j][r] = factor * z;
-                        H[r] = at < i ? X[j][r] * xk[r] : 0.0f;
-                        db = fmaf(z, xk[r], db);
+                        H[r] = at < i ? X[j][r] * xk[j][r] : 0.0f;
+                        db = fmaf(z, xk[j][r], db);
                     }
                 }
                 put4<PE, C, AP>(half == 0 ? et : ft, i, 16 * j + 4 * g, X[j]);
                 *reinterpret_cast<f32x4*>(ht + i * HP + 16 * j + 4 * g) = H;
             }
         }
+        const int g4 = lane_then >> 4 << 2;
         float qy = 0.0f, kr = 0.0f, ku = 0.0f;
 #pragma unroll
         for (int d = 0; d < KT; ++d) {
             f32x4 xq, xk;
             if constexpr (N == 1) {
-                xq = load4(qt + i * KP, d_of(d) + 4 * g, DK), xk = load4(kt + i * KP, d_of(d) + 4 * g, DK);
+                xq = load4(qt + i_then * KP, d_of(d) + g4, DK), xk = load4(kt + i_then * KP, d_of(d) + g4, DK);
             } else {
-                xq = load4(q + mine_at * a.q.st, d_of(d) + 4 * g, a.dk), xk = load4(k + mine_at * a.k.st, d_of(d) + 4 * g, a.dk);
+                xq = load4(q + mine_then * a.q.st, d_of(d) + g4, a.dk), xk = load4(k + mine_then * a.k.st, d_of(d) + g4, a.dk);
             }
 #pragma unroll
             for (int r = 0; r < 4; ++r) qy = fmaf(xq[r], Y[d][r], qy), kr = fmaf(xk[r], Yr[d][r], kr), ku = fmaf(xk[r], Yu[d][r], ku);
@@ -348,7 +361,7 @@ __global__ __launch_bounds__(GRAD_NT, 2) void chunk_grads(Rule a, float* sums) {
                 const double down = __shfl_down(s, o);
                 if (lane + o < 64) s += down;
             }
-            const int64_t at = (static_cast<int64_t>(b) * a.T + t0 + lane) * a.Hv + h;
+            const int64_t at = (static_cast<int64_t>(b) * a.T + t0 + lane_then) * a.Hv + h;
             if (lane < n) a.dg[at] = a.g[at] < LEAST ? 0.0f : static_cast<float>(s), a.dbeta[at] = dbs[0][lane] + dbs[1][lane];
         }
         // dQ = scale gamma Y + E K, dK = delta Yu - beta gamma Yr + F K + F^T K + E^T Q
@@ -359,11 +372,11 @@ __global__ __launch_bounds__(GRAD_NT, 2) void chunk_grads(Rule a, float* sums) {
         }
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            const Operand<PE> e = rows_of<PE, C, AP>(et, 16 * tile, 32 * s, lane), f = rows_of<PE, C, AP>(ft, 16 * tile, 32 * s, lane),
-                              ft_ = cols_of<PE, C, AP>(ft, 32 * s, 16 * tile, lane);
+            const Operand<PE> e = rows_of<PE, C, AP>(et, 16 * tile, 32 * s, lane_then), f = rows_of<PE, C, AP>(ft, 16 * tile, 32 * s, lane_then),
+                              ft_ = cols_of<PE, C, AP>(ft, 32 * s, 16 * tile, lane_then);
 #pragma unroll
             for (int d = 0; d < KT; ++d) {
-                const Operand<N> x = cols_of<N, C, KP>(kt, 32 * s, d_of(d), lane);
+                const Operand<N> x = cols_of<N, C, KP>(kt, 32 * s, d_of(d), lane_then);
                 product<PE - 1>(x, e, Y[d]), product<PE - 1>(x, f, Yu[d]), product<PE - 1>(x, ft_, Yu[d]);
             }
         }
@@ -374,15 +387,16 @@ __global__ __launch_bounds__(GRAD_NT, 2) void chunk_grads(Rule a, float* sums) {
         }
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            const Operand<PE> et_ = cols_of<PE, C, AP>(et, 32 * s, 16 * tile, lane);
+            const Operand<PE> et_ = cols_of<PE, C, AP>(et, 32 * s, 16 * tile, lane_then);
 #pragma unroll
-            for (int d = 0; d < KT; ++d) product<PE - 1>(cols_of<N, C, KP>(qt, 32 * s, d_of(d), lane), et_, Yu[d]);
+            for (int d = 0; d < KT; ++d) product<PE - 1>(cols_of<N, C, KP>(qt, 32 * s, d_of(d), lane_then), et_, Yu[d]);
         }
         const bool last = head_v == rep - 1;
-        T *dq = head<T>(a.dq, b, hk) + (static_cast<int64_t>(t0) + mine_at) * a.dq.st, *dk = head<T>(a.dk_, b, hk) + (static_cast<int64_t>(t0) + mine_at) * a.dk_.st;
+        float* mine = rows + i_then * DK;
+        T *dq = head<T>(a.dq, b, hk) + (static_cast<int64_t>(t0) + mine_then) * a.dq.st, *dk = head<T>(a.dk_, b, hk) + (static_cast<int64_t>(t0) + mine_then) * a.dk_.st;
 #pragma unroll
         for (int d = 0; d < KT; ++d) {
-            const int c = d_of(d) + 4 * g;
+            const int c = d_of(d) + g4;
             if (head_v > 0) Y[d] += *reinterpret_cast<const f32x4*>(mine + c), Yu[d] += *reinterpret_cast<const f32x4*>(mine + C * DK + c);
             if (!last) *reinterpret_cast<f32x4*>(mine + c) = Y[d], *reinterpret_cast<f32x4*>(mine + C * DK + c) = Yu[d];
             if (last && here) write4<BY>(dq, c, a.dk, Y[d]), write4<BY>(dk, c, a.dk, Yu[d]);
