@@ -30,71 +30,100 @@ struct Distill {
     float upstream;
 };
 
-// The teacher's side of a row, `top` values each in LDS: a slot's word, the student's logit there, the teacher's logit and later its probability.
+// The teacher's side of a row in LDS: a slot's word, the student's logit there, the teacher's logit and its probability. Four arrays of whole 16 bytes; what completes them is empty.
 struct Slots {
     int* at;
-    float *z, *p;
+    float *z, *t, *p;
+    int count;
 };
-__device__ inline Slots slots_in(float* lds, int top) { return Slots{reinterpret_cast<int*>(lds), lds + top, lds + 2 * top}; }
-
-template <typename T>
-__device__ inline void read_slots(const Distill& a, int64_t r, const T* x, const Slots& s, int n) {
-    for (int k = threadIdx.x; k < a.top; k += n) {
-        const int i = a.indices[r * a.top + k];
-        s.at[k] = i;
-        s.z[k] = i < 0 ? 0.0f : i < a.vocab ? elem(x, i) : NAN;  // a word that is none has no probability
-        s.p[k] = a.teacher[r * a.top + k];
-    }
+__host__ __device__ constexpr int pitch_of(int top) { return (top + 3) & ~3; }
+__device__ inline Slots slots_in(float* lds, int top) {
+    const int n = pitch_of(top);
+    return Slots{reinterpret_cast<int*>(lds), lds + n, lds + 2 * n, lds + 3 * n, n};
 }
-struct Row {
-    float top, per_sum, coef, sum_p;  // coef: upstream w tau; 0 where there is nothing to learn from the row
-    __device__ float power(float x, float s2) const { return __builtin_amdgcn_exp2f((x - top) * s2); }
+// A thread's first slot, asked for before the row is: the teacher's part is done while the row is on its way.
+struct Slot {
+    int at;
+    float t;
+};
+__device__ inline Slot slot(const Distill& a, int64_t r, int k) { return k < a.top ? Slot{a.indices[r * a.top + k], a.teacher[r * a.top + k]} : Slot{-1, 0.0f}; }
+// The words and logits of the teacher, and the student's logits but for the first slots', which are the result.
+template <typename T>
+__device__ inline float put_slots(const Distill& a, int64_t r, const T* x, const Slots& s, Slot first, int n) {
+    const auto logit = [&](int i) { return i < 0 ? 0.0f : i < a.vocab ? elem(x, i) : NAN; };  // a word that is none has no probability
+    const int k0 = threadIdx.x;
+    if (k0 < s.count) s.at[k0] = first.at, s.t[k0] = first.t;
+    for (int k = k0 + n; k < s.count; k += n) {
+        const Slot o = slot(a, r, k);
+        s.at[k] = o.at, s.t[k] = o.t, s.z[k] = logit(o.at);
+    }
+    return logit(first.at);
+}
+// What a row's gradient needs of its teacher.
+struct Teacher {
+    double lse;
+    float mass;  // the sum of the slots' probabilities
+    int words;   // 0: there is nothing to learn from the row
 };
 __device__ inline double wave_max(double x) {
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) x = fmax(x, __shfl_xor(x, o));
     return x;
 }
-// A wavefront: the slots' probabilities in place of the teacher's logits, the row's loss, and what its gradient is made of. Every lane has the same.
-__device__ inline Row finish(const Distill& a, int64_t r, const Slots& s, const RowSum& sum) {
+// A wavefront: the slots' probabilities. Every lane has the result.
+__device__ inline Teacher teacher_of(const Distill& a, int64_t r, const Slots& s) {
     const int lane = threadIdx.x & 63;
     const double per = a.per_tau;
-    double lse;
     int words = 0;
-    for (int k = lane; k < a.top; k += 64) words += s.at[k] >= 0;
-    if (!__ballot(words != 0)) {
-        if (lane == 0) a.kl[r] = 0.0f, a.row_loss[r] = 0.0;
-        return Row{0.0f, 0.0f, 0.0f, 0.0f};
-    }
+    for (int k = lane; k < s.count; k += 64) words += s.at[k] >= 0;
+    if (!__ballot(words != 0)) return Teacher{0.0, 0.0f, 0};
+    double lse;
     if (a.teacher_lse) {
         lse = a.teacher_lse[r];
     } else {
         double high = -INFINITY, all = 0.0;
-        for (int k = lane; k < a.top; k += 64)
-            if (s.at[k] >= 0) high = fmax(high, s.p[k] * per);
+        for (int k = lane; k < s.count; k += 64)
+            if (s.at[k] >= 0) high = fmax(high, s.t[k] * per);
         high = wave_max(high);
-        for (int k = lane; k < a.top; k += 64)
-            if (s.at[k] >= 0) all += exp(s.p[k] * per - high);
+        for (int k = lane; k < s.count; k += 64)
+            if (s.at[k] >= 0) all += exp(s.t[k] * per - high);
         lse = high + log(lanes_sum(all));  // no slot with a probability: no number
     }
-    double kl = 0.0, mass = 0.0;
-    for (int k = lane; k < a.top; k += 64) {
-        double p = 0.0;
-        if (s.at[k] >= 0) {
-            const double logp = s.p[k] * per - lse, logq = ((static_cast<double>(s.z[k]) - static_cast<double>(sum.top)) * a.s2 - sum.log2) * LN2;
-            p = exp(logp);
-            if (p != 0.0) kl += p * (logp - logq);  // a word that the teacher rules out adds nothing, also where the student does
-        }
+    double mass = 0.0;
+    for (int k = lane; k < s.count; k += 64) {
+        const double p = s.at[k] >= 0 ? exp(s.t[k] * per - lse) : 0.0;
         s.p[k] = static_cast<float>(p);
         mass += p;
     }
-    kl = lanes_sum(kl), mass = lanes_sum(mass);
-    const double w = a.weights[r], tau = a.tau;
+    return Teacher{lse, static_cast<float>(lanes_sum(mass)), 1};
+}
+// A wavefront, when the row is known: its loss. The probabilities are formed again in 64 bits, since the loss is a difference.
+__device__ inline void finish(const Distill& a, int64_t r, const Slots& s, const Teacher& t, const RowTotal& total) {
+    const int lane = threadIdx.x & 63;
+    double kl = 0.0;
+    if (t.words) {
+        const RowSum sum = row_sum(total.top, total.sum);
+        for (int k = lane; k < s.count; k += 64)
+            if (s.at[k] >= 0) {
+                const double logp = s.t[k] * a.per_tau - t.lse, logq = ((static_cast<double>(s.z[k]) - static_cast<double>(sum.top)) * a.s2 - sum.log2) * LN2;
+                const double p = exp(logp);
+                if (p != 0.0) kl += p * (logp - logq);  // a word that the teacher rules out adds nothing, also where the student does
+            }
+        kl = lanes_sum(kl);
+    }
     if (lane == 0) {
         a.kl[r] = static_cast<float>(kl);
-        a.row_loss[r] = w * tau * tau * kl;
+        a.row_loss[r] = t.words ? a.weights[r] * a.tau * a.tau * kl : 0.0;
     }
-    return Row{sum.top, static_cast<float>(exp2(-sum.log2)), static_cast<float>(w * tau * a.upstream), static_cast<float>(mass)};
+}
+struct Row {
+    float top, coef, even;  // coef: upstream w tau, 0 where there is nothing to learn from the row; even: what every word's probability is multiplied by
+    __device__ float power(float x, float s2) const { return __builtin_amdgcn_exp2f((x - top) * s2); }
+};
+__device__ inline Row row_of(const Distill& a, double w, float mass, int words, const RowTotal& t) {
+    if (!words) return Row{0.0f, 0.0f, 0.0f};
+    const float coef = static_cast<float>(w * a.tau * a.upstream), per_sum = t.sum == 0.0 ? NAN : static_cast<float>(1.0 / t.sum);
+    return Row{t.top, coef, mass * per_sum};
 }
 // The teacher's words written over, by the threads of a workgroup. A word that several slots name gets all of theirs, from each of them the same value.
 template <typename T>
@@ -103,8 +132,12 @@ __device__ inline void write_slots(const Distill& a, T* dx, const Slots& s, cons
         const int i = s.at[k];
         if (i < 0 || i >= a.vocab) continue;
         float p = 0.0f;
-        for (int j = 0; j < a.top; ++j) p += s.at[j] == i ? s.p[j] : 0.0f;
-        put(dx, i, o.coef * fmaf(o.sum_p * o.per_sum, o.power(s.z[k], s2), -p));
+        for (int j = 0; j < s.count; j += 4) {
+            const int4 at = *reinterpret_cast<const int4*>(s.at + j);
+            const float4 more = *reinterpret_cast<const float4*>(s.p + j);
+            p += at.x == i ? more.x : 0.0f, p += at.y == i ? more.y : 0.0f, p += at.z == i ? more.z : 0.0f, p += at.w == i ? more.w : 0.0f;
+        }
+        put(dx, i, o.coef * fmaf(o.even, o.power(s.z[k], s2), -p));
     }
 }
 
@@ -114,15 +147,18 @@ __global__ __launch_bounds__(ROW_NT) void distill_held(Distill a) {
     constexpr int WAVES = ROW_NT / 64, N = Piece<T>::N;
     __shared__ float sh_m[WAVES];
     __shared__ double sh_s[WAVES];
-    __shared__ Row sh_o;
-    extern __shared__ float lds[];
+    __shared__ float sh_mass;
+    __shared__ int sh_words;
+    extern __shared__ __attribute__((aligned(16))) float lds[];
     const Slots slots = slots_in(lds, a.top);
     const int64_t r = blockIdx.x;
     const int tid = threadIdx.x, V = a.vocab;
     const T* x = static_cast<const T*>(a.logits) + r * a.ld;
     T* dx = GRAD ? static_cast<T*>(a.dlogits) + r * a.dld : nullptr;
     const Cut<T> cut(x, V);
-    if (a.weights[r] == 0.0f) {
+    const Slot mine = slot(a, r, tid);
+    const float w = a.weights[r];
+    if (w == 0.0f) {
         if (tid == 0) a.kl[r] = 0.0f, a.row_loss[r] = 0.0;
         if (GRAD) zero_row<T, ROW_NT, PAST>(dx, cut, tid);
         return;
@@ -134,7 +170,14 @@ __global__ __launch_bounds__(ROW_NT) void distill_held(Distill a) {
         held[k] = p < cut.pieces ? load_piece<PAST>(x + cut.head + p * N) : Piece<T>::nothing();
     }
     const float edge = tid < cut.edges ? elem(x, cut.edge(tid)) : -INFINITY;
-    read_slots(a, r, x, slots, ROW_NT);
+    const float z = put_slots(a, r, x, slots, mine, ROW_NT);
+    __syncthreads();
+    Teacher teacher;
+    if (tid < 64) {
+        teacher = teacher_of(a, r, slots);
+        if (tid == 0) sh_mass = teacher.mass, sh_words = teacher.words;
+    }
+    keep_packed(held);
     float m = edge;
 #pragma unroll
     for (int k = 0; k < PER; ++k) held[k].each([&](float v) { m = fmaxf(m, v); });
@@ -154,26 +197,27 @@ __global__ __launch_bounds__(ROW_NT) void distill_held(Distill a) {
         s = lanes_sum(s);
     }
     if ((tid & 63) == 0) sh_m[tid >> 6] = s == 0.0 ? -INFINITY : ref, sh_s[tid >> 6] = s;
+    if (tid < slots.count) slots.z[tid] = z;
     __syncthreads();
-    if (tid < 64) {
-        const Row o = finish(a, r, slots, sum_of_row(a, sh_m, sh_s));
-        if (tid == 0) sh_o = o;
-    }
+    const RowTotal total = total_of_row(a, sh_m, sh_s);
     if constexpr (GRAD) {
-        __syncthreads();
-        const Row o = sh_o;
-        if (o.coef == 0.0f) return zero_row<T, ROW_NT, PAST>(dx, cut, tid);
-        const float s2 = a.scale * LOG2E, c = o.coef * o.sum_p * o.per_sum;
-        keep_packed(held);
+        const Row o = row_of(a, w, sh_mass, sh_words, total);
+        if (o.coef == 0.0f) {
+            zero_row<T, ROW_NT, PAST>(dx, cut, tid);
+        } else {
+            const float s2 = a.scale * LOG2E, c = o.coef * o.even;
+            keep_packed(held);
 #pragma unroll
-        for (int k = 0; k < PER; ++k) {
-            const int p = tid + k * ROW_NT;
-            if (p < cut.pieces) store_piece<PAST>(dx + cut.head + p * N, held[k].map([&](int, float v) { return c * o.power(v, s2); }));
+            for (int k = 0; k < PER; ++k) {
+                const int p = tid + k * ROW_NT;
+                if (p < cut.pieces) store_piece<PAST>(dx + cut.head + p * N, held[k].map([&](int, float v) { return c * o.power(v, s2); }));
+            }
+            if (tid < cut.edges) put(dx, cut.edge(tid), c * o.power(edge, s2));
+            __syncthreads();  // the row is there before its words are written over
+            write_slots(a, dx, slots, o, s2, ROW_NT);
         }
-        if (tid < cut.edges) put(dx, cut.edge(tid), c * o.power(edge, s2));
-        __syncthreads();  // the row is there before its words are written over
-        write_slots(a, dx, slots, o, s2, ROW_NT);
     }
+    if (tid < 64) finish(a, r, slots, teacher, total);
 }
 
 // Rows that no workgroup holds: read in strides with a running maximum and sum, and again for the gradient.
@@ -183,39 +227,49 @@ __global__ __launch_bounds__(LONG_NT) void distill_long(Distill a) {
     constexpr int WAVES = LONG_NT / 64, N = Piece<T>::N;
     __shared__ float sh_m[WAVES];
     __shared__ double sh_s[WAVES];
-    __shared__ Row sh_o;
-    extern __shared__ float lds[];
+    __shared__ float sh_mass;
+    __shared__ int sh_words;
+    extern __shared__ __attribute__((aligned(16))) float lds[];
     const Slots slots = slots_in(lds, a.top);
     const int64_t r = blockIdx.x;
     const int tid = threadIdx.x;
     const T* x = static_cast<const T*>(a.logits) + r * a.ld;
     T* dx = GRAD ? static_cast<T*>(a.dlogits) + r * a.dld : nullptr;
     const Cut<T> cut(x, a.vocab);
-    if (a.weights[r] == 0.0f) {
+    const Slot mine = slot(a, r, tid);
+    const float w = a.weights[r];
+    if (w == 0.0f) {
         if (tid == 0) a.kl[r] = 0.0f, a.row_loss[r] = 0.0;
         if (GRAD) zero_row<T, LONG_NT, PAST>(dx, cut, tid);
         return;
     }
     const float edge = tid < cut.edges ? elem(x, cut.edge(tid)) : -INFINITY;
-    read_slots(a, r, x, slots, LONG_NT);
-    running<T, LONG_NT>(a, x, cut, 0, cut.pieces, edge, sh_m, sh_s);
+    const float z = put_slots(a, r, x, slots, mine, LONG_NT);
+    if (tid < slots.count) slots.z[tid] = z;
+    running<T, LONG_NT>(a, x, cut, 0, cut.pieces, edge, sh_m, sh_s);  // its end waits for all
+    Teacher teacher;
     if (tid < 64) {
-        const Row o = finish(a, r, slots, sum_of_row(a, sh_m, sh_s));
-        if (tid == 0) sh_o = o;
+        teacher = teacher_of(a, r, slots);
+        if (tid == 0) sh_mass = teacher.mass, sh_words = teacher.words;
     }
+    __syncthreads();
+    const RowTotal total = total_of_row(a, sh_m, sh_s);
     if constexpr (GRAD) {
-        __syncthreads();
-        const Row o = sh_o;
-        if (o.coef == 0.0f) return zero_row<T, LONG_NT, PAST>(dx, cut, tid);
-        const float s2 = a.scale * LOG2E, c = o.coef * o.sum_p * o.per_sum;
-        for (int p = tid; p < cut.pieces; p += LONG_NT) {
-            const int j0 = cut.head + p * N;
-            store_piece<PAST>(dx + j0, load_piece<PAST>(x + j0).map([&](int, float v) { return c * o.power(v, s2); }));
+        const Row o = row_of(a, w, sh_mass, sh_words, total);
+        if (o.coef == 0.0f) {
+            zero_row<T, LONG_NT, PAST>(dx, cut, tid);
+        } else {
+            const float s2 = a.scale * LOG2E, c = o.coef * o.even;
+            for (int p = tid; p < cut.pieces; p += LONG_NT) {
+                const int j0 = cut.head + p * N;
+                store_piece<PAST>(dx + j0, load_piece<PAST>(x + j0).map([&](int, float v) { return c * o.power(v, s2); }));
+            }
+            if (tid < cut.edges) put(dx, cut.edge(tid), c * o.power(edge, s2));
+            __syncthreads();
+            write_slots(a, dx, slots, o, s2, LONG_NT);
         }
-        if (tid < cut.edges) put(dx, cut.edge(tid), c * o.power(edge, s2));
-        __syncthreads();
-        write_slots(a, dx, slots, o, s2, LONG_NT);
     }
+    if (tid < 64) finish(a, r, slots, teacher, total);
 }
 
 // The rows' losses in a fixed order.
@@ -232,7 +286,7 @@ template <typename T, bool PAST, bool GRAD>
 void launch_held(const Distill& a, hipStream_t st) {
     const dim3 grid(static_cast<unsigned>(a.rows));
     const int pieces = a.vocab / Piece<T>::N;
-    const size_t lds = 12 * static_cast<size_t>(a.top);
+    const size_t lds = 16 * static_cast<size_t>(pitch_of(a.top));
     if (pieces <= 64) return distill_held<T, 64, 1, PAST, GRAD><<<grid, 64, lds, st>>>(a);
     if (pieces <= 128) return distill_held<T, 64, 2, PAST, GRAD><<<grid, 64, lds, st>>>(a);
     if (pieces <= 256) return distill_held<T, 64, 4, PAST, GRAD><<<grid, 64, lds, st>>>(a);

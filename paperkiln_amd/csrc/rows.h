@@ -172,15 +172,24 @@ struct RowSum {
 };
 __device__ inline RowSum row_sum(float top, double sum) { return RowSum{top, sum == 0.0 ? static_cast<double>(NAN) : log2(sum)}; }  // a row without a word has no probabilities
 // From what each wavefront has: the logit that it took its exponentials against and their sum; one without a word has none to scale.
+struct RowTotal {
+    float top;
+    double sum;  // of 2^(s2 (x - top))
+};
 template <typename A, int WAVES>
-__device__ inline RowSum sum_of_row(const A& a, const float (&m)[WAVES], const double (&s)[WAVES]) {
+__device__ inline RowTotal total_of_row(const A& a, const float (&m)[WAVES], const double (&s)[WAVES]) {
     float top = m[0];
 #pragma unroll
     for (int w = 1; w < WAVES; ++w) top = fmaxf(top, m[w]);
     double sum = 0.0;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) sum += s[w] == 0.0 ? 0.0 : s[w] * power_of(a, m[w], top);
-    return row_sum(top, sum);
+    return RowTotal{top, sum};
+}
+template <typename A, int WAVES>
+__device__ inline RowSum sum_of_row(const A& a, const float (&m)[WAVES], const double (&s)[WAVES]) {
+    const RowTotal t = total_of_row(a, m, s);
+    return row_sum(t.top, t.sum);
 }
 
 // Rows that no workgroup holds are read in strides, with a running maximum and sum, and again for the gradient.
