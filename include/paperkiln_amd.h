@@ -435,8 +435,10 @@ int pk_distill_loss(const pk_distill_config* c, const void* logits, int64_t ld, 
  * q, k are [B, T, Hk, dk], v and o [B, T, Hv, dv] in any strides; a head of q and k serves Hv / Hk neighbouring heads of v. g (log-decays) and beta are fp32
  * [B, T, Hv], dense. state_in, state_out: fp32 [B, Hv, dk, dv], dense; NULL: begins with zeros, is not wanted; they may be the same. Keys are expected of
  * about unit length and beta in 0 to 2: past that the rule itself grows without bound. g = -inf (or below -1000) starts afresh, so several documents may follow one another in a
- * row; a token of g 0 and beta 0, finite in q, k and v, leaves the state as it is (padding). Up to 16 tokens the rule is walked through token by token, with
- * the state in registers and no workspace (its bytes are then 0): serving. Results lie clear of everything that is read, but for state_out. */
+ * row; a token of g 0 and beta 0, finite in q, k and v, leaves the state as it is (padding). Up to 8 tokens the rule is walked through token by token, with
+ * the state in registers and no workspace (its bytes are then 0): serving. A value of q, k, v, g or beta that is not a number spoils what its heads of v have from the beginning of
+ * its chunk of 64 tokens on, and nothing else. Results lie clear of one another, of the workspace and of what is read, but for state_out, which may be state_in: refused where
+ * it can be told (tensors of heads may lie between one another in one buffer). */
 typedef struct pk_delta_shape {
     int32_t B, T;    /* either may be 0; at most 2^20 heads of sequences and 2^25 chunks of 64 tokens */
     int32_t Hk, Hv;  /* Hv a multiple of Hk */

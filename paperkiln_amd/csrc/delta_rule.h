@@ -330,21 +330,6 @@ __device__ inline void put_block4(uint16_t* m, int row, int k, const f32x4& x) {
 #pragma unroll
     for (int i = 0; i < N; ++i) *reinterpret_cast<u32x2*>(to + i * BLOCKS * BLOCK) = p[i];
 }
-template <bool UPPER>
-__device__ inline bool has_block(int row, int k) {
-    return UPPER ? k >= 32 || row < 32 : k < 32 || row >= 32;
-}
-// A chunk's rows of q or k (n of them are there, the others zeros) as parts in LDS, by NT threads; columns past dk are zeros.
-template <typename T, int DK, int P, int NT>
-__device__ inline void tile_to_lds(const T* base, int64_t st, int n, int dk, uint16_t* m) {
-    constexpr int PER = DK / 8;
-    for (int i = threadIdx.x; i < C * PER; i += NT) {
-        const int r = i / PER, c = i % PER * 8;
-        const Operand<PARTS<T>> o = load8(base + (r < n ? r : 0) * st, c, r < n ? dk : 0);
-#pragma unroll
-        for (int p = 0; p < PARTS<T>; ++p) *reinterpret_cast<bf16x8*>(m + (p * C + r) * P + c) = o.part[p];
-    }
-}
 
 // A problem as the kernels see it. Strides are in elements.
 struct View {
@@ -387,8 +372,9 @@ template <typename F>
 int by_size(int dk, F&& f) {
     return dk <= 32 ? f(std::integral_constant<int, 32>{}) : dk <= 64 ? f(std::integral_constant<int, 64>{}) : f(std::integral_constant<int, 128>{});
 }
-// Columns to a workgroup of a walk: 32 where that many workgroups fill the chip, and a unit's matrices, q and k are then fetched half as often; else 16, a chunk of which takes half
-// the time.
+// Columns to a workgroup of a walk: 32 where that many workgroups fill the chip, and a unit's matrices, q and k are then fetched half as often; else 16, a chunk of which takes less time. The
+// forward of 4 x 2048 tokens, 16 heads of 128 in bf16 (256 workgroups of 32): 128 us, 134 in columns of 16; of 2 x 4096 tokens (128 of them) 207 and 161; of one sequence of
+// 4096 (64) 194 and 142.
 inline bool wide(const Rule& a) { return static_cast<int64_t>(a.B) * a.Hv * blocks(a.dv, 32) >= 256; }
 // Workgroups of one unit go to one XCD, whose L2 then has the unit's q, k and matrices for all of its blocks. Launch with grid.x = unit_grid.
 inline unsigned unit_grid(int64_t units, int per) { return static_cast<unsigned>((units + 7) / 8 * 8 * per); }
@@ -404,6 +390,14 @@ int launch_chunks(const Rule& a, int dtype, bool backward, hipStream_t st);
 int launch_states(const Rule& a, int dtype, hipStream_t st);
 int check(const char* who, const pk_delta_shape* s);
 bool view_of(const pk_tensor4* t, View& v);
+// Where a tensor lies, to refuse results on top of something else. Tensors of heads may lie between one another in one buffer, so between two of them only the same place is refused.
+struct Span {
+    uintptr_t from, to;
+    bool heads;
+};
+Span span_of(const void* dense, size_t bytes);
+Span span_of(const View& v, const pk_delta_shape* s, int heads, int width);
+bool apart(std::initializer_list<Span> written, std::initializer_list<Span> read);
 inline size_t pad(size_t bytes) { return (bytes + 255) & ~size_t{255}; }
 constexpr size_t MATRIX = BLOCKS * BLOCK * sizeof(uint16_t);
 

@@ -156,7 +156,8 @@ def gated_delta_rule_fwd(q, k, v, g, beta, scale, initial_state=None):
     """A sequence mixed through a state S [dk, dv] for every head of v: S_t = e^g_t S_{t-1} + k_t u_t^T with u_t = beta_t (v_t - e^g_t S_{t-1}^T k_t), o_t = scale S_t^T q_t.
     q, k: [B,T,Hk,dk], v: [B,T,Hv,dv] (any batch/token/head strides; a head of q and k serves Hv/Hk neighbouring heads of v; dk at most 128, dv 256), g (log-decays) and beta:
     float32 [B,T,Hv], initial_state: float32 [B,Hv,dk,dv], zeros without. Returns (o, the state behind the last token). Keys are expected of about unit length. g = -inf
-    starts afresh, so that documents may follow one another in a row; a token of g 0 and beta 0 leaves the state as it is (padding)."""
+    starts afresh, so that documents may follow one another in a row; a token of g 0 and beta 0 leaves the state as it is (padding). A value that is not a number spoils
+    its heads from the beginning of its 64 tokens on."""
     return _native.gated_delta_rule_fwd(q, k, v, g, beta, scale, initial_state)
 
 
@@ -172,7 +173,8 @@ def gated_delta_rule(q, k, v, g, beta, scale, initial_state=None):
 
 
 def gated_delta_step_(q, k, v, g, beta, scale, state):
-    """The same for the next token, or the next few, of sequences whose state is kept: moves ``state`` (float32 [B,Hv,dk,dv]) on in place and returns o."""
+    """The same for the next token, or the next few, of sequences whose state is kept: moves ``state`` (float32 [B,Hv,dk,dv]) on in place and returns o.
+    Not differentiable: refused where gradients are kept and ``state`` wants one."""
     return _native.gated_delta_step(q, k, v, g, beta, scale, state)
 
 

@@ -367,6 +367,7 @@ PyObject* py_delta_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Tensor o;
     {
         pybind11::gil_scoped_release no_gil;
+        if (at::GradMode::is_enabled() && state.requires_grad()) refuse(DELTA, "the state that is moved on in place must not require a gradient");
         o = delta_fwd(q, k, v, g, beta, scale, state, state).first;
     }
     return THPVariable_Wrap(std::move(o));

@@ -93,6 +93,18 @@ def delta(entry, **kw):
 DELTA = [(dict(B=-1), SHAPE), (dict(T=-1), SHAPE), (dict(Hk=0), SHAPE), (dict(Hv=0), SHAPE), (dict(Hk=2, Hv=3), SHAPE), (dict(dk=0), SHAPE), (dict(dk=129), SHAPE), (dict(dv=0), SHAPE),
          (dict(dv=257), SHAPE), (dict(dtype=2), ARGUMENT), (dict(scale=math.nan), ARGUMENT), (dict(scale=math.inf), ARGUMENT), (dict(B=1 << 20, Hv=2), SHAPE), (dict(T=(1 << 26) + 1), SHAPE),
          (dict(B=1 << 18, T=1 << 14), SHAPE), (dict(ws=None), WORKSPACE), (dict(ws_bytes=100), WORKSPACE), (dict(ws=C.c_void_p((17 << 24) + 8)), WORKSPACE)]
+# results on top of what is read or of one another; a step of 6400 elements between tensors of heads of 2 x 100 tokens of 64
+DELTA_OVER = {"fwd": [dict(o=T4(2 << 24)), dict(o=T4((9 << 24) + 64)), dict(s1=C.c_void_p((11 << 24) + 64)), dict(s1=at(0)), dict(s1=C.c_void_p((2 << 24) + 25000)), dict(s1=at(8)), dict(ws=at(1)),
+                      dict(ws=C.c_void_p((4 << 24) - 64)), dict(s1=at(3)), dict(ws=at(11)), dict(o=T4((9 << 24) + 13200, -6400, 64, 64))],
+              "bwd": [dict(dq=T4(1 << 24)), dict(dv_=T4(5 << 24)), dict(dq=T4(7 << 24)), dict(dg=at(8)), dict(dg=at(15)), dict(dbeta=at(9)), dict(ds0=at(10)), dict(ds0=at(12)), dict(ds0=at(7)),
+                      dict(ws=at(4)), dict(ws=at(14)), dict(ws=C.c_void_p((13 << 24) - 64)), dict(dk_=T4((16 << 24) + 396))]}
+
+
+@pytest.mark.parametrize("entry,change", [(e, c) for e, l in DELTA_OVER.items() for c in l], ids=str)
+def test_gated_delta_rule_refuses_results_on_top_of_others(entry, change):
+    assert delta(entry, **change) == ARGUMENT and b"clear of" in _lib.lib().pk_last_error()
+
+
 DELTA_NULL = {"fwd": ("q", "k", "v", "g", "beta", "o"), "bwd": ("d_o", "q", "k", "v", "g", "beta", "dq", "dk_", "dv_", "dg", "dbeta")}
 
 
@@ -108,7 +120,7 @@ def test_gated_delta_rule_refuses_null(entry):
         assert delta(entry, **{n: None}) == ARGUMENT, n
     assert delta(entry, B=0, **{n: None for n in DELTA_NULL[entry]}) == 0    # nothing to do
     L = _lib.lib()
-    for T, none in ((1, True), (16, True), (17, False)):
+    for T, none in ((1, True), (8, True), (9, False)):
         assert (L.pk_delta_rule_fwd_workspace_bytes(C.byref(_lib.DeltaShape(2, T, 1, 1, 64, 64, 1, 1.0))) == 0) == none
     assert L.pk_delta_rule_bwd_workspace_bytes(C.byref(_lib.DeltaShape(2, 1, 1, 1, 64, 64, 1, 1.0))) > 0
     assert L.pk_delta_rule_bwd_workspace_bytes(C.byref(_lib.DeltaShape(2, 1, 1, 1, 640, 64, 1, 1.0))) == 0

@@ -148,7 +148,7 @@ def check_delta(pk, q, k, v, g, beta, first, do, dlast, scale, times=1.0):
 
 
 DELTAS = [  # B, T, Hk, Hv, dk, dv, layout, state
-    (1, 1, 1, 1, 1, 1, "plain", True), (2, 1, 2, 4, 64, 64, "plain", True), (1, 2, 1, 1, 3, 5, "plain", False), (2, 15, 2, 2, 32, 32, "fused", True), (3, 16, 1, 3, 40, 72, "heads", False),
+    (1, 1, 1, 1, 1, 1, "plain", True), (2, 1, 2, 4, 64, 64, "plain", True), (1, 2, 1, 1, 3, 5, "plain", False), (2, 15, 2, 2, 32, 32, "fused", True), (3, 16, 1, 3, 40, 72, "heads", False), (2, 7, 2, 2, 32, 32, "fused", True), (3, 8, 1, 3, 40, 72, "heads", False), (1, 9, 1, 2, 128, 100, "offset", True),
     (2, 17, 2, 2, 64, 64, "plain", True), (1, 63, 1, 1, 128, 128, "plain", True), (2, 64, 3, 3, 64, 128, "heads", True), (1, 65, 2, 6, 48, 80, "offset", True),
     (2, 130, 1, 7, 64, 64, "fused", False), (1, 200, 2, 2, 128, 256, "plain", True), (1, 257, 1, 2, 127, 33, "offset", False), (3, 100, 2, 2, 16, 8, "plain", True),
     (1, 300, 3, 3, 33, 31, "heads", True), (9, 70, 1, 1, 96, 96, "fused", True), (1, 500, 1, 1, 31, 1, "plain", True), (1, 129, 1, 2, 1, 255, "offset", True),
@@ -165,7 +165,7 @@ def test_gated_delta_rule_against_64_bits(pk, case, dtype):
 
 
 @pytest.mark.parametrize("dtype", [FP32, BF16], ids=["fp32", "bf16"])
-@pytest.mark.parametrize("T", [9, 190])
+@pytest.mark.parametrize("T", [8, 9, 190])
 @pytest.mark.parametrize("which", ["no decay", "no beta", "documents", "strong", "mixed", "same keys", "reflections", "padding"])
 def test_gated_delta_rule_extremes(pk, which, T, dtype):
     """Decays of 1, of 0 and of nearly 0 among others, and sums of them that go far; keys that repeat with beta 1 (T's rows go back and forth) and beta 2, whose steps are
@@ -322,7 +322,7 @@ def test_gated_delta_rule_past_2_to_the_31(pk):
     views = [far[64 * i:].as_strided(x.shape, (0, pitch, 0, 1)) for i, x in enumerate((q, k, v, do))]
     for y, x in zip(views, (q, k, v, do)):
         y.copy_(x)
-    for T in (70, 9):   # by chunks; by tokens, the far ones
+    for T in (70, 7):   # by chunks; by tokens, the far ones
         part = lambda x: x[:, 70 - T:]  # noqa: E731
         near = [part(x).contiguous() for x in (q, k, v, g, beta, do)]
         away = [part(x) for x in views]
@@ -663,3 +663,164 @@ def test_norm_and_distill_under_graph_capture(pk):
         graph.replay()
         torch.cuda.synchronize()
         assert same(out, want), k
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16], ids=["fp32", "bf16"])
+def test_gated_delta_rule_under_graph_capture(pk, dtype):
+    """By chunks, back, and a token that moves a state on, recorded and replayed on new inputs between eager calls: each replay has the eager bits."""
+    q, k, v, g, beta, first, do, dlast = delta_inputs(2, 150, 2, 4, 64, 48, dtype, 20)
+    token = [x[:, 5:6].contiguous() for x in (q, k, v, g, beta)]
+    moved = torch.empty_like(first)
+
+    def calls():
+        torch.add(first, 0.0, out=moved)
+        o = pk.ops.gated_delta_step_(*token, 0.2, moved)
+        return [o, moved + 0.0, *pk.ops.gated_delta_rule_fwd(q, k, v, g, beta, 0.2, first), *pk.ops.gated_delta_rule_bwd(do, q, k, v, g, beta, 0.2, first, dlast)]
+    graph, out = graph_of(calls)
+    for seed in range(3):
+        for old, new in zip((q, k, v, g, beta, first, do, dlast), delta_inputs(2, 150, 2, 4, 64, 48, dtype, 30 + seed)):
+            old.copy_(new)
+        for old, new in zip(token, (q, k, v, g, beta)):
+            old.copy_(new[:, seed:seed + 1])
+        want = [x.clone() for x in calls()]
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert same(out, want), seed
+
+
+def test_backward_passes_under_graph_capture(pk):
+    """Both nodes recorded with their forwards and replayed between eager calls. While an eager graph of the same leaves lives, their gradients belong to its stream, which must
+    not wait for a recording: refused, and the next recording stands."""
+    *rule, do, dlast = delta_inputs(2, 90, 2, 4, 32, 32, BF16, 21)
+    x, r, w, b, dy, dh = norm_inputs(64, 96, 0, 0, FP32)
+    rule, norm = [y.detach().clone().requires_grad_() for y in rule], [y.detach().clone().requires_grad_() for y in (x, w, b, r)]
+
+    def mixed():
+        return torch.autograd.grad(pk.ops.gated_delta_rule(*rule[:5], 0.2, rule[5]), rule, [do, dlast])
+
+    def normed():
+        return torch.autograd.grad(pk.ops.layernorm(norm[0], norm[1], norm[2], 1e-5, norm[3]), norm, [dy, dh])
+
+    for leaves, fn, alive in ((rule, mixed, lambda: pk.ops.gated_delta_rule(*rule[:5], 0.2, rule[5])), (norm, normed, lambda: pk.ops.layernorm(*norm[:3], 1e-5, norm[3]))):
+        lives = alive()
+        with pytest.raises(RuntimeError, match="outside of the recording"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                fn()
+        del lives
+        graph, out = graph_of(fn)
+        gen = torch.Generator(device="cuda").manual_seed(2)
+        for _ in range(3):
+            with torch.no_grad():
+                for y in leaves[:3]:
+                    y.copy_(torch.nn.functional.normalize(torch.randn(y.shape, generator=gen, device="cuda"), dim=-1))
+            want = fn()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert same(out, want)
+
+
+def test_student_operators_on_two_streams_at_once(pk):
+    """The same calls queued on two streams over different inputs: the results of one after the other."""
+    sets = [(delta_inputs(2, 500, 2, 4, 64, 64, BF16, seed), norm_inputs(700, 512, 0, 0, BF16, seed), distill_inputs(100, 9000, 20, BF16, seed)) for seed in (1, 2)]
+
+    def work(s):
+        (q, k, v, g, beta, first, do, dlast), (x, r, w, b, dy, dh), (z, idx, t, weights, _) = s
+        y, h, mean, rstd = pk.ops.layernorm_fwd(x, w, b, 1e-5, r)
+        return [*pk.ops.gated_delta_rule_fwd(q, k, v, g, beta, 0.2, first), *pk.ops.gated_delta_rule_bwd(do, q, k, v, g, beta, 0.2, first, dlast), y, h,
+                *pk.ops.layernorm_bwd(dy, h, w, mean, rstd, dh), *pk.blockops.distill_loss(z, idx, t, weights, 2.0)]
+    want = [work(s) for s in sets]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in sets], [None, None]
+    for _ in range(3):
+        for i, (st, s) in enumerate(zip(streams, sets)):
+            with torch.cuda.stream(st):
+                got[i] = work(s)
+    torch.cuda.synchronize()
+    assert all(same(a, b) for a, b in zip(got, want))
+
+
+def test_student_operators_refuse(pk):
+    """What the C entries cannot see: types, devices, shapes of tensors that belong together, strides."""
+    q, k, v, g, beta, first, do, dlast = delta_inputs(2, 20, 2, 4, 32, 32, BF16, 22)
+    rule = pk.ops.gated_delta_rule_fwd
+    for bad in ((q.float(), k, v, g, beta, 1.0), (q, k[:, :9], v, g, beta, 1.0), (q, k, v[:1], g, beta, 1.0), (q, k, v[:, :, :3], g[..., :3], beta[..., :3], 1.0), (q, k, v, g.double(), beta, 1.0),
+                (q, k, v, g[:, :9], beta, 1.0), (q, k, v, g, beta.transpose(0, 1), 1.0), (q.transpose(2, 3), k.transpose(2, 3), v, g, beta, 1.0), (q.cpu(), k.cpu(), v.cpu(), g, beta, 1.0),
+                (q, k, v, g, beta, math.inf), (q, k, v, g, beta, 1.0, first.double()), (q, k, v, g, beta, 1.0, first[:1]), (q, k, v, g, beta, 1.0, first.transpose(2, 3)),
+                (q.half(), k.half(), v.half(), g, beta, 1.0), (q, k, v.cpu(), g, beta, 1.0), (q, k, v, g.cpu(), beta, 1.0)):
+        with pytest.raises(RuntimeError):
+            rule(*bad)
+    for bad in (dict(d_o=do[:, :9]), dict(d_o=do.float()), dict(d_state=dlast[:1]), dict(d_state=dlast.transpose(2, 3)), dict(initial_state=first.to(BF16))):
+        with pytest.raises(RuntimeError):
+            pk.ops.gated_delta_rule_bwd(**{**dict(d_o=do, q=q, k=k, v=v, g=g, beta=beta, scale=1.0, initial_state=first, d_state=dlast), **bad})
+    kept = first.clone()
+    for state in (first.clone().requires_grad_(), first[:1].expand(2, -1, -1, -1), first.cpu()):
+        with pytest.raises(RuntimeError):
+            pk.ops.gated_delta_step_(q, k, v, g, beta, 1.0, state)
+    assert torch.equal(first, kept)
+    x, r, w, b, dy, dh = norm_inputs(6, 32, 0, 0, BF16)
+    for bad in ((x, w[:9], b), (x, w.to(BF16), b), (x, w, b[:9]), (x, w, b, -1.0), (x, w, b, 1e-5, r[:3]), (x, w, b, 1e-5, r.float()), (x.t(), w[:6], b[:6]), (x.cpu(), w, b), (x[0], w, b)):
+        with pytest.raises(RuntimeError):
+            pk.ops.layernorm_fwd(*bad)
+    z, idx, t, weights, lse = distill_inputs(6, 50, 4, FP32)
+    for bad in (dict(indices=idx.long()), dict(indices=idx[:3]), dict(teacher_logits=t.double()), dict(teacher_logits=t[:, :2]), dict(weights=weights[:3]), dict(temperature=0.0),
+                dict(teacher_lse=lse[:3]), dict(out=z.to(BF16)), dict(out=z[:3]), dict(logits=z.t()), dict(logits=z.half()), dict(logits=z.cpu()), dict(upstream=math.nan)):
+        with pytest.raises(RuntimeError):
+            pk.blockops.distill_loss(**{**dict(logits=z, indices=idx, teacher_logits=t, weights=weights), **bad})
+
+
+def test_a_student_step_through_all_operators(pk):
+    """A layer of norm, gated delta rule and residual norm, a head, the loss against a teacher's top logits, and the optimiser, in fp32: loss, gradients of all eight
+    parameters and the parameters after the step against the same model in 64 bits; then the stepped model token by token against itself over the whole sequence. The longest
+    chain is twelve operators, each 64 u of its result's largest at most: 2^-14."""
+    B, T, Hk, Hv, dk, dv, V, top, d = 2, 70, 2, 4, 16, 24, 211, 12, 64
+    near = 2.0 ** -14
+    gen = torch.Generator().manual_seed(14)
+    randn = lambda *s: torch.randn(s, generator=gen)  # noqa: E731
+    cut = [Hk * dk, Hk * dk, Hv * dv, Hv, Hv]
+    params = {"emb": randn(V, d), "w1": 1 + 0.2 * randn(d), "b1": 0.2 * randn(d), "in": randn(d, sum(cut)) / 8, "out": randn(Hv * dv, d) / 10, "w2": 1 + 0.2 * randn(d), "b2": 0.2 * randn(d),
+              "head": randn(d, V) / 8}
+    ids = torch.randint(0, V, (B, T), generator=gen)
+    best = (2.5 * randn(B * T, V)).topk(top, 1)
+    weights = (torch.rand(B * T, generator=gen) > 0.2).float() / 100
+
+    def model(P, ids, norm, rule):
+        x = P["emb"][ids]
+        n = x.shape[1]
+        z = norm(x.view(-1, d), P["w1"], P["b1"], None).view(B, n, -1)
+        q, k, v, g, beta = z.matmul(P["in"]).split(cut, 2)
+        q, k = (torch.nn.functional.normalize(y.unflatten(2, (Hk, dk)), dim=-1) for y in (q, k))
+        o = rule(q, k, v.unflatten(2, (Hv, dv)), -torch.nn.functional.softplus(g), torch.sigmoid(beta))
+        return norm(o.reshape(B * n, -1) @ P["out"], P["w2"], P["b2"], x.view(-1, d)) @ P["head"]
+
+    def plain_normed(x, w, b, residual):
+        x = x if residual is None else x + residual
+        return torch.nn.functional.layer_norm(x, (d,), w, b, 1e-5)
+
+    P64 = {n: p.double().requires_grad_() for n, p in params.items()}
+    logits = model(P64, ids, plain_normed, lambda q, k, v, g, beta: plain_delta(q, k, v, g, beta, 0.25)[0])
+    logp, logq = torch.log_softmax(best.values.double() / 2, 1), torch.log_softmax(logits / 2, 1).gather(1, best.indices)
+    want_loss = 4 * (weights.double() * (logp.exp() * (logp - logq)).sum(1)).sum()
+    want = torch.autograd.grad(want_loss, list(P64.values()))
+
+    def normed(x, w, b, residual):
+        y = pk.ops.layernorm(x, w, b, 1e-5, residual)
+        return y if residual is None else y[0]
+    leaves = {n: p.cuda().requires_grad_() for n, p in params.items()}
+    out = model(leaves, ids.cuda(), normed, lambda *a: pk.ops.gated_delta_rule(*a, 0.25)[0])
+    loss, dlogits, _ = pk.blockops.distill_loss(out.detach(), best.indices.to(torch.int32).cuda(), best.values.cuda(), weights.cuda(), 2.0)
+    out.backward(dlogits)
+    assert abs(float(loss) - float(want_loss.detach())) <= near * float((4 * weights).sum())
+    for (n, leaf), ref in zip(leaves.items(), want):
+        assert float((leaf.grad.double().cpu() - ref).abs().max()) <= near * float(ref.abs().max()), n
+    ps, gs = [leaf.detach() for leaf in leaves.values()], [leaf.grad for leaf in leaves.values()]
+    pk.blockops.adamw_many_(ps, gs, pk.blockops.adamw_state(ps), 0.01, eps=1e-3)
+    for (n, leaf), ref, p in zip(leaves.items(), want, params.values()):
+        step = ref / (ref.abs() + 1e-3)   # m / c1 = g and sqrt(v / c2) = |g| at the first step
+        slack = 0.01 * (near * float(ref.abs().max()) / 1e-3 + 2.0 ** -18) + 2.0 ** -22 * float(p.abs().max())
+        assert float((leaf.detach().double().cpu() - (p.double() - 0.01 * (step + 0.01 * p.double()))).abs().max()) <= slack, n
+    with torch.no_grad():
+        whole = model(leaves, ids.cuda(), normed, lambda *a: pk.ops.gated_delta_rule(*a, 0.25)[0]).view(B, T, V)
+        state = torch.zeros(B, Hv, dk, dv, device="cuda")
+        tokens = [model(leaves, ids[:, t:t + 1].cuda(), normed, lambda *a: pk.ops.gated_delta_step_(*a, 0.25, state)) for t in range(T)]
+        assert float((torch.stack(tokens, 1) - whole).abs().max()) <= near * float(whole.abs().max())
