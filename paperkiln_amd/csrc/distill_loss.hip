@@ -171,13 +171,15 @@ __global__ __launch_bounds__(ROW_NT) void distill_held(Distill a) {
     }
     const float edge = tid < cut.edges ? elem(x, cut.edge(tid)) : -INFINITY;
     const float z = put_slots(a, r, x, slots, mine, ROW_NT);
-    __syncthreads();
     Teacher teacher;
-    if (tid < 64) {
-        teacher = teacher_of(a, r, slots);
-        if (tid == 0) sh_mass = teacher.mass, sh_words = teacher.words;
+    if constexpr (GRAD) {
+        __syncthreads();
+        if (tid < 64) {
+            teacher = teacher_of(a, r, slots);
+            if (tid == 0) sh_mass = teacher.mass, sh_words = teacher.words;
+        }
+        keep_packed(held);
     }
-    keep_packed(held);
     float m = edge;
 #pragma unroll
     for (int k = 0; k < PER; ++k) held[k].each([&](float v) { m = fmaxf(m, v); });
@@ -199,8 +201,8 @@ __global__ __launch_bounds__(ROW_NT) void distill_held(Distill a) {
     if ((tid & 63) == 0) sh_m[tid >> 6] = s == 0.0 ? -INFINITY : ref, sh_s[tid >> 6] = s;
     if (tid < slots.count) slots.z[tid] = z;
     __syncthreads();
-    const RowTotal total = total_of_row(a, sh_m, sh_s);
     if constexpr (GRAD) {
+        const RowTotal total = total_of_row(a, sh_m, sh_s);
         const Row o = row_of(a, w, sh_mass, sh_words, total);
         if (o.coef == 0.0f) {
             zero_row<T, ROW_NT, PAST>(dx, cut, tid);
@@ -216,8 +218,11 @@ __global__ __launch_bounds__(ROW_NT) void distill_held(Distill a) {
             __syncthreads();  // the row is there before its words are written over
             write_slots(a, dx, slots, o, s2, ROW_NT);
         }
+        if (tid < 64) finish(a, r, slots, teacher, total);
+    } else if (tid < 64) {  // beside the row the teacher's part would take registers past the 64 with which 1024 threads are on a CU twice
+        teacher = teacher_of(a, r, slots);
+        finish(a, r, slots, teacher, total_of_row(a, sh_m, sh_s));
     }
-    if (tid < 64) finish(a, r, slots, teacher, total);
 }
 
 // Rows that no workgroup holds: read in strides with a running maximum and sum, and again for the gradient.
