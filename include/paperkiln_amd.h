@@ -440,7 +440,7 @@ int pk_distill_loss(const pk_distill_config* c, const void* logits, int64_t ld, 
  * its chunk of 64 tokens on, and nothing else. Results lie clear of one another, of the workspace and of what is read, but for state_out, which may be state_in: refused where
  * it can be told (tensors of heads may lie between one another in one buffer). */
 typedef struct pk_delta_shape {
-    int32_t B, T;    /* either may be 0; at most 2^20 heads of sequences and 2^25 chunks of 64 tokens */
+    int32_t B, T;    /* either may be 0; at most 2^19 heads of sequences and 2^22 chunks of 64 tokens */
     int32_t Hk, Hv;  /* Hv a multiple of Hk */
     int32_t dk, dv;  /* 1 to 128, 1 to 256 */
     int32_t dtype;   /* PK_F32 | PK_BF16: q, k, v, o and their gradients */

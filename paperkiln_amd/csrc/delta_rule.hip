@@ -473,8 +473,9 @@ int check(const char* who, const pk_delta_shape* s) {
     if (!s) return fail(PK_ERR_ARGUMENT, w + ": null pointer");
     if (s->B < 0 || s->T < 0 || s->Hk < 1 || s->Hv < 1 || s->Hv % s->Hk) return fail(PK_ERR_SHAPE, w + ": shape mismatch (heads of v are shared out evenly to those of k)");
     if (s->dk < 1 || s->dk > 128 || s->dv < 1 || s->dv > 256) return fail(PK_ERR_SHAPE, w + ": shape mismatch (dk 1 to 128, dv 1 to 256)");
-    if (static_cast<int64_t>(s->B) * s->Hv > (1 << 20) || s->T > (1 << 26) || static_cast<int64_t>(s->B) * s->Hv * (chunks(s->T) + 1) > (1 << 25))
-        return fail(PK_ERR_SHAPE, w + ": shape mismatch (at most 2^20 heads of sequences and 2^25 chunks of 64 tokens)");
+    // a launch has fewer than 2^32 threads: 512 for each chunk, and for each of a head's 8 blocks of columns
+    if (static_cast<int64_t>(s->B) * s->Hv > (1 << 19) || s->T > (1 << 26) || static_cast<int64_t>(s->B) * s->Hv * (chunks(s->T) + 1) > (1 << 22))
+        return fail(PK_ERR_SHAPE, w + ": shape mismatch (at most 2^19 heads of sequences and 2^22 chunks of 64 tokens)");
     if (!known_dtype(s->dtype)) return fail(PK_ERR_ARGUMENT, w + ": dtype must be PK_F32 or PK_BF16");
     if (!std::isfinite(s->scale)) return fail(PK_ERR_ARGUMENT, w + ": scale must be finite");
     return PK_OK;

@@ -91,7 +91,7 @@ def delta(entry, **kw):
 
 
 DELTA = [(dict(B=-1), SHAPE), (dict(T=-1), SHAPE), (dict(Hk=0), SHAPE), (dict(Hv=0), SHAPE), (dict(Hk=2, Hv=3), SHAPE), (dict(dk=0), SHAPE), (dict(dk=129), SHAPE), (dict(dv=0), SHAPE),
-         (dict(dv=257), SHAPE), (dict(dtype=2), ARGUMENT), (dict(scale=math.nan), ARGUMENT), (dict(scale=math.inf), ARGUMENT), (dict(B=1 << 20, Hv=2), SHAPE), (dict(T=(1 << 26) + 1), SHAPE),
+         (dict(dv=257), SHAPE), (dict(dtype=2), ARGUMENT), (dict(scale=math.nan), ARGUMENT), (dict(scale=math.inf), ARGUMENT), (dict(B=1 << 20, Hv=2), SHAPE), (dict(B=(1 << 19) + 1, T=1), SHAPE), (dict(T=(1 << 26) + 1), SHAPE), (dict(B=1, T=(1 << 22) * 64), SHAPE), (dict(B=1 << 16, T=63 * 64 + 1), SHAPE),
          (dict(B=1 << 18, T=1 << 14), SHAPE), (dict(ws=None), WORKSPACE), (dict(ws_bytes=100), WORKSPACE), (dict(ws=C.c_void_p((17 << 24) + 8)), WORKSPACE)]
 # results on top of what is read or of one another; a step of 6400 elements between tensors of heads of 2 x 100 tokens of 64
 DELTA_OVER = {"fwd": [dict(o=T4(2 << 24)), dict(o=T4((9 << 24) + 64)), dict(s1=C.c_void_p((11 << 24) + 64)), dict(s1=at(0)), dict(s1=C.c_void_p((2 << 24) + 25000)), dict(s1=at(8)), dict(ws=at(1)),
