@@ -100,7 +100,7 @@ DELTA_OVER = {"fwd": [dict(o=T4(2 << 24)), dict(o=T4((9 << 24) + 64)), dict(s1=C
                       dict(ws=at(4)), dict(ws=at(14)), dict(ws=C.c_void_p((13 << 24) - 64)), dict(dk_=T4((16 << 24) + 396))]}
 
 
-@pytest.mark.parametrize("entry,change", [(e, c) for e, l in DELTA_OVER.items() for c in l], ids=str)
+@pytest.mark.parametrize("entry,change", [(e, c) for e, l in DELTA_OVER.items() for c in l], ids="-".join)
 def test_gated_delta_rule_refuses_results_on_top_of_others(entry, change):
     assert delta(entry, **change) == ARGUMENT and b"clear of" in _lib.lib().pk_last_error()
 
