@@ -21,7 +21,7 @@ __device__ inline double held(float g) { return g < -1000.0f ? -1000.0 : static_
 // T_ij = -T_ii sum_k M_ik T_kj, one diagonal after the other on the matrix cores. (All 64 rows by substitution are 2016 additions
 // one behind the other: 32 us however few the chunks.) Three wavefronts to a SIMD: of four the registers would be spilled (99 us in place of 78).
 constexpr int MP = C + 4, XP = 20;
-template <typename T, int DK, int PA, bool BACKWARD, Rows BY>
+template <typename T, int DK, bool BACKWARD, Rows BY>
 __global__ __launch_bounds__(256, PARTS<T> == 1 ? 3 : 2) void chunk_matrices(Rule a) {
     constexpr int N = PARTS<T>, MOST = N == 1 ? 0 : 2, KS = DK / 32;
     __shared__ float m[C * MP], tt[C * MP];  // M; T transposed
@@ -35,7 +35,7 @@ __global__ __launch_bounds__(256, PARTS<T> == 1 ? 3 : 2) void chunk_matrices(Rul
     const int64_t place = unit * a.chunks + chunk;
     const int hk = h / (a.Hv / a.Hk);
     const T *q = head<const T>(a.q, b, hk) + static_cast<int64_t>(t0) * a.q.st, *k = head<const T>(a.k, b, hk) + static_cast<int64_t>(t0) * a.k.st;
-    uint16_t *attn = a.attn + place * PA * (BLOCKS * BLOCK), *attn_t = BACKWARD ? a.attn_t + place * 3 * (BLOCKS * BLOCK) : nullptr;
+    uint16_t *attn = a.attn + place * 3 * (BLOCKS * BLOCK), *attn_t = BACKWARD ? a.attn_t + place * 3 * (BLOCKS * BLOCK) : nullptr;
     // wavefront w: rows 16w .. 16w+15 of both products, so the first one, with one tile of them, has time for the sum of the log-decays
     const int it = wave, i = 16 * it + c16;
     Eight<BY, T> ki[KS], qi[KS], kj[3][KS];
@@ -98,7 +98,7 @@ __global__ __launch_bounds__(256, PARTS<T> == 1 ? 3 : 2) void chunk_matrices(Rul
                 if (BACKWARD && (j <= it || j == it + 1))
                     put_block4<3, true>(attn_t, 16 * j + c16, 16 * it + 4 * g, qk[j]);
                 else if (!BACKWARD && (j <= it || j == it + 1))
-                    put_block4<PA, false>(attn, i, j4, qk[j]);
+                    put_block4<3, false>(attn, i, j4, qk[j]);
             }
         }
     }
@@ -194,7 +194,7 @@ constexpr bool TWO_K = PARTS<T> == 1 || DK < 128;  // two of K's tiles in LDS: t
 
 template <typename T, int DK, int VB, bool STATES, Rows BY>
 __global__ __launch_bounds__(16 * VB) void walk(Rule a) {
-    constexpr int N = PARTS<T>, KP = DK + 16, SP = DK + 8, KS = DK / 32, KT = (DK + 63) / 64, PO = N == 1 ? 2 : 3;  // PO: parts of U and A on their way to O
+    constexpr int N = PARTS<T>, KP = DK + 16, SP = DK + 8, KS = DK / 32, KT = (DK + 63) / 64;
     extern __shared__ uint16_t lds[];
     uint16_t *kt = lds, *st = kt + (TWO_K<T, DK> ? 2 : 1) * N * C * KP, *rt = st + 3 * VB * SP, *dt = rt + 3 * VB * CP, *ut = dt + 3 * VB * CP;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c16 = lane & 15;
@@ -225,7 +225,7 @@ __global__ __launch_bounds__(16 * VB) void walk(Rule a) {
     Eight<BY, T> Q[KS];
     Tokens<BY, T> V;
     Operand<3> inverse[2];
-    Operand<PO> attn[2];
+    Operand<3> attn[2];
     f32x4 gamma, delta, beta;
     float whole, gamma_o;
     const auto load_k = [&](int chunk) { K.load(k + static_cast<int64_t>(chunk) * C * a.k.st, a.k.st, min(C, a.T - chunk * C), a.dk); };
@@ -247,9 +247,9 @@ __global__ __launch_bounds__(16 * VB) void walk(Rule a) {
         if (!low) inverse[1] = matrix_block<3, false>(m, tile, 1, lane);
     };
     const auto load_attn = [&](int chunk) {
-        const uint16_t* m = a.attn + (first + chunk) * PO * (BLOCKS * BLOCK);
-        attn[0] = matrix_block<PO, false>(m, tile, 0, lane);
-        if (!low) attn[1] = matrix_block<PO, false>(m, tile, 1, lane);
+        const uint16_t* m = a.attn + (first + chunk) * 3 * (BLOCKS * BLOCK);
+        attn[0] = matrix_block<3, false>(m, tile, 0, lane);
+        if (!low) attn[1] = matrix_block<3, false>(m, tile, 1, lane);
     };
     load_k(0), load_rows(0), load_inverse(0);
     if (!STATES) load_attn(0);
@@ -272,12 +272,12 @@ __global__ __launch_bounds__(16 * VB) void walk(Rule a) {
         // R = beta (V - gamma K S), and gamma Q S
         f32x4 O = {0, 0, 0, 0};
         {
-            f32x4 P[3] = {}, QS[PO] = {};
+            f32x4 P[3] = {}, QS[3] = {};
 #pragma unroll
             for (int kk = 0; kk < KS; ++kk) {
                 const Operand<3> s = rows_of<3, VB, SP>(st, vt, 32 * kk, lane);
                 spread<2>(rows_of<N, C, KP>(kc, 16 * tile, 32 * kk, lane), s, P);
-                if (!STATES) spread<PO - 1>(s, Q[kk].operand(), QS);
+                if (!STATES) spread<2>(s, Q[kk].operand(), QS);
             }
             const f32x4 x = V.values(), p = gather(P);
             f32x4 R;
@@ -301,7 +301,7 @@ __global__ __launch_bounds__(16 * VB) void walk(Rule a) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) a.puts[(place * C + tokens + r) * a.dv + vc] = U[r];
             } else {
-                put4<PO, VB, CP>(ut, column, tokens, U);
+                put4<3, VB, CP>(ut, column, tokens, U);
             }
             put4<3, VB, CP>(dt, column, tokens, U * leave);
         }
@@ -320,9 +320,9 @@ __global__ __launch_bounds__(16 * VB) void walk(Rule a) {
             for (int i = 0; i < KT; ++i) S[i] = S[i] * end + gather(sums[i]);
         }
         if (!STATES) {
-            f32x4 sums[PO] = {};
-            spread<PO - 1>(rows_of<PO, VB, CP>(ut, vt, 0, lane), attn[0], sums);
-            if (!low) spread<PO - 1>(rows_of<PO, VB, CP>(ut, vt, 32, lane), attn[1], sums);
+            f32x4 sums[3] = {};
+            spread<2>(rows_of<3, VB, CP>(ut, vt, 0, lane), attn[0], sums);
+            if (!low) spread<2>(rows_of<3, VB, CP>(ut, vt, 32, lane), attn[1], sums);
             if (token < n) write4<BY>(out + static_cast<int64_t>(t0 + token) * a.o.st, vo, a.dv, O + gather(sums));
             load_attn(next);
         }
@@ -331,7 +331,7 @@ __global__ __launch_bounds__(16 * VB) void walk(Rule a) {
 }
 template <typename T, int DK, int VB, bool STATES>
 constexpr size_t walk_lds() {
-    return sizeof(uint16_t) * ((TWO_K<T, DK> ? 2 : 1) * PARTS<T> * C * (DK + 16) + 3 * VB * (DK + 8) + 6 * VB * CP + (STATES ? 0 : (PARTS<T> == 1 ? 2 : 3) * VB * CP));
+    return sizeof(uint16_t) * ((TWO_K<T, DK> ? 2 : 1) * PARTS<T> * C * (DK + 16) + 3 * VB * (DK + 8) + (STATES ? 6 : 9) * VB * CP);
 }
 
 // ---- token by token ----
@@ -436,7 +436,7 @@ int launch_matrices(const Rule& a, bool backward, hipStream_t st) {
         const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.B) * a.Hv * a.chunks));
         return by_rows(rows_by(a, DK, 1), [&](auto by) {
             constexpr Rows BY = decltype(by)::value;
-            backward ? chunk_matrices<T, DK, 3, true, BY><<<grid, 256, 0, st>>>(a) : chunk_matrices<T, DK, (PARTS<T> == 1 ? 2 : 3), false, BY><<<grid, 256, 0, st>>>(a);
+            backward ? chunk_matrices<T, DK, true, BY><<<grid, 256, 0, st>>>(a) : chunk_matrices<T, DK, false, BY><<<grid, 256, 0, st>>>(a);
             return launched();
         });
     });
@@ -456,7 +456,7 @@ struct Room {
 Room room_of(const pk_delta_shape* s) {
     const size_t places = static_cast<size_t>(s->B) * s->Hv * chunks(s->T);
     Room r;
-    r.inverse = pad(places * 3 * MATRIX), r.attn = pad(places * (s->dtype == PK_F32 ? 3 : 2) * MATRIX), r.scalars = pad(places * 3 * C * sizeof(float));
+    r.inverse = r.attn = pad(places * 3 * MATRIX), r.scalars = pad(places * 3 * C * sizeof(float));
     r.all = r.inverse + r.attn + r.scalars;
     return r;
 }

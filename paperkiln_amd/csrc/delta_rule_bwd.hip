@@ -162,7 +162,7 @@ constexpr int tile_size() {
 }
 template <typename T, int DK>
 constexpr size_t grads_lds() {
-    constexpr int PE = PARTS<T> == 1 ? 2 : 3, by = (6 * DK + 3 * C) * VQ, then = 4 * C * HP + 2 * PE * C * AP;
+    constexpr int by = (6 * DK + 3 * C) * VQ, then = 4 * C * HP + 6 * C * AP;
     return sizeof(uint16_t) * (BESIDE<T, DK> ? 2 * tile_size<T, DK>() + std::max(by, then) : std::max(by, tile_size<T, DK>() + then));
 }
 template <Rows BY, typename T, int DK, int P>
@@ -177,7 +177,7 @@ __device__ inline float over_groups(float x) {  // the four lanes of a token
 }
 template <typename T, int DK, Rows BY>
 __global__ __launch_bounds__(GRAD_NT, 2) void chunk_grads(Rule a, float* sums) {
-    constexpr int N = PARTS<T>, MOST = N == 1 ? 0 : 2, PE = N == 1 ? 2 : 3, KP = DK + 16, KS = DK / 32, KT = DK / 32, SN = (DK * (GB / 4) + GRAD_NT - 1) / GRAD_NT;
+    constexpr int N = PARTS<T>, MOST = N == 1 ? 0 : 2, KP = DK + 16, KS = DK / 32, KT = DK / 32, SN = (DK * (GB / 4) + GRAD_NT - 1) / GRAD_NT;
     constexpr bool BOTH = BESIDE<T, DK>, AHEAD = BOTH || BY != ANY;  // with everything held the loads ahead of rows of any size would not fit into the registers
     extern __shared__ uint16_t lds[];
     __shared__ double total[C];
@@ -185,7 +185,7 @@ __global__ __launch_bounds__(GRAD_NT, 2) void chunk_grads(Rule a, float* sums) {
     __shared__ float ends[2][C], tails[2][C], dbs[2][C], dots[8];
     uint16_t *kt = lds, *qt = BOTH ? kt + tile_size<T, DK>() : kt, *s0 = BOTH ? qt + tile_size<T, DK>() : lds;
     uint16_t *s1 = s0 + 3 * DK * VQ, *ut = s1 + 3 * DK * VQ;                                                          // while the columns of the state go by
-    uint16_t *hs = BOTH ? s0 : s0 + tile_size<T, DK>(), *et = hs + 4 * C * HP, *ft = et + PE * C * AP;  // then
+    uint16_t *hs = BOTH ? s0 : s0 + tile_size<T, DK>(), *et = hs + 4 * C * HP, *ft = et + 3 * C * AP;  // then
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), tile = wave & 3, half = wave >> 2, g = lane >> 4, c16 = lane & 15, i = 16 * tile + c16;
     float* ht = reinterpret_cast<float*>(hs) + half * C * HP;
     const int64_t group = blockIdx.x / static_cast<unsigned>(a.chunks);
@@ -315,7 +315,7 @@ __global__ __launch_bounds__(GRAD_NT, 2) void chunk_grads(Rule a, float* sums) {
                         db = fmaf(z, xk[j][r], db);
                     }
                 }
-                put4<PE, C, AP>(half == 0 ? et : ft, i, 16 * j + 4 * g, X[j]);
+                put4<3, C, AP>(half == 0 ? et : ft, i, 16 * j + 4 * g, X[j]);
                 *reinterpret_cast<f32x4*>(ht + i * HP + 16 * j + 4 * g) = H;
             }
         }
@@ -373,12 +373,12 @@ __global__ __launch_bounds__(GRAD_NT, 2) void chunk_grads(Rule a, float* sums) {
         }
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            const Operand<PE> e = rows_of<PE, C, AP>(et, 16 * tile, 32 * s, lane_then), f = rows_of<PE, C, AP>(ft, 16 * tile, 32 * s, lane_then),
-                              ft_ = cols_of<PE, C, AP>(ft, 32 * s, 16 * tile, lane_then);
+            const Operand<3> e = rows_of<3, C, AP>(et, 16 * tile, 32 * s, lane_then), f = rows_of<3, C, AP>(ft, 16 * tile, 32 * s, lane_then),
+                              ft_ = cols_of<3, C, AP>(ft, 32 * s, 16 * tile, lane_then);
 #pragma unroll
             for (int d = 0; d < KT; ++d) {
                 const Operand<N> x = cols_of<N, C, KP>(kt, 32 * s, d_of(d), lane_then);
-                product<PE - 1>(x, e, Y[d]), product<PE - 1>(x, f, Yu[d]), product<PE - 1>(x, ft_, Yu[d]);
+                product<2>(x, e, Y[d]), product<2>(x, f, Yu[d]), product<2>(x, ft_, Yu[d]);
             }
         }
         if (!BOTH) {
@@ -388,9 +388,9 @@ __global__ __launch_bounds__(GRAD_NT, 2) void chunk_grads(Rule a, float* sums) {
         }
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            const Operand<PE> et_ = cols_of<PE, C, AP>(et, 32 * s, 16 * tile, lane_then);
+            const Operand<3> et_ = cols_of<3, C, AP>(et, 32 * s, 16 * tile, lane_then);
 #pragma unroll
-            for (int d = 0; d < KT; ++d) product<PE - 1>(cols_of<N, C, KP>(qt, 32 * s, d_of(d), lane_then), et_, Yu[d]);
+            for (int d = 0; d < KT; ++d) product<2>(cols_of<N, C, KP>(qt, 32 * s, d_of(d), lane_then), et_, Yu[d]);
         }
         const bool last = head_v == rep - 1;
         float* mine = rows + i_then * DK;
