@@ -118,7 +118,6 @@ __device__ inline void finish(const Distill& a, int64_t r, const Slots& s, const
 }
 struct Row {
     float top, coef, even;  // coef: upstream w tau, 0 where there is nothing to learn from the row; even: what every word's probability is multiplied by
-    __device__ float power(float x, float s2) const { return __builtin_amdgcn_exp2f((x - top) * s2); }
 };
 __device__ inline Row row_of(const Distill& a, double w, float mass, int words, const RowTotal& t) {
     if (!words) return Row{0.0f, 0.0f, 0.0f};
@@ -127,7 +126,7 @@ __device__ inline Row row_of(const Distill& a, double w, float mass, int words, 
 }
 // The teacher's words written over, by the threads of a workgroup. A word that several slots name gets all of theirs, from each of them the same value.
 template <typename T>
-__device__ inline void write_slots(const Distill& a, T* dx, const Slots& s, const Row& o, float s2, int n) {
+__device__ inline void write_slots(const Distill& a, T* dx, const Slots& s, const Row& o, int n) {
     for (int k = threadIdx.x; k < a.top; k += n) {
         const int i = s.at[k];
         if (i < 0 || i >= a.vocab) continue;
@@ -137,7 +136,7 @@ __device__ inline void write_slots(const Distill& a, T* dx, const Slots& s, cons
             const float4 more = *reinterpret_cast<const float4*>(s.p + j);
             p += at.x == i ? more.x : 0.0f, p += at.y == i ? more.y : 0.0f, p += at.z == i ? more.z : 0.0f, p += at.w == i ? more.w : 0.0f;
         }
-        put(dx, i, o.coef * fmaf(o.even, o.power(s.z[k], s2), -p));
+        put(dx, i, o.coef * fmaf(o.even, power_of(a, s.z[k], o.top), -p));
     }
 }
 
@@ -207,16 +206,16 @@ __global__ __launch_bounds__(ROW_NT) void distill_held(Distill a) {
         if (o.coef == 0.0f) {
             zero_row<T, ROW_NT, PAST>(dx, cut, tid);
         } else {
-            const float s2 = a.scale * LOG2E, c = o.coef * o.even;
+            const float c = o.coef * o.even;
             keep_packed(held);
 #pragma unroll
             for (int k = 0; k < PER; ++k) {
                 const int p = tid + k * ROW_NT;
-                if (p < cut.pieces) store_piece<PAST>(dx + cut.head + p * N, held[k].map([&](int, float v) { return c * o.power(v, s2); }));
+                if (p < cut.pieces) store_piece<PAST>(dx + cut.head + p * N, held[k].map([&](int, float v) { return c * power_of(a, v, o.top); }));
             }
-            if (tid < cut.edges) put(dx, cut.edge(tid), c * o.power(edge, s2));
+            if (tid < cut.edges) put(dx, cut.edge(tid), c * power_of(a, edge, o.top));
             __syncthreads();  // the row is there before its words are written over
-            write_slots(a, dx, slots, o, s2, ROW_NT);
+            write_slots(a, dx, slots, o, ROW_NT);
         }
         if (tid < 64) finish(a, r, slots, teacher, total);
     } else if (tid < 64) {  // beside the row the teacher's part would take registers past the 64 with which 1024 threads are on a CU twice
@@ -264,14 +263,14 @@ __global__ __launch_bounds__(LONG_NT) void distill_long(Distill a) {
         if (o.coef == 0.0f) {
             zero_row<T, LONG_NT, PAST>(dx, cut, tid);
         } else {
-            const float s2 = a.scale * LOG2E, c = o.coef * o.even;
+            const float c = o.coef * o.even;
             for (int p = tid; p < cut.pieces; p += LONG_NT) {
                 const int j0 = cut.head + p * N;
-                store_piece<PAST>(dx + j0, load_piece<PAST>(x + j0).map([&](int, float v) { return c * o.power(v, s2); }));
+                store_piece<PAST>(dx + j0, load_piece<PAST>(x + j0).map([&](int, float v) { return c * power_of(a, v, o.top); }));
             }
-            if (tid < cut.edges) put(dx, cut.edge(tid), c * o.power(edge, s2));
+            if (tid < cut.edges) put(dx, cut.edge(tid), c * power_of(a, edge, o.top));
             __syncthreads();
-            write_slots(a, dx, slots, o, s2, LONG_NT);
+            write_slots(a, dx, slots, o, LONG_NT);
         }
     }
     if (tid < 64) finish(a, r, slots, teacher, total);

@@ -2,6 +2,8 @@
 inputs. Tolerances are counted as in test_student_ops_gpu.py: u = 2^-24, h half a step of the output's type."""
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -39,3 +41,25 @@ def test_gated_delta_rule_of_bf16_where_sums_cancel(pk, T, dk, dv, heads):
     given = scale * torch.einsum("bhkv,bthv->bthk", first.double(), do.double()).abs()
     within("dq", dq, want[0], HALF[BF16] * want[0].abs() + 16 * U * (2 * given + want[0].abs()))
     assert float(wo.abs().max()) < 2.0 ** -7 * float(before.max())
+
+
+# ---- distillation --------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("vocab", [4097, 8192, 40000])   # rows of a few pieces to a thread, of more, rows read twice
+def test_distill_loss_gradient_does_not_lean(pk, vocab):
+    """Words of probability 2^-64 to 2^-120, one by one: the exponent is rounded to 24 bits, 2^-17 apart at these sizes, so each is off by up to 2^-18 ln 2 either way and the
+    mean of n of them by 2^-17 ln 2 / sqrt(12 n), six times that here, besides 4 u of the exponential, the factor and the products. An exponent scale rounded to 32 bits before
+    the product would turn all of them the same way: by up to 2^-24 of 64 to 120, 50 u at these temperatures."""
+    worst = sorted((abs(float(torch.tensor(1 / (math.log(2) * k / 64), dtype=FP32)) * math.log(2) * k / 64 - 1), k / 64) for k in range(32, 257))[-3:]
+    assert worst[0][0] > 0.8 * U
+    gen = torch.Generator(device="cuda").manual_seed(vocab)
+    for _, tau in worst:
+        x = -tau * math.log(2) * (64 + 56 * torch.rand((2, vocab), generator=gen, device="cuda", dtype=F64)).to(FP32)
+        x[:, 5] = 0.0
+        idx, t, w = torch.full((2, 1), 5, dtype=torch.int32, device="cuda"), torch.ones(2, 1, device="cuda"), torch.tensor([0.5, 0.25], device="cuda")
+        _, d, _ = pk.blockops.distill_loss(x, idx, t, w, tau)
+        want = (w.double().cpu() * tau)[:, None] * torch.exp(x.double().cpu() / tau)   # the sum of the exponentials is 1 to 2^-48; torch's softmax of doubles on the GPU takes 32-bit exponentials
+        off = (d.double().cpu() / want - 1)[:, torch.arange(vocab) != 5]
+        assert float(off.abs().max()) <= 2.0 ** -18 * math.log(2) + 6 * U
+        assert float(off.mean(1).abs().max()) <= 6 * 2.0 ** -17 * math.log(2) / math.sqrt(12 * (vocab - 1)) + 4 * U
