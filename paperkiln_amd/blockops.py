@@ -227,7 +227,8 @@ def distill_loss(logits, indices, teacher_logits, weights, temperature=1.0, teac
     words], negative: an empty slot) and teacher_logits (float32) have columns. With q = softmax(logits / temperature) and p = softmax(teacher_logits / temperature) over
     the row's slots -- exp(teacher_logits / temperature - teacher_lse) where that is given, float32 [rows] -- kl is sum p (log p - log q) of each row, the loss
     temperature^2 * sum(weights * kl); dlogits is the gradient of upstream * loss, for ``logits.backward(dlogits)``, None with ``grad`` False. logits: [rows, vocab] fp32 or
-    bf16 (any row stride), weights: float32 [rows], mask and normalisation; a row of weight 0 is not read. ``out`` may be the logits."""
+    bf16 (any row stride), weights: float32 [rows], mask and normalisation; a row of weight 0 is not read. A word past the
+    vocabulary that the teacher gives something leaves its row without a number: kl, the loss and the row's dlogits are NaN. ``out`` may be the logits."""
     return _native.distill_loss(logits, indices, teacher_logits, weights, temperature, teacher_lse, upstream, grad, out)
 
 

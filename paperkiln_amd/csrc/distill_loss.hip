@@ -93,7 +93,7 @@ __device__ inline Teacher teacher_of(const Distill& a, int64_t r, const Slots& s
     for (int k = lane; k < s.count; k += 64) {
         const double p = s.at[k] >= 0 ? exp(s.t[k] * per - lse) : 0.0;
         s.p[k] = static_cast<float>(p);
-        mass += p;
+        mass += s.at[k] >= a.vocab && p != 0.0 ? NAN : p;  // a word that is none: the row has no gradient either
     }
     return Teacher{lse, static_cast<float>(lanes_sum(mass)), 1};
 }

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from test_post_ops_gpu import BF16, F64, FP32, HALF, U, within
-from test_student_ops_gpu import pk, plain_delta  # noqa: F401  (pk: a fixture)
+from test_student_ops_gpu import bits, distill_inputs, pk, plain_delta  # noqa: F401  (pk: a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -63,3 +63,23 @@ def test_distill_loss_gradient_does_not_lean(pk, vocab):
         off = (d.double().cpu() / want - 1)[:, torch.arange(vocab) != 5]
         assert float(off.abs().max()) <= 2.0 ** -18 * math.log(2) + 6 * U
         assert float(off.mean(1).abs().max()) <= 6 * 2.0 ** -17 * math.log(2) / math.sqrt(12 * (vocab - 1)) + 4 * U
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("vocab", [60, 3001, 70001])
+@pytest.mark.parametrize("tail", [False, True], ids=["top", "tail"])
+def test_distill_loss_of_words_that_are_none(pk, vocab, tail, dtype):
+    """A word past the vocabulary that the teacher gives something: its row has no loss and no gradient, and no other row knows. One that the teacher rules out adds nothing."""
+    x, idx, t, w, lse = distill_inputs(6, vocab, 5, dtype, 13)
+    lse = lse if tail else None
+    idx[1, 4], idx[3, 0], idx[4, 2] = vocab, 2 ** 31 - 1, vocab + 7
+    t[4, 2] = -math.inf
+    loss, d, kl = pk.blockops.distill_loss(x, idx, t, w, 2.0, lse)
+    _, none, alone = pk.blockops.distill_loss(x, idx, t, w, 2.0, lse, grad=False)
+    bad = torch.tensor([1, 3], device="cuda")
+    assert none is None and torch.equal(bits(alone), bits(kl)) and bool(torch.isnan(loss))
+    assert bool(torch.isnan(kl[bad]).all()) and bool(torch.isnan(d[bad].float()).all())
+    idx[1], idx[3], idx[4, 2] = -1, -1, -1
+    want = pk.blockops.distill_loss(x, idx, t, w, 2.0, lse)
+    good = torch.tensor([0, 2, 4, 5], device="cuda")
+    assert torch.equal(bits(d[good]), bits(want[1][good])) and torch.equal(kl[good], want[2][good])
