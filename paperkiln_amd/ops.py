@@ -174,7 +174,7 @@ def gated_delta_rule(q, k, v, g, beta, scale, initial_state=None):
 
 def gated_delta_step_(q, k, v, g, beta, scale, state):
     """The same for the next token, or the next few, of sequences whose state is kept: moves ``state`` (float32 [B,Hv,dk,dv]) on in place and returns o.
-    Not differentiable: refused where gradients are kept and ``state`` wants one."""
+    Not differentiable: refused where gradients are kept and any of its tensors wants one."""
     return _native.gated_delta_step(q, k, v, g, beta, scale, state)
 
 

@@ -367,7 +367,10 @@ PyObject* py_delta_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Tensor o;
     {
         pybind11::gil_scoped_release no_gil;
-        if (at::GradMode::is_enabled() && state.requires_grad()) refuse(DELTA, "the state that is moved on in place must not require a gradient");
+        for (const Tensor* t : {&q, &k, &v, &g, &beta, &state}) {
+            no_tangent(DELTA, *t);
+            if (at::GradMode::is_enabled() && t->requires_grad()) refuse(DELTA, "a step moves its state on in place and is not differentiable: no tensor of it may require a gradient (torch.no_grad)");
+        }
         o = delta_fwd(q, k, v, g, beta, scale, state, state).first;
     }
     return THPVariable_Wrap(std::move(o));

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from test_post_ops_gpu import BF16, F64, FP32, HALF, U, within
-from test_student_ops_gpu import bits, distill_inputs, pk, plain_delta  # noqa: F401  (pk: a fixture)
+from test_student_ops_gpu import bits, delta_inputs, distill_inputs, pk, plain_delta  # noqa: F401  (pk: a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -41,6 +41,26 @@ def test_gated_delta_rule_of_bf16_where_sums_cancel(pk, T, dk, dv, heads):
     given = scale * torch.einsum("bhkv,bthv->bthk", first.double(), do.double()).abs()
     within("dq", dq, want[0], HALF[BF16] * want[0].abs() + 16 * U * (2 * given + want[0].abs()))
     assert float(wo.abs().max()) < 2.0 ** -7 * float(before.max())
+
+
+def test_gated_delta_step_refuses_what_wants_a_gradient(pk):
+    """With gradients kept, a step that one of its tensors wants a gradient of, or that has a tangent, is refused before it moves the state; without, it is what it is."""
+    *rule, first, _, _ = delta_inputs(2, 3, 1, 2, 16, 24, BF16, 15)
+    kept = first.clone()
+    for i, x in enumerate((*rule, first)):
+        leaf = x.detach().clone().requires_grad_()
+        args = [leaf if i == j else y for j, y in enumerate(rule)]
+        with pytest.raises(RuntimeError, match="not differentiable"):
+            pk.ops.gated_delta_step_(*args, 0.5, leaf if i == 5 else first)
+        with torch.no_grad():
+            moved = (leaf if i == 5 else first).clone()
+            o = pk.ops.gated_delta_step_(*args, 0.5, moved)
+        assert not o.requires_grad and torch.equal(first, kept) and not torch.equal(moved, kept)
+        with torch.autograd.forward_ad.dual_level():
+            dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                pk.ops.gated_delta_step_(*(dual if i == j else y for j, y in enumerate(rule)), 0.5, dual if i == 5 else first)
+    assert torch.equal(first, kept)
 
 
 # ---- distillation --------------------------------------------------------------------------------------------------------
