@@ -421,7 +421,7 @@ int pk_layernorm_bwd(const pk_norm_shape* s, const void* dy, int64_t lddy, const
  * dlogits is the gradient of upstream * loss, NULL: the loss alone. kl[rows] receives KL_r, row_loss[rows] (64 bits) the terms of the loss (device, fp32), which
  * is their sum in a fixed order. The weights carry mask and normalisation: a row of weight 0 is not read, nor one learned from that has no word; kl and gradient
  * are 0. A word that several slots name gets all of their probabilities; one past the vocabulary makes its row's KL and gradient no numbers; a teacher's logit of -inf adds nothing. dlogits may
- * be the logits themselves (same ld), else lie clear of everything. */
+ * be the logits themselves (same ld); else every result lies clear of every other and of all that is read. row_loss is aligned to 8 bytes. */
 typedef struct pk_distill_config {
     double temperature;  /* 2^-20 to 2^20 */
     float upstream;

@@ -311,11 +311,6 @@ void launch_distill(const Distill& a, hipStream_t st) {
 }
 constexpr int64_t MOST_ROWS = (1 << 22) - 2;  // a launch has fewer than 2^32 threads, 1024 for a row at most
 
-bool clear_of(const void* p, int64_t bytes, const void* q, int64_t more) {
-    const uintptr_t x = reinterpret_cast<uintptr_t>(p), y = reinterpret_cast<uintptr_t>(q);
-    return !q || x + static_cast<uintptr_t>(bytes) <= y || y + static_cast<uintptr_t>(more) <= x;
-}
-
 }  // namespace
 }  // namespace pk
 
@@ -334,13 +329,17 @@ extern "C" int pk_distill_loss(const pk_distill_config* c, const void* logits, i
         if (!std::isfinite(c->upstream)) return fail(PK_ERR_ARGUMENT, who + ": upstream must be finite");
         if (ld < 0 || (dlogits && rows > 1 && dld < vocab)) return fail(PK_ERR_SHAPE, who + ": rows of logits overlap");
         if (rows > 0 && (!logits || !indices || !teacher || !weights || !kl || !row_loss)) return fail(PK_ERR_ARGUMENT, who + ": null pointer");
-        const int64_t es = elem_size(dtype), read = rows ? ((rows - 1) * ld + vocab) * es : 0, written = rows ? ((rows - 1) * dld + vocab) * es : 0;
-        if (dlogits && rows > 0) {
-            if (!(dlogits == logits && (ld == dld || rows == 1)) && !clear_of(dlogits, written, logits, read))
+        if (!aligned(row_loss, 8)) return fail(PK_ERR_ARGUMENT, who + ": row_loss must be aligned to 8 bytes");
+        if (rows > 0) {
+            const int64_t es = elem_size(dtype);
+            const Span read(logits, ld, rows, vocab, es), written(dlogits, dld, rows, vocab, es);
+            if (written.meets(read) && !(dlogits == logits && (ld == dld || rows == 1)))
                 return fail(PK_ERR_ARGUMENT, who + ": dlogits may lie where the logits do, row for row, or clear of them");
-            if (!clear_of(dlogits, written, indices, 4 * rows * top) || !clear_of(dlogits, written, teacher, 4 * rows * top) ||
-                !clear_of(dlogits, written, teacher_lse, 4 * rows) || !clear_of(dlogits, written, weights, 4 * rows))
-                return fail(PK_ERR_ARGUMENT, who + ": dlogits overlap the teacher's tensors or the weights");
+            const Span out_kl(kl, 1, rows, 1, 4), out_rows(row_loss, 1, rows, 1, 8), out_loss(loss, 0, 1, 1, 4);
+            if (read.meets(out_kl) || read.meets(out_rows) || read.meets(out_loss) ||
+                !clear_of_all({written, out_kl, out_rows, out_loss},
+                              {Span(indices, top, rows, top, 4), Span(teacher, top, rows, top, 4), Span(teacher_lse, 1, rows, 1, 4), Span(weights, 1, rows, 1, 4)}))
+                return fail(PK_ERR_ARGUMENT, who + ": a result overlaps another tensor of the call");
         }
         touch({logits, indices, teacher, teacher_lse, weights, dlogits, kl, row_loss, loss}, stream);
         hipStream_t st = static_cast<hipStream_t>(stream);

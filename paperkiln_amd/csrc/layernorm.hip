@@ -359,22 +359,6 @@ int check(const char* who, const pk_norm_shape* s) {
     if (!known_dtype(s->dtype)) return fail(PK_ERR_ARGUMENT, w + ": dtype must be PK_F32 or PK_BF16");
     return PK_OK;
 }
-struct Span {
-    uintptr_t begin, end;
-    Span(const void* p, int64_t ld, int64_t rows, int64_t cols, int64_t size)
-        : begin(reinterpret_cast<uintptr_t>(p)), end(p && rows > 0 ? begin + static_cast<uintptr_t>(((rows - 1) * ld + cols) * size) : begin) {}
-    bool meets(const Span& o) const { return begin < o.end && o.begin < end; }
-};
-// Every result clear of every other and of all that is read.
-bool clear_of_all(std::initializer_list<Span> written, std::initializer_list<Span> read) {
-    for (const Span* w = written.begin(); w != written.end(); ++w) {
-        for (const Span& r : read)
-            if (w->meets(r)) return false;
-        for (const Span* o = w + 1; o != written.end(); ++o)
-            if (w->meets(*o)) return false;
-    }
-    return true;
-}
 
 }  // namespace
 }  // namespace pk

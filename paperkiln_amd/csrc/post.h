@@ -43,6 +43,23 @@ inline int launched() {
     return e == hipSuccess ? PK_OK : hip_fail(e, "kernel launch");
 }
 inline void touch(std::initializer_list<const void*> used, void* stream) { dev_touch(used.begin(), used.size(), stream); }
+// Where rows of a tensor lie: `rows` of `cols` elements of `size` bytes, ld apart. A null pointer has no place.
+struct Span {
+    uintptr_t begin, end;
+    Span(const void* p, int64_t ld, int64_t rows, int64_t cols, int64_t size)
+        : begin(reinterpret_cast<uintptr_t>(p)), end(p && rows > 0 ? begin + static_cast<uintptr_t>(((rows - 1) * ld + cols) * size) : begin) {}
+    bool meets(const Span& o) const { return begin < o.end && o.begin < end; }
+};
+// Every result clear of every other and of all that is read.
+inline bool clear_of_all(std::initializer_list<Span> written, std::initializer_list<Span> read) {
+    for (const Span* w = written.begin(); w != written.end(); ++w) {
+        for (const Span& r : read)
+            if (w->meets(r)) return false;
+        for (const Span* o = w + 1; o != written.end(); ++o)
+            if (w->meets(*o)) return false;
+    }
+    return true;
+}
 // The body of a C entry: nothing thrown (a string that finds no memory) leaves it.
 template <typename F>
 int c_entry(F&& f) noexcept {
