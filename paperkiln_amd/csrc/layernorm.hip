@@ -284,9 +284,13 @@ __global__ __launch_bounds__(256) void norm_columns(NormGrad a) {
     const int j = blockIdx.x * 256 + threadIdx.x;
     if (j >= a.cols) return;
     float w = 0.0f, b = 0.0f;
-    for (int64_t r = blockIdx.y; r < a.rows; r += gridDim.y) {
-        const float d = elem(static_cast<const T*>(a.dy), r * a.lddy + j);
-        w = fmaf(d, (elem(static_cast<const T*>(a.h), r * a.ldh + j) - a.mean[r]) * a.rstd[r], w), b += d;
+    for (int64_t r = blockIdx.y; r < a.rows;) {  // 64 rows at a time: a term goes through 64 additions and a few, however many rows there are
+        float pw = 0.0f, pb = 0.0f;
+        for (int i = 0; i < 64 && r < a.rows; ++i, r += gridDim.y) {
+            const float d = elem(static_cast<const T*>(a.dy), r * a.lddy + j);
+            pw = fmaf(d, (elem(static_cast<const T*>(a.h), r * a.ldh + j) - a.mean[r]) * a.rstd[r], pw), pb += d;
+        }
+        w += pw, b += pb;
     }
     float* part = a.parts + static_cast<int64_t>(blockIdx.y) * 2 * a.cols;
     part[j] = w, part[a.cols + j] = b;

@@ -63,6 +63,25 @@ def test_gated_delta_step_refuses_what_wants_a_gradient(pk):
     assert torch.equal(first, kept)
 
 
+# ---- layer norm ----------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("rows,cols,dtype", [(5000, 16400, FP32), (70000, 16385, BF16), (1 << 18, 16400, BF16)], ids=str)
+def test_layernorm_weights_gradients_of_tall_inputs_of_long_rows(pk, rows, cols, dtype):
+    """dw and db past the rows that are held: 64 workgroups for a column, 64 of their rows added up at a time, those sums one behind the other (a 4096th of the rows), then 4
+    workgroups' and 16 of those; the term itself is the kernel's own statistics and 4 u. The same row every time, so that roundings of a long chain all go one way: a chain of a
+    64th of the rows would be off by up to a third of its length, 1400 u for the tallest."""
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    h, dy = (torch.randn((1, cols), generator=gen, device="cuda").to(dtype) for _ in range(2))
+    w = torch.ones(cols, device="cuda")
+    _, _, mean, rstd = pk.ops.layernorm_fwd(h, w)
+    _, dw, db = pk.ops.layernorm_bwd(dy.expand(rows, cols), h.expand(rows, cols), w, mean.expand(rows).contiguous(), rstd.expand(rows).contiguous())
+    n = 64 + rows / 4096 + 1 + 4 + 16 + 4
+    term = dy[0].double() * (h[0].double() - mean.double()) * rstd.double()
+    within("dw", dw, rows * term, n * U * rows * term.abs())
+    within("db", db, rows * dy[0].double(), n * U * rows * dy[0].double().abs())
+
+
 # ---- distillation --------------------------------------------------------------------------------------------------------
 
 
