@@ -180,6 +180,9 @@ __device__ inline void load_row(const NormGrad& a, int64_t r, int at, int pieces
     o.mean = row ? a.mean[r] : 0.0f, o.rstd = row ? a.rstd[r] : 0.0f;
 }
 
+// Rows that a walk adds up one behind the other in registers; what they come to is added to what the rows before have left. So however tall an input is, roundings that all go one way
+// stay below 2^-16 of a sum. 262144 rows of 4096 columns in bf16: 1215 us, 1189 with one chain, 1413 with a workgroup for every 256 rows.
+constexpr int MOST_CHAIN = 256;
 // A workgroup walks down the rows, WALKS of them side by side, each WAVES wavefronts' own. AHEAD: the next rows' loads are on their way while one is worked on.
 template <typename T, int WAVES, int PER, int WALKS, bool ADD, bool AHEAD>
 __global__ __launch_bounds__(WAVES * 64 * WALKS) void norm_grad(NormGrad a) {
@@ -196,11 +199,36 @@ __global__ __launch_bounds__(WAVES * 64 * WALKS) void norm_grad(NormGrad a) {
         if (at + k * ROW < pieces) load_weights(a.w + (at + k * ROW) * N, w[k]);
     }
     const float edge_w = at < tail ? a.w[end] : 0.0f, per_col = 1.0f / a.cols;
+    float* part = a.parts + static_cast<int64_t>(blockIdx.x) * 2 * a.cols;
+    float* mine = WALKS > 1 ? sums + walk * 2 * a.cols : part;
+    bool more = false;  // there are sums of rows before
+    const auto leave = [&] {
+        const auto add = [&](float* to, float x) { *to = more ? *to + x : x; };
+        int at_then = at;  // the addresses are formed here, not held through the rows
+        asm volatile("" : "+v"(at_then));
+        const int end = pieces * N + at_then;
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            const int p = at_then + k * ROW;
+            if (p >= pieces) continue;
+#pragma unroll
+            for (int j = 0; j < N; ++j) add(mine + p * N + j, aw[k][j]), add(mine + a.cols + p * N + j, ab[k][j]);
+        }
+        if (at_then < tail) add(mine + end, ew), add(mine + a.cols + end, eb);
+    };
     const int64_t step = static_cast<int64_t>(gridDim.x) * WALKS;
     GradRow<T, PER, ADD> next;
     int64_t r0 = static_cast<int64_t>(blockIdx.x) * WALKS;
     if (AHEAD) load_row<ROW, AHEAD>(a, r0 + walk, at, pieces, tail, next);
-    for (int turn = 0; r0 < a.rows; r0 += step, turn ^= 1) {  // all walks take as many steps: a row behind the last one is zeros
+    for (int turn = 0, rows = 0; r0 < a.rows; r0 += step, turn ^= 1) {  // all walks take as many steps: a row behind the last one is zeros
+        if (rows++ == MOST_CHAIN) {
+            leave();
+            more = true, rows = 1, ew = eb = 0.0f;
+#pragma unroll
+            for (int k = 0; k < PER; ++k)
+#pragma unroll
+                for (int j = 0; j < N; ++j) aw[k][j] = ab[k][j] = 0.0f;
+        }
         const int64_t r = r0 + walk;
         if (!AHEAD) load_row<ROW, AHEAD>(a, r, at, pieces, tail, next);
         const GradRow<T, PER, ADD> c = next;
@@ -240,16 +268,7 @@ __global__ __launch_bounds__(WAVES * 64 * WALKS) void norm_grad(NormGrad a) {
         }
         if (at < tail) put(dx, end, fmaf(c.rstd, fmaf(c.edge_dy, edge_w, -m1) - u * m2, c.edge_dh));
     }
-    float* part = a.parts + static_cast<int64_t>(blockIdx.x) * 2 * a.cols;
-    float* mine = WALKS > 1 ? sums + walk * 2 * a.cols : part;
-#pragma unroll
-    for (int k = 0; k < PER; ++k) {
-        const int p = at + k * ROW;
-        if (p >= pieces) continue;
-#pragma unroll
-        for (int j = 0; j < N; ++j) mine[p * N + j] = aw[k][j], mine[a.cols + p * N + j] = ab[k][j];
-    }
-    if (at < tail) mine[end] = ew, mine[a.cols + end] = eb;
+    leave();
     if constexpr (WALKS > 1) {
         __syncthreads();
         for (int j = tid; j < 2 * a.cols; j += ROW * WALKS) {

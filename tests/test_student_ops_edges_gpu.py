@@ -82,6 +82,21 @@ def test_layernorm_weights_gradients_of_tall_inputs_of_long_rows(pk, rows, cols,
     within("db", db, rows * dy[0].double(), n * U * rows * dy[0].double().abs())
 
 
+@pytest.mark.parametrize("rows,cols,dtype", [(70000, 4100, BF16), (1 << 20, 2052, BF16), (1 << 21, 1030, BF16), ((1 << 22) - 3, 24, FP32)], ids=str)
+def test_layernorm_weights_gradients_of_tall_inputs(pk, rows, cols, dtype):
+    """The same of rows that are held: a walk adds up 256 rows at a time, and those sums one behind the other (at most a 2^16th of the rows), a workgroup's 4 walks, a 16th of 512
+    workgroups, 16 of those; 4 u of the term. In a chain of a 256th of the rows, 4096 of the second case, up to a third of its length would be off."""
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    h, dy = (torch.randn((1, cols), generator=gen, device="cuda").to(dtype) for _ in range(2))
+    w = torch.ones(cols, device="cuda")
+    _, _, mean, rstd = pk.ops.layernorm_fwd(h, w)
+    _, dw, db = pk.ops.layernorm_bwd(dy.expand(rows, cols), h.expand(rows, cols), w, mean.expand(rows).contiguous(), rstd.expand(rows).contiguous())
+    n = 256 + rows / 2 ** 16 + 1 + 4 + 32 + 16 + 4
+    term = dy[0].double() * (h[0].double() - mean.double()) * rstd.double()
+    within("dw", dw, rows * term, n * U * rows * term.abs())
+    within("db", db, rows * dy[0].double(), n * U * rows * dy[0].double().abs())
+
+
 # ---- distillation --------------------------------------------------------------------------------------------------------
 
 
