@@ -438,7 +438,7 @@ int pk_distill_loss(const pk_distill_config* c, const void* logits, int64_t ld, 
  * row; a token of g 0 and beta 0, finite in q, k and v, leaves the state as it is (padding). Up to 8 tokens the rule is walked through token by token, with
  * the state in registers and no workspace (its bytes are then 0): serving. A value of q, k, v, g or beta that is not a number spoils what its heads of v have from the beginning of
  * its chunk of 64 tokens on, and nothing else. Results lie clear of one another, of the workspace and of what is read, but for state_out, which may be state_in: refused where
- * it can be told (tensors of heads may lie between one another in one buffer). */
+ * it can be told (tensors of heads that have gaps may lie between one another in one buffer; only the same place is refused of those). No two elements of a result share memory. */
 typedef struct pk_delta_shape {
     int32_t B, T;    /* either may be 0; at most 2^19 heads of sequences and 2^22 chunks of 64 tokens */
     int32_t Hk, Hv;  /* Hv a multiple of Hk */

@@ -390,14 +390,16 @@ int launch_chunks(const Rule& a, int dtype, bool backward, hipStream_t st);
 int launch_states(const Rule& a, int dtype, hipStream_t st);
 int check(const char* who, const pk_delta_shape* s);
 bool view_of(const pk_tensor4* t, View& v);
-// Where a tensor lies, to refuse results on top of something else. Tensors of heads may lie between one another in one buffer, so between two of them only the same place is refused.
+// Where a tensor lies, to refuse results on top of something else. Tensors of heads that have gaps may lie between one another in one buffer, so of two tensors of heads, one of
+// them with gaps, only the same place is refused.
 struct Span {
     uintptr_t from, to;
-    bool heads;
+    bool heads, gaps;
 };
 Span span_of(const void* dense, size_t bytes);
 Span span_of(const View& v, const pk_delta_shape* s, int heads, int width);
 bool apart(std::initializer_list<Span> written, std::initializer_list<Span> read);
+bool shares(const View& v, const pk_delta_shape* s, int heads);  // elements that are one in memory
 inline size_t pad(size_t bytes) { return (bytes + 255) & ~size_t{255}; }
 constexpr size_t MATRIX = BLOCKS * BLOCK * sizeof(uint16_t);
 

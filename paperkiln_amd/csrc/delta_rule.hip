@@ -487,20 +487,20 @@ bool view_of(const pk_tensor4* t, View& v) {
 }
 Span span_of(const void* dense, size_t bytes) {
     const uintptr_t p = reinterpret_cast<uintptr_t>(dense);
-    return Span{p, dense ? p + bytes : p, false};
+    return Span{p, dense ? p + bytes : p, false, false};
 }
 Span span_of(const View& v, const pk_delta_shape* s, int heads, int width) {
-    if (!v.ptr || !s->B || !s->T) return Span{0, 0, true};
+    if (!v.ptr || !s->B || !s->T) return Span{0, 0, true, true};
     int64_t low = 0, high = width;
     for (const int64_t reach : {(s->B - 1) * v.sb, (s->T - 1) * v.st, (heads - 1) * v.sh}) (reach < 0 ? low : high) += reach;
     const uintptr_t p = reinterpret_cast<uintptr_t>(v.ptr);
     const int64_t es = elem_size(s->dtype);
-    return Span{p + static_cast<uintptr_t>(low * es), p + static_cast<uintptr_t>(high * es), true};
+    return Span{p + static_cast<uintptr_t>(low * es), p + static_cast<uintptr_t>(high * es), true, high - low > static_cast<int64_t>(s->B) * s->T * heads * width};
 }
 bool apart(std::initializer_list<Span> written, std::initializer_list<Span> read) {
     const auto clash = [](const Span& x, const Span& y) {
         if (x.from == x.to || y.from == y.to) return false;
-        return x.heads && y.heads ? x.from == y.from : x.from < y.to && y.from < x.to;
+        return x.heads && y.heads && (x.gaps || y.gaps) ? x.from == y.from : x.from < y.to && y.from < x.to;
     };
     for (const Span* w = written.begin(); w != written.end(); ++w) {
         for (const Span& r : read)
@@ -510,6 +510,7 @@ bool apart(std::initializer_list<Span> written, std::initializer_list<Span> read
     }
     return true;
 }
+bool shares(const View& v, const pk_delta_shape* s, int heads) { return v.ptr && ((s->B > 1 && !v.sb) || (s->T > 1 && !v.st) || (heads > 1 && !v.sh)); }
 
 }  // namespace delta
 }  // namespace pk
@@ -536,6 +537,7 @@ int pk_delta_rule_fwd(const pk_delta_shape* s, const pk_tensor4* q, const pk_ten
         const size_t need = pk_delta_rule_fwd_workspace_bytes(s);
         if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
             return fail(PK_ERR_WORKSPACE, who + ": workspace too small (pk_delta_rule_fwd_workspace_bytes)");
+        if (shares(a.o, s, s->Hv)) return fail(PK_ERR_ARGUMENT, who + ": elements of o share memory");
         const size_t gates = sizeof(float) * s->B * s->T * s->Hv, state = sizeof(float) * s->B * s->Hv * s->dk * s->dv;
         if (!apart({span_of(a.o, s, s->Hv, s->dv), span_of(state_out, state), span_of(workspace, need)},
                    {span_of(a.q, s, s->Hk, s->dk), span_of(a.k, s, s->Hk, s->dk), span_of(a.v, s, s->Hv, s->dv), span_of(g, gates), span_of(beta, gates),

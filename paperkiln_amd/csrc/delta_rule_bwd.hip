@@ -480,6 +480,7 @@ int pk_delta_rule_bwd(const pk_delta_shape* s, const pk_tensor4* d_o, const floa
         const Room r = room_of(s);
         if (r.all && (!workspace || workspace_bytes < r.all || !aligned(workspace, 16)))
             return fail(PK_ERR_WORKSPACE, who + ": workspace too small (pk_delta_rule_bwd_workspace_bytes)");
+        if (shares(a.dq, s, s->Hk) || shares(a.dk_, s, s->Hk) || shares(a.dv_, s, s->Hv)) return fail(PK_ERR_ARGUMENT, who + ": elements of a gradient share memory");
         const size_t gates = sizeof(float) * s->B * s->T * s->Hv, state = sizeof(float) * s->B * s->Hv * s->dk * s->dv;
         if (!apart({span_of(a.dq, s, s->Hk, s->dk), span_of(a.dk_, s, s->Hk, s->dk), span_of(a.dv_, s, s->Hv, s->dv), span_of(dg, gates), span_of(dbeta, gates), span_of(dstate_in, state),
                     span_of(workspace, r.all)},

@@ -4,7 +4,7 @@ import ctypes as C
 import pytest
 
 from paperkiln_amd import _lib
-from test_student_ops import ARGUMENT, at, distill
+from test_student_ops import ARGUMENT, T4, at, delta, distill
 
 past = lambda i, n: C.c_void_p(at(i).value + n)  # noqa: E731
 
@@ -28,3 +28,20 @@ def test_distill_loss_refuses_results_in_logits_that_are_overwritten():
 def test_distill_loss_refuses_row_losses_between_words():
     for rows in (0, 4):
         assert distill(rows=rows, row=past(7, 4)) == ARGUMENT and b"8 bytes" in _lib.lib().pk_last_error()
+
+
+# q, k, v, o, d_o, dq, dk, dv of 2 x 100 tokens of 64 in bf16, dense, at 1 to 8 << 24: 25600 bytes each
+DELTA_PARTLY = [("fwd", dict(o=T4((3 << 24) + 128))), ("fwd", dict(o=T4((1 << 24) + 25598))), ("fwd", dict(o=T4((2 << 24) - 25598))), ("fwd", dict(o=T4((3 << 24) + 13000, -6400, 64, 64))),
+                ("bwd", dict(dq=T4((1 << 24) + 128))), ("bwd", dict(dq=T4((7 << 24) - 128))), ("bwd", dict(dk_=T4((8 << 24) + 25598))), ("bwd", dict(dv_=T4((5 << 24) - 64)))]
+DELTA_SHARED = [("fwd", dict(o=T4(4 << 24, 0, 64, 64))), ("fwd", dict(o=T4(4 << 24, 6400, 0, 64))), ("fwd", dict(o=T4(4 << 24, 12800, 64, 0), Hv=2)), ("bwd", dict(dq=T4(6 << 24, 0, 64, 64))),
+                ("bwd", dict(dk_=T4(7 << 24, 64, 0, 64))), ("bwd", dict(dv_=T4(8 << 24, 12800, 64, 0), Hv=2))]
+
+
+@pytest.mark.parametrize("entry,change", DELTA_PARTLY, ids=[f"{e}_{i}" for i, (e, _) in enumerate(DELTA_PARTLY)])
+def test_gated_delta_rule_refuses_dense_results_partly_on_top_of_others(entry, change):
+    assert delta(entry, **change) == ARGUMENT and b"clear of" in _lib.lib().pk_last_error()
+
+
+@pytest.mark.parametrize("entry,change", DELTA_SHARED, ids=[f"{e}_{i}" for i, (e, _) in enumerate(DELTA_SHARED)])
+def test_gated_delta_rule_refuses_results_that_share_their_elements(entry, change):
+    assert delta(entry, **change) == ARGUMENT and b"share memory" in _lib.lib().pk_last_error()

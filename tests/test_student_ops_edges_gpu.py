@@ -43,6 +43,32 @@ def test_gated_delta_rule_of_bf16_where_sums_cancel(pk, T, dk, dv, heads):
     assert float(wo.abs().max()) < 2.0 ** -7 * float(before.max())
 
 
+def test_gated_delta_rule_between_the_columns_of_one_buffer(pk):
+    """The C entries with every tensor of heads between the others' columns, sequences in reverse order in memory: what dense tensors give, to the bit."""
+    B, T, Hk, Hv, dk, dv = 3, 80, 2, 4, 32, 40
+    q, k, v, g, beta, first, do, dlast = delta_inputs(B, T, Hk, Hv, dk, dv, BF16, 16)
+    C, L, shape = pk.lib.C, pk.lib.lib(), pk.lib.DeltaShape(B, T, Hk, Hv, dk, dv, pk.lib.PK_BF16, 0.25)
+    widths = [Hk * dk, Hk * dk, Hv * dv, Hv * dv, Hv * dv, Hk * dk, Hk * dk, Hv * dv]   # q, k, v, o, d_o, dq, dk, dv
+    whole, row = torch.zeros(B, T, sum(widths), dtype=BF16, device="cuda"), sum(widths)
+    parts = [x.unflatten(2, (-1, d)) for x, d in zip(whole.split(widths, 2), (dk, dk, dv, dv, dv, dk, dk, dv))]
+    for part, x in zip(parts, (q, k, v, None, do)):
+        if x is not None:
+            part.copy_(x.flip(0))
+    place = lambda p: C.byref(pk.lib.Tensor4(p[B - 1].data_ptr(), -T * row, row, p.shape[3]))  # noqa: E731
+    tq, tk, tv, to, td, tdq, tdk, tdv = map(place, parts)
+    at = lambda t: C.c_void_p(t.data_ptr())  # noqa: E731
+    room = lambda n: torch.empty(n, dtype=torch.uint8, device="cuda")  # noqa: E731
+    last, dfirst, dg, dbeta = (torch.empty_like(x) for x in (first, first, g, beta))
+    ws, wb = room(L.pk_delta_rule_fwd_workspace_bytes(C.byref(shape))), room(L.pk_delta_rule_bwd_workspace_bytes(C.byref(shape)))
+    stream = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    pk.lib.check(L.pk_delta_rule_fwd(C.byref(shape), tq, tk, tv, at(g), at(beta), at(first), to, at(last), at(ws), ws.numel(), stream))
+    pk.lib.check(L.pk_delta_rule_bwd(C.byref(shape), td, at(dlast), tq, tk, tv, at(g), at(beta), at(first), tdq, tdk, tdv, at(dg), at(dbeta), at(dfirst), at(wb), wb.numel(), stream))
+    want = [*pk.ops.gated_delta_rule_fwd(q, k, v, g, beta, 0.25, first), *pk.ops.gated_delta_rule_bwd(do, q, k, v, g, beta, 0.25, first, dlast)]
+    o, dq, dk_, dv_ = (parts[i].flip(0) for i in (3, 5, 6, 7))
+    assert all(torch.equal(bits(a), bits(b)) for a, b in zip((o, last, dq, dk_, dv_, dg, dbeta, dfirst), want))
+    assert all(torch.equal(parts[i].flip(0), x) for i, x in ((0, q), (1, k), (2, v), (4, do)))
+
+
 def test_gated_delta_step_refuses_what_wants_a_gradient(pk):
     """With gradients kept, a step that one of its tensors wants a gradient of, or that has a tangent, is refused before it moves the state; without, it is what it is."""
     *rule, first, _, _ = delta_inputs(2, 3, 1, 2, 16, 24, BF16, 15)
