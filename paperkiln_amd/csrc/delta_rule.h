@@ -164,7 +164,6 @@ __device__ inline f32x4 load4(const uint16_t* row, int c, int n) {
     }
     return f32x4{c < n ? f(row[c]) : 0.0f, c + 1 < n ? f(row[c + 1]) : 0.0f, c + 2 < n ? f(row[c + 2]) : 0.0f, 0.0f};
 }
-__device__ inline Operand<3> load8(const float* row, int c, int n) { return split8<3>(load4(row, c, n), load4(row, c + 4, n)); }
 __device__ inline void store4(float* row, int c, int n, const f32x4& x) {
     if (c + 4 <= n) {
         *reinterpret_cast<f32x4_any*>(row + c) = x;
