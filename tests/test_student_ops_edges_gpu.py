@@ -123,6 +123,33 @@ def test_layernorm_weights_gradients_of_tall_inputs(pk, rows, cols, dtype):
     within("db", db, rows * dy[0].double(), n * U * rows * dy[0].double().abs())
 
 
+@pytest.mark.parametrize("cols", [520, 5000, 20000])   # rows of a wavefront, of a workgroup, read three times
+def test_layernorm_past_2_to_the_31(pk, cols):
+    """Rows 2^30 elements apart, read and with what goes through them; and dense results whose last rows lie past 2^31 elements: what near rows give, to the bit."""
+    gen = torch.Generator(device="cuda").manual_seed(cols)
+    x, r, dy, dh = (torch.randn((4, cols), generator=gen, device="cuda").to(BF16) for _ in range(4))
+    w, b = torch.randn(cols, generator=gen, device="cuda"), torch.randn(cols, generator=gen, device="cuda")
+    buffer = torch.zeros(3 * 2 ** 30 + 4 * cols, dtype=BF16, device="cuda")
+    far = [buffer[i * cols:].as_strided((4, cols), (2 ** 30, 1)) for i in range(4)]
+    for a, near in zip(far, (x, r, dy, dh)):
+        a.copy_(near)
+    want = pk.ops.layernorm_fwd(x, w, b, 1e-5, r)
+    got = pk.ops.layernorm_fwd(far[0], w, b, 1e-5, far[1])
+    assert all(torch.equal(bits(p), bits(q)) for p, q in zip(got, want))
+    far[0].copy_(want[1])
+    back = pk.ops.layernorm_bwd(dy, want[1], w, want[2], want[3], dh)
+    assert all(torch.equal(bits(p), bits(q)) for p, q in zip(pk.ops.layernorm_bwd(far[2], far[0], w, want[2], want[3], far[3]), back))
+    del buffer, far, got
+    rows = 2 ** 31 // cols + 5
+    many = lambda t: t[1:2].expand(rows, cols)  # noqa: E731
+    y, h, mean, rstd = pk.ops.layernorm_fwd(many(x), w, b, 1e-5, many(r))
+    for i in (0, rows - 5, rows - 1):
+        assert all(torch.equal(bits(p[i]), bits(q[1])) for p, q in zip((y, h, mean, rstd), want))
+    dx, _, _ = pk.ops.layernorm_bwd(many(dy), h, w, mean, rstd, many(dh))
+    for i in (0, rows - 5, rows - 1):
+        assert torch.equal(bits(dx[i]), bits(back[0][1]))
+
+
 # ---- distillation --------------------------------------------------------------------------------------------------------
 
 
@@ -163,3 +190,24 @@ def test_distill_loss_of_words_that_are_none(pk, vocab, tail, dtype):
     want = pk.blockops.distill_loss(x, idx, t, w, 2.0, lse)
     good = torch.tensor([0, 2, 4, 5], device="cuda")
     assert torch.equal(bits(d[good]), bits(want[1][good])) and torch.equal(kl[good], want[2][good])
+
+
+def test_distill_loss_past_2_to_the_31(pk):
+    """Rows of logits and of their gradient 2^30 elements apart, and a row whose slots begin 2^31 values into the teacher's tensors: what near ones give, to the bit."""
+    x, idx, t, w, lse = distill_inputs(4, 1000, 6, BF16, 17)
+    far = torch.zeros(3 * 2 ** 30 + 2000, dtype=BF16, device="cuda").as_strided((4, 1000), (2 ** 30, 1))
+    far.copy_(x)
+    want = pk.blockops.distill_loss(x, idx, t, w, 2.0, lse)
+    over = torch.zeros(3 * 2 ** 30 + 2000, dtype=BF16, device="cuda").as_strided((4, 1000), (2 ** 30, 1))
+    for out in (None, over, far):
+        got = pk.blockops.distill_loss(far, idx, t, w, 2.0, lse, out=out)
+        assert out is None or got[1].data_ptr() == out.data_ptr()
+        assert all(torch.equal(bits(a), bits(b)) for a, b in zip(got, want))
+    del far, over, got
+    rows, top = 2 ** 21 + 1, 1024
+    x, idx, t, w, _ = distill_inputs(1, 2000, top, BF16, 18)
+    many, given, weights = torch.full((rows, top), -1, dtype=torch.int32, device="cuda"), torch.zeros(rows, top, device="cuda"), torch.zeros(rows, device="cuda")
+    many[-1], given[-1], weights[-1] = idx[0], t[0], w[0]
+    loss, none, kl = pk.blockops.distill_loss(x.expand(rows, 2000), many, given, weights, grad=False)
+    alone = pk.blockops.distill_loss(x, idx, t, w, grad=False)
+    assert none is None and torch.equal(kl[-1:], alone[2]) and torch.equal(loss, alone[0]) and not kl[:-1].any()
