@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from test_post_ops_gpu import BF16, F64, FP32, HALF, U, within
-from test_student_ops_gpu import bits, delta_inputs, distill_inputs, pk, plain_delta  # noqa: F401  (pk: a fixture)
+from test_student_ops_gpu import bits, close, delta_inputs, distill_inputs, pk, plain_delta  # noqa: F401  (pk: a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -41,6 +41,26 @@ def test_gated_delta_rule_of_bf16_where_sums_cancel(pk, T, dk, dv, heads):
     given = scale * torch.einsum("bhkv,bthv->bthk", first.double(), do.double()).abs()
     within("dq", dq, want[0], HALF[BF16] * want[0].abs() + 16 * U * (2 * given + want[0].abs()))
     assert float(wo.abs().max()) < 2.0 ** -7 * float(before.max())
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("T,n", [(190, 184), (100, 65), (72, 64), (200, 64), (64, 9), (8, 5), (3, 1)])
+def test_gated_delta_rule_padding_leaves_the_state_to_the_bit(pk, T, n, dtype):
+    """Tokens of g 0 and beta 0 behind the last of n, whatever finite q, k and v they have: o and the state of the n alone, where both go by chunks or both by tokens."""
+    q, k, v, g, beta, first, do, dlast = delta_inputs(2, T, 2, 4, 48, 40, dtype, 19)
+    g[:, n:], beta[:, n:] = 0.0, 0.0
+    v[:, n:] = 1e3
+    o, state = pk.ops.gated_delta_rule_fwd(q, k, v, g, beta, 0.2, first)
+    part = [x[:, :n].contiguous() for x in (q, k, v, g, beta)]
+    want = pk.ops.gated_delta_rule_fwd(*part, 0.2, first)
+    assert torch.equal(bits(o[:, :n]), bits(want[0])) and torch.equal(bits(state), bits(want[1]))
+    do[:, n:] = 0.0
+    grads = pk.ops.gated_delta_rule_bwd(do, q, k, v, g, beta, 0.2, first, dlast)
+    alone = pk.ops.gated_delta_rule_bwd(do[:, :n].contiguous(), *part, 0.2, first, dlast)
+    assert not grads[0][:, n:].any() and not grads[1][:, n:].any() and not grads[2][:, n:].any()
+    for name, a, b in zip(("dq", "dk", "dv", "dg", "dbeta"), grads, alone):
+        close(name, a[:, :n], b, dtype, 1.0, 48, 2.0 ** 8)
+    close("dstate", grads[5], alone[5], dtype)
 
 
 def test_gated_delta_rule_between_the_columns_of_one_buffer(pk):
