@@ -436,7 +436,8 @@ int pk_distill_loss(const pk_distill_config* c, const void* logits, int64_t ld, 
  * [B, T, Hv], dense. state_in, state_out: fp32 [B, Hv, dk, dv], dense; NULL: begins with zeros, is not wanted; they may be the same. Keys are expected of
  * about unit length and beta in 0 to 2: past that the rule itself grows without bound. g = -inf (or below -1000) starts afresh, so several documents may follow one another in a
  * row; a token of g 0 and beta 0, finite in q, k and v, leaves the state as it is (padding). Up to 8 tokens the rule is walked through token by token, with
- * the state in registers and no workspace (its bytes are then 0): serving. A value of q, k, v, g or beta that is not a number spoils what its heads of v have from the beginning of
+ * the state in registers and no workspace (its bytes are then 0): serving. Past that the forward's workspace is 37.6 kB and the backward's 56.1 kB + 8 (dk + 64) dv bytes for each chunk of
+ * 64 tokens of each head of v (and 512 times dk, rounded up to 32, 64 or 128, for each head of k that several share): 154 MB and 1.03 GB for 4 x 4096 tokens of 16 heads of 128. A value of q, k, v, g or beta that is not a number spoils what its heads of v have from the beginning of
  * its chunk of 64 tokens on, and nothing else. Results lie clear of one another, of the workspace and of what is read, but for state_out, which may be state_in: refused where
  * it can be told (tensors of heads that have gaps may lie between one another in one buffer; only the same place is refused of those). No two elements of a result share memory. */
 typedef struct pk_delta_shape {

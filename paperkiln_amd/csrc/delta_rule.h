@@ -371,9 +371,10 @@ template <typename F>
 int by_size(int dk, F&& f) {
     return dk <= 32 ? f(std::integral_constant<int, 32>{}) : dk <= 64 ? f(std::integral_constant<int, 64>{}) : f(std::integral_constant<int, 128>{});
 }
-// Columns to a workgroup of a walk: 32 where that many workgroups fill the chip, and a unit's matrices, q and k are then fetched half as often; else 16, a chunk of which takes less time. The
-// forward of 4 x 2048 tokens, 16 heads of 128 in bf16 (256 workgroups of 32): 128 us, 134 in columns of 16; of 2 x 4096 tokens (128 of them) 207 and 161; of one sequence of
-// 4096 (64) 194 and 142.
+// Columns to a workgroup of a walk: 32 where that many workgroups fill the chip, and a unit's matrices, q and k are then fetched half as often; else 16, a chunk of which takes less time.
+// Forward and backward of 1024 tokens, us in columns of 32 and of 16, 256 workgroups of 32 and 128 of them: bf16 at 128 73, 258 (77, 267) and 64, 160 (52, 143); at 64 72, 268 (75, 274) and
+// 59, 149 (53, 139); at 32 93, 357 (98, 378) and 66, 186 (59, 178); fp32 at 128 125, 423 (154, 450) and 107, 224 (82, 217); at 64 94, 312 (116, 364) and 77, 186 (66, 170); at 32 117, 390
+// (130, 439) and 74, 218 (67, 205).
 inline bool wide(const Rule& a) { return static_cast<int64_t>(a.B) * a.Hv * blocks(a.dv, 32) >= 256; }
 // Workgroups of one unit go to one XCD, whose L2 then has the unit's q, k and matrices for all of its blocks. Launch with grid.x = unit_grid.
 inline unsigned unit_grid(int64_t units, int per) { return static_cast<unsigned>((units + 7) / 8 * 8 * per); }

@@ -3,9 +3,11 @@
 //   S_t = e^{g_t} S_{t-1} + k_t u_t^T,   u_t = beta_t (v_t - e^{g_t} S_{t-1}^T k_t),   o_t = scale S_t^T q_t
 //
 // In chunks (delta_rule.h) one launch forms what does not depend on a state, T and A of every chunk, and a second one walks down the chunks, a workgroup for 16 or 32 columns of a
-// head's state: the columns do not know of one another. What bounds the walk is its own chain: three products and three exchanges through LDS a chunk, 3.4 us of it.
-// 4 x 4096 tokens, 16 heads of 128 in bf16: the chunks' matrices 78 us (3.3 TB/s of 134 MB read and 126 written), the walk 221 us, 211 if it leaves the states for the backward in place of O.
-// Token by token, the state in registers, memory bounds it: the state read and written once. One token of 256 sequences, 16 heads of 128: 119 us, 4.5 TB/s; of one sequence 5 us.
+// head's state: the columns do not know of one another. What bounds the walk is its own chain: three products and three exchanges through LDS a chunk, 3.4 us of it. (One of the three, U = T R,
+// is there because T is kept by itself: U = T beta V - (T beta gamma K) S has its products with T outside of the chain, for as many more of them beside the chunks' matrices.)
+// 4 x 4096 tokens, 16 heads of 128 in bf16: the chunks' matrices 77 us (3.7 TB/s of 134 MB read and 154 written), the walk 216 us, 203 if it leaves the states for the backward in place of O.
+// Token by token, the state in registers, memory bounds one token: the state read and written once. One token of 256 sequences, 16 heads of 128: 119 us, 4.5 TB/s; of one sequence 5 us.
+// Of several tokens each one's k, q, v and decay are asked for in its own turn, behind the barrier of the one before: 8 tokens of those 256 sequences 345 us, 217 in fp32.
 #include "delta_rule.h"
 
 namespace pk {
@@ -410,8 +412,9 @@ __global__ __launch_bounds__(STEP_NT) void steps(Rule a) {
 
 // ---- launches ----
 
-// Up to here a sequence is walked through token by token. A token takes 1.1 to 1.6 us behind the first, a chunk of 64 what 8 to 10 tokens take: 16 heads of 128 of one sequence 16.2 us for 8
-// tokens and 28.5 for 16 by tokens, 14.1 by chunks; of 32 sequences 57, 102 and 58; of 256 sequences 342, 623 and 436.
+// Up to here a sequence is walked through token by token. A chunk takes what 7 tokens take (8 heads of 128 of one sequence in bf16: 15.7 us for 8 tokens by tokens, 13.5 by chunks) to 17 and more
+// (256 sequences of 16 heads in fp32): 8 tokens of 32 sequences of 16 heads by tokens and by chunks in bf16 56 and 58 us at 128, 20 and 30 at 64, 12 and 21 at 32; in fp32 37 and 79, 18 and 38,
+// 11 and 22; 16 tokens in bf16 100 and 58, 34 and 31, 21 and 21, in fp32 62 and 81, 32 and 38, 19 and 22; of 256 sequences at 128 345 and 446, in fp32 217 and 620.
 constexpr int FEW_TOKENS = 8;
 template <typename T, int DK, int VB, bool STATES, Rows BY>
 int launch_walk(const Rule& a, hipStream_t st) {

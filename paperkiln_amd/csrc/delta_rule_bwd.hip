@@ -11,8 +11,8 @@
 //
 // Four launches: the chunks' matrices; the states that the chunks begin with, formed again by the forward's walk (only the inputs are kept between the passes); the walk back, which like the
 // forward's takes 16 or 32 columns of a state by themselves; then, a workgroup for a chunk and a head of k, all that needs every column of a state. 4 x 4096 tokens, 16 heads of 128 in
-// bf16: 93, 211, 339 and 436 us. The walks are bound by their own chain, 3.3 and 5.3 us a chunk; the last launch by the states of all chunks (0.8 GB, 0.16 ms of a copy's rate), since a CU
-// has one workgroup's loads under way at a time: two would take twice the LDS and the registers.
+// bf16: 89, 203, 323 and 411 us. The walks are bound by their own chain, 3.2 and 5.0 us a chunk; the last launch by the states of all chunks (0.8 GB, 0.16 ms of a copy's rate), since a CU
+// has one workgroup's loads under way at a time: its wavefronts have tokens, so both states go through LDS, in three parts beside K and Q, and fill it.
 #include "delta_rule.h"
 
 namespace pk {

@@ -284,11 +284,11 @@ __global__ __launch_bounds__(1024) void distill_sum(const double* x, int64_t n, 
 
 // ---- launches ----
 
-// From here on logits and gradient do not stay in the 256 MB of the last-level cache together, and go past it: 8192 rows of 32000 in bf16 214 us, 223 through it; 4096 of 8000 (64 MB) 35.5
-// and 32.9.
+// From here on logits and gradient do not stay in the 256 MB of the last-level cache together, and go past it: 8192 rows of 32000 in bf16 200 us, 213 through it; 8192 of 2000 (31 MB) 28.7
+// and 26.8; between 60 and 96 MB it is level.
 constexpr int64_t PAST_BYTES = int64_t{96} << 20;
-// A row to as few threads as hold it in eight pieces each, in four where a wavefront or a few of them do: what is done once for a row is done by fewer. 8192 rows of 32000 in bf16: 214 us with
-// 512 threads of eight pieces, 317 with 1024 of four; 8192 of 2000: 26.8 with a wavefront, 34.0 with four; 4096 of 8000: 33 with 256 of four, 33.6 with 128 of eight.
+// A row to as few threads as hold it in eight pieces each, in four where a wavefront or a few of them do: what is done once for a row is done by fewer. 8192 rows of 32000 in bf16: 200 us with
+// 512 threads of eight pieces, 307 with 1024 of four; 8192 of 2000: 26.7 with a wavefront, 33.7 with four; 4096 of 8000: 38.2 with 256 of four, 39.9 with 128 of eight.
 template <typename T, bool PAST, bool GRAD>
 void launch_held(const Distill& a, hipStream_t st) {
     const dim3 grid(static_cast<unsigned>(a.rows));
